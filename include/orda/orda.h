@@ -308,6 +308,50 @@ int32_t orda_scale_gradients(int32_t device, void *hip_stream, const float *scal
                              const orda_scaled_gradient *gradients, int32_t count, char *err,
                              size_t err_len);
 
+/* ---- linear cross entropy without the logits ------------------------------ */
+/* Row losses of logits x = hidden · weightᵀ that are formed a piece of the
+ * vocabulary at a time and not kept:
+ *   lse[r] = log Σ_v e^x[r,v]
+ *   nll[r] = lse[r] - (1-ε)·x[r,y] - (ε/V)·Σ_v x[r,v],  ε = label_smoothing
+ * and, from the gradients of a loss into nll and lse (any weighting of rows),
+ * the gradients of hidden and weight. A row whose label is ignore_index is not
+ * read: its nll, lse and gradient row are 0. A label that is neither
+ * ignore_index nor a class makes its row's nll and gradients NaN (the calls do
+ * not wait for the device, so nothing else can report it); a NaN gradient row
+ * makes every row of grad_weight NaN.
+ * Everything is on `device`. The calls queue their kernels on hip_stream (NULL:
+ * the null stream) and return; they allocate nothing and can be captured into
+ * a graph. workspace is the call's alone until its kernels have run: calls (and
+ * captured graphs) that may overlap need one each. No counterpart in the
+ * reference, whose loss is a weighted mean. */
+typedef struct {
+    orda_tensor hidden;      /* [N,H], fp32 or bf16 */
+    orda_tensor weight;      /* [V,H], the same type; read in place where it is
+                                fp32, or 16-byte aligned with H and ld multiples
+                                of 8, else copied a piece at a time */
+    const int64_t *labels;   /* [N] */
+    int64_t n_labels;
+    int64_t ignore_index;
+    float label_smoothing;   /* in [0, 1] */
+    int64_t vocab_piece;     /* columns of a piece, rounded to whole 256s; 0:
+                                as many as 1 GiB of scratch holds */
+} orda_linear_ce;
+/* Bytes of workspace (256-byte aligned) of a forward call (backward 0), or of
+ * a backward call for grad_hidden (1), grad_weight (2) or both (3). */
+int32_t orda_linear_ce_workspace(const orda_linear_ce *args, int32_t backward, int64_t *bytes, char *err,
+                                 size_t err_len);
+/* nll, lse: [N] float32. */
+int32_t orda_linear_ce_forward(int32_t device, void *hip_stream, const orda_linear_ce *args, float *nll,
+                               float *lse, void *workspace, int64_t workspace_bytes, char *err,
+                               size_t err_len);
+/* lse as the forward call gave it; grad_nll, grad_lse: [N] float32 or NULL (0);
+ * grad_hidden [N,H] and grad_weight [V,H] in the inputs' type, each written
+ * when its data is set. */
+int32_t orda_linear_ce_backward(int32_t device, void *hip_stream, const orda_linear_ce *args,
+                                const float *lse, const float *grad_nll, const float *grad_lse,
+                                orda_tensor *grad_hidden, orda_tensor *grad_weight, void *workspace,
+                                int64_t workspace_bytes, char *err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

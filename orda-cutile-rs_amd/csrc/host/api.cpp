@@ -38,6 +38,15 @@
 
 using orda::DType;
 using orda::Error;
+using orda::check_view;
+using orda::copy_err;
+using orda::fail;
+using orda::hip_check;
+using orda::logits_pitch;
+using orda::round64;
+using orda::round8;
+using orda::tensor_ld;
+using orda::to_dtype;
 
 struct orda_ctx {
   int device = 0;
@@ -78,22 +87,6 @@ struct orda_ctx {
 
 namespace {
 
-[[noreturn]] void fail(int32_t status, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  throw Error{status, buf};
-}
-
-void hip_check(hipError_t e, const char* what) {
-  if (e == hipSuccess) return;
-  (void)hipGetLastError();
-  if (e == hipErrorOutOfMemory) fail(ORDA_ERR_OOM, "%s: device out of memory", what);
-  fail(ORDA_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-}
-
 // The end-of-call wait for the context's stream. It polls an event for up
 // to kSpinMicros, then blocks in hipStreamSynchronize: a short call's wait
 // ends sooner after its last operation when polled (Tied BT=256 H=512
@@ -114,11 +107,6 @@ void wait_stream(orda_ctx* c) {
   hip_check(hipStreamSynchronize(c->stream), "hipStreamSynchronize");
 }
 
-void copy_err(const Error& e, char* err, size_t len) {
-  if (!err || !len) return;
-  snprintf(err, len, "%s", e.msg.c_str());
-}
-
 // Rust's `{}` Display of an f32 (shortest round-trip digits, no exponent).
 std::string fmt_f32(float x) {
   if (isnan(x)) return "NaN";
@@ -136,38 +124,6 @@ std::string fmt_f32(float x) {
   int decimals = exp10 < 0 ? (p - 1 - exp10) : std::max(0, p - 1 - exp10);
   snprintf(buf, sizeof buf, "%.*f", decimals, d);
   return buf;
-}
-
-int64_t round8(int64_t x) { return (x + 7) / 8 * 8; }
-int64_t round64(int64_t x) { return (x + 63) / 64 * 64; }
-
-// Pitch of the logits staging rows: V rounded up to 64 elements, so that every
-// row starts on a 128-byte line (the backward GEMMs read these rows in
-// 128-byte K-slabs: at V = 50257 a pitch of round8(V) put every slab across two
-// lines, grad_hidden 0.524 of peak against 0.60, the row pass 0.65 against
-// 0.75). fp32 rows: plus 64 when that is a multiple of 1024, so that rows (and
-// the many row streams the row pass and the GEMMs walk in step) do not sit a
-// power of two apart. bf16 rows: further up to 64 past a multiple of 1024,
-// which measured the bf16 row pass (BT = 8192, paired rows, TB/s, two passes)
-// at V = 151936 5.9 against 5.0, at 50257 6.0 against 5.7, at 100000 and 128256
-// 1-2 % faster, at 32000 and 200064 1-3 % slower, elsewhere equal; the
-// backward GEMMs equal. (fp32 rows at V = 32000: the row pass 1.5 % slower,
-// so fp32 keeps the first rule.)
-int64_t logits_pitch(int64_t v, orda::DType lt) {
-  int64_t p = round64(v);
-  if (lt == orda::DType::BF16) {
-    while (p % 1024 != 64) p += 64;
-    return p;
-  }
-  return p % 1024 == 0 ? p + 64 : p;
-}
-
-int64_t tensor_ld(const orda_tensor& t) { return t.ld ? t.ld : t.cols; }
-
-DType to_dtype(int32_t d, const char* what) {
-  if (d == ORDA_F32) return DType::F32;
-  if (d == ORDA_BF16) return DType::BF16;
-  fail(ORDA_ERR_INVALID, "%s must be float32 or bfloat16", what);
 }
 
 // ------------------------------------------------------------ workspace
@@ -298,14 +254,6 @@ struct DMat {
   int64_t ld = 0, rows = 0, cols = 0;
   DType t = DType::F32;
 };
-
-// The checks every caller tensor passes before any kernel reads it: a
-// non-negative shape, a data pointer when it has elements, ld >= cols.
-void check_view(const orda_tensor& t, const char* what) {
-  if (t.rows < 0 || t.cols < 0) fail(ORDA_ERR_INVALID, "%s has a negative shape", what);
-  if (t.rows > 0 && t.cols > 0 && !t.data) fail(ORDA_ERR_INVALID, "%s has a null data pointer", what);
-  if (tensor_ld(t) < t.cols) fail(ORDA_ERR_INVALID, "%s has ld < cols", what);
-}
 
 // Device-resident view of an input matrix with a pitch that is a multiple of
 // 8 elements and a 16-byte aligned base; copies only when needed. A matrix

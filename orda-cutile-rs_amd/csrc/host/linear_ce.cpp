@@ -1,0 +1,387 @@
+// linear_ce.cpp — the linear cross entropy that keeps no logits
+// (orda_linear_ce_* of include/orda/orda.h): the rows that have a label are
+// compacted, and each piece of the vocabulary's columns is one product whose
+// epilogue leaves row statistics (forward) or the gradient of the logits
+// (backward, followed by the products of grad_hidden and grad_weight). The
+// count of those rows stays on the device, the scratch is the caller's: the
+// calls queue their kernels and return, and can be captured into a graph.
+#include <algorithm>
+#include <exception>
+
+#include "orda_host.h"
+
+namespace orda {
+namespace {
+
+constexpr int64_t kMaxWidth = int64_t{1} << 20;      // 32-bit offsets inside an operand's tile
+constexpr int64_t kMaxRows = int64_t{1} << 30;       // compact row numbers are 32 bits
+constexpr int64_t kMaxColumns = int64_t{1} << 30;
+// Scratch a piece may take: the larger the piece, the fewer the passes that
+// read and write the fp32 grad_hidden.
+constexpr int64_t kPieceBytes = int64_t{1} << 30;
+
+struct Ce {
+  DType t;
+  int64_t n, h, v;
+  const void *x, *w;
+  int64_t ldx, ldw;
+  bool planes;       // fp32: every product over three-plane operands
+  bool stage_w;      // bf16 weights that the products cannot read in place
+  bool gh, gw;       // backward: the gradients asked for
+  bool backward;
+  int64_t hp;        // pitch of the compact hidden rows, plane width with planes
+  int64_t piece;     // columns of a piece
+};
+
+int64_t ds_pitch(const Ce& c, int64_t cols) { return c.planes ? 3 * round64(cols) : logits_pitch(cols, DType::BF16); }
+
+int64_t column_bytes(const Ce& c) {   // of scratch, for each column of a piece
+  int64_t b = c.planes ? 6 * c.hp : c.stage_w ? 2 * c.hp : 0;
+  b += c.backward ? round64(c.n) * (c.planes ? 6 : 2) : (c.n * 16 + 255) / 256;
+  return b;
+}
+
+Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool gw) {
+  check_view(a.hidden, "hidden");
+  check_view(a.weight, "weight");
+  Ce c{};
+  c.t = to_dtype(a.hidden.dtype, "hidden");
+  if (to_dtype(a.weight.dtype, "weight") != c.t) fail(ORDA_ERR_INVALID, "hidden and weight must share one dtype");
+  if (a.hidden.location != ORDA_DEVICE || a.weight.location != ORDA_DEVICE)
+    fail(ORDA_ERR_INVALID, "hidden and weight must be on the device");
+  c.n = a.hidden.rows;
+  c.h = a.hidden.cols;
+  c.v = a.weight.rows;
+  if (a.weight.cols != c.h)
+    fail(ORDA_ERR_INVALID, "weight has %lld columns, hidden %lld", static_cast<long long>(a.weight.cols),
+         static_cast<long long>(c.h));
+  if (labels != c.n)
+    fail(ORDA_ERR_INVALID, "%lld labels for %lld rows", static_cast<long long>(labels), static_cast<long long>(c.n));
+  if (c.h < 1 || c.v < 1) fail(ORDA_ERR_INVALID, "hidden width and vocabulary must be > 0");
+  if (c.h > kMaxWidth || c.n > kMaxRows || c.v > kMaxColumns)
+    fail(ORDA_ERR_INVALID, "at most 2^20 columns, 2^30 rows and 2^30 classes");
+  if (!(a.label_smoothing >= 0.f && a.label_smoothing <= 1.f))
+    fail(ORDA_ERR_INVALID, "label_smoothing must be in [0, 1]");
+  if (a.vocab_piece < 0) fail(ORDA_ERR_INVALID, "vocab_piece must be >= 0");
+  c.x = a.hidden.data;
+  c.w = a.weight.data;
+  c.ldx = tensor_ld(a.hidden);
+  c.ldw = tensor_ld(a.weight);
+  c.planes = c.t == DType::F32;
+  c.stage_w = !c.planes && !(c.ldw % 8 == 0 && c.h % 8 == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0);
+  c.hp = c.planes ? round64(c.h) : round8(c.h);
+  c.backward = backward;
+  c.gh = gh;
+  c.gw = gw;
+  // Pieces of whole column tiles, all but the last alike.
+  int64_t most = a.vocab_piece > 0 ? a.vocab_piece : std::max<int64_t>(kPieceBytes / std::max<int64_t>(column_bytes(c), 1), 4096);
+  most = std::max<int64_t>(most / 256 * 256, 256);
+  const int64_t pieces = (c.v + most - 1) / most;
+  c.piece = pieces == 1 ? c.v : ((c.v + pieces - 1) / pieces + 255) / 256 * 256;
+  return c;
+}
+
+// The scratch of a call, laid out from base (null: only its size counts).
+struct Scratch {
+  CeRows rows;
+  void* x;           // compact hidden rows (the input's type)
+  void* x3;          // their planes
+  void* xt;          // transposed: grad_weight's K-major operand
+  void* w;           // a piece of the weights, padded or as planes
+  void* ds;          // gradient of a piece's logits
+  float* gh;         // grad_hidden of the compact rows
+  float4 *stats, *state, *coef;
+  float* xy;
+  float* split;
+  int64_t split_bytes, bytes;
+};
+
+GemmArgs product(const Ce& c, const Scratch& s) {
+  GemmArgs g{};
+  g.nprob = 1;
+  g.in_type = DType::BF16;
+  g.a_kmajor = true;
+  g.alpha = 1.f;
+  g.dyn_rows = s.rows.count;
+  g.split_ws = s.split;
+  g.split_ws_bytes = s.split_bytes;
+  return g;
+}
+
+// The piece's logits product: columns [v0, v0 + cols).
+GemmArgs logits_product(const Ce& c, const Scratch& s, int64_t v0, int64_t cols) {
+  GemmArgs g = product(c, s);
+  g.M = c.n;
+  g.N = cols;
+  g.K = c.hp;
+  g.lda = c.hp;
+  g.ldb = c.stage_w ? c.hp : c.ldw;
+  g.prob[0] = {s.x, c.stage_w ? s.w : static_cast<const char*>(c.w) + v0 * c.ldw * 2, nullptr};
+  g.b_kmajor = true;
+  g.group_m = 8;
+  g.ce.labels = s.rows.labels;
+  g.ce.col0 = v0;
+  if (c.planes) {
+    g.lda = g.ldb = 3 * c.hp;
+    g.plane_a = g.plane_b = c.hp;
+    g.prob[0] = {s.x3, s.w, nullptr};
+  } else {
+    g.K = c.h;
+  }
+  return g;
+}
+
+GemmArgs grad_hidden_product(const Ce& c, const Scratch& s, int64_t v0, int64_t cols) {
+  GemmArgs g = product(c, s);
+  g.M = c.n;
+  g.N = c.h;
+  g.K = c.planes ? round64(cols) : cols;
+  g.lda = ds_pitch(c, c.piece);
+  g.ldb = c.stage_w ? c.hp : c.ldw;
+  g.ldc = round8(c.h);
+  g.epi = v0 == 0 ? GemmEpilogue::StoreF32 : GemmEpilogue::AccumF32;
+  g.group_m = 4;
+  g.share_rounds = true;
+  g.prob[0] = {s.ds, c.stage_w ? s.w : static_cast<const char*>(c.w) + v0 * c.ldw * 2, s.gh};
+  if (c.planes) {
+    g.ldb = 3 * c.hp;
+    g.plane_a = round64(c.piece);
+    g.plane_b = c.hp;
+    g.prob[0].b = s.w;
+  }
+  return g;
+}
+
+GemmArgs grad_weight_product(const Ce& c, const Scratch& s, void* gw, int64_t ldg, int64_t v0, int64_t cols) {
+  GemmArgs g = product(c, s);
+  g.M = c.h;
+  g.N = cols;
+  g.K = c.planes ? round64(c.n) : c.n;
+  g.lda = round64(c.n);
+  g.ldb = ds_pitch(c, c.piece);
+  g.ldc = ldg;
+  g.c_trans = true;
+  g.c_type = c.t;
+  g.epi = GemmEpilogue::StoreF32;
+  g.group_m = 8;
+  g.prob[0] = {s.xt, s.ds, static_cast<char*>(gw) + v0 * ldg * dtype_size(c.t)};
+  if (c.planes) {
+    g.lda = 3 * round64(c.n);
+    g.plane_a = round64(c.n);
+    g.plane_b = round64(c.piece);
+  }
+  return g;
+}
+
+Scratch lay_out(const Ce& c, void* base) {
+  Scratch s{};
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) -> void* {
+    char* p = static_cast<char*>(base) + at;
+    at += (bytes + 255) / 256 * 256;
+    return base ? p : nullptr;
+  };
+  const int64_t np = round64(c.n);
+  s.rows.count = static_cast<int64_t*>(take(8));
+  s.rows.src = static_cast<int32_t*>(take(c.n * 4));
+  s.rows.pos = static_cast<int32_t*>(take(c.n * 4));
+  s.rows.labels = static_cast<int64_t*>(take(c.n * 8));
+  s.x = take(np * c.hp * dtype_size(c.t));
+  if (c.planes) s.x3 = take(np * 6 * c.hp);
+  if (c.planes) s.w = take(round64(c.piece) * 6 * c.hp);
+  else if (c.stage_w) s.w = take(c.piece * c.hp * 2);
+  if (!c.backward) {
+    const int64_t tiles = gemm_stat_tiles(c.piece);
+    s.stats = static_cast<float4*>(take(c.n * tiles * 16));
+    s.state = static_cast<float4*>(c.piece < c.v ? take(c.n * 16) : nullptr);
+    s.xy = static_cast<float*>(take(c.n * 4));
+  } else {
+    s.coef = static_cast<float4*>(take(c.n * 16));
+    s.ds = take(np * ds_pitch(c, c.piece) * 2);
+    if (c.gh) s.gh = static_cast<float*>(take(c.n * round8(c.h) * 4));
+    if (c.gw) s.xt = take(c.h * np * (c.planes ? 6 : 2));
+    // a piece and the last one split differently
+    const int64_t last = c.v - (c.v - 1) / c.piece * c.piece;
+    for (const int64_t cols : {c.piece, last}) {
+      if (c.gh) s.split_bytes = std::max(s.split_bytes, gemm_split_bytes(grad_hidden_product(c, s, 0, cols)));
+      if (c.gw) s.split_bytes = std::max(s.split_bytes, gemm_split_bytes(grad_weight_product(c, s, nullptr, c.h, 0, cols)));
+    }
+    s.split = s.split_bytes > 0 ? static_cast<float*>(take(s.split_bytes)) : nullptr;
+  }
+  s.bytes = at;
+  return s;
+}
+
+Scratch check_scratch(const Ce& c, void* workspace, int64_t bytes) {
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) fail(ORDA_ERR_INVALID, "workspace must be 256-byte aligned");
+  const int64_t need = lay_out(c, nullptr).bytes;
+  if (bytes < need || !workspace)
+    fail(ORDA_ERR_INVALID, "workspace of %lld bytes, %lld needed", static_cast<long long>(bytes),
+         static_cast<long long>(need));
+  return lay_out(c, workspace);
+}
+
+// The compact hidden rows, and their planes.
+void gather(const Ce& c, const Scratch& s, const CeGradRows& g, hipStream_t st) {
+  hip_check(launch_ce_gather(c.t, c.x, c.ldx, c.n, c.h, s.rows, s.x, c.hp, g, st), "linear cross entropy rows");
+  if (c.planes)
+    hip_check(launch_split3_rows(static_cast<const float*>(s.x), c.hp, c.n, c.hp, s.x3, round64(c.n), c.hp, st),
+              "linear cross entropy rows");
+}
+
+// The piece's weights where the products do not read them in place.
+void stage_weights(const Ce& c, const Scratch& s, int64_t v0, int64_t cols, hipStream_t st) {
+  if (c.planes)
+    hip_check(launch_split3_rows(static_cast<const float*>(c.w) + v0 * c.ldw, c.ldw, cols, c.h, s.w, round64(cols),
+                                 c.hp, st),
+              "linear cross entropy weights");
+  else if (c.stage_w)
+    hip_check(launch_convert_rows(DType::BF16, static_cast<const char*>(c.w) + v0 * c.ldw * 2, c.ldw, DType::BF16, s.w,
+                                  c.hp, cols, c.h, st),
+              "linear cross entropy weights");
+}
+
+void forward(const orda_linear_ce& a, const Ce& c, const Scratch& s, float* nll, float* lse, hipStream_t st) {
+  hip_check(launch_ce_rows(a.labels, c.n, c.v, a.ignore_index, s.rows, nll, lse, st), "linear cross entropy rows");
+  gather(c, s, CeGradRows{}, st);
+  for (int64_t v0 = 0; v0 < c.v; v0 += c.piece) {
+    const int64_t cols = std::min(c.piece, c.v - v0);
+    stage_weights(c, s, v0, cols, st);
+    GemmArgs g = logits_product(c, s, v0, cols);
+    g.epi = GemmEpilogue::CeStats;
+    g.ce.stats = s.stats;
+    g.ce.stats_ld = gemm_stat_tiles(c.piece);
+    g.ce.xy = s.xy;
+    hip_check(launch_gemm(g, st), "linear cross entropy logits");
+    CeLossArgs l{};
+    l.rows = s.rows;
+    l.stats = s.stats;
+    l.stats_ld = g.ce.stats_ld;
+    l.tiles = gemm_stat_tiles(cols);
+    l.state = s.state;
+    l.first = v0 == 0;
+    l.last = v0 + cols == c.v;
+    l.xy = s.xy;
+    l.smooth_each = a.label_smoothing / static_cast<float>(c.v);
+    l.target = 1.f - a.label_smoothing;
+    l.nll = nll;
+    l.lse = lse;
+    hip_check(launch_ce_losses(l, c.n, st), "linear cross entropy losses");
+  }
+}
+
+void backward(const orda_linear_ce& a, const Ce& c, const Scratch& s, CeGradRows gr, orda_tensor* gh, orda_tensor* gw,
+              hipStream_t st) {
+  hip_check(launch_ce_rows(a.labels, c.n, c.v, a.ignore_index, s.rows, nullptr, nullptr, st),
+            "linear cross entropy rows");
+  gr.smooth_each = a.label_smoothing / static_cast<float>(c.v);
+  gr.target = 1.f - a.label_smoothing;
+  gr.coef = s.coef;
+  gather(c, s, gr, st);
+  if (c.gw)
+    hip_check(c.planes ? launch_transpose_split3(static_cast<const float*>(s.x), c.hp, nullptr, 0, c.n, c.h, s.xt,
+                                                 round64(c.n), st)
+                       : launch_transpose_rows(s.x, c.hp, nullptr, 0, c.n, c.h, s.xt, round64(c.n), DType::BF16, st),
+              "linear cross entropy rows");
+  for (int64_t v0 = 0; v0 < c.v; v0 += c.piece) {
+    const int64_t cols = std::min(c.piece, c.v - v0);
+    stage_weights(c, s, v0, cols, st);
+    GemmArgs g = logits_product(c, s, v0, cols);
+    g.epi = GemmEpilogue::CeGrad;
+    g.logits_type = DType::BF16;
+    g.prob[0].c = s.ds;
+    g.ldc = ds_pitch(c, c.piece);
+    g.ce.plane = round64(c.piece);
+    g.ce.coef = s.coef;
+    hip_check(launch_gemm(g, st), "linear cross entropy gradient");
+    if (c.gh) hip_check(launch_gemm(grad_hidden_product(c, s, v0, cols), st), "grad_hidden");
+    if (c.gw) hip_check(launch_gemm(grad_weight_product(c, s, gw->data, tensor_ld(*gw), v0, cols), st), "grad_weight");
+  }
+  if (c.gh)
+    hip_check(launch_ce_scatter(s.gh, round8(c.h), s.rows.pos, c.n, c.h, c.t, gh->data, tensor_ld(*gh), st),
+              "grad_hidden");
+}
+
+bool wanted(const orda_tensor* g) { return g != nullptr && g->data != nullptr; }
+
+void check_grad(const orda_tensor& g, DType t, int64_t rows, int64_t cols, const char* what) {
+  check_view(g, what);
+  if (to_dtype(g.dtype, what) != t) fail(ORDA_ERR_INVALID, "%s must have its input's dtype", what);
+  if (g.location != ORDA_DEVICE) fail(ORDA_ERR_INVALID, "%s must be on the device", what);
+  if (g.rows != rows || g.cols != cols)
+    fail(ORDA_ERR_INVALID, "%s must be [%lld, %lld]", what, static_cast<long long>(rows), static_cast<long long>(cols));
+}
+
+template <class F>
+int32_t guarded(char* err, size_t err_len, F&& f) {
+  try {
+    f();
+    return ORDA_OK;
+  } catch (const Error& e) {
+    copy_err(e, err, err_len);
+    return e.status;
+  } catch (const std::exception& e) {
+    copy_err(Error{ORDA_ERR_INTERNAL, e.what()}, err, err_len);
+    return ORDA_ERR_INTERNAL;
+  }
+}
+
+}  // namespace
+}  // namespace orda
+
+using namespace orda;
+
+extern "C" {
+
+int32_t orda_linear_ce_workspace(const orda_linear_ce* args, int32_t backward, int64_t* bytes, char* err,
+                                 size_t err_len) {
+  return guarded(err, err_len, [&] {
+    if (!args || !bytes) fail(ORDA_ERR_INVALID, "null argument");
+    const Ce c = make_ce(*args, args->n_labels, backward != 0, (backward & 1) != 0, (backward & 2) != 0);
+    *bytes = c.n > 0 ? lay_out(c, nullptr).bytes : 0;
+  });
+}
+
+int32_t orda_linear_ce_forward(int32_t device, void* hip_stream, const orda_linear_ce* args, float* nll, float* lse,
+                               void* workspace, int64_t workspace_bytes, char* err, size_t err_len) {
+  return guarded(err, err_len, [&] {
+    if (!args) fail(ORDA_ERR_INVALID, "null argument");
+    const Ce c = make_ce(*args, args->n_labels, false, false, false);
+    if (c.n == 0) return;
+    if (!args->labels || !nll || !lse) fail(ORDA_ERR_INVALID, "null argument");
+    const Scratch s = check_scratch(c, workspace, workspace_bytes);
+    const DeviceScope scope(device);
+    forward(*args, c, s, nll, lse, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int32_t orda_linear_ce_backward(int32_t device, void* hip_stream, const orda_linear_ce* args, const float* lse,
+                                const float* grad_nll, const float* grad_lse, orda_tensor* grad_hidden,
+                                orda_tensor* grad_weight, void* workspace, int64_t workspace_bytes, char* err,
+                                size_t err_len) {
+  return guarded(err, err_len, [&] {
+    if (!args) fail(ORDA_ERR_INVALID, "null argument");
+    const Ce c = make_ce(*args, args->n_labels, true, wanted(grad_hidden), wanted(grad_weight));
+    if (c.gh) check_grad(*grad_hidden, c.t, c.n, c.h, "grad_hidden");
+    if (c.gw) check_grad(*grad_weight, c.t, c.v, c.h, "grad_weight");
+    if (!c.gh && !c.gw) return;
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    if (c.n == 0) {   // no rows: a weight gradient of zeros
+      if (!c.gw) return;
+      const DeviceScope scope(device);
+      hip_check(launch_ce_scatter(nullptr, 0, nullptr, c.v, c.h, c.t, grad_weight->data, tensor_ld(*grad_weight), st),
+                "grad_weight");
+      return;
+    }
+    if (!args->labels || !lse) fail(ORDA_ERR_INVALID, "null argument");
+    const Scratch s = check_scratch(c, workspace, workspace_bytes);
+    const DeviceScope scope(device);
+    CeGradRows gr{};
+    gr.lse = lse;
+    gr.grad_nll = grad_nll;
+    gr.grad_lse = grad_lse;
+    backward(*args, c, s, gr, grad_hidden, grad_weight, st);
+  });
+}
+
+}  // extern "C"

@@ -570,9 +570,10 @@ __device__ __forceinline__ TileCoord tile_at(int64_t pm, int64_t pn, int64_t Mt)
   return c;
 }
 
+// M: the product's rows (g.M, or fewer that only the device knows).
 template <int TM = kTile>
-__device__ __forceinline__ TileCoord map_tile(const GemmArgs& g, int64_t t) {
-  const int64_t Mt = (g.M + TM - 1) / TM;
+__device__ __forceinline__ TileCoord map_tile(const GemmArgs& g, int64_t M, int64_t t) {
+  const int64_t Mt = (M + TM - 1) / TM;
   const int64_t Nt = (g.N + kTile - 1) / kTile;
   int64_t Mv = Mt * g.nprob;
   int64_t T = Mv * Nt;
@@ -625,9 +626,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 // (MF = 8: 16 KB beside the ring; else in the ring), ring: the operand ring,
 // idle by now.
 template <int ES, GemmEpilogue EPI, typename LT, bool CT, int MF>
-__device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, const GemmProblem& pr, const TileCoord& tc,
-                                              f32x4 (&acc)[MF][kFrag], unsigned char* epi,
-                                              unsigned char* ring, int64_t lab_pre) {
+__device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, int64_t M, const GemmProblem& pr,
+                                              const TileCoord& tc, f32x4 (&acc)[MF][kFrag],
+                                              unsigned char* epi, unsigned char* ring, int64_t lab_pre) {
   constexpr bool kTeacherEpi = EPI == GemmEpilogue::LogitsTeacher || EPI == GemmEpilogue::LogitsTeacher16;
   constexpr int TM = 32 * MF;   // tile rows
   const int tid = threadIdx.x;
@@ -638,7 +639,7 @@ __device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, const GemmProbl
   const int lrow = lane & 15;
   const int lgrp = lane >> 4;
   if constexpr (EPI == GemmEpilogue::StoreF32 || EPI == GemmEpilogue::AccumF32) {
-    float* C = static_cast<float*>(pr.c);
+    LT* C = static_cast<LT*>(pr.c);   // float, or bf16 (CT stores only)
     const float alpha = g.alpha_ptr != nullptr ? g.alpha * *g.alpha_ptr : g.alpha;
     // acc[i][j][e] is row wm*16*MF + 16i + 4*lgrp + e, column wn*128 + 16j + lrow.
     const int row_w = tc.m0 + wm * (TM / 2);
@@ -652,24 +653,29 @@ __device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, const GemmProbl
       for (int j = 0; j < kFrag; ++j) {
         const int64_t n = col_l + j * 16;
         if (n >= g.N) continue;
-        float* cn = C + n * g.ldc;
+        LT* cn = C + n * g.ldc;
 #pragma unroll
         for (int i = 0; i < MF; ++i) {
           const int64_t m = row_w + i * 16 + lgrp * 4;
           f32x4 v = acc[i][j];
-          if (vec && m + 4 <= g.M) {
-            f32x4* dst = reinterpret_cast<f32x4*>(cn + m);
-            if constexpr (EPI == GemmEpilogue::AccumF32) v = alpha * (*dst + v);
-            else v = alpha * v;
-            *dst = v;
+          if (vec && m + 4 <= M) {
+            if constexpr (Elem<LT>::kSize == 2) {
+              v = alpha * v;
+              *reinterpret_cast<u32x2*>(cn + m) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+            } else {
+              f32x4* dst = reinterpret_cast<f32x4*>(cn + m);
+              if constexpr (EPI == GemmEpilogue::AccumF32) v = alpha * (*dst + v);
+              else v = alpha * v;
+              *dst = v;
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if (m + e < g.M) {
+              if (m + e < M) {
                 float x = v[e];
                 if constexpr (EPI == GemmEpilogue::AccumF32) x = alpha * (cn[m + e] + x);
                 else x = alpha * x;
-                cn[m + e] = x;
+                cn[m + e] = static_cast<LT>(x);
               }
             }
           }
@@ -682,8 +688,8 @@ __device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, const GemmProbl
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int64_t row = row_w + i * 16 + lgrp * 4 + e;
-        if (row >= g.M) continue;
-        float* crow = C + row * g.ldc;
+        if (row >= M) continue;
+        LT* crow = C + row * g.ldc;
 #pragma unroll
         for (int j = 0; j < kFrag; ++j) {
           const int64_t col = col_l + j * 16;
@@ -1195,14 +1201,196 @@ __device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, const GemmProbl
   }
 }
 
-template <typename T, bool AK, bool BK, GemmEpilogue EPI, typename LT, bool CT, bool P3 = false>
+// The epilogue of a logits tile whose logits are not stored (CeStats, CeGrad;
+// accumulators transposed as for Logits: a lane owns 32 columns of each of MF
+// rows, a row's 128 columns of a wave sit in the 4 lanes lrow + 16g).
+//   CeStats: per row max m and Σ e^(x-m), Σ x over the tile's 256 columns, the
+//   two waves' halves merged through LDS, and the label's logit.
+//   CeGrad: d = p·2^(x·log2e - l) - u - y·[label], one fma, one exponential and
+//   one more fma an element, from the fp32 accumulators; stored rounded to bf16
+//   (the backward products' operand: relative 2^-9, independent from element to
+//   element, as the gradient rows of the distillation loss), or, for three-plane
+//   operands, as the three planes of the fp32 value, row r's at C + r*ldc, plane
+//   k another g.ce.plane further. Columns from N up to the multiple of 8 (planes: 64)
+//   are written as zeros, and with planes the rows from M up to the multiple of
+//   64 too: the backward products read them beside zeros.
+// 16 bytes of bf16 a lane leave as in store_swapped, but temporal: the backward
+// products read the piece at once.
+template <GemmEpilogue EPI, int MF, bool P3>
+__device__ __forceinline__ void ce_epilogue(const GemmArgs& g, int64_t M, const GemmProblem& pr,
+                                            const TileCoord& tc, f32x4 (&acc)[MF][kFrag],
+                                            unsigned char* epi, int64_t lab_pre, float4 coef_pre) {
+  constexpr int TM = 32 * MF;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const int lrow = lane & 15, lgrp = lane >> 4;
+  int* lab = reinterpret_cast<int*>(epi);                            // [TM]: column in the tile, or < 0
+  float4* rows4 = reinterpret_cast<float4*>(epi + 4 * TM);           // CeStats [2][TM], CeGrad [TM]
+  if (TM == kThreads || tid < TM) {
+    const int64_t c = lab_pre - g.ce.col0 - tc.n0;
+    lab[tid] = c >= 0 && c < kTile ? static_cast<int>(c) : -1;
+    if constexpr (EPI == GemmEpilogue::CeGrad) rows4[tid] = coef_pre;
+  }
+  __syncthreads();
+  const int cw = wn * 128 + 4 * lgrp;   // this lane's column (j, e) = (0, 0) in the tile
+  const int64_t ncol64 = g.N - tc.n0 - cw;
+  const int ncol = static_cast<int>(ncol64 < 128 ? (ncol64 < 0 ? 0 : ncol64) : 128);
+  auto quad_max = [](float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+  };
+  auto quad_sum = [](float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+  };
+  if constexpr (EPI == GemmEpilogue::CeStats) {
+    auto rows = [&](auto full_c) {
+      constexpr bool kFull = decltype(full_c)::value;
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        f32x4 av[kFrag];
+#pragma unroll
+        for (int j = 0; j < kFrag; ++j) av[j] = from_acc(acc[i][j]);
+        const int rl = wm * (TM / 2) + i * 16 + lrow;
+        const int64_t row = static_cast<int64_t>(tc.m0) + rl;
+        const int yl = lab[rl] - cw;
+        float mx = -INFINITY;
+        if constexpr (kFull) {
+          mx = row_max32(av);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kFrag; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (j * 16 + e < ncol) mx = fmaxf(mx, av[j][e]);
+        }
+        mx = quad_max(mx);
+        // an infinite maximum: e^(x-0) is inf or 0, so the sum is that infinity
+        // or 0 without inf - inf
+        const float ref = fabsf(mx) <= FLT_MAX ? mx : 0.f;
+        const float o1 = -ref * kLog2e;
+        float d1 = 0.f, sx = 0.f;
+#pragma unroll
+        for (int j = 0; j < kFrag; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a1 = __builtin_amdgcn_exp2f(fmaf(av[j][e], kLog2e, o1));
+            if (kFull || j * 16 + e < ncol) {
+              d1 += a1;
+              sx += av[j][e];
+            }
+          }
+        d1 = quad_sum(d1);
+        sx = quad_sum(sx);
+        if (lgrp == 0) rows4[wn * TM + rl] = make_float4(mx == -INFINITY ? mx : ref, d1, sx, 0.f);
+        if (yl >= 0 && yl < 128 && (yl & 12) == 0 && row < M) {   // one lane of a row at most
+          const int jy = yl >> 4, ey = yl & 3;
+          float xy = 0.f;
+#pragma unroll
+          for (int j = 0; j < kFrag; ++j) {
+            float t = av[j][0];
+            t = ey == 1 ? av[j][1] : t;
+            t = ey == 2 ? av[j][2] : t;
+            t = ey == 3 ? av[j][3] : t;
+            xy = jy == j ? t : xy;
+          }
+          g.ce.xy[row] = xy;
+        }
+      }
+    };
+    if (tc.n0 + kTile <= g.N) rows(SlotC<1>{});
+    else rows(SlotC<0>{});
+    __syncthreads();
+    if ((TM == kThreads || tid < TM) && tc.m0 + tid < M) {
+      const float4 a = rows4[tid], b = rows4[TM + tid];
+      const float m = fmaxf(a.x, b.x);
+      float4 s = make_float4(m, 0.f, a.z + b.z, 0.f);
+      if (a.x != -INFINITY) s.y += a.y * __builtin_amdgcn_exp2f((a.x - m) * kLog2e);
+      if (b.x != -INFINITY) s.y += b.y * __builtin_amdgcn_exp2f((b.x - m) * kLog2e);
+      // an infinite or NaN sum stays one, whatever it is scaled by
+      if (!(a.y + b.y <= FLT_MAX)) s.y = a.y + b.y;
+      g.ce.stats[(tc.m0 + tid) * g.ce.stats_ld + tc.ntile] = s;
+    }
+  } else {
+    const int64_t npad = P3 ? (g.N + 63) / 64 * 64 : (g.N + 7) / 8 * 8;
+    const int64_t wcol64 = npad - tc.n0 - cw;
+    const int wcol = static_cast<int>(wcol64 < 128 ? (wcol64 < 0 ? 0 : wcol64) : 128);
+    const int64_t mpad = P3 ? (M + 63) / 64 * 64 : M;
+    __bf16* C = static_cast<__bf16*>(pr.c);
+    auto rows = [&](auto full_c) {
+      constexpr bool kFull = decltype(full_c)::value;
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        f32x4 av[kFrag];
+#pragma unroll
+        for (int j = 0; j < kFrag; ++j) av[j] = from_acc(acc[i][j]);
+        const int rl = wm * (TM / 2) + i * 16 + lrow;
+        const int64_t row = static_cast<int64_t>(tc.m0) + rl;
+        const int yl = lab[rl] - cw;
+        const float4 c = rows4[rl];
+        const bool live = !P3 || row < M;
+#pragma unroll
+        for (int j = 0; j < kFrag; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float d = fmaf(c.y, __builtin_amdgcn_exp2f(fmaf(av[j][e], kLog2e, -c.x)), -c.z);
+            if (j * 16 + e == yl) d -= c.w;
+            av[j][e] = (kFull || j * 16 + e < ncol) && live ? d : 0.f;
+          }
+        __bf16* crow = C + row * g.ldc + tc.n0 + wn * 128;
+        if constexpr (P3) {
+          if (row < mpad) {
+#pragma unroll
+            for (int j = 0; j < kFrag; ++j) {
+              if (!kFull && j * 16 >= wcol) continue;   // npad is a multiple of 4
+              uint32_t lo[3], hi[3];
+              split3_pack(av[j][0], av[j][1], lo);
+              split3_pack(av[j][2], av[j][3], hi);
+#pragma unroll
+              for (int k = 0; k < 3; ++k)
+                *reinterpret_cast<u32x2*>(crow + k * g.ce.plane + 4 * lgrp + 16 * j) = u32x2{lo[k], hi[k]};
+            }
+          }
+        } else if constexpr (kFull) {
+          u32x4 w[kFrag / 2];
+#pragma unroll
+          for (int jp = 0; jp < kFrag; jp += 2) {
+            const auto a = __builtin_amdgcn_permlane16_swap(pack_bf16(av[jp][0], av[jp][1]),
+                                                            pack_bf16(av[jp + 1][0], av[jp + 1][1]), false, false);
+            const auto b = __builtin_amdgcn_permlane16_swap(pack_bf16(av[jp][2], av[jp][3]),
+                                                            pack_bf16(av[jp + 1][2], av[jp + 1][3]), false, false);
+            w[jp / 2] = u32x4{a[0], b[0], a[1], b[1]};
+          }
+          if (row < M) {
+            const int c0 = 16 * (lgrp & 1) + 8 * (lgrp >> 1);
+#pragma unroll
+            for (int jp = 0; jp < kFrag; jp += 2) *reinterpret_cast<u32x4*>(crow + 16 * jp + c0) = w[jp / 2];
+          }
+        } else if (row < M) {
+#pragma unroll
+          for (int j = 0; j < kFrag; ++j)
+            if (j * 16 < wcol)   // npad is a multiple of 4
+              *reinterpret_cast<u32x2*>(crow + 4 * lgrp + 16 * j) =
+                  u32x2{pack_bf16(av[j][0], av[j][1]), pack_bf16(av[j][2], av[j][3])};
+        }
+      }
+    };
+    if (tc.n0 + kTile <= g.N) rows(SlotC<1>{});
+    else rows(SlotC<0>{});
+  }
+}
+
+template <typename T, bool AK, bool BK, GemmEpilogue EPI, typename LT, bool CT, bool P3 = false, bool DYN = false>
 __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
   static_assert(!P3 || Elem<T>::kSize == 2, "three-plane operands are bf16");
   // The logits epilogues: the product's own rows (Logits), or student rows
   // beside teacher logits read from memory (LogitsTeacher: fp32,
   // LogitsTeacher16: bf16).
   constexpr bool kTeacherEpi = EPI == GemmEpilogue::LogitsTeacher || EPI == GemmEpilogue::LogitsTeacher16;
-  constexpr bool kLogitsEpi = EPI == GemmEpilogue::Logits || kTeacherEpi;
+  constexpr bool kCeEpi = EPI == GemmEpilogue::CeStats || EPI == GemmEpilogue::CeGrad;
+  constexpr bool kLogitsEpi = EPI == GemmEpilogue::Logits || kTeacherEpi || kCeEpi;
   // Ring layout: A tiles of slots 0-3, then B tiles of slots 0-3 (16 KB
   // each), so every slot offset fits a DS instruction's immediate.
   // (Three-plane operands: two slots of 32 KB for B's planes, then three for
@@ -1218,15 +1406,30 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
   // Split K: workgroup s*T + t computes tile t over K range
   // [s*split_len, (s+1)*split_len) into split s's partial buffer.
   const int64_t tiles = ((g.M + kTile - 1) / kTile) * ((g.N + kTile - 1) / kTile) * g.nprob;
-  int64_t lin = blockIdx.x, kbeg = 0, Kl = g.K;
+  // The rows that only the device knows (dyn_rows): M, or K of a product stored
+  // transposed (three planes: up to whole 64s, which are zero past them).
+  int64_t M = g.M, K = g.K;
+  if constexpr (DYN) {
+    const int64_t n = *g.dyn_rows;
+    if constexpr (CT) K = P3 ? (n + 63) / 64 * 64 : n;
+    else M = n;
+  }
+  int64_t lin = blockIdx.x, kbeg = 0, Kl = K;
   int split = 0;
   if (g.split_k > 1) {
     split = static_cast<int>(lin / tiles);
     lin -= static_cast<int64_t>(split) * tiles;
     kbeg = static_cast<int64_t>(split) * g.split_len;
-    Kl = g.K - kbeg < g.split_len ? g.K - kbeg : g.split_len;
+    Kl = K - kbeg < g.split_len ? K - kbeg : g.split_len;
   }
-  const TileCoord tc = map_tile(g, lin);
+  if constexpr (DYN) {
+    if constexpr (CT) {
+      if (Kl < 0) Kl = 0;   // a part past the rows: zeros
+    } else {
+      if (lin >= (M + kTile - 1) / kTile * ((g.N + kTile - 1) / kTile)) return;
+    }
+  }
+  const TileCoord tc = map_tile(g, M, lin);
   GemmProblem pr = g.prob[tc.p];
   if (g.split_k > 1) {
     constexpr int ES = Elem<T>::kSize;
@@ -1243,7 +1446,7 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
         return;
       }
     }
-    l.init(pr.a, g.lda, g.M, Kl, tc.m0, wave, lane);
+    l.init(pr.a, g.lda, M, Kl, tc.m0, wave, lane);
   };
   // B loader over this workgroup's K range.
   using LoaderB = Loader<T, BK>;
@@ -1254,12 +1457,24 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
   // epilogue's out_row). A global (not flat) load: a flat load would also
   // count in lgkmcnt and turn the main loop's LDS waits into lgkmcnt(0).
   int64_t lab_pre = 0;
-  if constexpr (kLogitsEpi) {
+  float4 coef_pre = make_float4(0.f, 0.f, 0.f, 0.f);
+  if constexpr (kCeEpi) {
+    typedef __attribute__((address_space(1))) const int64_t global_i64;
+    typedef __attribute__((address_space(1))) const f32x4 global_f32x4;
+    const int64_t R = static_cast<int64_t>(tc.m0) + tid;
+    lab_pre = R < M ? *(global_i64*)(reinterpret_cast<uintptr_t>(g.ce.labels + R)) : -1;
+    if constexpr (EPI == GemmEpilogue::CeGrad) {
+      if (R < M) {
+        const f32x4 c = *(global_f32x4*)(reinterpret_cast<uintptr_t>(g.ce.coef + R));
+        coef_pre = make_float4(c[0], c[1], c[2], c[3]);
+      }
+    }
+  } else if constexpr (kLogitsEpi) {
     typedef __attribute__((address_space(1))) const int64_t global_i64;
     const int64_t R = static_cast<int64_t>(tc.m0) + tid;
     const int64_t prs = g.lg.pair_rows;
     const int64_t r = prs > 0 ? ((R >> 5) << 4) + (R & 15) : R;
-    const bool ok = prs > 0 ? r < prs : R < g.M;
+    const bool ok = prs > 0 ? r < prs : R < M;
     lab_pre = ok ? *(global_i64*)(reinterpret_cast<uintptr_t>(g.lg.labels + r)) : g.lg.ignore_index;
   }
 
@@ -1326,7 +1541,7 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
       // Past the last block the moves re-read it, into slots nobody reads.
       PairLoader<AK> pa;
       PairLoader<BK> pb;
-      pa.init(pr.a, g.lda, g.M, tc.m0, wave, lane);
+      pa.init(pr.a, g.lda, M, tc.m0, wave, lane);
       pb.init(pr.b, g.ldb, g.N, tc.n0, wave, lane);
       const int nkb = static_cast<int>(Kl / 64);
       FragReader<AK, AK> f3a;
@@ -1496,7 +1711,7 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
       if (EPI == GemmEpilogue::Logits && g.lg.pair_rows > 0)
         pa.init_paired(pr.a, g.lg.pair_teacher, g.lda, g.lg.pair_rows, tc.m0 >> 1, wave, lane);
       else
-        pa.init(pr.a, g.lda, g.M, tc.m0, wave, lane);
+        pa.init(pr.a, g.lda, M, tc.m0, wave, lane);
       pb.init(pr.b, g.ldb, g.N, tc.n0, wave, lane);
       const int np = nkf / 2;
       // Transfer x (0-7 A, 8-15 B) of a pair's DMA into double slot D, from
@@ -1640,7 +1855,7 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
       const int np = nkf / 2;
       const int ns = 2 * np;
       PairLoader<AK> pa;
-      pa.init(pr.a, g.lda, g.M, tc.m0, wave, lane);
+      pa.init(pr.a, g.lda, M, tc.m0, wave, lane);
       LoaderB lb;
       init_b(lb);
       // Transfer x (0-7) of an A pair into double slot D.
@@ -1840,7 +2055,8 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
   __builtin_amdgcn_s_waitcnt(kWaitAll);
   __builtin_amdgcn_s_barrier();
 
-  gemm_epilogue<Elem<T>::kSize, EPI, LT, CT, kFrag>(g, pr, tc, acc, epi, smem, lab_pre);
+  if constexpr (kCeEpi) ce_epilogue<EPI, kFrag, P3>(g, M, pr, tc, acc, epi, lab_pre, coef_pre);
+  else gemm_epilogue<Elem<T>::kSize, EPI, LT, CT, kFrag>(g, M, pr, tc, acc, epi, smem, lab_pre);
 }
 
 
@@ -1861,32 +2077,44 @@ constexpr int kMidA = kMidM * kSlab;            // bytes of A a stage
 constexpr int kMidRing = 3;
 constexpr int kMidX = kXfers + kXfers / 2;      // transfers per thread and stage
 
-template <bool BK, GemmEpilogue EPI, typename LT, bool CT>
+template <bool BK, GemmEpilogue EPI, typename LT, bool CT, bool DYN = false>
 __device__ __forceinline__ void mid_body(const GemmArgs& g) {
+  constexpr bool kCeEpi = EPI == GemmEpilogue::CeStats || EPI == GemmEpilogue::CeGrad;
   constexpr bool kLogitsEpi = EPI == GemmEpilogue::Logits || EPI == GemmEpilogue::LogitsTeacher ||
-                              EPI == GemmEpilogue::LogitsTeacher16;
+                              EPI == GemmEpilogue::LogitsTeacher16 || kCeEpi;
   // A tiles of slots 0-2, then B tiles of slots 0-2.
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kMidRing * (kMidA + kOpBytes)];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  const int64_t Kl = g.K;
-  const TileCoord tc = map_tile<kMidM>(g, blockIdx.x);
+  int64_t M = g.M, Kl = g.K;   // as in gemm_body
+  if constexpr (DYN) {
+    if constexpr (CT) Kl = *g.dyn_rows;
+    else M = *g.dyn_rows;
+    if (!CT && blockIdx.x >= (M + kMidM - 1) / kMidM * ((g.N + kTile - 1) / kTile)) return;
+  }
+  const TileCoord tc = map_tile<kMidM>(g, M, blockIdx.x);
   const GemmProblem pr = g.prob[tc.p];
   Loader<__bf16, true, kXfers / 2> la;
   Loader<__bf16, BK> lb;
   if (EPI == GemmEpilogue::Logits && g.lg.pair_rows > 0)
     la.init_paired(pr.a, g.lg.pair_teacher, g.lda, g.lg.pair_rows, Kl, tc.m0 >> 1, wave, lane);
   else
-    la.init(pr.a, g.lda, g.M, Kl, tc.m0, wave, lane);
+    la.init(pr.a, g.lda, M, Kl, tc.m0, wave, lane);
   lb.init(pr.b, g.ldb, g.N, Kl, tc.n0, wave, lane);
   int64_t lab_pre = 0;   // as in gemm_body
-  if constexpr (kLogitsEpi) {
+  float4 coef_pre = make_float4(0.f, 0.f, 0.f, 0.f);
+  if constexpr (kCeEpi) {
+    const int64_t R = static_cast<int64_t>(tc.m0) + tid;
+    const bool ok = tid < kMidM && R < M;
+    lab_pre = ok ? g.ce.labels[R] : -1;
+    if (EPI == GemmEpilogue::CeGrad && ok) coef_pre = g.ce.coef[R];
+  } else if constexpr (kLogitsEpi) {
     const int64_t R = static_cast<int64_t>(tc.m0) + tid;
     const int64_t prs = g.lg.pair_rows;
     const int64_t r = prs > 0 ? ((R >> 5) << 4) + (R & 15) : R;
-    const bool ok = tid < kMidM && (prs > 0 ? r < prs : R < g.M);
+    const bool ok = tid < kMidM && (prs > 0 ? r < prs : R < M);
     lab_pre = ok ? g.lg.labels[r] : g.lg.ignore_index;
   }
   f32x4 acc[kMidFrag][kFrag];
@@ -1967,7 +2195,8 @@ __device__ __forceinline__ void mid_body(const GemmArgs& g) {
   for (int i = 0; i < kMidFrag; ++i)
 #pragma unroll
     for (int j = 0; j < kFrag; ++j) asm volatile("" : "+a"(acc[i][j]));
-  gemm_epilogue<2, EPI, LT, CT, kMidFrag>(g, pr, tc, acc, smem, smem, lab_pre);
+  if constexpr (kCeEpi) ce_epilogue<EPI, kMidFrag, false>(g, M, pr, tc, acc, smem, lab_pre, coef_pre);
+  else gemm_epilogue<2, EPI, LT, CT, kMidFrag>(g, M, pr, tc, acc, smem, smem, lab_pre);
 }
 
 // One named entry point per variant, so that profiles and the build's ISA
@@ -2013,11 +2242,58 @@ ORDA_MID(gemm_kmt_mid_store_bf16, false, GemmEpilogue::StoreF32, float, true)
 ORDA_MID(gemm_kmt_mid_accum_bf16, false, GemmEpilogue::AccumF32, float, true)
 #undef ORDA_MID
 
+// The linear cross entropy's products, over rows that only the device counts
+// (GemmArgs::dyn_rows): gemm_<layouts>_[mid_]<ce epilogue, or dyn_ and the
+// epilogue>_<operands>[_<C's type>].
+#define ORDA_CE(NAME, BK, EPI, LT, CT, P3) \
+  __global__ __launch_bounds__(kThreads, 1) void NAME(GemmArgs g) { gemm_body<__bf16, true, BK, EPI, LT, CT, P3, true>(g); }
+ORDA_CE(gemm_kk_cestats_bf16, true, GemmEpilogue::CeStats, float, false, false)
+ORDA_CE(gemm_kk_cegrad_bf16, true, GemmEpilogue::CeGrad, __bf16, false, false)
+ORDA_CE(gemm_km_dyn_store_bf16, false, GemmEpilogue::StoreF32, float, false, false)
+ORDA_CE(gemm_km_dyn_accum_bf16, false, GemmEpilogue::AccumF32, float, false, false)
+ORDA_CE(gemm_kmt_dyn_store_bf16, false, GemmEpilogue::StoreF32, float, true, false)
+ORDA_CE(gemm_kmt_dyn_store_bf16_bf16, false, GemmEpilogue::StoreF32, __bf16, true, false)
+ORDA_CE(gemm_kk_cestats_bf16x3, true, GemmEpilogue::CeStats, float, false, true)
+ORDA_CE(gemm_kk_cegrad_bf16x3, true, GemmEpilogue::CeGrad, float, false, true)
+ORDA_CE(gemm_km_dyn_store_bf16x3, false, GemmEpilogue::StoreF32, float, false, true)
+ORDA_CE(gemm_km_dyn_accum_bf16x3, false, GemmEpilogue::AccumF32, float, false, true)
+ORDA_CE(gemm_kmt_dyn_store_bf16x3, false, GemmEpilogue::StoreF32, float, true, true)
+#undef ORDA_CE
+#define ORDA_CE_MID(NAME, BK, EPI, LT, CT) \
+  __global__ __launch_bounds__(kThreads, 2) void NAME(GemmArgs g) { mid_body<BK, EPI, LT, CT, true>(g); }
+ORDA_CE_MID(gemm_kk_mid_cestats_bf16, true, GemmEpilogue::CeStats, float, false)
+ORDA_CE_MID(gemm_kk_mid_cegrad_bf16, true, GemmEpilogue::CeGrad, __bf16, false)
+ORDA_CE_MID(gemm_kmt_mid_dyn_store_bf16_bf16, false, GemmEpilogue::StoreF32, __bf16, true)
+#undef ORDA_CE_MID
+
 typedef void (*GemmKernel)(GemmArgs);
+
+// Products over dyn_rows rows (launch_gemm has checked that the operands are bf16).
+GemmKernel select_dyn(const GemmArgs& g, bool mid) {
+  using E = GemmEpilogue;
+  const bool p3 = g.plane_a > 0, st = g.epi == E::StoreF32;
+  if (g.epi == E::CeStats || g.epi == E::CeGrad) {
+    if (!g.b_kmajor || g.c_trans) return nullptr;
+    if (g.epi == E::CeStats) return p3 ? gemm_kk_cestats_bf16x3 : mid ? gemm_kk_mid_cestats_bf16 : gemm_kk_cestats_bf16;
+    return p3 ? gemm_kk_cegrad_bf16x3 : mid ? gemm_kk_mid_cegrad_bf16 : gemm_kk_cegrad_bf16;
+  }
+  if (g.b_kmajor) return nullptr;
+  if (!g.c_trans) {
+    if (g.epi != E::StoreF32 && g.epi != E::AccumF32) return nullptr;
+    if (p3) return st ? gemm_km_dyn_store_bf16x3 : gemm_km_dyn_accum_bf16x3;
+    return st ? gemm_km_dyn_store_bf16 : gemm_km_dyn_accum_bf16;
+  }
+  if (!st) return nullptr;
+  if (p3) return g.c_type == DType::F32 ? gemm_kmt_dyn_store_bf16x3 : nullptr;
+  if (g.c_type == DType::F32) return gemm_kmt_dyn_store_bf16;
+  return mid ? gemm_kmt_mid_dyn_store_bf16_bf16 : gemm_kmt_dyn_store_bf16_bf16;
+}
 
 GemmKernel select_kernel(const GemmArgs& g, bool mid) {
   using E = GemmEpilogue;
   const bool bf = g.in_type == DType::BF16;
+  if (g.dyn_rows != nullptr) return select_dyn(g, mid);
+  if (g.epi == E::CeStats || g.epi == E::CeGrad || g.c_type != DType::F32) return nullptr;
   if (mid) {   // mid_tiles(g)
     if (g.c_trans) return g.epi == E::StoreF32 ? gemm_kmt_mid_store_bf16 : gemm_kmt_mid_accum_bf16;
     return g.logits_type == DType::BF16 ? gemm_kk_mid_logits_bf16_bf16 : gemm_kk_mid_logits_bf16_f32;
@@ -2058,9 +2334,10 @@ GemmKernel select_kernel(const GemmArgs& g, bool mid) {
 // columns of one row with 16-byte loads, and stores them with one 16-byte
 // store where C's pitch and base allow. The split loop is unrolled so that
 // its loads are in flight together; the additions stay in split order.
+template <typename CE = float>
 __global__ __launch_bounds__(256) void splitk_reduce_kernel(
     const float* ws, int64_t stride, int splits, int64_t rows, int64_t cols, int64_t ldp,
-    float* c0, float* c1, int64_t ldc, float alpha0, const float* alpha_ptr, bool accum) {
+    CE* c0, CE* c1, int64_t ldc, float alpha0, const float* alpha_ptr, bool accum) {
   const float alpha = alpha_ptr != nullptr ? alpha0 * *alpha_ptr : alpha0;
   const int64_t quads = (cols + 3) / 4;
   const int64_t per = rows * quads;
@@ -2078,8 +2355,15 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(
     f32x4 v = src[0];
 #pragma unroll 8
     for (int s = 1; s < splits; ++s) v += src[s * sq];
-    float* dst = (p ? c1 : c0) + r * ldc + q;
-    if (vec && q + 4 <= cols) {
+    CE* dst = (p ? c1 : c0) + r * ldc + q;
+    if constexpr (sizeof(CE) == 2) {   // bf16: a store only (GemmArgs::c_type)
+      if (vec && q + 4 <= cols) {
+        v = alpha * v;
+        *reinterpret_cast<u32x2*>(dst) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+      } else {
+        for (int k = 0; k < 4 && q + k < cols; ++k) dst[k] = static_cast<CE>(alpha * v[k]);
+      }
+    } else if (vec && q + 4 <= cols) {
       f32x4* d4 = reinterpret_cast<f32x4*>(dst);
       *d4 = accum ? alpha * (*d4 + v) : alpha * v;
     } else {
@@ -2207,6 +2491,10 @@ struct SplitPlan {
 };
 int64_t split_cap(const GemmArgs& g) { return g.split_cap > 0 ? g.split_cap : int64_t{256} << 20; }
 
+bool logits_epilogue(const GemmArgs& g) {   // a product over the vocabulary's columns, never split
+  return g.epi == GemmEpilogue::Logits || g.epi == GemmEpilogue::CeStats || g.epi == GemmEpilogue::CeGrad;
+}
+
 // Shared-round blocks (map_tile) for a product with share_rounds set: xn in
 // {1, 2, 4, 8} dividing the N-tiles, b = Nt/xn, a = 32/b; the most tiles per
 // XCD (at least 24), then the fewest operand strips per stage (a + b), then
@@ -2254,7 +2542,7 @@ void set_share_blocks(GemmArgs& g) {
 // already walks N twice with 128 MB live: equal).
 void set_band_blocks(GemmArgs& g) {
   constexpr int64_t kBandLive = int64_t{192} << 20, kBandMax = int64_t{128} << 20;
-  if (g.sh_a > 0 || g.epi != GemmEpilogue::Logits || g.in_type != DType::BF16) return;
+  if (g.sh_a > 0 || !logits_epilogue(g) || g.in_type != DType::BF16) return;
   const int64_t Mv = ((g.M + kTile - 1) / kTile) * g.nprob;
   const int64_t Nt = (g.N + kTile - 1) / kTile;
   const int64_t strip = int64_t{kTile} * g.K * (g.plane_a > 0 ? 6 : 2);
@@ -2292,7 +2580,7 @@ int64_t tile_count(const GemmArgs& g) {
 // against 594.)
 SplitPlan plan_split(const GemmArgs& g) {
   SplitPlan sp{1, g.K, 0, 0, 0, 0.0};
-  if (g.epi == GemmEpilogue::Logits || g.M <= 0 || g.N <= 0 || g.K <= 0) return sp;
+  if (logits_epilogue(g) || g.M <= 0 || g.N <= 0 || g.K <= 0) return sp;
   const int64_t tiles = tile_count(g);
   const int64_t per_split = g.nprob * (g.c_trans ? g.N * ((g.M + 3) / 4 * 4) : g.M * ((g.N + 3) / 4 * 4)) * 4;
   int64_t most = tiles < 192 ? (256 + tiles - 1) / tiles : 8;
@@ -2671,7 +2959,7 @@ hipError_t launch_small(const GemmArgs& g, hipStream_t stream) {
     if (g.partials_only) return hipGetLastError();
     const int64_t total = rows * ((cols + 3) / 4) * g.nprob;
     const unsigned blocks = static_cast<unsigned>((total + 255) / 256 < 8192 ? (total + 255) / 256 : 8192);
-    hipLaunchKernelGGL(splitk_reduce_kernel, dim3(blocks), dim3(256), 0, stream, g.split_ws,
+    hipLaunchKernelGGL(splitk_reduce_kernel<float>, dim3(blocks), dim3(256), 0, stream, g.split_ws,
                        sp.stride, sp.splits, rows, cols, sp.ldp, static_cast<float*>(g.prob[0].c),
                        g.nprob > 1 ? static_cast<float*>(g.prob[1].c) : nullptr, g.ldc, g.alpha,
                        g.alpha_ptr, g.epi == GemmEpilogue::AccumF32);
@@ -2755,8 +3043,8 @@ GemmArgs sub_product(const GemmArgs& g, int64_t r0, int64_t r1, int64_t c0, int6
   for (int p = 0; p < g.nprob; ++p) {
     t.prob[p].a = static_cast<const unsigned char*>(g.prob[p].a) + (g.a_kmajor ? r0 * g.lda : r0) * es;
     t.prob[p].b = static_cast<const unsigned char*>(g.prob[p].b) + (g.b_kmajor ? c0 * g.ldb : c0) * es;
-    t.prob[p].c = static_cast<float*>(g.prob[p].c) +
-                  (g.c_trans ? c0 * g.ldc + r0 : r0 * g.ldc + c0);
+    t.prob[p].c = static_cast<unsigned char*>(g.prob[p].c) +
+                  (g.c_trans ? c0 * g.ldc + r0 : r0 * g.ldc + c0) * dtype_size(g.c_type);
   }
   return t;
 }
@@ -2777,7 +3065,7 @@ struct TailSplit {
 };
 TailSplit plan_tail(const GemmArgs& g) {
   const TailSplit none{0, false};
-  if (g.epi == GemmEpilogue::Logits || g.split_k > 1 || g.M <= 0 || g.N <= 0) return none;
+  if (logits_epilogue(g) || g.split_k > 1 || g.M <= 0 || g.N <= 0) return none;
   const int64_t Mt = (g.M + kTile - 1) / kTile, Nt = (g.N + kTile - 1) / kTile;
   const int64_t Mv = Mt * g.nprob;
   const int64_t T = Mv * Nt, q = T / 256, r = T % 256;
@@ -2790,7 +3078,7 @@ TailSplit plan_tail(const GemmArgs& g) {
   };
   const int64_t n0 = 256 * q / Mv * kTile;
   if (n0 > 0 && n0 < g.N && pays(sub_product(g, 0, g.M, n0, g.N))) return {n0, true};
-  if ((256 * q) % (Nt * g.nprob) == 0) {
+  if ((256 * q) % (Nt * g.nprob) == 0 && (g.dyn_rows == nullptr || g.c_trans)) {
     const int64_t m0 = 256 * q / (Nt * g.nprob) * kTile;
     if (m0 < g.M && pays(sub_product(g, m0, g.M, 0, g.N))) return {m0, false};
   }
@@ -2849,7 +3137,8 @@ namespace {
 // against 84, 300 x 512 x 50257 80 against 60; at 2000 x 1536 x 128256, where
 // the rule keeps the larger tile, 737 against 957.
 bool mid_tiles(const GemmArgs& g) {
-  const bool logits = g.epi == GemmEpilogue::Logits;
+  const bool logits = logits_epilogue(g);
+  if (g.dyn_rows != nullptr && !logits && g.c_type == DType::F32) return false;   // not built: partials only
   if (g.in_type != DType::BF16 || g.plane_a > 0 || !g.a_kmajor || g.M <= 0 || g.N <= 0) return false;
   if (logits ? (!g.b_kmajor || g.c_trans || g.lg.teacher_logits != nullptr) : (g.b_kmajor || !g.c_trans))
     return false;
@@ -2875,8 +3164,10 @@ namespace {
 // may run on the small kernel.
 hipError_t launch_gemm_impl(const GemmArgs& g, hipStream_t stream, bool whole) {
   if (g.nprob < 1 || g.nprob > 2) return hipErrorInvalidValue;
-  if ((g.lda % 8) || (g.ldb % 8) || (g.ldc % 8 && g.epi == GemmEpilogue::Logits))
+  if ((g.lda % 8) || (g.ldb % 8) || (g.ldc % 8 && logits_epilogue(g) && g.prob[0].c != nullptr))
     return hipErrorInvalidValue;
+  if (g.dyn_rows != nullptr && (g.nprob != 1 || g.in_type != DType::BF16 || g.partials_only)) return hipErrorInvalidValue;
+  if (g.c_type != DType::F32 && (!g.c_trans || g.epi != GemmEpilogue::StoreF32)) return hipErrorInvalidValue;
   if (g.epi == GemmEpilogue::Logits && g.lg.pair_rows > 0 &&
       (g.nprob != 1 || g.lg.cross == nullptr || g.lg.pair_teacher == nullptr ||
        g.in_type != DType::BF16 || g.M != 2 * ((g.lg.pair_rows + 15) / 16 * 16)))
@@ -2920,6 +3211,7 @@ hipError_t launch_gemm_impl(const GemmArgs& g, hipStream_t stream, bool whole) {
     // orientation, then one reduction applying the requested epilogue.
     GemmArgs s = gr;
     s.epi = GemmEpilogue::StoreF32;
+    s.c_type = DType::F32;
     s.alpha = 1.f;
     s.alpha_ptr = nullptr;
     s.ldc = sp.ldp;
@@ -2935,7 +3227,13 @@ hipError_t launch_gemm_impl(const GemmArgs& g, hipStream_t stream, bool whole) {
     if (g.partials_only) return hipGetLastError();
     const int64_t total = rows * ((cols + 3) / 4) * g.nprob;
     const unsigned blocks = static_cast<unsigned>((total + 255) / 256 < 8192 ? (total + 255) / 256 : 8192);
-    hipLaunchKernelGGL(splitk_reduce_kernel, dim3(blocks), dim3(256), 0, stream, g.split_ws,
+    if (g.c_type == DType::BF16) {
+      hipLaunchKernelGGL(splitk_reduce_kernel<__bf16>, dim3(blocks), dim3(256), 0, stream, g.split_ws,
+                         sp.stride, sp.splits, rows, cols, sp.ldp, static_cast<__bf16*>(g.prob[0].c),
+                         static_cast<__bf16*>(nullptr), g.ldc, g.alpha, g.alpha_ptr, false);
+      return hipGetLastError();
+    }
+    hipLaunchKernelGGL(splitk_reduce_kernel<float>, dim3(blocks), dim3(256), 0, stream, g.split_ws,
                        sp.stride, sp.splits, rows, cols, sp.ldp, static_cast<float*>(g.prob[0].c),
                        g.nprob > 1 ? static_cast<float*>(g.prob[1].c) : nullptr, g.ldc, g.alpha,
                        g.alpha_ptr, g.epi == GemmEpilogue::AccumF32);

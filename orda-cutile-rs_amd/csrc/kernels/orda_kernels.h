@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace orda {
 
 enum class DType : int { F32 = 0, BF16 = 1 };
@@ -29,6 +31,10 @@ enum class GemmEpilogue : int {
   LogitsTeacher = 3,   // internal: a Logits product with fp32 lg.teacher_logits
   LogitsTeacher16 = 4, // internal: a Logits product with bf16 lg.teacher_logits
                        // (launch_gemm selects it; callers pass Logits)
+  CeStats = 5,     // logits that are not stored: per-row partial softmax
+                   // statistics of every 256-column tile and the label logit
+  CeGrad = 6,      // C = gradient of the logits, formed from the row's
+                   // log-sum-exp (CeArgs::coef); C in logits_type
 };
 
 struct GemmProblem {
@@ -84,6 +90,23 @@ struct LogitStatsArgs {
   DType teacher_type;
 };
 
+// The CeStats and CeGrad epilogues (one problem, bf16 operands, K-major both):
+// columns 0..N of the product are vocabulary columns col0..col0+N.
+struct CeArgs {
+  // CeStats: stats[m*stats_ld + n_tile] = {max, Σe^(x-max), Σx, 0} (max -inf
+  // and sum 0 where every logit is -inf; max 0 where the maximum is +inf)
+  float4* stats;
+  int64_t stats_ld;       // in float4 units, >= ceil(N/256)
+  float* xy;              // xy[m] = fp32 logit at the row's label column
+  const int64_t* labels;  // label column of row m
+  int64_t col0;
+  // CeGrad: with {l, p, u, y} = coef[m], column v's gradient is
+  // p·2^(x·log2e - l) - u, minus y at the label. Three-plane operands: C is
+  // three-plane rows, ldc elements apart, the planes `plane` elements apart.
+  const float4* coef;
+  int64_t plane;
+};
+
 struct GemmArgs {
   int nprob;              // 1 or 2
   GemmProblem prob[2];
@@ -130,6 +153,14 @@ struct GemmArgs {
   // fp32 operands: keep to the fp32 MFMA where launch_gemm would split the
   // values into planes itself (small products).
   bool fp32_mfma;
+  // Store with c_trans and bf16 operands: C's type (partials stay fp32).
+  DType c_type;
+  // When set (bf16 operands, one problem; CeStats, CeGrad, Store and Accum
+  // only), the number of rows is *dyn_rows, at most the M that is passed
+  // (c_trans: at most K). Tiles past it return at once. c_trans: A is finite up
+  // to the multiple of 8 at *dyn_rows.
+  const int64_t* dyn_rows;
+  CeArgs ce;
 };
 
 hipError_t launch_gemm(const GemmArgs& g, hipStream_t stream);
@@ -376,5 +407,47 @@ hipError_t launch_convert_rows(DType src_t, const void* src, int64_t lds, DType 
 // rows_pad, from row rows on.
 hipError_t launch_split3_rows(const float* src, int64_t lds, int64_t rows, int64_t cols, void* dst,
                               int64_t rows_pad, int64_t plane, hipStream_t stream);
+
+// ---------------------------------------------------------------- linear cross entropy
+// The rows of a call that have a label, in order: row src[i] with class
+// labels[i] (-1: a label that is no class) for i < *count, and each row's place
+// pos[r] among them (-1: ignored).
+struct CeRows {
+  int64_t* count;
+  int32_t* src;
+  int64_t* labels;
+  int32_t* pos;
+};
+// Fills r from n labels; with nll, also zeroes nll and lse of the ignored rows.
+hipError_t launch_ce_rows(const int64_t* labels, int64_t n, int64_t v, int64_t ignore, const CeRows& r, float* nll,
+                          float* lse, hipStream_t stream);
+// The gradients into the losses and log-sum-exps of all rows (each may be
+// null: 0) and the compact rows' coefficients made of them (null: none).
+struct CeGradRows {
+  const float *lse, *grad_nll, *grad_lse;
+  float smooth_each, target;   // label_smoothing / V, 1 - label_smoothing
+  float4* coef;
+};
+// Hidden rows [n][h] to compact rows of pitch ldd (a multiple of 8), zeros past
+// h and in the rows from the count to the next multiple of 64 (dst holds
+// round64(n) rows).
+hipError_t launch_ce_gather(DType t, const void* x, int64_t ldx, int64_t n, int64_t h, const CeRows& r, void* dst,
+                            int64_t ldd, const CeGradRows& g, hipStream_t stream);
+// Merges a piece's tile statistics (CeArgs::stats) into state (between
+// pieces) and on the last piece writes the rows' losses.
+struct CeLossArgs {
+  CeRows rows;
+  const float4* stats;
+  int64_t stats_ld, tiles;
+  float4* state;
+  bool first, last;
+  const float* xy;
+  float smooth_each, target;
+  float *nll, *lse;
+};
+hipError_t launch_ce_losses(const CeLossArgs& a, int64_t n, hipStream_t stream);
+// dst[r] = src[pos[r]] in type t, or zeros where pos[r] < 0 (pos null: everywhere).
+hipError_t launch_ce_scatter(const float* src, int64_t lds, const int32_t* pos, int64_t rows, int64_t h, DType t,
+                             void* dst, int64_t ldd, hipStream_t stream);
 
 }  // namespace orda

@@ -76,6 +76,12 @@ class ScaledGradient(C.Structure):
                 ("dst_dtype", C.c_int32)]
 
 
+class LinearCeC(C.Structure):
+    _fields_ = [("hidden", Tensor), ("weight", Tensor), ("labels", C.c_void_p),
+                ("n_labels", C.c_int64), ("ignore_index", C.c_int64),
+                ("label_smoothing", C.c_float), ("vocab_piece", C.c_int64)]
+
+
 # (name, restype, argtypes) for every entry point of include/orda/orda.h.
 SIGNATURES = [
     ("orda_abi_version", C.c_int32, []),
@@ -123,6 +129,14 @@ SIGNATURES = [
     ("orda_scale_gradients", C.c_int32,
      [C.c_int32, C.c_void_p, C.c_void_p, C.POINTER(ScaledGradient), C.c_int32, C.c_char_p,
       C.c_size_t]),
+    ("orda_linear_ce_workspace", C.c_int32,
+     [C.POINTER(LinearCeC), C.c_int32, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
+    ("orda_linear_ce_forward", C.c_int32,
+     [C.c_int32, C.c_void_p, C.POINTER(LinearCeC), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
+      C.c_char_p, C.c_size_t]),
+    ("orda_linear_ce_backward", C.c_int32,
+     [C.c_int32, C.c_void_p, C.POINTER(LinearCeC), C.c_void_p, C.c_void_p, C.c_void_p,
+      C.POINTER(Tensor), C.POINTER(Tensor), C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t]),
 ]
 
 _lib = None

@@ -20,7 +20,8 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import Context, distillation_loss
+from . import (Context, distillation_loss, linear_cross_entropy,
+               linear_cross_entropy_backward)
 from . import _lib as L
 from .types import LossOptions, OrdaError, Teacher, TeacherMode
 
@@ -121,3 +122,41 @@ def distillation_loss_autograd(student_hidden: torch.Tensor, weight: torch.Tenso
     tw = teacher.weight if mode == TeacherMode.Separate else None
     tl = teacher.logits if mode == TeacherMode.Precomputed else None
     return DistillCEFunction.apply(student_hidden, weight, th, tw, labels, tl, mode, opts, ctx)
+
+
+class LinearCrossEntropyFunction(torch.autograd.Function):
+    """nll, lse = LinearCrossEntropyFunction.apply(hidden, weight, labels,
+    ignore_index, label_smoothing, vocab_piece)."""
+
+    @staticmethod
+    def forward(fctx, hidden, weight, labels, ignore_index, label_smoothing, vocab_piece):
+        fctx.opts = dict(ignore_index=ignore_index, label_smoothing=label_smoothing,
+                         vocab_piece=vocab_piece)
+        nll, lse = linear_cross_entropy(hidden.detach(), weight.detach(), labels, **fctx.opts)
+        # (hidden, weight and labels are read again: autograd's version counters
+        # report a change in place before the backward)
+        fctx.save_for_backward(hidden, weight, labels, lse)
+        fctx.set_materialize_grads(False)
+        return nll, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(fctx, g_nll, g_lse):
+        hidden, weight, labels, lse = fctx.saved_tensors
+        want_h, want_w = fctx.needs_input_grad[:2]
+        if (g_nll is None and g_lse is None) or not (want_h or want_w):
+            return (None,) * 6
+        gh, gw = linear_cross_entropy_backward(hidden.detach(), weight.detach(), labels, lse.detach(), g_nll,
+                                               g_lse, grad_hidden=want_h, grad_weight=want_w, **fctx.opts)
+        return gh, gw, None, None, None, None
+
+
+def linear_cross_entropy_autograd(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *,
+                                  ignore_index: int = -100, label_smoothing: float = 0.0,
+                                  vocab_piece: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Differentiable form of ``linear_cross_entropy``: float32 ``(nll, lse)``,
+    each [N]. Any loss of them (a mean, row weights, ``lse ** 2``) sends its
+    gradient to ``hidden`` and ``weight`` in their types; the backward forms the
+    logits again, a piece of the vocabulary at a time."""
+    return LinearCrossEntropyFunction.apply(hidden, weight, labels, ignore_index, label_smoothing,
+                                            vocab_piece)

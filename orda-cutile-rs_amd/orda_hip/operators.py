@@ -1,0 +1,186 @@
+"""Operators beside the distillation loss, on GPU tensors.
+
+* ``linear_cross_entropy`` / ``linear_cross_entropy_backward``: row losses of a
+  language-model head without keeping its logits.
+
+Every call queues its kernels on torch's current stream of the inputs' device
+and returns without waiting; outputs and scratch come from torch's allocator, so
+the calls follow the stream and may be captured into a graph (each captured
+graph then owns its scratch). Their differentiable forms are in
+``orda_hip.autograd``. They have no counterpart in the reference, whose loss is
+a weighted mean with the gradients in the same call (src/api.rs:188-422).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+from . import _lib as L
+from .types import OrdaError
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _gpu_tensor(x, what: str):
+    """x itself, where it is a tensor in GPU memory of its own (not a wrapper
+    such as functorch makes, whose memory the library cannot read)."""
+    torch = _torch()
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise OrdaError(f"{what} must be a GPU tensor")
+    try:
+        plain = type(x) in (torch.Tensor, torch.nn.Parameter) and (x.numel() == 0 or x.data_ptr() != 0)
+    except RuntimeError:
+        plain = False
+    if not plain or x.layout != torch.strided or x.is_neg():
+        raise OrdaError(f"{what} must be a plain tensor with memory of its own")
+    return x
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t.device != device:
+            raise OrdaError(f"{name} is on {t.device}, not on {device}")
+
+
+def _matrix(x, what: str):
+    """x as a 2-D tensor with adjacent columns and rows that do not overlap (a
+    copy where it is none)."""
+    if x.dim() != 2:
+        raise OrdaError(f"{what} must be 2-D")
+    if (x.size(1) > 1 and x.stride(1) != 1) or (x.size(0) > 1 and x.stride(0) < x.size(1)):
+        x = x.contiguous()
+    return x
+
+
+_DTYPES = None
+
+
+def _dtype(x, what: str) -> int:
+    global _DTYPES
+    if _DTYPES is None:
+        torch = _torch()
+        _DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16}
+    if x.dtype not in _DTYPES:
+        raise OrdaError(f"{what} must be float32 or bfloat16, got {x.dtype}")
+    return _DTYPES[x.dtype]
+
+
+def _desc(x, what: str) -> L.Tensor:
+    """orda_tensor of a _matrix."""
+    return L.Tensor(data=x.data_ptr(), rows=x.size(0), cols=x.size(1),
+                    ld=x.stride(0) if x.size(0) > 1 else x.size(1), dtype=_dtype(x, what),
+                    location=L.DEVICE)
+
+
+def _call(fn, *args):
+    err = C.create_string_buffer(512)
+    rc = fn(*args, err, 512)
+    if rc != L.ORDA_OK:
+        raise OrdaError(err.value.decode(), rc)
+
+
+def _stream(device):
+    return _torch().cuda.current_stream(device).cuda_stream
+
+
+def _bytes(n: int, device):
+    return _torch().empty(n, dtype=_torch().uint8, device=device)
+
+
+# ------------------------------------------------------------------ linear cross entropy
+def _ce_args(hidden, weight, labels, ignore_index, label_smoothing, vocab_piece):
+    """(orda_linear_ce, the tensors it points into)."""
+    torch = _torch()
+    h = _matrix(_gpu_tensor(hidden, "hidden"), "hidden")
+    w = _matrix(_gpu_tensor(weight, "weight"), "weight")
+    y = _gpu_tensor(labels, "labels")
+    if y.dim() != 1:
+        raise OrdaError("labels must be 1-D")
+    if y.dtype not in (torch.int64, torch.int32):
+        raise OrdaError(f"labels must be int64 or int32, got {y.dtype}")
+    _same_device(h.device, weight=w, labels=y)
+    y = y.to(torch.int64).contiguous()
+    if vocab_piece is not None and vocab_piece < 1:
+        raise OrdaError("vocab_piece must be >= 1")
+    a = L.LinearCeC(hidden=_desc(h, "hidden"), weight=_desc(w, "weight"), labels=y.data_ptr(),
+                    n_labels=y.numel(), ignore_index=ignore_index, label_smoothing=label_smoothing,
+                    vocab_piece=vocab_piece or 0)
+    return a, (h, w, y)
+
+
+def _ce_workspace(lib, a, backward: int, device):
+    n = C.c_int64()
+    _call(lib.orda_linear_ce_workspace, C.byref(a), backward, C.byref(n))
+    return _bytes(n.value, device)
+
+
+def linear_cross_entropy(hidden, weight, labels, *, ignore_index: int = -100,
+                         label_smoothing: float = 0.0, vocab_piece: Optional[int] = None) -> Tuple:
+    """Row losses of the logits ``x = hidden @ weight.T``, which are formed a
+    piece of the vocabulary at a time and not kept.
+
+    ``hidden`` [N, H] and ``weight`` [V, H] are float32 or bfloat16 GPU tensors,
+    ``labels`` [N] int64 or int32. Returns float32 ``(nll, lse)``, each [N]:
+
+    * ``lse[r] = log(sum_v exp(x[r, v]))``
+    * ``nll[r] = lse[r] - (1 - e) x[r, y] - (e / V) sum_v x[r, v]`` with
+      ``e = label_smoothing``
+
+    Rows labelled ``ignore_index`` are not read and have ``nll = lse = 0``; a
+    label that is no class makes its row's ``nll`` NaN. ``vocab_piece`` sets the
+    columns of a piece (whole 256s; default: what 1 GiB of scratch holds).
+    """
+    torch = _torch()
+    a, (h, w, y) = _ce_args(hidden, weight, labels, ignore_index, label_smoothing, vocab_piece)
+    lib = L.load()
+    ws = _ce_workspace(lib, a, 0, h.device)
+    nll = torch.empty(h.size(0), dtype=torch.float32, device=h.device)
+    lse = torch.empty_like(nll)
+    _call(lib.orda_linear_ce_forward, h.device.index, _stream(h.device), C.byref(a), nll.data_ptr(),
+          lse.data_ptr(), ws.data_ptr(), ws.numel())
+    return nll, lse
+
+
+def _row_gradient(g, n: int, device, what: str):
+    """A float32 [n] gradient with adjacent elements, or None."""
+    if g is None:
+        return None
+    torch = _torch()
+    g = _gpu_tensor(g, what)
+    _same_device(device, **{what: g})
+    if g.dtype != torch.float32 or tuple(g.shape) != (n,):
+        raise OrdaError(f"{what} must be float32 [{n}]")
+    return g.contiguous()
+
+
+def linear_cross_entropy_backward(hidden, weight, labels, lse, grad_nll, grad_lse=None, *,
+                                  ignore_index: int = -100, label_smoothing: float = 0.0,
+                                  vocab_piece: Optional[int] = None, grad_hidden: bool = True,
+                                  grad_weight: bool = True) -> Tuple:
+    """Gradients of a loss with respect to ``hidden`` and ``weight`` (in their
+    types; None where not asked for), given its gradients into ``nll`` and
+    ``lse`` of ``linear_cross_entropy`` (float32 [N], either may be None: 0) and
+    the ``lse`` that call returned. Ignored rows have zero gradients whatever
+    comes in for them; a label that is no class makes its row of ``grad_hidden``
+    and all of ``grad_weight`` NaN.
+    """
+    torch = _torch()
+    a, (h, w, y) = _ce_args(hidden, weight, labels, ignore_index, label_smoothing, vocab_piece)
+    lib = L.load()
+    n = h.size(0)
+    if lse is None:
+        raise OrdaError("lse must be a GPU tensor")
+    lse = _row_gradient(lse, n, h.device, "lse")
+    gn = _row_gradient(grad_nll, n, h.device, "grad_nll")
+    gl = _row_gradient(grad_lse, n, h.device, "grad_lse")
+    ws = _ce_workspace(lib, a, int(grad_hidden) + 2 * int(grad_weight), h.device)
+    gh = torch.empty(h.shape, dtype=h.dtype, device=h.device) if grad_hidden else None
+    gw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if grad_weight else None
+    _call(lib.orda_linear_ce_backward, h.device.index, _stream(h.device), C.byref(a), lse.data_ptr(),
+          gn.data_ptr() if gn is not None else None, gl.data_ptr() if gl is not None else None,
+          C.byref(_desc(gh, "grad_hidden")) if gh is not None else None,
+          C.byref(_desc(gw, "grad_weight")) if gw is not None else None, ws.data_ptr(), ws.numel())
+    return gh, gw

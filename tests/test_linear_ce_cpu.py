@@ -1,0 +1,94 @@
+"""The linear cross entropy's refusals, without a GPU: the Python checks, and the
+C entry points' checks of their arguments (made before any device call)."""
+import ctypes as C
+
+import pytest
+import torch
+
+import orda_hip as H
+from orda_hip import _lib as L
+
+
+def args(n=4, h=8, v=16, **kw):
+    a = L.LinearCeC(hidden=L.Tensor(data=256, rows=n, cols=h, dtype=L.BF16, location=L.DEVICE),
+                    weight=L.Tensor(data=256, rows=v, cols=h, dtype=L.BF16, location=L.DEVICE),
+                    labels=256, n_labels=n, ignore_index=-100)
+    for k, x in kw.items():
+        if "." in k:
+            t, f = k.split(".")
+            setattr(getattr(a, t), f, x)
+        else:
+            setattr(a, k, x)
+    return a
+
+
+def workspace(a, backward=0):
+    n, err = C.c_int64(), C.create_string_buffer(512)
+    rc = L.load().orda_linear_ce_workspace(C.byref(a), backward, C.byref(n), err, 512)
+    return rc, n.value, err.value.decode()
+
+
+@pytest.mark.parametrize("change, message", [
+    ({"weight.cols": 9}, "columns"),
+    ({"n_labels": 3}, "labels"),
+    ({"weight.dtype": L.F32}, "dtype"),
+    ({"hidden.dtype": L.I8}, "float32 or bfloat16"),
+    ({"hidden.location": L.HOST}, "device"),
+    ({"weight.location": L.HOST}, "device"),
+    ({"hidden.rows": -1}, "negative"),
+    ({"hidden.data": None}, "null"),
+    ({"weight.ld": 7}, "ld < cols"),
+    ({"label_smoothing": -0.1}, "label_smoothing"),
+    ({"label_smoothing": 1.5}, "label_smoothing"),
+    ({"label_smoothing": float("nan")}, "label_smoothing"),
+    ({"vocab_piece": -1}, "vocab_piece"),
+    ({"weight.rows": 0}, "> 0"),
+    ({"hidden.cols": 0, "weight.cols": 0}, "> 0"),
+    ({"hidden.cols": 2 ** 21, "weight.cols": 2 ** 21}, "at most"),
+])
+def test_arguments_refused(change, message):
+    a = args(**change)
+    rc, _, err = workspace(a)
+    assert rc == L.ORDA_ERR_INVALID and message in err
+    err = C.create_string_buffer(512)
+    rc = L.load().orda_linear_ce_forward(0, None, C.byref(a), 256, 256, 256, 1 << 40, err, 512)
+    assert rc == L.ORDA_ERR_INVALID and message in err.value.decode()
+
+
+def test_null_and_small_workspaces_refused():
+    lib, a, err = L.load(), args(), C.create_string_buffer(512)
+    assert workspace(a)[0] == L.ORDA_OK
+    need = workspace(a)[1]
+    assert lib.orda_linear_ce_forward(0, None, C.byref(a), 256, 256, 256, need - 1, err, 512) == L.ORDA_ERR_INVALID
+    assert "workspace" in err.value.decode()
+    assert lib.orda_linear_ce_forward(0, None, C.byref(a), 256, 256, 264, need, err, 512) == L.ORDA_ERR_INVALID
+    assert "aligned" in err.value.decode()
+    assert lib.orda_linear_ce_forward(0, None, C.byref(a), None, 256, 256, need, err, 512) == L.ORDA_ERR_INVALID
+    assert lib.orda_linear_ce_workspace(None, 0, None, err, 512) == L.ORDA_ERR_INVALID
+    g = L.Tensor(data=256, rows=4, cols=8, dtype=L.F32, location=L.DEVICE)
+    rc = lib.orda_linear_ce_backward(0, None, C.byref(a), 256, 256, None, C.byref(g), None, 256, 1 << 40, err, 512)
+    assert rc == L.ORDA_ERR_INVALID and "dtype" in err.value.decode()
+    g = L.Tensor(data=256, rows=5, cols=8, dtype=L.BF16, location=L.DEVICE)
+    rc = lib.orda_linear_ce_backward(0, None, C.byref(a), 256, 256, None, None, C.byref(g), 256, 1 << 40, err, 512)
+    assert rc == L.ORDA_ERR_INVALID and "grad_weight" in err.value.decode()
+
+
+def test_scratch_follows_the_piece():
+    """Smaller pieces take less scratch (beside the partial sums of products that
+    are split); a piece is whole 256s; a default call of a large batch stays near
+    a GiB beside its rows."""
+    big = dict(n=8192, h=4096, v=131072)
+    sizes = [workspace(args(**big, vocab_piece=p), 3)[1] for p in (1, 256, 16384, 65536, 131072)]
+    assert sizes[0] == sizes[1] < sizes[2] < sizes[3] < sizes[4]
+    assert workspace(args(**big), 3)[1] < 3 << 29
+    assert workspace(args(**big), 0)[1] < 3 << 28
+    # no rows: nothing to hold
+    assert workspace(args(n=0, **{"hidden.data": None}))[:2] == (L.ORDA_OK, 0)
+
+
+def test_python_refuses_cpu_tensors():
+    h, w, y = torch.zeros(2, 8), torch.zeros(3, 8), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(H.OrdaError, match="GPU tensor"):
+        H.linear_cross_entropy(h, w, y)
+    with pytest.raises(H.OrdaError, match="GPU tensor"):
+        H.linear_cross_entropy_backward(h, w, y, torch.zeros(2), torch.zeros(2))
