@@ -352,6 +352,31 @@ int32_t orda_linear_ce_backward(int32_t device, void *hip_stream, const orda_lin
                                 orda_tensor *grad_hidden, orda_tensor *grad_weight, void *workspace,
                                 int64_t workspace_bytes, char *err, size_t err_len);
 
+/* ---- embedding ------------------------------------------------------------- */
+/* The other use of a tied [V,H] weight, and its share of that weight's
+ * gradient. Everything is on `device`; the calls queue their kernels on
+ * hip_stream (NULL: the null stream) and return, allocate nothing and can be
+ * captured. At most 2^30 ids and rows, 2^20 columns. No counterpart in the
+ * reference.
+ *
+ * out[t] = scale * weight[ids[t]], rounded once to the weight's type; a row of
+ * NaN where the id is no row. ids_bytes: 4 (int32) or 8 (int64). */
+int32_t orda_embedding(int32_t device, void *hip_stream, const void *ids, int32_t ids_bytes, int64_t n,
+                       const orda_tensor *weight, float scale, orda_tensor *out, char *err,
+                       size_t err_len);
+/* out[v] = scale * Σ grad[t] over ids[t] == v, added in the order of t in fp32
+ * (the same bits whatever the launch) and rounded once to out's type; with
+ * accumulate, that plus out's old value, and rows no id names are not touched.
+ * Ids equal to padding_idx (negative: none), or that are no row, add nothing.
+ * grad [n,H] and out [V,H] are fp32 or bf16 each. workspace (256-byte aligned)
+ * is the call's alone until its kernels have run. */
+int32_t orda_embedding_backward_workspace(int64_t n, int64_t rows, int64_t cols, int32_t grad_dtype,
+                                          int64_t *bytes, char *err, size_t err_len);
+int32_t orda_embedding_backward(int32_t device, void *hip_stream, const void *ids, int32_t ids_bytes,
+                                int64_t n, const orda_tensor *grad, int64_t padding_idx, float scale,
+                                int32_t accumulate, orda_tensor *out, void *workspace,
+                                int64_t workspace_bytes, char *err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

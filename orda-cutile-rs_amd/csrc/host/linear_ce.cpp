@@ -6,7 +6,6 @@
 // count of those rows stays on the device, the scratch is the caller's: the
 // calls queue their kernels and return, and can be captured into a graph.
 #include <algorithm>
-#include <exception>
 
 #include "orda_host.h"
 
@@ -310,20 +309,6 @@ void check_grad(const orda_tensor& g, DType t, int64_t rows, int64_t cols, const
   if (g.location != ORDA_DEVICE) fail(ORDA_ERR_INVALID, "%s must be on the device", what);
   if (g.rows != rows || g.cols != cols)
     fail(ORDA_ERR_INVALID, "%s must be [%lld, %lld]", what, static_cast<long long>(rows), static_cast<long long>(cols));
-}
-
-template <class F>
-int32_t guarded(char* err, size_t err_len, F&& f) {
-  try {
-    f();
-    return ORDA_OK;
-  } catch (const Error& e) {
-    copy_err(e, err, err_len);
-    return e.status;
-  } catch (const std::exception& e) {
-    copy_err(Error{ORDA_ERR_INTERNAL, e.what()}, err, err_len);
-    return ORDA_ERR_INTERNAL;
-  }
 }
 
 }  // namespace

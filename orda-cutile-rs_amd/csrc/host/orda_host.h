@@ -6,6 +6,7 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -91,6 +92,21 @@ inline void check_view(const orda_tensor& t, const char* what) {
   if (t.rows < 0 || t.cols < 0) fail(ORDA_ERR_INVALID, "%s has a negative shape", what);
   if (t.rows > 0 && t.cols > 0 && !t.data) fail(ORDA_ERR_INVALID, "%s has a null data pointer", what);
   if (tensor_ld(t) < t.cols) fail(ORDA_ERR_INVALID, "%s has ld < cols", what);
+}
+
+// A C entry point's body: no exception leaves it.
+template <class F>
+int32_t guarded(char* err, size_t err_len, F&& f) {
+  try {
+    f();
+    return ORDA_OK;
+  } catch (const Error& e) {
+    copy_err(e, err, err_len);
+    return e.status;
+  } catch (const std::exception& e) {
+    copy_err(Error{ORDA_ERR_INTERNAL, e.what()}, err, err_len);
+    return ORDA_ERR_INTERNAL;
+  }
 }
 
 // The calling thread's current device for the scope of a call.

@@ -1,0 +1,550 @@
+// embedding.hip — rows of the vocabulary weight by token id, and the gradient of
+// that weight by sorted tokens.
+//
+// Both are bound by HBM: the lookup reads and writes a row a token, the gradient
+// reads a row a token and writes every row of the weight once.
+//
+// The gradient sorts (id, place) pairs by id, stable, so that a token's rows are
+// added in the order they stand in the batch whatever the launch; the sums are
+// fp32 and rounded once. Work is cut over the sorted pairs, not over the ids: a
+// wave takes kChunk pairs and 1 KB of columns, so that an id that makes up a
+// tenth of the batch costs no more than any other tenth. A sum that a chunk's
+// border cuts goes to scratch and is joined by a second kernel, in order.
+#include <math.h>
+
+#include "orda_kernels.h"
+
+namespace orda {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// kV elements of a row from p: a vector of 16 bytes (VEC), else elements 64
+// apart, of which those from column `left` on (relative to p) are 0.
+template <typename E, bool VEC>
+struct Cols {
+  static constexpr int kV = 16 / sizeof(E);
+  static constexpr int kStep = VEC ? 1 : 64;   // columns from one of a lane's elements to the next
+  static __device__ __forceinline__ int first(int lane) { return VEC ? lane * kV : lane; }
+  static __device__ __forceinline__ void load(const E* p, int left, float (&x)[kV]) {
+    if constexpr (VEC) {
+      alignas(16) E w[kV];
+      *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+      for (int k = 0; k < kV; ++k) x[k] = static_cast<float>(w[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kV; ++k) x[k] = k * 64 < left ? static_cast<float>(p[k * 64]) : 0.f;
+    }
+  }
+};
+
+// ------------------------------------------------------------ lookup
+// A wave moves up to kLookBytes of one row, so that a lane has four 16-byte
+// loads in flight.
+constexpr int kLookBytes = 4096;
+
+template <typename E, typename I, bool VEC>
+__global__ __launch_bounds__(256) void embedding_kernel(const I* ids, int64_t n, const E* w, int64_t ldw, int64_t v,
+                                                        int64_t h, float scale, E* out, int64_t ldo, int64_t parts) {
+  constexpr int kV = 16 / sizeof(E);
+  constexpr int kCols = kLookBytes / sizeof(E);
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
+  const int64_t t = unit / parts;
+  if (t >= n) return;
+  const int64_t c0 = (unit - t * parts) * kCols;
+  const int64_t id = static_cast<int64_t>(ids[t]);
+  const bool ok = id >= 0 && id < v;
+  const E* s = w + (ok ? id : 0) * ldw + c0;
+  E* d = out + t * ldo + c0;
+  const int cols = static_cast<int>(h - c0 < kCols ? h - c0 : kCols);
+  if constexpr (VEC) {
+    u32x4 x[kCols / (64 * kV)];
+#pragma unroll
+    for (int i = 0; i < kCols / (64 * kV); ++i) {
+      const int c = (i * 64 + lane) * kV;
+      if (c + kV <= cols) x[i] = *reinterpret_cast<const u32x4*>(s + c);
+    }
+#pragma unroll
+    for (int i = 0; i < kCols / (64 * kV); ++i) {
+      const int c = (i * 64 + lane) * kV;
+      alignas(16) E e[kV];
+      *reinterpret_cast<u32x4*>(e) = x[i];
+#pragma unroll
+      for (int k = 0; k < kV; ++k) e[k] = ok ? static_cast<E>(static_cast<float>(e[k]) * scale) : static_cast<E>(NAN);
+      if (c + kV <= cols) *reinterpret_cast<u32x4*>(d + c) = *reinterpret_cast<const u32x4*>(e);
+    }
+  } else {
+    for (int c = lane; c < cols; c += 64)
+      d[c] = ok ? static_cast<E>(static_cast<float>(s[c]) * scale) : static_cast<E>(NAN);
+  }
+}
+
+// ------------------------------------------------------------ sort
+// Ids that take no gradient (padding, or no row of the weight) sort as v, last.
+template <typename I>
+__device__ __forceinline__ uint32_t key_of(I id, int64_t v, int64_t pad) {
+  const int64_t i = static_cast<int64_t>(id);
+  return static_cast<uint32_t>(i >= 0 && i < v && i != pad ? i : v);
+}
+
+// Few tokens: every token's place is the number of pairs before it, counted
+// against all of them from LDS, with (key, place) packed into 32 bits. 2 VALU
+// operations a comparison: 1000 tokens take 4 workgroups 4 us, one launch, where
+// the passes below take four.
+template <typename I>
+__global__ __launch_bounds__(256) void embed_rank_kernel(const I* ids, int n, int64_t v, int64_t pad, uint32_t* keys,
+                                                         uint32_t* vals) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t all[];   // n, up to whole fours
+  const int n4 = (n + 3) / 4 * 4;
+  for (int i = threadIdx.x; i < n4; i += 256)
+    all[i] = i < n ? key_of(ids[i], v, pad) * static_cast<uint32_t>(n) + i : 0xffffffffu;
+  __syncthreads();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const uint32_t me = all[i];
+  uint32_t before = 0;
+  for (int j = 0; j < n4; j += 4) {
+    const u32x4 o = *reinterpret_cast<const u32x4*>(all + j);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) before += o[k] < me ? 1u : 0u;
+  }
+  keys[before] = me / static_cast<uint32_t>(n);
+  vals[before] = static_cast<uint32_t>(i);
+}
+
+// More: stable passes over digits of kDigitBits, from the lowest. A workgroup
+// holds kSortTile pairs, a wave 64·kSortSteps consecutive ones; lanes of one digit
+// find each other by a ballot for each of its bits, and a wave's counters in LDS
+// carry the ranks from step to step.
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
+constexpr int kSortWaves = 16, kSortSteps = 4, kSortTile = kSortWaves * 64 * kSortSteps;
+
+// Pairs of a pass: from the ids (first pass), or the last pass's.
+template <typename I>
+struct Pairs {
+  const I* ids;
+  const uint32_t *keys, *vals;
+  int64_t n, v, pad;
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return ids != nullptr ? key_of(ids[i], v, pad) : keys[i]; }
+  __device__ __forceinline__ uint32_t val(int64_t i) const { return ids != nullptr ? static_cast<uint32_t>(i) : vals[i]; }
+};
+
+template <typename I>
+__global__ __launch_bounds__(1024) void embed_count_kernel(Pairs<I> p, int shift, uint32_t* counts) {
+  __shared__ uint32_t c[kDigits];
+  for (int d = threadIdx.x; d < kDigits; d += 1024) c[d] = 0;
+  __syncthreads();
+  const int64_t i0 = blockIdx.x * static_cast<int64_t>(kSortTile);
+  for (int k = threadIdx.x; k < kSortTile; k += 1024)
+    if (i0 + k < p.n) atomicAdd(&c[(p.key(i0 + k) >> shift) & (kDigits - 1)], 1u);   // whole numbers: any order
+  __syncthreads();
+  for (int d = threadIdx.x; d < kDigits; d += 1024) counts[blockIdx.x * kDigits + d] = c[d];
+}
+
+template <typename I>
+__global__ __launch_bounds__(1024) void embed_place_kernel(Pairs<I> p, int shift, const uint32_t* counts, uint32_t* keys,
+                                                           uint32_t* vals) {
+  __shared__ uint32_t wave_n[kSortWaves][kDigits];   // a wave's pairs of each digit, then where they begin
+  __shared__ uint32_t part[2][kDigits], wave_sum[kDigits / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int d = lane; d < kDigits; d += 64) wave_n[wave][d] = 0;
+  // Pairs of digit d in earlier workgroups and in all, each half of the
+  // workgroup half of the workgroups' counts.
+  const int d = tid & (kDigits - 1), half = tid >> kDigitBits;
+  static_assert(2 * kDigits == 1024, "two threads a digit");
+  uint32_t earlier = 0, total = 0;
+  for (int b = half; b < static_cast<int>(gridDim.x); b += 2) {
+    const uint32_t c = counts[static_cast<int64_t>(b) * kDigits + d];
+    total += c;
+    if (b < static_cast<int>(blockIdx.x)) earlier += c;
+  }
+  __syncthreads();
+  if (half == 1) {
+    part[0][d] = earlier;
+    part[1][d] = total;
+  }
+  // Ranks within the wave, step by step.
+  const int64_t i0 = blockIdx.x * static_cast<int64_t>(kSortTile) + wave * (64 * kSortSteps) + lane;
+  uint32_t key[kSortSteps], val[kSortSteps], rank[kSortSteps];
+#pragma unroll
+  for (int s = 0; s < kSortSteps; ++s) {
+    const bool in = i0 + s * 64 < p.n;
+    key[s] = in ? p.key(i0 + s * 64) : 0;
+    val[s] = in ? p.val(i0 + s * 64) : 0;
+  }
+#pragma unroll
+  for (int s = 0; s < kSortSteps; ++s) {
+    const bool in = i0 + s * 64 < p.n;
+    const uint32_t dig = (key[s] >> shift) & (kDigits - 1);
+    uint64_t same = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < kDigitBits; ++b) {
+      const bool bit = ((dig >> b) & 1) != 0;
+      const uint64_t m = __ballot(bit);
+      same &= bit ? m : ~m;
+    }
+    const int below = __popcll(same & ((uint64_t{1} << lane) - 1));
+    const uint32_t had = in ? wave_n[wave][dig] : 0;
+    rank[s] = had + below;
+    __builtin_amdgcn_wave_barrier();   // every lane has read before the first of each digit writes
+    if (in && below == 0) wave_n[wave][dig] = had + static_cast<uint32_t>(__popcll(same));
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  // Where each digit begins: all smaller digits, then earlier workgroups, then
+  // earlier waves.
+  if (half == 0) {
+    earlier += part[0][d];
+    total += part[1][d];
+    uint32_t incl = total;
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) {
+      const uint32_t t = __shfl_up(incl, k);
+      if (lane >= k) incl += t;
+    }
+    if (lane == 63) wave_sum[wave] = incl;
+    part[1][d] = incl - total;
+  }
+  __syncthreads();
+  if (half == 0) {
+    uint32_t at = part[1][d] + earlier;
+    for (int w = 0; w < wave; ++w) at += wave_sum[w];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = wave_n[w][d];
+      wave_n[w][d] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < kSortSteps; ++s) {
+    if (i0 + s * 64 >= p.n) continue;
+    const uint32_t at = wave_n[wave][(key[s] >> shift) & (kDigits - 1)] + rank[s];
+    keys[at] = key[s];
+    vals[at] = val[s];
+  }
+}
+
+// ------------------------------------------------------------ gradient
+// First sorted place whose key is at least k: the wave's lanes probe 64 places
+// a step.
+__device__ __forceinline__ int64_t first_at_least(const uint32_t* keys, int64_t n, uint32_t k, int lane) {
+  int64_t lo = 0, hi = n;   // keys[lo - 1] < k <= keys[hi]
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const bool less = at < hi && keys[at] < k;
+    const int c = __popcll(__ballot(less));   // the first c probes are less
+    if (c == 0) return lo;
+    const int64_t last = lo + (c - 1) * step;
+    hi = last + step < hi ? last + step : hi;
+    lo = last + 1;
+  }
+  return lo;
+}
+
+// One wave's columns of a gradient row, scaled and rounded (added to what is
+// there with acc). O's stores are 8 or 16 bytes a lane where VEC.
+template <typename E, typename O, bool VEC>
+__device__ __forceinline__ void put_row(const EmbedGradArgs& a, int64_t row, int64_t c0, int lane,
+                                        const float (&x)[Cols<E, VEC>::kV]) {
+  using C = Cols<E, VEC>;
+  O* d = static_cast<O*>(a.out) + row * a.ldo + c0 + C::first(lane);
+  const int left = static_cast<int>(a.h - c0) - C::first(lane);
+  if constexpr (VEC) {
+    if (left < C::kV) return;
+    constexpr int kB = C::kV * sizeof(O) / 16;   // 16-byte vectors, 0: one of 8 bytes
+    alignas(16) O o[C::kV];
+    if (a.accumulate) {
+      if constexpr (kB == 0) *reinterpret_cast<uint64_t*>(o) = *reinterpret_cast<const uint64_t*>(d);
+#pragma unroll
+      for (int b = 0; b < kB; ++b) reinterpret_cast<u32x4*>(o)[b] = reinterpret_cast<const u32x4*>(d)[b];
+    }
+#pragma unroll
+    for (int k = 0; k < C::kV; ++k) {
+      const float s = x[k] * a.scale;
+      o[k] = static_cast<O>(a.accumulate ? static_cast<float>(o[k]) + s : s);
+    }
+    if constexpr (kB == 0) *reinterpret_cast<uint64_t*>(d) = *reinterpret_cast<const uint64_t*>(o);
+#pragma unroll
+    for (int b = 0; b < kB; ++b) reinterpret_cast<u32x4*>(d)[b] = reinterpret_cast<const u32x4*>(o)[b];
+  } else {
+#pragma unroll
+    for (int k = 0; k < C::kV; ++k)
+      if (k * 64 < left) {
+        const float s = x[k] * a.scale;
+        d[k * 64] = static_cast<O>(a.accumulate ? static_cast<float>(d[k * 64]) + s : s);
+      }
+  }
+}
+
+// Partial sums of a chunk: its first sum where an earlier chunk began it (slot
+// 0), its last where it goes on (slot 1; slot 0 where it is the first too).
+template <typename E, bool VEC>
+__device__ __forceinline__ float* partial(const EmbedGradArgs& a, int64_t chunk, int slot, int64_t c0, int lane) {
+  return a.parts + (chunk * 2 + slot) * a.ldp + c0 + Cols<E, VEC>::first(lane);
+}
+template <typename E, bool VEC>
+__device__ __forceinline__ void put_partial(float* d, const float (&x)[Cols<E, VEC>::kV]) {
+  constexpr int kV = Cols<E, VEC>::kV;   // scratch rows hold whole columns of waves
+#pragma unroll
+  for (int k = 0; k < kV; k += VEC ? 4 : 1) {
+    if constexpr (VEC) *reinterpret_cast<f32x4*>(d + k) = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]};
+    else d[k * 64] = x[k];
+  }
+}
+template <typename E, bool VEC>
+__device__ __forceinline__ void add_partial(const float* s, float (&x)[Cols<E, VEC>::kV]) {
+  constexpr int kV = Cols<E, VEC>::kV;
+#pragma unroll
+  for (int k = 0; k < kV; k += VEC ? 4 : 1) {
+    if constexpr (VEC) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(s + k);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[k + q] += v[q];
+    } else {
+      x[k] += s[k * 64];
+    }
+  }
+}
+
+// Waves [0, chunks·slabs): the sums of a chunk of sorted pairs, kLoads rows in
+// flight. The waves after them zero the rows no pair names, fill_rows
+// consecutive ones each, found by one search of the sorted keys.
+template <typename E, typename O, bool VEC>
+__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
+  using C = Cols<E, VEC>;
+  constexpr int kV = C::kV, kLoads = 8;
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = blockIdx.x * int64_t{4} + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (unit < a.chunks * a.slabs) {
+    const int64_t chunk = unit / a.slabs, c0 = (unit - chunk * a.slabs) * (64 * kV);
+    const int64_t b = chunk * a.chunk, e = b + a.chunk < a.n ? b + a.chunk : a.n;
+    const int left = static_cast<int>(a.h - c0) - C::first(lane);
+    const E* src = static_cast<const E*>(a.grad) + c0 + C::first(lane);
+    const bool on = VEC ? left >= kV : left > 0;
+    float x[kV] = {};
+    uint32_t key = a.keys[b];
+    bool head = b > 0 && a.keys[b - 1] == key;   // the sum began in an earlier chunk
+    auto flush = [&](bool tail) {   // tail: it goes on in the next one
+      if (static_cast<int64_t>(key) < a.v) {
+        if (head || tail) put_partial<E, VEC>(partial<E, VEC>(a, chunk, head ? 0 : 1, c0, lane), x);
+        else put_row<E, O, VEC>(a, key, c0, lane, x);
+      }
+#pragma unroll
+      for (int k = 0; k < kV; ++k) x[k] = 0.f;
+      head = false;
+    };
+    for (int64_t i = b; i < e; i += kLoads) {
+      float y[kLoads][kV];
+      uint32_t ks[kLoads];
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) {
+        const int64_t j = i + q < e ? i + q : e - 1;
+        ks[q] = a.keys[j];
+        const int64_t r = a.vals[j];
+        if (on && static_cast<int64_t>(ks[q]) < a.v) {
+          C::load(src + r * a.ldg, left, y[q]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kV; ++k) y[q][k] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) {
+        if (i + q < e) {
+          if (ks[q] != key) {
+            flush(false);
+            key = ks[q];
+          }
+#pragma unroll
+          for (int k = 0; k < kV; ++k) x[k] += y[q][k];
+        }
+      }
+    }
+    flush(e < a.n && a.keys[e] == key);
+    return;
+  }
+  if (a.accumulate) return;
+  const int64_t r0 = (unit - a.chunks * a.slabs) * a.fill_rows;
+  if (r0 >= a.v) return;
+  const int64_t r1 = r0 + a.fill_rows < a.v ? r0 + a.fill_rows : a.v;
+  int64_t at = first_at_least(a.keys, a.n, static_cast<uint32_t>(r0), lane);
+  int64_t r = r0;
+  while (r < r1) {
+    // rows up to the next key are zero
+    const int64_t next = at < a.n && static_cast<int64_t>(a.keys[at]) < r1 ? a.keys[at] : r1;
+    for (; r < next; ++r) {
+      O* d = static_cast<O*>(a.out) + r * a.ldo;
+      if (VEC) {
+        constexpr int kO = 16 / sizeof(O);
+        for (int64_t c = lane * kO; c < a.h; c += 64 * kO) *reinterpret_cast<u32x4*>(d + c) = u32x4{0, 0, 0, 0};
+      } else {
+        for (int64_t c = lane; c < a.h; c += 64) d[c] = static_cast<O>(0.f);
+      }
+    }
+    if (r >= r1) break;
+    // past the pairs of row r
+    const uint64_t same = __ballot(at + lane < a.n && static_cast<int64_t>(a.keys[at + lane < a.n ? at + lane : at]) == r);
+    at = ~same == 0 ? first_at_least(a.keys, a.n, static_cast<uint32_t>(r + 1), lane) : at + __popcll(same);
+    ++r;
+  }
+}
+
+// Sums that a chunk begins and a later one ends, a wave for each chunk and its
+// columns: the parts in order.
+template <typename E, typename O, bool VEC>
+__global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradArgs a) {
+  using C = Cols<E, VEC>;
+  constexpr int kV = C::kV;
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = blockIdx.x * int64_t{4} + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (unit >= (a.chunks - 1) * a.slabs) return;
+  const int64_t chunk = unit / a.slabs, c0 = (unit - chunk * a.slabs) * (64 * kV);
+  const int64_t b = chunk * a.chunk, e = b + a.chunk;   // not the last chunk: whole
+  const uint32_t key = a.keys[e - 1];
+  if (static_cast<int64_t>(key) >= a.v || a.keys[e] != key) return;    // nothing goes on
+  if (b > 0 && a.keys[b] == key && a.keys[b - 1] == key) return;       // begun earlier
+  // the last chunk that begins with this key
+  const int64_t end = first_at_least(a.keys, a.n, key + 1, lane);
+  const int64_t last = (end - 1) / a.chunk;
+  float x[kV] = {};
+  add_partial<E, VEC>(partial<E, VEC>(a, chunk, 1, c0, lane), x);
+  int64_t j = chunk + 1;
+  for (; j + 3 <= last; j += 4) {   // four loads in flight, added in order
+    float y[4][kV] = {};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) add_partial<E, VEC>(partial<E, VEC>(a, j + q, 0, c0, lane), y[q]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int k = 0; k < kV; ++k) x[k] += y[q][k];
+  }
+  for (; j <= last; ++j) add_partial<E, VEC>(partial<E, VEC>(a, j, 0, c0, lane), x);
+  put_row<E, O, VEC>(a, key, c0, lane, x);
+}
+
+bool aligned16(const void* p, int64_t ld, int64_t h, int64_t es) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0 && h * es % 16 == 0;
+}
+
+int passes_of(int64_t v) {   // digits of keys 0..v
+  int bits = 0;
+  while (bits < 32 && (v >> bits) != 0) ++bits;
+  return bits <= kDigitBits ? 1 : (bits + kDigitBits - 1) / kDigitBits;
+}
+
+// Tokens whose ranks are counted: the packed pairs must fit 32 bits and LDS.
+// (Counted against the passes at 1024 to 4096 tokens: see embed_rank_kernel.)
+constexpr int64_t kRankTokens = 2048;
+bool ranked(int64_t n, int64_t v) { return n <= kRankTokens && (v + 1) * n <= int64_t{0xffffffff}; }
+
+}  // namespace
+
+hipError_t launch_embedding(DType t, const void* ids, bool ids64, int64_t n, const void* w, int64_t ldw, int64_t v,
+                            int64_t h, float scale, void* out, int64_t ldo, hipStream_t stream) {
+  if (n <= 0 || h <= 0) return hipSuccess;
+  const int64_t es = dtype_size(t);
+  const bool vec = aligned16(w, ldw, h, es) && aligned16(out, ldo, h, es);
+  const int64_t parts = (h * es + kLookBytes - 1) / kLookBytes;
+  const int64_t blocks = (n * parts + 3) / 4;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  auto run = [&](auto* e, auto* i) {
+    using E = std::remove_pointer_t<decltype(e)>;
+    using I = std::remove_pointer_t<decltype(i)>;
+    auto* k = vec ? embedding_kernel<E, I, true> : embedding_kernel<E, I, false>;
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, static_cast<const I*>(ids), n,
+                       static_cast<const E*>(w), ldw, v, h, scale, static_cast<E*>(out), ldo, parts);
+  };
+  int64_t* i64 = nullptr;
+  int32_t* i32 = nullptr;
+  __bf16* b = nullptr;
+  float* f = nullptr;
+  if (t == DType::BF16) ids64 ? run(b, i64) : run(b, i32);
+  else ids64 ? run(f, i64) : run(f, i32);
+  return hipGetLastError();
+}
+
+EmbedScratch embed_scratch(DType grad, int64_t n, int64_t v, int64_t h) {
+  EmbedScratch s{};
+  const int64_t cols = 64 * 16 / dtype_size(grad);   // of a wave
+  s.chunk = 32;
+  while (s.chunk < 256 && n / s.chunk > 4096) s.chunk *= 2;
+  s.chunks = (n + s.chunk - 1) / s.chunk;
+  s.slabs = (h + cols - 1) / cols;
+  s.ldp = s.slabs * cols;
+  auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+  const int64_t pair = up(n * 4);
+  s.keys[0] = 0;
+  s.vals[0] = pair;
+  s.bytes = 2 * pair;
+  if (!ranked(n, v)) {
+    s.keys[1] = s.bytes;
+    s.vals[1] = s.bytes + pair;
+    s.counts = s.bytes + 2 * pair;
+    s.bytes = s.counts + up((n + kSortTile - 1) / kSortTile * kDigits * 4);
+  }
+  s.parts = s.bytes;
+  if (s.chunks > 1) s.bytes += up(s.chunks * 2 * s.ldp * 4);
+  return s;
+}
+
+hipError_t launch_embed_sort(const void* ids, bool ids64, int64_t n, int64_t v, int64_t pad, void* ws,
+                             const EmbedScratch& s, const uint32_t** keys, const uint32_t** vals, hipStream_t stream) {
+  char* base = static_cast<char*>(ws);
+  auto u32 = [&](int64_t at) { return reinterpret_cast<uint32_t*>(base + at); };
+  auto run = [&](auto* i) {
+    using I = std::remove_pointer_t<decltype(i)>;
+    const I* id = static_cast<const I*>(ids);
+    if (ranked(n, v)) {
+      hipLaunchKernelGGL(embed_rank_kernel<I>, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256),
+                         static_cast<unsigned>((n + 3) / 4 * 16), stream, id, static_cast<int>(n), v, pad,
+                         u32(s.keys[0]), u32(s.vals[0]));
+      *keys = u32(s.keys[0]);
+      *vals = u32(s.vals[0]);
+      return;
+    }
+    const int passes = passes_of(v);
+    const unsigned blocks = static_cast<unsigned>((n + kSortTile - 1) / kSortTile);
+    for (int p = 0; p < passes; ++p) {
+      const int to = p & 1;
+      const Pairs<I> pr{p == 0 ? id : nullptr, u32(s.keys[1 - to]), u32(s.vals[1 - to]), n, v, pad};
+      hipLaunchKernelGGL(embed_count_kernel<I>, dim3(blocks), dim3(1024), 0, stream, pr, p * kDigitBits, u32(s.counts));
+      hipLaunchKernelGGL(embed_place_kernel<I>, dim3(blocks), dim3(1024), 0, stream, pr, p * kDigitBits,
+                         static_cast<const uint32_t*>(u32(s.counts)), u32(s.keys[to]), u32(s.vals[to]));
+      *keys = u32(s.keys[to]);
+      *vals = u32(s.vals[to]);
+    }
+  };
+  int64_t* i64 = nullptr;
+  int32_t* i32 = nullptr;
+  ids64 ? run(i64) : run(i32);
+  return hipGetLastError();
+}
+
+hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t stream) {
+  const bool vec = aligned16(a.grad, a.ldg, a.h, dtype_size(grad)) && aligned16(a.out, a.ldo, a.h, dtype_size(out));
+  // rows a wave zeroes: enough waves to fill the chip, at most 64 rows each
+  a.fill_rows = a.v / 8192 < 1 ? 1 : a.v / 8192 > 64 ? 64 : a.v / 8192;
+  const int64_t fill = a.accumulate ? 0 : (a.v + a.fill_rows - 1) / a.fill_rows;
+  const int64_t sum = (a.chunks * a.slabs + fill + 3) / 4, join = ((a.chunks - 1) * a.slabs + 3) / 4;
+  if (sum > 0x7fffffff) return hipErrorInvalidValue;
+  auto run = [&](auto* e, auto* o) {
+    using E = std::remove_pointer_t<decltype(e)>;
+    using O = std::remove_pointer_t<decltype(o)>;
+    auto* k = vec ? embed_sum_kernel<E, O, true> : embed_sum_kernel<E, O, false>;
+    auto* j = vec ? embed_join_kernel<E, O, true> : embed_join_kernel<E, O, false>;
+    if (sum > 0) hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(sum)), dim3(256), 0, stream, a);
+    if (join > 0) hipLaunchKernelGGL(j, dim3(static_cast<unsigned>(join)), dim3(256), 0, stream, a);
+  };
+  __bf16* b = nullptr;
+  float* f = nullptr;
+  if (grad == DType::BF16) out == DType::BF16 ? run(b, b) : run(b, f);
+  else out == DType::BF16 ? run(f, b) : run(f, f);
+  return hipGetLastError();
+}
+
+}  // namespace orda

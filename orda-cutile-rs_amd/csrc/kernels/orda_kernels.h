@@ -450,4 +450,38 @@ hipError_t launch_ce_losses(const CeLossArgs& a, int64_t n, hipStream_t stream);
 hipError_t launch_ce_scatter(const float* src, int64_t lds, const int32_t* pos, int64_t rows, int64_t h, DType t,
                              void* dst, int64_t ldd, hipStream_t stream);
 
+// ---------------------------------------------------------------- embedding
+// out[t] = scale * w[ids[t]] in the weight's type, rounded once; NaN where the id
+// is no row.
+hipError_t launch_embedding(DType t, const void* ids, bool ids64, int64_t n, const void* w, int64_t ldw, int64_t v,
+                            int64_t h, float scale, void* out, int64_t ldo, hipStream_t stream);
+// Scratch of the gradient: byte offsets (pairs sorted back and forth between two
+// buffers, or into the first), and how its sums are cut.
+struct EmbedScratch {
+  int64_t keys[2], vals[2], counts, parts, bytes;
+  int64_t chunk, chunks, slabs, ldp;
+};
+EmbedScratch embed_scratch(DType grad, int64_t n, int64_t v, int64_t h);
+// (id, place) of every token, sorted by id, stable; ids without a gradient (pad,
+// or no row) sort last, as v.
+hipError_t launch_embed_sort(const void* ids, bool ids64, int64_t n, int64_t v, int64_t pad, void* ws,
+                             const EmbedScratch& s, const uint32_t** keys, const uint32_t** vals, hipStream_t stream);
+// out[k] (+)= scale * Σ grad[vals[i]] over keys[i] = k < v, in the sorted order;
+// without accumulate, rows no key names are zero.
+struct EmbedGradArgs {
+  const uint32_t *keys, *vals;
+  int64_t n, v, h;
+  const void* grad;
+  int64_t ldg;
+  void* out;
+  int64_t ldo;
+  float scale;
+  bool accumulate;
+  int64_t chunk, chunks, slabs;
+  float* parts;        // [chunks][2][ldp]
+  int64_t ldp;
+  int64_t fill_rows;   // set by launch_embed_grad
+};
+hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t stream);
+
 }  // namespace orda

@@ -137,6 +137,14 @@ SIGNATURES = [
     ("orda_linear_ce_backward", C.c_int32,
      [C.c_int32, C.c_void_p, C.POINTER(LinearCeC), C.c_void_p, C.c_void_p, C.c_void_p,
       C.POINTER(Tensor), C.POINTER(Tensor), C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t]),
+    ("orda_embedding", C.c_int32,
+     [C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.POINTER(Tensor), C.c_float,
+      C.POINTER(Tensor), C.c_char_p, C.c_size_t]),
+    ("orda_embedding_backward_workspace", C.c_int32,
+     [C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
+    ("orda_embedding_backward", C.c_int32,
+     [C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.POINTER(Tensor), C.c_int64,
+      C.c_float, C.c_int32, C.POINTER(Tensor), C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t]),
 ]
 
 _lib = None

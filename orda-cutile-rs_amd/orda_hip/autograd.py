@@ -20,8 +20,8 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import (Context, distillation_loss, linear_cross_entropy,
-               linear_cross_entropy_backward)
+from . import (Context, distillation_loss, embedding, embedding_backward,
+               linear_cross_entropy, linear_cross_entropy_backward)
 from . import _lib as L
 from .types import LossOptions, OrdaError, Teacher, TeacherMode
 
@@ -160,3 +160,32 @@ def linear_cross_entropy_autograd(hidden: torch.Tensor, weight: torch.Tensor, la
     logits again, a piece of the vocabulary at a time."""
     return LinearCrossEntropyFunction.apply(hidden, weight, labels, ignore_index, label_smoothing,
                                             vocab_piece)
+
+
+class EmbeddingFunction(torch.autograd.Function):
+    """out = EmbeddingFunction.apply(ids, weight, scale, padding_idx)."""
+
+    @staticmethod
+    def forward(fctx, ids, weight, scale, padding_idx):
+        out = embedding(ids, weight.detach(), scale=scale)
+        if padding_idx is not None and not -weight.size(0) <= padding_idx < weight.size(0):
+            raise OrdaError(f"padding_idx must be a row of {weight.size(0)}, got {padding_idx}")
+        fctx.save_for_backward(ids)
+        fctx.opts = dict(num_rows=weight.size(0), scale=scale, padding_idx=padding_idx)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(fctx, grad):
+        (ids,) = fctx.saved_tensors
+        if not fctx.needs_input_grad[1]:
+            return None, None, None, None
+        return None, embedding_backward(grad, ids, **fctx.opts), None, None
+
+
+def embedding_autograd(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
+                       padding_idx: Optional[int] = None) -> torch.Tensor:
+    """Differentiable form of ``embedding``: its backward delivers the gradient
+    of ``weight`` by sorted tokens, the same bits in every run; ``padding_idx``
+    names a row that gets none."""
+    return EmbeddingFunction.apply(ids, weight, scale, padding_idx)

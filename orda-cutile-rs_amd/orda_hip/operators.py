@@ -2,6 +2,8 @@
 
 * ``linear_cross_entropy`` / ``linear_cross_entropy_backward``: row losses of a
   language-model head without keeping its logits.
+* ``embedding`` / ``embedding_backward``: rows of the same weight by token id,
+  and their share of its gradient.
 
 Every call queues its kernels on torch's current stream of the inputs' device
 and returns without waiting; outputs and scratch come from torch's allocator, so
@@ -53,6 +55,15 @@ def _matrix(x, what: str):
     if (x.size(1) > 1 and x.stride(1) != 1) or (x.size(0) > 1 and x.stride(0) < x.size(1)):
         x = x.contiguous()
     return x
+
+
+def _overlap(a, b) -> bool:
+    """Whether the memory of two matrices overlaps."""
+    def span(x):
+        return x.data_ptr(), x.data_ptr() + (((x.size(0) - 1) * x.stride(0) + x.size(1)) * x.element_size()
+                                             if x.numel() else 0)
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
 
 
 _DTYPES = None
@@ -184,3 +195,83 @@ def linear_cross_entropy_backward(hidden, weight, labels, lse, grad_nll, grad_ls
           C.byref(_desc(gh, "grad_hidden")) if gh is not None else None,
           C.byref(_desc(gw, "grad_weight")) if gw is not None else None, ws.data_ptr(), ws.numel())
     return gh, gw
+
+
+# ------------------------------------------------------------------ embedding
+def _ids(ids, device, what: str = "ids"):
+    """ids as a contiguous 1-D int32 or int64 GPU tensor."""
+    torch = _torch()
+    ids = _gpu_tensor(ids, what)
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise OrdaError(f"{what} must be int64 or int32, got {ids.dtype}")
+    _same_device(device, **{what: ids})
+    return ids.reshape(-1).contiguous()
+
+
+def embedding(ids, weight, *, scale: float = 1.0):
+    """``scale * weight[ids]``: ``ids`` (int64 or int32, any shape) select rows of
+    ``weight`` [V, H] (float32 or bfloat16); the product is rounded once to the
+    weight's type. Returns ``[*ids.shape, H]``. An id that is no row gives a row
+    of NaN."""
+    torch = _torch()
+    w = _matrix(_gpu_tensor(weight, "weight"), "weight")
+    wd = _desc(w, "weight")
+    i = _ids(ids, w.device)
+    out = torch.empty((i.numel(), w.size(1)), dtype=w.dtype, device=w.device)
+    _call(L.load().orda_embedding, w.device.index, _stream(w.device), i.data_ptr(), i.element_size(),
+          i.numel(), C.byref(wd), scale, C.byref(_desc(out, "out")))
+    return out.view(*ids.shape, w.size(1))
+
+
+def embedding_backward(grad, ids, num_rows: int, *, scale: float = 1.0,
+                       padding_idx: Optional[int] = None, out=None, accumulate: bool = False):
+    """Gradient of ``embedding`` with respect to its weight: row ``v`` is ``scale *
+    sum(grad[t] for ids[t] == v)``, added in the order of the tokens in fp32 and
+    rounded once.
+
+    ``grad`` is ``[*ids.shape, H]``, float32 or bfloat16. The result is
+    ``[num_rows, H]`` in grad's type, or goes to ``out`` (float32 or bfloat16, 2-D
+    with adjacent columns); with ``accumulate`` it is added to ``out``, of which
+    only the rows that an id names are read and written (a tied weight's
+    gradient, after its other use). Tokens equal to ``padding_idx`` (counted from
+    the end where negative), and ids that are no row, add nothing.
+    """
+    torch = _torch()
+    g = _gpu_tensor(grad, "grad")
+    i = _ids(ids, g.device)
+    if g.dim() != ids.dim() + 1 or tuple(g.shape[:-1]) != tuple(ids.shape):
+        raise OrdaError(f"grad must be [*ids.shape, H], got {list(g.shape)} for ids {list(ids.shape)}")
+    h = g.size(-1)
+    g = _matrix(g.reshape(-1, h) if h else g.new_empty((i.numel(), 0)), "grad")
+    gd = _desc(g, "grad")
+    if num_rows < 0:
+        raise OrdaError("num_rows must be >= 0")
+    pad = -1
+    if padding_idx is not None:
+        pad = padding_idx + num_rows if padding_idx < 0 else padding_idx
+        if not 0 <= pad < num_rows:
+            raise OrdaError(f"padding_idx must be a row of {num_rows}, got {padding_idx}")
+    if out is None:
+        if accumulate:
+            raise OrdaError("accumulate needs out")
+        out = torch.empty((num_rows, h), dtype=g.dtype, device=g.device)
+    else:
+        out = _gpu_tensor(out, "out")
+        _same_device(g.device, out=out)
+        if tuple(out.shape) != (num_rows, h):
+            raise OrdaError(f"out must be [{num_rows}, {h}]")
+        if _matrix(out, "out") is not out:
+            raise OrdaError("out must have adjacent columns and rows that do not overlap")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise OrdaError("out must not require a gradient")
+        if _overlap(out, g):
+            raise OrdaError("out must not share memory with grad")
+    od = _desc(out, "out")
+    lib = L.load()
+    n = C.c_int64()
+    _call(lib.orda_embedding_backward_workspace, i.numel(), num_rows, h, gd.dtype, C.byref(n))
+    ws = _bytes(n.value, g.device)
+    _call(lib.orda_embedding_backward, g.device.index, _stream(g.device), i.data_ptr(), i.element_size(),
+          i.numel(), C.byref(gd), pad, scale, int(accumulate), C.byref(od), ws.data_ptr(), ws.numel())
+    torch.autograd.graph.increment_version(out)   # written in place
+    return out
