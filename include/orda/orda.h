@@ -377,6 +377,40 @@ int32_t orda_embedding_backward(int32_t device, void *hip_stream, const void *id
                                 int32_t accumulate, orda_tensor *out, void *workspace,
                                 int64_t workspace_bytes, char *err, size_t err_len);
 
+/* ---- e4m3 with block scales -------------------------------------------------- */
+/* Matrices in 8-bit floating point (e4m3: 4 exponent bits, 3 of mantissa, no
+ * infinity, largest value 448) with one fp32 scale for each block of 128 columns
+ * and block_rows rows, and their product: the logits of a teacher whose head is
+ * held in 8 bits, for orda_teacher's logits. Everything is on `device`; the
+ * calls queue their kernels on hip_stream (NULL: the null stream) and return,
+ * allocate nothing and can be captured. At most 2^30 rows and 2^20 columns. No
+ * counterpart in the reference, whose quantisation is INT8 by rows. */
+typedef struct {
+    void *codes;          /* [rows,cols], one byte each, rows ld bytes apart */
+    int64_t rows, cols, ld;
+    float *scales;        /* block (i,j) at i*scale_row + j*scale_col */
+    int64_t scale_row, scale_col;
+    int32_t block_rows;   /* 1 or 128 */
+} orda_fp8_matrix;
+/* scale = max(largest |m| of the block / 448, 2^-126), code = m / scale rounded to
+ * nearest even, both quotients in fp32; a block with an infinity or a NaN has the
+ * scale NaN and codes NaN. m [rows,cols] fp32 or bf16. out gives the buffers:
+ * codes 8-byte aligned, ld a multiple of 8 (the columns from cols up to the next
+ * multiple of 8 are written too). */
+int32_t orda_quant_fp8_blocks(int32_t device, void *hip_stream, const orda_tensor *m,
+                              orda_fp8_matrix *out, char *err, size_t err_len);
+/* out[m,n] = Σ_j scale_a[m,j]·scale_b[n/128,j]·Σ_k code_a[m,k]·code_b[n,k], k over
+ * the 128 columns of block j; sums in fp32, rounded once to out's type (fp32 or
+ * bf16). a has block_rows 1, b 128. Codes whose base or pitch is no multiple of
+ * 16 are copied into workspace first (256-byte aligned, the call's alone until
+ * its kernels have run). Columns of codes between cols and ld are not read as
+ * values. Scale strides are at least 0; a's rows' at most 2^22. */
+int32_t orda_fp8_block_matmul_workspace(const orda_fp8_matrix *a, const orda_fp8_matrix *b, int64_t *bytes,
+                                        char *err, size_t err_len);
+int32_t orda_fp8_block_matmul(int32_t device, void *hip_stream, const orda_fp8_matrix *a,
+                              const orda_fp8_matrix *b, orda_tensor *out, void *workspace,
+                              int64_t workspace_bytes, char *err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,410 @@
+// fp8.hip — matrices in e4m3 with one fp32 scale for each block of 128 columns
+// (and of 1 or 128 rows): the quantiser and the product.
+#include <float.h>
+#include <math.h>
+
+#include "lds_dma.h"
+#include "orda_kernels.h"
+
+namespace orda {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) const float lds_f32;
+
+// ------------------------------------------------------------ quantiser
+// scale = max(amax / 448, 2^-126), code = x / scale rounded to nearest even, both
+// quotients in fp32: |x / scale| is at most 448 but for its rounding, which the
+// clamp takes back. A block with an infinity or a NaN has the scale NaN and codes
+// NaN. Bound by HBM (each value is read once into registers; the two IEEE
+// divisions cost about as long as the bytes of bf16 values).
+constexpr float kE4m3Max = 448.f;
+
+__device__ __forceinline__ float scale_of(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return fmaxf(__uint_as_float(amax_bits) / kE4m3Max, FLT_MIN);
+}
+__device__ __forceinline__ float coded(float x, float s) {
+  const float q = x / s;
+  return q != q ? q : fminf(fmaxf(q, -kE4m3Max), kE4m3Max);
+}
+__device__ __forceinline__ uint32_t codes4(const float* x, float s) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(coded(x[0], s), coded(x[1], s), 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(coded(x[2], s), coded(x[3], s), w, true);
+  return static_cast<uint32_t>(w);
+}
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Eight values of a row from column c on (0 past cols).
+template <typename E, bool VEC>
+__device__ __forceinline__ void load8(const E* row, int64_t c, int64_t cols, float (&x)[8]) {
+  if (VEC && c + 8 <= cols) {
+    alignas(16) E w[8];
+#pragma unroll
+    for (int b = 0; b < static_cast<int>(sizeof(w)) / 16; ++b)
+      reinterpret_cast<u32x4*>(w)[b] = reinterpret_cast<const u32x4*>(row + c)[b];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = static_cast<float>(w[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = c + k < cols ? static_cast<float>(row[c + k]) : 0.f;
+  }
+}
+// Their codes, the eight that hold the last column whole.
+__device__ __forceinline__ void store8(uint8_t* row, int64_t c, int64_t cols, const float (&x)[8], float s) {
+  if (c < cols) *reinterpret_cast<u32x2*>(row + c) = u32x2{codes4(x, s), codes4(x + 4, s)};
+}
+
+// Blocks of one row: 16 lanes a block of 128, a wave 4 blocks of each of 4 rows,
+// a workgroup 16 rows, whose scales leave as 64 bytes a block.
+template <typename E, bool VEC>
+__global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a) {
+  __shared__ float sc[4][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t groups = (a.cols + 511) / 512;
+  const int64_t r0 = blockIdx.x / groups * 16, c0 = blockIdx.x % groups * 512;
+  const int64_t c = c0 + lane * 8;
+  const E* src = static_cast<const E*>(a.src);
+  float x[4][8];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int64_t r = r0 + wave * 4 + q;
+    load8<E, VEC>(src + (r < a.rows ? r : a.rows - 1) * a.lds, c, a.cols, x[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int64_t r = r0 + wave * 4 + q;
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = abs_bits(x[q][k]) > m ? abs_bits(x[q][k]) : m;
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+      const uint32_t o = __shfl_xor(m, d);
+      m = o > m ? o : m;
+    }
+    const float s = scale_of(m);
+    if (r < a.rows) store8(a.codes + r * a.ldc, c, a.cols, x[q], s);
+    if ((lane & 15) == 0) sc[lane >> 4][wave * 4 + q] = s;
+  }
+  __syncthreads();
+  const int b = threadIdx.x >> 4, k = threadIdx.x & 15;
+  if (b < 4 && c0 + b * 128 < a.cols && r0 + k < a.rows)
+    a.scales[(r0 + k) * a.scale_row + (c0 / 128 + b) * a.scale_col] = sc[b][k];
+}
+
+// Blocks of 128 rows: a workgroup holds a block in registers, 8 rows x 8
+// columns a thread.
+template <typename E, bool VEC>
+__global__ __launch_bounds__(256) void fp8_quant_blocks_kernel(Fp8QuantArgs a) {
+  __shared__ uint32_t top[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t cb = (a.cols + 127) / 128;
+  const int64_t rb = blockIdx.x / cb, kb = blockIdx.x % cb;
+  const int64_t c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
+  const E* src = static_cast<const E*>(a.src);
+  float x[8][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int64_t r = r0 + 16 * q;
+    load8<E, VEC>(src + (r < a.rows ? r : a.rows - 1) * a.lds, c, a.cols, x[q]);   // the last row again
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = abs_bits(x[q][k]) > m ? abs_bits(x[q][k]) : m;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t o = __shfl_xor(m, d);
+    m = o > m ? o : m;
+  }
+  if (lane == 0) top[wave] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = top[w] > m ? top[w] : m;
+  const float s = scale_of(m);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int64_t r = r0 + 16 * q;
+    if (r < a.rows) store8(a.codes + r * a.ldc, c, a.cols, x[q], s);
+  }
+  if (threadIdx.x == 0) a.scales[rb * a.scale_row + kb * a.scale_col] = s;
+}
+
+// Rows of codes at a pitch of whole 16s, zeros past cols.
+__global__ __launch_bounds__(256) void fp8_pack_kernel(const uint8_t* src, int64_t lds, int64_t rows, int64_t cols,
+                                                       uint8_t* dst, int64_t ldd) {
+  const int64_t per = ldd / 16;
+  for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < rows * per; i += gridDim.x * int64_t{256}) {
+    const int64_t r = i / per, c = (i - r * per) * 16;
+    alignas(16) uint8_t w[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) w[k] = c + k < cols ? src[r * lds + c + k] : 0;
+    *reinterpret_cast<u32x4*>(dst + r * ldd + c) = *reinterpret_cast<const u32x4*>(w);
+  }
+}
+
+// ------------------------------------------------------------ product
+// C[m, n] = Σ_b sa[m, b] · sb[n / 128, b] · Σ_{k in block b} a[m, k] · b[n, k].
+//
+// One 16x16x128 MFMA is one block of K: its result is a block's plain sum, which
+// is scaled into the fp32 accumulators by a fma an element. The vector units
+// reach only half of a wave's 512 registers, so a wave holds 128 x 64 of C there
+// (128 registers), and a workgroup of 8 waves 256 x 256; while one of a SIMD's two
+// waves scales, the other multiplies. K advances one block at a time through two
+// 64 KB stages in LDS, moved by DMA while the other is read: rows of 128
+// bytes, their eight 16-byte chunks swizzled by row (by the choice of the chunk a
+// lane fetches), so that fragment reads meet no bank twice. The operands enter
+// the MFMA swapped: a lane then owns four consecutive columns of a row.
+//
+// The e4m3 MFMAs (all four shapes, measured) add their products to fewer bits than
+// fp32: a sum of 128 comes out 1.5e-5 off relative to the sums' norm. Beside bf16
+// outputs, rounded at 1.7e-3, that is nothing; for fp32 outputs (WIDE) the codes
+// are widened to bf16, exactly, as fragments are read, and a block is four
+// 16x16x32 bf16 MFMAs (9e-9 off), at half the matrix rate.
+constexpr int kTile = 256, kThreads = 512;
+constexpr int kOp = kTile * 128;                      // an operand's stage
+constexpr int kScales = kTile * 4 + 64;               // A's row scales, B's two
+constexpr int kStage = 2 * kOp;
+
+__device__ __forceinline__ void dma4(uint64_t sbase, uint32_t voff, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %0"
+               :
+               : "s"(sbase), "v"(voff), "s"(m0)
+               : "memory", "m0");
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// Tile t of the raster: XCDs take contiguous ranges, walked in groups of 8
+// M-tiles, so that the tiles of an XCD share operand strips in its L2.
+__device__ __forceinline__ void tile_of(int64_t t, int64_t mt, int64_t nt, int64_t& m, int64_t& n) {
+  const int64_t per = mt * nt / 8;
+  if (t < per * 8) t = (t % 8) * per + t / 8;
+  const int64_t group = 8 * nt, first = t / group * 8, size = mt - first < 8 ? mt - first : 8, r = t % group;
+  m = first + r % size;
+  n = r / size;
+}
+
+// A fragment's 32 codes of a lane as bf16, eight for each of four MFMAs.
+struct Wide {
+  bf16x8 k[4];
+};
+__device__ __forceinline__ Wide widened(const i32x8& f) {
+  Wide w;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * q + h], 1.f, false);
+      const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * q + h], 1.f, true);
+      w.k[q][4 * h] = lo[0];
+      w.k[q][4 * h + 1] = lo[1];
+      w.k[q][4 * h + 2] = hi[0];
+      w.k[q][4 * h + 3] = hi[1];
+    }
+  }
+  return w;
+}
+
+template <typename OT, bool WIDE>
+__global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * kStage + 2 * kScales];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  int64_t mi, ni;
+  tile_of(blockIdx.x, (a.m + kTile - 1) / kTile, (a.n + kTile - 1) / kTile, mi, ni);
+  const int64_t m0 = mi * kTile, n0 = ni * kTile;
+  // This thread's four 16-byte chunks of each operand's stage: LDS chunk p =
+  // t·512 + tid is chunk p % 8 of row p / 8. Rows past the edge are the last one
+  // (their outputs are not stored).
+  uint32_t offA[4], offB[4];
+  int kcol;   // first K of the chunk, the same for all four
+  {
+    const int r = tid >> 3, q = (tid & 7) ^ (r & 7);
+    kcol = q * 16;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int64_t rr = r + 64 * t;
+      const int64_t ra = m0 + rr < a.m ? rr : a.m - 1 - m0, rb = n0 + rr < a.n ? rr : a.n - 1 - n0;
+      offA[t] = static_cast<uint32_t>(ra * a.lda + kcol);
+      offB[t] = static_cast<uint32_t>(rb * a.ldb + kcol);
+    }
+  }
+  const unsigned char* const pa = a.a + m0 * a.lda;
+  const unsigned char* const pb = a.b + n0 * a.ldb;
+  // Scales of a stage: waves 0-3 fetch a row's each, wave 4 B's two blocks'.
+  const float* const psa = a.sa + m0 * a.sa_row;
+  const int64_t nb0 = n0 / 128, nbs = (a.n + 127) / 128;
+  const float* const psb = a.sb + nb0 * a.sb_row;
+  uint32_t offS = 0;
+  if (wave < 4) {
+    const int64_t r = m0 + tid < a.m ? tid : a.m - 1 - m0;
+    offS = static_cast<uint32_t>(r * a.sa_row * 4);
+  } else if (wave == 4) {
+    offS = static_cast<uint32_t>(((lane & 1) != 0 && nb0 + 1 < nbs ? 1 : 0) * a.sb_row * 4);
+  }
+  const uint32_t lds0 = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
+      static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)smem))));
+  const int nkb = static_cast<int>((a.k + 127) / 128);
+  auto issue = [&](int kb, int buf) {
+    const uint32_t st = lds0 + buf * kStage + wave * 1024;
+    const unsigned char* const sa = pa + kb * int64_t{128};
+    const unsigned char* const sb = pb + kb * int64_t{128};
+    const int krem = static_cast<int>(a.k - kb * int64_t{128});
+    if (krem >= 128) {
+      const uint64_t ua = uniform64(sa), ub = uniform64(sb);
+      dma16_at<0>(ua, offA[0], st);
+      dma16_at<8192>(ua, offA[1], st);
+      dma16_at<16384>(ua, offA[2], st);
+      dma16_at<24576>(ua, offA[3], st);
+      dma16_at<kOp>(ub, offB[0], st);
+      dma16_at<kOp + 8192>(ub, offB[1], st);
+      dma16_at<kOp + 16384>(ub, offB[2], st);
+      dma16_at<kOp + 24576>(ub, offB[3], st);
+    } else {   // the last, partial block: zeros past K
+      unsigned char* const l = smem + buf * kStage + wave * 1024 + lane * 16;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const unsigned char* const src = t < 4 ? sa + offA[t & 3] : sb + offB[t & 3];
+        alignas(16) unsigned char w[16];
+        if (kcol + 16 <= krem) {
+          *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(src);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) w[k] = kcol + k < krem ? src[k] : 0;
+        }
+        *reinterpret_cast<u32x4*>(l + (t & 3) * 8192 + (t < 4 ? 0 : kOp)) = *reinterpret_cast<const u32x4*>(w);
+      }
+    }
+    const uint32_t sc = lds0 + 2 * kStage + buf * kScales;
+    if (wave < 4) dma4(uniform64(psa + kb * a.sa_col), offS, sc + wave * 256);
+    else if (wave == 4 && lane < 2) dma4(uniform64(psb + kb * a.sb_col), offS, sc + 1024);
+  };
+  f32x4 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int lrow = lane & 15, lgrp = lane >> 4;
+  // Fragment of 16 rows from LDS address base: lane (row lrow, group lgrp) holds
+  // K 32·lgrp .. +31, chunks 2·lgrp and 2·lgrp + 1 (both operands alike).
+  const uint32_t f0 = static_cast<uint32_t>(lrow * 128 + (((2 * lgrp) ^ (lrow & 7)) << 4));
+  const uint32_t f1 = static_cast<uint32_t>(lrow * 128 + (((2 * lgrp + 1) ^ (lrow & 7)) << 4));
+  auto frag = [&](uint32_t base) {
+    const u32x4 lo = *(const lds_u32x4*)(static_cast<uintptr_t>(base + f0));
+    const u32x4 hi = *(const lds_u32x4*)(static_cast<uintptr_t>(base + f1));
+    return __builtin_bit_cast(i32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  issue(0, 0);
+  for (int kb = 0; kb < nkb; ++kb) {
+    const int buf = kb & 1;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kWaitAll);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (kb + 1 < nkb) issue(kb + 1, buf ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t st = lds0 + buf * kStage, sc = lds0 + 2 * kStage + buf * kScales;
+    using F = std::conditional_t<WIDE, Wide, i32x8>;
+    auto operand = [&](uint32_t base) -> F {
+      if constexpr (WIDE) return widened(frag(base));
+      else return frag(base);
+    };
+    F b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = operand(st + kOp + (wn * 64 + j * 16) * 128);
+    const float s_b = *(const lds_f32*)(static_cast<uintptr_t>(sc + 1024 + (wn >> 1) * 4));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const F x = operand(st + (wm * 128 + i * 16) * 128);
+      const float s = s_b * *(const lds_f32*)(static_cast<uintptr_t>(sc + (wm * 128 + i * 16 + lrow) * 4));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 p = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j].k[q], x.k[q], p, 0, 0, 0);
+        } else {
+          p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], x, p, 0, 0, 0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(s, p[e], acc[i][j][e]);
+      }
+    }
+  }
+  // acc[i][j][e] is row m0 + wm·128 + 16i + lrow, column n0 + wn·64 + 16j + 4·lgrp + e.
+  OT* const C = static_cast<OT*>(a.c);
+  const int64_t col0 = n0 + wn * 64 + 4 * lgrp;
+  const bool vec = a.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(C) % (4 * sizeof(OT)) == 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = m0 + wm * 128 + i * 16 + lrow;
+    if (row >= a.m) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      OT* const d = C + row * a.ldc + col0 + j * 16;
+      const f32x4 v = acc[i][j];
+      if (vec && col0 + j * 16 + 4 <= a.n) {
+        if constexpr (sizeof(OT) == 2) *reinterpret_cast<u32x2*>(d) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+        else *reinterpret_cast<f32x4*>(d) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col0 + j * 16 + e < a.n) d[e] = static_cast<OT>(v[e]);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_fp8_quant(const Fp8QuantArgs& a, DType t, bool blocks, hipStream_t stream) {
+  if (a.rows <= 0 || a.cols <= 0) return hipSuccess;
+  if (a.ldc % 8 != 0 || reinterpret_cast<uintptr_t>(a.codes) % 8 != 0) return hipErrorInvalidValue;
+  const bool vec = a.lds * dtype_size(t) % 16 == 0 && reinterpret_cast<uintptr_t>(a.src) % 16 == 0;
+  const int64_t grid = blocks ? (a.rows + 127) / 128 * ((a.cols + 127) / 128) : (a.rows + 15) / 16 * ((a.cols + 511) / 512);
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  using K = void (*)(Fp8QuantArgs);
+  K k;
+  if (blocks)
+    k = t == DType::BF16 ? (vec ? fp8_quant_blocks_kernel<__bf16, true> : fp8_quant_blocks_kernel<__bf16, false>)
+                         : (vec ? fp8_quant_blocks_kernel<float, true> : fp8_quant_blocks_kernel<float, false>);
+  else
+    k = t == DType::BF16 ? (vec ? fp8_quant_rows_kernel<__bf16, true> : fp8_quant_rows_kernel<__bf16, false>)
+                         : (vec ? fp8_quant_rows_kernel<float, true> : fp8_quant_rows_kernel<float, false>);
+  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_fp8_pack(const uint8_t* src, int64_t lds, int64_t rows, int64_t cols, uint8_t* dst, int64_t ldd,
+                           hipStream_t stream) {
+  if (ldd % 16 != 0 || reinterpret_cast<uintptr_t>(dst) % 16 != 0) return hipErrorInvalidValue;
+  const int64_t n = (rows * (ldd / 16) + 255) / 256;
+  if (n <= 0) return hipSuccess;
+  hipLaunchKernelGGL(fp8_pack_kernel, dim3(static_cast<unsigned>(n < 65536 ? n : 65536)), dim3(256), 0, stream, src, lds,
+                     rows, cols, dst, ldd);
+  return hipGetLastError();
+}
+
+hipError_t launch_fp8_mm(const Fp8MmArgs& a, DType out, hipStream_t stream) {
+  if (a.m <= 0 || a.n <= 0) return hipSuccess;
+  if (a.lda % 16 != 0 || a.ldb % 16 != 0 || reinterpret_cast<uintptr_t>(a.a) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(a.b) % 16 != 0)
+    return hipErrorInvalidValue;
+  const int64_t tiles = (a.m + kTile - 1) / kTile * ((a.n + kTile - 1) / kTile);
+  if (tiles > 0x7fffffff) return hipErrorInvalidValue;
+  auto* k = out == DType::BF16 ? fp8_mm_kernel<__bf16, false> : fp8_mm_kernel<float, true>;
+  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace orda

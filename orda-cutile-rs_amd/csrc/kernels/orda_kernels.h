@@ -484,4 +484,33 @@ struct EmbedGradArgs {
 };
 hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t stream);
 
+// ---------------------------------------------------------------- e4m3 with block scales
+// codes (e4m3, rows of pitch ldc, a multiple of 8; the last eight of a row is
+// written whole) and scales of blocks of 128 columns and 1 row (or 128, `blocks`) of src.
+struct Fp8QuantArgs {
+  const void* src;
+  int64_t lds, rows, cols;
+  uint8_t* codes;
+  int64_t ldc;
+  float* scales;           // block (r, c) at r*scale_row + c*scale_col
+  int64_t scale_row, scale_col;
+};
+hipError_t launch_fp8_quant(const Fp8QuantArgs& a, DType t, bool blocks, hipStream_t stream);
+// Rows of codes at a pitch of whole 16s.
+hipError_t launch_fp8_pack(const uint8_t* src, int64_t lds, int64_t rows, int64_t cols, uint8_t* dst, int64_t ldd,
+                           hipStream_t stream);
+// C[m,n] = A[m,k] · B[n,k]ᵀ: A with a scale for each row and 128 columns, B for
+// each 128 rows and 128 columns. Bases 16-byte aligned, pitches multiples of 16
+// and at most 2^24, scale strides at most 2^22.
+struct Fp8MmArgs {
+  const unsigned char *a, *b;
+  int64_t lda, ldb;
+  const float *sa, *sb;
+  int64_t sa_row, sa_col, sb_row, sb_col;
+  void* c;
+  int64_t ldc;
+  int64_t m, n, k;
+};
+hipError_t launch_fp8_mm(const Fp8MmArgs& a, DType out, hipStream_t stream);
+
 }  // namespace orda

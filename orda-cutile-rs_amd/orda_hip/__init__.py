@@ -17,8 +17,8 @@ from typing import Any, Optional
 import numpy as np
 
 from . import _lib as L
-from .operators import (embedding, embedding_backward, linear_cross_entropy,
-                        linear_cross_entropy_backward)
+from .operators import (embedding, embedding_backward, fp8_block_matmul, linear_cross_entropy,
+                        linear_cross_entropy_backward, quantize_fp8_blocks)
 from .types import (Backend, ChunkPlan, ChunkSize, DistillationLossOutput, KernelConfig,
                     LossOptions, OrdaError, Profile, Reduction, Teacher, TeacherMode,
                     DEFAULT_MAX_FUSED_SIZE, is_power_of_two)
@@ -27,9 +27,10 @@ __all__ = [
     "Backend", "ChunkPlan", "ChunkSize", "Context", "DistillationLossOutput", "KernelConfig",
     "LossOptions", "OrdaError", "Profile", "Reduction", "Teacher", "TeacherMode",
     "DEFAULT_MAX_FUSED_SIZE", "chunk_doubling_schedule", "chunks_from_raw",
-    "default_max_chunks_limit", "distillation_loss", "embedding", "embedding_backward", "is_available", "is_power_of_two",
+    "default_max_chunks_limit", "distillation_loss", "embedding", "embedding_backward",
+    "fp8_block_matmul", "is_available", "is_power_of_two",
     "kl_ce_on_logits_chunk", "linear_cross_entropy", "linear_cross_entropy_backward",
-    "quant_rows_int8", "resolve_chunk_size", "lib_path",
+    "quant_rows_int8", "quantize_fp8_blocks", "resolve_chunk_size", "lib_path",
 ]
 
 lib_path = L.LIB_PATH

@@ -82,6 +82,12 @@ class LinearCeC(C.Structure):
                 ("label_smoothing", C.c_float), ("vocab_piece", C.c_int64)]
 
 
+class Fp8MatrixC(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("ld", C.c_int64),
+                ("scales", C.c_void_p), ("scale_row", C.c_int64), ("scale_col", C.c_int64),
+                ("block_rows", C.c_int32)]
+
+
 # (name, restype, argtypes) for every entry point of include/orda/orda.h.
 SIGNATURES = [
     ("orda_abi_version", C.c_int32, []),
@@ -145,6 +151,13 @@ SIGNATURES = [
     ("orda_embedding_backward", C.c_int32,
      [C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.POINTER(Tensor), C.c_int64,
       C.c_float, C.c_int32, C.POINTER(Tensor), C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t]),
+    ("orda_quant_fp8_blocks", C.c_int32,
+     [C.c_int32, C.c_void_p, C.POINTER(Tensor), C.POINTER(Fp8MatrixC), C.c_char_p, C.c_size_t]),
+    ("orda_fp8_block_matmul_workspace", C.c_int32,
+     [C.POINTER(Fp8MatrixC), C.POINTER(Fp8MatrixC), C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
+    ("orda_fp8_block_matmul", C.c_int32,
+     [C.c_int32, C.c_void_p, C.POINTER(Fp8MatrixC), C.POINTER(Fp8MatrixC), C.POINTER(Tensor),
+      C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t]),
 ]
 
 _lib = None

@@ -4,6 +4,9 @@
   language-model head without keeping its logits.
 * ``embedding`` / ``embedding_backward``: rows of the same weight by token id,
   and their share of its gradient.
+* ``quantize_fp8_blocks`` / ``fp8_block_matmul``: matrices in e4m3 with a scale for
+  each block of 128, and their product (a teacher's logits from a head held in 8
+  bits, for ``Teacher.Precomputed``). Not differentiable.
 
 Every call queues its kernels on torch's current stream of the inputs' device
 and returns without waiting; outputs and scratch come from torch's allocator, so
@@ -274,4 +277,79 @@ def embedding_backward(grad, ids, num_rows: int, *, scale: float = 1.0,
     _call(lib.orda_embedding_backward, g.device.index, _stream(g.device), i.data_ptr(), i.element_size(),
           i.numel(), C.byref(gd), pad, scale, int(accumulate), C.byref(od), ws.data_ptr(), ws.numel())
     torch.autograd.graph.increment_version(out)   # written in place
+    return out
+
+
+# ------------------------------------------------------------------ e4m3 with block scales
+def _fp8_desc(codes, scales, block_rows: int, what: str):
+    """(orda_fp8_matrix, the tensors it points into) of codes [R, C] and scales
+    [ceil(R / block_rows), ceil(C / 128)]."""
+    torch = _torch()
+    c = _gpu_tensor(codes, what)
+    if c.dtype != torch.float8_e4m3fn:
+        raise OrdaError(f"{what} must be float8_e4m3fn, got {c.dtype}")
+    c = _matrix(c, what)
+    s = _gpu_tensor(scales, f"{what}'s scales")
+    _same_device(c.device, **{f"{what}'s scales": s})
+    shape = (-(-c.size(0) // block_rows), -(-c.size(1) // 128))
+    if s.dtype != torch.float32 or tuple(s.shape) != shape:
+        raise OrdaError(f"{what}'s scales must be float32 {list(shape)}")
+    d = L.Fp8MatrixC(codes=c.data_ptr(), rows=c.size(0), cols=c.size(1),
+                     ld=c.stride(0) if c.size(0) > 1 else -(-c.size(1) // 16) * 16,
+                     scales=s.data_ptr(), scale_row=s.stride(0) if shape[0] > 1 else 0,
+                     scale_col=s.stride(1) if shape[1] > 1 else 0, block_rows=block_rows)
+    return d, (c, s)
+
+
+def quantize_fp8_blocks(m, *, block_rows: int = 1) -> Tuple:
+    """``(codes, scales)`` of ``m`` [R, C] (float32 or bfloat16): float8_e4m3fn codes
+    [R, C] and one float32 scale for each block of 128 columns and ``block_rows``
+    rows (1 or 128), [ceil(R / block_rows), ceil(C / 128)].
+
+    ``scale = max(amax / 448, 2**-126)`` and ``code = m / scale`` rounded to nearest
+    even, both quotients in float32; a block with an infinity or a NaN has the
+    scale NaN and codes NaN. The rows of ``codes`` lie a multiple of 16 bytes apart,
+    and the scales of single rows block by block, as ``fp8_block_matmul`` reads
+    them best.
+    """
+    torch = _torch()
+    m = _matrix(_gpu_tensor(m, "m"), "m")
+    md = _desc(m, "m")
+    if block_rows not in (1, 128):
+        raise OrdaError(f"block_rows must be 1 or 128, got {block_rows}")
+    r, c = m.shape
+    pitch = -(-c // 16) * 16
+    codes = torch.empty((r, pitch), dtype=torch.float8_e4m3fn, device=m.device)[:, :c]
+    rb, cb = -(-r // block_rows), -(-c // 128)
+    scales = (torch.empty((cb, rb), dtype=torch.float32, device=m.device).t() if block_rows == 1
+              else torch.empty((rb, cb), dtype=torch.float32, device=m.device))
+    d = L.Fp8MatrixC(codes=codes.data_ptr(), rows=r, cols=c, ld=pitch, scales=scales.data_ptr(),
+                     scale_row=1 if block_rows == 1 else cb, scale_col=rb if block_rows == 1 else 1,
+                     block_rows=block_rows)
+    _call(L.load().orda_quant_fp8_blocks, m.device.index, _stream(m.device), C.byref(md), C.byref(d))
+    return codes, scales
+
+
+def fp8_block_matmul(a, a_scales, b, b_scales, *, out_dtype=None):
+    """``A @ B.T`` of quantised matrices: ``a`` [M, K] with a scale for each row and 128
+    columns (``a_scales`` [M, ceil(K / 128)]), ``b`` [N, K] for each 128 rows and 128
+    columns (``b_scales`` [ceil(N / 128), ceil(K / 128)]), as ``quantize_fp8_blocks``
+    makes them with ``block_rows`` 1 and 128, or a checkpoint holds them. Sums are
+    float32, rounded once to ``out_dtype`` (bfloat16, the default, or float32).
+    Returns [M, N]. Codes whose memory or pitch is not 16-byte aligned are copied
+    first."""
+    torch = _torch()
+    ad, (a, _sa) = _fp8_desc(a, a_scales, 1, "a")
+    bd, (b, _sb) = _fp8_desc(b, b_scales, 128, "b")
+    _same_device(a.device, b=b)
+    out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise OrdaError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+    lib = L.load()
+    n = C.c_int64()
+    _call(lib.orda_fp8_block_matmul_workspace, C.byref(ad), C.byref(bd), C.byref(n))
+    ws = _bytes(n.value, a.device)
+    out = torch.empty((a.size(0), b.size(0)), dtype=out_dtype, device=a.device)
+    _call(lib.orda_fp8_block_matmul, a.device.index, _stream(a.device), C.byref(ad), C.byref(bd),
+          C.byref(_desc(out, "out")), ws.data_ptr(), ws.numel())
     return out
