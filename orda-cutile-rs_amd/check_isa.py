@@ -133,7 +133,7 @@ def check(path):
     checked = 0
     for fn in re.split(r"\n(?=_Z\w+:)", text):
         name = fn.split(":")[0]
-        if not re.search(r"gemm_(kk|km|kmt)_(logits|logits_pre|logits_pre16|store|accum|cestats|cegrad|dyn_store|dyn_accum)_bf16", name):
+        if not re.search(r"gemm_(kk|km|kmt)_(logits|logits_pre|logits_pre16|store|accum|cestats|cegrad|dyn_store)_bf16", name):
             continue
         checked += 1
         end = fn.find("s_endpgm")
@@ -160,8 +160,8 @@ def check(path):
                     entry[j] = merged
                     if j not in work:
                         work.append(j)
-    if checked < 23:
-        errors.add(f"expected the 23 bf16 GEMM variants with inline MFMAs, found {checked}")
+    if checked < 21:
+        errors.add(f"expected the 21 bf16 GEMM variants with inline MFMAs, found {checked}")
     return sorted(errors)
 
 

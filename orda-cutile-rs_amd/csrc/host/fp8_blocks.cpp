@@ -8,8 +8,6 @@ namespace {
 
 constexpr int64_t kMaxPitch = int64_t{1} << 20, kMaxStride = int64_t{1} << 22, kMaxRows = int64_t{1} << 30;
 
-int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
-
 // A quantised matrix: its shape, pitch and scale strides.
 void check_matrix(const orda_fp8_matrix& m, const char* what) {
   if (m.rows < 0 || m.cols < 0) fail(ORDA_ERR_INVALID, "%s has a negative shape", what);

@@ -80,11 +80,10 @@ Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool
   return c;
 }
 
-// The scratch of a call, laid out from base (null: only its size counts).
+// The scratch of a call, laid out from base.
 struct Scratch {
   CeRows rows;
-  void* x;           // compact hidden rows (the input's type)
-  void* x3;          // their planes
+  void* x;           // compact hidden rows, or their planes
   void* xt;          // transposed: grad_weight's K-major operand
   void* w;           // a piece of the weights, padded or as planes
   void* ds;          // gradient of a piece's logits
@@ -123,14 +122,16 @@ GemmArgs logits_product(const Ce& c, const Scratch& s, int64_t v0, int64_t cols)
   if (c.planes) {
     g.lda = g.ldb = 3 * c.hp;
     g.plane_a = g.plane_b = c.hp;
-    g.prob[0] = {s.x3, s.w, nullptr};
+    g.prob[0] = {s.x, s.w, nullptr};
   } else {
     g.K = c.h;
   }
   return g;
 }
 
-GemmArgs grad_hidden_product(const Ce& c, const Scratch& s, int64_t v0, int64_t cols) {
+// The piece's share of grad_hidden: added to the pieces before it in s.gh, and
+// with the last piece written to its rows' places.
+GemmArgs grad_hidden_product(const Ce& c, const Scratch& s, const orda_tensor* gh, int64_t v0, int64_t cols) {
   GemmArgs g = product(c, s);
   g.M = c.n;
   g.N = c.h;
@@ -138,9 +139,16 @@ GemmArgs grad_hidden_product(const Ce& c, const Scratch& s, int64_t v0, int64_t 
   g.lda = ds_pitch(c, c.piece);
   g.ldb = c.stage_w ? c.hp : c.ldw;
   g.ldc = round8(c.h);
-  g.epi = v0 == 0 ? GemmEpilogue::StoreF32 : GemmEpilogue::AccumF32;
+  g.epi = GemmEpilogue::StoreF32;
   g.group_m = 4;
   g.share_rounds = true;
+  g.ce.accum = v0 > 0;
+  if (gh != nullptr && v0 + cols == c.v) {
+    g.ce.src = s.rows.src;
+    g.ce.out = gh->data;
+    g.ce.ldo = tensor_ld(*gh);
+    g.ce.out_type = c.t;
+  }
   g.prob[0] = {s.ds, c.stage_w ? s.w : static_cast<const char*>(c.w) + v0 * c.ldw * 2, s.gh};
   if (c.planes) {
     g.ldb = 3 * c.hp;
@@ -172,21 +180,22 @@ GemmArgs grad_weight_product(const Ce& c, const Scratch& s, void* gw, int64_t ld
   return g;
 }
 
+// (Sizes depend on which pointers are set, so a layout is made from a base that
+// is not null also where only its size counts.)
 Scratch lay_out(const Ce& c, void* base) {
   Scratch s{};
   int64_t at = 0;
   auto take = [&](int64_t bytes) -> void* {
     char* p = static_cast<char*>(base) + at;
     at += (bytes + 255) / 256 * 256;
-    return base ? p : nullptr;
+    return p;
   };
   const int64_t np = round64(c.n);
   s.rows.count = static_cast<int64_t*>(take(8));
   s.rows.src = static_cast<int32_t*>(take(c.n * 4));
   s.rows.pos = static_cast<int32_t*>(take(c.n * 4));
   s.rows.labels = static_cast<int64_t*>(take(c.n * 8));
-  s.x = take(np * c.hp * dtype_size(c.t));
-  if (c.planes) s.x3 = take(np * 6 * c.hp);
+  s.x = take(np * c.hp * (c.planes ? 6 : 2));
   if (c.planes) s.w = take(round64(c.piece) * 6 * c.hp);
   else if (c.stage_w) s.w = take(c.piece * c.hp * 2);
   if (!c.backward) {
@@ -197,12 +206,12 @@ Scratch lay_out(const Ce& c, void* base) {
   } else {
     s.coef = static_cast<float4*>(take(c.n * 16));
     s.ds = take(np * ds_pitch(c, c.piece) * 2);
-    if (c.gh) s.gh = static_cast<float*>(take(c.n * round8(c.h) * 4));
+    if (c.gh && c.piece < c.v) s.gh = static_cast<float*>(take(c.n * round8(c.h) * 4));
     if (c.gw) s.xt = take(c.h * np * (c.planes ? 6 : 2));
     // a piece and the last one split differently
     const int64_t last = c.v - (c.v - 1) / c.piece * c.piece;
     for (const int64_t cols : {c.piece, last}) {
-      if (c.gh) s.split_bytes = std::max(s.split_bytes, gemm_split_bytes(grad_hidden_product(c, s, 0, cols)));
+      if (c.gh) s.split_bytes = std::max(s.split_bytes, gemm_split_bytes(grad_hidden_product(c, s, nullptr, 0, cols)));
       if (c.gw) s.split_bytes = std::max(s.split_bytes, gemm_split_bytes(grad_weight_product(c, s, nullptr, c.h, 0, cols)));
     }
     s.split = s.split_bytes > 0 ? static_cast<float*>(take(s.split_bytes)) : nullptr;
@@ -211,21 +220,31 @@ Scratch lay_out(const Ce& c, void* base) {
   return s;
 }
 
+int64_t scratch_bytes(const Ce& c) { return lay_out(c, reinterpret_cast<void*>(uintptr_t{256})).bytes; }
+
 Scratch check_scratch(const Ce& c, void* workspace, int64_t bytes) {
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) fail(ORDA_ERR_INVALID, "workspace must be 256-byte aligned");
-  const int64_t need = lay_out(c, nullptr).bytes;
-  if (bytes < need || !workspace)
+  if (!workspace) fail(ORDA_ERR_INVALID, "null workspace");
+  const Scratch s = lay_out(c, workspace);
+  if (bytes < s.bytes)
     fail(ORDA_ERR_INVALID, "workspace of %lld bytes, %lld needed", static_cast<long long>(bytes),
-         static_cast<long long>(need));
-  return lay_out(c, workspace);
+         static_cast<long long>(s.bytes));
+  return s;
 }
 
-// The compact hidden rows, and their planes.
-void gather(const Ce& c, const Scratch& s, const CeGradRows& g, hipStream_t st) {
-  hip_check(launch_ce_gather(c.t, c.x, c.ldx, c.n, c.h, s.rows, s.x, c.hp, g, st), "linear cross entropy rows");
-  if (c.planes)
-    hip_check(launch_split3_rows(static_cast<const float*>(s.x), c.hp, c.n, c.hp, s.x3, round64(c.n), c.hp, st),
-              "linear cross entropy rows");
+CePrepArgs prepare_rows(const orda_linear_ce& a, const Ce& c, const Scratch& s) {
+  CePrepArgs p{};
+  p.x = c.x;
+  p.ldx = c.ldx;
+  p.n = c.n;
+  p.h = c.h;
+  p.labels = a.labels;
+  p.v = c.v;
+  p.ignore = a.ignore_index;
+  p.rows = s.rows;
+  p.dst = s.x;
+  p.pitch = c.hp;
+  return p;
 }
 
 // The piece's weights where the products do not read them in place.
@@ -241,8 +260,10 @@ void stage_weights(const Ce& c, const Scratch& s, int64_t v0, int64_t cols, hipS
 }
 
 void forward(const orda_linear_ce& a, const Ce& c, const Scratch& s, float* nll, float* lse, hipStream_t st) {
-  hip_check(launch_ce_rows(a.labels, c.n, c.v, a.ignore_index, s.rows, nll, lse, st), "linear cross entropy rows");
-  gather(c, s, CeGradRows{}, st);
+  CePrepArgs p = prepare_rows(a, c, s);
+  p.nll = nll;
+  p.lse_out = lse;
+  hip_check(launch_ce_prep(p, c.t, c.planes, st), "linear cross entropy rows");
   for (int64_t v0 = 0; v0 < c.v; v0 += c.piece) {
     const int64_t cols = std::min(c.piece, c.v - v0);
     stage_weights(c, s, v0, cols, st);
@@ -269,19 +290,20 @@ void forward(const orda_linear_ce& a, const Ce& c, const Scratch& s, float* nll,
   }
 }
 
-void backward(const orda_linear_ce& a, const Ce& c, const Scratch& s, CeGradRows gr, orda_tensor* gh, orda_tensor* gw,
+void backward(const orda_linear_ce& a, const Ce& c, const Scratch& s, const CeGradRows& gr, orda_tensor* gh, orda_tensor* gw,
               hipStream_t st) {
-  hip_check(launch_ce_rows(a.labels, c.n, c.v, a.ignore_index, s.rows, nullptr, nullptr, st),
-            "linear cross entropy rows");
-  gr.smooth_each = a.label_smoothing / static_cast<float>(c.v);
-  gr.target = 1.f - a.label_smoothing;
-  gr.coef = s.coef;
-  gather(c, s, gr, st);
-  if (c.gw)
-    hip_check(c.planes ? launch_transpose_split3(static_cast<const float*>(s.x), c.hp, nullptr, 0, c.n, c.h, s.xt,
-                                                 round64(c.n), st)
-                       : launch_transpose_rows(s.x, c.hp, nullptr, 0, c.n, c.h, s.xt, round64(c.n), DType::BF16, st),
-              "linear cross entropy rows");
+  CePrepArgs p = prepare_rows(a, c, s);
+  p.grad = gr;
+  p.grad.smooth_each = a.label_smoothing / static_cast<float>(c.v);
+  p.grad.target = 1.f - a.label_smoothing;
+  p.grad.coef = s.coef;
+  p.trans = s.xt;
+  p.ldt = round64(c.n);
+  if (c.gh) {
+    p.zero = gh->data;
+    p.ldz = tensor_ld(*gh);
+  }
+  hip_check(launch_ce_prep(p, c.t, c.planes, st), "linear cross entropy rows");
   for (int64_t v0 = 0; v0 < c.v; v0 += c.piece) {
     const int64_t cols = std::min(c.piece, c.v - v0);
     stage_weights(c, s, v0, cols, st);
@@ -293,12 +315,9 @@ void backward(const orda_linear_ce& a, const Ce& c, const Scratch& s, CeGradRows
     g.ce.plane = round64(c.piece);
     g.ce.coef = s.coef;
     hip_check(launch_gemm(g, st), "linear cross entropy gradient");
-    if (c.gh) hip_check(launch_gemm(grad_hidden_product(c, s, v0, cols), st), "grad_hidden");
+    if (c.gh) hip_check(launch_gemm(grad_hidden_product(c, s, gh, v0, cols), st), "grad_hidden");
     if (c.gw) hip_check(launch_gemm(grad_weight_product(c, s, gw->data, tensor_ld(*gw), v0, cols), st), "grad_weight");
   }
-  if (c.gh)
-    hip_check(launch_ce_scatter(s.gh, round8(c.h), s.rows.pos, c.n, c.h, c.t, gh->data, tensor_ld(*gh), st),
-              "grad_hidden");
 }
 
 bool wanted(const orda_tensor* g) { return g != nullptr && g->data != nullptr; }
@@ -323,7 +342,7 @@ int32_t orda_linear_ce_workspace(const orda_linear_ce* args, int32_t backward, i
   return guarded(err, err_len, [&] {
     if (!args || !bytes) fail(ORDA_ERR_INVALID, "null argument");
     const Ce c = make_ce(*args, args->n_labels, backward != 0, (backward & 1) != 0, (backward & 2) != 0);
-    *bytes = c.n > 0 ? lay_out(c, nullptr).bytes : 0;
+    *bytes = c.n > 0 ? scratch_bytes(c) : 0;
   });
 }
 
@@ -354,8 +373,7 @@ int32_t orda_linear_ce_backward(int32_t device, void* hip_stream, const orda_lin
     if (c.n == 0) {   // no rows: a weight gradient of zeros
       if (!c.gw) return;
       const DeviceScope scope(device);
-      hip_check(launch_ce_scatter(nullptr, 0, nullptr, c.v, c.h, c.t, grad_weight->data, tensor_ld(*grad_weight), st),
-                "grad_weight");
+      hip_check(launch_zero_rows(c.t, grad_weight->data, tensor_ld(*grad_weight), c.v, c.h, st), "grad_weight");
       return;
     }
     if (!args->labels || !lse) fail(ORDA_ERR_INVALID, "null argument");

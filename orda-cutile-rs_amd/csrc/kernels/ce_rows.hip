@@ -9,6 +9,7 @@
 #include <math.h>
 
 #include "orda_kernels.h"
+#include "split3.h"
 
 namespace orda {
 namespace {
@@ -23,6 +24,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // wave and over the waves, then the stores. Bound by latency, a load and two
 // barriers an iteration.
 constexpr int kScanThreads = 1024, kScanPer = 8;
+constexpr int64_t kScanRows = 16384;   // up to here each workgroup of ce_prep_kernel counts for itself
 
 __global__ __launch_bounds__(kScanThreads) void ce_rows_kernel(const int64_t* labels, int64_t n, int64_t v,
                                                                int64_t ignore, CeRows r, float* nll, float* lse) {
@@ -74,39 +76,163 @@ __global__ __launch_bounds__(kScanThreads) void ce_rows_kernel(const int64_t* la
 }
 
 // ------------------------------------------------------------ hidden rows
-// A wave copies a row to its compact place: 16-byte vectors where the source
-// allows, zeros up to the pitch, and zero rows from the count up to the next
-// multiple of 64 (finite values beside the zeros of the backward products). With
-// coef, the row's CeGrad coefficients too (CeArgs::coef).
-template <typename E, bool VEC>
-__global__ __launch_bounds__(256) void ce_gather_kernel(const E* x, int64_t ldx, int64_t h, CeRows r, E* dst,
-                                                        int64_t ldd, CeGradRows g) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
-  const int64_t n = *r.count;
-  if (row >= (n + 63) / 64 * 64) return;
-  E* d = dst + row * ldd;
-  constexpr int kVec = 16 / sizeof(E);
-  const int64_t i = row < n ? r.src[row] : 0;
-  const E* s = x + i * ldx;
-  for (int64_t c = lane * kVec; c < ldd; c += 64 * kVec) {
-    alignas(16) E w[kVec] = {};
-    if (row < n) {
-      if (VEC && c + kVec <= h) {
-        *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(s + c);
-      } else {
+// A workgroup takes 64 rows of the batch and kPrepCols of their columns, and
+// writes what the products read of those that have a label, at their compact
+// places: the rows (a pitch of whole vectors, zeros past h), and for the backward
+// products the transposed rows, which pass through LDS 64 x 64 at a time. OUT 0
+// keeps the type, OUT 1 writes fp32 values as three bf16 planes (split3.h). The
+// workgroups of the last 64 rows also write the zeros up to the next multiple of 64
+// (finite values beside the zeros of the backward products), those of the first
+// columns the rows' numbers, classes, losses of ignored rows and coefficients.
+//
+// SCAN: the places are counted here, from all labels before (a batch of up to
+// kScanRows: 4 us at 8192, where a kernel of its own takes 13 and a launch), else
+// read from pos, which ce_rows_kernel has written.
+constexpr int kPrepCols = 256;
+
+template <typename E, int OUT, bool VEC, bool SCAN>
+__global__ __launch_bounds__(256) void ce_prep_kernel(CePrepArgs a) {
+  constexpr int kVec = 16 / sizeof(E), kLanes = 64 / kVec, kPass = 256 / kLanes;   // rows a pass
+  __shared__ int place[64];
+  __shared__ int sums[4];
+  __shared__ E tile[64][65];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64, first = static_cast<int64_t>(blockIdx.y) * kPrepCols;
+  const CeRows& r = a.rows;
+  const bool lead = blockIdx.y == 0, last_rows = r0 + 64 >= a.n;
+  int64_t base = 0;   // labelled rows before r0
+  if constexpr (SCAN) {
+    int mine = 0;
+    for (int64_t i = tid * 8; i < r0; i += 2048) {   // r0 is a multiple of 64
 #pragma unroll
-        for (int k = 0; k < kVec; ++k)
-          if (c + k < h) w[k] = s[c + k];
+      for (int k = 0; k < 8; ++k) mine += a.labels[i + k] != a.ignore ? 1 : 0;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) mine += __shfl_xor(mine, d);
+    if (lane == 0) sums[wave] = mine;
+    __syncthreads();
+    base = sums[0] + sums[1] + sums[2] + sums[3];
+  }
+  if (wave == 0) {
+    const int64_t i = r0 + lane;
+    const int64_t y = i < a.n ? a.labels[i] : a.ignore;
+    int p = -1;
+    if constexpr (SCAN) {
+      const uint64_t has = __ballot(y != a.ignore);
+      if (y != a.ignore) p = static_cast<int>(base) + __popcll(has & ((uint64_t{1} << lane) - 1));
+      if (lead && last_rows && lane == 0) *r.count = base + __popcll(has);
+      if (lead && i < a.n) {
+        r.pos[i] = p;
+        if (p >= 0) {
+          r.src[p] = static_cast<int32_t>(i);
+          r.labels[p] = y >= 0 && y < a.v ? y : -1;
+        } else if (a.nll != nullptr) {
+          a.nll[i] = 0.f;
+          a.lse_out[i] = 0.f;
+        }
+      }
+    } else {
+      if (i < a.n) p = r.pos[i];
+    }
+    if (lead && a.grad.coef != nullptr && p >= 0) {
+      const CeGradRows& g = a.grad;
+      const float gn = g.grad_nll != nullptr ? g.grad_nll[i] : 0.f, gl = g.grad_lse != nullptr ? g.grad_lse[i] : 0.f;
+      float4 c = make_float4(g.lse[i] * kLog2e, gn + gl, gn * g.smooth_each, gn * g.target);
+      if (y < 0 || y >= a.v) c = make_float4(NAN, NAN, NAN, NAN);   // no such class
+      g.coef[p] = c;
+    }
+    place[lane] = p;
+  }
+  __syncthreads();
+  const E* const x = static_cast<const E*>(a.x);
+  const int row_in = tid / kLanes, col_in = tid % kLanes * kVec;
+  for (int64_t c0 = first; c0 < first + kPrepCols && c0 < a.pitch; c0 += 64) {
+#pragma unroll
+    for (int q = 0; q < 64 / kPass; ++q) {
+      const int rl = q * kPass + row_in, p = place[rl];
+      const int64_t i = r0 + rl, c = c0 + col_in;
+      alignas(16) E w[kVec] = {};
+      if (p >= 0) {
+        const E* src = x + i * a.ldx + c;
+        if (VEC && c + kVec <= a.h) {
+          *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(src);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kVec; ++k)
+            if (c + k < a.h) w[k] = src[k];
+        }
+        if (a.dst != nullptr && c < a.pitch) {
+          if constexpr (OUT == 0) {
+            *reinterpret_cast<u32x4*>(static_cast<E*>(a.dst) + p * a.pitch + c) = *reinterpret_cast<const u32x4*>(w);
+          } else {
+            uint32_t lo[3], hi[3];
+            split3_pack(w[0], w[1], lo);
+            split3_pack(w[2], w[3], hi);
+            uint16_t* d = static_cast<uint16_t*>(a.dst) + 3 * p * a.pitch + c;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2*>(d + k * a.pitch) = make_uint2(lo[k], hi[k]);
+          }
+        }
+      } else if (a.zero != nullptr && i < a.n && c < a.h) {   // an ignored row's gradient
+        E* d = static_cast<E*>(a.zero) + i * a.ldz + c;
+        if (a.zero_vec && c + kVec <= a.h) {
+          *reinterpret_cast<u32x4*>(d) = u32x4{0, 0, 0, 0};
+        } else {
+#pragma unroll
+          for (int k = 0; k < kVec; ++k)
+            if (c + k < a.h) d[k] = E(0);
+        }
+      }
+      if (a.trans != nullptr) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) tile[rl][col_in + k] = w[k];
       }
     }
-    *reinterpret_cast<u32x4*>(d + c) = *reinterpret_cast<const u32x4*>(w);
+    if (a.trans == nullptr) continue;
+    __syncthreads();
+    const int p = place[lane];
+    for (int q = wave; q < 64; q += 4) {
+      const int64_t c = c0 + q;
+      if (c >= a.h || p < 0) continue;
+      const E e = tile[lane][q];
+      if constexpr (OUT == 0) {
+        static_cast<E*>(a.trans)[c * a.ldt + p] = e;
+      } else {
+        float h, m, l;
+        split3(e, h, m, l);
+        __bf16* d = static_cast<__bf16*>(a.trans) + 3 * c * a.ldt + p;
+        d[0] = static_cast<__bf16>(h);
+        d[a.ldt] = static_cast<__bf16>(m);
+        d[2 * a.ldt] = static_cast<__bf16>(l);
+      }
+    }
+    __syncthreads();
   }
-  if (g.coef != nullptr && lane == 0 && row < n) {
-    const float gn = g.grad_nll != nullptr ? g.grad_nll[i] : 0.f, gl = g.grad_lse != nullptr ? g.grad_lse[i] : 0.f;
-    float4 c = make_float4(g.lse[i] * kLog2e, gn + gl, gn * g.smooth_each, gn * g.target);
-    if (r.labels[row] < 0) c = make_float4(NAN, NAN, NAN, NAN);   // no such class
-    g.coef[row] = c;
+  if (!last_rows) return;
+  // zeros from the count up
+  const int64_t n = SCAN ? base + __popcll(__ballot(place[lane] >= 0)) : *r.count;
+  const int64_t end = a.whole ? (a.n + 63) / 64 * 64 : (n + 63) / 64 * 64;
+  constexpr int kPlanes = OUT == 0 ? 1 : 3;
+  constexpr int kOutBytes = OUT == 0 ? sizeof(E) : 2;
+  const int64_t c1 = first + kPrepCols < a.pitch ? first + kPrepCols : a.pitch;
+  if (lead && a.whole)
+    for (int64_t p = n + tid; p < end; p += 256) {
+      if (p < a.n) r.labels[p] = -1;
+      if (p < a.n && a.grad.coef != nullptr) a.grad.coef[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  for (int64_t p = n + wave; p < end; p += 4) {
+    for (int k = 0; a.dst != nullptr && k < kPlanes; ++k)
+      for (int64_t c = first + lane; c < c1; c += 64) {
+        char* d = static_cast<char*>(a.dst) + ((p * kPlanes + k) * a.pitch + c) * kOutBytes;
+        if constexpr (kOutBytes == 2) *reinterpret_cast<uint16_t*>(d) = 0;
+        else *reinterpret_cast<uint32_t*>(d) = 0;
+      }
+    for (int k = 0; a.trans != nullptr && k < kPlanes; ++k)
+      for (int64_t c = first + lane; c < c1 && c < a.h; c += 64) {
+        char* d = static_cast<char*>(a.trans) + ((c * kPlanes + k) * a.ldt + p) * kOutBytes;
+        if constexpr (kOutBytes == 2) *reinterpret_cast<uint16_t*>(d) = 0;
+        else *reinterpret_cast<uint32_t*>(d) = 0;
+      }
   }
 }
 
@@ -129,7 +255,7 @@ __global__ __launch_bounds__(256) void ce_losses_kernel(CeLossArgs a) {
   float sum = 0.f, sx = 0.f, ext = 0.f;
   for (int64_t t = lane; t < a.tiles; t += 64) {
     const float4 s = st[t];
-    sx += s.z;
+    sx += s.w;
     if (!(s.y <= FLT_MAX)) ext += s.y;
     else if (s.x != -INFINITY) sum += s.y * __builtin_amdgcn_exp2f((s.x - m) * kLog2e);
   }
@@ -158,64 +284,45 @@ __global__ __launch_bounds__(256) void ce_losses_kernel(CeLossArgs a) {
   a.nll[i] = nll;
 }
 
-// ------------------------------------------------------------ grad_hidden
-// The compact fp32 gradient rows to their places in the output's type; rows
-// without a label (with pos null: all) are zero.
-template <typename O, bool VEC>
-__global__ __launch_bounds__(256) void ce_scatter_kernel(const float* src, int64_t lds, const int32_t* pos,
-                                                         int64_t rows, int64_t h, O* dst, int64_t ldd) {
-  const int lane = threadIdx.x & 63;
+template <typename E>
+__global__ __launch_bounds__(256) void zero_rows_kernel(E* p, int64_t ld, int64_t rows, int64_t cols) {
   const int64_t row = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
   if (row >= rows) return;
-  const int64_t p = pos != nullptr ? pos[row] : -1;
-  const float* s = src + (p < 0 ? 0 : p) * lds;
-  O* d = dst + row * ldd;
-  for (int64_t c = lane * 4; c < h; c += 256) {
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if (p >= 0) x = *reinterpret_cast<const f32x4*>(s + c);   // lds is a multiple of 4, >= h
-    if (VEC && c + 4 <= h) {
-      alignas(16) O o[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = static_cast<O>(x[k]);
-      if constexpr (sizeof(O) == 4) *reinterpret_cast<u32x4*>(d + c) = *reinterpret_cast<const u32x4*>(o);
-      else *reinterpret_cast<uint64_t*>(d + c) = *reinterpret_cast<const uint64_t*>(o);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (c + k < h) d[c + k] = static_cast<O>(x[k]);
-    }
-  }
+  for (int64_t c = threadIdx.x & 63; c < cols; c += 64) p[row * ld + c] = E(0);
 }
 
 unsigned row_blocks(int64_t rows) { return static_cast<unsigned>((rows + 3) / 4); }
 
 }  // namespace
 
-hipError_t launch_ce_rows(const int64_t* labels, int64_t n, int64_t v, int64_t ignore, const CeRows& r, float* nll,
-                          float* lse, hipStream_t stream) {
-  hipLaunchKernelGGL(ce_rows_kernel, dim3(1), dim3(kScanThreads), 0, stream, labels, n, v, ignore, r, nll, lse);
-  return hipGetLastError();
-}
-
-hipError_t launch_ce_gather(DType t, const void* x, int64_t ldx, int64_t n, int64_t h, const CeRows& r, void* dst,
-                            int64_t ldd, const CeGradRows& g, hipStream_t stream) {
-  if (ldd % 8 != 0 || ldd < h || reinterpret_cast<uintptr_t>(dst) % 16 != 0) return hipErrorInvalidValue;
-  const dim3 grid(row_blocks((n + 63) / 64 * 64));
-  const bool vec = (ldx * dtype_size(t)) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  auto run = [&](auto kernel, auto* e) {
-    using E = std::remove_pointer_t<decltype(e)>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, static_cast<const E*>(x), ldx, h, r, static_cast<E*>(dst),
-                       ldd, g);
-  };
-  if (t == DType::BF16) {
-    uint16_t* e = nullptr;
-    if (vec) run(ce_gather_kernel<uint16_t, true>, e);
-    else run(ce_gather_kernel<uint16_t, false>, e);
-  } else {
-    uint32_t* e = nullptr;
-    if (vec) run(ce_gather_kernel<uint32_t, true>, e);
-    else run(ce_gather_kernel<uint32_t, false>, e);
+hipError_t launch_ce_prep(const CePrepArgs& in, DType t, bool planes, hipStream_t stream) {
+  CePrepArgs a = in;
+  if (a.n <= 0) return hipSuccess;
+  if (a.pitch % 8 != 0 || a.pitch < a.h || (planes && t != DType::F32)) return hipErrorInvalidValue;
+  if (reinterpret_cast<uintptr_t>(a.dst) % 16 != 0 || reinterpret_cast<uintptr_t>(a.trans) % 16 != 0)
+    return hipErrorInvalidValue;
+  const int64_t es = dtype_size(t);
+  const bool vec = (a.ldx * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
+  a.zero_vec = (a.ldz * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.zero) % 16 == 0;
+  const bool scan = a.n <= kScanRows;
+  if (!scan) {
+    hipLaunchKernelGGL(ce_rows_kernel, dim3(1), dim3(kScanThreads), 0, stream, a.labels, a.n, a.v, a.ignore, a.rows, a.nll,
+                       a.lse_out);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
+  const dim3 grid(static_cast<unsigned>((a.n + 63) / 64), static_cast<unsigned>((a.pitch + kPrepCols - 1) / kPrepCols));
+  using K = void (*)(CePrepArgs);
+  auto pick = [&](auto e, auto out_c) -> K {
+    using E = decltype(e);
+    constexpr int kOut = decltype(out_c)::value;
+    if (scan) return vec ? ce_prep_kernel<E, kOut, true, true> : ce_prep_kernel<E, kOut, false, true>;
+    return vec ? ce_prep_kernel<E, kOut, true, false> : ce_prep_kernel<E, kOut, false, false>;
+  };
+  const K k = t == DType::BF16 ? pick(uint16_t{}, std::integral_constant<int, 0>{})
+              : planes         ? pick(float{}, std::integral_constant<int, 1>{})
+                               : pick(float{}, std::integral_constant<int, 0>{});
+  hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -224,21 +331,11 @@ hipError_t launch_ce_losses(const CeLossArgs& a, int64_t n, hipStream_t stream) 
   return hipGetLastError();
 }
 
-hipError_t launch_ce_scatter(const float* src, int64_t lds, const int32_t* pos, int64_t rows, int64_t h, DType t,
-                             void* dst, int64_t ldd, hipStream_t stream) {
-  if (lds % 4 != 0 || reinterpret_cast<uintptr_t>(src) % 16 != 0) return hipErrorInvalidValue;
-  const int64_t align = 4 * dtype_size(t);
-  const bool vec = (ldd * dtype_size(t)) % align == 0 && reinterpret_cast<uintptr_t>(dst) % align == 0;
-  const dim3 grid(row_blocks(rows));
-  if (t == DType::BF16) {
-    auto* d = static_cast<__bf16*>(dst);
-    if (vec) hipLaunchKernelGGL((ce_scatter_kernel<__bf16, true>), grid, dim3(256), 0, stream, src, lds, pos, rows, h, d, ldd);
-    else hipLaunchKernelGGL((ce_scatter_kernel<__bf16, false>), grid, dim3(256), 0, stream, src, lds, pos, rows, h, d, ldd);
-  } else {
-    auto* d = static_cast<float*>(dst);
-    if (vec) hipLaunchKernelGGL((ce_scatter_kernel<float, true>), grid, dim3(256), 0, stream, src, lds, pos, rows, h, d, ldd);
-    else hipLaunchKernelGGL((ce_scatter_kernel<float, false>), grid, dim3(256), 0, stream, src, lds, pos, rows, h, d, ldd);
-  }
+hipError_t launch_zero_rows(DType t, void* p, int64_t ld, int64_t rows, int64_t cols, hipStream_t stream) {
+  if (t == DType::BF16)
+    hipLaunchKernelGGL(zero_rows_kernel<uint16_t>, dim3(row_blocks(rows)), dim3(256), 0, stream, static_cast<uint16_t*>(p), ld, rows, cols);
+  else
+    hipLaunchKernelGGL(zero_rows_kernel<uint32_t>, dim3(row_blocks(rows)), dim3(256), 0, stream, static_cast<uint32_t*>(p), ld, rows, cols);
   return hipGetLastError();
 }
 

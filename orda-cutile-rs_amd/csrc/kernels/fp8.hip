@@ -170,13 +170,6 @@ constexpr int kOp = kTile * 128;                      // an operand's stage
 constexpr int kScales = kTile * 4 + 64;               // A's row scales, B's two
 constexpr int kStage = 2 * kOp;
 
-__device__ __forceinline__ void dma4(uint64_t sbase, uint32_t voff, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %0"
-               :
-               : "s"(sbase), "v"(voff), "s"(m0)
-               : "memory", "m0");
-}
-
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};

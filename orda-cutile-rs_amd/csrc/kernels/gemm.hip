@@ -506,6 +506,42 @@ constexpr int plane_set(int i, bool a) {
 }
 static_assert(plane_set(11, true) == 1 && plane_set(11, false) == 1, "stage 12 is stage 0's set again");
 
+// Products over dyn_rows rows that are not transposed (grad_hidden of the linear
+// cross entropy): how many tiles there are only the device knows, and with it how
+// far the last round of 256 workgroups is filled. So the tiles of whole rounds run
+// as they are, and the rest with K split into `splits` parts of `len`, by the cost
+// plan_split uses: at 8192 x 4096 x 131072 with 40 % of the rows ignored, 320
+// tiles a piece, the product takes 1.25 rounds instead of two. The launch has a
+// workgroup for the most that any count up to M needs; each computes this from
+// the count and the ones left over return.
+constexpr int64_t kStageNs = 700, kStageNsP3 = 4200;     // 32 elements of K, as stage_us
+constexpr int64_t kDynRoundNs = 8000, kDynPartNs = 130;  // a round's fixed cost; a partial tile written and read
+constexpr int64_t kDynTailBlocks = 1024;                 // most workgroups of the last, split rounds
+struct DynPlan {
+  int64_t whole, tail, splits, len;
+};
+// (whole numbers: the host's and the device's plans are the same)
+__host__ __device__ inline DynPlan dyn_plan(int64_t tiles, int64_t K, int64_t stage_ns) {
+  DynPlan p{tiles / 256 * 256, tiles % 256, 1, K};
+  if (p.tail == 0) return p;
+  int64_t best = K * stage_ns / 32 + kDynRoundNs;
+  for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+    int64_t s = 256 * rounds / p.tail;
+    if (s > K / 128) s = K / 128;
+    if (s > 128) s = 128;
+    if (s < 2) continue;
+    const int64_t len = ((K + s - 1) / s + 63) / 64 * 64, n = (K + len - 1) / len;
+    if (n < 2 || n * p.tail > kDynTailBlocks) continue;
+    const int64_t ns = (p.tail * n + 255) / 256 * (len * stage_ns / 32 + kDynRoundNs) + kDynPartNs * n * p.tail + 3000;
+    if (ns < best) {
+      best = ns;
+      p.splits = n;
+      p.len = len;
+    }
+  }
+  return p;
+}
+
 struct TileCoord {
   int p, m0, n0, ntile;
 };
@@ -1234,7 +1270,7 @@ __device__ __forceinline__ void ce_epilogue(const GemmArgs& g, int64_t M, const 
           }
         d1 = quad_sum(d1);
         sx = quad_sum(sx);
-        if (lgrp == 0) rows4[wn * TM + rl] = make_float4(mx == -INFINITY ? mx : ref, d1, sx, 0.f);
+        if (lgrp == 0) rows4[wn * TM + rl] = make_float4(mx == -INFINITY ? mx : ref, d1, 0.f, sx);
         if (yl >= 0 && yl < 128 && (yl & 12) == 0 && row < M) {   // one lane of a row at most
           const int jy = yl >> 4, ey = yl & 3;
           float xy = 0.f;
@@ -1256,7 +1292,7 @@ __device__ __forceinline__ void ce_epilogue(const GemmArgs& g, int64_t M, const 
     if ((TM == kThreads || tid < TM) && tc.m0 + tid < M) {
       const float4 a = rows4[tid], b = rows4[TM + tid];
       const float m = fmaxf(a.x, b.x);
-      float4 s = make_float4(m, 0.f, a.z + b.z, 0.f);
+      float4 s = make_float4(m, 0.f, 0.f, a.w + b.w);
       if (a.x != -INFINITY) s.y += a.y * __builtin_amdgcn_exp2f((a.x - m) * kLog2e);
       if (b.x != -INFINITY) s.y += b.y * __builtin_amdgcn_exp2f((b.x - m) * kLog2e);
       // an infinite or NaN sum stays one, whatever it is scaled by
@@ -1332,6 +1368,53 @@ __device__ __forceinline__ void ce_epilogue(const GemmArgs& g, int64_t M, const 
   }
 }
 
+// One element of a product over compact rows: to C, or to its row's place in
+// out (CeArgs::accum, out).
+__device__ __forceinline__ void put_dyn(const GemmArgs& g, float* C, int64_t row, int64_t src, int64_t col, float v) {
+  if (g.ce.accum) v += C[row * g.ldc + col];
+  if (g.ce.out == nullptr) C[row * g.ldc + col] = v;
+  else if (g.ce.out_type == DType::BF16) static_cast<__bf16*>(g.ce.out)[src * g.ce.ldo + col] = static_cast<__bf16>(v);
+  else static_cast<float*>(g.ce.out)[src * g.ce.ldo + col] = v;
+}
+
+// The epilogue of a tile of such a product: element (row wm·128 + 16i + 4·lgrp + e,
+// column wn·128 + 16j + lrow) by put_dyn, or a part of a split tile, as it is, to
+// the 256 x 256 floats at part.
+__device__ __forceinline__ void rows_epilogue(const GemmArgs& g, int64_t M, const GemmProblem& pr, const TileCoord& tc,
+                                              f32x4 (&acc)[kFrag][kFrag], float* part) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row_l = (wave >> 1) * 128 + (lane >> 4) * 4, col_l = (wave & 1) * 128 + (lane & 15);
+  if (part != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kFrag; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < kFrag; ++j) part[(row_l + i * 16 + e) * kTile + col_l + j * 16] = acc[i][j][e];
+    return;
+  }
+  float* const C = static_cast<float*>(pr.c);
+#pragma unroll
+  for (int i = 0; i < kFrag; ++i) {
+    f32x4 av[kFrag];
+#pragma unroll
+    for (int j = 0; j < kFrag; ++j) av[j] = from_acc(acc[i][j]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t row = static_cast<int64_t>(tc.m0) + row_l + i * 16 + e;
+      if (row >= M) continue;
+      const int64_t src = g.ce.out != nullptr ? g.ce.src[row] : 0;
+#pragma unroll
+      for (int j = 0; j < kFrag; ++j) {
+        const int64_t col = static_cast<int64_t>(tc.n0) + col_l + j * 16;
+        if (col < g.N) put_dyn(g, C, row, src, col, av[j][e]);
+      }
+      __builtin_amdgcn_sched_barrier(0);   // not all rows' addresses at once
+    }
+  }
+}
+
 template <typename T, bool AK, bool BK, GemmEpilogue EPI, typename LT, bool CT, bool P3 = false, bool DYN = false>
 __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
   static_assert(!P3 || Elem<T>::kSize == 2, "three-plane operands are bf16");
@@ -1366,22 +1449,38 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
   }
   int64_t lin = blockIdx.x, kbeg = 0, Kl = K;
   int split = 0;
-  if (g.split_k > 1) {
+  if ((!DYN || CT) && g.split_k > 1) {
     split = static_cast<int>(lin / tiles);
     lin -= static_cast<int64_t>(split) * tiles;
     kbeg = static_cast<int64_t>(split) * g.split_len;
     Kl = K - kbeg < g.split_len ? K - kbeg : g.split_len;
   }
-  if constexpr (DYN) {
-    if constexpr (CT) {
-      if (Kl < 0) Kl = 0;   // a part past the rows: zeros
+  float* part = nullptr;   // where a part of a split tile goes
+  if constexpr (DYN && CT) {
+    if (Kl < 0) Kl = 0;   // a part past the rows: zeros
+  } else if constexpr (DYN) {
+    const int64_t all = (M + kTile - 1) / kTile * ((g.N + kTile - 1) / kTile);
+    if constexpr (kCeEpi) {
+      if (lin >= all) return;
     } else {
-      if (lin >= (M + kTile - 1) / kTile * ((g.N + kTile - 1) / kTile)) return;
+      const DynPlan d = dyn_plan(all, K, P3 ? kStageNsP3 : kStageNs);
+      if (lin >= d.whole + d.tail * d.splits) return;
+      if (lin >= d.whole && d.splits > 1) {
+        const int64_t at = lin - d.whole;
+        part = g.split_ws + at * (kTile * kTile);
+        lin = d.whole + at % d.tail;
+        kbeg = at / d.tail * d.len;
+        Kl = K - kbeg < d.len ? K - kbeg : d.len;
+      }
     }
   }
   const TileCoord tc = map_tile(g, M, lin);
   GemmProblem pr = g.prob[tc.p];
-  if (g.split_k > 1) {
+  if constexpr (DYN && !CT && !kCeEpi) {
+    constexpr int ES = Elem<T>::kSize;
+    pr.a = static_cast<const unsigned char*>(pr.a) + kbeg * ES;
+    pr.b = static_cast<const unsigned char*>(pr.b) + kbeg * g.ldb * ES;
+  } else if (g.split_k > 1) {
     constexpr int ES = Elem<T>::kSize;
     pr.a = static_cast<const unsigned char*>(pr.a) + kbeg * (AK ? 1 : g.lda) * ES;
     pr.b = static_cast<const unsigned char*>(pr.b) + kbeg * (BK ? 1 : g.ldb) * ES;
@@ -2006,6 +2105,7 @@ __device__ __forceinline__ void gemm_body(const GemmArgs& g) {
   __builtin_amdgcn_s_barrier();
 
   if constexpr (kCeEpi) ce_epilogue<EPI, kFrag, P3>(g, M, pr, tc, acc, epi, lab_pre, coef_pre);
+  else if constexpr (DYN && !CT) rows_epilogue(g, M, pr, tc, acc, part);
   else gemm_epilogue<Elem<T>::kSize, EPI, LT, CT, kFrag>(g, M, pr, tc, acc, epi, smem, lab_pre);
 }
 
@@ -2200,13 +2300,11 @@ ORDA_MID(gemm_kmt_mid_accum_bf16, false, GemmEpilogue::AccumF32, float, true)
 ORDA_CE(gemm_kk_cestats_bf16, true, GemmEpilogue::CeStats, float, false, false)
 ORDA_CE(gemm_kk_cegrad_bf16, true, GemmEpilogue::CeGrad, __bf16, false, false)
 ORDA_CE(gemm_km_dyn_store_bf16, false, GemmEpilogue::StoreF32, float, false, false)
-ORDA_CE(gemm_km_dyn_accum_bf16, false, GemmEpilogue::AccumF32, float, false, false)
 ORDA_CE(gemm_kmt_dyn_store_bf16, false, GemmEpilogue::StoreF32, float, true, false)
 ORDA_CE(gemm_kmt_dyn_store_bf16_bf16, false, GemmEpilogue::StoreF32, __bf16, true, false)
 ORDA_CE(gemm_kk_cestats_bf16x3, true, GemmEpilogue::CeStats, float, false, true)
 ORDA_CE(gemm_kk_cegrad_bf16x3, true, GemmEpilogue::CeGrad, float, false, true)
 ORDA_CE(gemm_km_dyn_store_bf16x3, false, GemmEpilogue::StoreF32, float, false, true)
-ORDA_CE(gemm_km_dyn_accum_bf16x3, false, GemmEpilogue::AccumF32, float, false, true)
 ORDA_CE(gemm_kmt_dyn_store_bf16x3, false, GemmEpilogue::StoreF32, float, true, true)
 #undef ORDA_CE
 #define ORDA_CE_MID(NAME, BK, EPI, LT, CT) \
@@ -2228,12 +2326,8 @@ GemmKernel select_dyn(const GemmArgs& g, bool mid) {
     return p3 ? gemm_kk_cegrad_bf16x3 : mid ? gemm_kk_mid_cegrad_bf16 : gemm_kk_cegrad_bf16;
   }
   if (g.b_kmajor) return nullptr;
-  if (!g.c_trans) {
-    if (g.epi != E::StoreF32 && g.epi != E::AccumF32) return nullptr;
-    if (p3) return st ? gemm_km_dyn_store_bf16x3 : gemm_km_dyn_accum_bf16x3;
-    return st ? gemm_km_dyn_store_bf16 : gemm_km_dyn_accum_bf16;
-  }
   if (!st) return nullptr;
+  if (!g.c_trans) return p3 ? gemm_km_dyn_store_bf16x3 : gemm_km_dyn_store_bf16;
   if (p3) return g.c_type == DType::F32 ? gemm_kmt_dyn_store_bf16x3 : nullptr;
   if (g.c_type == DType::F32) return gemm_kmt_dyn_store_bf16;
   return mid ? gemm_kmt_mid_dyn_store_bf16_bf16 : gemm_kmt_dyn_store_bf16_bf16;
@@ -2320,6 +2414,30 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(
       for (int k = 0; k < 4 && q + k < cols; ++k) dst[k] = accum ? alpha * (dst[k] + v[k]) : alpha * v[k];
     }
   }
+}
+
+// The split tiles of a product over dyn_rows rows: their parts added in order, four
+// columns a thread, 64 workgroups a tile.
+template <bool P3>
+__global__ __launch_bounds__(256) void gemm_dyn_join_kernel(GemmArgs g) {
+  const int64_t M = *g.dyn_rows;
+  const int64_t all = (M + kTile - 1) / kTile * ((g.N + kTile - 1) / kTile);
+  const DynPlan d = dyn_plan(all, g.K, P3 ? kStageNsP3 : kStageNs);
+  const int64_t t = blockIdx.x >> 6;
+  if (d.splits < 2 || t >= d.tail) return;
+  const TileCoord tc = map_tile(g, M, d.whole + t);
+  const int q = (blockIdx.x & 63) * 256 + threadIdx.x;   // four of the tile's columns
+  const int64_t row = tc.m0 + (q >> 6), col = tc.n0 + (q & 63) * 4;
+  if (row >= M || col >= g.N) return;
+  const f32x4* src = reinterpret_cast<const f32x4*>(g.split_ws + t * (kTile * kTile)) + q;
+  const int64_t step = d.tail * (kTile * kTile / 4);
+  f32x4 v = src[0];
+#pragma unroll 4
+  for (int64_t s = 1; s < d.splits; ++s) v += src[s * step];
+  const int64_t to = g.ce.out != nullptr ? g.ce.src[row] : 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (col + e < g.N) put_dyn(g, static_cast<float*>(g.prob[0].c), row, to, col + e, v[e]);
 }
 
 // Transposed staging (launch_transpose_rows): a 64 x 64 block of source
@@ -2434,6 +2552,26 @@ __global__ __launch_bounds__(256) void transpose_split3_kernel(const float* a, i
   }
 }
 
+// What launches of a product over dyn_rows rows must provide for: the most
+// workgroups, and split tiles, of any count up to M.
+struct DynMost {
+  int64_t blocks, tail, parts;
+};
+bool dyn_rows_product(const GemmArgs& g) {
+  return g.dyn_rows != nullptr && !g.c_trans && g.epi == GemmEpilogue::StoreF32;
+}
+DynMost dyn_most(const GemmArgs& g) {
+  DynMost m{0, 0, 0};
+  const int64_t nt = (g.N + kTile - 1) / kTile;
+  for (int64_t mt = (g.M + kTile - 1) / kTile; mt > 0; --mt) {
+    const DynPlan d = dyn_plan(mt * nt, g.K, g.plane_a > 0 ? kStageNsP3 : kStageNs);
+    m.blocks = d.whole + d.tail * d.splits > m.blocks ? d.whole + d.tail * d.splits : m.blocks;
+    if (d.splits > 1 && d.tail > m.tail) m.tail = d.tail;
+    if (d.splits > 1 && d.tail * d.splits > m.parts) m.parts = d.tail * d.splits;
+  }
+  return m;
+}
+
 struct SplitPlan {
   int splits;
   int64_t len, ldp, stride, bytes;
@@ -2530,7 +2668,7 @@ int64_t tile_count(const GemmArgs& g) {
 // against 594.)
 SplitPlan plan_split(const GemmArgs& g) {
   SplitPlan sp{1, g.K, 0, 0, 0, 0.0};
-  if (logits_epilogue(g) || g.M <= 0 || g.N <= 0 || g.K <= 0) return sp;
+  if (dyn_rows_product(g) || logits_epilogue(g) || g.M <= 0 || g.N <= 0 || g.K <= 0) return sp;
   const int64_t tiles = tile_count(g);
   const int64_t per_split = g.nprob * (g.c_trans ? g.N * ((g.M + 3) / 4 * 4) : g.M * ((g.N + 3) / 4 * 4)) * 4;
   int64_t most = tiles < 192 ? (256 + tiles - 1) / tiles : 8;
@@ -3015,7 +3153,7 @@ struct TailSplit {
 };
 TailSplit plan_tail(const GemmArgs& g) {
   const TailSplit none{0, false};
-  if (logits_epilogue(g) || g.split_k > 1 || g.M <= 0 || g.N <= 0) return none;
+  if (dyn_rows_product(g) || logits_epilogue(g) || g.split_k > 1 || g.M <= 0 || g.N <= 0) return none;
   const int64_t Mt = (g.M + kTile - 1) / kTile, Nt = (g.N + kTile - 1) / kTile;
   const int64_t Mv = Mt * g.nprob;
   const int64_t T = Mv * Nt, q = T / 256, r = T % 256;
@@ -3028,7 +3166,7 @@ TailSplit plan_tail(const GemmArgs& g) {
   };
   const int64_t n0 = 256 * q / Mv * kTile;
   if (n0 > 0 && n0 < g.N && pays(sub_product(g, 0, g.M, n0, g.N))) return {n0, true};
-  if ((256 * q) % (Nt * g.nprob) == 0 && (g.dyn_rows == nullptr || g.c_trans)) {
+  if ((256 * q) % (Nt * g.nprob) == 0) {
     const int64_t m0 = 256 * q / (Nt * g.nprob) * kTile;
     if (m0 < g.M && pays(sub_product(g, m0, g.M, 0, g.N))) return {m0, false};
   }
@@ -3054,6 +3192,7 @@ GemmSplit gemm_split_plan(const GemmArgs& g) {
 }
 
 int64_t gemm_split_bytes(const GemmArgs& g) {
+  if (dyn_rows_product(g)) return dyn_most(g).parts * (kTile * kTile * 4);
   if (small_f32(g)) {
     const SplitPlan sp = plan_split_small(g);
     return sp.splits > 1 ? sp.bytes : 0;
@@ -3143,6 +3282,22 @@ hipError_t launch_gemm_impl(const GemmArgs& g, hipStream_t stream, bool whole) {
       if (e != hipSuccess) return e;
       return launch_gemm_impl(tail_part(g, ts, true), stream, false);
     }
+  }
+  if (dyn_rows_product(g)) {
+    const DynMost most = dyn_most(g);
+    if (most.parts > 0 && (g.split_ws == nullptr || g.split_ws_bytes < most.parts * (kTile * kTile * 4)))
+      return hipErrorInvalidValue;
+    GemmArgs d = g;
+    d.split_k = 1;
+    set_share_blocks(d);
+    const GemmKernel k = select_kernel(d, false);
+    if (k == nullptr) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(most.blocks)), dim3(kThreads), 0, stream, d);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || most.tail == 0) return e;
+    auto* join = d.plane_a > 0 ? gemm_dyn_join_kernel<true> : gemm_dyn_join_kernel<false>;
+    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(most.tail * 64)), dim3(256), 0, stream, d);
+    return hipGetLastError();
   }
   const bool mid = whole && mid_tiles(g);
   const int64_t tiles = mid ? ((g.M + kMidM - 1) / kMidM) * ((g.N + kTile - 1) / kTile) * g.nprob

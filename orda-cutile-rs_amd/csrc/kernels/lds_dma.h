@@ -49,6 +49,13 @@ __device__ __forceinline__ void dma16_at(uint64_t sbase, uint32_t voff, uint32_t
                : "s"(sbase), "v"(voff), "s"(m0base), "n"(IMM)
                : "memory", "m0", "scc");
 }
+// 4 bytes a lane, to M0 + 4 * lane.
+__device__ __forceinline__ void dma4(uint64_t sbase, uint32_t voff, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %0"
+               :
+               : "s"(sbase), "v"(voff), "s"(m0)
+               : "memory", "m0");
+}
 #pragma clang diagnostic pop
 // A wave-uniform 64-bit value in an SGPR pair.
 __device__ __forceinline__ uint64_t uniform64(const void* p) {

@@ -93,7 +93,7 @@ struct LogitStatsArgs {
 // The CeStats and CeGrad epilogues (one problem, bf16 operands, K-major both):
 // columns 0..N of the product are vocabulary columns col0..col0+N.
 struct CeArgs {
-  // CeStats: stats[m*stats_ld + n_tile] = {max, Σe^(x-max), Σx, 0} (max -inf
+  // CeStats: stats[m*stats_ld + n_tile] = {max, Σe^(x-max), 0, Σx} (max -inf
   // and sum 0 where every logit is -inf; max 0 where the maximum is +inf)
   float4* stats;
   int64_t stats_ld;       // in float4 units, >= ceil(N/256)
@@ -105,6 +105,14 @@ struct CeArgs {
   // three-plane rows, ldc elements apart, the planes `plane` elements apart.
   const float4* coef;
   int64_t plane;
+  // Store of a product over dyn_rows rows that is not transposed: with accum the
+  // old C is added; with out, row m goes to row src[m] of out (out_type, pitch
+  // ldo) instead of C.
+  bool accum;
+  const int32_t* src;
+  void* out;
+  int64_t ldo;
+  DType out_type;
 };
 
 struct GemmArgs {
@@ -155,10 +163,10 @@ struct GemmArgs {
   bool fp32_mfma;
   // Store with c_trans and bf16 operands: C's type (partials stay fp32).
   DType c_type;
-  // When set (bf16 operands, one problem; CeStats, CeGrad, Store and Accum
-  // only), the number of rows is *dyn_rows, at most the M that is passed
-  // (c_trans: at most K). Tiles past it return at once. c_trans: A is finite up
-  // to the multiple of 8 at *dyn_rows.
+  // When set (bf16 operands, one problem; CeStats, CeGrad and Store only), the
+  // number of rows is *dyn_rows, at most the M that is passed (c_trans: at most
+  // K). Tiles past it return at once. c_trans: A is finite up to the multiple of 8
+  // at *dyn_rows. Not transposed: split_ws of gemm_split_bytes bytes is needed.
   const int64_t* dyn_rows;
   CeArgs ce;
 };
@@ -418,9 +426,6 @@ struct CeRows {
   int64_t* labels;
   int32_t* pos;
 };
-// Fills r from n labels; with nll, also zeroes nll and lse of the ignored rows.
-hipError_t launch_ce_rows(const int64_t* labels, int64_t n, int64_t v, int64_t ignore, const CeRows& r, float* nll,
-                          float* lse, hipStream_t stream);
 // The gradients into the losses and log-sum-exps of all rows (each may be
 // null: 0) and the compact rows' coefficients made of them (null: none).
 struct CeGradRows {
@@ -428,11 +433,32 @@ struct CeGradRows {
   float smooth_each, target;   // label_smoothing / V, 1 - label_smoothing
   float4* coef;
 };
-// Hidden rows [n][h] to compact rows of pitch ldd (a multiple of 8), zeros past
-// h and in the rows from the count to the next multiple of 64 (dst holds
-// round64(n) rows).
-hipError_t launch_ce_gather(DType t, const void* x, int64_t ldx, int64_t n, int64_t h, const CeRows& r, void* dst,
-                            int64_t ldd, const CeGradRows& g, hipStream_t stream);
+// Fills rows from n labels and gathers the hidden rows x [n][h] that have one:
+// dst, compact rows of `pitch` elements (a multiple of 8, zeros past h), and trans,
+// their transpose [h][ldt], either of which may be null; with planes (fp32) as
+// three-plane rows (GemmArgs::plane_a) of planes of pitch and ldt elements. Rows
+// from the count to the next multiple of 64 are zeros (dst holds round64(n) rows,
+// ldt is at least that); with whole, all rows up to round64(n), and their labels
+// are -1 and coefficients 0 (products over n rows). Ignored rows: nll and lse_out
+// (null: none) are zeroed, and the rows of zero (x's type, null: none).
+struct CePrepArgs {
+  const void* x;
+  int64_t ldx, n, h;
+  const int64_t* labels;
+  int64_t v, ignore;
+  CeRows rows;
+  float *nll, *lse_out;
+  CeGradRows grad;
+  void* dst;
+  int64_t pitch;
+  void* trans;
+  int64_t ldt;
+  void* zero;
+  int64_t ldz;
+  bool whole;
+  bool zero_vec;   // set by launch_ce_prep
+};
+hipError_t launch_ce_prep(const CePrepArgs& a, DType t, bool planes, hipStream_t stream);
 // Merges a piece's tile statistics (CeArgs::stats) into state (between
 // pieces) and on the last piece writes the rows' losses.
 struct CeLossArgs {
@@ -446,9 +472,8 @@ struct CeLossArgs {
   float *nll, *lse;
 };
 hipError_t launch_ce_losses(const CeLossArgs& a, int64_t n, hipStream_t stream);
-// dst[r] = src[pos[r]] in type t, or zeros where pos[r] < 0 (pos null: everywhere).
-hipError_t launch_ce_scatter(const float* src, int64_t lds, const int32_t* pos, int64_t rows, int64_t h, DType t,
-                             void* dst, int64_t ldd, hipStream_t stream);
+// Zeros a matrix.
+hipError_t launch_zero_rows(DType t, void* p, int64_t ld, int64_t rows, int64_t cols, hipStream_t stream);
 
 // ---------------------------------------------------------------- embedding
 // out[t] = scale * w[ids[t]] in the weight's type, rounded once; NaN where the id

@@ -24,9 +24,15 @@ from . import _lib as L
 from .types import OrdaError
 
 
+_module = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _module
+    if _module is None:
+        import torch
+        _module = torch
+    return _module
 
 
 def _gpu_tensor(x, what: str):
@@ -36,7 +42,7 @@ def _gpu_tensor(x, what: str):
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise OrdaError(f"{what} must be a GPU tensor")
     try:
-        plain = type(x) in (torch.Tensor, torch.nn.Parameter) and (x.numel() == 0 or x.data_ptr() != 0)
+        plain = type(x) in (torch.Tensor, torch.nn.Parameter) and (x.data_ptr() != 0 or x.numel() == 0)
     except RuntimeError:
         plain = False
     if not plain or x.layout != torch.strided or x.is_neg():
@@ -55,9 +61,10 @@ def _matrix(x, what: str):
     copy where it is none)."""
     if x.dim() != 2:
         raise OrdaError(f"{what} must be 2-D")
-    if (x.size(1) > 1 and x.stride(1) != 1) or (x.size(0) > 1 and x.stride(0) < x.size(1)):
-        x = x.contiguous()
-    return x
+    if x.is_contiguous():
+        return x
+    (r, c), (sr, sc) = x.shape, x.stride()
+    return x.contiguous() if (c > 1 and sc != 1) or (r > 1 and sr < c) else x
 
 
 def _overlap(a, b) -> bool:
@@ -84,9 +91,8 @@ def _dtype(x, what: str) -> int:
 
 def _desc(x, what: str) -> L.Tensor:
     """orda_tensor of a _matrix."""
-    return L.Tensor(data=x.data_ptr(), rows=x.size(0), cols=x.size(1),
-                    ld=x.stride(0) if x.size(0) > 1 else x.size(1), dtype=_dtype(x, what),
-                    location=L.DEVICE)
+    r, c = x.shape
+    return L.Tensor(x.data_ptr(), r, c, x.stride(0) if r > 1 else c, _dtype(x, what), L.DEVICE)
 
 
 def _call(fn, *args):
@@ -97,7 +103,8 @@ def _call(fn, *args):
 
 
 def _stream(device):
-    return _torch().cuda.current_stream(device).cuda_stream
+    """The handle of torch's current stream (a Stream object costs 2 us more)."""
+    return _torch()._C._cuda_getCurrentRawStream(device.index)
 
 
 def _bytes(n: int, device):
@@ -116,7 +123,8 @@ def _ce_args(hidden, weight, labels, ignore_index, label_smoothing, vocab_piece)
     if y.dtype not in (torch.int64, torch.int32):
         raise OrdaError(f"labels must be int64 or int32, got {y.dtype}")
     _same_device(h.device, weight=w, labels=y)
-    y = y.to(torch.int64).contiguous()
+    if y.dtype != torch.int64 or not y.is_contiguous():
+        y = y.to(torch.int64).contiguous()
     if vocab_piece is not None and vocab_piece < 1:
         raise OrdaError("vocab_piece must be >= 1")
     a = L.LinearCeC(hidden=_desc(h, "hidden"), weight=_desc(w, "weight"), labels=y.data_ptr(),
@@ -208,7 +216,7 @@ def _ids(ids, device, what: str = "ids"):
     if ids.dtype not in (torch.int64, torch.int32):
         raise OrdaError(f"{what} must be int64 or int32, got {ids.dtype}")
     _same_device(device, **{what: ids})
-    return ids.reshape(-1).contiguous()
+    return ids if ids.dim() == 1 and ids.is_contiguous() else ids.reshape(-1).contiguous()
 
 
 def embedding(ids, weight, *, scale: float = 1.0):
@@ -223,7 +231,7 @@ def embedding(ids, weight, *, scale: float = 1.0):
     out = torch.empty((i.numel(), w.size(1)), dtype=w.dtype, device=w.device)
     _call(L.load().orda_embedding, w.device.index, _stream(w.device), i.data_ptr(), i.element_size(),
           i.numel(), C.byref(wd), scale, C.byref(_desc(out, "out")))
-    return out.view(*ids.shape, w.size(1))
+    return out if ids.dim() == 1 else out.view(*ids.shape, w.size(1))
 
 
 def embedding_backward(grad, ids, num_rows: int, *, scale: float = 1.0,

@@ -62,6 +62,14 @@ def test_pieces_of_the_vocabulary(dtype, piece):
     check(*inputs(300, 200, 5001, dtype, seed=2, ignored=0.2), label_smoothing=0.05, vocab_piece=piece)
 
 
+@pytest.mark.parametrize("n, h, v, ignored", [(5000, 4096, 600, 0.1), (5000, 4096, 600, 0.4), (17000, 40, 300, 0.3),
+                                              (16384, 24, 70, 0.02), (8200, 1032, 500, 0.0)])
+def test_many_rows(n, h, v, ignored):
+    """Whole rounds of tiles with a split tail, and more rows than a workgroup
+    counts for itself."""
+    check(*inputs(n, h, v, "bf16", seed=4, ignored=ignored), vocab_piece=256)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_no_row_left(dtype):
     x, w, y, gn, gl = inputs(70, 48, 300, dtype)

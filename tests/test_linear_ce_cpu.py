@@ -86,6 +86,29 @@ def test_scratch_follows_the_piece():
     assert workspace(args(n=0, **{"hidden.data": None}))[:2] == (L.ORDA_OK, 0)
 
 
+@pytest.mark.parametrize("n, h, v, piece", [(1, 1, 1, 0), (100, 33, 1000, 0), (64, 64, 300, 256), (5000, 4096, 600, 256),
+                                            (4915, 4096, 131072, 65536), (700, 520, 50257, 0), (17000, 40, 300, 0)])
+@pytest.mark.parametrize("dtype", [L.BF16, L.F32])
+def test_the_scratch_asked_for_is_the_scratch_laid_out(n, h, v, piece, dtype):
+    """A call with exactly the bytes that were asked for gets past the check of
+    the layout it will use (and ends at a device that does not exist); with 256
+    fewer it does not."""
+    a = args(n=n, h=h, v=v, vocab_piece=piece, **{"hidden.dtype": dtype, "weight.dtype": dtype})
+    lib, err = L.load(), C.create_string_buffer(512)
+    need = workspace(a)[1]
+    for less, want in ((0, L.ORDA_ERR_HIP), (256, L.ORDA_ERR_INVALID)):
+        assert lib.orda_linear_ce_forward(9999, None, C.byref(a), 256, 256, 256, need - less, err, 512) == want
+    gh = L.Tensor(data=256, rows=n, cols=h, dtype=dtype, location=L.DEVICE)
+    gw = L.Tensor(data=256, rows=v, cols=h, dtype=dtype, location=L.DEVICE)
+    for which, out in ((1, (gh, None)), (2, (None, gw)), (3, (gh, gw))):
+        need = workspace(a, which)[1]
+        for less, want in ((0, L.ORDA_ERR_HIP), (256, L.ORDA_ERR_INVALID)):
+            rc = lib.orda_linear_ce_backward(9999, None, C.byref(a), 256, 256, None,
+                                             *(C.byref(t) if t is not None else None for t in out), 256, need - less,
+                                             err, 512)
+            assert rc == want, err.value
+
+
 def test_python_refuses_cpu_tensors():
     h, w, y = torch.zeros(2, 8), torch.zeros(3, 8), torch.zeros(2, dtype=torch.int64)
     with pytest.raises(H.OrdaError, match="GPU tensor"):
