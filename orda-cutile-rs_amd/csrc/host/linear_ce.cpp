@@ -25,7 +25,8 @@ struct Ce {
   const void *x, *w;
   int64_t ldx, ldw;
   bool planes;       // fp32: every product over three-plane operands
-  bool stage_w;      // bf16 weights that the products cannot read in place
+  bool direct;       // small fp32 calls: the logits in memory, fp32 operands
+  bool stage_w;      // weights that the products cannot read in place
   bool gh, gw;       // backward: the gradients asked for
   bool backward;
   int64_t hp;        // pitch of the compact hidden rows, plane width with planes
@@ -35,10 +36,12 @@ struct Ce {
 int64_t ds_pitch(const Ce& c, int64_t cols) { return c.planes ? 3 * round64(cols) : logits_pitch(cols, DType::BF16); }
 
 int64_t column_bytes(const Ce& c) {   // of scratch, for each column of a piece
-  int64_t b = c.planes ? 6 * c.hp : c.stage_w ? 2 * c.hp : 0;
+  int64_t b = c.planes ? 6 * c.hp : c.stage_w ? dtype_size(c.t) * c.hp : 0;
   b += c.backward ? round64(c.n) * (c.planes ? 6 : 2) : (c.n * 16 + 255) / 256;
   return b;
 }
+
+void choose_direct(Ce& c);
 
 Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool gw) {
   check_view(a.hidden, "hidden");
@@ -67,7 +70,7 @@ Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool
   c.ldx = tensor_ld(a.hidden);
   c.ldw = tensor_ld(a.weight);
   c.planes = c.t == DType::F32;
-  c.stage_w = !c.planes && !(c.ldw % 8 == 0 && c.h % 8 == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0);
+  c.stage_w = !(c.ldw % 8 == 0 && c.h % 8 == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0);
   c.hp = c.planes ? round64(c.h) : round8(c.h);
   c.backward = backward;
   c.gh = gh;
@@ -77,6 +80,7 @@ Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool
   most = std::max<int64_t>(most / 256 * 256, 256);
   const int64_t pieces = (c.v + most - 1) / most;
   c.piece = pieces == 1 ? c.v : ((c.v + pieces - 1) / pieces + 255) / 256 * 256;
+  choose_direct(c);
   return c;
 }
 
@@ -88,6 +92,7 @@ struct Scratch {
   void* w;           // a piece of the weights, padded or as planes
   void* ds;          // gradient of a piece's logits
   float* gh;         // grad_hidden of the compact rows
+  float* logits;     // direct: the logits; the gradient of the logits is ds
   float4 *stats, *state, *coef;
   float* xy;
   float* split;
@@ -180,6 +185,93 @@ GemmArgs grad_weight_product(const Ce& c, const Scratch& s, void* gw, int64_t ld
   return g;
 }
 
+// The direct form's products: fp32 operands, rows from the count on zeros.
+int64_t direct_pitch(const Ce& c) { return logits_pitch(c.v, DType::F32); }
+GemmArgs direct_product(const Ce& c, const Scratch& s) {
+  GemmArgs g{};
+  g.nprob = 1;
+  g.in_type = DType::F32;
+  g.a_kmajor = true;
+  g.alpha = 1.f;
+  g.epi = GemmEpilogue::StoreF32;
+  g.split_ws = s.split;
+  g.split_ws_bytes = s.split_bytes;
+  return g;
+}
+const void* direct_weight(const Ce& c, const Scratch& s) { return c.stage_w ? s.w : c.w; }
+GemmArgs direct_logits_product(const Ce& c, const Scratch& s) {
+  GemmArgs g = direct_product(c, s);
+  g.M = c.n;
+  g.N = c.v;
+  g.K = c.h;
+  g.lda = c.hp;
+  g.ldb = c.stage_w ? c.hp : c.ldw;
+  g.ldc = direct_pitch(c);
+  g.b_kmajor = true;
+  g.group_m = 8;
+  g.prob[0] = {s.x, direct_weight(c, s), s.logits};
+  return g;
+}
+GemmArgs direct_hidden_product(const Ce& c, const Scratch& s) {
+  GemmArgs g = direct_product(c, s);
+  g.M = c.n;
+  g.N = c.h;
+  g.K = c.v;
+  g.lda = direct_pitch(c);
+  g.ldb = c.stage_w ? c.hp : c.ldw;
+  g.ldc = round8(c.h);
+  g.group_m = 4;
+  g.share_rounds = true;
+  g.prob[0] = {s.ds, direct_weight(c, s), s.gh};
+  return g;
+}
+GemmArgs direct_weight_product(const Ce& c, const Scratch& s, void* gw, int64_t ldg) {
+  GemmArgs g = direct_product(c, s);
+  g.M = c.h;
+  g.N = c.v;
+  g.K = c.n;
+  g.lda = round64(c.n);
+  g.ldb = direct_pitch(c);
+  g.ldc = ldg;
+  g.c_trans = true;
+  g.group_m = 8;
+  g.prob[0] = {s.xt, s.ds, gw};
+  return g;
+}
+
+// Whether an fp32 call keeps its logits and multiplies fp32 operands: where the
+// passes that make planes of the weights, and tiles of 256 rows, cost more than
+// the logits' way through memory. Both sides by the products' own measure
+// (gemm_us; 4.2 us for every 32 elements of K and 20 us a round of 256 tiles over
+// planes) and 4 TB/s: 256 x 512 x 8192, forward and backward, 250 us of kernels
+// over planes.
+void choose_direct(Ce& c) {
+  if (!c.planes || c.piece < c.v || c.n > 8192) return;
+  const double pass = (static_cast<double>(c.v) + c.n) * c.h * 10 * 0.25e-6;
+  auto tiles = [](int64_t m, int64_t n) { return (m + 255) / 256 * ((n + 255) / 256); };
+  auto rounds = [](int64_t t, int64_t k) { return static_cast<double>((t + 255) / 256) * (k / 32.0 * 4.2 + 20.0); };
+  double planes = pass + rounds(tiles(c.n, c.v), c.hp);
+  Ce d = c;
+  d.planes = false;
+  d.hp = round8(c.h);
+  const Scratch none{};
+  double direct = gemm_us(direct_logits_product(d, none)) + static_cast<double>(c.n) * c.v * 8 * 0.25e-6 + 4.0 +
+                  (c.stage_w ? static_cast<double>(c.v) * c.h * 8 * 0.25e-6 : 0.0);
+  if (c.backward) {
+    const double kv = static_cast<double>(c.v);
+    // over planes K is split until the chip is full
+    if (c.gh) planes += std::max(tiles(c.n, c.h) * kv / 32 * 4.2 / 256, 20.0) + 12.0;
+    if (c.gw) planes += std::max(tiles(c.h, c.v) / 256.0, 1.0) * (round64(c.n) / 32.0 * 4.2 + 12.0);
+    if (c.gh) direct += gemm_us(direct_hidden_product(d, none)) + 4.0;
+    if (c.gw) direct += gemm_us(direct_weight_product(d, none, nullptr, c.h));
+    direct += static_cast<double>(c.n) * c.v * 8 * 0.25e-6;
+  }
+  if (direct >= planes) return;
+  c.planes = false;
+  c.direct = true;
+  c.hp = round8(c.h);
+}
+
 // (Sizes depend on which pointers are set, so a layout is made from a base that
 // is not null also where only its size counts.)
 Scratch lay_out(const Ce& c, void* base) {
@@ -195,7 +287,31 @@ Scratch lay_out(const Ce& c, void* base) {
   s.rows.src = static_cast<int32_t*>(take(c.n * 4));
   s.rows.pos = static_cast<int32_t*>(take(c.n * 4));
   s.rows.labels = static_cast<int64_t*>(take(c.n * 8));
-  s.x = take(np * c.hp * (c.planes ? 6 : 2));
+  s.x = take(np * c.hp * (c.planes ? 6 : dtype_size(c.t)));
+  if (c.direct) {
+    const int64_t ld = direct_pitch(c);
+    s.logits = static_cast<float*>(take(c.n * ld * 4));
+    if (c.stage_w) s.w = take(c.v * c.hp * 4);
+    s.split_bytes = gemm_split_bytes(direct_logits_product(c, s));
+    if (!c.backward) {
+      s.stats = static_cast<float4*>(take(c.n * ce_direct_tiles(c.v) * 16));
+      s.xy = static_cast<float*>(take(c.n * 4));
+    } else {
+      s.coef = static_cast<float4*>(take(c.n * 16));
+      s.ds = take(c.n * ld * 4);
+      if (c.gh) {
+        s.gh = static_cast<float*>(take(c.n * round8(c.h) * 4));
+        s.split_bytes = std::max(s.split_bytes, gemm_split_bytes(direct_hidden_product(c, s)));
+      }
+      if (c.gw) {
+        s.xt = take(c.h * np * 4);
+        s.split_bytes = std::max(s.split_bytes, gemm_split_bytes(direct_weight_product(c, s, nullptr, c.h)));
+      }
+    }
+    s.split = s.split_bytes > 0 ? static_cast<float*>(take(s.split_bytes)) : nullptr;
+    s.bytes = at;
+    return s;
+  }
   if (c.planes) s.w = take(round64(c.piece) * 6 * c.hp);
   else if (c.stage_w) s.w = take(c.piece * c.hp * 2);
   if (!c.backward) {
@@ -244,6 +360,7 @@ CePrepArgs prepare_rows(const orda_linear_ce& a, const Ce& c, const Scratch& s) 
   p.rows = s.rows;
   p.dst = s.x;
   p.pitch = c.hp;
+  p.whole = c.direct;
   return p;
 }
 
@@ -259,11 +376,58 @@ void stage_weights(const Ce& c, const Scratch& s, int64_t v0, int64_t cols, hipS
               "linear cross entropy weights");
 }
 
+// The direct form's logits, the parts of a split product left apart.
+CeDirectArgs direct_logits(const orda_linear_ce& a, const Ce& c, const Scratch& s, hipStream_t st) {
+  if (c.stage_w)
+    hip_check(launch_convert_rows(DType::F32, c.w, c.ldw, DType::F32, s.w, c.hp, c.v, c.h, st),
+              "linear cross entropy weights");
+  GemmArgs g = direct_logits_product(c, s);
+  const GemmSplit plan = gemm_split_plan(g);
+  g.partials_only = plan.splits > 1;
+  hip_check(launch_gemm(g, st), "linear cross entropy logits");
+  CeDirectArgs d{};
+  d.rows = s.rows;
+  d.v = c.v;
+  d.logits = plan.splits > 1 ? s.split : s.logits;
+  d.ld = plan.splits > 1 ? plan.ldp : g.ldc;
+  d.stride = plan.splits > 1 ? plan.stride : 0;
+  d.splits = plan.splits > 1 ? plan.splits : 1;
+  d.stats = s.stats;
+  d.stats_ld = ce_direct_tiles(c.v);
+  d.xy = s.xy;
+  d.coef = s.coef;
+  d.grad = static_cast<float*>(s.ds);
+  d.grad_ld = g.ldc;
+  return d;
+}
+
+CeLossArgs losses(const orda_linear_ce& a, const Ce& c, const Scratch& s, float* nll, float* lse) {
+  CeLossArgs l{};
+  l.rows = s.rows;
+  l.stats = s.stats;
+  l.state = s.state;
+  l.first = l.last = true;
+  l.xy = s.xy;
+  l.smooth_each = a.label_smoothing / static_cast<float>(c.v);
+  l.target = 1.f - a.label_smoothing;
+  l.nll = nll;
+  l.lse = lse;
+  return l;
+}
+
 void forward(const orda_linear_ce& a, const Ce& c, const Scratch& s, float* nll, float* lse, hipStream_t st) {
   CePrepArgs p = prepare_rows(a, c, s);
   p.nll = nll;
   p.lse_out = lse;
   hip_check(launch_ce_prep(p, c.t, c.planes, st), "linear cross entropy rows");
+  if (c.direct) {
+    const CeDirectArgs d = direct_logits(a, c, s, st);
+    hip_check(launch_ce_direct(d, c.n, false, st), "linear cross entropy losses");
+    CeLossArgs l = losses(a, c, s, nll, lse);
+    l.stats_ld = l.tiles = d.stats_ld;
+    hip_check(launch_ce_losses(l, c.n, st), "linear cross entropy losses");
+    return;
+  }
   for (int64_t v0 = 0; v0 < c.v; v0 += c.piece) {
     const int64_t cols = std::min(c.piece, c.v - v0);
     stage_weights(c, s, v0, cols, st);
@@ -273,19 +437,11 @@ void forward(const orda_linear_ce& a, const Ce& c, const Scratch& s, float* nll,
     g.ce.stats_ld = gemm_stat_tiles(c.piece);
     g.ce.xy = s.xy;
     hip_check(launch_gemm(g, st), "linear cross entropy logits");
-    CeLossArgs l{};
-    l.rows = s.rows;
-    l.stats = s.stats;
+    CeLossArgs l = losses(a, c, s, nll, lse);
     l.stats_ld = g.ce.stats_ld;
     l.tiles = gemm_stat_tiles(cols);
-    l.state = s.state;
     l.first = v0 == 0;
     l.last = v0 + cols == c.v;
-    l.xy = s.xy;
-    l.smooth_each = a.label_smoothing / static_cast<float>(c.v);
-    l.target = 1.f - a.label_smoothing;
-    l.nll = nll;
-    l.lse = lse;
     hip_check(launch_ce_losses(l, c.n, st), "linear cross entropy losses");
   }
 }
@@ -304,6 +460,16 @@ void backward(const orda_linear_ce& a, const Ce& c, const Scratch& s, const CeGr
     p.ldz = tensor_ld(*gh);
   }
   hip_check(launch_ce_prep(p, c.t, c.planes, st), "linear cross entropy rows");
+  if (c.direct) {
+    hip_check(launch_ce_direct(direct_logits(a, c, s, st), c.n, true, st), "linear cross entropy gradient");
+    if (c.gh) {
+      hip_check(launch_gemm(direct_hidden_product(c, s), st), "grad_hidden");
+      hip_check(launch_ce_scatter(s.gh, round8(c.h), s.rows, c.n, c.h, static_cast<float*>(gh->data), tensor_ld(*gh), st),
+                "grad_hidden");
+    }
+    if (c.gw) hip_check(launch_gemm(direct_weight_product(c, s, gw->data, tensor_ld(*gw)), st), "grad_weight");
+    return;
+  }
   for (int64_t v0 = 0; v0 < c.v; v0 += c.piece) {
     const int64_t cols = std::min(c.piece, c.v - v0);
     stage_weights(c, s, v0, cols, st);

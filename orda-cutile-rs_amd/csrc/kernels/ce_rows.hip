@@ -284,6 +284,108 @@ __global__ __launch_bounds__(256) void ce_losses_kernel(CeLossArgs a) {
   a.nll[i] = nll;
 }
 
+// ------------------------------------------------------------ logits in memory
+// Small fp32 calls (CeDirectArgs): a workgroup sums 2048 columns of a row over
+// the parts of a product that was split, in order, and leaves their statistics,
+// or writes the gradient of the logits (rows from the count on: zeros). 8 columns
+// a thread, 16-byte vectors; the rows' pitches hold whole ones.
+constexpr int kDirectCols = 2048;
+
+__device__ __forceinline__ void direct_logits(const CeDirectArgs& a, int64_t row, int64_t c0, f32x4 (&x)[2]) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int64_t c = c0 + q * (kDirectCols / 2) + threadIdx.x * 4;
+    x[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (c >= a.v) continue;
+    const float* p = a.logits + row * a.ld + c;
+    x[q] = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll 8
+    for (int s = 1; s < a.splits; ++s) x[q] += *reinterpret_cast<const f32x4*>(p + s * a.stride);
+  }
+}
+
+__global__ __launch_bounds__(256) void ce_direct_stats_kernel(CeDirectArgs a) {
+  __shared__ float red[4][3];
+  const int64_t row = blockIdx.y, c0 = static_cast<int64_t>(blockIdx.x) * kDirectCols;
+  if (row >= *a.rows.count) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  f32x4 x[2];
+  direct_logits(a, row, c0, x);
+  const int64_t y = a.rows.labels[row];
+  float m = -INFINITY, sx = 0.f;
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t c = c0 + q * (kDirectCols / 2) + threadIdx.x * 4 + e;
+      if (c >= a.v) continue;
+      m = fmaxf(m, x[q][e]);
+      sx += x[q][e];
+      if (c == y) a.xy[row] = x[q][e];
+    }
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) {
+    m = fmaxf(m, __shfl_xor(m, d));
+    sx += __shfl_xor(sx, d);
+  }
+  if (lane == 0) red[wave][0] = m, red[wave][1] = sx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, red[w][0]);
+  sx = red[0][1] + red[1][1] + red[2][1] + red[3][1];
+  const float ref = fabsf(m) <= FLT_MAX ? m : 0.f;   // as in the products' epilogue
+  float sum = 0.f;
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c0 + q * (kDirectCols / 2) + threadIdx.x * 4 + e < a.v)
+        sum += __builtin_amdgcn_exp2f(fmaf(x[q][e], kLog2e, -ref * kLog2e));
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
+  if (lane == 0) red[wave][2] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    a.stats[row * a.stats_ld + blockIdx.x] =
+        make_float4(m == -INFINITY ? m : ref, red[0][2] + red[1][2] + red[2][2] + red[3][2], 0.f, sx);
+}
+
+__global__ __launch_bounds__(256) void ce_direct_grad_kernel(CeDirectArgs a) {
+  const int64_t row = blockIdx.y, c0 = static_cast<int64_t>(blockIdx.x) * kDirectCols;
+  f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  const bool live = row < *a.rows.count;
+  float4 k = make_float4(0.f, 0.f, 0.f, 0.f);
+  int64_t y = -1;
+  if (live) {
+    direct_logits(a, row, c0, x);
+    k = a.coef[row];
+    y = a.rows.labels[row];
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int64_t c = c0 + q * (kDirectCols / 2) + threadIdx.x * 4;
+    if (c >= a.v) continue;
+    f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (live && c + e < a.v) {
+        d[e] = fmaf(k.y, __builtin_amdgcn_exp2f(fmaf(x[q][e], kLog2e, -k.x)), -k.z);
+        if (c + e == y) d[e] -= k.w;
+      }
+    *reinterpret_cast<f32x4*>(a.grad + row * a.grad_ld + c) = d;
+  }
+}
+
+// Compact fp32 gradient rows to their places; rows without a label are zero
+// already (CePrepArgs::zero).
+__global__ __launch_bounds__(256) void ce_scatter_kernel(const float* src, int64_t lds, CeRows r, int64_t h, float* dst,
+                                                         int64_t ldd) {
+  const int64_t row = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
+  if (row >= *r.count) return;
+  float* d = dst + r.src[row] * ldd;
+  for (int64_t c = threadIdx.x & 63; c < h; c += 64) d[c] = src[row * lds + c];
+}
+
 template <typename E>
 __global__ __launch_bounds__(256) void zero_rows_kernel(E* p, int64_t ld, int64_t rows, int64_t cols) {
   const int64_t row = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
@@ -328,6 +430,26 @@ hipError_t launch_ce_prep(const CePrepArgs& in, DType t, bool planes, hipStream_
 
 hipError_t launch_ce_losses(const CeLossArgs& a, int64_t n, hipStream_t stream) {
   hipLaunchKernelGGL(ce_losses_kernel, dim3(row_blocks(n)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+int64_t ce_direct_tiles(int64_t v) { return (v + kDirectCols - 1) / kDirectCols; }
+
+hipError_t launch_ce_direct(const CeDirectArgs& a, int64_t n, bool grad, hipStream_t stream) {
+  if (n <= 0) return hipSuccess;
+  if (a.ld % 4 != 0 || a.stride % 4 != 0 || reinterpret_cast<uintptr_t>(a.logits) % 16 != 0 || n > 65535 ||
+      (grad && (a.grad_ld % 4 != 0 || reinterpret_cast<uintptr_t>(a.grad) % 16 != 0)))
+    return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(ce_direct_tiles(a.v)), static_cast<unsigned>(n));
+  if (grad) hipLaunchKernelGGL(ce_direct_grad_kernel, grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL(ce_direct_stats_kernel, grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_ce_scatter(const float* src, int64_t lds, const CeRows& r, int64_t n, int64_t h, float* dst, int64_t ldd,
+                             hipStream_t stream) {
+  if (n <= 0) return hipSuccess;
+  hipLaunchKernelGGL(ce_scatter_kernel, dim3(row_blocks(n)), dim3(256), 0, stream, src, lds, r, h, dst, ldd);
   return hipGetLastError();
 }
 

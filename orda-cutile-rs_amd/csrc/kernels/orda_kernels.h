@@ -472,6 +472,27 @@ struct CeLossArgs {
   float *nll, *lse;
 };
 hipError_t launch_ce_losses(const CeLossArgs& a, int64_t n, hipStream_t stream);
+// Small fp32 calls keep a call's logits: from them (the sum of `splits` parts,
+// `stride` apart, in order) the tile statistics of 2048 columns and the label
+// logits, or the gradient of the logits. Pitches are multiples of 4.
+struct CeDirectArgs {
+  CeRows rows;
+  const float* logits;
+  int64_t ld, stride;
+  int splits;
+  int64_t v;
+  float4* stats;           // [row][stats_ld], ce_direct_tiles(v) of them
+  int64_t stats_ld;
+  float* xy;
+  const float4* coef;
+  float* grad;
+  int64_t grad_ld;
+};
+int64_t ce_direct_tiles(int64_t v);
+hipError_t launch_ce_direct(const CeDirectArgs& a, int64_t n, bool grad, hipStream_t stream);
+// dst[r.src[i]] = src[i], fp32.
+hipError_t launch_ce_scatter(const float* src, int64_t lds, const CeRows& r, int64_t n, int64_t h, float* dst, int64_t ldd,
+                             hipStream_t stream);
 // Zeros a matrix.
 hipError_t launch_zero_rows(DType t, void* p, int64_t ld, int64_t rows, int64_t cols, hipStream_t stream);
 

@@ -62,6 +62,14 @@ def test_pieces_of_the_vocabulary(dtype, piece):
     check(*inputs(300, 200, 5001, dtype, seed=2, ignored=0.2), label_smoothing=0.05, vocab_piece=piece)
 
 
+@pytest.mark.parametrize("n, h, v", [(1, 8, 300), (17, 72, 257), (129, 520, 513), (300, 33, 1001), (700, 1000, 2300)])
+@pytest.mark.parametrize("ignored", [0.0, 0.5])
+def test_fp32_over_planes(n, h, v, ignored):
+    """fp32 in pieces of the vocabulary takes three-plane operands whatever its
+    size (small calls in one piece keep their logits)."""
+    check(*inputs(n, h, v, "f32", seed=6, ignored=ignored), label_smoothing=0.1, vocab_piece=256)
+
+
 @pytest.mark.parametrize("n, h, v, ignored", [(5000, 4096, 600, 0.1), (5000, 4096, 600, 0.4), (17000, 40, 300, 0.3),
                                               (16384, 24, 70, 0.02), (8200, 1032, 500, 0.0)])
 def test_many_rows(n, h, v, ignored):
