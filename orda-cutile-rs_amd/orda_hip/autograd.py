@@ -20,9 +20,10 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import (Context, distillation_loss, embedding, embedding_backward,
-               linear_cross_entropy, linear_cross_entropy_backward)
+from . import (Context, distillation_loss, embedding, linear_cross_entropy,
+               linear_cross_entropy_backward)
 from . import _lib as L
+from .operators import _embed_grad, _gpu_tensor, _ids, _padding_row
 from .types import LossOptions, OrdaError, Teacher, TeacherMode
 
 
@@ -124,30 +125,42 @@ def distillation_loss_autograd(student_hidden: torch.Tensor, weight: torch.Tenso
     return DistillCEFunction.apply(student_hidden, weight, th, tw, labels, tl, mode, opts, ctx)
 
 
+def _first_order(gradients):
+    """The backward of a Function whose gradients come from the library: for a
+    gradient of the gradient (create_graph) torch's once_differentiable, which
+    then reports that there is none, and costs the other calls 5 us."""
+    once = torch.autograd.function.once_differentiable(gradients)
+
+    def backward(fctx, *grads):
+        return once(fctx, *grads) if torch.is_grad_enabled() else gradients(fctx, *grads)
+    return staticmethod(backward)
+
+
 class LinearCrossEntropyFunction(torch.autograd.Function):
     """nll, lse = LinearCrossEntropyFunction.apply(hidden, weight, labels,
     ignore_index, label_smoothing, vocab_piece)."""
 
     @staticmethod
     def forward(fctx, hidden, weight, labels, ignore_index, label_smoothing, vocab_piece):
-        fctx.opts = dict(ignore_index=ignore_index, label_smoothing=label_smoothing,
-                         vocab_piece=vocab_piece)
-        nll, lse = linear_cross_entropy(hidden.detach(), weight.detach(), labels, **fctx.opts)
+        nll, lse = linear_cross_entropy(hidden, weight, labels, ignore_index=ignore_index,
+                                        label_smoothing=label_smoothing, vocab_piece=vocab_piece)
         # (hidden, weight and labels are read again: autograd's version counters
         # report a change in place before the backward)
         fctx.save_for_backward(hidden, weight, labels, lse)
+        fctx.opts = ignore_index, label_smoothing, vocab_piece
         fctx.set_materialize_grads(False)
         return nll, lse
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(fctx, g_nll, g_lse):
-        hidden, weight, labels, lse = fctx.saved_tensors
         want_h, want_w = fctx.needs_input_grad[:2]
         if (g_nll is None and g_lse is None) or not (want_h or want_w):
             return (None,) * 6
-        gh, gw = linear_cross_entropy_backward(hidden.detach(), weight.detach(), labels, lse.detach(), g_nll,
-                                               g_lse, grad_hidden=want_h, grad_weight=want_w, **fctx.opts)
+        hidden, weight, labels, lse = fctx.saved_tensors
+        ignore_index, label_smoothing, vocab_piece = fctx.opts
+        gh, gw = linear_cross_entropy_backward(hidden, weight, labels, lse, g_nll, g_lse, ignore_index=ignore_index,
+                                               label_smoothing=label_smoothing, vocab_piece=vocab_piece,
+                                               grad_hidden=want_h, grad_weight=want_w)
         return gh, gw, None, None, None, None
 
 
@@ -167,20 +180,19 @@ class EmbeddingFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(fctx, ids, weight, scale, padding_idx):
-        out = embedding(ids, weight.detach(), scale=scale)
-        if padding_idx is not None and not -weight.size(0) <= padding_idx < weight.size(0):
-            raise OrdaError(f"padding_idx must be a row of {weight.size(0)}, got {padding_idx}")
+        rows = weight.size(0)
+        fctx.opts = rows, scale, _padding_row(padding_idx, rows)
+        out = embedding(ids, weight, scale=scale)
         fctx.save_for_backward(ids)
-        fctx.opts = dict(num_rows=weight.size(0), scale=scale, padding_idx=padding_idx)
         return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(fctx, grad):
-        (ids,) = fctx.saved_tensors
         if not fctx.needs_input_grad[1]:
             return None, None, None, None
-        return None, embedding_backward(grad, ids, **fctx.opts), None, None
+        (ids,) = fctx.saved_tensors
+        g = _gpu_tensor(grad, "grad")
+        return None, _embed_grad(g, _ids(ids, g.device), *fctx.opts), None, None
 
 
 def embedding_autograd(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,

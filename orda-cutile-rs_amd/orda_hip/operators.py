@@ -18,6 +18,7 @@ a weighted mean with the gradients in the same call (src/api.rs:188-422).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Tuple
 
 from . import _lib as L
@@ -39,13 +40,16 @@ def _gpu_tensor(x, what: str):
     """x itself, where it is a tensor in GPU memory of its own (not a wrapper
     such as functorch makes, whose memory the library cannot read)."""
     torch = _torch()
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise OrdaError(f"{what} must be a GPU tensor")
+    kind = type(x)
+    if (kind is not torch.Tensor and kind is not torch.nn.Parameter) or not x.is_cuda:
+        if not isinstance(x, torch.Tensor) or not x.is_cuda:
+            raise OrdaError(f"{what} must be a GPU tensor")
+        raise OrdaError(f"{what} must be a plain tensor with memory of its own")
     try:
-        plain = type(x) in (torch.Tensor, torch.nn.Parameter) and (x.data_ptr() != 0 or x.numel() == 0)
+        plain = x.data_ptr() != 0 or x.numel() == 0
     except RuntimeError:
         plain = False
-    if not plain or x.layout != torch.strided or x.is_neg():
+    if not plain or x.layout is not torch.strided or x.is_neg():
         raise OrdaError(f"{what} must be a plain tensor with memory of its own")
     return x
 
@@ -108,7 +112,15 @@ def _stream(device):
 
 
 def _bytes(n: int, device):
-    return _torch().empty(n, dtype=_torch().uint8, device=device)
+    torch = _torch()
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _embed_bytes(n: int, rows: int, cols: int, dtype: int) -> int:
+    b = C.c_int64()
+    _call(L.load().orda_embedding_backward_workspace, n, rows, cols, dtype, C.byref(b))
+    return b.value
 
 
 # ------------------------------------------------------------------ linear cross entropy
@@ -247,44 +259,57 @@ def embedding_backward(grad, ids, num_rows: int, *, scale: float = 1.0,
     gradient, after its other use). Tokens equal to ``padding_idx`` (counted from
     the end where negative), and ids that are no row, add nothing.
     """
-    torch = _torch()
     g = _gpu_tensor(grad, "grad")
     i = _ids(ids, g.device)
-    if g.dim() != ids.dim() + 1 or tuple(g.shape[:-1]) != tuple(ids.shape):
+    if g.dim() != ids.dim() + 1 or g.shape[:-1] != ids.shape:
         raise OrdaError(f"grad must be [*ids.shape, H], got {list(g.shape)} for ids {list(ids.shape)}")
-    h = g.size(-1)
-    g = _matrix(g.reshape(-1, h) if h else g.new_empty((i.numel(), 0)), "grad")
-    gd = _desc(g, "grad")
     if num_rows < 0:
         raise OrdaError("num_rows must be >= 0")
-    pad = -1
-    if padding_idx is not None:
-        pad = padding_idx + num_rows if padding_idx < 0 else padding_idx
-        if not 0 <= pad < num_rows:
-            raise OrdaError(f"padding_idx must be a row of {num_rows}, got {padding_idx}")
+    pad = _padding_row(padding_idx, num_rows)
     if out is None:
         if accumulate:
             raise OrdaError("accumulate needs out")
-        out = torch.empty((num_rows, h), dtype=g.dtype, device=g.device)
-    else:
-        out = _gpu_tensor(out, "out")
-        _same_device(g.device, out=out)
-        if tuple(out.shape) != (num_rows, h):
-            raise OrdaError(f"out must be [{num_rows}, {h}]")
-        if _matrix(out, "out") is not out:
-            raise OrdaError("out must have adjacent columns and rows that do not overlap")
-        if out.requires_grad and torch.is_grad_enabled():
-            raise OrdaError("out must not require a gradient")
-        if _overlap(out, g):
-            raise OrdaError("out must not share memory with grad")
-    od = _desc(out, "out")
-    lib = L.load()
-    n = C.c_int64()
-    _call(lib.orda_embedding_backward_workspace, i.numel(), num_rows, h, gd.dtype, C.byref(n))
-    ws = _bytes(n.value, g.device)
-    _call(lib.orda_embedding_backward, g.device.index, _stream(g.device), i.data_ptr(), i.element_size(),
-          i.numel(), C.byref(gd), pad, scale, int(accumulate), C.byref(od), ws.data_ptr(), ws.numel())
+        return _embed_grad(g, i, num_rows, scale, pad)
+    torch = _torch()
+    out = _gpu_tensor(out, "out")
+    _same_device(g.device, out=out)
+    if tuple(out.shape) != (num_rows, g.size(-1)):
+        raise OrdaError(f"out must be [{num_rows}, {g.size(-1)}]")
+    if _matrix(out, "out") is not out:
+        raise OrdaError("out must have adjacent columns and rows that do not overlap")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise OrdaError("out must not require a gradient")
+    if _overlap(out, g.reshape(-1, g.size(-1)) if g.numel() else g.new_empty((0, 0))):
+        raise OrdaError("out must not share memory with grad")
+    _embed_grad(g, i, num_rows, scale, pad, out, accumulate)
     torch.autograd.graph.increment_version(out)   # written in place
+    return out
+
+
+def _padding_row(padding_idx, num_rows: int) -> int:
+    if padding_idx is None:
+        return -1
+    pad = padding_idx + num_rows if padding_idx < 0 else padding_idx
+    if not 0 <= pad < num_rows:
+        raise OrdaError(f"padding_idx must be a row of {num_rows}, got {padding_idx}")
+    return pad
+
+
+def _embed_grad(g, i, num_rows: int, scale: float, pad: int, out=None, accumulate: bool = False):
+    """embedding_backward on checked tensors (g [*, H], i 1-D)."""
+    torch = _torch()
+    h = g.size(-1)
+    if g.dim() != 2:
+        g = g.reshape(-1, h) if h else g.new_empty((i.numel(), 0))
+    g = _matrix(g, "grad")
+    gd = _desc(g, "grad")
+    if out is None:
+        out = torch.empty((num_rows, h), dtype=g.dtype, device=g.device)
+    n = i.numel()
+    b = _embed_bytes(n, num_rows, h, gd.dtype)
+    ws = _bytes(b, g.device)
+    _call(L.load().orda_embedding_backward, g.device.index, _stream(g.device), i.data_ptr(), i.element_size(), n,
+          C.byref(gd), pad, scale, accumulate, C.byref(_desc(out, "out")), ws.data_ptr(), b)
     return out
 
 

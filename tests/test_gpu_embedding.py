@@ -171,6 +171,16 @@ def test_autograd(dtype):
         assert torch.equal(embedding_autograd(ids, w), w[ids])
 
 
+def test_no_second_derivative():
+    """A gradient of the gradient is reported, not silently zero."""
+    w = grad_of(40, 16, "f32").requires_grad_(True)
+    ids = tokens(30, 40, "text")
+    g = grad_of(30, 16, "f32").requires_grad_(True)
+    (gw,) = torch.autograd.grad(embedding_autograd(ids, w), w, g, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        gw.sum().backward()
+
+
 def test_the_same_bits_and_another_stream():
     ids, g = tokens(6000, 3000, "text"), grad_of(6000, 200, "f32")
     want = H.embedding_backward(g, ids, 3000)

@@ -196,6 +196,17 @@ def test_autograd_reports_changed_inputs():
         nll.sum().backward()
 
 
+def test_no_second_derivative():
+    """A gradient of the gradient is reported, not silently zero."""
+    x, w, y, gn, gl = inputs(20, 64, 300, "f32")
+    x.requires_grad_(True)
+    gn.requires_grad_(True)
+    nll, _ = linear_cross_entropy_autograd(x, w, y)
+    (gx,) = torch.autograd.grad(nll, x, gn, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        gx.sum().backward()
+
+
 def test_batched_gradients_refused():
     x, w, y, gn, gl = inputs(20, 64, 300, "bf16")
     x.requires_grad_(True)
