@@ -40,14 +40,13 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float s) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Eight values of a row from column c on (0 past cols).
-template <typename E, bool VEC>
+// Eight values of a row from column c on (0 past cols). The vectors need no
+// alignment but their elements': rows of any pitch load as wide.
+template <typename E>
 __device__ __forceinline__ void load8(const E* row, int64_t c, int64_t cols, float (&x)[8]) {
-  if (VEC && c + 8 <= cols) {
-    alignas(16) E w[8];
-#pragma unroll
-    for (int b = 0; b < static_cast<int>(sizeof(w)) / 16; ++b)
-      reinterpret_cast<u32x4*>(w)[b] = reinterpret_cast<const u32x4*>(row + c)[b];
+  if (c + 8 <= cols) {
+    E w[8];
+    __builtin_memcpy(w, row + c, sizeof(w));
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = static_cast<float>(w[k]);
   } else {
@@ -62,7 +61,7 @@ __device__ __forceinline__ void store8(uint8_t* row, int64_t c, int64_t cols, co
 
 // Blocks of one row: 16 lanes a block of 128, a wave 4 blocks of each of 4 rows,
 // a workgroup 16 rows, whose scales leave as 64 bytes a block.
-template <typename E, bool VEC>
+template <typename E>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a) {
   __shared__ float sc[4][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -74,7 +73,7 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int64_t r = r0 + wave * 4 + q;
-    load8<E, VEC>(src + (r < a.rows ? r : a.rows - 1) * a.lds, c, a.cols, x[q]);
+    load8<E>(src + (r < a.rows ? r : a.rows - 1) * a.lds, c, a.cols, x[q]);
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -99,7 +98,7 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a) {
 
 // Blocks of 128 rows: a workgroup holds a block in registers, 8 rows x 8
 // columns a thread.
-template <typename E, bool VEC>
+template <typename E>
 __global__ __launch_bounds__(256) void fp8_quant_blocks_kernel(Fp8QuantArgs a) {
   __shared__ uint32_t top[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -112,7 +111,7 @@ __global__ __launch_bounds__(256) void fp8_quant_blocks_kernel(Fp8QuantArgs a) {
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     const int64_t r = r0 + 16 * q;
-    load8<E, VEC>(src + (r < a.rows ? r : a.rows - 1) * a.lds, c, a.cols, x[q]);   // the last row again
+    load8<E>(src + (r < a.rows ? r : a.rows - 1) * a.lds, c, a.cols, x[q]);   // the last row again
 #pragma unroll
     for (int k = 0; k < 8; ++k) m = abs_bits(x[q][k]) > m ? abs_bits(x[q][k]) : m;
   }
@@ -234,7 +233,7 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
   }
   const unsigned char* const pa = a.a + m0 * a.lda;
   const unsigned char* const pb = a.b + n0 * a.ldb;
-  // Scales of a stage: waves 0-3 fetch a row's each, wave 4 B's two blocks'.
+  // Scales of a stage: waves 0-3 fetch a row's each, the others B's two blocks'.
   const float* const psa = a.sa + m0 * a.sa_row;
   const int64_t nb0 = n0 / 128, nbs = (a.n + 127) / 128;
   const float* const psb = a.sb + nb0 * a.sb_row;
@@ -242,45 +241,30 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
   if (wave < 4) {
     const int64_t r = m0 + tid < a.m ? tid : a.m - 1 - m0;
     offS = static_cast<uint32_t>(r * a.sa_row * 4);
-  } else if (wave == 4) {
+  } else {
     offS = static_cast<uint32_t>(((lane & 1) != 0 && nb0 + 1 < nbs ? 1 : 0) * a.sb_row * 4);
   }
   const uint32_t lds0 = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
       static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)smem))));
-  const int nkb = static_cast<int>((a.k + 127) / 128);
-  auto issue = [&](int kb, int buf) {
-    const uint32_t st = lds0 + buf * kStage + wave * 1024;
-    const unsigned char* const sa = pa + kb * int64_t{128};
-    const unsigned char* const sb = pb + kb * int64_t{128};
-    const int krem = static_cast<int>(a.k - kb * int64_t{128});
-    if (krem >= 128) {
-      const uint64_t ua = uniform64(sa), ub = uniform64(sb);
-      dma16_at<0>(ua, offA[0], st);
-      dma16_at<8192>(ua, offA[1], st);
-      dma16_at<16384>(ua, offA[2], st);
-      dma16_at<24576>(ua, offA[3], st);
-      dma16_at<kOp>(ub, offB[0], st);
-      dma16_at<kOp + 8192>(ub, offB[1], st);
-      dma16_at<kOp + 16384>(ub, offB[2], st);
-      dma16_at<kOp + 24576>(ub, offB[3], st);
-    } else {   // the last, partial block: zeros past K
-      unsigned char* const l = smem + buf * kStage + wave * 1024 + lane * 16;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const unsigned char* const src = t < 4 ? sa + offA[t & 3] : sb + offB[t & 3];
-        alignas(16) unsigned char w[16];
-        if (kcol + 16 <= krem) {
-          *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(src);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) w[k] = kcol + k < krem ? src[k] : 0;
-        }
-        *reinterpret_cast<u32x4*>(l + (t & 3) * 8192 + (t < 4 ? 0 : kOp)) = *reinterpret_cast<const u32x4*>(w);
-      }
-    }
+  // Block kb into stage `buf`: nine transfers a wave (waves 4-7 all move B's
+  // scales, the same values to the same place, so that every wave counts alike).
+  auto issue_scales = [&](int kb, int buf) {
     const uint32_t sc = lds0 + 2 * kStage + buf * kScales;
     if (wave < 4) dma4(uniform64(psa + kb * a.sa_col), offS, sc + wave * 256);
-    else if (wave == 4 && lane < 2) dma4(uniform64(psb + kb * a.sb_col), offS, sc + 1024);
+    else if (lane < 2) dma4(uniform64(psb + kb * a.sb_col), offS, sc + 1024);
+  };
+  auto issue = [&](int kb, int buf) {
+    const uint32_t st = lds0 + buf * kStage + wave * 1024;
+    const uint64_t ua = uniform64(pa + kb * int64_t{128}), ub = uniform64(pb + kb * int64_t{128});
+    dma16_at<0>(ua, offA[0], st);
+    dma16_at<8192>(ua, offA[1], st);
+    dma16_at<16384>(ua, offA[2], st);
+    dma16_at<24576>(ua, offA[3], st);
+    dma16_at<kOp>(ub, offB[0], st);
+    dma16_at<kOp + 8192>(ub, offB[1], st);
+    dma16_at<kOp + 16384>(ub, offB[2], st);
+    dma16_at<kOp + 24576>(ub, offB[3], st);
+    issue_scales(kb, buf);
   };
   f32x4 acc[8][4];
 #pragma unroll
@@ -288,41 +272,40 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int lrow = lane & 15, lgrp = lane >> 4;
-  // Fragment of 16 rows from LDS address base: lane (row lrow, group lgrp) holds
-  // K 32·lgrp .. +31, chunks 2·lgrp and 2·lgrp + 1 (both operands alike).
-  const uint32_t f0 = static_cast<uint32_t>(lrow * 128 + (((2 * lgrp) ^ (lrow & 7)) << 4));
-  const uint32_t f1 = static_cast<uint32_t>(lrow * 128 + (((2 * lgrp + 1) ^ (lrow & 7)) << 4));
-  auto frag = [&](uint32_t base) {
-    const u32x4 lo = *(const lds_u32x4*)(static_cast<uintptr_t>(base + f0));
-    const u32x4 hi = *(const lds_u32x4*)(static_cast<uintptr_t>(base + f1));
+  // Fragment of 16 rows: lane (row lrow, group lgrp) holds K 32·lgrp .. +31, chunks
+  // 2·lgrp and 2·lgrp + 1 (both operands alike). Addresses of fragment 0 in stage 0,
+  // which lies 64 KB below stage 1.
+  const uint32_t f0 = lds0 + static_cast<uint32_t>(lrow * 128 + (((2 * lgrp) ^ (lrow & 7)) << 4));
+  const uint32_t f1 = lds0 + static_cast<uint32_t>(lrow * 128 + (((2 * lgrp + 1) ^ (lrow & 7)) << 4));
+  uint32_t a0 = f0 + wm * 16384, a1 = f1 + wm * 16384;
+  uint32_t b0 = f0 + kOp + wn * 8192, b1 = f1 + kOp + wn * 8192;
+  uint32_t sa_at = lds0 + 2 * kStage + (wm * 128 + lrow) * 4, sb_at = lds0 + 2 * kStage + 1024 + (wn >> 1) * 4;
+  auto frag = [&](uint32_t lo_at, uint32_t hi_at, int f) {
+    const u32x4 lo = *(const lds_u32x4*)(static_cast<uintptr_t>(lo_at + f * 2048));
+    const u32x4 hi = *(const lds_u32x4*)(static_cast<uintptr_t>(hi_at + f * 2048));
     return __builtin_bit_cast(i32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  issue(0, 0);
-  for (int kb = 0; kb < nkb; ++kb) {
-    const int buf = kb & 1;
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(kWaitAll);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    if (kb + 1 < nkb) issue(kb + 1, buf ^ 1);
-    __builtin_amdgcn_sched_barrier(0);
-    const uint32_t st = lds0 + buf * kStage, sc = lds0 + 2 * kStage + buf * kScales;
+  auto scale = [&](uint32_t at, int f) { return *(const lds_f32*)(static_cast<uintptr_t>(at + f * 64)); };
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  // One block from stage `buf`, which has landed for all waves.
+  auto block = [&](int buf) {
+    const uint32_t at = buf * kStage, sc = buf * kScales;
     using F = std::conditional_t<WIDE, Wide, i32x8>;
-    auto operand = [&](uint32_t base) -> F {
-      if constexpr (WIDE) return widened(frag(base));
-      else return frag(base);
+    auto operand = [&](uint32_t lo_at, uint32_t hi_at, int f) -> F {
+      if constexpr (WIDE) return widened(frag(lo_at, hi_at, f));
+      else return frag(lo_at, hi_at, f);
     };
     F b[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = operand(st + kOp + (wn * 64 + j * 16) * 128);
-    const float s_b = *(const lds_f32*)(static_cast<uintptr_t>(sc + 1024 + (wn >> 1) * 4));
+    for (int j = 0; j < 4; ++j) b[j] = operand(b0 + at, b1 + at, j);
+    const float s_b = scale(sb_at + sc, 0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const F x = operand(st + (wm * 128 + i * 16) * 128);
-      const float s = s_b * *(const lds_f32*)(static_cast<uintptr_t>(sc + (wm * 128 + i * 16 + lrow) * 4));
+      const F x = operand(a0 + at, a1 + at, i);
+      const float s = s_b * scale(sa_at + sc, i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f32x4 p = {0.f, 0.f, 0.f, 0.f};
+        f32x4 p = zero;
         if constexpr (WIDE) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j].k[q], x.k[q], p, 0, 0, 0);
@@ -333,6 +316,122 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
         for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(s, p[e], acc[i][j][e]);
       }
     }
+  };
+  const int nfull = static_cast<int>(a.k / 128);
+  if constexpr (WIDE) {
+    if (nfull > 0) issue(0, 0);
+    for (int kb = 0; kb < nfull; ++kb) {
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(kWaitAll);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      if (kb + 1 < nfull) issue(kb + 1, (kb + 1) & 1);
+      __builtin_amdgcn_sched_barrier(0);
+      block(kb & 1);
+    }
+  } else if (nfull > 0) {
+    // Row i of the wave's fragments is four MFMAs; beside them run the fmas of
+    // row i - 1 and the reads of row i + 2. With row 6 every wave has read the
+    // whole stage and its own transfers of the next one have landed: one barrier,
+    // after which the stage is free for the transfers of block kb + 2, which so have
+    // a whole iteration to land, and the next block's first fragments are read
+    // under rows 6 and 7.
+    i32x8 b[4], x[4];
+    f32x4 p[2][4];
+    float row_scale[4], s[2] = {0.f, 0.f};
+    issue(0, 0);
+    if (nfull > 1) {
+      issue(1, 1);
+      __builtin_amdgcn_s_waitcnt(vm_wait(9));
+    } else {
+      __builtin_amdgcn_s_waitcnt(kWaitAll);
+    }
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    x[0] = frag(a0, a1, 0);
+    x[1] = frag(a0, a1, 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      b[j] = frag(b0, b1, j);
+      p[1][j] = zero;   // row -1: nothing
+    }
+    float s_b = scale(sb_at, 0);
+    row_scale[0] = scale(sa_at, 0);
+    row_scale[1] = scale(sa_at, 1);
+    // (The last block's iteration reads ahead too, what is in the other stage.)
+    for (int kb = 0; kb < nfull; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (i == 6) {
+          __builtin_amdgcn_s_waitcnt(kWaitAll);
+          __builtin_amdgcn_s_barrier();
+          __builtin_amdgcn_sched_barrier(0);
+          if (kb + 2 < nfull) issue(kb + 2, kb & 1);
+          const uint32_t flip = (kb & 1) != 0 ? 0u - kStage : kStage;   // to the other stage
+          const uint32_t flip_s = (kb & 1) != 0 ? 0u - kScales : kScales;
+          a0 += flip;
+          a1 += flip;
+          b0 += flip;
+          b1 += flip;
+          sa_at += flip_s;
+          sb_at += flip_s;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const int ahead = (i + 2) & 7;   // rows 0 and 1: of the next block
+        x[(i + 2) & 3] = frag(a0, a1, ahead);
+        row_scale[(i + 2) & 3] = scale(sa_at, ahead);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], x[i & 3], zero, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[(i + 7) & 7][j][e] = fmaf(s[(i + 1) & 1], p[(i + 1) & 1][j][e], acc[(i + 7) & 7][j][e]);
+          asm volatile("" : "+v"(acc[(i + 7) & 7][j]));   // here, not behind the loop's other blocks
+          if (i == 7) b[j] = frag(b0, b1, j);
+        }
+        s[i & 1] = s_b * row_scale[i & 3];
+        if (i == 7) s_b = scale(sb_at, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[7][j][e] = fmaf(s[1], p[1][j][e], acc[7][j][e]);
+    // back to stage 0's addresses for the partial block
+    if ((nfull & 1) != 0) {
+      a0 -= kStage;
+      a1 -= kStage;
+      b0 -= kStage;
+      b1 -= kStage;
+      sa_at -= kScales;
+      sb_at -= kScales;
+    }
+  }
+  if (nfull * int64_t{128} < a.k) {   // the last, partial block: zeros past K
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kWaitAll);
+    __builtin_amdgcn_s_barrier();
+    const int krem = static_cast<int>(a.k - nfull * int64_t{128});
+    unsigned char* const l = smem + wave * 1024 + lane * 16;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const unsigned char* const src = (t < 4 ? pa + offA[t & 3] : pb + offB[t & 3]) + nfull * int64_t{128};
+      alignas(16) unsigned char w[16];
+      if (kcol + 16 <= krem) {
+        *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(src);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) w[k] = kcol + k < krem ? src[k] : 0;
+      }
+      *reinterpret_cast<u32x4*>(l + (t & 3) * 8192 + (t < 4 ? 0 : kOp)) = *reinterpret_cast<const u32x4*>(w);
+    }
+    issue_scales(nfull, 0);
+    __builtin_amdgcn_s_waitcnt(kWaitAll);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    block(0);
   }
   // acc[i][j][e] is row m0 + wm·128 + 16i + lrow, column n0 + wn·64 + 16j + 4·lgrp + e.
   OT* const C = static_cast<OT*>(a.c);
@@ -363,17 +462,11 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
 hipError_t launch_fp8_quant(const Fp8QuantArgs& a, DType t, bool blocks, hipStream_t stream) {
   if (a.rows <= 0 || a.cols <= 0) return hipSuccess;
   if (a.ldc % 8 != 0 || reinterpret_cast<uintptr_t>(a.codes) % 8 != 0) return hipErrorInvalidValue;
-  const bool vec = a.lds * dtype_size(t) % 16 == 0 && reinterpret_cast<uintptr_t>(a.src) % 16 == 0;
   const int64_t grid = blocks ? (a.rows + 127) / 128 * ((a.cols + 127) / 128) : (a.rows + 15) / 16 * ((a.cols + 511) / 512);
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   using K = void (*)(Fp8QuantArgs);
-  K k;
-  if (blocks)
-    k = t == DType::BF16 ? (vec ? fp8_quant_blocks_kernel<__bf16, true> : fp8_quant_blocks_kernel<__bf16, false>)
-                         : (vec ? fp8_quant_blocks_kernel<float, true> : fp8_quant_blocks_kernel<float, false>);
-  else
-    k = t == DType::BF16 ? (vec ? fp8_quant_rows_kernel<__bf16, true> : fp8_quant_rows_kernel<__bf16, false>)
-                         : (vec ? fp8_quant_rows_kernel<float, true> : fp8_quant_rows_kernel<float, false>);
+  const K k = blocks ? (t == DType::BF16 ? static_cast<K>(fp8_quant_blocks_kernel<__bf16>) : fp8_quant_blocks_kernel<float>)
+                     : (t == DType::BF16 ? static_cast<K>(fp8_quant_rows_kernel<__bf16>) : fp8_quant_rows_kernel<float>);
   hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
