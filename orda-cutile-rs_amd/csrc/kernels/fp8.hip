@@ -156,7 +156,10 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const uint8_t* src, int64
 // waves scales, the other multiplies. K advances one block at a time through two
 // 64 KB stages in LDS, moved by DMA while the other is read: rows of 128
 // bytes, their eight 16-byte chunks swizzled by row (by the choice of the chunk a
-// lane fetches), so that fragment reads meet no bank twice. The operands enter
+// lane fetches). Lane group g reads chunks g and 4 + g of its row, so that the
+// lanes served together (8 rows, two neighbouring groups) meet no bank twice; with
+// chunks 2g and 2g + 1 every read took twice as long. (Which K a lane holds does
+// not matter while both operands hold the same.) The operands enter
 // the MFMA swapped: a lane then owns four consecutive columns of a row.
 //
 // The e4m3 MFMAs (all four shapes, measured) add their products to fewer bits than
@@ -246,25 +249,29 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
   }
   const uint32_t lds0 = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(
       static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)smem))));
-  // Block kb into stage `buf`: nine transfers a wave (waves 4-7 all move B's
+  // Block kb into stage `buf`: nine transfers a wave in all (waves 4-7 all move B's
   // scales, the same values to the same place, so that every wave counts alike).
   auto issue_scales = [&](int kb, int buf) {
     const uint32_t sc = lds0 + 2 * kStage + buf * kScales;
     if (wave < 4) dma4(uniform64(psa + kb * a.sa_col), offS, sc + wave * 256);
     else if (lane < 2) dma4(uniform64(psb + kb * a.sb_col), offS, sc + 1024);
   };
-  auto issue = [&](int kb, int buf) {
+  auto issue_a = [&](int kb, int buf) {   // and the scales: five transfers a wave
     const uint32_t st = lds0 + buf * kStage + wave * 1024;
-    const uint64_t ua = uniform64(pa + kb * int64_t{128}), ub = uniform64(pb + kb * int64_t{128});
-    dma16_at<0>(ua, offA[0], st);
-    dma16_at<8192>(ua, offA[1], st);
-    dma16_at<16384>(ua, offA[2], st);
-    dma16_at<24576>(ua, offA[3], st);
-    dma16_at<kOp>(ub, offB[0], st);
-    dma16_at<kOp + 8192>(ub, offB[1], st);
-    dma16_at<kOp + 16384>(ub, offB[2], st);
-    dma16_at<kOp + 24576>(ub, offB[3], st);
+    const uint64_t u = uniform64(pa + kb * int64_t{128});
+    dma16_at<0>(u, offA[0], st);
+    dma16_at<8192>(u, offA[1], st);
+    dma16_at<16384>(u, offA[2], st);
+    dma16_at<24576>(u, offA[3], st);
     issue_scales(kb, buf);
+  };
+  auto issue_b = [&](int kb, int buf) {   // four
+    const uint32_t st = lds0 + buf * kStage + kOp + wave * 1024;
+    const uint64_t u = uniform64(pb + kb * int64_t{128});
+    dma16_at<0>(u, offB[0], st);
+    dma16_at<8192>(u, offB[1], st);
+    dma16_at<16384>(u, offB[2], st);
+    dma16_at<24576>(u, offB[3], st);
   };
   f32x4 acc[8][4];
 #pragma unroll
@@ -272,11 +279,10 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int lrow = lane & 15, lgrp = lane >> 4;
-  // Fragment of 16 rows: lane (row lrow, group lgrp) holds K 32·lgrp .. +31, chunks
-  // 2·lgrp and 2·lgrp + 1 (both operands alike). Addresses of fragment 0 in stage 0,
-  // which lies 64 KB below stage 1.
-  const uint32_t f0 = lds0 + static_cast<uint32_t>(lrow * 128 + (((2 * lgrp) ^ (lrow & 7)) << 4));
-  const uint32_t f1 = lds0 + static_cast<uint32_t>(lrow * 128 + (((2 * lgrp + 1) ^ (lrow & 7)) << 4));
+  // Fragment of 16 rows: lane (row lrow, group lgrp) holds chunks lgrp and
+  // 4 + lgrp. Addresses of fragment 0 in stage 0, which lies 64 KB below stage 1.
+  const uint32_t f0 = lds0 + static_cast<uint32_t>(lrow * 128 + ((lgrp ^ (lrow & 7)) << 4));
+  const uint32_t f1 = lds0 + static_cast<uint32_t>(lrow * 128 + (((4 + lgrp) ^ (lrow & 7)) << 4));
   uint32_t a0 = f0 + wm * 16384, a1 = f1 + wm * 16384;
   uint32_t b0 = f0 + kOp + wn * 8192, b1 = f1 + kOp + wn * 8192;
   uint32_t sa_at = lds0 + 2 * kStage + (wm * 128 + lrow) * 4, sb_at = lds0 + 2 * kStage + 1024 + (wn >> 1) * 4;
@@ -319,29 +325,33 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
   };
   const int nfull = static_cast<int>(a.k / 128);
   if constexpr (WIDE) {
-    if (nfull > 0) issue(0, 0);
+    if (nfull > 0) issue_b(0, 0), issue_a(0, 0);
     for (int kb = 0; kb < nfull; ++kb) {
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_waitcnt(kWaitAll);
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
-      if (kb + 1 < nfull) issue(kb + 1, (kb + 1) & 1);
+      if (kb + 1 < nfull) issue_b(kb + 1, (kb + 1) & 1), issue_a(kb + 1, (kb + 1) & 1);
       __builtin_amdgcn_sched_barrier(0);
       block(kb & 1);
     }
   } else if (nfull > 0) {
     // Row i of the wave's fragments is four MFMAs; beside them run the fmas of
-    // row i - 1 and the reads of row i + 2. With row 6 every wave has read the
-    // whole stage and its own transfers of the next one have landed: one barrier,
-    // after which the stage is free for the transfers of block kb + 2, which so have
-    // a whole iteration to land, and the next block's first fragments are read
-    // under rows 6 and 7.
+    // row i - 1 and the reads of row i + 2. By row 1 every wave holds its fragments
+    // of B: a barrier, and B of block kb + 2 moves into their place. By row 6 it has
+    // read all of A, and its own transfers of the next block have landed (all but
+    // the four of B just begun): a barrier, A and the scales of block kb + 2 move in,
+    // and the next block's first fragments are read under rows 6 and 7. So A has
+    // one iteration to land, B one and five eighths. (Both from row 6 on: the
+    // matrix units 48 % busy, waiting for the transfers.)
     i32x8 b[4], x[4];
     f32x4 p[2][4];
     float row_scale[4], s[2] = {0.f, 0.f};
-    issue(0, 0);
+    issue_b(0, 0);
+    issue_a(0, 0);
     if (nfull > 1) {
-      issue(1, 1);
+      issue_b(1, 1);
+      issue_a(1, 1);
       __builtin_amdgcn_s_waitcnt(vm_wait(9));
     } else {
       __builtin_amdgcn_s_waitcnt(kWaitAll);
@@ -363,11 +373,19 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         __builtin_amdgcn_sched_barrier(0);
-        if (i == 6) {
-          __builtin_amdgcn_s_waitcnt(kWaitAll);
+        if (i == 1) {
+          __builtin_amdgcn_s_waitcnt(kWaitLds);
           __builtin_amdgcn_s_barrier();
           __builtin_amdgcn_sched_barrier(0);
-          if (kb + 2 < nfull) issue(kb + 2, kb & 1);
+          if (kb + 2 < nfull) issue_b(kb + 2, kb & 1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (i == 6) {
+          if (kb + 2 < nfull) __builtin_amdgcn_s_waitcnt(vm_wait(4));
+          else __builtin_amdgcn_s_waitcnt(kWaitAll);
+          __builtin_amdgcn_s_barrier();
+          __builtin_amdgcn_sched_barrier(0);
+          if (kb + 2 < nfull) issue_a(kb + 2, kb & 1);
           const uint32_t flip = (kb & 1) != 0 ? 0u - kStage : kStage;   // to the other stage
           const uint32_t flip_s = (kb & 1) != 0 ? 0u - kScales : kScales;
           a0 += flip;
