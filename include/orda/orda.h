@@ -404,7 +404,7 @@ int32_t orda_quant_fp8_blocks(int32_t device, void *hip_stream, const orda_tenso
  * bf16). a has block_rows 1, b 128. Codes whose base or pitch is no multiple of
  * 16 are copied into workspace first (256-byte aligned, the call's alone until
  * its kernels have run). Columns of codes between cols and ld are not read as
- * values. Scale strides are at least 0; a's rows' at most 2^22. */
+ * values. Scale strides are at least 0; scale_row at most 2^22. */
 int32_t orda_fp8_block_matmul_workspace(const orda_fp8_matrix *a, const orda_fp8_matrix *b, int64_t *bytes,
                                         char *err, size_t err_len);
 int32_t orda_fp8_block_matmul(int32_t device, void *hip_stream, const orda_fp8_matrix *a,

@@ -16,7 +16,7 @@ void check_matrix(const orda_fp8_matrix& m, const char* what) {
   if (m.rows == 0 || m.cols == 0) return;
   if (!m.codes || !m.scales) fail(ORDA_ERR_INVALID, "%s has a null data pointer", what);
   if (m.ld < m.cols || m.ld > kMaxPitch + 16) fail(ORDA_ERR_INVALID, "%s has a pitch out of range", what);
-  if (m.scale_row < 0 || m.scale_col < 0 || m.scale_row > (m.block_rows == 1 ? kMaxStride : kMaxRows))
+  if (m.scale_row < 0 || m.scale_col < 0 || m.scale_row > kMaxStride)
     fail(ORDA_ERR_INVALID, "%s has scale strides out of range", what);
 }
 

@@ -154,13 +154,19 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const uint8_t* src, int64
 // reach only half of a wave's 512 registers, so a wave holds 128 x 64 of C there
 // (128 registers), and a workgroup of 8 waves 256 x 256; while one of a SIMD's two
 // waves scales, the other multiplies. K advances one block at a time through two
-// 64 KB stages in LDS, moved by DMA while the other is read: rows of 128
-// bytes, their eight 16-byte chunks swizzled by row (by the choice of the chunk a
-// lane fetches). Lane group g reads chunks g and 4 + g of its row, so that the
-// lanes served together (8 rows, two neighbouring groups) meet no bank twice; with
-// chunks 2g and 2g + 1 every read took twice as long. (Which K a lane holds does
-// not matter while both operands hold the same.) The operands enter
-// the MFMA swapped: a lane then owns four consecutive columns of a row.
+// 64 KB stages in LDS, moved by DMA while the other is read: rows of 128 bytes,
+// their eight 16-byte chunks swizzled by row (by the choice of the chunk a lane
+// fetches). Lane group g reads chunks g and 4 + g of its row: a 16-byte read
+// serves lanes 0-3, 12-15 and 20-27 together, then the others of 32, and these meet
+// no bank twice; with chunks 2g and 2g + 1 every read took twice as long. (Which K
+// a lane holds does not matter while both operands hold the same.) The operands
+// enter the MFMA swapped: a lane then owns four consecutive columns of a row.
+//
+// Bound by the SIMDs' instruction and register ports: 16 cycles an MFMA, 4 a vector
+// instruction, 4 a register an LDS read returns, 47 of the 32 that the matrix unit
+// takes (this fits the loop without transfers, 3.6 ms at 8192 x 4096 x 131072,
+// without barriers too, 3.3, and without reads, 2.3, against 4.1 with all). 32x32x64
+// MFMAs, half the port time, leave too few registers to keep two pairs apart: 4.6.
 //
 // The e4m3 MFMAs (all four shapes, measured) add their products to fewer bits than
 // fp32: a sum of 128 comes out 1.5e-5 off relative to the sums' norm. Beside bf16
@@ -452,25 +458,41 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
     block(0);
   }
   // acc[i][j][e] is row m0 + wm·128 + 16i + lrow, column n0 + wn·64 + 16j + 4·lgrp + e.
+  // Rows of bf16 leave as 16 bytes a lane: a swap of neighbouring groups of 16
+  // lanes gives each eight consecutive columns of one fragment of a pair. Stored
+  // past the caches: nothing here reads them again.
   OT* const C = static_cast<OT*>(a.c);
-  const int64_t col0 = n0 + wn * 64 + 4 * lgrp;
-  const bool vec = a.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(C) % (4 * sizeof(OT)) == 0;
+  const int64_t colw = n0 + wn * 64;
+  const bool vec = n0 + kTile <= a.n && a.ldc * static_cast<int64_t>(sizeof(OT)) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(C) % 16 == 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t row = m0 + wm * 128 + i * 16 + lrow;
-    if (row >= a.m) continue;
+    OT* const d = C + row * a.ldc + colw;
+    if (vec) {
+      if constexpr (sizeof(OT) == 2) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      OT* const d = C + row * a.ldc + col0 + j * 16;
-      const f32x4 v = acc[i][j];
-      if (vec && col0 + j * 16 + 4 <= a.n) {
-        if constexpr (sizeof(OT) == 2) *reinterpret_cast<u32x2*>(d) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-        else *reinterpret_cast<f32x4*>(d) = v;
+        for (int j = 0; j < 4; j += 2) {
+          const f32x4 v = acc[i][j], w = acc[i][j + 1];
+          const auto lo = __builtin_amdgcn_permlane16_swap(pack_bf16(v[0], v[1]), pack_bf16(w[0], w[1]), false, false);
+          const auto hi = __builtin_amdgcn_permlane16_swap(pack_bf16(v[2], v[3]), pack_bf16(w[2], w[3]), false, false);
+          if (row < a.m)
+            __builtin_nontemporal_store(u32x4{lo[0], hi[0], lo[1], hi[1]},
+                                        reinterpret_cast<u32x4*>(d + 16 * (j + (lgrp & 1)) + 8 * (lgrp >> 1)));
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col0 + j * 16 + e < a.n) d[e] = static_cast<OT>(v[e]);
+        for (int j = 0; j < 4; ++j)
+          if (row < a.m) __builtin_nontemporal_store(acc[i][j], reinterpret_cast<f32x4*>(d + 16 * j + 4 * lgrp));
       }
+    } else if (row < a.m) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = 16 * j + 4 * lgrp + e;
+          if (colw + c < a.n) d[c] = static_cast<OT>(acc[i][j][e]);
+        }
     }
   }
 }
