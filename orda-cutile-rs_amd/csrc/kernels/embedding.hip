@@ -20,22 +20,21 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// kV elements of a row from p: a vector of 16 bytes (VEC), else elements 64
-// apart, of which those from column `left` on (relative to p) are 0.
-template <typename E, bool VEC>
+// A lane's kV neighbouring columns, 16 bytes of E, of which the first `left` exist.
+// The vectors need no alignment but their elements' (rows of any pitch move as
+// wide).
+template <typename E>
 struct Cols {
   static constexpr int kV = 16 / sizeof(E);
-  static constexpr int kStep = VEC ? 1 : 64;   // columns from one of a lane's elements to the next
-  static __device__ __forceinline__ int first(int lane) { return VEC ? lane * kV : lane; }
   static __device__ __forceinline__ void load(const E* p, int left, float (&x)[kV]) {
-    if constexpr (VEC) {
-      alignas(16) E w[kV];
-      *reinterpret_cast<u32x4*>(w) = *reinterpret_cast<const u32x4*>(p);
+    E w[kV];
+    if (left >= kV) {
+      __builtin_memcpy(w, p, sizeof(w));
 #pragma unroll
       for (int k = 0; k < kV; ++k) x[k] = static_cast<float>(w[k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < kV; ++k) x[k] = k * 64 < left ? static_cast<float>(p[k * 64]) : 0.f;
+      for (int k = 0; k < kV; ++k) x[k] = k < left ? static_cast<float>(p[k]) : 0.f;
     }
   }
 };
@@ -45,10 +44,10 @@ struct Cols {
 // loads in flight.
 constexpr int kLookBytes = 4096;
 
-template <typename E, typename I, bool VEC>
+template <typename E, typename I>
 __global__ __launch_bounds__(256) void embedding_kernel(const I* ids, int64_t n, const E* w, int64_t ldw, int64_t v,
                                                         int64_t h, float scale, E* out, int64_t ldo, int64_t parts) {
-  constexpr int kV = 16 / sizeof(E);
+  constexpr int kV = 16 / sizeof(E), kLoads = kLookBytes / 1024;
   constexpr int kCols = kLookBytes / sizeof(E);
   const int lane = threadIdx.x & 63;
   const int64_t unit = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
@@ -60,25 +59,24 @@ __global__ __launch_bounds__(256) void embedding_kernel(const I* ids, int64_t n,
   const E* s = w + (ok ? id : 0) * ldw + c0;
   E* d = out + t * ldo + c0;
   const int cols = static_cast<int>(h - c0 < kCols ? h - c0 : kCols);
-  if constexpr (VEC) {
-    u32x4 x[kCols / (64 * kV)];
+  E x[kLoads][kV];
 #pragma unroll
-    for (int i = 0; i < kCols / (64 * kV); ++i) {
-      const int c = (i * 64 + lane) * kV;
-      if (c + kV <= cols) x[i] = *reinterpret_cast<const u32x4*>(s + c);
+  for (int i = 0; i < kLoads; ++i) {
+    const int c = (i * 64 + lane) * kV;
+    if (ok && c + kV <= cols) __builtin_memcpy(x[i], s + c, sizeof(x[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int c = (i * 64 + lane) * kV;
+    if (c + kV <= cols) {
+#pragma unroll
+      for (int k = 0; k < kV; ++k)
+        x[i][k] = ok ? static_cast<E>(static_cast<float>(x[i][k]) * scale) : static_cast<E>(NAN);
+      __builtin_memcpy(d + c, x[i], sizeof(x[i]));
+    } else {
+      for (int k = 0; k < kV && c + k < cols; ++k)
+        d[c + k] = ok ? static_cast<E>(static_cast<float>(s[c + k]) * scale) : static_cast<E>(NAN);
     }
-#pragma unroll
-    for (int i = 0; i < kCols / (64 * kV); ++i) {
-      const int c = (i * 64 + lane) * kV;
-      alignas(16) E e[kV];
-      *reinterpret_cast<u32x4*>(e) = x[i];
-#pragma unroll
-      for (int k = 0; k < kV; ++k) e[k] = ok ? static_cast<E>(static_cast<float>(e[k]) * scale) : static_cast<E>(NAN);
-      if (c + kV <= cols) *reinterpret_cast<u32x4*>(d + c) = *reinterpret_cast<const u32x4*>(e);
-    }
-  } else {
-    for (int c = lane; c < cols; c += 64)
-      d[c] = ok ? static_cast<E>(static_cast<float>(s[c]) * scale) : static_cast<E>(NAN);
   }
 }
 
@@ -106,6 +104,7 @@ __global__ __launch_bounds__(256) void embed_rank_kernel(const I* ids, int n, in
   if (i >= n) return;
   const uint32_t me = all[i];
   uint32_t before = 0;
+#pragma unroll 8
   for (int j = 0; j < n4; j += 4) {
     const u32x4 o = *reinterpret_cast<const u32x4*>(all + j);
 #pragma unroll
@@ -246,93 +245,73 @@ __device__ __forceinline__ int64_t first_at_least(const uint32_t* keys, int64_t 
   return lo;
 }
 
-// One wave's columns of a gradient row, scaled and rounded (added to what is
-// there with acc). O's stores are 8 or 16 bytes a lane where VEC.
-template <typename E, typename O, bool VEC>
-__device__ __forceinline__ void put_row(const EmbedGradArgs& a, int64_t row, int64_t c0, int lane,
-                                        const float (&x)[Cols<E, VEC>::kV]) {
-  using C = Cols<E, VEC>;
-  O* d = static_cast<O*>(a.out) + row * a.ldo + c0 + C::first(lane);
-  const int left = static_cast<int>(a.h - c0) - C::first(lane);
-  if constexpr (VEC) {
-    if (left < C::kV) return;
-    constexpr int kB = C::kV * sizeof(O) / 16;   // 16-byte vectors, 0: one of 8 bytes
-    alignas(16) O o[C::kV];
-    if (a.accumulate) {
-      if constexpr (kB == 0) *reinterpret_cast<uint64_t*>(o) = *reinterpret_cast<const uint64_t*>(d);
+// One lane's columns of a gradient row from column c on, scaled and rounded (added
+// to what is there with accumulate).
+template <typename E, typename O>
+__device__ __forceinline__ void put_row(const EmbedGradArgs& a, int64_t row, int64_t c, const float (&x)[Cols<E>::kV]) {
+  constexpr int kV = Cols<E>::kV;
+  O* d = static_cast<O*>(a.out) + row * a.ldo + c;
+  const int left = static_cast<int>(a.h - c);
+  if (left >= kV) {
+    O o[kV];
+    if (a.accumulate) __builtin_memcpy(o, d, sizeof(o));
 #pragma unroll
-      for (int b = 0; b < kB; ++b) reinterpret_cast<u32x4*>(o)[b] = reinterpret_cast<const u32x4*>(d)[b];
-    }
-#pragma unroll
-    for (int k = 0; k < C::kV; ++k) {
+    for (int k = 0; k < kV; ++k) {
       const float s = x[k] * a.scale;
       o[k] = static_cast<O>(a.accumulate ? static_cast<float>(o[k]) + s : s);
     }
-    if constexpr (kB == 0) *reinterpret_cast<uint64_t*>(d) = *reinterpret_cast<const uint64_t*>(o);
-#pragma unroll
-    for (int b = 0; b < kB; ++b) reinterpret_cast<u32x4*>(d)[b] = reinterpret_cast<const u32x4*>(o)[b];
+    __builtin_memcpy(d, o, sizeof(o));
   } else {
 #pragma unroll
-    for (int k = 0; k < C::kV; ++k)
-      if (k * 64 < left) {
+    for (int k = 0; k < kV; ++k)
+      if (k < left) {
         const float s = x[k] * a.scale;
-        d[k * 64] = static_cast<O>(a.accumulate ? static_cast<float>(d[k * 64]) + s : s);
+        d[k] = static_cast<O>(a.accumulate ? static_cast<float>(d[k]) + s : s);
       }
   }
 }
 
 // Partial sums of a chunk: its first sum where an earlier chunk began it (slot
-// 0), its last where it goes on (slot 1; slot 0 where it is the first too).
-template <typename E, bool VEC>
-__device__ __forceinline__ float* partial(const EmbedGradArgs& a, int64_t chunk, int slot, int64_t c0, int lane) {
-  return a.parts + (chunk * 2 + slot) * a.ldp + c0 + Cols<E, VEC>::first(lane);
+// 0), its last where it goes on (slot 1; slot 0 where it is the first too). Their
+// rows hold whole waves' columns.
+__device__ __forceinline__ float* partial(const EmbedGradArgs& a, int64_t chunk, int slot, int64_t c) {
+  return a.parts + (chunk * 2 + slot) * a.ldp + c;
 }
-template <typename E, bool VEC>
-__device__ __forceinline__ void put_partial(float* d, const float (&x)[Cols<E, VEC>::kV]) {
-  constexpr int kV = Cols<E, VEC>::kV;   // scratch rows hold whole columns of waves
+template <int kV>
+__device__ __forceinline__ void put_partial(float* d, const float (&x)[kV]) {
 #pragma unroll
-  for (int k = 0; k < kV; k += VEC ? 4 : 1) {
-    if constexpr (VEC) *reinterpret_cast<f32x4*>(d + k) = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]};
-    else d[k * 64] = x[k];
-  }
+  for (int k = 0; k < kV; k += 4) *reinterpret_cast<f32x4*>(d + k) = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]};
 }
-template <typename E, bool VEC>
-__device__ __forceinline__ void add_partial(const float* s, float (&x)[Cols<E, VEC>::kV]) {
-  constexpr int kV = Cols<E, VEC>::kV;
+template <int kV>
+__device__ __forceinline__ void add_partial(const float* s, float (&x)[kV]) {
 #pragma unroll
-  for (int k = 0; k < kV; k += VEC ? 4 : 1) {
-    if constexpr (VEC) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(s + k);
+  for (int k = 0; k < kV; k += 4) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(s + k);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) x[k + q] += v[q];
-    } else {
-      x[k] += s[k * 64];
-    }
+    for (int q = 0; q < 4; ++q) x[k + q] += v[q];
   }
 }
 
 // Waves [0, chunks·slabs): the sums of a chunk of sorted pairs, kLoads rows in
 // flight. The waves after them zero the rows no pair names, fill_rows
 // consecutive ones each, found by one search of the sorted keys.
-template <typename E, typename O, bool VEC>
+template <typename E, typename O>
 __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
-  using C = Cols<E, VEC>;
-  constexpr int kV = C::kV, kLoads = 8;
+  constexpr int kV = Cols<E>::kV, kLoads = 8;
   const int lane = threadIdx.x & 63;
   const int64_t unit = blockIdx.x * int64_t{4} + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (unit < a.chunks * a.slabs) {
-    const int64_t chunk = unit / a.slabs, c0 = (unit - chunk * a.slabs) * (64 * kV);
+    const int64_t chunk = unit / a.slabs, c = (unit - chunk * a.slabs) * (64 * kV) + lane * kV;
     const int64_t b = chunk * a.chunk, e = b + a.chunk < a.n ? b + a.chunk : a.n;
-    const int left = static_cast<int>(a.h - c0) - C::first(lane);
-    const E* src = static_cast<const E*>(a.grad) + c0 + C::first(lane);
-    const bool on = VEC ? left >= kV : left > 0;
+    const int left = static_cast<int>(a.h - c);
+    const E* src = static_cast<const E*>(a.grad) + c;
     float x[kV] = {};
     uint32_t key = a.keys[b];
     bool head = b > 0 && a.keys[b - 1] == key;   // the sum began in an earlier chunk
     auto flush = [&](bool tail) {   // tail: it goes on in the next one
       if (static_cast<int64_t>(key) < a.v) {
-        if (head || tail) put_partial<E, VEC>(partial<E, VEC>(a, chunk, head ? 0 : 1, c0, lane), x);
-        else put_row<E, O, VEC>(a, key, c0, lane, x);
+        if (head || tail) put_partial(partial(a, chunk, head ? 0 : 1, c), x);
+        else if (left > 0) put_row<E, O>(a, key, c, x);
       }
 #pragma unroll
       for (int k = 0; k < kV; ++k) x[k] = 0.f;
@@ -346,8 +325,8 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
         const int64_t j = i + q < e ? i + q : e - 1;
         ks[q] = a.keys[j];
         const int64_t r = a.vals[j];
-        if (on && static_cast<int64_t>(ks[q]) < a.v) {
-          C::load(src + r * a.ldg, left, y[q]);
+        if (static_cast<int64_t>(ks[q]) < a.v) {
+          Cols<E>::load(src + r * a.ldg, left, y[q]);
         } else {
 #pragma unroll
           for (int k = 0; k < kV; ++k) y[q][k] = 0.f;
@@ -379,12 +358,13 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
     const int64_t next = at < a.n && static_cast<int64_t>(a.keys[at]) < r1 ? a.keys[at] : r1;
     for (; r < next; ++r) {
       O* d = static_cast<O*>(a.out) + r * a.ldo;
-      if (VEC) {
-        constexpr int kO = 16 / sizeof(O);
-        for (int64_t c = lane * kO; c < a.h; c += 64 * kO) *reinterpret_cast<u32x4*>(d + c) = u32x4{0, 0, 0, 0};
-      } else {
-        for (int64_t c = lane; c < a.h; c += 64) d[c] = static_cast<O>(0.f);
+      constexpr int kO = 16 / sizeof(O);
+      int64_t c = lane * kO;
+      for (; c + kO <= a.h; c += 64 * kO) {
+        const O z[kO] = {};
+        __builtin_memcpy(d + c, z, sizeof(z));
       }
+      for (int k = 0; k < kO && c + k < a.h; ++k) d[c + k] = static_cast<O>(0.f);
     }
     if (r >= r1) break;
     // past the pairs of row r
@@ -396,14 +376,13 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
 
 // Sums that a chunk begins and a later one ends, a wave for each chunk and its
 // columns: the parts in order.
-template <typename E, typename O, bool VEC>
+template <typename E, typename O>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradArgs a) {
-  using C = Cols<E, VEC>;
-  constexpr int kV = C::kV;
+  constexpr int kV = Cols<E>::kV;
   const int lane = threadIdx.x & 63;
   const int64_t unit = blockIdx.x * int64_t{4} + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (unit >= (a.chunks - 1) * a.slabs) return;
-  const int64_t chunk = unit / a.slabs, c0 = (unit - chunk * a.slabs) * (64 * kV);
+  const int64_t chunk = unit / a.slabs, c = (unit - chunk * a.slabs) * (64 * kV) + lane * kV;
   const int64_t b = chunk * a.chunk, e = b + a.chunk;   // not the last chunk: whole
   const uint32_t key = a.keys[e - 1];
   if (static_cast<int64_t>(key) >= a.v || a.keys[e] != key) return;    // nothing goes on
@@ -412,23 +391,19 @@ __global__ __launch_bounds__(256) void embed_join_kernel(EmbedGradArgs a) {
   const int64_t end = first_at_least(a.keys, a.n, key + 1, lane);
   const int64_t last = (end - 1) / a.chunk;
   float x[kV] = {};
-  add_partial<E, VEC>(partial<E, VEC>(a, chunk, 1, c0, lane), x);
+  add_partial(partial(a, chunk, 1, c), x);
   int64_t j = chunk + 1;
-  for (; j + 3 <= last; j += 4) {   // four loads in flight, added in order
-    float y[4][kV] = {};
+  for (; j + 7 <= last; j += 8) {   // eight loads in flight, added in order
+    float y[8][kV] = {};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) add_partial<E, VEC>(partial<E, VEC>(a, j + q, 0, c0, lane), y[q]);
+    for (int q = 0; q < 8; ++q) add_partial(partial(a, j + q, 0, c), y[q]);
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < 8; ++q)
 #pragma unroll
       for (int k = 0; k < kV; ++k) x[k] += y[q][k];
   }
-  for (; j <= last; ++j) add_partial<E, VEC>(partial<E, VEC>(a, j, 0, c0, lane), x);
-  put_row<E, O, VEC>(a, key, c0, lane, x);
-}
-
-bool aligned16(const void* p, int64_t ld, int64_t h, int64_t es) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0 && h * es % 16 == 0;
+  for (; j <= last; ++j) add_partial(partial(a, j, 0, c), x);
+  if (c < a.h) put_row<E, O>(a, key, c, x);
 }
 
 int passes_of(int64_t v) {   // digits of keys 0..v
@@ -448,15 +423,13 @@ hipError_t launch_embedding(DType t, const void* ids, bool ids64, int64_t n, con
                             int64_t h, float scale, void* out, int64_t ldo, hipStream_t stream) {
   if (n <= 0 || h <= 0) return hipSuccess;
   const int64_t es = dtype_size(t);
-  const bool vec = aligned16(w, ldw, h, es) && aligned16(out, ldo, h, es);
   const int64_t parts = (h * es + kLookBytes - 1) / kLookBytes;
   const int64_t blocks = (n * parts + 3) / 4;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   auto run = [&](auto* e, auto* i) {
     using E = std::remove_pointer_t<decltype(e)>;
     using I = std::remove_pointer_t<decltype(i)>;
-    auto* k = vec ? embedding_kernel<E, I, true> : embedding_kernel<E, I, false>;
-    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, static_cast<const I*>(ids), n,
+    hipLaunchKernelGGL((embedding_kernel<E, I>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, static_cast<const I*>(ids), n,
                        static_cast<const E*>(w), ldw, v, h, scale, static_cast<E*>(out), ldo, parts);
   };
   int64_t* i64 = nullptr;
@@ -526,7 +499,6 @@ hipError_t launch_embed_sort(const void* ids, bool ids64, int64_t n, int64_t v, 
 }
 
 hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t stream) {
-  const bool vec = aligned16(a.grad, a.ldg, a.h, dtype_size(grad)) && aligned16(a.out, a.ldo, a.h, dtype_size(out));
   // rows a wave zeroes: enough waves to fill the chip, at most 64 rows each
   a.fill_rows = a.v / 8192 < 1 ? 1 : a.v / 8192 > 64 ? 64 : a.v / 8192;
   const int64_t fill = a.accumulate ? 0 : (a.v + a.fill_rows - 1) / a.fill_rows;
@@ -535,10 +507,8 @@ hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t
   auto run = [&](auto* e, auto* o) {
     using E = std::remove_pointer_t<decltype(e)>;
     using O = std::remove_pointer_t<decltype(o)>;
-    auto* k = vec ? embed_sum_kernel<E, O, true> : embed_sum_kernel<E, O, false>;
-    auto* j = vec ? embed_join_kernel<E, O, true> : embed_join_kernel<E, O, false>;
-    if (sum > 0) hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(sum)), dim3(256), 0, stream, a);
-    if (join > 0) hipLaunchKernelGGL(j, dim3(static_cast<unsigned>(join)), dim3(256), 0, stream, a);
+    if (sum > 0) hipLaunchKernelGGL((embed_sum_kernel<E, O>), dim3(static_cast<unsigned>(sum)), dim3(256), 0, stream, a);
+    if (join > 0) hipLaunchKernelGGL((embed_join_kernel<E, O>), dim3(static_cast<unsigned>(join)), dim3(256), 0, stream, a);
   };
   __bf16* b = nullptr;
   float* f = nullptr;

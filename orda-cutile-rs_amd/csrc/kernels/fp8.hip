@@ -21,8 +21,9 @@ typedef __attribute__((address_space(3))) const float lds_f32;
 // scale = max(amax / 448, 2^-126), code = x / scale rounded to nearest even, both
 // quotients in fp32: |x / scale| is at most 448 but for its rounding, which the
 // clamp takes back. A block with an infinity or a NaN has the scale NaN and codes
-// NaN. Bound by HBM (each value is read once into registers; the two IEEE
-// divisions cost about as long as the bytes of bf16 values).
+// NaN. Bound by HBM, each value being read once into registers: the quotient is a
+// product with the reciprocal wherever that cannot change the code (`doubtful`),
+// an IEEE division for every value took twice as long.
 constexpr float kE4m3Max = 448.f;
 
 __device__ __forceinline__ float scale_of(uint32_t amax_bits) {
@@ -33,9 +34,29 @@ __device__ __forceinline__ float coded(float x, float s) {
   const float q = x / s;
   return q != q ? q : fminf(fmaxf(q, -kE4m3Max), kE4m3Max);
 }
-__device__ __forceinline__ uint32_t codes4(const float* x, float s) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(coded(x[0], s), coded(x[1], s), 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(coded(x[2], s), coded(x[3], s), w, true);
+// Whether x / s might round to another code than q = x * (1/s), which is at most 3
+// units in the last place off the rounded quotient: near a midpoint of two
+// codes (three bits of mantissa are kept: the other 20 near one half), or below
+// the smallest normal code, where the midpoints lie elsewhere.
+__device__ __forceinline__ bool doubtful(float q) {
+  const uint32_t u = __float_as_uint(q) & 0x7fffffffu;
+  return (u & 0xfffffu) - 0x7fffcu <= 8u || (u < 0x3c800004u && u != 0u) || u >= 0x7f800000u;
+}
+__device__ __forceinline__ uint32_t codes4(const float* x, float s, float r) {
+  float q[4];
+  bool doubt = false;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    q[k] = x[k] * r;
+    doubt |= doubtful(q[k]);
+    q[k] = fminf(fmaxf(q[k], -kE4m3Max), kE4m3Max);
+  }
+  if (doubt) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[k] = coded(x[k], s);
+  }
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
   return static_cast<uint32_t>(w);
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -56,7 +77,8 @@ __device__ __forceinline__ void load8(const E* row, int64_t c, int64_t cols, flo
 }
 // Their codes, the eight that hold the last column whole.
 __device__ __forceinline__ void store8(uint8_t* row, int64_t c, int64_t cols, const float (&x)[8], float s) {
-  if (c < cols) *reinterpret_cast<u32x2*>(row + c) = u32x2{codes4(x, s), codes4(x + 4, s)};
+  const float r = __builtin_amdgcn_rcpf(s);
+  if (c < cols) *reinterpret_cast<u32x2*>(row + c) = u32x2{codes4(x, s, r), codes4(x + 4, s, r)};
 }
 
 // Blocks of one row: 16 lanes a block of 128, a wave 4 blocks of each of 4 rows,
@@ -497,6 +519,169 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
   }
 }
 
+// ------------------------------------------------------------ few rows
+// Up to 64 rows of A (a token, a small batch): bound by the bytes of B, which
+// each go once from memory to the registers of one wave, with no LDS and no
+// barrier. A wave takes 16·R rows of B and all rows of A (F fragments of 16, from the
+// caches), loads the next U blocks while it multiplies these, and scales as above.
+// R = 4, U = 1 (8 KB of B in flight a wave) where that leaves every CU four waves;
+// else R = 1, U = 2. One row at 131072 x 4096: 142 us on the tiles.
+template <typename OT, bool WIDE, int F, int R, int U>
+__global__ __launch_bounds__(256) void fp8_few_kernel(Fp8MmArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n0 = (blockIdx.x * int64_t{4} + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * (16 * R);
+  if (n0 >= a.n) return;
+  const int lrow = lane & 15, lgrp = lane >> 4;
+  const unsigned char *pa[F], *pb[R];
+  const float* sa[F];
+#pragma unroll
+  for (int i = 0; i < F; ++i) {
+    const int64_t r = i * 16 + lrow < a.m ? i * 16 + lrow : a.m - 1;   // the last row again: not stored
+    pa[i] = a.a + r * a.lda + lgrp * 16;
+    sa[i] = a.sa + r * a.sa_row;
+  }
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int64_t r = n0 + j * 16 + lrow < a.n ? n0 + j * 16 + lrow : a.n - 1;
+    pb[j] = a.b + r * a.ldb + lgrp * 16;
+  }
+  const float* const sb = a.sb + n0 / 128 * a.sb_row;
+  f32x4 acc[F][R];
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Block {
+    i32x8 a[F], b[R];
+    float s[F];
+  };
+  // Chunks lgrp and 4 + lgrp of a row's block kb (as on the tiles).
+  auto chunk = [&](const unsigned char* p, int64_t kb) {
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(p + kb * 128);
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(p + kb * 128 + 64);
+    return __builtin_bit_cast(i32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  auto load = [&](Block& w, int64_t kb) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) w.b[j] = chunk(pb[j], kb);
+#pragma unroll
+    for (int i = 0; i < F; ++i) w.a[i] = chunk(pa[i], kb);
+    const float s_b = sb[kb * a.sb_col];
+#pragma unroll
+    for (int i = 0; i < F; ++i) w.s[i] = s_b * sa[i][kb * a.sa_col];
+  };
+  auto use = [&](const Block& w) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      if constexpr (WIDE) {
+        const Wide n = widened(w.b[j]);
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+          const Wide m = widened(w.a[i]);
+          f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(n.k[q], m.k[q], p, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(w.s[i], p[e], acc[i][j][e]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+          const f32x4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.b[j], w.a[i], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0,
+                                                                           0, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(w.s[i], p[e], acc[i][j][e]);
+        }
+      }
+    }
+  };
+  const int64_t nfull = a.k / 128;
+  int64_t kb = 0;
+  if (nfull >= 2 * U) {
+    Block w[2][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(w[0][u], u);
+    for (; kb + 3 * U <= nfull; kb += 2 * U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) load(w[1][u], kb + U + u);
+#pragma unroll
+      for (int u = 0; u < U; ++u) use(w[0][u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) load(w[0][u], kb + 2 * U + u < nfull ? kb + 2 * U + u : nfull - 1);
+#pragma unroll
+      for (int u = 0; u < U; ++u) use(w[1][u]);
+    }
+    // w[0] holds blocks kb .. kb + U - 1, where they exist
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (kb + u < nfull) use(w[0][u]);
+    kb = kb + U < nfull ? kb + U : nfull;
+  }
+  for (; kb < nfull; ++kb) {
+    Block w;
+    load(w, kb);
+    use(w);
+  }
+  const int krem = static_cast<int>(a.k - nfull * 128);
+  if (krem > 0) {   // the partial block: zeros past K
+    auto part = [&](const unsigned char* p) {
+      alignas(16) unsigned char b[32];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = lgrp * 16 + h * 64;
+        const unsigned char* q = p + nfull * 128 + h * 64;
+        if (c + 16 <= krem) {
+          *reinterpret_cast<u32x4*>(b + h * 16) = *reinterpret_cast<const u32x4*>(q);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) b[h * 16 + k] = c + k < krem ? q[k] : 0;
+        }
+      }
+      i32x8 r;
+      __builtin_memcpy(&r, b, 32);
+      return r;
+    };
+    Block w;
+#pragma unroll
+    for (int j = 0; j < R; ++j) w.b[j] = part(pb[j]);
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      w.a[i] = part(pa[i]);
+      w.s[i] = sb[nfull * a.sb_col] * sa[i][nfull * a.sa_col];
+    }
+    use(w);
+  }
+  OT* const C = static_cast<OT*>(a.c);
+  const bool vec = a.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(C) % (4 * sizeof(OT)) == 0;
+#pragma unroll
+  for (int i = 0; i < F; ++i) {
+    const int64_t row = i * 16 + lrow;
+    if (row >= a.m) continue;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int64_t col = n0 + j * 16 + 4 * lgrp;
+      OT* const d = C + row * a.ldc + col;
+      const f32x4 v = acc[i][j];
+      if (vec && col + 4 <= a.n) {
+        if constexpr (sizeof(OT) == 2) *reinterpret_cast<u32x2*>(d) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+        else *reinterpret_cast<f32x4*>(d) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < a.n) d[e] = static_cast<OT>(v[e]);
+      }
+    }
+  }
+}
+
+constexpr int64_t kFewRows = 64;
+template <typename OT, bool WIDE>
+void (*few_kernel(int64_t m, bool wide_rows))(Fp8MmArgs) {
+  if (m <= 16) return wide_rows ? fp8_few_kernel<OT, WIDE, 1, 4, 1> : fp8_few_kernel<OT, WIDE, 1, 1, 2>;
+  if (m <= 32) return wide_rows ? fp8_few_kernel<OT, WIDE, 2, 4, 1> : fp8_few_kernel<OT, WIDE, 2, 1, 2>;
+  return wide_rows ? fp8_few_kernel<OT, WIDE, 4, 4, 1> : fp8_few_kernel<OT, WIDE, 4, 1, 2>;
+}
+
 }  // namespace
 
 hipError_t launch_fp8_quant(const Fp8QuantArgs& a, DType t, bool blocks, hipStream_t stream) {
@@ -526,6 +711,13 @@ hipError_t launch_fp8_mm(const Fp8MmArgs& a, DType out, hipStream_t stream) {
   if (a.lda % 16 != 0 || a.ldb % 16 != 0 || reinterpret_cast<uintptr_t>(a.a) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(a.b) % 16 != 0)
     return hipErrorInvalidValue;
+  if (a.m <= kFewRows) {
+    const bool wide_rows = (a.n + 63) / 64 >= 4 * 256;
+    const int64_t waves = (a.n + (wide_rows ? 63 : 15)) / (wide_rows ? 64 : 16);
+    auto* k = out == DType::BF16 ? few_kernel<__bf16, false>(a.m, wide_rows) : few_kernel<float, true>(a.m, wide_rows);
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, stream, a);
+    return hipGetLastError();
+  }
   const int64_t tiles = (a.m + kTile - 1) / kTile * ((a.n + kTile - 1) / kTile);
   if (tiles > 0x7fffffff) return hipErrorInvalidValue;
   auto* k = out == DType::BF16 ? fp8_mm_kernel<__bf16, false> : fp8_mm_kernel<float, true>;

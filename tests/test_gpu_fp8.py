@@ -115,6 +115,46 @@ def test_product(m, k, n, out):
     check_product(got, a, sa, b, sb)
 
 
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("m", [1, 15, 17, 33, 63, 64, 65])
+@pytest.mark.parametrize("k, n", [(100, 40), (256, 1000), (384, 700), (640, 66001), (900, 66001), (1160, 33)])
+def test_product_of_few_rows(m, k, n, out):
+    """Up to 64 rows, at few and many columns, whole and partial blocks of K, an
+    even and an odd number of them."""
+    x, w = normal(m, k), normal(n, k, seed=1, std=0.1)
+    a, sa = H.quantize_fp8_blocks(x)
+    b, sb = H.quantize_fp8_blocks(w, block_rows=128)
+    check_product(H.fp8_block_matmul(a, sa, b, sb, out_dtype=DT[out]), a, sa, b, sb)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantiser_near_midpoints(dtype):
+    """Quotients at and next to the midpoints of two codes, normal and subnormal,
+    where the rounded quotient decides."""
+    codes = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    mid = (codes[1:] + codes[:-1]) / 2
+    rows = []
+    for top in (448.0, 447.0, 1.0, 3.7, 1e-3, 12345.0, 2.0 ** -100, 2.0 ** 90):
+        s = (torch.tensor(top, dtype=torch.float32) / torch.tensor(448.0)).double()
+        v = (mid * s).to(DT[dtype])
+        near = [v]
+        for d in (1, -1, 2, -2, 3, -3):   # neighbours in the input's type
+            near.append((v.view(torch.int16 if dtype == "bf16" else torch.int32) + d).view(DT[dtype]))
+        flat = torch.cat(near)
+        flat = flat[flat.abs().double() <= top]
+        for part in flat.split(127):
+            row = torch.zeros(128, dtype=DT[dtype])
+            row[0] = top
+            row[1:1 + len(part)] = part * (1 - 2 * (torch.arange(len(part)) % 2)).to(DT[dtype])
+            rows.append(row)
+    m = torch.stack(rows).cuda()
+    for block_rows in (1,):
+        got, scales = H.quantize_fp8_blocks(m, block_rows=block_rows)
+        want, s = quantized(m, block_rows)
+        assert torch.equal(scales.cpu(), s)
+        same_codes(got, want)
+
+
 @pytest.mark.parametrize("k", [128, 1000, 1500])
 def test_product_layouts(k):
     """Contiguous codes (pitches that are no multiple of 16 are copied), column
