@@ -20,23 +20,11 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// A lane's kV neighbouring columns, 16 bytes of E, of which the first `left` exist.
-// The vectors need no alignment but their elements' (rows of any pitch move as
-// wide).
+// Columns of a wave's lane, 16 bytes of E. The vectors need no alignment but their
+// elements' (rows of any pitch move as wide).
 template <typename E>
 struct Cols {
   static constexpr int kV = 16 / sizeof(E);
-  static __device__ __forceinline__ void load(const E* p, int left, float (&x)[kV]) {
-    E w[kV];
-    if (left >= kV) {
-      __builtin_memcpy(w, p, sizeof(w));
-#pragma unroll
-      for (int k = 0; k < kV; ++k) x[k] = static_cast<float>(w[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kV; ++k) x[k] = k < left ? static_cast<float>(p[k]) : 0.f;
-    }
-  }
 };
 
 // ------------------------------------------------------------ lookup
@@ -60,10 +48,12 @@ __global__ __launch_bounds__(256) void embedding_kernel(const I* ids, int64_t n,
   E* d = out + t * ldo + c0;
   const int cols = static_cast<int>(h - c0 < kCols ? h - c0 : kCols);
   E x[kLoads][kV];
+  if (ok) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int c = (i * 64 + lane) * kV;
-    if (ok && c + kV <= cols) __builtin_memcpy(x[i], s + c, sizeof(x[i]));
+    for (int i = 0; i < kLoads; ++i) {
+      const int c = (i * 64 + lane) * kV;
+      if (c + kV <= cols) __builtin_memcpy(x[i], s + c, sizeof(x[i]));
+    }
   }
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
@@ -245,6 +235,26 @@ __device__ __forceinline__ int64_t first_at_least(const uint32_t* keys, int64_t 
   return lo;
 }
 
+// 16 bytes, past the caches with `stream`: the gradient of a large vocabulary
+// (EmbedGradArgs::stream) is not read again before gigabytes of other traffic, and
+// displaces the rows still to be read. (8192 x 4096 into 131072 rows of bf16: 198
+// us against 224, 65536 tokens 610 with the join against 630.)
+__device__ __forceinline__ void put16(void* d, u32x4 v, bool stream) {
+  if (stream && reinterpret_cast<uintptr_t>(d) % 16 == 0) __builtin_nontemporal_store(v, static_cast<u32x4*>(d));
+  else __builtin_memcpy(d, &v, 16);
+}
+
+// A wave zeroes a row: 16-byte vectors from the first aligned address on.
+template <typename O>
+__device__ __forceinline__ void zero_row(O* d, int64_t h, int lane, bool stream) {
+  constexpr int kO = 16 / sizeof(O);
+  const int64_t skew = (16 - reinterpret_cast<uintptr_t>(d) % 16) % 16 / sizeof(O), head = skew < h ? skew : h;
+  if (lane < head) d[lane] = static_cast<O>(0.f);
+  int64_t c = head + lane * kO;
+  for (; c + kO <= h; c += 64 * kO) put16(d + c, u32x4{0, 0, 0, 0}, stream);
+  for (int k = 0; k < kO && c + k < h; ++k) d[c + k] = static_cast<O>(0.f);
+}
+
 // One lane's columns of a gradient row from column c on, scaled and rounded (added
 // to what is there with accumulate).
 template <typename E, typename O>
@@ -260,7 +270,16 @@ __device__ __forceinline__ void put_row(const EmbedGradArgs& a, int64_t row, int
       const float s = x[k] * a.scale;
       o[k] = static_cast<O>(a.accumulate ? static_cast<float>(o[k]) + s : s);
     }
-    __builtin_memcpy(d, o, sizeof(o));
+    if constexpr (sizeof(o) % 16 == 0) {
+#pragma unroll
+      for (int k = 0; k < static_cast<int>(sizeof(o)) / 16; ++k) {
+        u32x4 w;
+        __builtin_memcpy(&w, o + k * (16 / sizeof(O)), 16);
+        put16(d + k * (16 / sizeof(O)), w, a.stream);
+      }
+    } else {
+      __builtin_memcpy(d, o, sizeof(o));
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < kV; ++k)
@@ -318,19 +337,23 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
       head = false;
     };
     for (int64_t i = b; i < e; i += kLoads) {
-      float y[kLoads][kV];
+      E w[kLoads][kV];
       uint32_t ks[kLoads];
+      int64_t at[kLoads];
 #pragma unroll
       for (int q = 0; q < kLoads; ++q) {
         const int64_t j = i + q < e ? i + q : e - 1;
         ks[q] = a.keys[j];
-        const int64_t r = a.vals[j];
-        if (static_cast<int64_t>(ks[q]) < a.v) {
-          Cols<E>::load(src + r * a.ldg, left, y[q]);
-        } else {
+        at[q] = a.vals[j] * a.ldg;   // (a row without a gradient is read, not added)
+      }
+      if (left >= kV) {   // one branch for all rows: around each load it made them wait for one another
 #pragma unroll
-          for (int k = 0; k < kV; ++k) y[q][k] = 0.f;
-        }
+        for (int q = 0; q < kLoads; ++q) __builtin_memcpy(w[q], src + at[q], sizeof(w[q]));
+      } else {
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q)
+#pragma unroll
+          for (int k = 0; k < kV; ++k) w[q][k] = k < left ? src[at[q] + k] : static_cast<E>(0.f);
       }
 #pragma unroll
       for (int q = 0; q < kLoads; ++q) {
@@ -340,7 +363,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
             key = ks[q];
           }
 #pragma unroll
-          for (int k = 0; k < kV; ++k) x[k] += y[q][k];
+          for (int k = 0; k < kV; ++k) x[k] += static_cast<float>(w[q][k]);
         }
       }
     }
@@ -357,14 +380,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
     // rows up to the next key are zero
     const int64_t next = at < a.n && static_cast<int64_t>(a.keys[at]) < r1 ? a.keys[at] : r1;
     for (; r < next; ++r) {
-      O* d = static_cast<O*>(a.out) + r * a.ldo;
-      constexpr int kO = 16 / sizeof(O);
-      int64_t c = lane * kO;
-      for (; c + kO <= a.h; c += 64 * kO) {
-        const O z[kO] = {};
-        __builtin_memcpy(d + c, z, sizeof(z));
-      }
-      for (int k = 0; k < kO && c + k < a.h; ++k) d[c + k] = static_cast<O>(0.f);
+      zero_row(static_cast<O*>(a.out) + r * a.ldo, a.h, lane, a.stream);
     }
     if (r >= r1) break;
     // past the pairs of row r
@@ -444,8 +460,8 @@ hipError_t launch_embedding(DType t, const void* ids, bool ids64, int64_t n, con
 EmbedScratch embed_scratch(DType grad, int64_t n, int64_t v, int64_t h) {
   EmbedScratch s{};
   const int64_t cols = 64 * 16 / dtype_size(grad);   // of a wave
-  s.chunk = 32;
-  while (s.chunk < 256 && n / s.chunk > 4096) s.chunk *= 2;
+  s.chunk = 32;   // pairs a wave sums: enough waves of few tokens, few joins of many
+  while (s.chunk < 256 && n / s.chunk > 1024) s.chunk *= 2;
   s.chunks = (n + s.chunk - 1) / s.chunk;
   s.slabs = (h + cols - 1) / cols;
   s.ldp = s.slabs * cols;
@@ -499,6 +515,10 @@ hipError_t launch_embed_sort(const void* ids, bool ids64, int64_t n, int64_t v, 
 }
 
 hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t stream) {
+  // more than the last cache holds, and rows of whole lines (a line two rows share
+  // would go to memory twice)
+  const int64_t row = a.ldo * dtype_size(out);
+  a.stream = a.v * row > int64_t{256} << 20 && row % 128 == 0 && reinterpret_cast<uintptr_t>(a.out) % 128 == 0;
   // rows a wave zeroes: enough waves to fill the chip, at most 64 rows each
   a.fill_rows = a.v / 8192 < 1 ? 1 : a.v / 8192 > 64 ? 64 : a.v / 8192;
   const int64_t fill = a.accumulate ? 0 : (a.v + a.fill_rows - 1) / a.fill_rows;

@@ -61,19 +61,27 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float s, float r) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Eight values of a row from column c on (0 past cols). The vectors need no
-// alignment but their elements': rows of any pitch load as wide.
-template <typename E>
-__device__ __forceinline__ void load8(const E* row, int64_t c, int64_t cols, float (&x)[8]) {
-  if (c + 8 <= cols) {
-    E w[8];
-    __builtin_memcpy(w, row + c, sizeof(w));
+// kC neighbouring values from column c on (0 past cols) of N rows by one load each, aligned to their size or of any alignment. One branch
+// for all the rows: a branch around each load made it wait for the one before.
+template <typename E, int N, int kC, bool ALIGNED>
+__device__ __forceinline__ void load_rows(const E* const (&row)[N], int64_t c, int64_t cols, float (&x)[N][kC]) {
+  E w[N][kC];
+  if (c + kC <= cols) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = static_cast<float>(w[k]);
+    for (int q = 0; q < N; ++q) {
+      if constexpr (ALIGNED) __builtin_memcpy(w[q], __builtin_assume_aligned(row[q] + c, sizeof(w[q])), sizeof(w[q]));
+      else __builtin_memcpy(w[q], row[q] + c, sizeof(w[q]));
+    }
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = c + k < cols ? static_cast<float>(row[c + k]) : 0.f;
+    for (int q = 0; q < N; ++q)
+#pragma unroll
+      for (int k = 0; k < kC; ++k) w[q][k] = c + k < cols ? row[q][c + k] : static_cast<E>(0.f);
   }
+#pragma unroll
+  for (int q = 0; q < N; ++q)
+#pragma unroll
+    for (int k = 0; k < kC; ++k) x[q][k] = static_cast<float>(w[q][k]);
 }
 // Their codes, the eight that hold the last column whole.
 __device__ __forceinline__ void store8(uint8_t* row, int64_t c, int64_t cols, const float (&x)[8], float s) {
@@ -92,11 +100,13 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a) {
   const int64_t c = c0 + lane * 8;
   const E* src = static_cast<const E*>(a.src);
   float x[4][8];
+  const E* row[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int64_t r = r0 + wave * 4 + q;
-    load8<E>(src + (r < a.rows ? r : a.rows - 1) * a.lds, c, a.cols, x[q]);
+    row[q] = src + (r < a.rows ? r : a.rows - 1) * a.lds;
   }
+  load_rows<E, 4, 8, false>(row, c, a.cols, x);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int64_t r = r0 + wave * 4 + q;
@@ -118,25 +128,32 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(Fp8QuantArgs a) {
     a.scales[(r0 + k) * a.scale_row + (c0 / 128 + b) * a.scale_col] = sc[b][k];
 }
 
-// Blocks of 128 rows: a workgroup holds a block in registers, 8 rows x 8
-// columns a thread.
-template <typename E>
+// Blocks of 128 rows: a workgroup holds a block in registers, 64 / kC rows of kC
+// columns a thread, kC as wide as the rows' alignment allows.
+template <typename E, int kC, bool ALIGNED>
 __global__ __launch_bounds__(256) void fp8_quant_blocks_kernel(Fp8QuantArgs a) {
+  constexpr int kLanes = 128 / kC, kRows = 64 / kC, kStep = 256 / kLanes;
   __shared__ uint32_t top[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t cb = (a.cols + 127) / 128;
-  const int64_t rb = blockIdx.x / cb, kb = blockIdx.x % cb;
-  const int64_t c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
+  // (Neighbouring blocks on one XCD: where rows are no whole lines they share them.)
+  const int64_t per = gridDim.x / 8, at = blockIdx.x < per * 8 ? blockIdx.x % 8 * per + blockIdx.x / 8 : blockIdx.x;
+  const int64_t rb = at / cb, kb = at % cb;
+  const int64_t c = kb * 128 + threadIdx.x % kLanes * kC, r0 = rb * 128 + threadIdx.x / kLanes;
   const E* src = static_cast<const E*>(a.src);
-  float x[8][8];
+  float x[kRows][kC];
+  const E* row[kRows];
   uint32_t m = 0;
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const int64_t r = r0 + 16 * q;
-    load8<E>(src + (r < a.rows ? r : a.rows - 1) * a.lds, c, a.cols, x[q]);   // the last row again
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m = abs_bits(x[q][k]) > m ? abs_bits(x[q][k]) : m;
+  for (int q = 0; q < kRows; ++q) {
+    const int64_t r = r0 + kStep * q;
+    row[q] = src + (r < a.rows ? r : a.rows - 1) * a.lds;   // the last row again
   }
+  load_rows<E, kRows, kC, ALIGNED>(row, c, a.cols, x);
+#pragma unroll
+  for (int q = 0; q < kRows; ++q)
+#pragma unroll
+    for (int k = 0; k < kC; ++k) m = abs_bits(x[q][k]) > m ? abs_bits(x[q][k]) : m;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const uint32_t o = __shfl_xor(m, d);
@@ -146,11 +163,21 @@ __global__ __launch_bounds__(256) void fp8_quant_blocks_kernel(Fp8QuantArgs a) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 4; ++w) m = top[w] > m ? top[w] : m;
-  const float s = scale_of(m);
+  const float s = scale_of(m), r1 = __builtin_amdgcn_rcpf(s);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const int64_t r = r0 + 16 * q;
-    if (r < a.rows) store8(a.codes + r * a.ldc, c, a.cols, x[q], s);
+  for (int q = 0; q < kRows; ++q) {
+    const int64_t r = r0 + kStep * q;
+    if (r >= a.rows || c >= a.cols) continue;
+    uint8_t* d = a.codes + r * a.ldc + c;
+    if constexpr (kC >= 4) {
+#pragma unroll
+      for (int k = 0; k < kC; k += 4) *reinterpret_cast<uint32_t*>(d + k) = codes4(x[q] + k, s, r1);
+    } else {
+      float y[4] = {x[q][0], kC > 1 ? x[q][kC - 1] : 0.f, 0.f, 0.f};
+      const uint32_t w = codes4(y, s, r1);
+      if constexpr (kC == 2) *reinterpret_cast<uint16_t*>(d) = static_cast<uint16_t>(w);
+      else *d = static_cast<uint8_t>(w);
+    }
   }
   if (threadIdx.x == 0) a.scales[rb * a.scale_row + kb * a.scale_col] = s;
 }
@@ -520,14 +547,15 @@ __global__ __launch_bounds__(kThreads, 2) void fp8_mm_kernel(Fp8MmArgs a) {
 }
 
 // ------------------------------------------------------------ few rows
-// Up to 64 rows of A (a token, a small batch): bound by the bytes of B, which
-// each go once from memory to the registers of one wave, with no LDS and no
-// barrier. A wave takes 16·R rows of B and all rows of A (F fragments of 16, from the
-// caches), loads the next U blocks while it multiplies these, and scales as above.
-// R = 4, U = 1 (8 KB of B in flight a wave) where that leaves every CU four waves;
-// else R = 1, U = 2. One row at 131072 x 4096: 142 us on the tiles.
-template <typename OT, bool WIDE, int F, int R, int U>
+// A token, a small batch: bound by the bytes of B, which each go once from memory
+// to the registers of one wave, with no LDS and no barrier. A wave takes 16 rows of
+// B and all rows of A (F fragments of 16, from the caches), loads the next two
+// blocks while it multiplies these, and scales as above. One row at 131072 x 4096:
+// 92 us, 5.9 TB/s (64 rows of B a wave, a block at a time, 115; four blocks 95; on
+// the tiles 142).
+template <typename OT, bool WIDE, int F>
 __global__ __launch_bounds__(256) void fp8_few_kernel(Fp8MmArgs a) {
+  constexpr int R = 1, U = 2;   // fragments of B, blocks in flight
   const int lane = threadIdx.x & 63;
   const int64_t n0 = (blockIdx.x * int64_t{4} + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * (16 * R);
   if (n0 >= a.n) return;
@@ -674,12 +702,22 @@ __global__ __launch_bounds__(256) void fp8_few_kernel(Fp8MmArgs a) {
   }
 }
 
-constexpr int64_t kFewRows = 64;
 template <typename OT, bool WIDE>
-void (*few_kernel(int64_t m, bool wide_rows))(Fp8MmArgs) {
-  if (m <= 16) return wide_rows ? fp8_few_kernel<OT, WIDE, 1, 4, 1> : fp8_few_kernel<OT, WIDE, 1, 1, 2>;
-  if (m <= 32) return wide_rows ? fp8_few_kernel<OT, WIDE, 2, 4, 1> : fp8_few_kernel<OT, WIDE, 2, 1, 2>;
-  return wide_rows ? fp8_few_kernel<OT, WIDE, 4, 4, 1> : fp8_few_kernel<OT, WIDE, 4, 1, 2>;
+void (*few_kernel(int64_t m))(Fp8MmArgs) {
+  return m <= 16 ? fp8_few_kernel<OT, WIDE, 1> : m <= 32 ? fp8_few_kernel<OT, WIDE, 2> : fp8_few_kernel<OT, WIDE, 4>;
+}
+
+// Whether the product runs there: always up to 16 rows; up to 64 where reading A in
+// every wave costs less than the tiles' rounds. Both sides' us fitted at 32 and 64
+// rows of 4096 x 131072 (203 and 211 against 147), 4096 x 32000 (50 and 114, fp32
+// 46 and 78, against 51, fp32 111) and 1000 x 11000 (18 against 25 to 48).
+bool few_rows(const Fp8MmArgs& a, bool wide) {
+  if (a.m <= 16) return true;
+  if (a.m > 64) return false;
+  const double few = static_cast<double>(a.n) * a.k * (a.m <= 32 ? 3.8e-7 : wide ? 5.9e-7 : 8.7e-7);
+  const double blocks = static_cast<double>((a.k + 127) / 128);
+  const double tiles = static_cast<double>(((a.n + kTile - 1) / kTile + 255) / 256) * (blocks * (wide ? 3.3 : 1.4) + 8.0);
+  return few < tiles;
 }
 
 }  // namespace
@@ -690,8 +728,16 @@ hipError_t launch_fp8_quant(const Fp8QuantArgs& a, DType t, bool blocks, hipStre
   const int64_t grid = blocks ? (a.rows + 127) / 128 * ((a.cols + 127) / 128) : (a.rows + 15) / 16 * ((a.cols + 511) / 512);
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   using K = void (*)(Fp8QuantArgs);
-  const K k = blocks ? (t == DType::BF16 ? static_cast<K>(fp8_quant_blocks_kernel<__bf16>) : fp8_quant_blocks_kernel<float>)
-                     : (t == DType::BF16 ? static_cast<K>(fp8_quant_rows_kernel<__bf16>) : fp8_quant_rows_kernel<float>);
+  const int64_t at = reinterpret_cast<uintptr_t>(a.src) | static_cast<uint64_t>(a.lds * dtype_size(t));
+  K k;
+  if (!blocks) k = t == DType::BF16 ? static_cast<K>(fp8_quant_rows_kernel<__bf16>) : fp8_quant_rows_kernel<float>;
+  else if (t == DType::F32) k = at % 16 == 0 ? fp8_quant_blocks_kernel<float, 4, true>
+                              : at % 8 == 0  ? fp8_quant_blocks_kernel<float, 2, true>
+                                             : fp8_quant_blocks_kernel<float, 1, true>;
+  else k = at % 16 == 0  ? fp8_quant_blocks_kernel<__bf16, 8, true>
+           : at % 8 == 0 ? fp8_quant_blocks_kernel<__bf16, 4, true>
+           : at % 4 == 0 ? fp8_quant_blocks_kernel<__bf16, 2, true>
+                         : fp8_quant_blocks_kernel<__bf16, 8, false>;
   hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
@@ -711,10 +757,9 @@ hipError_t launch_fp8_mm(const Fp8MmArgs& a, DType out, hipStream_t stream) {
   if (a.lda % 16 != 0 || a.ldb % 16 != 0 || reinterpret_cast<uintptr_t>(a.a) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(a.b) % 16 != 0)
     return hipErrorInvalidValue;
-  if (a.m <= kFewRows) {
-    const bool wide_rows = (a.n + 63) / 64 >= 4 * 256;
-    const int64_t waves = (a.n + (wide_rows ? 63 : 15)) / (wide_rows ? 64 : 16);
-    auto* k = out == DType::BF16 ? few_kernel<__bf16, false>(a.m, wide_rows) : few_kernel<float, true>(a.m, wide_rows);
+  if (few_rows(a, out == DType::F32)) {
+    const int64_t waves = (a.n + 15) / 16;
+    auto* k = out == DType::BF16 ? few_kernel<__bf16, false>(a.m) : few_kernel<float, true>(a.m);
     hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, stream, a);
     return hipGetLastError();
   }

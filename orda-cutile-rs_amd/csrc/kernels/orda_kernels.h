@@ -526,7 +526,8 @@ struct EmbedGradArgs {
   int64_t chunk, chunks, slabs;
   float* parts;        // [chunks][2][ldp]
   int64_t ldp;
-  int64_t fill_rows;   // set by launch_embed_grad
+  int64_t fill_rows;   // set by launch_embed_grad, as
+  bool stream;         // out is written past the caches
 };
 hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t stream);
 

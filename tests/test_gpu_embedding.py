@@ -87,6 +87,8 @@ def test_lookup_shapes_strides_and_ids_out_of_range():
     bad = torch.tensor([0, 100, -1, 99, 2 ** 40], device="cuda")
     out = H.embedding(bad, w)
     assert torch.equal(out[[0, 3]], w[[0, 99]]) and torch.isnan(out[[1, 2, 4]]).all()
+    none = H.embedding(bad, torch.zeros(0, 96, device="cuda"))   # no rows at all
+    assert none.shape == (5, 96) and torch.isnan(none).all()
     w[3] = float("inf")
     assert torch.equal(H.embedding(torch.tensor([3], device="cuda"), w, scale=2.0)[0], w[3])
 
