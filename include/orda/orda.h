@@ -368,8 +368,9 @@ int32_t orda_embedding(int32_t device, void *hip_stream, const void *ids, int32_
  * (the same bits whatever the launch) and rounded once to out's type; with
  * accumulate, that plus out's old value, and rows no id names are not touched.
  * Ids equal to padding_idx (negative: none), or that are no row, add nothing.
- * grad [n,H] and out [V,H] are fp32 or bf16 each. workspace (256-byte aligned)
- * is the call's alone until its kernels have run. */
+ * grad [n,H] and out [V,H] are fp32 or bf16 each; out shares no memory with ids
+ * or grad. workspace (256-byte aligned) is the call's alone until its kernels
+ * have run. */
 int32_t orda_embedding_backward_workspace(int64_t n, int64_t rows, int64_t cols, int32_t grad_dtype,
                                           int64_t *bytes, char *err, size_t err_len);
 int32_t orda_embedding_backward(int32_t device, void *hip_stream, const void *ids, int32_t ids_bytes,

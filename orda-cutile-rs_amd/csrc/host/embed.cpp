@@ -76,9 +76,10 @@ int32_t orda_embedding_backward(int32_t device, void* hip_stream, const void* id
     const DeviceScope scope(device);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     EmbedGradArgs a{};
-    if (n > 0)
-      hip_check(launch_embed_sort(ids, ids_bytes == 8, n, out->rows, padding_idx, workspace, s, &a.keys, &a.vals, st),
-                "embedding gradient sort");
+    EmbedFill fill{};
+    if (!accumulate) fill = embed_fill(ot, out->data, tensor_ld(*out), out->rows, out->cols);
+    hip_check(launch_embed_sort(ids, ids_bytes == 8, n, out->rows, padding_idx, workspace, s, fill, &a.keys, &a.vals, st),
+              "embedding gradient sort");
     a.n = n;
     a.v = out->rows;
     a.h = out->cols;

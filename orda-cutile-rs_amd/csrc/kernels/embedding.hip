@@ -71,6 +71,9 @@ __global__ __launch_bounds__(256) void embedding_kernel(const I* ids, int64_t n,
 }
 
 // ------------------------------------------------------------ sort
+constexpr int kFillBytes = 16384;                      // of a wave: 1 GB in 163 us, of 4096 bytes in 180
+constexpr int64_t kStreamBytes = int64_t{256} << 20;   // more than the last cache holds
+
 // Ids that take no gradient (padding, or no row of the weight) sort as v, last.
 template <typename I>
 __device__ __forceinline__ uint32_t key_of(I id, int64_t v, int64_t pad) {
@@ -78,28 +81,69 @@ __device__ __forceinline__ uint32_t key_of(I id, int64_t v, int64_t pad) {
   return static_cast<uint32_t>(i >= 0 && i < v && i != pad ? i : v);
 }
 
-// Few tokens: every token's place is the number of pairs before it, counted
-// against all of them from LDS, with (key, place) packed into 32 bits. 2 VALU
-// operations a comparison: 1000 tokens take 4 workgroups 4 us, one launch, where
-// the passes below take four.
+// 16 bytes, past the caches with `stream`: the gradient of a large vocabulary is
+// not read again before gigabytes of other traffic, and displaces the rows still
+// to be read.
+__device__ __forceinline__ void put16(void* d, u32x4 v, bool stream) {
+  if (stream && reinterpret_cast<uintptr_t>(d) % 16 == 0) __builtin_nontemporal_store(v, static_cast<u32x4*>(d));
+  else __builtin_memcpy(d, &v, 16);
+}
+
+// A launch's share of the zeroes: its workgroups from `first` on, of 16 waves, each
+// a span of kFillBytes at a time. The gradient is zeroed whole while the tokens are
+// sorted, which leaves most of the chip idle, and the sums then write the rows that
+// a token names: zeroing just the others takes a search of the sorted keys and
+// writes in rows.
+__device__ __forceinline__ void fill_zero(const EmbedFill& f, int first) {
+  const int lane = threadIdx.x & 63;
+  const int64_t waves = (static_cast<int64_t>(gridDim.x) - first) * 16;
+  for (int64_t u = f.from + (static_cast<int64_t>(blockIdx.x) - first) * 16 + (threadIdx.x >> 6); u < f.to; u += waves) {
+    const int64_t row = u / f.spans;
+    // spans begin at whole lines, the first one before the row
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(f.out) + row * f.pitch, end = begin + f.bytes;
+    const uintptr_t at = begin / 128 * 128 + (u - row * f.spans) * kFillBytes;
+#pragma unroll
+    for (int i = 0; i < kFillBytes / 1024; ++i) {
+      const uintptr_t d = at + i * 1024 + lane * 16;
+      if (d >= begin && d + 16 <= end) put16(reinterpret_cast<void*>(d), u32x4{0, 0, 0, 0}, f.stream);
+      else
+        for (uintptr_t e = d; e < d + 16; e += 2)   // elements of 2 or 4 bytes
+          if (e >= begin && e < end) *reinterpret_cast<uint16_t*>(e) = 0;
+    }
+  }
+}
+
+// Few tokens: a token's place is the number of pairs before it, counted against
+// all of them from LDS, with (key, place) packed into 32 bits: 64 tokens a
+// workgroup, each wave against a sixteenth of the pairs. One launch, where the
+// passes below take two a digit.
 template <typename I>
-__global__ __launch_bounds__(256) void embed_rank_kernel(const I* ids, int n, int64_t v, int64_t pad, uint32_t* keys,
-                                                         uint32_t* vals) {
-  extern __shared__ __attribute__((aligned(16))) uint32_t all[];   // n, up to whole fours
-  const int n4 = (n + 3) / 4 * 4;
-  for (int i = threadIdx.x; i < n4; i += 256)
+__global__ __launch_bounds__(1024) void embed_rank_kernel(const I* ids, int n, int64_t v, int64_t pad, uint32_t* keys,
+                                                          uint32_t* vals, EmbedFill fill) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t all[];   // n, up to whole 64s, then the waves' counts
+  const int blocks = (n + 63) / 64;
+  if (static_cast<int>(blockIdx.x) >= blocks) return fill_zero(fill, blocks);
+  const int np = blocks * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t* part = all + np;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < np; i += 1024)
     all[i] = i < n ? key_of(ids[i], v, pad) * static_cast<uint32_t>(n) + i : 0xffffffffu;
   __syncthreads();
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
+  const int i = blockIdx.x * 64 + lane;
   const uint32_t me = all[i];
   uint32_t before = 0;
-#pragma unroll 8
-  for (int j = 0; j < n4; j += 4) {
+#pragma unroll 4
+  for (int j = wave * (np / 16); j < (wave + 1) * (np / 16); j += 4) {
     const u32x4 o = *reinterpret_cast<const u32x4*>(all + j);
 #pragma unroll
     for (int k = 0; k < 4; ++k) before += o[k] < me ? 1u : 0u;
   }
+  part[wave * 64 + lane] = before;
+  __syncthreads();
+  if (wave != 0 || i >= n) return;
+  before = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) before += part[w * 64 + lane];
   keys[before] = me / static_cast<uint32_t>(n);
   vals[before] = static_cast<uint32_t>(i);
 }
@@ -122,8 +166,10 @@ struct Pairs {
 };
 
 template <typename I>
-__global__ __launch_bounds__(1024) void embed_count_kernel(Pairs<I> p, int shift, uint32_t* counts) {
+__global__ __launch_bounds__(1024) void embed_count_kernel(Pairs<I> p, int shift, int blocks, uint32_t* counts,
+                                                           EmbedFill fill) {
   __shared__ uint32_t c[kDigits];
+  if (static_cast<int>(blockIdx.x) >= blocks) return fill_zero(fill, blocks);
   for (int d = threadIdx.x; d < kDigits; d += 1024) c[d] = 0;
   __syncthreads();
   const int64_t i0 = blockIdx.x * static_cast<int64_t>(kSortTile);
@@ -134,8 +180,9 @@ __global__ __launch_bounds__(1024) void embed_count_kernel(Pairs<I> p, int shift
 }
 
 template <typename I>
-__global__ __launch_bounds__(1024) void embed_place_kernel(Pairs<I> p, int shift, const uint32_t* counts, uint32_t* keys,
-                                                           uint32_t* vals) {
+__global__ __launch_bounds__(1024) void embed_place_kernel(Pairs<I> p, int shift, int blocks, const uint32_t* counts,
+                                                           uint32_t* keys, uint32_t* vals, EmbedFill fill) {
+  if (static_cast<int>(blockIdx.x) >= blocks) return fill_zero(fill, blocks);
   __shared__ uint32_t wave_n[kSortWaves][kDigits];   // a wave's pairs of each digit, then where they begin
   __shared__ uint32_t part[2][kDigits], wave_sum[kDigits / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -145,7 +192,7 @@ __global__ __launch_bounds__(1024) void embed_place_kernel(Pairs<I> p, int shift
   const int d = tid & (kDigits - 1), half = tid >> kDigitBits;
   static_assert(2 * kDigits == 1024, "two threads a digit");
   uint32_t earlier = 0, total = 0;
-  for (int b = half; b < static_cast<int>(gridDim.x); b += 2) {
+  for (int b = half; b < blocks; b += 2) {
     const uint32_t c = counts[static_cast<int64_t>(b) * kDigits + d];
     total += c;
     if (b < static_cast<int>(blockIdx.x)) earlier += c;
@@ -235,26 +282,6 @@ __device__ __forceinline__ int64_t first_at_least(const uint32_t* keys, int64_t 
   return lo;
 }
 
-// 16 bytes, past the caches with `stream`: the gradient of a large vocabulary
-// (EmbedGradArgs::stream) is not read again before gigabytes of other traffic, and
-// displaces the rows still to be read. (8192 x 4096 into 131072 rows of bf16: 198
-// us against 224, 65536 tokens 610 with the join against 630.)
-__device__ __forceinline__ void put16(void* d, u32x4 v, bool stream) {
-  if (stream && reinterpret_cast<uintptr_t>(d) % 16 == 0) __builtin_nontemporal_store(v, static_cast<u32x4*>(d));
-  else __builtin_memcpy(d, &v, 16);
-}
-
-// A wave zeroes a row: 16-byte vectors from the first aligned address on.
-template <typename O>
-__device__ __forceinline__ void zero_row(O* d, int64_t h, int lane, bool stream) {
-  constexpr int kO = 16 / sizeof(O);
-  const int64_t skew = (16 - reinterpret_cast<uintptr_t>(d) % 16) % 16 / sizeof(O), head = skew < h ? skew : h;
-  if (lane < head) d[lane] = static_cast<O>(0.f);
-  int64_t c = head + lane * kO;
-  for (; c + kO <= h; c += 64 * kO) put16(d + c, u32x4{0, 0, 0, 0}, stream);
-  for (int k = 0; k < kO && c + k < h; ++k) d[c + k] = static_cast<O>(0.f);
-}
-
 // One lane's columns of a gradient row from column c on, scaled and rounded (added
 // to what is there with accumulate).
 template <typename E, typename O>
@@ -311,83 +338,62 @@ __device__ __forceinline__ void add_partial(const float* s, float (&x)[kV]) {
   }
 }
 
-// Waves [0, chunks·slabs): the sums of a chunk of sorted pairs, kLoads rows in
-// flight. The waves after them zero the rows no pair names, fill_rows
-// consecutive ones each, found by one search of the sorted keys.
+// The sums of a chunk of sorted pairs, a wave for each chunk and its columns,
+// kLoads rows in flight.
 template <typename E, typename O>
 __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
   constexpr int kV = Cols<E>::kV, kLoads = 8;
   const int lane = threadIdx.x & 63;
   const int64_t unit = blockIdx.x * int64_t{4} + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (unit < a.chunks * a.slabs) {
-    const int64_t chunk = unit / a.slabs, c = (unit - chunk * a.slabs) * (64 * kV) + lane * kV;
-    const int64_t b = chunk * a.chunk, e = b + a.chunk < a.n ? b + a.chunk : a.n;
-    const int left = static_cast<int>(a.h - c);
-    const E* src = static_cast<const E*>(a.grad) + c;
-    float x[kV] = {};
-    uint32_t key = a.keys[b];
-    bool head = b > 0 && a.keys[b - 1] == key;   // the sum began in an earlier chunk
-    auto flush = [&](bool tail) {   // tail: it goes on in the next one
-      if (static_cast<int64_t>(key) < a.v) {
-        if (head || tail) put_partial(partial(a, chunk, head ? 0 : 1, c), x);
-        else if (left > 0) put_row<E, O>(a, key, c, x);
-      }
+  if (unit >= a.chunks * a.slabs) return;
+  const int64_t chunk = unit / a.slabs, c = (unit - chunk * a.slabs) * (64 * kV) + lane * kV;
+  const int64_t b = chunk * a.chunk, e = b + a.chunk < a.n ? b + a.chunk : a.n;
+  const int left = static_cast<int>(a.h - c);
+  const E* src = static_cast<const E*>(a.grad) + c;
+  float x[kV] = {};
+  uint32_t key = a.keys[b];
+  bool head = b > 0 && a.keys[b - 1] == key;   // the sum began in an earlier chunk
+  auto flush = [&](bool tail) {   // tail: it goes on in the next one
+    if (static_cast<int64_t>(key) < a.v) {
+      if (head || tail) put_partial(partial(a, chunk, head ? 0 : 1, c), x);
+      else if (left > 0) put_row<E, O>(a, key, c, x);
+    }
 #pragma unroll
-      for (int k = 0; k < kV; ++k) x[k] = 0.f;
-      head = false;
-    };
-    for (int64_t i = b; i < e; i += kLoads) {
-      E w[kLoads][kV];
-      uint32_t ks[kLoads];
-      int64_t at[kLoads];
+    for (int k = 0; k < kV; ++k) x[k] = 0.f;
+    head = false;
+  };
+  for (int64_t i = b; i < e; i += kLoads) {
+    E w[kLoads][kV];
+    uint32_t ks[kLoads];
+    int64_t at[kLoads];
 #pragma unroll
-      for (int q = 0; q < kLoads; ++q) {
-        const int64_t j = i + q < e ? i + q : e - 1;
-        ks[q] = a.keys[j];
-        at[q] = a.vals[j] * a.ldg;   // (a row without a gradient is read, not added)
-      }
-      if (left >= kV) {   // one branch for all rows: around each load it made them wait for one another
+    for (int q = 0; q < kLoads; ++q) {
+      const int64_t j = i + q < e ? i + q : e - 1;
+      ks[q] = a.keys[j];
+      at[q] = a.vals[j] * a.ldg;   // (a row without a gradient is read, not added)
+    }
+    if (left >= kV) {   // one branch for all rows: around each load it made them wait for one another
 #pragma unroll
-        for (int q = 0; q < kLoads; ++q) __builtin_memcpy(w[q], src + at[q], sizeof(w[q]));
-      } else {
+      for (int q = 0; q < kLoads; ++q) __builtin_memcpy(w[q], src + at[q], sizeof(w[q]));
+    } else {
 #pragma unroll
-        for (int q = 0; q < kLoads; ++q)
+      for (int q = 0; q < kLoads; ++q)
 #pragma unroll
-          for (int k = 0; k < kV; ++k) w[q][k] = k < left ? src[at[q] + k] : static_cast<E>(0.f);
-      }
+        for (int k = 0; k < kV; ++k) w[q][k] = k < left ? src[at[q] + k] : static_cast<E>(0.f);
+    }
 #pragma unroll
-      for (int q = 0; q < kLoads; ++q) {
-        if (i + q < e) {
-          if (ks[q] != key) {
-            flush(false);
-            key = ks[q];
-          }
-#pragma unroll
-          for (int k = 0; k < kV; ++k) x[k] += static_cast<float>(w[q][k]);
+    for (int q = 0; q < kLoads; ++q) {
+      if (i + q < e) {
+        if (ks[q] != key) {
+          flush(false);
+          key = ks[q];
         }
+#pragma unroll
+        for (int k = 0; k < kV; ++k) x[k] += static_cast<float>(w[q][k]);
       }
     }
-    flush(e < a.n && a.keys[e] == key);
-    return;
   }
-  if (a.accumulate) return;
-  const int64_t r0 = (unit - a.chunks * a.slabs) * a.fill_rows;
-  if (r0 >= a.v) return;
-  const int64_t r1 = r0 + a.fill_rows < a.v ? r0 + a.fill_rows : a.v;
-  int64_t at = first_at_least(a.keys, a.n, static_cast<uint32_t>(r0), lane);
-  int64_t r = r0;
-  while (r < r1) {
-    // rows up to the next key are zero
-    const int64_t next = at < a.n && static_cast<int64_t>(a.keys[at]) < r1 ? a.keys[at] : r1;
-    for (; r < next; ++r) {
-      zero_row(static_cast<O*>(a.out) + r * a.ldo, a.h, lane, a.stream);
-    }
-    if (r >= r1) break;
-    // past the pairs of row r
-    const uint64_t same = __ballot(at + lane < a.n && static_cast<int64_t>(a.keys[at + lane < a.n ? at + lane : at]) == r);
-    at = ~same == 0 ? first_at_least(a.keys, a.n, static_cast<uint32_t>(r + 1), lane) : at + __popcll(same);
-    ++r;
-  }
+  flush(e < a.n && a.keys[e] == key);
 }
 
 // Sums that a chunk begins and a later one ends, a wave for each chunk and its
@@ -428,9 +434,10 @@ int passes_of(int64_t v) {   // digits of keys 0..v
   return bits <= kDigitBits ? 1 : (bits + kDigitBits - 1) / kDigitBits;
 }
 
-// Tokens whose ranks are counted: the packed pairs must fit 32 bits and LDS.
-// (Counted against the passes at 1024 to 4096 tokens: see embed_rank_kernel.)
-constexpr int64_t kRankTokens = 2048;
+// Tokens whose ranks are counted: the packed pairs must fit 32 bits and 64 KB of
+// LDS, less the waves' counts. 8192 tokens' ranks take 14 us and the passes 25,
+// 15000 tokens' 23 and 27, 1024 tokens' 4 and 15.
+constexpr int64_t kRankTokens = 15360;
 bool ranked(int64_t n, int64_t v) { return n <= kRankTokens && (v + 1) * n <= int64_t{0xffffffff}; }
 
 }  // namespace
@@ -460,8 +467,8 @@ hipError_t launch_embedding(DType t, const void* ids, bool ids64, int64_t n, con
 EmbedScratch embed_scratch(DType grad, int64_t n, int64_t v, int64_t h) {
   EmbedScratch s{};
   const int64_t cols = 64 * 16 / dtype_size(grad);   // of a wave
-  s.chunk = 32;   // pairs a wave sums: enough waves of few tokens, few joins of many
-  while (s.chunk < 256 && n / s.chunk > 1024) s.chunk *= 2;
+  s.chunk = 8;   // pairs a wave sums: enough waves of few tokens (1000 x 1531: 9 us, of 32 pairs 22), few joins of many
+  while (s.chunk < 256 && n / s.chunk > 512) s.chunk *= 2;
   s.chunks = (n + s.chunk - 1) / s.chunk;
   s.slabs = (h + cols - 1) / cols;
   s.ldp = s.slabs * cols;
@@ -481,19 +488,42 @@ EmbedScratch embed_scratch(DType grad, int64_t n, int64_t v, int64_t h) {
   return s;
 }
 
+EmbedFill embed_fill(DType out, void* d, int64_t ldo, int64_t v, int64_t h) {
+  const int64_t es = dtype_size(out);
+  EmbedFill f{};
+  f.out = d;
+  const bool whole = ldo == h || v == 1;   // rows that follow each other are one
+  f.rows = whole ? 1 : v;
+  f.bytes = (whole ? v * h : h) * es;
+  f.pitch = ldo * es;
+  f.spans = f.bytes > 0 ? (f.bytes + 126 + kFillBytes - 1) / kFillBytes : 0;   // (a row begins up to 126 bytes into its line)
+  f.stream = v * ldo * es > kStreamBytes;
+  return f;
+}
+
 hipError_t launch_embed_sort(const void* ids, bool ids64, int64_t n, int64_t v, int64_t pad, void* ws,
-                             const EmbedScratch& s, const uint32_t** keys, const uint32_t** vals, hipStream_t stream) {
+                             const EmbedScratch& s, EmbedFill fill, const uint32_t** keys, const uint32_t** vals,
+                             hipStream_t stream) {
   char* base = static_cast<char*>(ws);
   auto u32 = [&](int64_t at) { return reinterpret_cast<uint32_t*>(base + at); };
   auto run = [&](auto* i) {
     using I = std::remove_pointer_t<decltype(i)>;
     const I* id = static_cast<const I*>(ids);
+    const int64_t units = fill.rows * fill.spans;
+    // launch l of `of` zeroes its part, a wave a span until the grid is large
+    auto share = [&](int l, int of) {
+      fill.from = units * l / of;
+      fill.to = units * (l + 1) / of;
+      const int64_t wgs = (fill.to - fill.from + 15) / 16;
+      return static_cast<unsigned>(wgs < 8192 ? wgs : 8192);
+    };
     if (ranked(n, v)) {
-      hipLaunchKernelGGL(embed_rank_kernel<I>, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256),
-                         static_cast<unsigned>((n + 3) / 4 * 16), stream, id, static_cast<int>(n), v, pad,
-                         u32(s.keys[0]), u32(s.vals[0]));
+      const unsigned blocks = static_cast<unsigned>((n + 63) / 64), more = share(0, 1);
       *keys = u32(s.keys[0]);
       *vals = u32(s.vals[0]);
+      if (blocks + more > 0)
+        hipLaunchKernelGGL(embed_rank_kernel<I>, dim3(blocks + more), dim3(1024), blocks * 256 + 4096, stream, id,
+                           static_cast<int>(n), v, pad, u32(s.keys[0]), u32(s.vals[0]), fill);
       return;
     }
     const int passes = passes_of(v);
@@ -501,9 +531,13 @@ hipError_t launch_embed_sort(const void* ids, bool ids64, int64_t n, int64_t v, 
     for (int p = 0; p < passes; ++p) {
       const int to = p & 1;
       const Pairs<I> pr{p == 0 ? id : nullptr, u32(s.keys[1 - to]), u32(s.vals[1 - to]), n, v, pad};
-      hipLaunchKernelGGL(embed_count_kernel<I>, dim3(blocks), dim3(1024), 0, stream, pr, p * kDigitBits, u32(s.counts));
-      hipLaunchKernelGGL(embed_place_kernel<I>, dim3(blocks), dim3(1024), 0, stream, pr, p * kDigitBits,
-                         static_cast<const uint32_t*>(u32(s.counts)), u32(s.keys[to]), u32(s.vals[to]));
+      unsigned more = share(2 * p, 2 * passes);
+      hipLaunchKernelGGL(embed_count_kernel<I>, dim3(blocks + more), dim3(1024), 0, stream, pr, p * kDigitBits,
+                         static_cast<int>(blocks), u32(s.counts), fill);
+      more = share(2 * p + 1, 2 * passes);
+      hipLaunchKernelGGL(embed_place_kernel<I>, dim3(blocks + more), dim3(1024), 0, stream, pr, p * kDigitBits,
+                         static_cast<int>(blocks), static_cast<const uint32_t*>(u32(s.counts)), u32(s.keys[to]),
+                         u32(s.vals[to]), fill);
       *keys = u32(s.keys[to]);
       *vals = u32(s.vals[to]);
     }
@@ -518,11 +552,8 @@ hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t
   // more than the last cache holds, and rows of whole lines (a line two rows share
   // would go to memory twice)
   const int64_t row = a.ldo * dtype_size(out);
-  a.stream = a.v * row > int64_t{256} << 20 && row % 128 == 0 && reinterpret_cast<uintptr_t>(a.out) % 128 == 0;
-  // rows a wave zeroes: enough waves to fill the chip, at most 64 rows each
-  a.fill_rows = a.v / 8192 < 1 ? 1 : a.v / 8192 > 64 ? 64 : a.v / 8192;
-  const int64_t fill = a.accumulate ? 0 : (a.v + a.fill_rows - 1) / a.fill_rows;
-  const int64_t sum = (a.chunks * a.slabs + fill + 3) / 4, join = ((a.chunks - 1) * a.slabs + 3) / 4;
+  a.stream = a.v * row > kStreamBytes && row % 128 == 0 && reinterpret_cast<uintptr_t>(a.out) % 128 == 0;
+  const int64_t sum = (a.chunks * a.slabs + 3) / 4, join = ((a.chunks - 1) * a.slabs + 3) / 4;
   if (sum > 0x7fffffff) return hipErrorInvalidValue;
   auto run = [&](auto* e, auto* o) {
     using E = std::remove_pointer_t<decltype(e)>;

@@ -508,12 +508,21 @@ struct EmbedScratch {
   int64_t chunk, chunks, slabs, ldp;
 };
 EmbedScratch embed_scratch(DType grad, int64_t n, int64_t v, int64_t h);
+// Memory that the sort's launches zero beside it: rows of `bytes`, each of `spans`
+// spans, of which one launch takes [from, to).
+struct EmbedFill {
+  void* out;
+  int64_t rows, bytes, pitch, spans, from, to;
+  bool stream;   // past the caches
+};
+EmbedFill embed_fill(DType out, void* d, int64_t ldo, int64_t v, int64_t h);   // rows [v, h]
 // (id, place) of every token, sorted by id, stable; ids without a gradient (pad,
-// or no row) sort last, as v.
+// or no row) sort last, as v. Zeroes `fill` (spans 0: nothing).
 hipError_t launch_embed_sort(const void* ids, bool ids64, int64_t n, int64_t v, int64_t pad, void* ws,
-                             const EmbedScratch& s, const uint32_t** keys, const uint32_t** vals, hipStream_t stream);
-// out[k] (+)= scale * Σ grad[vals[i]] over keys[i] = k < v, in the sorted order;
-// without accumulate, rows no key names are zero.
+                             const EmbedScratch& s, EmbedFill fill, const uint32_t** keys, const uint32_t** vals,
+                             hipStream_t stream);
+// out[k] = scale * Σ grad[vals[i]] over keys[i] = k < v, in the sorted order, added
+// to out with accumulate; rows no key names are left alone.
 struct EmbedGradArgs {
   const uint32_t *keys, *vals;
   int64_t n, v, h;
@@ -526,8 +535,7 @@ struct EmbedGradArgs {
   int64_t chunk, chunks, slabs;
   float* parts;        // [chunks][2][ldp]
   int64_t ldp;
-  int64_t fill_rows;   // set by launch_embed_grad, as
-  bool stream;         // out is written past the caches
+  bool stream;         // set by launch_embed_grad: out is written past the caches
 };
 hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t stream);
 

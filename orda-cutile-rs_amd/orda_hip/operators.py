@@ -281,6 +281,8 @@ def embedding_backward(grad, ids, num_rows: int, *, scale: float = 1.0,
         raise OrdaError("out must not require a gradient")
     if _overlap(out, g.reshape(-1, g.size(-1)) if g.numel() else g.new_empty((0, 0))):
         raise OrdaError("out must not share memory with grad")
+    if _overlap(out, i.reshape(1, -1)):
+        raise OrdaError("out must not share memory with ids")
     _embed_grad(g, i, num_rows, scale, pad, out, accumulate)
     torch.autograd.graph.increment_version(out)   # written in place
     return out

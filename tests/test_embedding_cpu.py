@@ -60,9 +60,11 @@ def test_gradient_refused(kw, message):
 def test_workspace_grows_with_the_tokens(n):
     out, err = C.c_int64(), C.create_string_buffer(512)
     assert L.load().orda_embedding_backward_workspace(n, 131072, 4096, L.BF16, C.byref(out), err, 512) == L.ORDA_OK
-    # pairs, twice where they are sorted in passes, and two fp32 rows a chunk of 32 to 256 tokens
+    # pairs, twice where they are sorted in passes (with 512 counts for every 4096), and two fp32 rows a
+    # chunk: of 8 tokens, or more where that makes over 512 chunks, up to 256 tokens
     assert out.value >= 8 * n
-    assert out.value <= 16 * n + 4096 * 1024 + 2 * (n / 32 + 1) * 4096 * 4
+    chunks = min(n / 8 + 1, max(513, n / 256 + 1))
+    assert out.value <= 16 * n + (n / 4096 + 1) * 2048 + 2 * chunks * 4096 * 4 + 6 * 256
 
 
 def test_python_refuses_cpu_tensors():

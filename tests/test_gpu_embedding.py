@@ -108,6 +108,34 @@ def test_gradient(t, h, v, kind, dtype):
     check_grad(H.embedding_backward(g, ids, v), g, ids, v)
 
 
+@pytest.mark.parametrize("kind", ["uniform", "one", "text"])
+@pytest.mark.parametrize("t", [1023, 1025, 2049, 8192, 15360, 15361, 40000])   # counted ranks up to 15360, then passes
+def test_gradient_of_many_tokens(t, kind):
+    v, h = 3000, 40
+    ids, g = tokens(t, v, kind), grad_of(t, h, "bf16")
+    check_grad(H.embedding_backward(g, ids, v), g, ids, v)
+
+
+@pytest.mark.parametrize("kind", ["uniform", "one", "text"])
+@pytest.mark.parametrize("t", [0, 5, 4000, 20000])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_without_tokens_are_zero_and_nothing_else_is(t, kind, dtype):
+    """Whole and strided outputs at every start within a line, over memory that held something else."""
+    v, h = 701, 33
+    ids, g = tokens(t, v, kind), grad_of(t, h, dtype)
+    want = H.embedding_backward(g, ids, v)
+    check_grad(want, g, ids, v)
+    for at in (0, 1, 5, 31, 63):
+        flat = torch.full((at + v * h + 70,), 7.0, dtype=DT[dtype], device="cuda")
+        H.embedding_backward(g, ids, v, out=flat[at:at + v * h].view(v, h))
+        assert torch.equal(flat[at:at + v * h].view(v, h), want)
+        assert (flat[:at] == 7).all() and (flat[at + v * h:] == 7).all()
+        frame = torch.full((v, h + 70), 7.0, dtype=DT[dtype], device="cuda")
+        H.embedding_backward(g, ids, v, out=frame[:, at:at + h])
+        assert torch.equal(frame[:, at:at + h], want)
+        assert (frame[:, :at] == 7).all() and (frame[:, at + h:] == 7).all()
+
+
 @pytest.mark.parametrize("dtype, out", [("bf16", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("f32", "f32")])
 @pytest.mark.parametrize("t, h, v", [(40, 64, 30), (300, 77, 1000), (5000, 64, 1000)])
 def test_accumulated(t, h, v, dtype, out):
@@ -235,5 +263,9 @@ def test_refusals():
         a.update(kw)
         with pytest.raises(H.OrdaError):
             H.embedding_backward(**a)
+    memory = torch.zeros(50 * 64, dtype=torch.bfloat16, device="cuda")
+    shared = memory[:80].view(torch.int64)   # 20 ids in out's first row
+    with pytest.raises(H.OrdaError, match="share memory"):
+        H.embedding_backward(g, shared, 50, out=memory.view(50, 64))
     with pytest.raises(H.OrdaError):
         embedding_autograd(ids, w, padding_idx=50)
