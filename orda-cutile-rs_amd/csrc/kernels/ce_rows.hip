@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kScanThreads) void ce_rows_kernel(const int64_t* la
 }
 
 // ------------------------------------------------------------ hidden rows
-// A workgroup takes 64 rows of the batch and kPrepCols of their columns, and
+// A workgroup takes 64 rows of the batch and CePrepArgs::cols of their columns, and
 // writes what the products read of those that have a label, at their compact
 // places: the rows (a pitch of whole vectors, zeros past h), and for the backward
 // products the transposed rows, which pass through LDS 64 x 64 at a time. OUT 0
@@ -88,7 +88,11 @@ __global__ __launch_bounds__(kScanThreads) void ce_rows_kernel(const int64_t* la
 // SCAN: the places are counted here, from all labels before (a batch of up to
 // kScanRows: 4 us at 8192, where a kernel of its own takes 13 and a launch), else
 // read from pos, which ce_rows_kernel has written.
-constexpr int kPrepCols = 256;
+//
+// cols: 64 while that makes at most 2048 workgroups (1000 x 1536, both directions:
+// 8 + 12 us, of 256 columns 15 + 24), then up to 256 (8192 x 4096, forward: 28 us,
+// of 64 columns 48, as each workgroup counts for itself).
+constexpr int kMinPrepCols = 64, kMaxPrepCols = 256;
 
 template <typename E, int OUT, bool VEC, bool SCAN>
 __global__ __launch_bounds__(256) void ce_prep_kernel(CePrepArgs a) {
@@ -97,7 +101,7 @@ __global__ __launch_bounds__(256) void ce_prep_kernel(CePrepArgs a) {
   __shared__ int sums[4];
   __shared__ E tile[64][65];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64, first = static_cast<int64_t>(blockIdx.y) * kPrepCols;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64, first = static_cast<int64_t>(blockIdx.y) * a.cols;
   const CeRows& r = a.rows;
   const bool lead = blockIdx.y == 0, last_rows = r0 + 64 >= a.n;
   int64_t base = 0;   // labelled rows before r0
@@ -146,7 +150,7 @@ __global__ __launch_bounds__(256) void ce_prep_kernel(CePrepArgs a) {
   __syncthreads();
   const E* const x = static_cast<const E*>(a.x);
   const int row_in = tid / kLanes, col_in = tid % kLanes * kVec;
-  for (int64_t c0 = first; c0 < first + kPrepCols && c0 < a.pitch; c0 += 64) {
+  for (int64_t c0 = first; c0 < first + a.cols && c0 < a.pitch; c0 += 64) {
 #pragma unroll
     for (int q = 0; q < 64 / kPass; ++q) {
       const int rl = q * kPass + row_in, p = place[rl];
@@ -214,7 +218,7 @@ __global__ __launch_bounds__(256) void ce_prep_kernel(CePrepArgs a) {
   const int64_t end = a.whole ? (a.n + 63) / 64 * 64 : (n + 63) / 64 * 64;
   constexpr int kPlanes = OUT == 0 ? 1 : 3;
   constexpr int kOutBytes = OUT == 0 ? sizeof(E) : 2;
-  const int64_t c1 = first + kPrepCols < a.pitch ? first + kPrepCols : a.pitch;
+  const int64_t c1 = first + a.cols < a.pitch ? first + a.cols : a.pitch;
   if (lead && a.whole)
     for (int64_t p = n + tid; p < end; p += 256) {
       if (p < a.n) r.labels[p] = -1;
@@ -413,7 +417,10 @@ hipError_t launch_ce_prep(const CePrepArgs& in, DType t, bool planes, hipStream_
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  const dim3 grid(static_cast<unsigned>((a.n + 63) / 64), static_cast<unsigned>((a.pitch + kPrepCols - 1) / kPrepCols));
+  const int64_t rows = (a.n + 63) / 64;
+  a.cols = kMinPrepCols;
+  while (a.cols < kMaxPrepCols && rows * ((a.pitch + a.cols - 1) / a.cols) > 2048) a.cols *= 2;
+  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>((a.pitch + a.cols - 1) / a.cols));
   using K = void (*)(CePrepArgs);
   auto pick = [&](auto e, auto out_c) -> K {
     using E = decltype(e);

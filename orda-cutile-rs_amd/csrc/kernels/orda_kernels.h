@@ -456,7 +456,8 @@ struct CePrepArgs {
   void* zero;
   int64_t ldz;
   bool whole;
-  bool zero_vec;   // set by launch_ce_prep
+  bool zero_vec;   // set by launch_ce_prep, as
+  int64_t cols;    // a workgroup's columns
 };
 hipError_t launch_ce_prep(const CePrepArgs& a, DType t, bool planes, hipStream_t stream);
 // Merges a piece's tile statistics (CeArgs::stats) into state (between
