@@ -322,19 +322,21 @@ int32_t orda_scale_gradients(int32_t device, void *hip_stream, const float *scal
  * Everything is on `device`. The calls queue their kernels on hip_stream (NULL:
  * the null stream) and return; they allocate nothing and can be captured into
  * a graph. workspace is the call's alone until its kernels have run: calls (and
- * captured graphs) that may overlap need one each. No counterpart in the
- * reference, whose loss is a weighted mean. */
+ * captured graphs) that may overlap need one each. At most 2^21 rows, 2^20
+ * columns and 2^30 classes. No counterpart in the reference, whose loss is a
+ * weighted mean. */
 typedef struct {
     orda_tensor hidden;      /* [N,H], fp32 or bf16 */
     orda_tensor weight;      /* [V,H], the same type; read in place where it is
                                 fp32, or 16-byte aligned with H and ld multiples
-                                of 8, else copied a piece at a time */
+                                of 8 and ld at most 2^20, else copied a piece at
+                                a time */
     const int64_t *labels;   /* [N] */
     int64_t n_labels;
     int64_t ignore_index;
     float label_smoothing;   /* in [0, 1] */
-    int64_t vocab_piece;     /* columns of a piece, rounded to whole 256s; 0:
-                                as many as 1 GiB of scratch holds */
+    int64_t vocab_piece;     /* columns of a piece, rounded to whole 256s, at
+                                most 2^21; 0: as many as 1 GiB of scratch holds */
 } orda_linear_ce;
 /* Bytes of workspace (256-byte aligned) of a forward call (backward 0), or of
  * a backward call for grad_hidden (1), grad_weight (2) or both (3). */

@@ -12,8 +12,11 @@
 namespace orda {
 namespace {
 
-constexpr int64_t kMaxWidth = int64_t{1} << 20;      // 32-bit offsets inside an operand's tile
-constexpr int64_t kMaxRows = int64_t{1} << 30;       // compact row numbers are 32 bits
+// A product's operand is read with 32-bit byte offsets inside a tile of 256 rows:
+// 255 rows of 2^21 columns in three planes of bf16 are 3.2 GB. A row of an operand
+// is a row of hidden or weight, a column of hidden (its transpose) or a piece's
+// gradient of the logits.
+constexpr int64_t kMaxWidth = int64_t{1} << 20, kMaxRows = int64_t{1} << 21, kMaxPiece = int64_t{1} << 21;
 constexpr int64_t kMaxColumns = int64_t{1} << 30;
 // Scratch a piece may take: the larger the piece, the fewer the passes that
 // read and write the fp32 grad_hidden.
@@ -61,7 +64,7 @@ Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool
     fail(ORDA_ERR_INVALID, "%lld labels for %lld rows", static_cast<long long>(labels), static_cast<long long>(c.n));
   if (c.h < 1 || c.v < 1) fail(ORDA_ERR_INVALID, "hidden width and vocabulary must be > 0");
   if (c.h > kMaxWidth || c.n > kMaxRows || c.v > kMaxColumns)
-    fail(ORDA_ERR_INVALID, "at most 2^20 columns, 2^30 rows and 2^30 classes");
+    fail(ORDA_ERR_INVALID, "at most 2^20 columns, 2^21 rows and 2^30 classes");
   if (!(a.label_smoothing >= 0.f && a.label_smoothing <= 1.f))
     fail(ORDA_ERR_INVALID, "label_smoothing must be in [0, 1]");
   if (a.vocab_piece < 0) fail(ORDA_ERR_INVALID, "vocab_piece must be >= 0");
@@ -70,14 +73,14 @@ Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool
   c.ldx = tensor_ld(a.hidden);
   c.ldw = tensor_ld(a.weight);
   c.planes = c.t == DType::F32;
-  c.stage_w = !(c.ldw % 8 == 0 && c.h % 8 == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0);
+  c.stage_w = !(c.ldw <= kMaxWidth && c.ldw % 8 == 0 && c.h % 8 == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0);
   c.hp = c.planes ? round64(c.h) : round8(c.h);
   c.backward = backward;
   c.gh = gh;
   c.gw = gw;
   // Pieces of whole column tiles, all but the last alike.
   int64_t most = a.vocab_piece > 0 ? a.vocab_piece : std::max<int64_t>(kPieceBytes / std::max<int64_t>(column_bytes(c), 1), 4096);
-  most = std::max<int64_t>(most / 256 * 256, 256);
+  most = std::max<int64_t>(std::min(most, kMaxPiece) / 256 * 256, 256);
   const int64_t pieces = (c.v + most - 1) / most;
   c.piece = pieces == 1 ? c.v : ((c.v + pieces - 1) / pieces + 255) / 256 * 256;
   choose_direct(c);

@@ -300,3 +300,18 @@ def test_refusals():
         kw.update(bad)
         with pytest.raises(H.OrdaError):
             H.linear_cross_entropy_backward(**kw)
+
+
+def test_a_weight_at_a_wide_pitch():
+    """Columns of a table 2^23 + 72 wide: 300 rows lie 5 GB apart."""
+    table = torch.empty((300, 2 ** 23 + 72), dtype=torch.bfloat16, device="cuda")
+    w = table[:, 8:72]
+    w.copy_(torch.randn(300, 64, generator=torch.Generator().manual_seed(1)).mul_(0.2))
+    h = torch.randn(70, 64, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    y = torch.randint(0, 300, (70,), generator=torch.Generator().manual_seed(3)).cuda()
+    nll, lse = H.linear_cross_entropy(h, w, y)
+    Exact(h, w.contiguous(), y).check_losses(nll, lse)
+    g = torch.ones_like(nll)
+    got = H.linear_cross_entropy_backward(h, w, y, lse, g)
+    for a, b in zip(got, H.linear_cross_entropy_backward(h, w.contiguous(), y, lse, g)):
+        assert torch.equal(a, b)

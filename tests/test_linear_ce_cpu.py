@@ -109,6 +109,25 @@ def test_the_scratch_asked_for_is_the_scratch_laid_out(n, h, v, piece, dtype):
             assert rc == want, err.value
 
 
+@pytest.mark.parametrize("dtype", [L.BF16, L.F32])
+def test_operands_stay_within_32_bit_offsets(dtype):
+    """A tile of a product's operand is 256 rows at 32-bit byte offsets: batches whose transpose passes them are
+    refused, larger pieces cut, weights at larger pitches copied."""
+    both = {"hidden.dtype": dtype, "weight.dtype": dtype}
+    top = 2 ** 21
+    assert workspace(args(n=top, v=300, **both), 3)[0] == L.ORDA_OK
+    rc, _, err = workspace(args(n=top + 1, v=300, **both), 3)
+    assert rc == L.ORDA_ERR_INVALID and "2^21 rows" in err
+    # the gradient of a piece's logits is the largest part of the scratch
+    cut = workspace(args(n=512, v=4 * top, vocab_piece=top, **both), 3)[1]
+    assert cut >= 512 * top * 2
+    assert workspace(args(n=512, v=4 * top, vocab_piece=2 * top, **both), 3)[1] == cut
+    assert workspace(args(n=1, v=4 * top, **both), 3)[1] <= workspace(args(n=1, v=4 * top, vocab_piece=top, **both), 3)[1]
+    if dtype == L.BF16:
+        wide = workspace(args(v=1000, **{"weight.ld": 2 ** 20}), 3)[1]
+        assert workspace(args(v=1000, **{"weight.ld": 2 ** 20 + 8}), 3)[1] >= wide + 1000 * 8 * 2
+
+
 def test_python_refuses_cpu_tensors():
     h, w, y = torch.zeros(2, 8), torch.zeros(3, 8), torch.zeros(2, dtype=torch.int64)
     with pytest.raises(H.OrdaError, match="GPU tensor"):
