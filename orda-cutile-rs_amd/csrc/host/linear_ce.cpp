@@ -29,6 +29,7 @@ struct Ce {
   int64_t ldx, ldw;
   bool planes;       // fp32: every product over three-plane operands
   bool direct;       // small fp32 calls: the logits in memory, fp32 operands
+  bool few;          // bf16, few rows: the logits by waves of 16 classes
   bool stage_w;      // weights that the products cannot read in place
   bool gh, gw;       // backward: the gradients asked for
   bool backward;
@@ -40,11 +41,27 @@ int64_t ds_pitch(const Ce& c, int64_t cols) { return c.planes ? 3 * round64(cols
 
 int64_t column_bytes(const Ce& c) {   // of scratch, for each column of a piece
   int64_t b = c.planes ? 6 * c.hp : c.stage_w ? dtype_size(c.t) * c.hp : 0;
-  b += c.backward ? round64(c.n) * (c.planes ? 6 : 2) : (c.n * 16 + 255) / 256;
+  b += c.backward ? round64(c.n) * (c.planes ? 6 : 2) : c.few ? (c.n * 16 + 63) / 64 : (c.n * 16 + 255) / 256;
   return b;
 }
 
+int64_t stat_tiles(const Ce& c, int64_t cols) { return c.few ? ce_few_tiles(cols) : gemm_stat_tiles(cols); }
+
 void choose_direct(Ce& c);
+
+// Whether the logits of few rows go by waves of 16 classes: where that is quicker
+// than tiles of 256, each of which takes as long as K asks while fewer tiles than
+// CUs leave the memory idle. Both sides' us: 14334 x 4032, 18 rows 31 against 75;
+// 32000 x 2048, one row 23 against 41, 32 rows 47 against 40; 131072 x 4096, one row
+// 200 against 184 (all tiles' CUs at work: the weight at 5.8 TB/s).
+bool few_rows(const Ce& c) {
+  if (c.planes || c.n > kCeFewRows) return false;
+  const double terms = static_cast<double>(c.v) * static_cast<double>(c.hp);
+  const double few = terms * (c.n <= 16 ? 4.5e-7 : c.n <= 32 ? 6.9e-7 : 11.8e-7) + 2.0;
+  const double rounds = static_cast<double>(((c.v + 255) / 256 + 255) / 256);
+  const double tiles = std::max(rounds * (static_cast<double>(c.hp) * 0.0185 + 3.0), terms * 2 / 5.8e6);
+  return few < tiles;
+}
 
 Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool gw) {
   check_view(a.hidden, "hidden");
@@ -78,6 +95,7 @@ Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool
   c.backward = backward;
   c.gh = gh;
   c.gw = gw;
+  c.few = few_rows(c);
   // Pieces of whole column tiles, all but the last alike.
   int64_t most = a.vocab_piece > 0 ? a.vocab_piece : std::max<int64_t>(kPieceBytes / std::max<int64_t>(column_bytes(c), 1), 4096);
   most = std::max<int64_t>(std::min(most, kMaxPiece) / 256 * 256, 256);
@@ -186,6 +204,21 @@ GemmArgs grad_weight_product(const Ce& c, const Scratch& s, void* gw, int64_t ld
     g.plane_b = round64(c.piece);
   }
   return g;
+}
+
+// The same of few rows.
+CeFewArgs few_logits(const Ce& c, const Scratch& s, int64_t v0, int64_t cols) {
+  const GemmArgs g = logits_product(c, s, v0, cols);
+  CeFewArgs f{};
+  f.x = g.prob[0].a;
+  f.ldx = g.lda;
+  f.w = g.prob[0].b;
+  f.ldw = g.ldb;
+  f.k = c.hp;
+  f.cols = cols;
+  f.col0 = v0;
+  f.rows = s.rows;
+  return f;
 }
 
 // The direct form's products: fp32 operands, rows from the count on zeros.
@@ -318,7 +351,7 @@ Scratch lay_out(const Ce& c, void* base) {
   if (c.planes) s.w = take(round64(c.piece) * 6 * c.hp);
   else if (c.stage_w) s.w = take(c.piece * c.hp * 2);
   if (!c.backward) {
-    const int64_t tiles = gemm_stat_tiles(c.piece);
+    const int64_t tiles = stat_tiles(c, c.piece);
     s.stats = static_cast<float4*>(take(c.n * tiles * 16));
     s.state = static_cast<float4*>(c.piece < c.v ? take(c.n * 16) : nullptr);
     s.xy = static_cast<float*>(take(c.n * 4));
@@ -434,15 +467,24 @@ void forward(const orda_linear_ce& a, const Ce& c, const Scratch& s, float* nll,
   for (int64_t v0 = 0; v0 < c.v; v0 += c.piece) {
     const int64_t cols = std::min(c.piece, c.v - v0);
     stage_weights(c, s, v0, cols, st);
-    GemmArgs g = logits_product(c, s, v0, cols);
-    g.epi = GemmEpilogue::CeStats;
-    g.ce.stats = s.stats;
-    g.ce.stats_ld = gemm_stat_tiles(c.piece);
-    g.ce.xy = s.xy;
-    hip_check(launch_gemm(g, st), "linear cross entropy logits");
+    const int64_t stats_ld = stat_tiles(c, c.piece);
+    if (c.few) {
+      CeFewArgs f = few_logits(c, s, v0, cols);
+      f.stats = s.stats;
+      f.stats_ld = stats_ld;
+      f.xy = s.xy;
+      hip_check(launch_ce_few(f, c.n, false, st), "linear cross entropy logits");
+    } else {
+      GemmArgs g = logits_product(c, s, v0, cols);
+      g.epi = GemmEpilogue::CeStats;
+      g.ce.stats = s.stats;
+      g.ce.stats_ld = stats_ld;
+      g.ce.xy = s.xy;
+      hip_check(launch_gemm(g, st), "linear cross entropy logits");
+    }
     CeLossArgs l = losses(a, c, s, nll, lse);
-    l.stats_ld = g.ce.stats_ld;
-    l.tiles = gemm_stat_tiles(cols);
+    l.stats_ld = stats_ld;
+    l.tiles = stat_tiles(c, cols);
     l.first = v0 == 0;
     l.last = v0 + cols == c.v;
     hip_check(launch_ce_losses(l, c.n, st), "linear cross entropy losses");
@@ -476,14 +518,22 @@ void backward(const orda_linear_ce& a, const Ce& c, const Scratch& s, const CeGr
   for (int64_t v0 = 0; v0 < c.v; v0 += c.piece) {
     const int64_t cols = std::min(c.piece, c.v - v0);
     stage_weights(c, s, v0, cols, st);
-    GemmArgs g = logits_product(c, s, v0, cols);
-    g.epi = GemmEpilogue::CeGrad;
-    g.logits_type = DType::BF16;
-    g.prob[0].c = s.ds;
-    g.ldc = ds_pitch(c, c.piece);
-    g.ce.plane = round64(c.piece);
-    g.ce.coef = s.coef;
-    hip_check(launch_gemm(g, st), "linear cross entropy gradient");
+    if (c.few) {
+      CeFewArgs f = few_logits(c, s, v0, cols);
+      f.coef = s.coef;
+      f.ds = s.ds;
+      f.ldds = ds_pitch(c, c.piece);
+      hip_check(launch_ce_few(f, c.n, true, st), "linear cross entropy gradient");
+    } else {
+      GemmArgs g = logits_product(c, s, v0, cols);
+      g.epi = GemmEpilogue::CeGrad;
+      g.logits_type = DType::BF16;
+      g.prob[0].c = s.ds;
+      g.ldc = ds_pitch(c, c.piece);
+      g.ce.plane = round64(c.piece);
+      g.ce.coef = s.coef;
+      hip_check(launch_gemm(g, st), "linear cross entropy gradient");
+    }
     if (c.gh) hip_check(launch_gemm(grad_hidden_product(c, s, gh, v0, cols), st), "grad_hidden");
     if (c.gw) hip_check(launch_gemm(grad_weight_product(c, s, gw->data, tensor_ld(*gw), v0, cols), st), "grad_weight");
   }

@@ -460,6 +460,26 @@ struct CePrepArgs {
   int64_t cols;    // a workgroup's columns
 };
 hipError_t launch_ce_prep(const CePrepArgs& a, DType t, bool planes, hipStream_t stream);
+// The logits of at most kCeFewRows rows of bf16 against `cols` classes from col0 on:
+// their statistics (tiles of 64 classes, as CeArgs::stats) and xy, or with grad their
+// gradients in bf16 (zeros up to whole eights). x and w are 16-byte aligned, k and the
+// pitches multiples of 8.
+constexpr int64_t kCeFewRows = 64;
+struct CeFewArgs {
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw, k, cols, col0;
+  CeRows rows;
+  float4* stats;
+  int64_t stats_ld;
+  float* xy;
+  const float4* coef;
+  void* ds;
+  int64_t ldds;
+};
+int64_t ce_few_tiles(int64_t cols);
+hipError_t launch_ce_few(const CeFewArgs& a, int64_t n, bool grad, hipStream_t stream);
 // Merges a piece's tile statistics (CeArgs::stats) into state (between
 // pieces) and on the last piece writes the rows' losses.
 struct CeLossArgs {

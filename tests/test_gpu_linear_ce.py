@@ -315,3 +315,48 @@ def test_a_weight_at_a_wide_pitch():
     got = H.linear_cross_entropy_backward(h, w, y, lse, g)
     for a, b in zip(got, H.linear_cross_entropy_backward(h, w.contiguous(), y, lse, g)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("v, h", [(1000, 64), (4339, 520), (997, 200), (129, 8), (33, 1304), (2000, 264)])
+@pytest.mark.parametrize("n", [1, 16, 17, 32, 33, 64, 65])
+def test_few_rows(n, v, h):
+    """Rows by waves of 16 classes (up to 64 of them) beside the tiles' (65): widths of parts of 128 columns,
+    vocabularies of parts of 16 and 64 classes, ignored and bad labels, both outputs' gradients."""
+    g = torch.Generator().manual_seed(n * 7 + v)
+    x = (torch.randn(n, h, generator=g)).bfloat16().cuda()
+    w = (torch.randn(v, h, generator=g) * 0.2).bfloat16().cuda()
+    y = torch.randint(0, v, (n,), generator=g)
+    y[-1] = v - 1
+    if n > 8:
+        y[::5] = -100
+    y = y.cuda()
+    exact = Exact(x, w, y, label_smoothing=0.1)
+    nll, lse = H.linear_cross_entropy(x, w, y, label_smoothing=0.1)
+    exact.check_losses(nll, lse)
+    gn, gl = torch.randn(n, generator=g).cuda(), torch.randn(n, generator=g).cuda()
+    gh, gw = H.linear_cross_entropy_backward(x, w, y, lse, gn, gl, label_smoothing=0.1)
+    exact.check_gradients(gh, gw, gn, gl)
+    pieces = H.linear_cross_entropy(x, w, y, label_smoothing=0.1, vocab_piece=256)
+    exact.check_losses(*pieces)
+
+
+@pytest.mark.parametrize("n", [1, 40, 200])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_few_rows_of_infinite_logits(n, value):
+    """One class whose logit is infinite or NaN in every row: lse is what logsumexp gives."""
+    x = torch.zeros(n, 64, dtype=torch.bfloat16, device="cuda")
+    x[:, :2] = 1.0
+    w = torch.randn(500, 64, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    w[77, 0] = value
+    y = torch.full((n,), 3, device="cuda")
+    nll, lse = H.linear_cross_entropy(x, w, y)
+    logits = (w[:, 0].double() + w[:, 1].double()).cpu()
+    want = torch.logsumexp(logits, 0)
+    # (two exact terms a logit; 2^-22 an exponential, 64 + 1 additions, the maximum twice)
+    bound = 2.0 ** -22 + 70 * 2.0 ** -24 + 6 * 2.0 ** -24 * 8
+    if torch.isfinite(want):
+        assert ((lse.double().cpu() - want).abs() <= bound).all()
+        assert ((nll.double().cpu() - (want - logits[3])).abs() <= bound + 2.0 ** -24 * 16).all()
+    else:
+        assert torch.equal(lse.double().cpu(), want.expand(n)) or (torch.isnan(want) and torch.isnan(lse).all())
+        assert torch.equal(nll.isnan(), lse.isnan())
