@@ -7,6 +7,10 @@ The public surface mirrors the reference crate (src/lib.rs:57-64):
 ``ChunkPlan``, ``Teacher``, ``TeacherMode``, ``is_available`` and the
 resolver functions. Compute runs in liborda_hip.so through the C ABI of
 include/orda/orda.h; torch tensors (or numpy arrays) carry the memory.
+
+Beside it stand operators that the crate does not have (orda_hip/operators.py):
+``linear_cross_entropy``, ``embedding`` and their gradients,
+``quantize_fp8_blocks`` and ``fp8_block_matmul``, on torch's GPU tensors.
 """
 from __future__ import annotations
 
