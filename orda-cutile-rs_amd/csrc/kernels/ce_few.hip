@@ -6,7 +6,10 @@
 // all rows (F fragments of 16, from the caches) and loads the next 128 columns, or
 // two times 128, while it multiplies these; the workgroup's 64 classes are one tile
 // of statistics. A tile of the large product holds 256 classes, so that 14000
-// classes are 56 workgroups on 256 CUs.
+// classes are 56 workgroups on 256 CUs. One row at 32000 x 2048: 23 us, 5.8 TB/s (on
+// the tiles 41); 18 rows at 14334 x 4032 31 us, 3.7 TB/s (75), where the rows' way
+// from the second-level caches, as many bytes as the weight's for each 16 rows,
+// bounds it.
 #include <float.h>
 #include <math.h>
 

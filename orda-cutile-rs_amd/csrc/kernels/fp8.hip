@@ -61,8 +61,9 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float s, float r) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// kC neighbouring values from column c on (0 past cols) of N rows by one load each, aligned to their size or of any alignment. One branch
-// for all the rows: a branch around each load made it wait for the one before.
+// kC neighbouring values from column c on (0 past cols) of N rows by one load each,
+// aligned to their size or of any alignment. One branch for all the rows: a branch
+// around each load made it wait for the one before.
 template <typename E, int N, int kC, bool ALIGNED>
 __device__ __forceinline__ void load_rows(const E* const (&row)[N], int64_t c, int64_t cols, float (&x)[N][kC]) {
   E w[N][kC];

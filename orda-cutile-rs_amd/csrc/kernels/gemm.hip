@@ -1194,7 +1194,7 @@ __device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, int64_t M, cons
 //   two waves' halves merged through LDS, and the label's logit.
 //   CeGrad: d = p·2^(x·log2e - l) - u - y·[label], one fma, one exponential and
 //   one more fma an element, from the fp32 accumulators; stored rounded to bf16
-//   (the backward products' operand: relative 2^-9, independent from element to
+//   (the backward products' operand: relative 2^-8, independent from element to
 //   element, as the gradient rows of the distillation loss), or, for three-plane
 //   operands, as the three planes of the fp32 value, row r's at C + r*ldc, plane
 //   k another g.ce.plane further. Columns from N up to the multiple of 8 (planes: 64)
