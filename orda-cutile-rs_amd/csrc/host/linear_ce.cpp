@@ -407,16 +407,15 @@ void stage_weights(const Ce& c, const Scratch& s, int64_t v0, int64_t cols, hipS
                                  c.hp, st),
               "linear cross entropy weights");
   else if (c.stage_w)
-    hip_check(launch_convert_rows(DType::BF16, static_cast<const char*>(c.w) + v0 * c.ldw * 2, c.ldw, DType::BF16, s.w,
-                                  c.hp, cols, c.h, st),
+    hip_check(launch_ce_stage(DType::BF16, static_cast<const char*>(c.w) + v0 * c.ldw * 2, c.ldw, s.w, c.hp, cols, c.h,
+                              st),
               "linear cross entropy weights");
 }
 
 // The direct form's logits, the parts of a split product left apart.
 CeDirectArgs direct_logits(const orda_linear_ce& a, const Ce& c, const Scratch& s, hipStream_t st) {
   if (c.stage_w)
-    hip_check(launch_convert_rows(DType::F32, c.w, c.ldw, DType::F32, s.w, c.hp, c.v, c.h, st),
-              "linear cross entropy weights");
+    hip_check(launch_ce_stage(DType::F32, c.w, c.ldw, s.w, c.hp, c.v, c.h, st), "linear cross entropy weights");
   GemmArgs g = direct_logits_product(c, s);
   const GemmSplit plan = gemm_split_plan(g);
   g.partials_only = plan.splits > 1;

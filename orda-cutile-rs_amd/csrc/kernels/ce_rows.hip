@@ -240,6 +240,44 @@ __global__ __launch_bounds__(256) void ce_prep_kernel(CePrepArgs a) {
   }
 }
 
+// ------------------------------------------------------------ weights
+// Rows of any pitch and alignment at a pitch of whole 16 bytes, zeros past cols: a
+// wave a row, four 16-byte vectors a lane in flight, which need no alignment but
+// their elements'. Bound by HBM: 51192 x 2426 of bf16 84 us, 5.9 TB/s (with loads as
+// wide as a row's alignment allows, a vector a thread, 252).
+template <typename E>
+__global__ __launch_bounds__(256) void ce_stage_kernel(const E* src, int64_t lds, E* dst, int64_t ldd, int64_t rows,
+                                                       int64_t cols) {
+  constexpr int kV = 16 / sizeof(E), kLoads = 4, kStep = 64 * kV;
+  const int lane = threadIdx.x & 63;
+  const int64_t r = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const E* s = src + r * lds;
+  E* d = dst + r * ldd;
+  for (int64_t c = lane * kV; c < ldd; c += kLoads * kStep) {
+    u32x4 w[kLoads];
+    if (c + (kLoads - 1) * kStep + kV <= cols) {
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) __builtin_memcpy(&w[q], s + c + q * kStep, 16);
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) *reinterpret_cast<u32x4*>(d + c + q * kStep) = w[q];
+      continue;
+    }
+    for (int q = 0; q < kLoads; ++q) {
+      const int64_t at = c + q * kStep;
+      if (at >= ldd) break;
+      E x[kV];
+      if (at + kV <= cols) {
+        __builtin_memcpy(x, s + at, 16);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kV; ++k) x[k] = at + k < cols ? s[at + k] : E(0);
+      }
+      __builtin_memcpy(__builtin_assume_aligned(d + at, 16), x, 16);
+    }
+  }
+}
+
 // ------------------------------------------------------------ losses
 // A wave merges a row's tile statistics, the maximum first and then the sums
 // relative to it (the second read comes from the cache), and on the last piece
@@ -432,6 +470,21 @@ hipError_t launch_ce_prep(const CePrepArgs& in, DType t, bool planes, hipStream_
               : planes         ? pick(float{}, std::integral_constant<int, 1>{})
                                : pick(float{}, std::integral_constant<int, 0>{});
   hipLaunchKernelGGL(k, grid, dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_ce_stage(DType t, const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols,
+                           hipStream_t stream) {
+  if (rows <= 0 || cols <= 0) return hipSuccess;
+  if (ldd * dtype_size(t) % 16 != 0 || reinterpret_cast<uintptr_t>(dst) % 16 != 0 || ldd < cols)
+    return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
+  if (t == DType::BF16)
+    hipLaunchKernelGGL(ce_stage_kernel<uint16_t>, grid, dim3(256), 0, stream, static_cast<const uint16_t*>(src), lds,
+                       static_cast<uint16_t*>(dst), ldd, rows, cols);
+  else
+    hipLaunchKernelGGL(ce_stage_kernel<float>, grid, dim3(256), 0, stream, static_cast<const float*>(src), lds,
+                       static_cast<float*>(dst), ldd, rows, cols);
   return hipGetLastError();
 }
 

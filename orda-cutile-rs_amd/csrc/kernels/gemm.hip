@@ -644,10 +644,11 @@ __device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, int64_t M, cons
         for (int i = 0; i < MF; ++i) {
           const int64_t m = row_w + i * 16 + lgrp * 4;
           f32x4 v = acc[i][j];
-          if (vec && m + 4 <= M) {
-            if constexpr (Elem<LT>::kSize == 2) {
+          if ((vec || Elem<LT>::kSize == 2) && m + 4 <= M) {
+            if constexpr (Elem<LT>::kSize == 2) {   // 8 bytes at any alignment
               v = alpha * v;
-              *reinterpret_cast<u32x2*>(cn + m) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+              const u32x2 w = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+              __builtin_memcpy(cn + m, &w, 8);
             } else {
               f32x4* dst = reinterpret_cast<f32x4*>(cn + m);
               if constexpr (EPI == GemmEpilogue::AccumF32) v = alpha * (*dst + v);

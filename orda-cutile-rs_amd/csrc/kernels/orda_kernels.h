@@ -460,6 +460,9 @@ struct CePrepArgs {
   int64_t cols;    // a workgroup's columns
 };
 hipError_t launch_ce_prep(const CePrepArgs& a, DType t, bool planes, hipStream_t stream);
+// Rows of src at a pitch of whole 16 bytes, zeros past cols.
+hipError_t launch_ce_stage(DType t, const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols,
+                           hipStream_t stream);
 // The logits of at most kCeFewRows rows of bf16 against `cols` classes from col0 on:
 // their statistics (tiles of 64 classes, as CeArgs::stats) and xy, or with grad their
 // gradients in bf16 (zeros up to whole eights). x and w are 16-byte aligned, k and the

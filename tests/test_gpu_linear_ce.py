@@ -360,3 +360,22 @@ def test_few_rows_of_infinite_logits(n, value):
     else:
         assert torch.equal(lse.double().cpu(), want.expand(n)) or (torch.isnan(want) and torch.isnan(lse).all())
         assert torch.equal(nll.isnan(), lse.isnan())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("at", [0, 1, 3])
+@pytest.mark.parametrize("n, h, v", [(5, 2426, 300), (90, 2051, 333), (5, 1543, 77), (3, 4099, 130), (200, 2050, 65)])
+def test_widths_that_are_copied(n, h, v, at, dtype):
+    """Weights whose rows begin anywhere, wider than a wave's vectors, between NaN on both sides."""
+    g = torch.Generator().manual_seed(n + h)
+    frame = torch.full((v, h + 9), float("nan"), dtype=dtype, device="cuda")
+    w = frame[:, at:at + h]
+    w.copy_((torch.randn(v, h, generator=g) * 0.1).to(dtype))
+    x = torch.randn(n, h, generator=g).to(dtype).cuda()
+    y = torch.randint(0, v, (n,), generator=g).cuda()
+    exact = Exact(x, w, y)
+    nll, lse = H.linear_cross_entropy(x, w, y)
+    exact.check_losses(nll, lse)
+    gn = torch.randn(n, generator=g).cuda()
+    gh, gw = H.linear_cross_entropy_backward(x, w, y, lse, gn)
+    exact.check_gradients(gh, gw, gn, torch.zeros_like(gn))
