@@ -330,7 +330,7 @@ typedef struct {
     orda_tensor weight;      /* [V,H], the same type; read in place where it is
                                 fp32, or 16-byte aligned with H and ld multiples
                                 of 8 and ld at most 2^20, else copied a piece at
-                                a time */
+                                a time where a product needs it */
     const int64_t *labels;   /* [N] */
     int64_t n_labels;
     int64_t ignore_index;

@@ -29,7 +29,7 @@ struct Ce {
   int64_t ldx, ldw;
   bool planes;       // fp32: every product over three-plane operands
   bool direct;       // small fp32 calls: the logits in memory, fp32 operands
-  bool few;          // bf16, few rows: the logits by waves of 16 classes
+  bool few;          // few rows (bf16, or direct): the logits by waves of 16 classes
   bool stage_w;      // weights that the products cannot read in place
   bool gh, gw;       // backward: the gradients asked for
   bool backward;
@@ -45,22 +45,38 @@ int64_t column_bytes(const Ce& c) {   // of scratch, for each column of a piece
   return b;
 }
 
-int64_t stat_tiles(const Ce& c, int64_t cols) { return c.few ? ce_few_tiles(cols) : gemm_stat_tiles(cols); }
+int64_t stat_tiles(const Ce& c, int64_t cols) {
+  return c.few ? ce_few_tiles(cols) : c.direct ? ce_direct_tiles(cols) : gemm_stat_tiles(cols);
+}
 
 void choose_direct(Ce& c);
 
-// Whether the logits of few rows go by waves of 16 classes: where that is quicker
-// than tiles of 256, each of which takes as long as K asks while fewer tiles than
-// CUs leave the memory idle. Both sides' us: 14334 x 4032, 18 rows 31 against 75;
-// 32000 x 2048, one row 23 against 41, 32 rows 47 against 40; 131072 x 4096, one row
-// 200 against 184 (all tiles' CUs at work: the weight at 5.8 TB/s).
+// us of the logits of few rows by waves of 16 classes: the weight's bytes at the rate
+// that the rows' way from the caches leaves, or a wave's own way through K. fp32
+// (beside fp32 tiles): 32000 x 4096, one row 117 (531), 64 rows 333 (546); 8000 x
+// 1024, 64 rows 49 (31, taken).
+double few_us(const Ce& c) {
+  const bool f32 = c.t == DType::F32;
+  const double terms = static_cast<double>(c.v) * static_cast<double>(c.h) * (f32 ? 2.0 : 1.0);
+  const double all = terms * (c.n <= 16 ? 4.5e-7 : c.n <= 32 ? 6.9e-7 : 11.8e-7) + 2.0;
+  const double f = c.n <= 16 ? 1.0 : c.n <= 32 ? 2.0 : 4.0;
+  const double wave = static_cast<double>(c.h) * (f32 ? (0.5 + 0.62 * f) / 64 : (0.35 + 0.5 * f) / 128);
+  return std::max(all, wave);
+}
+
+// Whether bf16 logits of few rows go that way: where it is quicker than tiles of
+// 256, each of which takes as long as K asks while fewer tiles than CUs leave the
+// memory idle. Both sides' us: 14334 x 4032, 18 rows 31 against 75; 32000 x 2048, one
+// row 23 against 41, 32 rows 47 against 40; 2000 x 4096, 16 rows 31 against 70, 64
+// rows 74 against 70; 131072 x 4096, one row 200 against 184 (all tiles' CUs at work:
+// the weight at 5.8 TB/s). Weights that the tiles cannot read in place take a copy
+// first, 5.9 TB/s.
 bool few_rows(const Ce& c) {
   if (c.planes || c.n > kCeFewRows) return false;
   const double terms = static_cast<double>(c.v) * static_cast<double>(c.hp);
-  const double few = terms * (c.n <= 16 ? 4.5e-7 : c.n <= 32 ? 6.9e-7 : 11.8e-7) + 2.0;
   const double rounds = static_cast<double>(((c.v + 255) / 256 + 255) / 256);
-  const double tiles = std::max(rounds * (static_cast<double>(c.hp) * 0.0185 + 3.0), terms * 2 / 5.8e6);
-  return few < tiles;
+  const double tiles = std::max(rounds * (static_cast<double>(c.hp) * 0.0155 + 8.0), terms * 2 / 5.8e6);
+  return few_us(c) < tiles + (c.stage_w && !c.gh ? terms * 4 / 5.9e6 : 0.0);
 }
 
 Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool gw) {
@@ -206,18 +222,23 @@ GemmArgs grad_weight_product(const Ce& c, const Scratch& s, void* gw, int64_t ld
   return g;
 }
 
-// The same of few rows.
+// The same of few rows, the weights read where they are.
 CeFewArgs few_logits(const Ce& c, const Scratch& s, int64_t v0, int64_t cols) {
-  const GemmArgs g = logits_product(c, s, v0, cols);
   CeFewArgs f{};
-  f.x = g.prob[0].a;
-  f.ldx = g.lda;
-  f.w = g.prob[0].b;
-  f.ldw = g.ldb;
-  f.k = c.hp;
+  f.x = s.x;
+  f.ldx = c.hp;
+  f.w = static_cast<const char*>(c.w) + v0 * c.ldw * dtype_size(c.t);
+  f.ldw = c.ldw;
+  f.n = c.n;
+  f.k = c.h;
   f.cols = cols;
   f.col0 = v0;
   f.rows = s.rows;
+  f.xy = s.xy;
+  f.coef = s.coef;
+  f.stats = s.stats;
+  f.stats_ld = stat_tiles(c, c.piece);
+  f.ds = s.ds;
   return f;
 }
 
@@ -291,8 +312,11 @@ void choose_direct(Ce& c) {
   d.planes = false;
   d.hp = round8(c.h);
   const Scratch none{};
-  double direct = gemm_us(direct_logits_product(d, none)) + static_cast<double>(c.n) * c.v * 8 * 0.25e-6 + 4.0 +
-                  (c.stage_w ? static_cast<double>(c.v) * c.h * 8 * 0.25e-6 : 0.0);
+  double logits = gemm_us(direct_logits_product(d, none)) + static_cast<double>(c.n) * c.v * 8 * 0.25e-6 + 4.0;
+  d.few = c.n <= kCeFewRows && few_us(d) < logits;
+  if (d.few) logits = few_us(d);
+  double direct = logits;
+  if (c.stage_w && (!d.few || c.gh)) direct += static_cast<double>(c.v) * c.h * 8 * 0.25e-6;
   if (c.backward) {
     const double kv = static_cast<double>(c.v);
     // over planes K is split until the chip is full
@@ -300,13 +324,17 @@ void choose_direct(Ce& c) {
     if (c.gw) planes += std::max(tiles(c.h, c.v) / 256.0, 1.0) * (round64(c.n) / 32.0 * 4.2 + 12.0);
     if (c.gh) direct += gemm_us(direct_hidden_product(d, none)) + 4.0;
     if (c.gw) direct += gemm_us(direct_weight_product(d, none, nullptr, c.h));
-    direct += static_cast<double>(c.n) * c.v * 8 * 0.25e-6;
+    if (!d.few) direct += static_cast<double>(c.n) * c.v * 8 * 0.25e-6;
   }
   if (direct >= planes) return;
   c.planes = false;
   c.direct = true;
+  c.few = d.few;
   c.hp = round8(c.h);
 }
+
+// Weights that the products cannot read in place (few rows' logits can).
+bool copies_weight(const Ce& c) { return c.stage_w && (!c.few || c.gh); }
 
 // (Sizes depend on which pointers are set, so a layout is made from a base that
 // is not null also where only its size counts.)
@@ -326,11 +354,13 @@ Scratch lay_out(const Ce& c, void* base) {
   s.x = take(np * c.hp * (c.planes ? 6 : dtype_size(c.t)));
   if (c.direct) {
     const int64_t ld = direct_pitch(c);
-    s.logits = static_cast<float*>(take(c.n * ld * 4));
-    if (c.stage_w) s.w = take(c.v * c.hp * 4);
-    s.split_bytes = gemm_split_bytes(direct_logits_product(c, s));
+    if (copies_weight(c)) s.w = take(c.v * c.hp * 4);
+    if (!c.few) {
+      s.logits = static_cast<float*>(take(c.n * ld * 4));
+      s.split_bytes = gemm_split_bytes(direct_logits_product(c, s));
+    }
     if (!c.backward) {
-      s.stats = static_cast<float4*>(take(c.n * ce_direct_tiles(c.v) * 16));
+      s.stats = static_cast<float4*>(take(c.n * stat_tiles(c, c.v) * 16));
       s.xy = static_cast<float*>(take(c.n * 4));
     } else {
       s.coef = static_cast<float4*>(take(c.n * 16));
@@ -349,7 +379,7 @@ Scratch lay_out(const Ce& c, void* base) {
     return s;
   }
   if (c.planes) s.w = take(round64(c.piece) * 6 * c.hp);
-  else if (c.stage_w) s.w = take(c.piece * c.hp * 2);
+  else if (copies_weight(c)) s.w = take(c.piece * c.hp * 2);
   if (!c.backward) {
     const int64_t tiles = stat_tiles(c, c.piece);
     s.stats = static_cast<float4*>(take(c.n * tiles * 16));
@@ -406,16 +436,19 @@ void stage_weights(const Ce& c, const Scratch& s, int64_t v0, int64_t cols, hipS
     hip_check(launch_split3_rows(static_cast<const float*>(c.w) + v0 * c.ldw, c.ldw, cols, c.h, s.w, round64(cols),
                                  c.hp, st),
               "linear cross entropy weights");
-  else if (c.stage_w)
+  else if (copies_weight(c))
     hip_check(launch_ce_stage(DType::BF16, static_cast<const char*>(c.w) + v0 * c.ldw * 2, c.ldw, s.w, c.hp, cols, c.h,
                               st),
               "linear cross entropy weights");
 }
 
-// The direct form's logits, the parts of a split product left apart.
-CeDirectArgs direct_logits(const orda_linear_ce& a, const Ce& c, const Scratch& s, hipStream_t st) {
-  if (c.stage_w)
+void stage_direct(const Ce& c, const Scratch& s, hipStream_t st) {
+  if (copies_weight(c))
     hip_check(launch_ce_stage(DType::F32, c.w, c.ldw, s.w, c.hp, c.v, c.h, st), "linear cross entropy weights");
+}
+
+// The direct form's logits, the parts of a split product left apart.
+CeDirectArgs direct_logits(const Ce& c, const Scratch& s, hipStream_t st) {
   GemmArgs g = direct_logits_product(c, s);
   const GemmSplit plan = gemm_split_plan(g);
   g.partials_only = plan.splits > 1;
@@ -428,7 +461,7 @@ CeDirectArgs direct_logits(const orda_linear_ce& a, const Ce& c, const Scratch& 
   d.stride = plan.splits > 1 ? plan.stride : 0;
   d.splits = plan.splits > 1 ? plan.splits : 1;
   d.stats = s.stats;
-  d.stats_ld = ce_direct_tiles(c.v);
+  d.stats_ld = stat_tiles(c, c.v);
   d.xy = s.xy;
   d.coef = s.coef;
   d.grad = static_cast<float*>(s.ds);
@@ -456,10 +489,11 @@ void forward(const orda_linear_ce& a, const Ce& c, const Scratch& s, float* nll,
   p.lse_out = lse;
   hip_check(launch_ce_prep(p, c.t, c.planes, st), "linear cross entropy rows");
   if (c.direct) {
-    const CeDirectArgs d = direct_logits(a, c, s, st);
-    hip_check(launch_ce_direct(d, c.n, false, st), "linear cross entropy losses");
+    stage_direct(c, s, st);
+    if (c.few) hip_check(launch_ce_few(few_logits(c, s, 0, c.v), c.t, false, st), "linear cross entropy logits");
+    else hip_check(launch_ce_direct(direct_logits(c, s, st), c.n, false, st), "linear cross entropy losses");
     CeLossArgs l = losses(a, c, s, nll, lse);
-    l.stats_ld = l.tiles = d.stats_ld;
+    l.stats_ld = l.tiles = stat_tiles(c, c.v);
     hip_check(launch_ce_losses(l, c.n, st), "linear cross entropy losses");
     return;
   }
@@ -468,11 +502,7 @@ void forward(const orda_linear_ce& a, const Ce& c, const Scratch& s, float* nll,
     stage_weights(c, s, v0, cols, st);
     const int64_t stats_ld = stat_tiles(c, c.piece);
     if (c.few) {
-      CeFewArgs f = few_logits(c, s, v0, cols);
-      f.stats = s.stats;
-      f.stats_ld = stats_ld;
-      f.xy = s.xy;
-      hip_check(launch_ce_few(f, c.n, false, st), "linear cross entropy logits");
+      hip_check(launch_ce_few(few_logits(c, s, v0, cols), c.t, false, st), "linear cross entropy logits");
     } else {
       GemmArgs g = logits_product(c, s, v0, cols);
       g.epi = GemmEpilogue::CeStats;
@@ -505,7 +535,14 @@ void backward(const orda_linear_ce& a, const Ce& c, const Scratch& s, const CeGr
   }
   hip_check(launch_ce_prep(p, c.t, c.planes, st), "linear cross entropy rows");
   if (c.direct) {
-    hip_check(launch_ce_direct(direct_logits(a, c, s, st), c.n, true, st), "linear cross entropy gradient");
+    stage_direct(c, s, st);
+    if (c.few) {
+      CeFewArgs f = few_logits(c, s, 0, c.v);
+      f.ldds = direct_pitch(c);
+      hip_check(launch_ce_few(f, c.t, true, st), "linear cross entropy gradient");
+    } else {
+      hip_check(launch_ce_direct(direct_logits(c, s, st), c.n, true, st), "linear cross entropy gradient");
+    }
     if (c.gh) {
       hip_check(launch_gemm(direct_hidden_product(c, s), st), "grad_hidden");
       hip_check(launch_ce_scatter(s.gh, round8(c.h), s.rows, c.n, c.h, static_cast<float*>(gh->data), tensor_ld(*gh), st),
@@ -519,10 +556,8 @@ void backward(const orda_linear_ce& a, const Ce& c, const Scratch& s, const CeGr
     stage_weights(c, s, v0, cols, st);
     if (c.few) {
       CeFewArgs f = few_logits(c, s, v0, cols);
-      f.coef = s.coef;
-      f.ds = s.ds;
       f.ldds = ds_pitch(c, c.piece);
-      hip_check(launch_ce_few(f, c.n, true, st), "linear cross entropy gradient");
+      hip_check(launch_ce_few(f, c.t, true, st), "linear cross entropy gradient");
     } else {
       GemmArgs g = logits_product(c, s, v0, cols);
       g.epi = GemmEpilogue::CeGrad;

@@ -463,16 +463,17 @@ hipError_t launch_ce_prep(const CePrepArgs& a, DType t, bool planes, hipStream_t
 // Rows of src at a pitch of whole 16 bytes, zeros past cols.
 hipError_t launch_ce_stage(DType t, const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols,
                            hipStream_t stream);
-// The logits of at most kCeFewRows rows of bf16 against `cols` classes from col0 on:
-// their statistics (tiles of 64 classes, as CeArgs::stats) and xy, or with grad their
-// gradients in bf16 (zeros up to whole eights). x and w are 16-byte aligned, k and the
-// pitches multiples of 8.
+// The logits of at most kCeFewRows rows against `cols` classes from col0 on: their
+// statistics (tiles of 64 classes, as CeArgs::stats) and xy, or with grad their
+// gradients: in bf16 rows up to the count and zeros up to whole eights of columns; in
+// fp32 all n rows (zeros from the count on) and whole fours. x is 16-byte aligned at
+// a pitch of whole vectors, zeros past k.
 constexpr int64_t kCeFewRows = 64;
 struct CeFewArgs {
   const void* x;
   int64_t ldx;
   const void* w;
-  int64_t ldw, k, cols, col0;
+  int64_t ldw, n, k, cols, col0;
   CeRows rows;
   float4* stats;
   int64_t stats_ld;
@@ -482,7 +483,7 @@ struct CeFewArgs {
   int64_t ldds;
 };
 int64_t ce_few_tiles(int64_t cols);
-hipError_t launch_ce_few(const CeFewArgs& a, int64_t n, bool grad, hipStream_t stream);
+hipError_t launch_ce_few(const CeFewArgs& a, DType t, bool grad, hipStream_t stream);
 // Merges a piece's tile statistics (CeArgs::stats) into state (between
 // pieces) and on the last piece writes the rows' losses.
 struct CeLossArgs {

@@ -317,14 +317,15 @@ def test_a_weight_at_a_wide_pitch():
         assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("v, h", [(1000, 64), (4339, 520), (997, 200), (129, 8), (33, 1304), (2000, 264)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("v, h", [(1000, 64), (4339, 520), (997, 200), (129, 8), (33, 1304), (2000, 264), (700, 1003), (301, 67)])
 @pytest.mark.parametrize("n", [1, 16, 17, 32, 33, 64, 65])
-def test_few_rows(n, v, h):
+def test_few_rows(n, v, h, dtype):
     """Rows by waves of 16 classes (up to 64 of them) beside the tiles' (65): widths of parts of 128 columns,
     vocabularies of parts of 16 and 64 classes, ignored and bad labels, both outputs' gradients."""
     g = torch.Generator().manual_seed(n * 7 + v)
-    x = (torch.randn(n, h, generator=g)).bfloat16().cuda()
-    w = (torch.randn(v, h, generator=g) * 0.2).bfloat16().cuda()
+    x = (torch.randn(n, h, generator=g)).to(dtype).cuda()
+    w = (torch.randn(v, h, generator=g) * 0.2).to(dtype).cuda()
     y = torch.randint(0, v, (n,), generator=g)
     y[-1] = v - 1
     if n > 8:
