@@ -139,3 +139,27 @@ def test_a_serving_step_captured():
         torch.cuda.synchronize()
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once():
+    """Each call's scratch is its own: interleaved on two streams, the results of one after the other."""
+    a, b = parts(torch.bfloat16, n=700, v=3000, h=256), parts(torch.float32, n=90, v=900, h=64)
+
+    def calls(p):
+        ids, labels, weight, _, rows, head = p
+        x = H.embedding(ids, weight, scale=SCALE)
+        nll, lse = H.linear_cross_entropy(x, weight, labels)
+        gh, gw = H.linear_cross_entropy_backward(x, weight, labels, lse, torch.ones_like(nll), lse)
+        return x, nll, lse, gh, gw, H.embedding_backward(gh, ids, weight.size(0)), teacher_logits(rows, head)
+
+    want = [calls(a), calls(b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(6):
+        for s, p in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                got.append(calls(p))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert all(torch.equal(x, y) for x, y in zip(out, want[i % 2]))
