@@ -39,8 +39,11 @@ struct Ce {
 
 int64_t ds_pitch(const Ce& c, int64_t cols) { return c.planes ? 3 * round64(cols) : logits_pitch(cols, DType::BF16); }
 
+// Weights that the products cannot read in place (few rows' logits can).
+bool copies_weight(const Ce& c) { return c.stage_w && (!c.few || c.gh); }
+
 int64_t column_bytes(const Ce& c) {   // of scratch, for each column of a piece
-  int64_t b = c.planes ? 6 * c.hp : c.stage_w ? dtype_size(c.t) * c.hp : 0;
+  int64_t b = c.planes ? 6 * c.hp : copies_weight(c) ? dtype_size(c.t) * c.hp : 0;
   b += c.backward ? round64(c.n) * (c.planes ? 6 : 2) : c.few ? (c.n * 16 + 63) / 64 : (c.n * 16 + 255) / 256;
   return b;
 }
@@ -49,7 +52,8 @@ int64_t stat_tiles(const Ce& c, int64_t cols) {
   return c.few ? ce_few_tiles(cols) : c.direct ? ce_direct_tiles(cols) : gemm_stat_tiles(cols);
 }
 
-void choose_direct(Ce& c);
+void choose_direct(Ce& c, bool one_piece);
+int64_t scratch_bytes(const Ce& c);
 
 // us of the logits of few rows by waves of 16 classes: the weight's bytes at the rate
 // that the rows' way from the caches leaves, or a wave's own way through K. fp32
@@ -117,7 +121,8 @@ Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool
   most = std::max<int64_t>(std::min(most, kMaxPiece) / 256 * 256, 256);
   const int64_t pieces = (c.v + most - 1) / most;
   c.piece = pieces == 1 ? c.v : ((c.v + pieces - 1) / pieces + 255) / 256 * 256;
-  choose_direct(c);
+  // (The planes' scratch cuts pieces that the direct form, which makes no planes, does not need.)
+  choose_direct(c, c.v <= (a.vocab_piece > 0 ? c.piece : kMaxPiece));
   return c;
 }
 
@@ -301,9 +306,13 @@ GemmArgs direct_weight_product(const Ce& c, const Scratch& s, void* gw, int64_t 
 // the logits' way through memory. Both sides by the products' own measure
 // (gemm_us; 4.2 us for every 32 elements of K and 20 us a round of 256 tiles over
 // planes) and 4 TB/s: 256 x 512 x 8192, forward and backward, 250 us of kernels
-// over planes.
-void choose_direct(Ce& c) {
-  if (!c.planes || c.piece < c.v || c.n > 8192) return;
+// over planes. It takes the vocabulary in one piece (one_piece: the caller allows
+// that), and where the planes would be cut by their scratch, it stays within the
+// same bound itself: the losses of one row at 131072 x 4096 take 1 MB and 0.45 ms (the
+// planes 770 MB and 2.45), of 64 rows 1.21 ms (2.47), both gradients too 2.1 (4.1) and
+// 3.2 (4.4).
+void choose_direct(Ce& c, bool one_piece) {
+  if (!c.planes || !one_piece || c.n > 8192) return;
   const double pass = (static_cast<double>(c.v) + c.n) * c.h * 10 * 0.25e-6;
   auto tiles = [](int64_t m, int64_t n) { return (m + 255) / 256 * ((n + 255) / 256); };
   auto rounds = [](int64_t t, int64_t k) { return static_cast<double>((t + 255) / 256) * (k / 32.0 * 4.2 + 20.0); };
@@ -327,14 +336,11 @@ void choose_direct(Ce& c) {
     if (!d.few) direct += static_cast<double>(c.n) * c.v * 8 * 0.25e-6;
   }
   if (direct >= planes) return;
-  c.planes = false;
-  c.direct = true;
-  c.few = d.few;
-  c.hp = round8(c.h);
+  d.direct = true;
+  const bool cut = c.piece < c.v;
+  d.piece = d.v;
+  if (!cut || scratch_bytes(d) <= kPieceBytes) c = d;
 }
-
-// Weights that the products cannot read in place (few rows' logits can).
-bool copies_weight(const Ce& c) { return c.stage_w && (!c.few || c.gh); }
 
 // (Sizes depend on which pointers are set, so a layout is made from a base that
 // is not null also where only its size counts.)

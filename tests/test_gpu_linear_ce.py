@@ -380,3 +380,17 @@ def test_widths_that_are_copied(n, h, v, at, dtype):
     gn = torch.randn(n, generator=g).cuda()
     gh, gw = H.linear_cross_entropy_backward(x, w, y, lse, gn)
     exact.check_gradients(gh, gw, gn, torch.zeros_like(gn))
+
+
+@pytest.mark.parametrize("n, h, v", [(3, 4096, 44000), (64, 1000, 180001)])
+def test_few_fp32_rows_of_a_large_weight(n, h, v):
+    """Weights that three planes would cut into pieces: few rows stream them whole, odd vocabularies too."""
+    g = torch.Generator(device="cuda").manual_seed(n + h)
+    x = torch.randn(n, h, generator=g, device="cuda")
+    w = torch.randn(v, h, generator=g, device="cuda") * (2.0 / h ** 0.5)
+    y = torch.randint(0, v, (n,), generator=g, device="cuda")
+    y[0] = v - 1
+    if n > 8:
+        y[1::5] = -100
+    gn, gl = torch.randn(n, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda")
+    check(x, w, y, gn, gl, label_smoothing=0.1)

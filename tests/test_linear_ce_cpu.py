@@ -134,3 +134,24 @@ def test_python_refuses_cpu_tensors():
         H.linear_cross_entropy(h, w, y)
     with pytest.raises(H.OrdaError, match="GPU tensor"):
         H.linear_cross_entropy_backward(h, w, y, torch.zeros(2), torch.zeros(2))
+
+
+@pytest.mark.parametrize("v, h", [(32000, 4096), (44000, 4096), (50257, 4096), (131072, 2048), (131072, 4096), (2 ** 20, 512)])
+@pytest.mark.parametrize("n", [1, 16, 64])
+def test_few_fp32_rows_take_no_planes(n, v, h):
+    """Few fp32 rows stream the weight whatever its size: the scratch holds the rows and 16 bytes of statistics for
+    each of them and 64 classes (with gradients their logits' rows and split products), not the weight."""
+    f32 = {"hidden.dtype": L.F32, "weight.dtype": L.F32}
+    need = workspace(args(n=n, h=h, v=v, **f32))[1]
+    assert need <= 2 * n * (v / 64 + 1) * 16 + 4 * 64 * h + (1 << 16)
+    whole = workspace(args(n=n, h=h, v=v, vocab_piece=v // 256 * 256 + 256, **f32))[1]
+    assert need == whole
+    assert workspace(args(n=n, h=h, v=v, **f32), 2)[1] <= 4 * n * (v + 2048) * 2 + 4 * 64 * 2 * h + (1 << 20)
+    assert workspace(args(n=n, h=h, v=v, **f32), 3)[1] <= 1 << 30
+
+
+def test_asked_for_pieces_are_kept():
+    """vocab_piece bounds the scratch of fp32 calls too: smaller pieces, less of it."""
+    f32 = {"hidden.dtype": L.F32, "weight.dtype": L.F32}
+    sizes = [workspace(args(n=512, h=4096, v=131072, vocab_piece=p, **f32), 3)[1] for p in (256, 4096, 16384, 65536)]
+    assert sizes == sorted(sizes) and sizes[0] < sizes[-1]
