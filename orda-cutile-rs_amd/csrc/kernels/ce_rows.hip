@@ -514,10 +514,16 @@ hipError_t launch_ce_scatter(const float* src, int64_t lds, const CeRows& r, int
 }
 
 hipError_t launch_zero_rows(DType t, void* p, int64_t ld, int64_t rows, int64_t cols, hipStream_t stream) {
-  if (t == DType::BF16)
-    hipLaunchKernelGGL(zero_rows_kernel<uint16_t>, dim3(row_blocks(rows)), dim3(256), 0, stream, static_cast<uint16_t*>(p), ld, rows, cols);
-  else
-    hipLaunchKernelGGL(zero_rows_kernel<uint32_t>, dim3(row_blocks(rows)), dim3(256), 0, stream, static_cast<uint32_t*>(p), ld, rows, cols);
+  auto run = [&](auto* d) {
+    using E = std::remove_pointer_t<decltype(d)>;
+    constexpr int64_t kMost = most_blocks(256) * 4;   // rows of a launch
+    for (int64_t r = 0; r < rows; r += kMost) {
+      const int64_t m = rows - r < kMost ? rows - r : kMost;
+      hipLaunchKernelGGL(zero_rows_kernel<E>, dim3(row_blocks(m)), dim3(256), 0, stream, d + r * ld, ld, m, cols);
+    }
+  };
+  if (t == DType::BF16) run(static_cast<uint16_t*>(p));
+  else run(static_cast<uint32_t*>(p));
   return hipGetLastError();
 }
 

@@ -449,13 +449,16 @@ hipError_t launch_embedding(DType t, const void* ids, bool ids64, int64_t n, con
   if (n <= 0 || h <= 0) return hipSuccess;
   const int64_t es = dtype_size(t);
   const int64_t parts = (h * es + kLookBytes - 1) / kLookBytes;
-  const int64_t blocks = (n * parts + 3) / 4;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  const int64_t most = most_blocks(256) * 4 / parts;   // tokens of a launch
   auto run = [&](auto* e, auto* i) {
     using E = std::remove_pointer_t<decltype(e)>;
     using I = std::remove_pointer_t<decltype(i)>;
-    hipLaunchKernelGGL((embedding_kernel<E, I>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, static_cast<const I*>(ids), n,
-                       static_cast<const E*>(w), ldw, v, h, scale, static_cast<E*>(out), ldo, parts);
+    for (int64_t t = 0; t < n; t += most) {
+      const int64_t m = n - t < most ? n - t : most;
+      hipLaunchKernelGGL((embedding_kernel<E, I>), dim3(static_cast<unsigned>((m * parts + 3) / 4)), dim3(256), 0, stream,
+                         static_cast<const I*>(ids) + t, m, static_cast<const E*>(w), ldw, v, h, scale,
+                         static_cast<E*>(out) + t * ldo, ldo, parts);
+    }
   };
   int64_t* i64 = nullptr;
   int32_t* i32 = nullptr;
@@ -556,7 +559,7 @@ hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t
   const int64_t row = a.ldo * dtype_size(out);
   a.stream = a.v * row > kStreamBytes && row % 128 == 0 && reinterpret_cast<uintptr_t>(a.out) % 128 == 0;
   const int64_t sum = (a.chunks * a.slabs + 3) / 4, join = ((a.chunks - 1) * a.slabs + 3) / 4;
-  if (sum > 0x7fffffff) return hipErrorInvalidValue;
+  if (sum > most_blocks(256)) return hipErrorInvalidValue;   // 68 GB of fp32 parts: more than the gradients that fit
   auto run = [&](auto* e, auto* o) {
     using E = std::remove_pointer_t<decltype(e)>;
     using O = std::remove_pointer_t<decltype(o)>;

@@ -726,8 +726,8 @@ bool few_rows(const Fp8MmArgs& a, bool wide) {
 hipError_t launch_fp8_quant(const Fp8QuantArgs& a, DType t, bool blocks, hipStream_t stream) {
   if (a.rows <= 0 || a.cols <= 0) return hipSuccess;
   if (a.ldc % 8 != 0 || reinterpret_cast<uintptr_t>(a.codes) % 8 != 0) return hipErrorInvalidValue;
-  const int64_t grid = blocks ? (a.rows + 127) / 128 * ((a.cols + 127) / 128) : (a.rows + 15) / 16 * ((a.cols + 511) / 512);
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  const int64_t each = blocks ? 128 : 16, across = blocks ? (a.cols + 127) / 128 : (a.cols + 511) / 512;
+  const int64_t most = most_blocks(256) / across * each;   // rows of a launch
   using K = void (*)(Fp8QuantArgs);
   const int64_t at = reinterpret_cast<uintptr_t>(a.src) | static_cast<uint64_t>(a.lds * dtype_size(t));
   K k;
@@ -739,7 +739,14 @@ hipError_t launch_fp8_quant(const Fp8QuantArgs& a, DType t, bool blocks, hipStre
            : at % 8 == 0 ? fp8_quant_blocks_kernel<__bf16, 4, true>
            : at % 4 == 0 ? fp8_quant_blocks_kernel<__bf16, 2, true>
                          : fp8_quant_blocks_kernel<__bf16, 8, false>;
-  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, a);
+  for (int64_t r = 0; r < a.rows; r += most) {
+    Fp8QuantArgs p = a;
+    p.rows = a.rows - r < most ? a.rows - r : most;
+    p.src = static_cast<const char*>(a.src) + r * a.lds * dtype_size(t);
+    p.codes = a.codes + r * a.ldc;
+    p.scales = a.scales + r / (blocks ? 128 : 1) * a.scale_row;
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((p.rows + each - 1) / each * across)), dim3(256), 0, stream, p);
+  }
   return hipGetLastError();
 }
 
@@ -759,13 +766,20 @@ hipError_t launch_fp8_mm(const Fp8MmArgs& a, DType out, hipStream_t stream) {
       reinterpret_cast<uintptr_t>(a.b) % 16 != 0)
     return hipErrorInvalidValue;
   if (few_rows(a, out == DType::F32)) {
-    const int64_t waves = (a.n + 15) / 16;
     auto* k = out == DType::BF16 ? few_kernel<__bf16, false>(a.m) : few_kernel<float, true>(a.m);
-    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, stream, a);
+    constexpr int64_t kMost = most_blocks(256) / 2 * 128;   // columns of a launch, whole blocks of B
+    for (int64_t n0 = 0; n0 < a.n; n0 += kMost) {
+      Fp8MmArgs p = a;
+      p.n = a.n - n0 < kMost ? a.n - n0 : kMost;
+      p.b = a.b + n0 * a.ldb;
+      p.sb = a.sb + n0 / 128 * a.sb_row;
+      p.c = static_cast<char*>(a.c) + n0 * dtype_size(out);
+      hipLaunchKernelGGL(k, dim3(static_cast<unsigned>((p.n + 63) / 64)), dim3(256), 0, stream, p);
+    }
     return hipGetLastError();
   }
   const int64_t tiles = (a.m + kTile - 1) / kTile * ((a.n + kTile - 1) / kTile);
-  if (tiles > 0x7fffffff) return hipErrorInvalidValue;
+  if (tiles > most_blocks(kThreads)) return hipErrorInvalidValue;   // 1 TB of outputs
   auto* k = out == DType::BF16 ? fp8_mm_kernel<__bf16, false> : fp8_mm_kernel<float, true>;
   hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, stream, a);
   return hipGetLastError();

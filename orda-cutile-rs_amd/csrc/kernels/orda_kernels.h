@@ -12,6 +12,9 @@ namespace orda {
 
 enum class DType : int { F32 = 0, BF16 = 1 };
 
+// Workgroups that one launch may have: HIP takes fewer than 2^32 threads.
+constexpr int64_t most_blocks(int threads) { return ((int64_t{1} << 32) - 1) / threads; }
+
 inline int dtype_size(DType t) { return t == DType::F32 ? 4 : 2; }
 
 // ---------------------------------------------------------------- GEMM

@@ -201,6 +201,18 @@ def test_autograd(dtype):
         assert torch.equal(embedding_autograd(ids, w), w[ids])
 
 
+def test_more_tokens_than_one_launch_holds():
+    """2^26 tokens' rows are 2^32 threads of the lookup, which HIP takes in no one launch."""
+    w = grad_of(1000, 8, "bf16")
+    ids = torch.randint(-1, 1000, (2 ** 26 + 70,), dtype=torch.int32, device="cuda",
+                        generator=torch.Generator(device="cuda").manual_seed(1))
+    out = H.embedding(ids, w)
+    for i, o in zip(ids.split(2 ** 24), out.split(2 ** 24)):
+        want = w[i.clamp_min(0).long()]
+        want[i < 0] = float("nan")
+        assert torch.equal(o.isnan(), want.isnan()) and torch.equal(o.nan_to_num(), want.nan_to_num())
+
+
 def test_no_second_derivative():
     """A gradient of the gradient is reported, not silently zero."""
     w = grad_of(40, 16, "f32").requires_grad_(True)

@@ -155,6 +155,33 @@ def test_quantiser_near_midpoints(dtype):
         same_codes(got, want)
 
 
+def test_quantiser_of_more_rows_than_one_launch_holds():
+    """2^28 rows are 2^32 threads, which HIP takes in no one launch. A block of one value has its code at the top."""
+    r = 2 ** 28 + 33
+    m = torch.empty(r, 1, dtype=torch.bfloat16, device="cuda").uniform_(0.5, 2.0)
+    m[::3].neg_()
+    codes, scales = H.quantize_fp8_blocks(m)
+    assert torch.equal(scales[:, 0], m[:, 0].abs().float().div_(torch.full((1,), 448.0, device="cuda")))
+    assert torch.equal(codes.view(torch.uint8)[:, 0], torch.where(m[:, 0] < 0, 0xfe, 0x7e).to(torch.uint8))
+
+
+def test_product_of_more_columns_than_one_launch_holds():
+    """One row by 2^30: 2^32 threads. The first and last columns hold values, the others zeros."""
+    n, k = 2 ** 30, 16
+    a, sa = H.quantize_fp8_blocks(normal(1, k))
+    b = torch.zeros(n, k, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    sb = torch.ones(n // 128, 1, device="cuda")
+    part, sp = H.quantize_fp8_blocks(normal(1024, k, seed=1), block_rows=128)
+    b.view(torch.uint8)[:1024] = part.view(torch.uint8)
+    b.view(torch.uint8)[-1024:] = part.view(torch.uint8)
+    sb[:8], sb[-8:] = sp, sp
+    got = H.fp8_block_matmul(a, sa, b, sb)
+    want = H.fp8_block_matmul(a, sa, part, sp)
+    assert torch.equal(got[:, :1024], want) and torch.equal(got[:, -1024:], want)
+    assert (got[:, 1024:-1024] == 0).all()
+    check_product(want, a, sa, part, sp)
+
+
 @pytest.mark.parametrize("k", [128, 1000, 1500])
 def test_product_layouts(k):
     """Contiguous codes (pitches that are no multiple of 16 are copied), column

@@ -96,6 +96,18 @@ def test_no_rows(dtype):
     assert (gw == 0).all() and gw.shape == w.shape
 
 
+def test_no_rows_of_more_classes_than_one_launch_holds():
+    """The zeros of 2^26 classes are 2^32 threads, which HIP takes in no one launch."""
+    v = 2 ** 26 + 5
+    w = torch.zeros(v, 1, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(0, 1, dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros(0, dtype=torch.int64, device="cuda")
+    torch.full((v, 1), 7.0, dtype=torch.bfloat16, device="cuda")   # what the gradient's memory held before
+    _, lse = H.linear_cross_entropy(x, w, y)
+    _, gw = H.linear_cross_entropy_backward(x, w, y, lse, lse, grad_hidden=False)
+    assert gw.shape == w.shape and (gw == 0).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
 def test_masked_rows_are_not_read(dtype, what):
