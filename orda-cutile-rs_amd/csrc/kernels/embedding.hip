@@ -181,6 +181,43 @@ __global__ __launch_bounds__(1024) void embed_count_kernel(Pairs<I> p, int shift
   for (int d = threadIdx.x; d < kDigits; d += 1024) counts[blockIdx.x * kDigits + d] = c[d];
 }
 
+// Up to kSumBlocks workgroups, each sums the others' counts itself as it places its
+// pairs, which grows with their square; beyond, a launch before it turns them into
+// sums: row b of counts into the pairs of each digit before workgroup b, the row
+// after the last into all. A workgroup takes 8 digits, each of its 128 threads a
+// digit a run of rows, read twice (2^30 tokens: 0.5 GB). Gradients of 8 columns, us
+// without the launch and with it: 2^17 tokens 172 and 171, 2^18 176 and 168, 2^20 229
+// and 176, 2^24 17910 and 2195.
+constexpr int64_t kSumBlocks = 32;
+constexpr int kSumDigits = 8, kSumRuns = 1024 / kSumDigits;
+
+__global__ __launch_bounds__(1024) void embed_sums_kernel(uint32_t* counts, int64_t blocks) {
+  __shared__ uint32_t runs[kSumRuns][kSumDigits];
+  const int d = threadIdx.x % kSumDigits, run = threadIdx.x / kSumDigits;
+  uint32_t* const c = counts + blockIdx.x * kSumDigits + d;
+  const int64_t per = (blocks + kSumRuns - 1) / kSumRuns;
+  const int64_t from = run * per < blocks ? run * per : blocks, to = from + per < blocks ? from + per : blocks;
+  uint32_t mine = 0;
+#pragma unroll 8
+  for (int64_t b = from; b < to; ++b) mine += c[b * kDigits];
+  runs[run][d] = mine;
+  __syncthreads();
+  for (int k = 1; k < kSumRuns; k *= 2) {
+    const uint32_t other = run >= k ? runs[run - k][d] : 0;
+    __syncthreads();
+    runs[run][d] += other;
+    __syncthreads();
+  }
+  uint32_t at = runs[run][d] - mine;
+  if (run == kSumRuns - 1) c[blocks * kDigits] = at + mine;
+#pragma unroll 8
+  for (int64_t b = from; b < to; ++b) {
+    const uint32_t n = c[b * kDigits];
+    c[b * kDigits] = at;
+    at += n;
+  }
+}
+
 template <typename I>
 __global__ __launch_bounds__(1024) void embed_place_kernel(Pairs<I> p, int shift, int blocks, const uint32_t* counts,
                                                            uint32_t* keys, uint32_t* vals, EmbedFill fill) {
@@ -189,15 +226,22 @@ __global__ __launch_bounds__(1024) void embed_place_kernel(Pairs<I> p, int shift
   __shared__ uint32_t part[2][kDigits], wave_sum[kDigits / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int d = lane; d < kDigits; d += 64) wave_n[wave][d] = 0;
-  // Pairs of digit d in earlier workgroups and in all, each half of the
-  // workgroup half of the workgroups' counts.
+  // Pairs of digit d in earlier workgroups and in all: read (many workgroups, see
+  // embed_sums_kernel), or each half of the workgroup sums half of the counts.
   const int d = tid & (kDigits - 1), half = tid >> kDigitBits;
   static_assert(2 * kDigits == 1024, "two threads a digit");
   uint32_t earlier = 0, total = 0;
-  for (int b = half; b < blocks; b += 2) {
-    const uint32_t c = counts[static_cast<int64_t>(b) * kDigits + d];
-    total += c;
-    if (b < static_cast<int>(blockIdx.x)) earlier += c;
+  if (blocks > kSumBlocks) {
+    if (half == 0) {
+      earlier = counts[static_cast<int64_t>(blockIdx.x) * kDigits + d];
+      total = counts[static_cast<int64_t>(blocks) * kDigits + d];
+    }
+  } else {
+    for (int b = half; b < blocks; b += 2) {
+      const uint32_t c = counts[static_cast<int64_t>(b) * kDigits + d];
+      total += c;
+      if (b < static_cast<int>(blockIdx.x)) earlier += c;
+    }
   }
   __syncthreads();
   if (half == 1) {
@@ -486,7 +530,8 @@ EmbedScratch embed_scratch(DType grad, int64_t n, int64_t v, int64_t h) {
     s.keys[1] = s.bytes;
     s.vals[1] = s.bytes + pair;
     s.counts = s.bytes + 2 * pair;
-    s.bytes = s.counts + up((n + kSortTile - 1) / kSortTile * kDigits * 4);
+    const int64_t blocks = (n + kSortTile - 1) / kSortTile;
+    s.bytes = s.counts + up((blocks + (blocks > kSumBlocks ? 1 : 0)) * kDigits * 4);
   }
   s.parts = s.bytes;
   if (s.chunks > 1) s.bytes += up(s.chunks * 2 * s.ldp * 4);
@@ -539,6 +584,9 @@ hipError_t launch_embed_sort(const void* ids, bool ids64, int64_t n, int64_t v, 
       unsigned more = share(2 * p, 2 * passes);
       hipLaunchKernelGGL(embed_count_kernel<I>, dim3(blocks + more), dim3(1024), 0, stream, pr, p * kDigitBits,
                          static_cast<int>(blocks), u32(s.counts), fill);
+      if (blocks > kSumBlocks)
+        hipLaunchKernelGGL(embed_sums_kernel, dim3(kDigits / kSumDigits), dim3(1024), 0, stream, u32(s.counts),
+                           static_cast<int64_t>(blocks));
       more = share(2 * p + 1, 2 * passes);
       hipLaunchKernelGGL(embed_place_kernel<I>, dim3(blocks + more), dim3(1024), 0, stream, pr, p * kDigitBits,
                          static_cast<int>(blocks), static_cast<const uint32_t*>(u32(s.counts)), u32(s.keys[to]),

@@ -67,6 +67,17 @@ def test_workspace_grows_with_the_tokens(n):
     assert out.value <= 16 * n + (n / 4096 + 1) * 2048 + 2 * chunks * 4096 * 4 + 6 * 256
 
 
+@pytest.mark.parametrize("n", [1 << 17, (1 << 17) + 1, 1 << 24, 1 << 30])
+def test_workspace_of_many_tokens(n):
+    """Pairs twice, 512 counts for every 4096 of them and, where a launch sums these, one row more; two fp32 rows for
+    each chunk of 256."""
+    out, err = C.c_int64(), C.create_string_buffer(512)
+    assert L.load().orda_embedding_backward_workspace(n, 131072, 8, L.BF16, C.byref(out), err, 512) == L.ORDA_OK
+    rows = -(-n // 4096) + (1 if n > 1 << 17 else 0)
+    up = lambda b: -(-b // 256) * 256
+    assert out.value == 4 * up(4 * n) + rows * 2048 + up(-(-n // 256) * 2 * 512 * 4)
+
+
 def test_python_refuses_cpu_tensors():
     with pytest.raises(H.OrdaError, match="GPU tensor"):
         H.embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(5, 8))

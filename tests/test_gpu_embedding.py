@@ -116,6 +116,15 @@ def test_gradient_of_many_tokens(t, kind):
     check_grad(H.embedding_backward(g, ids, v), g, ids, v)
 
 
+@pytest.mark.parametrize("kind", ["uniform", "one", "few", "text"])
+@pytest.mark.parametrize("t, v", [(131072, 600), (131073, 600), (135169, 400), (530001, 300000), (4194305, 5000)])
+def test_gradient_of_more_workgroups_than_count_for_themselves(t, v, kind):
+    """Past 32 workgroups of 4096 pairs their counts are summed by a launch of its own: 128 runs of them, one or many
+    rows each, digits in one to three passes."""
+    ids, g = tokens(t, v, kind), grad_of(t, 3, "bf16")
+    check_grad(H.embedding_backward(g, ids, v), g, ids, v)
+
+
 @pytest.mark.parametrize("kind", ["uniform", "one", "text"])
 @pytest.mark.parametrize("t", [0, 5, 4000, 20000])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
