@@ -117,6 +117,25 @@ def test_gradient_of_many_tokens(t, kind):
 
 
 @pytest.mark.parametrize("kind", ["uniform", "one", "few", "text"])
+@pytest.mark.parametrize("t, v", [(16385, 511), (16385, 512), (16500, 262143), (16384, 262144), (15000, 300000), (20000, 2 ** 27)])
+def test_digits_of_the_sort(t, v, kind):
+    """Sorts in passes of 9 bits where the ids (and v, which stands for no id) end at and after a digit: one to four
+    passes. (Of 2^27 rows only those that are named are compared, the others looked at.)"""
+    ids, g = tokens(t, v, kind), grad_of(t, 2, "bf16")
+    if kind == "uniform":
+        ids[::100] = v - 1
+    if v < 2 ** 20:
+        check_grad(H.embedding_backward(g, ids, v), g, ids, v)
+        return
+    out = torch.zeros(v, 2, dtype=torch.bfloat16, device="cuda")
+    H.embedding_backward(g, ids, v, out=out, accumulate=True)
+    named, place = torch.unique(ids, return_inverse=True)
+    check_grad(out[named], g, place, len(named))
+    out[named] = 0
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["uniform", "one", "few", "text"])
 @pytest.mark.parametrize("t, v", [(131072, 600), (131073, 600), (135169, 400), (530001, 300000), (4194305, 5000)])
 def test_gradient_of_more_workgroups_than_count_for_themselves(t, v, kind):
     """Past 32 workgroups of 4096 pairs their counts are summed by a launch of its own: 128 runs of them, one or many

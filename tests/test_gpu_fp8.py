@@ -155,6 +155,33 @@ def test_quantiser_near_midpoints(dtype):
         same_codes(got, want)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("pitch", [128, 130, 132, 129])
+def test_block_quantiser_near_midpoints(dtype, pitch):
+    """Blocks of 128 rows whose quotients lie at and next to the midpoints of two codes, normal and subnormal, read at
+    every width the rows' alignment allows."""
+    codes = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    mid = (codes[1:] + codes[:-1]) / 2
+    made = []
+    for top in (448.0, 447.0, 1.0, 3.7, 1e-3, 12345.0, 2.0 ** -100, 2.0 ** 90):
+        s = (torch.tensor(top, dtype=torch.float32) / torch.tensor(448.0)).double()
+        v = (mid * s).to(DT[dtype])
+        bits = v.view(torch.int16 if dtype == "bf16" else torch.int32)
+        flat = torch.cat([v] + [(bits + d).view(DT[dtype]) for d in (1, -1, 2, -2, 3, -3)])
+        flat = flat[flat.abs().double() <= top]
+        block = flat[torch.arange(128 * 128) % len(flat)].view(128, 128).clone()
+        block[1::2] = -block[1::2]
+        block[77, 5] = top
+        made.append(block)
+    frame = torch.zeros(128 * len(made), pitch, dtype=DT[dtype], device="cuda")
+    m = frame[:, pitch - 128:]
+    m.copy_(torch.cat(made))
+    got, scales = H.quantize_fp8_blocks(m, block_rows=128)
+    want, s = quantized(m, 128)
+    assert torch.equal(scales.cpu(), s)
+    same_codes(got, want)
+
+
 def test_quantiser_of_more_rows_than_one_launch_holds():
     """2^28 rows are 2^32 threads, which HIP takes in no one launch. A block of one value has its code at the top."""
     r = 2 ** 28 + 33

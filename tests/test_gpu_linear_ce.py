@@ -406,3 +406,24 @@ def test_few_fp32_rows_of_a_large_weight(n, h, v):
         y[1::5] = -100
     gn, gl = torch.randn(n, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda")
     check(x, w, y, gn, gl, label_smoothing=0.1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n, h, v", [(1, 200, 997), (16, 264, 2000), (17, 1003, 700), (33, 67, 301), (64, 520, 1025), (5, 72, 513)])
+def test_few_rows_in_pieces(n, h, v, dtype):
+    """Gradients of few rows over pieces of 256 classes, the last one shorter: labels past the first piece,
+    grad_hidden added from piece to piece, weights copied by pieces (odd widths)."""
+    x, w, y, gn, gl = inputs(n, h, v, dtype, seed=7)
+    y[-1] = v - 1
+    if n > 8:
+        y[::5] = -100
+    check(x, w, y, gn, gl, label_smoothing=0.1, vocab_piece=256)
+
+
+@pytest.mark.parametrize("n, h, v, dtype, ignored", [(12545, 8192, 300, "bf16", 0.0), (12545, 8192, 300, "bf16", 0.4),
+                                                     (20000, 6208, 260, "bf16", 0.1), (12545, 2688, 300, "f32", 0.0),
+                                                     (12545, 2688, 300, "f32", 0.3)])
+def test_rows_in_bands(n, h, v, dtype, ignored):
+    """Batches whose rows overflow the last cache walk their tiles in bands of 32 M-tiles, with a count of rows that
+    only the device knows: whole bands and rows past them, and (0.4 ignored) fewer rows than a band."""
+    check(*inputs(n, h, v, dtype, seed=8, ignored=ignored), vocab_piece=256)
