@@ -2628,7 +2628,10 @@ void set_share_blocks(GemmArgs& g) {
 // Not applied where it did not gain: H = 16384 (a 256 MB band, or 128 MB in
 // 2 x 16 blocks with 18 strips a stage: 0.50 against 0.51), H = 5120 (A
 // 168 MB: 0.51 against 0.52), BT = 16384 at H = 4096 (the grouped raster
-// already walks N twice with 128 MB live: equal).
+// already walks N twice with 128 MB live: equal). The linear cross entropy's logits,
+// whose rows only the device counts, gain more: 16384 x 8192 x 32000 6.16 ms of losses
+// against 6.78, 12800 x 8192 x 32000 4.83 against 5.33, 16384 x 6400 x 128256 19.0
+// against 19.7.
 void set_band_blocks(GemmArgs& g) {
   constexpr int64_t kBandLive = int64_t{192} << 20, kBandMax = int64_t{128} << 20;
   if (g.sh_a > 0 || !logits_epilogue(g) || g.in_type != DType::BF16) return;

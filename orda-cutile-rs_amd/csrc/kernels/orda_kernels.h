@@ -541,7 +541,6 @@ EmbedScratch embed_scratch(DType grad, int64_t n, int64_t v, int64_t h);
 struct EmbedFill {
   void* out;
   int64_t rows, bytes, pitch, spans, from, to;
-  bool stream;   // past the caches
 };
 EmbedFill embed_fill(DType out, void* d, int64_t ldo, int64_t v, int64_t h);   // rows [v, h]
 // (id, place) of every token, sorted by id, stable; ids without a gradient (pad,
@@ -563,9 +562,8 @@ struct EmbedGradArgs {
   int64_t chunk, chunks, slabs;
   float* parts;        // [chunks][2][ldp]
   int64_t ldp;
-  bool stream;         // set by launch_embed_grad: out is written past the caches
 };
-hipError_t launch_embed_grad(EmbedGradArgs a, DType grad, DType out, hipStream_t stream);
+hipError_t launch_embed_grad(const EmbedGradArgs& a, DType grad, DType out, hipStream_t stream);
 
 // ---------------------------------------------------------------- e4m3 with block scales
 // codes (e4m3, rows of pitch ldc, a multiple of 8; the last eight of a row is
