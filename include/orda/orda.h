@@ -336,7 +336,8 @@ typedef struct {
     int64_t ignore_index;
     float label_smoothing;   /* in [0, 1] */
     int64_t vocab_piece;     /* columns of a piece, rounded to whole 256s, at
-                                most 2^21; 0: as many as 1 GiB of scratch holds */
+                                most 2^21 and 2^39 / N; 0: as many as 1 GiB of
+                                scratch holds */
 } orda_linear_ce;
 /* Bytes of workspace (256-byte aligned) of a forward call (backward 0), or of
  * a backward call for grad_hidden (1), grad_weight (2) or both (3). */

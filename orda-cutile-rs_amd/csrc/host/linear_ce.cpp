@@ -118,7 +118,9 @@ Ce make_ce(const orda_linear_ce& a, int64_t labels, bool backward, bool gh, bool
   c.few = few_rows(c);
   // Pieces of whole column tiles, all but the last alike.
   int64_t most = a.vocab_piece > 0 ? a.vocab_piece : std::max<int64_t>(kPieceBytes / std::max<int64_t>(column_bytes(c), 1), 4096);
-  most = std::max<int64_t>(std::min(most, kMaxPiece) / 256 * 256, 256);
+  // (a logits product's tiles, of 128 rows at least, in one launch)
+  most = std::min({most, kMaxPiece, most_blocks(256) / std::max<int64_t>((c.n + 127) / 128, 1) * 256});
+  most = std::max<int64_t>(most / 256 * 256, 256);
   const int64_t pieces = (c.v + most - 1) / most;
   c.piece = pieces == 1 ? c.v : ((c.v + pieces - 1) / pieces + 255) / 256 * 256;
   // (The planes' scratch cuts pieces that the direct form, which makes no planes, does not need.)

@@ -150,6 +150,15 @@ def test_few_fp32_rows_take_no_planes(n, v, h):
     assert workspace(args(n=n, h=h, v=v, **f32), 3)[1] <= 1 << 30
 
 
+@pytest.mark.parametrize("n", [2 ** 20, 2 ** 21])
+def test_a_piece_is_one_launch(n):
+    """HIP takes fewer than 2^32 threads in a launch, 256 for each tile of 128 or 256 rows by 256 classes: larger
+    pieces are cut, which the statistics' scratch (16 bytes a row and tile) shows."""
+    need = workspace(args(n=n, h=64, v=2 ** 21, vocab_piece=2 ** 21))[1]
+    tiles = (2 ** 24 - 1) // (n // 128)
+    assert n * tiles * 16 // 2 <= need <= n * (tiles * 16 + 64 * 2 + 64)
+
+
 def test_asked_for_pieces_are_kept():
     """vocab_piece bounds the scratch of fp32 calls too: smaller pieces, less of it."""
     f32 = {"hidden.dtype": L.F32, "weight.dtype": L.F32}
