@@ -390,7 +390,8 @@ int32_t orda_embedding_backward(int32_t device, void *hip_stream, const void *id
  * allocate nothing and can be captured. At most 2^30 rows and 2^20 columns. No
  * counterpart in the reference, whose quantisation is INT8 by rows. */
 typedef struct {
-    void *codes;          /* [rows,cols], one byte each, rows ld bytes apart */
+    void *codes;          /* [rows,cols], one byte each, rows ld bytes apart
+                             (at most 2^20 + 16) */
     int64_t rows, cols, ld;
     float *scales;        /* block (i,j) at i*scale_row + j*scale_col */
     int64_t scale_row, scale_col;

@@ -316,6 +316,9 @@ def _embed_grad(g, i, num_rows: int, scale: float, pad: int, out=None, accumulat
 
 
 # ------------------------------------------------------------------ e4m3 with block scales
+_FP8_PITCH, _FP8_STRIDE = 2 ** 20 + 16, 2 ** 22   # the most that orda_fp8_matrix takes between rows of codes, of scales
+
+
 def _fp8_desc(codes, scales, block_rows: int, what: str):
     """(orda_fp8_matrix, the tensors it points into) of codes [R, C] and scales
     [ceil(R / block_rows), ceil(C / 128)]."""
@@ -324,11 +327,15 @@ def _fp8_desc(codes, scales, block_rows: int, what: str):
     if c.dtype != torch.float8_e4m3fn:
         raise OrdaError(f"{what} must be float8_e4m3fn, got {c.dtype}")
     c = _matrix(c, what)
+    if c.size(0) > 1 and c.stride(0) > _FP8_PITCH:
+        c = c.contiguous()
     s = _gpu_tensor(scales, f"{what}'s scales")
     _same_device(c.device, **{f"{what}'s scales": s})
     shape = (-(-c.size(0) // block_rows), -(-c.size(1) // 128))
     if s.dtype != torch.float32 or tuple(s.shape) != shape:
         raise OrdaError(f"{what}'s scales must be float32 {list(shape)}")
+    if shape[0] > 1 and s.stride(0) > _FP8_STRIDE:
+        s = s.contiguous()
     d = L.Fp8MatrixC(codes=c.data_ptr(), rows=c.size(0), cols=c.size(1),
                      ld=c.stride(0) if c.size(0) > 1 else -(-c.size(1) // 16) * 16,
                      scales=s.data_ptr(), scale_row=s.stride(0) if shape[0] > 1 else 0,
@@ -371,8 +378,8 @@ def fp8_block_matmul(a, a_scales, b, b_scales, *, out_dtype=None):
     columns (``b_scales`` [ceil(N / 128), ceil(K / 128)]), as ``quantize_fp8_blocks``
     makes them with ``block_rows`` 1 and 128, or a checkpoint holds them. Sums are
     float32, rounded once to ``out_dtype`` (bfloat16, the default, or float32).
-    Returns [M, N]. Codes whose memory or pitch is not 16-byte aligned are copied
-    first."""
+    Returns [M, N]. Codes whose memory or pitch is not 16-byte aligned, or whose
+    rows lie over 2^20 + 16 bytes apart, are copied first."""
     torch = _torch()
     ad, (a, _sa) = _fp8_desc(a, a_scales, 1, "a")
     bd, (b, _sb) = _fp8_desc(b, b_scales, 128, "b")

@@ -227,6 +227,23 @@ def test_product_layouts(k):
     check_product(got, a, torch.ones_like(sa), b, torch.ones_like(sb))
 
 
+def test_codes_at_a_wide_pitch():
+    """Columns of a table up to 2^24 + 32 bytes wide: 300 rows lie 5 GB apart."""
+    a, sa = H.quantize_fp8_blocks(normal(70, 144))
+    b, sb = H.quantize_fp8_blocks(normal(300, 144, seed=1), block_rows=128)
+    want = H.fp8_block_matmul(a, sa, b, sb)
+    for pitch in (2 ** 20 + 16, 2 ** 20 + 32, 2 ** 24 + 32):
+        table = torch.empty((300, pitch), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+        for at in (0, 16):
+            wide = table[:, at:at + 144]
+            wide.view(torch.uint8).copy_(b.view(torch.uint8))
+            assert torch.equal(H.fp8_block_matmul(a, sa, wide, sb), want)
+            assert torch.equal(H.fp8_block_matmul(a[:3], sa[:3], wide, sb), want[:3])
+    far = torch.empty((70, 2 ** 22 + 4), device="cuda")[:, 1:3]
+    far.copy_(sa)
+    assert torch.equal(H.fp8_block_matmul(a, far, b, sb), want)
+
+
 def test_product_carries_nan():
     x, w = normal(40, 300), normal(200, 300, seed=1)
     x[3, 200] = float("nan")
