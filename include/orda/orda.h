@@ -319,6 +319,7 @@ int32_t orda_scale_gradients(int32_t device, void *hip_stream, const float *scal
  * ignore_index nor a class makes its row's nll and gradients NaN (the calls do
  * not wait for the device, so nothing else can report it); a NaN gradient row
  * makes every row of grad_weight NaN.
+ * Logits beyond 2^127 in magnitude count as infinite.
  * Everything is on `device`. The calls queue their kernels on hip_stream (NULL:
  * the null stream) and return; they allocate nothing and can be captured into
  * a graph. workspace is the call's alone until its kernels have run: calls (and

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeFewArgs a) {
         if (e < ncol) mx = fmaxf(mx, v[e]);
       mx = quad_max(mx);
       // (an infinite maximum: the sum is that infinity or 0, without inf - inf)
-      const float ref = fabsf(mx) <= FLT_MAX ? mx : 0.f;
+      const float ref = fabsf(mx) <= kCeLargest ? mx : 0.f;
       float sum = 0.f, sx = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void ce_few_kernel(CeFewArgs a) {
         }
       sum = quad_sum(sum);
       sx = quad_sum(sx);
-      if (lgrp == 0) part[wave][row] = make_float4(mx == -INFINITY ? mx : ref, sum, 0.f, sx);
+      if (lgrp == 0) part[wave][row] = make_float4(mx < -kCeLargest ? -INFINITY : ref, sum, 0.f, sx);
     }
   }
   if constexpr (!GRAD) {

@@ -375,7 +375,7 @@ __global__ __launch_bounds__(256) void ce_direct_stats_kernel(CeDirectArgs a) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) m = fmaxf(m, red[w][0]);
   sx = red[0][1] + red[1][1] + red[2][1] + red[3][1];
-  const float ref = fabsf(m) <= FLT_MAX ? m : 0.f;   // as in the products' epilogue
+  const float ref = fabsf(m) <= kCeLargest ? m : 0.f;   // as in the products' epilogue
   float sum = 0.f;
 #pragma unroll
   for (int q = 0; q < 2; ++q)
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(256) void ce_direct_stats_kernel(CeDirectArgs a) {
   __syncthreads();
   if (threadIdx.x == 0)
     a.stats[row * a.stats_ld + blockIdx.x] =
-        make_float4(m == -INFINITY ? m : ref, red[0][2] + red[1][2] + red[2][2] + red[3][2], 0.f, sx);
+        make_float4(m < -kCeLargest ? -INFINITY : ref, red[0][2] + red[1][2] + red[2][2] + red[3][2], 0.f, sx);
 }
 
 __global__ __launch_bounds__(256) void ce_direct_grad_kernel(CeDirectArgs a) {

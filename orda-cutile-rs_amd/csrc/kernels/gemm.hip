@@ -1256,7 +1256,7 @@ __device__ __forceinline__ void ce_epilogue(const GemmArgs& g, int64_t M, const 
         mx = quad_max(mx);
         // an infinite maximum: e^(x-0) is inf or 0, so the sum is that infinity
         // or 0 without inf - inf
-        const float ref = fabsf(mx) <= FLT_MAX ? mx : 0.f;
+        const float ref = fabsf(mx) <= kCeLargest ? mx : 0.f;
         const float o1 = -ref * kLog2e;
         float d1 = 0.f, sx = 0.f;
 #pragma unroll
@@ -1271,7 +1271,7 @@ __device__ __forceinline__ void ce_epilogue(const GemmArgs& g, int64_t M, const 
           }
         d1 = quad_sum(d1);
         sx = quad_sum(sx);
-        if (lgrp == 0) rows4[wn * TM + rl] = make_float4(mx == -INFINITY ? mx : ref, d1, 0.f, sx);
+        if (lgrp == 0) rows4[wn * TM + rl] = make_float4(mx < -kCeLargest ? -INFINITY : ref, d1, 0.f, sx);
         if (yl >= 0 && yl < 128 && (yl & 12) == 0 && row < M) {   // one lane of a row at most
           const int jy = yl >> 4, ey = yl & 3;
           float xy = 0.f;

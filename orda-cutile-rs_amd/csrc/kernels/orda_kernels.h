@@ -93,11 +93,16 @@ struct LogitStatsArgs {
   DType teacher_type;
 };
 
+// Row maxima beyond this count as infinite: times log2 e they would be, and
+// e^(x - max) with them 0 or NaN.
+constexpr float kCeLargest = 0x1p127f;
+
 // The CeStats and CeGrad epilogues (one problem, bf16 operands, K-major both):
 // columns 0..N of the product are vocabulary columns col0..col0+N.
 struct CeArgs {
   // CeStats: stats[m*stats_ld + n_tile] = {max, Σe^(x-max), 0, Σx} (max -inf
-  // and sum 0 where every logit is -inf; max 0 where the maximum is +inf)
+  // and sum 0 where every logit is below -kCeLargest; max 0 and sum inf where the
+  // maximum is beyond kCeLargest)
   float4* stats;
   int64_t stats_ld;       // in float4 units, >= ceil(N/256)
   float* xy;              // xy[m] = fp32 logit at the row's label column

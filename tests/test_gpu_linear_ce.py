@@ -164,6 +164,26 @@ def test_large_logits():
     assert not torch.isfinite(lse).any() and not torch.isfinite(nll).any()
 
 
+@pytest.mark.parametrize("dtype, piece", [("bf16", None), ("f32", None), ("f32", 256)])
+@pytest.mark.parametrize("n", [1, 40, 100])
+def test_logits_at_the_end_of_the_range(n, dtype, piece):
+    """A class 2^127 above the others is the whole sum; beyond, it counts as infinite; classes as far below add
+    nothing; all so far below are minus infinity."""
+    x = torch.zeros(n, 64, dtype=DT[dtype], device="cuda")
+    x[:, 0] = 2.0 ** 64
+    w = torch.zeros(600, 64, dtype=DT[dtype], device="cuda")
+    y = torch.full((n,), 300, device="cuda")
+    for top, low, want in ((2.0 ** 63, 0.0, 2.0 ** 127), (1.9 * 2.0 ** 63, 0.0, float("inf")),
+                           (2.0 ** 63, -1.75 * 2.0 ** 63, 2.0 ** 127), (-1.75 * 2.0 ** 63, -1.875 * 2.0 ** 63, -float("inf")),
+                           (-2.0 ** 63, -1.875 * 2.0 ** 63, -2.0 ** 127)):
+        w[:, 0] = low
+        w[300, 0] = top
+        nll, lse = H.linear_cross_entropy(x, w, y, vocab_piece=piece)
+        assert (lse == want).all(), (top, low, lse[:3])
+        if abs(want) < float("inf"):
+            assert (nll == 0).all()
+
+
 @pytest.mark.parametrize("want", [(True, False), (False, True), (False, False)])
 def test_single_gradients(want):
     x, w, y, gn, gl = inputs(100, 64, 700, "bf16", ignored=0.3)
