@@ -2748,9 +2748,8 @@ SplitPlan plan_split_small(const GemmArgs& g) {
   SplitPlan sp{1, g.K, 0, 0, 0, 0.0};
   if (g.K <= 0) return sp;
   const int64_t tiles = small_tiles(g);
-  if (tiles >= 192) return sp;
   const int64_t per_split = g.nprob * (g.c_trans ? g.N * ((g.M + 3) / 4 * 4) : g.M * ((g.N + 3) / 4 * 4)) * 4;
-  int64_t most = (256 + tiles - 1) / tiles;
+  int64_t most = tiles < 192 ? (256 + tiles - 1) / tiles : 1;
   const int64_t by_k = g.K / 128, by_ws = split_cap(g) / per_split;
   if (most > by_k) most = by_k;
   if (most > 64) most = 64;

@@ -159,6 +159,15 @@ def test_a_piece_is_one_launch(n):
     assert n * tiles * 16 // 2 <= need <= n * (tiles * 16 + 64 * 2 + 64)
 
 
+@pytest.mark.parametrize("n, h, v", [(2048, 2048, 32000), (1024, 4096, 32000), (900, 4096, 32000), (4096, 1024, 30000)])
+def test_large_fp32_gradients_take_planes(n, h, v):
+    """The form that keeps its logits is for small calls: a grad_hidden of 48 to 64 tiles of 256 over a whole
+    vocabulary goes over planes (6 bytes for each element of the weight, and of the logits), as both gradients do."""
+    f32 = {"hidden.dtype": L.F32, "weight.dtype": L.F32}
+    for which in (1, 2, 3):
+        assert workspace(args(n=n, h=h, v=v, **f32), which)[1] >= 6 * v * (h + n)
+
+
 def test_asked_for_pieces_are_kept():
     """vocab_piece bounds the scratch of fp32 calls too: smaller pieces, less of it."""
     f32 = {"hidden.dtype": L.F32, "weight.dtype": L.F32}
