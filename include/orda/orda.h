@@ -328,10 +328,12 @@ int32_t orda_scale_gradients(int32_t device, void *hip_stream, const float *scal
  * weighted mean. */
 typedef struct {
     orda_tensor hidden;      /* [N,H], fp32 or bf16 */
-    orda_tensor weight;      /* [V,H], the same type; read in place where it is
-                                fp32, or 16-byte aligned with H and ld multiples
-                                of 8 and ld at most 2^20, else copied a piece at
-                                a time where a product needs it */
+    orda_tensor weight;      /* [V,H], the same type. Read in place where it is
+                                16-byte aligned with H and ld multiples of 8 and
+                                ld at most 2^20, and at any pitch by the logits
+                                of few rows; else copied a piece at a time where
+                                a product needs it. fp32 calls that are not small
+                                rewrite each piece as three planes of bf16 */
     const int64_t *labels;   /* [N] */
     int64_t n_labels;
     int64_t ignore_index;
@@ -406,8 +408,11 @@ typedef struct {
 int32_t orda_quant_fp8_blocks(int32_t device, void *hip_stream, const orda_tensor *m,
                               orda_fp8_matrix *out, char *err, size_t err_len);
 /* out[m,n] = Σ_j scale_a[m,j]·scale_b[n/128,j]·Σ_k code_a[m,k]·code_b[n,k], k over
- * the 128 columns of block j; sums in fp32, rounded once to out's type (fp32 or
- * bf16). a has block_rows 1, b 128. Codes whose base or pitch is no multiple of
+ * the 128 columns of block j; blocks are added in fp32, and the sum rounded once
+ * to out's type (fp32 or bf16). For fp32 outputs the sum over a block is fp32 too;
+ * for bf16 outputs the matrix units add its 128 products to fewer bits (1.5e-5 off
+ * relative to the sums' norm, against the rounding's 1.7e-3), so that an element
+ * whose products cancel may be further off than its rounding. a has block_rows 1, b 128. Codes whose base or pitch is no multiple of
  * 16 are copied into workspace first (256-byte aligned, the call's alone until
  * its kernels have run). Columns of codes between cols and ld are not read as
  * values. Scale strides are at least 0; scale_row at most 2^22. */

@@ -376,8 +376,10 @@ def fp8_block_matmul(a, a_scales, b, b_scales, *, out_dtype=None):
     """``A @ B.T`` of quantised matrices: ``a`` [M, K] with a scale for each row and 128
     columns (``a_scales`` [M, ceil(K / 128)]), ``b`` [N, K] for each 128 rows and 128
     columns (``b_scales`` [ceil(N / 128), ceil(K / 128)]), as ``quantize_fp8_blocks``
-    makes them with ``block_rows`` 1 and 128, or a checkpoint holds them. Sums are
-    float32, rounded once to ``out_dtype`` (bfloat16, the default, or float32).
+    makes them with ``block_rows`` 1 and 128, or a checkpoint holds them. Blocks are
+    added in float32 and rounded once to ``out_dtype`` (bfloat16, the default, or
+    float32); the sum over a block of 128 is float32 for float32 outputs, and held
+    to fewer bits for bfloat16 ones (1.5e-5 relative to the sums' norm).
     Returns [M, N]. Codes whose memory or pitch is not 16-byte aligned, or whose
     rows lie over 2^20 + 16 bytes apart, are copied first."""
     torch = _torch()
