@@ -173,3 +173,10 @@ def test_asked_for_pieces_are_kept():
     f32 = {"hidden.dtype": L.F32, "weight.dtype": L.F32}
     sizes = [workspace(args(n=512, h=4096, v=131072, vocab_piece=p, **f32), 3)[1] for p in (256, 4096, 16384, 65536)]
     assert sizes == sorted(sizes) and sizes[0] < sizes[-1]
+
+
+@pytest.mark.parametrize("n, h, v, piece", [(3, 4096, 44000, 0), (64, 1000, 180001, 0), (64, 2426, 131072, 0), (1, 512, 2 ** 21, 0),
+                                            (1, 64, 2 ** 21 + 300, 0), (2048, 2048, 32000, 0), (1000, 4096, 50257, 0)])
+def test_the_scratch_of_large_fp32_calls_is_the_scratch_laid_out(n, h, v, piece):
+    """As above, at and past the vocabularies that the planes' scratch cuts into pieces."""
+    test_the_scratch_asked_for_is_the_scratch_laid_out(n, h, v, piece, L.F32)
