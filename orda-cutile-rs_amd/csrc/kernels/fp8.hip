@@ -220,10 +220,10 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(const uint8_t* src, int64
 // MFMAs, half the port time, leave too few registers to keep two pairs apart: 4.6.
 //
 // The e4m3 MFMAs (all four shapes, measured) add their products to fewer bits than
-// fp32: a sum of 128 comes out 1.5e-5 off relative to the sums' norm. Beside bf16
-// outputs, rounded at 1.7e-3, that is nothing; for fp32 outputs (WIDE) the codes
-// are widened to bf16, exactly, as fragments are read, and a block is four
-// 16x16x32 bf16 MFMAs (9e-9 off), at half the matrix rate.
+// fp32: a sum of 4 to 128 comes out 1.5e-5 of the root of the sum of squares off,
+// 1e-4 at most. Beside bf16 outputs, rounded at 1.7e-3, that is nothing; for fp32
+// outputs (WIDE) the codes are widened to bf16, exactly, as fragments are read, and
+// a block is four 16x16x32 bf16 MFMAs (9e-9 off), at half the matrix rate.
 constexpr int kTile = 256, kThreads = 512;
 constexpr int kOp = kTile * 128;                      // an operand's stage
 constexpr int kScales = kTile * 4 + 64;               // A's row scales, B's two

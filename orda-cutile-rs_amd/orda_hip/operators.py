@@ -379,7 +379,8 @@ def fp8_block_matmul(a, a_scales, b, b_scales, *, out_dtype=None):
     makes them with ``block_rows`` 1 and 128, or a checkpoint holds them. Blocks are
     added in float32 and rounded once to ``out_dtype`` (bfloat16, the default, or
     float32); the sum over a block of 128 is float32 for float32 outputs, and held
-    to fewer bits for bfloat16 ones (1.5e-5 relative to the sums' norm).
+    to fewer bits for bfloat16 ones (off by 1.5e-5 of the root of the sum of the
+    products' squares, at most 1e-4).
     Returns [M, N]. Codes whose memory or pitch is not 16-byte aligned, or whose
     rows lie over 2^20 + 16 bytes apart, are copied first."""
     torch = _torch()
