@@ -423,6 +423,98 @@ int32_t orda_fp8_block_matmul(int32_t device, void *hip_stream, const orda_fp8_m
                               const orda_fp8_matrix *b, orda_tensor *out, void *workspace,
                               int64_t workspace_bytes, char *err, size_t err_len);
 
+/* ---- root-mean-square norm --------------------------------------------------- */
+/* The norm before the head, with the residual's addition in the same pass:
+ *   t   = x + residual, rounded to the rows' type (x itself without a residual)
+ *   s   = 1 / sqrt(mean over the row of t² + eps)
+ *   out = t·s·(w + weight_offset), rounded once to the rows' type
+ * Everything is on `device`; the calls queue their kernels on hip_stream (NULL:
+ * the null stream) and return, allocate nothing and can be captured. Outputs share
+ * no memory with inputs. The mean is formed in 64 bits. At most 2^30 rows and 2^20
+ * columns. No counterpart in the reference. */
+typedef struct {
+    orda_tensor x;          /* [N,H], fp32 or bf16 */
+    orda_tensor residual;   /* the same, or without data: none */
+    orda_tensor weight;     /* [1,H], fp32 or bf16 */
+    double eps;             /* >= 0 */
+    double weight_offset;   /* 0, or 1 where weights are held around zero */
+} orda_rms_norm;
+/* total (t) and out are [N,H] in the rows' type; total may be without data. */
+int32_t orda_rms_norm_forward(int32_t device, void *hip_stream, const orda_rms_norm *args,
+                              orda_tensor *total, orda_tensor *out, char *err, size_t err_len);
+/* The same with codes and scales of t·s·(w + weight_offset), as
+ * orda_quant_fp8_blocks defines them for block_rows 1, of the values in fp32 (not
+ * rounded to the rows' type before). out as in that call. */
+int32_t orda_rms_norm_fp8(int32_t device, void *hip_stream, const orda_rms_norm *args,
+                          orda_tensor *total, orda_fp8_matrix *out, char *err, size_t err_len);
+/* Gradients from grad_out (into out) and grad_total (into t beside its norm; without
+ * data: 0), both [N,H] in the rows' type; args as in the forward call but x = t and no
+ * residual. grad_x [N,H], in the rows' type, is the gradient of x and of the residual
+ * alike; grad_weight [1,H], in the weight's type, is the sum over the rows in fp32,
+ * rounded once, the same bits in every run. Either may be without data. workspace
+ * (256-byte aligned) is the call's alone until its kernels have run. */
+int32_t orda_rms_norm_backward_workspace(int64_t n, int64_t h, int64_t *bytes, char *err, size_t err_len);
+int32_t orda_rms_norm_backward(int32_t device, void *hip_stream, const orda_rms_norm *args,
+                               const orda_tensor *grad_out, const orda_tensor *grad_total,
+                               orda_tensor *grad_x, orda_tensor *grad_weight, void *workspace,
+                               int64_t workspace_bytes, char *err, size_t err_len);
+
+/* ---- gradient norm and clipping ------------------------------------------------ */
+/* norm = sqrt(Σ g²) over all the gradients, squares and sums in 64 bits, and
+ * g · min(1, max_norm / (norm + eps)), rounded once to the destination's type. A
+ * gradient is a matrix, fp32 or bf16 (a contiguous tensor of any shape: one row);
+ * dst without data: scaled in place, and where the norm is within max_norm not
+ * touched; else written to dst, of the same shape. A norm that is NaN makes every
+ * gradient NaN, an infinite one makes the finite values 0 and the others NaN.
+ * Destinations (in place: the gradients) share no memory with one another or with
+ * other gradients. norm is one float32. At most 2^20 gradients of 2^40 values
+ * together. Device, stream and workspace as above. No counterpart in the reference. */
+typedef struct {
+    orda_tensor src;
+    orda_tensor dst;
+} orda_gradient;
+int32_t orda_clip_gradients_workspace(const orda_gradient *gradients, int64_t count, int64_t *bytes,
+                                      char *err, size_t err_len);
+int32_t orda_gradient_norm(int32_t device, void *hip_stream, const orda_gradient *gradients,
+                           int64_t count, float *norm, void *workspace, int64_t workspace_bytes,
+                           char *err, size_t err_len);
+int32_t orda_clip_gradients(int32_t device, void *hip_stream, const orda_gradient *gradients,
+                            int64_t count, double max_norm, double eps, float *norm, void *workspace,
+                            int64_t workspace_bytes, char *err, size_t err_len);
+
+/* ---- drawing tokens ------------------------------------------------------------ */
+/* One token of each row of logits x [N,V], fp32 or bf16, by the row's number u in
+ * [0,1). With temperature T > 0 a token's mass is e^((x - max)/T), 0 under e^-700. Of
+ * the tokens in descending order of logits (equal ones: the lowest first) are kept
+ *   top_k: the first k (k <= 0: all),
+ *   top_p: of those, the ones whose mass before them is below p times the mass of
+ *          all of those, and the first (p >= 1: all),
+ *   min_p: of those, the ones whose mass is at least m times the largest, and the
+ *          first.
+ * The token is the first in the order of the vocabulary up to which the kept masses
+ * add to more than u times their sum (the last kept one where none is), logprob the
+ * log of its share of that sum. T = 0: the largest logit, the lowest such token,
+ * logprob 0. Where the largest logit is +infinity the tokens that have it share the
+ * mass. Masses and their sums are formed in 64 bits.
+ * A row with a NaN, or with no logit over -infinity, or whose T is negative or not
+ * finite, whose p or m is NaN or whose u is no number of [0,1], gets token -1 and
+ * logprob NaN.
+ * Parameters with data are per row ([N], on the device), the others hold for all
+ * rows. Device, stream and workspace as above. At most 2^20 rows and columns. */
+typedef struct {
+    orda_tensor logits;
+    const float *uniform;                       /* [N] */
+    const float *temperatures, *top_ps, *min_ps; /* [N] or NULL */
+    const int32_t *top_ks;
+    float temperature, top_p, min_p;
+    int32_t top_k;
+} orda_sampling;
+int32_t orda_sample_tokens_workspace(int64_t n, int64_t v, int64_t *bytes, char *err, size_t err_len);
+/* tokens [N]; logprobs [N] or NULL. */
+int32_t orda_sample_tokens(int32_t device, void *hip_stream, const orda_sampling *args, int64_t *tokens,
+                           float *logprobs, void *workspace, int64_t workspace_bytes, char *err,
+                           size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

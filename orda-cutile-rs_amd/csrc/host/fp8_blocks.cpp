@@ -8,8 +8,9 @@ namespace {
 
 constexpr int64_t kMaxPitch = int64_t{1} << 20, kMaxStride = int64_t{1} << 22, kMaxRows = int64_t{1} << 30;
 
-// A quantised matrix: its shape, pitch and scale strides.
-void check_matrix(const orda_fp8_matrix& m, const char* what) {
+}  // namespace
+
+void check_fp8_matrix(const orda_fp8_matrix& m, const char* what) {
   if (m.rows < 0 || m.cols < 0) fail(ORDA_ERR_INVALID, "%s has a negative shape", what);
   if (m.block_rows != 1 && m.block_rows != 128) fail(ORDA_ERR_INVALID, "%s: block_rows must be 1 or 128", what);
   if (m.rows > kMaxRows || m.cols > kMaxPitch) fail(ORDA_ERR_INVALID, "%s: at most 2^30 rows and 2^20 columns", what);
@@ -20,6 +21,8 @@ void check_matrix(const orda_fp8_matrix& m, const char* what) {
     fail(ORDA_ERR_INVALID, "%s has scale strides out of range", what);
 }
 
+namespace {
+
 bool in_place(const orda_fp8_matrix& m) {
   return m.ld % 16 == 0 && reinterpret_cast<uintptr_t>(m.codes) % 16 == 0;
 }
@@ -29,8 +32,8 @@ int64_t packed_bytes(const orda_fp8_matrix& m) {
 }
 
 int64_t check_product(const orda_fp8_matrix& a, const orda_fp8_matrix& b) {
-  check_matrix(a, "a");
-  check_matrix(b, "b");
+  check_fp8_matrix(a, "a");
+  check_fp8_matrix(b, "b");
   if (a.block_rows != 1) fail(ORDA_ERR_INVALID, "a must have a scale for each row (block_rows 1)");
   if (b.block_rows != 128) fail(ORDA_ERR_INVALID, "b must have a scale for each 128 rows (block_rows 128)");
   if (a.cols != b.cols)
@@ -53,7 +56,7 @@ int32_t orda_quant_fp8_blocks(int32_t device, void* hip_stream, const orda_tenso
     check_view(*m, "m");
     const DType t = to_dtype(m->dtype, "m");
     if (m->location != ORDA_DEVICE) fail(ORDA_ERR_INVALID, "m must be on the device");
-    check_matrix(*out, "out");
+    check_fp8_matrix(*out, "out");
     if (out->rows != m->rows || out->cols != m->cols) fail(ORDA_ERR_INVALID, "out must have the shape of m");
     if (m->rows == 0 || m->cols == 0) return;
     if (out->ld % 8 != 0 || reinterpret_cast<uintptr_t>(out->codes) % 8 != 0)

@@ -1,0 +1,212 @@
+// gradients.cpp — the norm of many gradients and their clipping
+// (orda_gradient_norm, orda_clip_gradients of include/orda/orda.h). The calls queue
+// their kernels and return; the scratch is the caller's.
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "orda_host.h"
+
+namespace orda {
+namespace {
+
+constexpr int64_t kMostGradients = int64_t{1} << 20, kMostValues = int64_t{1} << 40;
+
+// One row where nothing lies between the rows.
+GradPart part_of(const orda_tensor& src, const orda_tensor& dst) {
+  GradPart p{};
+  p.src = src.data;
+  p.dst = dst.data;
+  p.rows = src.rows;
+  p.cols = src.cols;
+  p.lds = tensor_ld(src);
+  p.ldd = tensor_ld(dst);
+  p.src_bf16 = src.dtype == ORDA_BF16;
+  p.dst_bf16 = dst.dtype == ORDA_BF16;
+  if (p.rows == 1 || (p.lds == p.cols && p.ldd == p.cols)) {
+    p.cols *= p.rows;
+    p.rows = 1;
+  }
+  return p;
+}
+
+// How the gradients are cut: launches of up to kGradParts of them, pieces of a row,
+// one sum for each workgroup.
+struct Cut {
+  int64_t piece;
+  std::vector<GradPart> parts;   // those that have values
+  struct Launch {
+    size_t from, to;
+    int64_t pieces;
+    int blocks, first;           // of its sums
+  };
+  std::vector<Launch> launches;
+  int sums = 0;
+  bool in_place = false;
+};
+
+int64_t pieces_of(const GradPart& p, int64_t piece) { return p.rows * ceil_div(p.cols, piece); }
+
+// Workgroups of all launches together: eight a CU. Each of the scaling ones adds all
+// sums up by itself.
+constexpr int64_t kBlocks = 2048;
+
+Cut cut(const orda_gradient* g, int64_t count, bool scale) {
+  if (count < 0 || count > kMostGradients) fail(ORDA_ERR_INVALID, "at most 2^20 gradients");
+  if (count > 0 && !g) fail(ORDA_ERR_INVALID, "null argument");
+  Cut c;
+  int64_t values = 0;
+  bool placed[2] = {false, false};
+  for (int64_t i = 0; i < count; ++i) {
+    const orda_tensor &s = g[i].src, &d = g[i].dst;
+    char what[48];
+    snprintf(what, sizeof what, "gradient %lld", static_cast<long long>(i));
+    check_view(s, what);
+    to_dtype(s.dtype, what);
+    if (s.location != ORDA_DEVICE) fail(ORDA_ERR_INVALID, "%s must be on the device", what);
+    if (s.rows > kMostValues || s.cols > kMostValues || (s.cols > 0 && s.rows > kMostValues / s.cols))
+      fail(ORDA_ERR_INVALID, "%s: at most 2^40 values", what);
+    values += s.rows * s.cols;
+    if (values > kMostValues) fail(ORDA_ERR_INVALID, "at most 2^40 values");
+    if (s.rows == 0 || s.cols == 0) continue;
+    placed[d.data != nullptr] = true;
+    if (d.data) {
+      check_view(d, "a destination");
+      to_dtype(d.dtype, "a destination");
+      if (d.location != ORDA_DEVICE) fail(ORDA_ERR_INVALID, "a destination must be on the device");
+      if (d.rows != s.rows || d.cols != s.cols)
+        fail(ORDA_ERR_INVALID, "the destination of %s must be [%lld, %lld]", what, static_cast<long long>(s.rows),
+             static_cast<long long>(s.cols));
+    }
+    c.parts.push_back(part_of(s, scale && d.data ? d : s));
+  }
+  if (scale && placed[0] && placed[1]) fail(ORDA_ERR_INVALID, "either all gradients have a destination or none");
+  c.in_place = !placed[1];
+  // Pieces of 4096 values or more: sixteen a thread; larger where there are many.
+  c.piece = std::min<int64_t>(std::max<int64_t>(ceil_div(ceil_div(values, kBlocks * 4), 2048) * 2048, 4096), 1 << 16);
+  int64_t pieces = 0;
+  for (const GradPart& p : c.parts) pieces += pieces_of(p, c.piece);
+  for (size_t at = 0; at < c.parts.size();) {
+    Cut::Launch l{at, std::min(at + kGradParts, c.parts.size()), 0, 0, c.sums};
+    for (; at < l.to; ++at) {
+      c.parts[at].first = l.pieces;
+      l.pieces += pieces_of(c.parts[at], c.piece);
+    }
+    // its share of the workgroups
+    l.blocks = static_cast<int>(std::min<int64_t>(l.pieces, std::max<int64_t>(1, kBlocks * l.pieces / pieces)));
+    c.sums += l.blocks;
+    c.launches.push_back(l);
+  }
+  return c;
+}
+
+// Memory from `from` to `to`, rows of `cols` bytes `ld` bytes apart.
+struct Span {
+  uintptr_t from, to;
+  int64_t cols, ld;
+  bool written;
+  bool operator<(const Span& o) const { return from < o.from; }
+};
+bool meet(const Span& a, const Span& b) {
+  if (a.to <= b.from || b.to <= a.from) return false;
+  // column ranges of one frame
+  const int64_t ld = a.ld;
+  if (ld == b.ld && a.cols < ld && b.cols < ld) {
+    const int64_t d = static_cast<int64_t>(b.from - a.from) % ld;   // (from is sorted)
+    return !(d >= a.cols && d + b.cols <= ld);
+  }
+  return true;
+}
+void check_apart(const Cut& c) {
+  std::vector<Span> spans;
+  auto add = [&](const void* p, const GradPart& g, int64_t ld, int64_t es, bool written) {
+    const auto from = reinterpret_cast<uintptr_t>(p);
+    spans.push_back({from, from + ((g.rows - 1) * ld + g.cols) * es, g.cols * es, g.rows == 1 ? 0 : ld * es, written});
+  };
+  for (const GradPart& g : c.parts) {
+    add(g.src, g, g.lds, g.src_bf16 ? 2 : 4, c.in_place);
+    if (!c.in_place) add(g.dst, g, g.ldd, g.dst_bf16 ? 2 : 4, true);
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 0; i < spans.size(); ++i)
+    for (size_t j = i + 1; j < spans.size() && spans[j].from < spans[i].to; ++j)
+      if ((spans[i].written || spans[j].written) && meet(spans[i], spans[j]))
+        fail(ORDA_ERR_INVALID, "gradients that are written share memory with others");
+}
+
+int64_t sum_bytes(const Cut& c) { return (c.sums * int64_t{8} + 255) / 256 * 256; }
+
+void run(int32_t device, hipStream_t st, const Cut& c, bool scale, double max_norm, double eps, float* norm, void* ws,
+         int64_t ws_bytes) {
+  const int64_t need = sum_bytes(c);
+  if (reinterpret_cast<uintptr_t>(ws) % 256 != 0) fail(ORDA_ERR_INVALID, "workspace must be 256-byte aligned");
+  if (ws_bytes < need || (need > 0 && !ws))
+    fail(ORDA_ERR_INVALID, "workspace of %lld bytes, %lld needed", static_cast<long long>(ws_bytes),
+         static_cast<long long>(need));
+  const DeviceScope scope(device);
+  auto* sums = static_cast<double*>(ws);
+  auto args = [&](const Cut::Launch& l) {
+    GradArgs a{};
+    std::copy(c.parts.begin() + l.from, c.parts.begin() + l.to, a.part);
+    a.count = static_cast<int32_t>(l.to - l.from);
+    a.pieces = l.pieces;
+    a.piece = c.piece;
+    a.sums = sums + l.first;
+    return a;
+  };
+  for (const Cut::Launch& l : c.launches) hip_check(launch_grad_sums(args(l), l.blocks, st), "gradient norm");
+  if (!scale || c.launches.empty()) {
+    hip_check(launch_grad_norm(sums, c.sums, norm, st), "gradient norm");
+    return;
+  }
+  for (size_t i = 0; i < c.launches.size(); ++i) {
+    GradArgs a = args(c.launches[i]);
+    a.all = sums;
+    a.n_sums = c.sums;
+    a.in_place = c.in_place;
+    a.max_norm = max_norm;
+    a.eps = eps;
+    a.norm = i == 0 ? norm : nullptr;
+    hip_check(launch_grad_scale(a, c.launches[i].blocks, st), "gradient clipping");
+  }
+}
+
+}  // namespace
+}  // namespace orda
+
+using namespace orda;
+
+extern "C" {
+
+int32_t orda_clip_gradients_workspace(const orda_gradient* gradients, int64_t count, int64_t* bytes, char* err,
+                                      size_t err_len) {
+  return guarded(err, err_len, [&] {
+    if (!bytes) fail(ORDA_ERR_INVALID, "null argument");
+    *bytes = std::max(sum_bytes(cut(gradients, count, true)), sum_bytes(cut(gradients, count, false)));
+  });
+}
+
+int32_t orda_gradient_norm(int32_t device, void* hip_stream, const orda_gradient* gradients, int64_t count, float* norm,
+                           void* workspace, int64_t workspace_bytes, char* err, size_t err_len) {
+  return guarded(err, err_len, [&] {
+    if (!norm) fail(ORDA_ERR_INVALID, "null argument");
+    const Cut c = cut(gradients, count, false);
+    run(device, static_cast<hipStream_t>(hip_stream), c, false, 0., 0., norm, workspace, workspace_bytes);
+  });
+}
+
+int32_t orda_clip_gradients(int32_t device, void* hip_stream, const orda_gradient* gradients, int64_t count,
+                            double max_norm, double eps, float* norm, void* workspace, int64_t workspace_bytes, char* err,
+                            size_t err_len) {
+  return guarded(err, err_len, [&] {
+    if (!norm) fail(ORDA_ERR_INVALID, "null argument");
+    if (!(max_norm >= 0.)) fail(ORDA_ERR_INVALID, "max_norm must be >= 0");
+    if (!(eps >= 0.) || !isfinite(eps)) fail(ORDA_ERR_INVALID, "eps must be >= 0 and finite");
+    const Cut c = cut(gradients, count, true);
+    check_apart(c);
+    run(device, static_cast<hipStream_t>(hip_stream), c, true, max_norm, eps, norm, workspace, workspace_bytes);
+  });
+}
+
+}  // extern "C"

@@ -94,6 +94,9 @@ inline void check_view(const orda_tensor& t, const char* what) {
   if (tensor_ld(t) < t.cols) fail(ORDA_ERR_INVALID, "%s has ld < cols", what);
 }
 
+// The same for a quantised matrix: its shape, pitch and scale strides.
+void check_fp8_matrix(const orda_fp8_matrix& m, const char* what);
+
 // A C entry point's body: no exception leaves it.
 template <class F>
 int32_t guarded(char* err, size_t err_len, F&& f) {

@@ -3,6 +3,7 @@
 #include <float.h>
 #include <math.h>
 
+#include "fp8_codes.h"
 #include "lds_dma.h"
 #include "orda_kernels.h"
 
@@ -23,43 +24,7 @@ typedef __attribute__((address_space(3))) const float lds_f32;
 // clamp takes back. A block with an infinity or a NaN has the scale NaN and codes
 // NaN. Bound by HBM, each value being read once into registers: the quotient is a
 // product with the reciprocal wherever that cannot change the code (`doubtful`),
-// an IEEE division for every value took twice as long.
-constexpr float kE4m3Max = 448.f;
-
-__device__ __forceinline__ float scale_of(uint32_t amax_bits) {
-  if (amax_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-  return fmaxf(__uint_as_float(amax_bits) / kE4m3Max, FLT_MIN);
-}
-__device__ __forceinline__ float coded(float x, float s) {
-  const float q = x / s;
-  return q != q ? q : fminf(fmaxf(q, -kE4m3Max), kE4m3Max);
-}
-// Whether x / s might round to another code than q = x * (1/s), which is at most 3
-// units in the last place off the rounded quotient: near a midpoint of two
-// codes (three bits of mantissa are kept: the other 20 near one half), or below
-// the smallest normal code, where the midpoints lie elsewhere.
-__device__ __forceinline__ bool doubtful(float q) {
-  const uint32_t u = __float_as_uint(q) & 0x7fffffffu;
-  return (u & 0xfffffu) - 0x7fffcu <= 8u || (u < 0x3c800004u && u != 0u) || u >= 0x7f800000u;
-}
-__device__ __forceinline__ uint32_t codes4(const float* x, float s, float r) {
-  float q[4];
-  bool doubt = false;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    q[k] = x[k] * r;
-    doubt |= doubtful(q[k]);
-    q[k] = fminf(fmaxf(q[k], -kE4m3Max), kE4m3Max);
-  }
-  if (doubt) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) q[k] = coded(x[k], s);
-  }
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
-  return static_cast<uint32_t>(w);
-}
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// an IEEE division for every value took twice as long (fp8_codes.h).
 
 // kC neighbouring values from column c on (0 past cols) of N rows by one load each,
 // aligned to their size or of any alignment. One branch for all the rows: a branch
@@ -83,11 +48,6 @@ __device__ __forceinline__ void load_rows(const E* const (&row)[N], int64_t c, i
   for (int q = 0; q < N; ++q)
 #pragma unroll
     for (int k = 0; k < kC; ++k) x[q][k] = static_cast<float>(w[q][k]);
-}
-// Their codes, the eight that hold the last column whole.
-__device__ __forceinline__ void store8(uint8_t* row, int64_t c, int64_t cols, const float (&x)[8], float s) {
-  const float r = __builtin_amdgcn_rcpf(s);
-  if (c < cols) *reinterpret_cast<u32x2*>(row + c) = u32x2{codes4(x, s, r), codes4(x + 4, s, r)};
 }
 
 // Blocks of one row: 16 lanes a block of 128, a wave 4 blocks of each of 4 rows,

@@ -1,0 +1,539 @@
+// norm.hip — the root-mean-square norm with the residual's addition, its output in
+// the rows' type or in e4m3, and its gradients.
+#include <math.h>
+
+#include "fp8_codes.h"
+#include "orda_kernels.h"
+
+namespace orda {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Eight neighbouring values as they lie in memory.
+template <typename E>
+struct Raw8 {
+  u32x4 q[sizeof(E) / 2];
+};
+
+// Columns c to c + 7 of a row of h. Every lane loads, those past the row's end from
+// within it, so that no branch makes a load wait for the one before. TAIL (h no
+// multiple of 8): the last eight that the row has, moved into place by `widened`.
+template <typename E, bool TAIL>
+__device__ __forceinline__ Raw8<E> fetch8(const E* row, int64_t c, int64_t h) {
+  Raw8<E> r;
+  if (TAIL && h < 8) {
+    E v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < h ? row[c + k] : static_cast<E>(0.f);
+    __builtin_memcpy(&r, v, sizeof r);
+  } else {
+    const int64_t at = TAIL ? (c <= h - 8 ? c : h - 8) : (c < h ? c : 0);
+    __builtin_memcpy(&r, row + at, sizeof r);
+  }
+  return r;
+}
+// Their values, 0 past the row's end.
+template <typename E, bool TAIL>
+__device__ __forceinline__ void widened(const Raw8<E>& r, int64_t c, int64_t h, float (&x)[8]) {
+  E v[8];
+  __builtin_memcpy(v, &r, sizeof r);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) x[k] = static_cast<float>(v[k]);
+  if constexpr (TAIL) {
+    if (h < 8) return;
+    const int64_t past = c - (h - 8);
+    const int d = past < 0 ? 0 : past < 8 ? static_cast<int>(past) : 8;
+#pragma unroll
+    for (int b = 4; b; b /= 2)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = (d & b) ? (k + b < 8 ? x[k + b] : 0.f) : x[k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = d >= 8 ? 0.f : x[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = c < h ? x[k] : 0.f;
+  }
+}
+template <typename E, bool TAIL>
+__device__ __forceinline__ void put8(E* row, int64_t c, int64_t h, const float (&x)[8]) {
+  E v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = static_cast<E>(x[k]);
+  if (c + 8 <= h) {
+    __builtin_memcpy(row + c, v, sizeof v);
+  } else if (TAIL) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < h) row[c + k] = v[k];
+  }
+}
+
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int d = 32; d; d /= 2) x += __shfl_xor(x, d);
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int d = 32; d; d /= 2) x += __shfl_xor(x, d);
+  return x;
+}
+
+// Codes and scales of a lane's eight values; 16 lanes hold a block of 128.
+__device__ __forceinline__ void put_codes(const NormArgs& a, int64_t row, int64_t c, const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m = abs_bits(v[k]) > m ? abs_bits(v[k]) : m;
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) {
+    const uint32_t o = __shfl_xor(m, d);
+    m = o > m ? o : m;
+  }
+  const float s = scale_of(m);
+  store8(a.codes + row * a.ldc, c, a.h, v, s);
+  if ((threadIdx.x & 15) == 0 && c < a.h) a.scales[row * a.scale_row + c / 128 * a.scale_col] = s;
+}
+
+// v = t·s·(w + offset). To e4m3 in 64 bits, rounded to fp32 at the end: next to a
+// border of two codes fp32's own roundings would decide, and the codes are those of
+// the formula.
+template <bool FP8>
+__device__ __forceinline__ void normed(const float (&t)[8], double s, const float (&w)[8], double offset, float (&v)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if constexpr (FP8) {
+      v[k] = static_cast<float>(static_cast<double>(t[k]) * s * (static_cast<double>(w[k]) + offset));
+    } else {
+      v[k] = t[k] * static_cast<float>(s) * (w[k] + static_cast<float>(offset));
+    }
+  }
+}
+
+// NT threads hold a row in registers, NV vectors of eight columns each.
+template <typename E, typename W, int NT, int NV, bool TAIL, bool FP8>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(NormArgs a) {
+  constexpr int kTeams = NT < 256 ? 256 / NT : 1, kWaves = NT / 64;
+  __shared__ double part[kTeams][kWaves];
+  const int team = threadIdx.x / NT, at = threadIdx.x % NT;
+  const int64_t row0 = blockIdx.x * int64_t{kTeams} + team;
+  const bool live = row0 < a.n;
+  const int64_t row = live ? row0 : a.n - 1;
+  Raw8<E> x[NV], r[NV];
+  Raw8<W> wr[NV];
+  const E* px = static_cast<const E*>(a.x) + row * a.ldx;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) x[i] = fetch8<E, TAIL>(px, (i * NT + at) * int64_t{8}, a.h);
+  if (a.r) {
+    const E* pr = static_cast<const E*>(a.r) + row * a.ldr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) r[i] = fetch8<E, TAIL>(pr, (i * NT + at) * int64_t{8}, a.h);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) wr[i] = fetch8<W, TAIL>(static_cast<const W*>(a.w), (i * NT + at) * int64_t{8}, a.h);
+  float t[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) widened<E, TAIL>(x[i], (i * NT + at) * int64_t{8}, a.h, t[i]);
+  if (a.r) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float y[8];
+      widened<E, TAIL>(r[i], (i * NT + at) * int64_t{8}, a.h, y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t[i][k] = static_cast<float>(static_cast<E>(t[i][k] + y[k]));
+    }
+  }
+  if (a.total && live) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      put8<E, TAIL>(static_cast<E*>(a.total) + row * a.ldt, (i * NT + at) * int64_t{8}, a.h, t[i]);
+  }
+  double sum = 0.;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum = fma(static_cast<double>(t[i][k]), static_cast<double>(t[i][k]), sum);
+  sum = wave_sum(sum);
+  if constexpr (kWaves > 1) {
+    if ((at & 63) == 0) part[team][at >> 6] = sum;
+    __syncthreads();
+    sum = 0.;
+#pragma unroll
+    for (int q = 0; q < kWaves; ++q) sum += part[team][q];
+  }
+  const double s = 1. / sqrt(sum / static_cast<double>(a.h) + a.eps);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t c = (i * NT + at) * int64_t{8};
+    float w[8], v[8];
+    widened<W, TAIL>(wr[i], c, a.h, w);
+    normed<FP8>(t[i], s, w, a.offset, v);
+    if constexpr (FP8) {
+      if (live) put_codes(a, row, c, v);
+    } else {
+      if (live) put8<E, TAIL>(static_cast<E*>(a.out) + row * a.ldo, c, a.h, v);
+    }
+  }
+}
+
+// Rows longer than registers hold: a workgroup a row, read twice.
+template <typename E, typename W, bool FP8>
+__global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
+  __shared__ double part[16];
+  const int64_t row = blockIdx.x;
+  const E* px = static_cast<const E*>(a.x) + row * a.ldx;
+  const E* pr = a.r ? static_cast<const E*>(a.r) + row * a.ldr : nullptr;
+  auto totals = [&](int64_t c, float (&t)[8]) {
+    widened<E, true>(fetch8<E, true>(px, c, a.h), c, a.h, t);
+    if (!pr) return;
+    float y[8];
+    widened<E, true>(fetch8<E, true>(pr, c, a.h), c, a.h, y);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = static_cast<float>(static_cast<E>(t[k] + y[k]));
+  };
+  double sum = 0.;
+  for (int64_t c = threadIdx.x * int64_t{8}; c < a.h; c += 8192) {
+    float t[8];
+    totals(c, t);
+    if (a.total) put8<E, true>(static_cast<E*>(a.total) + row * a.ldt, c, a.h, t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum = fma(static_cast<double>(t[k]), static_cast<double>(t[k]), sum);
+  }
+  sum = wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = 0.;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) sum += part[q];
+  const double s = 1. / sqrt(sum / static_cast<double>(a.h) + a.eps);
+  // (Whole waves take part in a block's maximum: the columns past the end are 0.)
+  for (int64_t c = threadIdx.x * int64_t{8}; c - threadIdx.x % 64 * 8 < a.h; c += 8192) {
+    float t[8], w[8], v[8];
+    totals(c, t);
+    widened<W, true>(fetch8<W, true>(static_cast<const W*>(a.w), c, a.h), c, a.h, w);
+    normed<FP8>(t, s, w, a.offset, v);
+    if constexpr (FP8) put_codes(a, row, c, v);
+    else put8<E, true>(static_cast<E*>(a.out) + row * a.ldo, c, a.h, v);
+  }
+}
+
+// ------------------------------------------------------------ gradients
+// A row's two sums and what follows from them.
+struct RowGrad {
+  float s, k;   // dx = s·(g·q - t·k) + gt
+};
+__device__ __forceinline__ RowGrad row_grad(double sq, float dot, const NormGradArgs& a) {
+  const double s = 1. / sqrt(sq / static_cast<double>(a.h) + a.eps);
+  return {static_cast<float>(s), static_cast<float>(s * s * (static_cast<double>(dot) / static_cast<double>(a.h)))};
+}
+
+// Workgroups of teams of NT threads, a row a team at a time; a thread's columns of
+// the weight and of its gradient stay in registers. ws: a row of fp32 a workgroup.
+template <typename E, typename W, int NT, int NV, bool TAIL>
+__global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a) {
+  constexpr int kTeams = 1024 / NT, kWaves = NT / 64;
+  __shared__ double part_sq[2][kTeams][kWaves];
+  __shared__ float part_dot[2][kTeams][kWaves];
+  __shared__ float acc[NT * NV * 8];
+  const int team = threadIdx.x / NT, at = threadIdx.x % NT;
+  float q[NV][8], dw[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t c = (i * NT + at) * int64_t{8};
+    widened<W, TAIL>(fetch8<W, TAIL>(static_cast<const W*>(a.w), c, a.h), c, a.h, q[i]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      q[i][k] = c + k < a.h ? q[i][k] + static_cast<float>(a.offset) : 0.f;
+      dw[i][k] = 0.f;
+    }
+  }
+  const int64_t step = gridDim.x * int64_t{kTeams};
+  int turn = 0;
+  for (int64_t r0 = blockIdx.x * int64_t{kTeams}; r0 < a.n; r0 += step, turn ^= 1) {
+    const bool live = r0 + team < a.n;
+    const int64_t row = live ? r0 + team : a.n - 1;
+    Raw8<E> rg[NV], rt[NV], rx[NV];
+    const E* pg = static_cast<const E*>(a.g) + row * a.ldg;
+    const E* pt = static_cast<const E*>(a.t) + row * a.ldt;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      rg[i] = fetch8<E, TAIL>(pg, (i * NT + at) * int64_t{8}, a.h);
+      rt[i] = fetch8<E, TAIL>(pt, (i * NT + at) * int64_t{8}, a.h);
+    }
+    if (a.gt) {
+      const E* px = static_cast<const E*>(a.gt) + row * a.ldgt;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) rx[i] = fetch8<E, TAIL>(px, (i * NT + at) * int64_t{8}, a.h);
+    }
+    float g[NV][8], t[NV][8];
+    double sq = 0.;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (i * NT + at) * int64_t{8};
+      widened<E, TAIL>(rg[i], c, a.h, g[i]);
+      widened<E, TAIL>(rt[i], c, a.h, t[i]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        sq = fma(static_cast<double>(t[i][k]), static_cast<double>(t[i][k]), sq);
+        dot = fmaf(g[i][k] * q[i][k], t[i][k], dot);
+      }
+    }
+    sq = wave_sum(sq);
+    dot = wave_sum(dot);
+    if constexpr (kWaves > 1) {
+      if ((at & 63) == 0) {
+        part_sq[turn][team][at >> 6] = sq;
+        part_dot[turn][team][at >> 6] = dot;
+      }
+      __syncthreads();
+      sq = 0.;
+      dot = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        sq += part_sq[turn][team][w];
+        dot += part_dot[turn][team][w];
+      }
+    }
+    const RowGrad f = row_grad(sq, dot, a);
+    if (!live) continue;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (i * NT + at) * int64_t{8};
+      float y[8], d[8];
+      if (a.gt) widened<E, TAIL>(rx[i], c, a.h, y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        d[k] = f.s * (g[i][k] * q[i][k] - t[i][k] * f.k);
+        if (a.gt) d[k] += y[k];
+        dw[i][k] = fmaf(g[i][k], t[i][k] * f.s, dw[i][k]);
+      }
+      if (a.dx) put8<E, TAIL>(static_cast<E*>(a.dx) + row * a.ldd, c, a.h, d);
+    }
+  }
+  if (!a.dw) return;
+  // the teams' sums in their order
+  for (int p = 0; p < kTeams; ++p) {
+    if (p == team) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float& s = acc[(k * NV + i) * NT + at];
+          s = p ? s + dw[i][k] : dw[i][k];
+        }
+    }
+    __syncthreads();
+  }
+  float* out = static_cast<float*>(a.ws) + blockIdx.x * a.h;
+  for (int64_t c = threadIdx.x; c < a.h; c += 1024) {
+    const int v = static_cast<int>(c / 8);
+    out[c] = acc[(static_cast<int>(c % 8) * NV + v / NT) * NT + v % NT];
+  }
+}
+
+// Longer rows: their factors first (a workgroup a row), then tiles of 2048 columns
+// and `each` rows.
+template <typename E, typename W>
+__global__ __launch_bounds__(1024) void norm_grad_rows_kernel(NormGradArgs a) {
+  __shared__ double part_sq[16];
+  __shared__ float part_dot[16];
+  const int64_t row = blockIdx.x;
+  const E* pg = static_cast<const E*>(a.g) + row * a.ldg;
+  const E* pt = static_cast<const E*>(a.t) + row * a.ldt;
+  double sq = 0.;
+  float dot = 0.f;
+  for (int64_t c = threadIdx.x * int64_t{8}; c < a.h; c += 8192) {
+    float g[8], t[8], q[8];
+    widened<E, true>(fetch8<E, true>(pg, c, a.h), c, a.h, g);
+    widened<E, true>(fetch8<E, true>(pt, c, a.h), c, a.h, t);
+    widened<W, true>(fetch8<W, true>(static_cast<const W*>(a.w), c, a.h), c, a.h, q);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      sq = fma(static_cast<double>(t[k]), static_cast<double>(t[k]), sq);
+      dot = fmaf(g[k] * (q[k] + static_cast<float>(a.offset)), t[k], dot);
+    }
+  }
+  sq = wave_sum(sq);
+  dot = wave_sum(dot);
+  if ((threadIdx.x & 63) == 0) {
+    part_sq[threadIdx.x >> 6] = sq;
+    part_dot[threadIdx.x >> 6] = dot;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  sq = 0.;
+  dot = 0.f;
+  for (int w = 0; w < 16; ++w) {
+    sq += part_sq[w];
+    dot += part_dot[w];
+  }
+  static_cast<RowGrad*>(a.ws)[row] = row_grad(sq, dot, a);
+}
+template <typename E, typename W>
+__global__ __launch_bounds__(256) void norm_grad_tiles_kernel(NormGradArgs a, const RowGrad* rows, float* parts,
+                                                              int64_t each) {
+  const int64_t across = (a.h + 2047) / 2048, tile = blockIdx.x % across, band = blockIdx.x / across;
+  const int64_t c = (tile * 256 + threadIdx.x) * 8;
+  float q[8], dw[8];
+  widened<W, true>(fetch8<W, true>(static_cast<const W*>(a.w), c, a.h), c, a.h, q);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    q[k] += static_cast<float>(a.offset);
+    dw[k] = 0.f;
+  }
+  const int64_t end = (band + 1) * each < a.n ? (band + 1) * each : a.n;
+  for (int64_t row = band * each; row < end; ++row) {
+    float g[8], t[8], y[8], d[8];
+    widened<E, true>(fetch8<E, true>(static_cast<const E*>(a.g) + row * a.ldg, c, a.h), c, a.h, g);
+    widened<E, true>(fetch8<E, true>(static_cast<const E*>(a.t) + row * a.ldt, c, a.h), c, a.h, t);
+    if (a.gt) widened<E, true>(fetch8<E, true>(static_cast<const E*>(a.gt) + row * a.ldgt, c, a.h), c, a.h, y);
+    const RowGrad f = rows[row];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      d[k] = f.s * (g[k] * q[k] - t[k] * f.k);
+      if (a.gt) d[k] += y[k];
+      dw[k] = fmaf(g[k], t[k] * f.s, dw[k]);
+    }
+    if (a.dx) put8<E, true>(static_cast<E*>(a.dx) + row * a.ldd, c, a.h, d);
+  }
+  if (a.dw) put8<float, true>(parts + band * a.h, c, a.h, dw);
+}
+
+// dw[c] = Σ_p parts[p][c]: 64 columns a workgroup, 16 threads a column.
+template <typename W>
+__global__ __launch_bounds__(1024) void norm_grad_join_kernel(const float* parts, int64_t count, int64_t h, W* dw) {
+  __shared__ float sums[16][64];
+  const int k = threadIdx.x & 63, p0 = threadIdx.x >> 6;
+  const int64_t c = blockIdx.x * int64_t{64} + k;
+  float s = 0.f;
+  if (c < h)
+    for (int64_t p = p0; p < count; p += 16) s += parts[p * h + c];
+  sums[p0][k] = s;
+  __syncthreads();
+  if (p0 == 0 && c < h) {
+    for (int p = 1; p < 16; ++p) s += sums[p][k];
+    dw[c] = static_cast<W>(s);
+  }
+}
+
+// ------------------------------------------------------------ launches
+using NormKernel = void (*)(NormArgs);
+struct NormLaunch {
+  NormKernel k;
+  int threads, teams;
+};
+template <typename E, typename W, bool TAIL, bool FP8>
+NormLaunch norm_launch(int64_t n, int64_t h) {
+  // Few rows: as many threads as a row has vectors.
+  if (n < 1024) {
+    if (h <= 2048) return {norm_kernel<E, W, 256, 1, TAIL, FP8>, 256, 1};
+    if (h <= 8192) return {norm_kernel<E, W, 1024, 1, TAIL, FP8>, 1024, 1};
+  }
+  if (h <= 1024) return {norm_kernel<E, W, 64, 2, TAIL, FP8>, 256, 4};
+  if (h <= 2048) return {norm_kernel<E, W, 64, 4, TAIL, FP8>, 256, 4};
+  if (h <= 4096) return {norm_kernel<E, W, 64, 8, TAIL, FP8>, 256, 4};
+  if (h <= 8192) return {norm_kernel<E, W, 256, 4, TAIL, FP8>, 256, 1};
+  if (h <= 32768) return {norm_kernel<E, W, 1024, 4, TAIL, FP8>, 1024, 1};
+  return {norm_long_kernel<E, W, FP8>, 1024, 1};
+}
+template <typename E, typename W>
+NormLaunch norm_launch(const NormArgs& a) {
+  if (a.codes)
+    return a.h % 8 ? norm_launch<E, W, true, true>(a.n, a.h) : norm_launch<E, W, false, true>(a.n, a.h);
+  return a.h % 8 ? norm_launch<E, W, true, false>(a.n, a.h) : norm_launch<E, W, false, false>(a.n, a.h);
+}
+
+using GradKernel = void (*)(NormGradArgs);
+struct GradLaunch {
+  GradKernel k;   // null: rows too long for registers
+  int teams;
+};
+template <typename E, typename W, bool TAIL>
+GradLaunch grad_launch(int64_t h) {
+  if (h <= 512) return {norm_grad_kernel<E, W, 64, 1, TAIL>, 16};
+  if (h <= 2048) return {norm_grad_kernel<E, W, 256, 1, TAIL>, 4};
+  if (h <= 4096) return {norm_grad_kernel<E, W, 256, 2, TAIL>, 4};
+  if (h <= 8192) return {norm_grad_kernel<E, W, 1024, 1, TAIL>, 1};
+  if (h <= 16384) return {norm_grad_kernel<E, W, 1024, 2, TAIL>, 1};
+  return {nullptr, 0};
+}
+int grad_teams(int64_t h) { return h <= 512 ? 16 : h <= 4096 ? 4 : 1; }
+
+constexpr int64_t kGradBlocks = 256;   // workgroups that keep sums of the weight's gradient
+constexpr int64_t kLongRow = 16384;
+
+int64_t grad_blocks(int64_t n, int64_t h) {
+  const int64_t b = (n + grad_teams(h) - 1) / grad_teams(h);
+  return b < kGradBlocks ? b : kGradBlocks;
+}
+// Bands of rows of the tiles of long rows: enough tiles to fill the device.
+int64_t grad_bands(int64_t n, int64_t h) {
+  const int64_t across = (h + 2047) / 2048, want = (1024 + across - 1) / across;
+  return n < want ? n : want;
+}
+
+template <typename E, typename W>
+hipError_t norm_grad(const NormGradArgs& a, hipStream_t stream) {
+  const float* parts = static_cast<const float*>(a.ws);
+  int64_t count;
+  const GradLaunch l = a.h % 8 ? grad_launch<E, W, true>(a.h) : grad_launch<E, W, false>(a.h);
+  if (l.k) {
+    count = grad_blocks(a.n, a.h);
+    hipLaunchKernelGGL(l.k, dim3(static_cast<unsigned>(count)), dim3(1024), 0, stream, a);
+  } else {
+    float* p = static_cast<float*>(a.ws) + (a.n * 2 + 63) / 64 * 64;
+    const int64_t bands = grad_bands(a.n, a.h), each = (a.n + bands - 1) / bands;
+    count = (a.n + each - 1) / each;
+    constexpr int64_t kMost = most_blocks(1024);
+    if (a.n > kMost) return hipErrorInvalidValue;   // 128 GiB of rows
+    hipLaunchKernelGGL((norm_grad_rows_kernel<E, W>), dim3(static_cast<unsigned>(a.n)), dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((norm_grad_tiles_kernel<E, W>), dim3(static_cast<unsigned>(count * ((a.h + 2047) / 2048))),
+                       dim3(256), 0, stream, a, static_cast<const RowGrad*>(a.ws), p, each);
+    parts = p;
+  }
+  if (a.dw)
+    hipLaunchKernelGGL((norm_grad_join_kernel<W>), dim3(static_cast<unsigned>((a.h + 63) / 64)), dim3(1024), 0, stream,
+                       parts, count, a.h, static_cast<W*>(a.dw));
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_norm(const NormArgs& a, DType rows, DType weight, hipStream_t stream) {
+  const NormLaunch l = rows == DType::BF16
+                           ? (weight == DType::BF16 ? norm_launch<__bf16, __bf16>(a) : norm_launch<__bf16, float>(a))
+                           : (weight == DType::BF16 ? norm_launch<float, __bf16>(a) : norm_launch<float, float>(a));
+  const int64_t es = dtype_size(rows), most = most_blocks(l.threads) / l.teams * l.teams;   // rows of a launch
+  for (int64_t r = 0; r < a.n; r += most) {
+    NormArgs p = a;
+    p.n = a.n - r < most ? a.n - r : most;
+    auto past = [&](const void* d, int64_t ld) {
+      return d ? static_cast<char*>(const_cast<void*>(d)) + r * ld * es : nullptr;
+    };
+    p.x = past(a.x, a.ldx);
+    p.r = past(a.r, a.ldr);
+    p.total = past(a.total, a.ldt);
+    p.out = past(a.out, a.ldo);
+    if (a.codes) {
+      p.codes = a.codes + r * a.ldc;
+      p.scales = a.scales + r * a.scale_row;
+    }
+    hipLaunchKernelGGL(l.k, dim3(static_cast<unsigned>((p.n + l.teams - 1) / l.teams)), dim3(l.threads), 0, stream, p);
+  }
+  return hipGetLastError();
+}
+
+int64_t norm_grad_scratch(int64_t n, int64_t h) {
+  if (n == 0 || h == 0) return 0;
+  const int64_t words = h <= kLongRow ? grad_blocks(n, h) * h : (n * 2 + 63) / 64 * 64 + grad_bands(n, h) * h;
+  return (words * 4 + 255) / 256 * 256;
+}
+
+hipError_t launch_norm_grad(const NormGradArgs& a, DType rows, DType weight, hipStream_t stream) {
+  if (rows == DType::BF16)
+    return weight == DType::BF16 ? norm_grad<__bf16, __bf16>(a, stream) : norm_grad<__bf16, float>(a, stream);
+  return weight == DType::BF16 ? norm_grad<float, __bf16>(a, stream) : norm_grad<float, float>(a, stream);
+}
+
+}  // namespace orda

@@ -599,4 +599,80 @@ struct Fp8MmArgs {
 };
 hipError_t launch_fp8_mm(const Fp8MmArgs& a, DType out, hipStream_t stream);
 
+// ---------------------------------------------------------------- root-mean-square norm
+// t = x + r in the rows' type (t = x without r), s = (mean t² + eps)^-1/2 of a row,
+// v = t·s·(w + offset): out = v in the rows' type, or codes and scales of v (blocks
+// of one row and 128 columns). total, out and codes are written where set.
+struct NormArgs {
+  const void *x, *r;      // r null: none
+  int64_t ldx, ldr;
+  const void* w;
+  int64_t n, h;
+  double eps, offset;
+  void *total, *out;
+  int64_t ldt, ldo;
+  uint8_t* codes;         // pitch a multiple of 8, as Fp8QuantArgs
+  int64_t ldc;
+  float* scales;
+  int64_t scale_row, scale_col;
+};
+hipError_t launch_norm(const NormArgs& a, DType rows, DType weight, hipStream_t stream);
+// With q = w + offset, d = Σ_h g·q·t:  dx = s·(g·q - t·s²·d/h) + gt, and
+// dw[h] = Σ_rows g·t·s, the rows added in an order that n, h and the device fix.
+struct NormGradArgs {
+  const void *g, *t, *gt;  // gt null: none
+  int64_t ldg, ldt, ldgt;
+  const void* w;
+  int64_t n, h;
+  double eps, offset;
+  void *dx, *dw;           // written where set
+  int64_t ldd;
+  void* ws;
+};
+int64_t norm_grad_scratch(int64_t n, int64_t h);
+hipError_t launch_norm_grad(const NormGradArgs& a, DType rows, DType weight, hipStream_t stream);
+
+// ---------------------------------------------------------------- gradient norm and clipping
+// A matrix of gradients: rows of cols values, ld apart (contiguous ones: one row).
+struct GradPart {
+  const void* src;
+  void* dst;               // null: the norm alone
+  int64_t rows, cols, lds, ldd;
+  int64_t first;           // of its pieces among the launch's
+  int32_t src_bf16, dst_bf16;
+};
+constexpr int kGradParts = 56;   // of one launch: they travel in its arguments
+struct GradArgs {
+  GradPart part[kGradParts];
+  int32_t count;
+  int64_t pieces, piece;   // of `piece` values each (a row's last one fewer)
+  double* sums;            // the launch's, one a workgroup
+  // clipping: all launches' sums
+  const double* all;
+  int32_t n_sums, in_place;
+  double max_norm, eps;
+  float* norm;             // written by one workgroup where set
+};
+hipError_t launch_grad_sums(const GradArgs& a, int blocks, hipStream_t stream);
+hipError_t launch_grad_scale(const GradArgs& a, int blocks, hipStream_t stream);
+hipError_t launch_grad_norm(const double* sums, int n, float* norm, hipStream_t stream);
+
+// ---------------------------------------------------------------- drawing tokens
+struct SampleArgs {
+  const void* x;           // logits [n,v]
+  int64_t n, v, ldx;
+  const float* u;
+  const float *t, *p, *m;  // a row's own, or null: the one value beside
+  const int32_t* k;
+  float t1, p1, m1;
+  int32_t k1;
+  int64_t* token;
+  float* logprob;          // or null
+  uint32_t *tops, *firsts; // largest keys of the row's 64s and of its 1024s
+  double* masses;          // of its 1024s
+  int64_t n64, n1024;
+};
+int64_t sample_scratch(int64_t n, int64_t v, int64_t* tops, int64_t* firsts);   // bytes; masses come first
+hipError_t launch_sample(const SampleArgs& a, DType t, hipStream_t stream);
+
 }  // namespace orda

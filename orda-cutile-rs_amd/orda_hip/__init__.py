@@ -9,8 +9,9 @@ resolver functions. Compute runs in liborda_hip.so through the C ABI of
 include/orda/orda.h; torch tensors (or numpy arrays) carry the memory.
 
 Beside it stand operators that the crate does not have (orda_hip/operators.py):
-``linear_cross_entropy``, ``embedding`` and their gradients,
-``quantize_fp8_blocks`` and ``fp8_block_matmul``, on torch's GPU tensors.
+``linear_cross_entropy``, ``embedding``, ``rms_norm`` and their gradients,
+``quantize_fp8_blocks``, ``fp8_block_matmul`` and ``rms_norm_fp8``, ``sample_tokens``
+and ``clip_gradients``, on torch's GPU tensors.
 """
 from __future__ import annotations
 
@@ -21,8 +22,9 @@ from typing import Any, Optional
 import numpy as np
 
 from . import _lib as L
-from .operators import (embedding, embedding_backward, fp8_block_matmul, linear_cross_entropy,
-                        linear_cross_entropy_backward, quantize_fp8_blocks)
+from .operators import (clip_gradients, embedding, embedding_backward, fp8_block_matmul, gradient_norm,
+                        linear_cross_entropy, linear_cross_entropy_backward, quantize_fp8_blocks, rms_norm,
+                        rms_norm_backward, rms_norm_fp8, sample_tokens)
 from .types import (Backend, ChunkPlan, ChunkSize, DistillationLossOutput, KernelConfig,
                     LossOptions, OrdaError, Profile, Reduction, Teacher, TeacherMode,
                     DEFAULT_MAX_FUSED_SIZE, is_power_of_two)
@@ -30,11 +32,12 @@ from .types import (Backend, ChunkPlan, ChunkSize, DistillationLossOutput, Kerne
 __all__ = [
     "Backend", "ChunkPlan", "ChunkSize", "Context", "DistillationLossOutput", "KernelConfig",
     "LossOptions", "OrdaError", "Profile", "Reduction", "Teacher", "TeacherMode",
-    "DEFAULT_MAX_FUSED_SIZE", "chunk_doubling_schedule", "chunks_from_raw",
+    "DEFAULT_MAX_FUSED_SIZE", "chunk_doubling_schedule", "chunks_from_raw", "clip_gradients",
     "default_max_chunks_limit", "distillation_loss", "embedding", "embedding_backward",
-    "fp8_block_matmul", "is_available", "is_power_of_two",
+    "fp8_block_matmul", "gradient_norm", "is_available", "is_power_of_two",
     "kl_ce_on_logits_chunk", "linear_cross_entropy", "linear_cross_entropy_backward",
-    "quant_rows_int8", "quantize_fp8_blocks", "resolve_chunk_size", "lib_path",
+    "quant_rows_int8", "quantize_fp8_blocks", "resolve_chunk_size", "rms_norm", "rms_norm_backward",
+    "rms_norm_fp8", "sample_tokens", "lib_path",
 ]
 
 lib_path = L.LIB_PATH

@@ -88,6 +88,22 @@ class Fp8MatrixC(C.Structure):
                 ("block_rows", C.c_int32)]
 
 
+class RmsNormC(C.Structure):
+    _fields_ = [("x", Tensor), ("residual", Tensor), ("weight", Tensor), ("eps", C.c_double),
+                ("weight_offset", C.c_double)]
+
+
+class GradientC(C.Structure):
+    _fields_ = [("src", Tensor), ("dst", Tensor)]
+
+
+class SamplingC(C.Structure):
+    _fields_ = [("logits", Tensor), ("uniform", C.c_void_p), ("temperatures", C.c_void_p),
+                ("top_ps", C.c_void_p), ("min_ps", C.c_void_p), ("top_ks", C.c_void_p),
+                ("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("top_k", C.c_int32)]
+
+
 # (name, restype, argtypes) for every entry point of include/orda/orda.h.
 SIGNATURES = [
     ("orda_abi_version", C.c_int32, []),
@@ -158,6 +174,30 @@ SIGNATURES = [
     ("orda_fp8_block_matmul", C.c_int32,
      [C.c_int32, C.c_void_p, C.POINTER(Fp8MatrixC), C.POINTER(Fp8MatrixC), C.POINTER(Tensor),
       C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t]),
+    ("orda_rms_norm_forward", C.c_int32,
+     [C.c_int32, C.c_void_p, C.POINTER(RmsNormC), C.POINTER(Tensor), C.POINTER(Tensor), C.c_char_p,
+      C.c_size_t]),
+    ("orda_rms_norm_fp8", C.c_int32,
+     [C.c_int32, C.c_void_p, C.POINTER(RmsNormC), C.POINTER(Tensor), C.POINTER(Fp8MatrixC), C.c_char_p,
+      C.c_size_t]),
+    ("orda_rms_norm_backward_workspace", C.c_int32,
+     [C.c_int64, C.c_int64, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
+    ("orda_rms_norm_backward", C.c_int32,
+     [C.c_int32, C.c_void_p, C.POINTER(RmsNormC), C.POINTER(Tensor), C.POINTER(Tensor), C.POINTER(Tensor),
+      C.POINTER(Tensor), C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t]),
+    ("orda_clip_gradients_workspace", C.c_int32,
+     [C.c_void_p, C.c_int64, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
+    ("orda_gradient_norm", C.c_int32,
+     [C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_char_p,
+      C.c_size_t]),
+    ("orda_clip_gradients", C.c_int32,
+     [C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_double, C.c_double, C.c_void_p, C.c_void_p,
+      C.c_int64, C.c_char_p, C.c_size_t]),
+    ("orda_sample_tokens_workspace", C.c_int32,
+     [C.c_int64, C.c_int64, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
+    ("orda_sample_tokens", C.c_int32,
+     [C.c_int32, C.c_void_p, C.POINTER(SamplingC), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
+      C.c_char_p, C.c_size_t]),
 ]
 
 _lib = None

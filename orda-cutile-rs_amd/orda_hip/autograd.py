@@ -21,7 +21,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import (Context, distillation_loss, embedding, linear_cross_entropy,
-               linear_cross_entropy_backward)
+               linear_cross_entropy_backward, rms_norm, rms_norm_backward)
 from . import _lib as L
 from .operators import _embed_grad, _gpu_tensor, _ids, _padding_row
 from .types import LossOptions, OrdaError, Teacher, TeacherMode
@@ -201,3 +201,40 @@ def embedding_autograd(ids: torch.Tensor, weight: torch.Tensor, *, scale: float 
     of ``weight`` by sorted tokens, the same bits in every run; ``padding_idx``
     names a row that gets none."""
     return EmbeddingFunction.apply(ids, weight, scale, padding_idx)
+
+
+class RmsNormFunction(torch.autograd.Function):
+    """out, total = RmsNormFunction.apply(x, weight, residual, eps, weight_offset);
+    total is None without a residual."""
+
+    @staticmethod
+    def forward(fctx, x, weight, residual, eps, weight_offset):
+        if residual is None:
+            out, total = rms_norm(x, weight, eps=eps, weight_offset=weight_offset), None
+        else:
+            out, total = rms_norm(x, weight, residual=residual, eps=eps, weight_offset=weight_offset)
+        fctx.save_for_backward(x if total is None else total, weight)
+        fctx.opts = eps, weight_offset
+        fctx.set_materialize_grads(False)
+        return out, total
+
+    @_first_order
+    def backward(fctx, g_out, g_total):
+        want_x, want_w, want_r = fctx.needs_input_grad[:3]
+        total, weight = fctx.saved_tensors
+        eps, weight_offset = fctx.opts
+        if g_out is None:   # the norm's result went nowhere
+            return (g_total if want_x else None, torch.zeros_like(weight) if want_w else None,
+                    g_total if want_r else None, None, None)
+        gx, gw = rms_norm_backward(g_out, total, weight, grad_total=g_total, eps=eps, weight_offset=weight_offset,
+                                   grad_x=want_x or want_r, grad_weight=want_w)
+        return gx if want_x else None, gw, gx if want_r else None, None, None
+
+
+def rms_norm_autograd(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
+                      eps: float = 1e-6, weight_offset: float = 0.0):
+    """Differentiable form of ``rms_norm``: its result, with a residual ``(result, t)``,
+    where ``t`` is the sum for the next residual. The sum is rounded to x's type, which
+    the gradients count as the identity."""
+    out, total = RmsNormFunction.apply(x, weight, residual, eps, weight_offset)
+    return out if residual is None else (out, total)

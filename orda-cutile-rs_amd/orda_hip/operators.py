@@ -7,6 +7,11 @@
 * ``quantize_fp8_blocks`` / ``fp8_block_matmul``: matrices in e4m3 with a scale for
   each block of 128, and their product (a teacher's logits from a head held in 8
   bits, for ``Teacher.Precomputed``). Not differentiable.
+* ``rms_norm`` / ``rms_norm_backward``: the norm before the head, with the
+  residual's addition; ``rms_norm_fp8``: its output in e4m3, for ``fp8_block_matmul``.
+* ``sample_tokens``: tokens drawn from the head's logits.
+* ``clip_gradients`` / ``gradient_norm``: the norm of all gradients together, and
+  their scaling to a limit.
 
 Every call queues its kernels on torch's current stream of the inputs' device
 and returns without waiting; outputs and scratch come from torch's allocator, so
@@ -19,6 +24,8 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
+import struct
 from typing import Optional, Tuple
 
 from . import _lib as L
@@ -398,3 +405,312 @@ def fp8_block_matmul(a, a_scales, b, b_scales, *, out_dtype=None):
     _call(lib.orda_fp8_block_matmul, a.device.index, _stream(a.device), C.byref(ad), C.byref(bd),
           C.byref(_desc(out, "out")), ws.data_ptr(), ws.numel())
     return out
+
+
+# ------------------------------------------------------------------ root-mean-square norm
+def _rows(x, h: int, what: str):
+    """x [..., h] as a _matrix."""
+    if x.dim() == 2:
+        return _matrix(x, what)
+    return _matrix(x.reshape(-1, h) if h else x.new_empty((math.prod(x.shape[:-1]), 0)), what)
+
+
+def _weight(weight, h: int, device):
+    w = _gpu_tensor(weight, "weight")
+    _same_device(device, weight=w)
+    if w.dim() != 1 or w.size(0) != h:
+        raise OrdaError(f"weight must be [{h}]")
+    return w.contiguous()
+
+
+def _row_desc(w, what: str) -> L.Tensor:
+    """orda_tensor of a contiguous vector as one row."""
+    n = w.size(0)
+    return L.Tensor(w.data_ptr(), 1, n, n, _dtype(w, what), L.DEVICE)
+
+
+def _norm_args(x, weight, residual, eps: float, weight_offset: float):
+    """(orda_rms_norm, x as a matrix, the tensors it points into)."""
+    x = _gpu_tensor(x, "x")
+    if x.dim() < 1:
+        raise OrdaError("x must be [..., H]")
+    h = x.size(-1)
+    w = _weight(weight, h, x.device)
+    m, r = _rows(x, h, "x"), None
+    a = L.RmsNormC(x=_desc(m, "x"), weight=_row_desc(w, "weight"), eps=eps, weight_offset=weight_offset)
+    if residual is not None:
+        r = _gpu_tensor(residual, "residual")
+        _same_device(x.device, residual=r)
+        if r.shape != x.shape or r.dtype != x.dtype:
+            raise OrdaError("residual must have the shape and dtype of x")
+        r = _rows(r, h, "residual")
+        a.residual = _desc(r, "residual")
+    return a, m, (w, r)
+
+
+def rms_norm(x, weight, *, residual=None, eps: float = 1e-6, weight_offset: float = 0.0):
+    """``t / sqrt(mean(t**2) + eps) * (weight + weight_offset)`` over the last dimension
+    of ``t = x + residual`` (``t = x`` without a residual).
+
+    ``x`` and ``residual`` are [..., H], float32 or bfloat16, ``weight`` [H] either of
+    them. ``t`` is rounded to x's type, the mean formed in 64 bits, the result
+    rounded once to x's type. Returns the result, with a residual ``(result, t)``.
+    """
+    torch = _torch()
+    a, m, _keep = _norm_args(x, weight, residual, eps, weight_offset)
+    out = torch.empty(m.shape, dtype=m.dtype, device=m.device)
+    total = torch.empty_like(out) if residual is not None else None
+    _call(L.load().orda_rms_norm_forward, m.device.index, _stream(m.device), C.byref(a),
+          C.byref(_desc(total, "total")) if total is not None else None, C.byref(_desc(out, "out")))
+    if x.dim() != 2:
+        out, total = out.view(x.shape), total.view(x.shape) if total is not None else None
+    return out if total is None else (out, total)
+
+
+def rms_norm_fp8(x, weight, *, residual=None, eps: float = 1e-6, weight_offset: float = 0.0) -> Tuple:
+    """``rms_norm`` with its result in e4m3: ``(codes, scales)``, with a residual
+    ``(codes, scales, t)``. The codes [N, H] of x's N rows and the scales [N, ceil(H / 128)]
+    are those that ``quantize_fp8_blocks`` gives of the result in float32 (which is not
+    rounded to x's type before), laid out as ``fp8_block_matmul`` reads them best."""
+    torch = _torch()
+    a, m, _keep = _norm_args(x, weight, residual, eps, weight_offset)
+    n, h = m.shape
+    pitch, cb = -(-h // 16) * 16, -(-h // 128)
+    codes = torch.empty((n, pitch), dtype=torch.float8_e4m3fn, device=m.device)[:, :h]
+    scales = torch.empty((cb, n), dtype=torch.float32, device=m.device).t()
+    d = L.Fp8MatrixC(codes=codes.data_ptr(), rows=n, cols=h, ld=pitch, scales=scales.data_ptr(), scale_row=1,
+                     scale_col=n, block_rows=1)
+    total = torch.empty(m.shape, dtype=m.dtype, device=m.device) if residual is not None else None
+    _call(L.load().orda_rms_norm_fp8, m.device.index, _stream(m.device), C.byref(a),
+          C.byref(_desc(total, "total")) if total is not None else None, C.byref(d))
+    return (codes, scales) if total is None else (codes, scales, total.view(x.shape))
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_bytes(n: int, h: int) -> int:
+    b = C.c_int64()
+    _call(L.load().orda_rms_norm_backward_workspace, n, h, C.byref(b))
+    return b.value
+
+
+def rms_norm_backward(grad_out, total, weight, *, grad_total=None, eps: float = 1e-6, weight_offset: float = 0.0,
+                      grad_x: bool = True, grad_weight: bool = True) -> Tuple:
+    """``(grad_x, grad_weight)`` of ``rms_norm``, given the gradient into its result, ``total``
+    (``t`` as it returned it; ``x`` where there was no residual) and, where the sum is
+    used beside the norm, the gradient into ``t``. ``grad_x``, in x's type, is also the
+    residual's gradient; ``grad_weight`` is summed over the rows in float32, in an order
+    that the sizes fix, and rounded once to the weight's type. None where not asked for.
+    """
+    torch = _torch()
+    a, t, _keep = _norm_args(total, weight, None, eps, weight_offset)
+    h = t.size(1)
+    grads = []
+    for g, what in ((grad_out, "grad_out"), (grad_total, "grad_total")):
+        if g is None:
+            if what == "grad_out":
+                raise OrdaError("grad_out must be a GPU tensor")
+            grads.append(None)
+            continue
+        g = _gpu_tensor(g, what)
+        _same_device(t.device, **{what: g})
+        if g.shape != total.shape or g.dtype != t.dtype:
+            raise OrdaError(f"{what} must have the shape and dtype of total")
+        grads.append(_rows(g, h, what))
+    g, gt = grads
+    w = _keep[0]
+    gx = torch.empty(t.shape, dtype=t.dtype, device=t.device) if grad_x else None
+    gw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if grad_weight else None
+    b = _norm_bytes(t.size(0), h)
+    ws = _bytes(b, t.device)
+    _call(L.load().orda_rms_norm_backward, t.device.index, _stream(t.device), C.byref(a),
+          C.byref(_desc(g, "grad_out")), C.byref(_desc(gt, "grad_total")) if gt is not None else None,
+          C.byref(_desc(gx, "grad_x")) if gx is not None else None,
+          C.byref(_row_desc(gw, "grad_weight")) if gw is not None else None, ws.data_ptr(), b)
+    return gx.view(total.shape) if gx is not None else None, gw
+
+
+# ------------------------------------------------------------------ gradient norm and clipping
+_GRADIENT = struct.Struct("=QqqqiiQqqqii")   # orda_gradient
+
+
+def _view(g, what: str):
+    """(rows, cols, pitch) of a tensor's memory: one row where it is dense, in
+    whatever order of its dimensions."""
+    n = g.numel()
+    if g.is_contiguous():
+        return 1, n, n
+    at = 1
+    for stride, size in sorted((s, k) for k, s in zip(g.shape, g.stride()) if k > 1):
+        if stride != at:
+            break
+        at *= size
+    else:
+        return 1, n, n
+    if g.dim() == 2 and _matrix(g, what) is g:
+        return g.size(0), g.size(1), g.stride(0)
+    if g.dim() == 2 and _matrix(g.t(), what).data_ptr() == g.data_ptr():
+        return g.size(1), g.size(0), g.stride(1)
+    raise OrdaError(f"{what} must be dense, or a matrix with adjacent columns or rows")
+
+
+def _gradients(grads, out):
+    """(orda_gradient array, their number, device)."""
+    grads = list(grads)
+    if out is None:
+        grads = [g for g in grads if g is not None]
+    else:
+        out = list(out)
+        if len(out) != len(grads):
+            raise OrdaError(f"out must have {len(grads)} tensors")
+    if not grads:
+        raise OrdaError("there are no gradients")
+    buf = bytearray(_GRADIENT.size * len(grads))
+    device = _gpu_tensor(grads[0], "gradient 0").device
+    for i, g in enumerate(grads):
+        what = f"gradient {i}"
+        g = _gpu_tensor(g, what)
+        if g.device != device:
+            raise OrdaError(f"{what} is on {g.device}, not on {device}")
+        r, c, ld = _view(g, what)
+        if out is None:
+            _GRADIENT.pack_into(buf, i * _GRADIENT.size, g.data_ptr(), r, c, ld, _dtype(g, what), L.DEVICE,
+                                0, 0, 0, 0, 0, 0)
+            continue
+        o = _gpu_tensor(out[i], f"out {i}")
+        if o.device != device:
+            raise OrdaError(f"out {i} is on {o.device}, not on {device}")
+        if o.shape != g.shape or (g.stride() != o.stride() and not (g.is_contiguous() and o.is_contiguous())):
+            raise OrdaError(f"out {i} must have the shape and strides of {what}")
+        if o.requires_grad and _torch().is_grad_enabled():
+            raise OrdaError(f"out {i} must not require a gradient")
+        _GRADIENT.pack_into(buf, i * _GRADIENT.size, g.data_ptr(), r, c, ld, _dtype(g, what), L.DEVICE,
+                            o.data_ptr(), r, c, ld, _dtype(o, f"out {i}"), L.DEVICE)
+    return (C.c_char * len(buf)).from_buffer(buf), grads, device
+
+
+def _norm_workspace(lib, a, n: int, device):
+    b = C.c_int64()
+    _call(lib.orda_clip_gradients_workspace, a, n, C.byref(b))
+    return _bytes(b.value, device)
+
+
+def gradient_norm(grads):
+    """The 2-norm of all gradients together, a 0-dim float32 tensor. Gradients are
+    float32 or bfloat16 GPU tensors of any shape, dense in any order or matrices
+    with adjacent columns; None is skipped. Squares and sums are formed in 64 bits."""
+    torch = _torch()
+    a, grads, device = _gradients(grads, None)
+    lib = L.load()
+    ws = _norm_workspace(lib, a, len(grads), device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    _call(lib.orda_gradient_norm, device.index, _stream(device), a, len(grads), norm.data_ptr(), ws.data_ptr(),
+          ws.numel())
+    return norm
+
+
+def clip_gradients(grads, max_norm: float, *, eps: float = 1e-6, out=None):
+    """Scales all gradients by ``min(1, max_norm / (norm + eps))`` and returns their
+    ``gradient_norm`` before that.
+
+    In place, where nothing is written if the factor is 1; or to the tensors of ``out``,
+    of the same shapes and strides, float32 or bfloat16, whatever the factor (the
+    gradients then stay as they are, and none may be None). A norm that is NaN makes
+    all of them NaN. Does not wait for the device. Tensors that are written share no
+    memory with others of the call."""
+    torch = _torch()
+    a, grads, device = _gradients(grads, out)
+    lib = L.load()
+    ws = _norm_workspace(lib, a, len(grads), device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    _call(lib.orda_clip_gradients, device.index, _stream(device), a, len(grads), max_norm, eps, norm.data_ptr(),
+          ws.data_ptr(), ws.numel())
+    for t in grads if out is None else out:
+        torch.autograd.graph.increment_version(t)   # written in place
+    return norm
+
+
+# ------------------------------------------------------------------ drawing tokens
+def _per_row(value, n: int, shape, device, what: str, dtype, none):
+    """(tensor or None, the one value)."""
+    torch = _torch()
+    if value is None:
+        return None, none
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    v = _gpu_tensor(value, what)
+    _same_device(device, **{what: v})
+    if v.shape != shape:
+        raise OrdaError(f"{what} must be a number or of shape {list(shape)}")
+    if dtype == torch.int32:
+        if v.dtype not in (torch.int32, torch.int64):
+            raise OrdaError(f"{what} must be int32 or int64, got {v.dtype}")
+        if v.dtype == torch.int64:
+            v = v.clamp(0, 2 ** 31 - 1).to(torch.int32)
+    elif v.dtype != torch.float32:
+        raise OrdaError(f"{what} must be float32, got {v.dtype}")
+    return v.reshape(-1).contiguous(), none
+
+
+@functools.lru_cache(maxsize=1024)
+def _sample_bytes(n: int, v: int) -> int:
+    b = C.c_int64()
+    _call(L.load().orda_sample_tokens_workspace, n, v, C.byref(b))
+    return b.value
+
+
+def sample_tokens(logits, uniform, *, temperature=1.0, top_k=None, top_p=None, min_p=None) -> Tuple:
+    """One token of each row of ``logits`` [..., V] (float32 or bfloat16) by that row's
+    number of ``uniform`` [...] (float32, in [0, 1)): ``(tokens, logprobs)``, int64 and
+    float32 [...].
+
+    A token's mass is ``exp((x - max) / temperature)``. Of the tokens in descending order
+    (equal logits: the lowest first) are kept the first ``top_k``; of those the ones whose
+    mass before them is below ``top_p`` times the mass of all of those; of those the ones
+    whose mass is at least ``min_p`` times the largest; the first always. The token is the
+    first in the vocabulary's order up to which the kept masses add to more than
+    ``uniform`` times their sum, its log-probability that of its share of the sum.
+    ``temperature`` 0 gives the largest logit, the lowest such token, with log-probability
+    0. Masses and sums are formed in 64 bits.
+
+    Each parameter is a number, or a tensor [...] with a row's own (float32, ``top_k``
+    int32 or int64); ``None`` and ``top_k <= 0`` filter nothing. A row with a NaN, without
+    a logit over -infinity, or with a parameter of a tensor that is out of range
+    (temperature negative or not finite, ``top_p`` or ``min_p`` NaN, ``uniform`` outside
+    [0, 1]) gets token -1 and log-probability NaN.
+    """
+    torch = _torch()
+    x = _gpu_tensor(logits, "logits")
+    if x.dim() < 1:
+        raise OrdaError("logits must be [..., V]")
+    shape, v = x.shape[:-1], x.size(-1)
+    if v < 1:
+        raise OrdaError("logits must have columns")
+    m = _rows(x, v, "logits")
+    n = m.size(0)
+    u = _gpu_tensor(uniform, "uniform")
+    _same_device(m.device, uniform=u)
+    if u.dtype != torch.float32 or u.shape != shape:
+        raise OrdaError(f"uniform must be float32 {list(shape)}")
+    u = u.reshape(-1).contiguous()
+    d = m.device
+    t, t1 = _per_row(temperature, n, shape, d, "temperature", torch.float32, 1.0)
+    k, k1 = _per_row(top_k, n, shape, d, "top_k", torch.int32, 0)
+    p, p1 = _per_row(top_p, n, shape, d, "top_p", torch.float32, 1.0)
+    q, q1 = _per_row(min_p, n, shape, d, "min_p", torch.float32, 0.0)
+    a = L.SamplingC(logits=_desc(m, "logits"), uniform=u.data_ptr(), temperature=t1, top_p=p1, min_p=q1,
+                    top_k=max(0, min(int(k1), 2 ** 31 - 1)))
+    if t is not None:
+        a.temperatures = t.data_ptr()
+    if k is not None:
+        a.top_ks = k.data_ptr()
+    if p is not None:
+        a.top_ps = p.data_ptr()
+    if q is not None:
+        a.min_ps = q.data_ptr()
+    b = _sample_bytes(n, v)
+    ws = _bytes(b, d)
+    tokens = torch.empty(shape, dtype=torch.int64, device=d)
+    logprobs = torch.empty(shape, dtype=torch.float32, device=d)
+    _call(L.load().orda_sample_tokens, d.index, _stream(d), C.byref(a), tokens.data_ptr(), logprobs.data_ptr(),
+          ws.data_ptr(), b)
+    return tokens, logprobs
