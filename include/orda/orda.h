@@ -484,7 +484,7 @@ int32_t orda_clip_gradients(int32_t device, void *hip_stream, const orda_gradien
 
 /* ---- drawing tokens ------------------------------------------------------------ */
 /* One token of each row of logits x [N,V], fp32 or bf16, by the row's number u in
- * [0,1). With temperature T > 0 a token's mass is e^((x - max)/T), 0 under e^-700. Of
+ * [0,1). With temperature T > 0 a token's mass is e^((x - max)/T), 0 under e^-690. Of
  * the tokens in descending order of logits (equal ones: the lowest first) are kept
  *   top_k: the first k (k <= 0: all),
  *   top_p: of those, the ones whose mass before them is below p times the mass of

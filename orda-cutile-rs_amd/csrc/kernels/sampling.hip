@@ -27,33 +27,50 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// e^z of z <= 0, 0 below e^-700: z = n·ln 2 + y, and e^y by its series (|y| <= ln 2 / 2:
-// the first term left out is 6e-15).
-__device__ __forceinline__ double exp_of(double z) {
-  const double n = rint(z * 1.4426950408889634074);
-  double y = fma(n, -0.69314718055994528623, z);
-  y = fma(n, -2.3190468138462995584e-17, y);
-  double p = 1. / 39916800.;
-  p = fma(p, y, 1. / 3628800.);
-  p = fma(p, y, 1. / 362880.);
-  p = fma(p, y, 1. / 40320.);
-  p = fma(p, y, 1. / 5040.);
-  p = fma(p, y, 1. / 720.);
-  p = fma(p, y, 1. / 120.);
-  p = fma(p, y, 1. / 24.);
-  p = fma(p, y, 1. / 6.);
-  p = fma(p, y, .5);
-  p = fma(p, y, 1.);
-  p = fma(p, y, 1.);
-  const int e = static_cast<int>(n);
-  const double r = __hiloint2double(__double2hiint(p) + e * (1 << 20), __double2loint(p));
-  return z > -700. ? r : 0.;   // (and where z is NaN)
+// e^z of z <= 0 in 64 bits: z·32/ln 2 = 32·n + j + f, |f| <= 1/2, and e^z = 2^n · 2^(j/32)
+// · e^(f ln 2/32), the last by its series (the first term left out is 1.2e-12), 2^(j/32)
+// from a table in LDS whose 64 words lie in 64 banks. 15 vector instructions and a read
+// of LDS; without a table the series takes eight terms more.
+__device__ const double kPowers[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
+struct Exp {
+  const double* powers;   // kPowers, in LDS
+  double top, scale;      // of e^((x - top) / t): scale = 32 / (t ln 2)
+  // (Next to nothing, not 0, below e^-690.)
+  __device__ __forceinline__ double rough(float x) const {
+    constexpr double kMagic = 6755399441055744., y = 0.021660849392498290084;   // 1.5 · 2^52; ln 2 / 32
+    const double t = fmax((static_cast<double>(x) - top) * scale, -32000.);
+    const double d = t + kMagic;   // its low word is round(t)
+    const double f = t - (d - kMagic);
+    double p = fma(f, y * y * y * y / 24., y * y * y / 6.);
+    p = fma(p, f, y * y / 2.);
+    p = fma(p, f, y);
+    p = fma(p, f, 1.);
+    const int k = __double2loint(d);
+    p *= powers[k & 31];
+    return __hiloint2double(__double2hiint(p) + (k >> 5) * (1 << 20), __double2loint(p));
+  }
+  // 0 below e^-690 (and of -infinity).
+  __device__ __forceinline__ double operator()(float x) const {
+    return (static_cast<double>(x) - top) * scale > -690. * 46.166241308446828384 ? rough(x) : 0.;
+  }
+};
+__device__ __forceinline__ void load_powers(double* powers) {
+  if (threadIdx.x < 32) powers[threadIdx.x] = kPowers[threadIdx.x];
 }
 
 struct Row {
   float t, p, m, u;
   int64_t k;
-  double inv_t;
+  double scale;      // 32 / (t ln 2)
   bool bad, first;   // first: only the largest logit is kept
 };
 __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
@@ -66,7 +83,7 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
   r.bad = !(r.t >= 0.f) || r.t == INFINITY || r.p != r.p || r.m != r.m || !(r.u >= 0.f && r.u <= 1.f);
   if (r.k <= 0 || r.k >= a.v) r.k = 0;
   r.first = r.t == 0.f || r.k == 1 || r.p <= 0.f || r.m > 1.f;
-  r.inv_t = 1. / static_cast<double>(r.t);
+  r.scale = 46.166241308446828384 / static_cast<double>(r.t);
   return r;
 }
 // Whether the masses of all tokens are needed.
@@ -111,52 +128,71 @@ struct Tokens {
 };
 
 // ---------------------------------------------------------------- first pass
-// A wave a group: the largest keys of its 64s and of all of it, and where they are
-// needed its masses' sum, relative to its largest.
+// The largest of each 64 and of each 1024 tokens, as keys, and where they are needed
+// the sum of each 1024's masses, relative to its largest: one read of the logits.
+__device__ __forceinline__ float max3(float a, float b, float c) {   // (a NaN is looked for apart)
+  float m;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
+  return m;
+}
 template <typename E>
 __global__ __launch_bounds__(256) void sample_groups_kernel(SampleArgs a) {
   using T = Tokens<E>;
-  const int64_t id = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
+  __shared__ double powers[32];
+  load_powers(powers);
+  __syncthreads();
+  const int64_t row = blockIdx.y, group = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  if (id >= a.n * a.n1024) return;
-  const int64_t row = id / a.n1024, group = id - row * a.n1024;
+  if (group >= a.n1024) return;
   T t;
   t.load(static_cast<const E*>(a.x) + row * a.ldx, group, a.v);
   constexpr int kLanes = 64 / T::kPer;   // that hold 64 neighbouring tokens
-  uint32_t top = 0;
+  float top = -INFINITY;
+  bool nan = false;
 #pragma unroll
   for (int i = 0; i < T::kLoads; ++i) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int k = 0; k < T::kPer; ++k) {
-      const uint32_t key = key_of(t.x[i * T::kPer + k]);
-      m = key > m ? key : m;
+    const float* y = t.x + i * T::kPer;
+    float m = max3(y[0], y[1], y[2]);
+    bool bad = __builtin_isunordered(y[0], y[1]) || __builtin_isunordered(y[2], y[3]);
+    if constexpr (T::kPer == 8) {
+      m = max3(max3(m, y[3], y[4]), y[5], max3(y[6], y[7], y[7]));
+      bad = bad || __builtin_isunordered(y[4], y[5]) || __builtin_isunordered(y[6], y[7]);
+    } else {
+      m = max3(m, y[3], y[3]);
     }
+    uint32_t key = bad ? kNan : key_of(m);
 #pragma unroll
     for (int d = 1; d < kLanes; d *= 2) {
-      const uint32_t o = __shfl_xor(m, d);
-      m = o > m ? o : m;
+      const uint32_t o = __shfl_xor(key, d);
+      key = o > key ? o : key;
     }
     const int64_t at = group * (kGroup / 64) + i * T::kPer + lane / kLanes;
-    if (lane % kLanes == 0 && at < a.n64) a.tops[row * a.n64 + at] = m;
-    top = m > top ? m : top;
+    if (lane % kLanes == 0 && at < a.n64) a.tops[row * a.n64 + at] = key;
+    nan = nan || key == kNan;
+    top = max3(top, value_of(key), top);
   }
+  uint32_t key = nan ? kNan : key_of(top);
 #pragma unroll
   for (int d = kLanes; d < 64; d *= 2) {
-    const uint32_t o = __shfl_xor(top, d);
-    top = o > top ? o : top;
+    const uint32_t o = __shfl_xor(key, d);
+    key = o > key ? o : key;
   }
-  if (lane == 0) a.firsts[row * a.n1024 + group] = top;
+  if (lane == 0) a.firsts[row * a.n1024 + group] = key;
   const Row r = row_of(a, row);
   if (!whole(r)) return;
   double mass = 0.;
-  if (top >= kInf) {
+  if (key >= kInf) {
 #pragma unroll
     for (int k = 0; k < 16; ++k) mass += t.x[k] == INFINITY ? 1. : 0.;
-  } else if (top > kNone) {
-    const double most = static_cast<double>(value_of(top));
+  } else if (key > kNone) {
+    const Exp e{powers, static_cast<double>(value_of(key)), r.scale};
+    double part = 0.;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) mass += exp_of((static_cast<double>(t.x[k]) - most) * r.inv_t);
+    for (int k = 0; k < 16; k += 2) {
+      mass += e.rough(t.x[k]);
+      part += e.rough(t.x[k + 1]);
+    }
+    mass += part;
   }
   mass = wave_sum(mass);
   if (lane == 0) a.masses[row * a.n1024 + group] = mass;
@@ -165,22 +201,36 @@ __global__ __launch_bounds__(256) void sample_groups_kernel(SampleArgs a) {
 // ---------------------------------------------------------------- picking
 struct Shared {
   uint64_t list[kList];        // candidates, key over the token's complement
-  uint64_t mass[kBins];        // fixed point
+  uint64_t mass[kBins];        // of bins, in fixed point; or of groups
   uint32_t count[2 * kBins];   // of bins; or the 64s that hold candidates
   double group[kGroup];
-  double waves[kWaves];
-  uint64_t waves64[kWaves];
-  uint32_t n;
-  uint32_t found;
-  double before;
+  double powers[32];
+  uint64_t waves[2][kWaves];
+  uint32_t n, found;
+  double value;
 };
 
 __device__ __forceinline__ uint64_t order_of(float x, int64_t c) {
   return static_cast<uint64_t>(key_of(x)) << 32 | static_cast<uint32_t>(~static_cast<uint32_t>(c));
 }
+__device__ __forceinline__ int64_t token_of(uint32_t low) { return static_cast<int64_t>(static_cast<uint32_t>(~low)); }
 
+// A mass of at most 1 in fixed point, added in any order the same: 2^20 of them fit
+// in 64 bits. (The sum's mantissa holds it: 512 has 2^-43 as its last bit.)
+constexpr double kFixed = 8796093022208.;
+__device__ __forceinline__ unsigned long long fixed_of(double w) {
+  return static_cast<unsigned long long>(__double_as_longlong(w + 512.)) & ((1ull << 52) - 1);
+}
+
+// What one lane writes to LDS is there for the others of its wave.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+// Over the workgroup: the largest.
 template <typename T>
-__device__ __forceinline__ T block_most(T v, T* waves) {   // largest of the block's
+__device__ __forceinline__ T block_most(T v, Shared& s) {
+  T* waves = reinterpret_cast<T*>(s.waves[0]);
 #pragma unroll
   for (int d = 32; d; d /= 2) {
     const T o = __shfl_xor(v, d);
@@ -193,17 +243,24 @@ __device__ __forceinline__ T block_most(T v, T* waves) {   // largest of the blo
   for (int w = 0; w < kWaves; ++w) v = waves[w] > v ? waves[w] : v;
   return v;
 }
-// Sum of the values up to this thread's, and of all.
 template <typename T>
-__device__ __forceinline__ T block_scan(T v, T* waves, T& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ T wave_scan(T v) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const T o = __shfl_up(v, d);
     if (lane >= d) v += o;
   }
+  return v;
+}
+// Sum of the values up to this thread's, and of all.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, Shared& s, T& all) {
+  T* waves = reinterpret_cast<T*>(s.waves[1]);
+  const int wave = threadIdx.x >> 6;
+  v = wave_scan(v);
   __syncthreads();
-  if (lane == 63) waves[wave] = v;
+  if ((threadIdx.x & 63) == 63) waves[wave] = v;
   __syncthreads();
   T before = 0;
   all = 0;
@@ -223,56 +280,58 @@ struct Pick {
   const int64_t row;
   const Row r;
   const E* x;
-  float top;
+  Exp mass_of;
   bool inf;   // the largest is +infinity: those tokens count as 0, the others as -infinity
 
+  __device__ __forceinline__ float top() const { return static_cast<float>(mass_of.top); }
   __device__ __forceinline__ float value(float y) const { return inf ? (y == INFINITY ? 0.f : -INFINITY) : y; }
-  __device__ __forceinline__ float at(int64_t c) const { return value(static_cast<float>(x[c])); }
-  __device__ __forceinline__ double exponent(float y) const { return (static_cast<double>(y) - static_cast<double>(top)) * r.inv_t; }
-  __device__ __forceinline__ double weight(float y) const { return exp_of(exponent(y)); }
+  __device__ __forceinline__ double weight(float y) const { return mass_of(y); }
 
+  __device__ __forceinline__ void none() const {
+    if (threadIdx.x) return;
+    a.token[row] = -1;
+    if (a.logprob) a.logprob[row] = NAN;
+  }
   __device__ __forceinline__ void done(int64_t c, double logp) const {
     a.token[row] = c;
     if (a.logprob) a.logprob[row] = static_cast<float>(logp);
   }
+  __device__ __forceinline__ void done(int64_t c, float y, double mass) const {
+    done(c, (static_cast<double>(y) - mass_of.top) / static_cast<double>(r.t) - log(mass));
+  }
 
-  // Thread t's share of a sum that crosses `target`: the first whose sum up to it is
+  // The thread in whose share a sum crosses `target`: the first whose sum up to it is
   // over the target, the last with a share where none is. Leaves the sum before it in
-  // s.before.
+  // s.value.
   __device__ __forceinline__ int crossing(double share, double upto, double target) {
     uint32_t mine = 0;   // larger: earlier
     if (share > 0.) mine = upto > target ? 0x80000000u | (kThreads - threadIdx.x) : 1u + threadIdx.x;
-    const uint32_t best = block_most(mine, reinterpret_cast<uint32_t*>(s.waves64));
+    const uint32_t best = block_most(mine, s);
     const int t = best & 0x80000000u ? kThreads - static_cast<int>(best & 0x7fffffffu) : best ? static_cast<int>(best) - 1 : 0;
-    if (static_cast<int>(threadIdx.x) == t) s.before = upto - share;
+    if (static_cast<int>(threadIdx.x) == t) s.value = upto - share;
     __syncthreads();
     return t;
   }
 
-  // The token of `group` where the kept masses, `before` those of its groups before,
-  // cross the target.
-  __device__ __forceinline__ void in_group(int64_t group, double before, double target, double mass, uint64_t cut, double least) {
-    const int64_t c = group * kGroup + threadIdx.x;
+  // Where the groups' masses, thread t's group's here, cross u times their sum, the
+  // group's token: of the tokens from `cut` on in descending order, with masses of at
+  // least `least`.
+  __device__ __forceinline__ void by_groups(double mine, uint64_t cut, double least) {
+    double mass, all;
+    const double upto = block_scan(mine, s, mass);
+    const double target = static_cast<double>(r.u) * mass;
+    const int64_t c = crossing(mine, upto, target) * int64_t{kGroup} + threadIdx.x;
+    const double before = s.value;
     float y = -INFINITY;
     double w = 0.;
     if (c < a.v) {
-      y = at(c);
+      y = value(static_cast<float>(x[c]));
       w = weight(y);
       if (order_of(y, c) < cut || w < least) w = 0.;
     }
-    double all;
-    const double upto = before + block_scan(w, s.waves, all);
-    const int t = crossing(w, upto, target);
-    if (static_cast<int>(threadIdx.x) == t) done(c, exponent(y) - log(mass));
-  }
-
-  // Where the groups' masses cross u times their sum.
-  __device__ __forceinline__ void by_groups(double mine, uint64_t cut, double least) {
-    double mass;
-    const double upto = block_scan(mine, s.waves, mass);
-    const double target = static_cast<double>(r.u) * mass;
-    const int g = crossing(mine, upto, target);
-    in_group(g, s.before, target, mass, cut, least);
+    const double sum = before + block_scan(w, s, all);
+    const int t = crossing(w, sum, target);
+    if (static_cast<int>(threadIdx.x) == t) done(c, y, mass);
   }
 
   // The mass of thread t's group, all tokens counted.
@@ -288,13 +347,45 @@ struct Pick {
   __device__ __forceinline__ void largest(uint32_t key) {
     uint32_t mine = 0;
     if (static_cast<int64_t>(threadIdx.x) < a.n1024 && a.firsts[row * a.n1024 + threadIdx.x] == key) mine = kThreads - threadIdx.x;
-    const int64_t group = kThreads - static_cast<int64_t>(block_most(mine, reinterpret_cast<uint32_t*>(s.waves64)));
+    const int64_t group = kThreads - static_cast<int64_t>(block_most(mine, s));
     const int64_t c = group * kGroup + threadIdx.x;
     mine = c < a.v && key_of(static_cast<float>(x[c])) == key ? kThreads - threadIdx.x : 0;
-    const int t = kThreads - static_cast<int>(block_most(mine, reinterpret_cast<uint32_t*>(s.waves64)));
+    const int t = kThreads - static_cast<int>(block_most(mine, s));
     if (static_cast<int>(threadIdx.x) == t) done(c, 0.);
   }
 
+  // ---- few tokens: lists
+  // A key that at least k of the 64s' largest keys reach, and not many more: from their
+  // counts in bins of equal width.
+  __device__ __forceinline__ uint32_t near_top(int64_t k) {
+    const uint32_t* tops = a.tops + row * a.n64;
+    uint32_t most = 0;   // of the complements
+    for (int64_t i = threadIdx.x; i < a.n64; i += kThreads) {
+      const uint32_t key = tops[i];
+      if (key > kNone) most = ~key > most ? ~key : most;
+    }
+    for (int b = threadIdx.x; b < kBins; b += kThreads) s.count[b] = 0;
+    const float high = top(), low = value_of(~block_most(most, s));
+    const float width = static_cast<float>(kBins - 1) / (high - low);   // (none: infinite)
+    auto bin = [&](float y) { return static_cast<uint32_t>(fminf(fmaxf((high - y) * width, 0.f), kBins - 1.f)); };
+    for (int64_t i = threadIdx.x; i < a.n64; i += kThreads) {
+      const uint32_t key = tops[i];
+      if (key > kNone) atomicAdd(&s.count[bin(value_of(key))], 1u);
+    }
+    __syncthreads();
+    const int b = 2 * static_cast<int>(threadIdx.x);
+    const uint32_t c0 = s.count[b], c1 = s.count[b + 1];
+    uint32_t all;
+    const uint32_t upto = block_scan(c0 + c1, s, all);
+    if (threadIdx.x == 0) s.found = kBins - 1;
+    __syncthreads();
+    if (upto >= k && upto - c0 - c1 < k) s.found = upto - c1 >= k ? b : b + 1;
+    __syncthreads();
+    // its lower end, and a little less for the roundings
+    const float end = high - (static_cast<float>(s.found) + 1.f) / width;
+    const float less = end - 1e-6f * (fabsf(high) + fabsf(end));
+    return less > -INFINITY && s.found < kBins - 1 ? key_of(less) : kNone + 1;
+  }
   // The k-th largest of the 64s' largest keys (1 <= k <= n64), 11, 11 and 10 bits at a time.
   __device__ __forceinline__ uint32_t kth_top(int64_t k) {
     const uint32_t* tops = a.tops + row * a.n64;
@@ -312,14 +403,14 @@ struct Pick {
       }
       __syncthreads();
       const int b = kBins - 2 - 2 * static_cast<int>(threadIdx.x);   // bins b + 1, then b
-      const uint64_t hi = s.count[b + 1], lo = s.count[b];
-      uint64_t all;
-      const uint64_t upto = block_scan<uint64_t>(hi + lo, s.waves64, all);
+      const uint32_t hi = s.count[b + 1], lo = s.count[b];
+      uint32_t all;
+      const uint32_t upto = block_scan(hi + lo, s, all);
       if (upto >= rank && upto - hi - lo < rank) {
-        const uint64_t before = upto - hi - lo;
+        const uint32_t before = upto - hi - lo;
         const bool in_hi = before + hi >= rank;
         s.found = static_cast<uint32_t>(in_hi ? b + 1 : b);
-        s.n = static_cast<uint32_t>(rank - (in_hi ? before : before + hi));
+        s.n = rank - (in_hi ? before : before + hi);
       }
       __syncthreads();
       prefix |= s.found << shift;
@@ -369,15 +460,30 @@ struct Pick {
   }
 
   // The list's first n in descending order; how many entries that are with the zeros
-  // after them (a power of two).
+  // after them (a power of two). Distances under 64 go from lane to lane.
   __device__ __forceinline__ uint32_t sort(uint32_t n) {
     uint32_t size = 64;
     while (size < n) size *= 2;
     __syncthreads();
     for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = 0;
     __syncthreads();
-    for (uint32_t run = 2; run <= size; run *= 2) {
-      for (uint32_t d = run / 2; d; d /= 2) {
+    // runs of up to 64, and after each longer distance the ones under 64, in registers
+    auto lanes = [&](uint32_t run_from, uint32_t run_to) {
+      for (uint32_t i = threadIdx.x; i < size; i += kThreads) {
+        uint64_t o = s.list[i];
+        for (uint32_t run = run_from; run <= run_to; run *= 2)
+          for (uint32_t d = run / 2 < 32 ? run / 2 : 32; d; d /= 2) {
+            const uint64_t w = __shfl_xor(o, d);
+            const bool larger = ((i & run) == 0) == ((i & d) == 0);   // keeps the larger of the two
+            o = (o > w) == larger ? o : w;
+          }
+        s.list[i] = o;
+      }
+      __syncthreads();
+    };
+    lanes(2, 64);
+    for (uint32_t run = 128; run <= size; run *= 2) {
+      for (uint32_t d = run / 2; d >= 64; d /= 2) {
         for (uint32_t q = threadIdx.x; q < size / 2; q += kThreads) {
           const uint32_t i = q / d * 2 * d + q % d, j = i + d;
           const uint64_t u = s.list[i], w = s.list[j];
@@ -388,36 +494,89 @@ struct Pick {
         }
         __syncthreads();
       }
+      lanes(run, run);
     }
     return size;
   }
 
-  __device__ __forceinline__ float listed(uint32_t i) const { return value_of(static_cast<uint32_t>(s.list[i] >> 32)); }
+  __device__ __forceinline__ static float listed(uint64_t o) { return value_of(static_cast<uint32_t>(o >> 32)); }
+
+  // Up to 64 candidates by one wave (the others wait): each entry's rank is how many are
+  // over it. The token, or false where the cut is not among them; `share`: of all masses.
+  __device__ __forceinline__ bool from_few(uint32_t n, bool complete, double all_mass, double& share) {
+    if (threadIdx.x < 64) {
+      const uint32_t i = threadIdx.x;
+      uint64_t o = i < n ? s.list[i] : 0;
+      uint32_t rank = 0;
+      for (uint32_t j = 0; j < n; ++j) rank += s.list[j] > o;
+      wave_sync();
+      if (i < n) s.list[rank] = o;
+      wave_sync();
+      const uint32_t most = r.k && r.k < n ? static_cast<uint32_t>(r.k) : n;
+      o = i < most ? s.list[i] : 0;
+      const double w = i < most ? weight(listed(o)) : 0.;
+      const double upto = wave_scan(w), all = __shfl(upto, 63);
+      const double limit = r.p < 1.f ? static_cast<double>(r.p) * (r.k ? all : all_mass) : INFINITY;
+      const bool keep = i < most && (i == 0 || (upto - w < limit && w >= static_cast<double>(r.m)));
+      const uint32_t count = static_cast<uint32_t>(__popcll(__ballot(keep)));
+      const bool found = r.k || complete || count < n;
+      if (found) {
+        // in the order of the vocabulary
+        if (keep) s.list[i] = o << 32 | o >> 32;
+        wave_sync();
+        const uint64_t mine = keep ? s.list[i] : 0;
+        uint32_t place = 0;
+        for (uint32_t j = 0; j < count; ++j) place += s.list[j] > mine;
+        wave_sync();
+        if (keep) s.list[place] = mine;
+        wave_sync();
+        const uint64_t e = i < count ? s.list[i] : 0;
+        const float y = value_of(static_cast<uint32_t>(e));
+        const double m = i < count ? weight(y) : 0.;
+        const double sum = wave_scan(m), mass = __shfl(sum, 63);
+        const double target = static_cast<double>(r.u) * mass;
+        const uint64_t over = __ballot(m > 0. && sum > target), any = __ballot(m > 0.);
+        const int t = over ? __ffsll(static_cast<unsigned long long>(over)) - 1 : 63 - __clzll(static_cast<long long>(any));
+        if (static_cast<int>(i) == t) done(token_of(static_cast<uint32_t>(e >> 32)), y, mass);
+      }
+      if (i == 0) {
+        s.found = found;
+        s.value = all;
+      }
+    }
+    __syncthreads();
+    share = s.value / all_mass;
+    const bool found = s.found;
+    __syncthreads();
+    return found;
+  }
 
   // From the tokens whose keys are at least `least`, where they are few enough and
   // known to hold all that are kept (`complete`, or the cut is among them).
-  __device__ __forceinline__ bool from_list(uint32_t least, bool complete, double all_mass) {
+  __device__ __forceinline__ bool from_list(uint32_t least, bool complete, double all_mass, double& share) {
+    share = 1.;
     const uint32_t n = candidates(least);
     if (n > kList) return false;
+    if (n <= 64) return from_few(n, complete, all_mass, share);
     const uint32_t size = sort(n), per = size > kThreads ? size / kThreads : 1, i0 = threadIdx.x * per;
-    const uint32_t most = r.k ? static_cast<uint32_t>(r.k) : n;
+    const uint32_t most = r.k && r.k < n ? static_cast<uint32_t>(r.k) : n;
     double w[kList / kThreads], mine = 0., all;
 #pragma unroll
     for (uint32_t q = 0; q < kList / kThreads; ++q) {
-      w[q] = q < per && i0 + q < n && i0 + q < most ? weight(listed(i0 + q)) : 0.;
+      w[q] = q < per && i0 + q < most ? weight(listed(s.list[i0 + q])) : 0.;
       mine += w[q];
     }
-    const double upto = block_scan(mine, s.waves, all);
+    double before = block_scan(mine, s, all) - mine;
     const double limit = r.p < 1.f ? static_cast<double>(r.p) * (r.k ? all : all_mass) : INFINITY;
-    double before = upto - mine;
     uint32_t kept = 0;
 #pragma unroll
     for (uint32_t q = 0; q < kList / kThreads; ++q) {
       const uint32_t i = i0 + q;
-      if (q < per && i < n && i < most && (i == 0 || (before < limit && w[q] >= static_cast<double>(r.m)))) kept = i + 1;
+      if (q < per && i < most && (i == 0 || (before < limit && w[q] >= static_cast<double>(r.m)))) kept = i + 1;
       before += w[q];
     }
-    const uint32_t count = block_most(kept, reinterpret_cast<uint32_t*>(s.waves64));
+    const uint32_t count = block_most(kept, s);
+    share = all / all_mass;
     if (!r.k && !complete && count == n) return false;
     // the kept ones in the order of the vocabulary
     __syncthreads();
@@ -429,91 +588,126 @@ struct Pick {
       w[q] = q < per2 && j0 + q < count ? weight(value_of(static_cast<uint32_t>(s.list[j0 + q]))) : 0.;
       mine += w[q];
     }
-    const double upto2 = block_scan(mine, s.waves, all);
+    const double upto = block_scan(mine, s, all);
     const double target = static_cast<double>(r.u) * all;
-    const int t = crossing(mine, upto2, target);
+    const int t = crossing(mine, upto, target);
     if (static_cast<int>(threadIdx.x) == t) {
-      double sum = upto2 - mine;
+      double sum = upto - mine;
       uint32_t pick = j0;
 #pragma unroll
       for (uint32_t q = 0; q < kList / kThreads; ++q) {
-        if (q < per2 && j0 + q < count && w[q] > 0.) {
+        if (w[q] > 0.) {
           if (!(sum > target)) pick = j0 + q;
           sum += w[q];
         }
       }
       const uint64_t e = s.list[pick];
-      done(static_cast<int64_t>(static_cast<uint32_t>(~static_cast<uint32_t>(e >> 32))),
-           exponent(value_of(static_cast<uint32_t>(e))) - log(all));
+      done(token_of(static_cast<uint32_t>(e >> 32)), value_of(static_cast<uint32_t>(e)), all);
     }
     return true;
   }
 
-  // ---- rows whose kept tokens are many: selection over the whole row
-  template <typename F>
-  __device__ __forceinline__ void each(F&& f) const {
-    for (int64_t c = threadIdx.x; c < (a.v + kThreads - 1) / kThreads * kThreads; c += kThreads)
-      f(c, c < a.v ? at(c) : -INFINITY);
+  // ---- many tokens: selection over the whole row
+  // f(token, value) of every token, a wave a group; ended(group) after each.
+  template <typename F, typename G>
+  __device__ __forceinline__ void each(F&& f, G&& ended) const {
+    for (int64_t g = threadIdx.x >> 6; g < a.n1024; g += kWaves) {
+      Tokens<E> t;
+      t.load(x, g, a.v);
+#pragma unroll
+      for (int i = 0; i < Tokens<E>::kLoads; ++i)
+#pragma unroll
+        for (int k = 0; k < Tokens<E>::kPer; ++k)
+          f(Tokens<E>::column(g, i) + k, value(t.x[i * Tokens<E>::kPer + k]));
+      ended(g);
+    }
   }
 
-  // Of the tokens from `cut` on in descending order, the last one kept: the k-th (`by`
-  // k), or the first up to which the masses add to `goal` (k 0). `mass`: of the tokens
-  // up to it.
-  __device__ __forceinline__ uint64_t select(uint64_t cut, int64_t k, double goal, double& mass) {
-    // Bins of equal width below the largest value; where one of them holds too many
-    // tokens, bins of equal width of its keys.
-    const float width = fminf(static_cast<float>(kBins) / 24.f * static_cast<float>(r.inv_t), 1e30f);
+  // The groups' masses of the tokens from `cut` on, those of at least `least`.
+  __device__ __forceinline__ void group_masses(uint64_t cut, double least) {
+    double sum = 0.;
+    __syncthreads();
+    each([&](int64_t c, float y) {
+      const double w = weight(y);
+      if (order_of(y, c) >= cut && w >= least) sum += w;
+    }, [&](int64_t g) {
+      sum = wave_sum(sum);
+      if ((threadIdx.x & 63) == 0) s.group[g] = sum;
+      sum = 0.;
+    });
+    __syncthreads();
+  }
+
+  // Of the tokens from `cut` on in descending order the last one kept: the k-th (COUNT),
+  // or the first up to which the masses add to `goal`. With `last` leaves the kept
+  // tokens' masses of at least `least` in s.group and, those that stood in the list,
+  // in s.mass; else returns all kept tokens' mass in `mass`.
+  //
+  // A pass counts or weighs the tokens in bins of equal width below the largest; the
+  // bin that the cut is in goes to a list in the next, which also adds up what lies
+  // above it, and the list is sorted. Where it is too long its keys are cut into bins
+  // again.
+  template <bool COUNT>
+  __device__ __forceinline__ uint64_t select(uint64_t cut, bool cut_is, int64_t k, double goal, bool last, double least, double& mass) {
+    // 24 units of e^x hold all masses that count; by ranks, what the 64s' largest span.
+    float span = 24.f * r.t;
+    if constexpr (COUNT) {
+      uint32_t most = 0;
+      for (int64_t i = threadIdx.x; i < a.n64; i += kThreads) {
+        const uint32_t key = a.tops[row * a.n64 + i];
+        if (key > kNone) most = ~key > most ? ~key : most;
+      }
+      const float low = value_of(~block_most(most, s));
+      if (!inf) span = (top() - low) * 1.25f;
+    }
+    const float high = top(), width = fminf(static_cast<float>(kBins) / span, 1e30f);
     uint32_t first = 0, lo = 0, hi = 0;
     int level = 0, shift = 0;
     double above = 0.;
-    int64_t n_above = 0;
-    // weights in fixed point, at most 2^42 each: added in any order they are the same
-    constexpr double kOne = 4398046511104.;
-    auto bin0 = [&](float y) { return static_cast<uint32_t>(fminf((top - y) * width, static_cast<float>(kBins - 1))); };
-    auto member = [&](int64_t c, float y) {
-      return y > -INFINITY && order_of(y, c) >= cut && (level == 0 || (bin0(y) == first && key_of(y) >= lo && key_of(y) <= hi));
-    };
+    uint32_t n_above = 0, n;
+    auto bin0 = [&](float y) { return static_cast<uint32_t>(fminf((high - y) * width, kBins - 1.f)); };
+    auto eligible = [&](int64_t c, float y) { return y > -INFINITY && (!cut_is || order_of(y, c) >= cut); };
     while (true) {
       __syncthreads();
       for (int b = threadIdx.x; b < kBins; b += kThreads) {
-        s.count[b] = 0;
-        s.mass[b] = 0;
+        if constexpr (COUNT) s.count[b] = 0;
+        else s.mass[b] = 0;
       }
       __syncthreads();
       each([&](int64_t c, float y) {
-        if (!member(c, y)) return;
-        const uint32_t b = level == 0 ? bin0(y) : (hi - key_of(y)) >> shift;
-        atomicAdd(&s.count[b], 1u);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]),
-                  static_cast<unsigned long long>(weight(y) * kOne + .5));
-      });
+        if (!eligible(c, y)) return;
+        uint32_t b = bin0(y);
+        if (level) {
+          const uint32_t key = key_of(y);
+          if (b != first || key < lo || key > hi) return;
+          b = (hi - key) >> shift;
+        }
+        if constexpr (COUNT) atomicAdd(&s.count[b], 1u);
+        else atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), fixed_of(mass_of.rough(y)));
+      }, [](int64_t) {});
       __syncthreads();
-      const int b = 2 * static_cast<int>(threadIdx.x);
-      const uint64_t c0 = s.count[b], c1 = s.count[b + 1], m0 = s.mass[b], m1 = s.mass[b + 1];
-      uint64_t n_all, m_all;
-      const uint64_t n_upto = block_scan<uint64_t>(c0 + c1, s.waves64, n_all);
-      const uint64_t m_upto = block_scan<uint64_t>(m0 + m1, s.waves64, m_all);
-      auto reached = [&](uint64_t n, uint64_t m) {
-        return k ? n_above + static_cast<int64_t>(n) >= k : above + static_cast<double>(m) / kOne >= goal;
-      };
       // the first bin that reaches it, or else the last one with tokens
+      const int b = 2 * static_cast<int>(threadIdx.x);
+      uint64_t v0, v1;
+      if constexpr (COUNT) v0 = s.count[b], v1 = s.count[b + 1];
+      else v0 = s.mass[b], v1 = s.mass[b + 1];
+      uint64_t all;
+      const uint64_t upto = block_scan<uint64_t>(v0 + v1, s, all);
+      auto reached = [&](uint64_t q) {
+        if constexpr (COUNT) return n_above + static_cast<int64_t>(q) >= k;
+        else return above + static_cast<double>(q) / kFixed >= goal;
+      };
       uint32_t mine = 0;
-      if (c0 && reached(n_upto - c1, m_upto - m1)) mine = 0x80000000u | (kBins - b);
-      else if (c1 && reached(n_upto, m_upto)) mine = 0x80000000u | (kBins - b - 1);
-      else if (c1) mine = 2u + b;
-      else if (c0) mine = 1u + b;
-      const uint32_t best = block_most(mine, reinterpret_cast<uint32_t*>(s.waves));
-      const uint32_t bin = best & 0x80000000u ? kBins - (best & 0x7fffffffu) : best - 1;
-      if (bin / 2 == threadIdx.x) {
-        const bool odd = bin & 1;
-        s.waves64[0] = n_upto - c1 - (odd ? 0 : c0);
-        s.waves64[1] = m_upto - m1 - (odd ? 0 : m0);
-      }
+      if (v0 && reached(upto - v1)) mine = 0x80000000u | (kBins - b);
+      else if (v1 && reached(upto)) mine = 0x80000000u | (kBins - b - 1);
+      else if (v1) mine = 2u + b;
+      else if (v0) mine = 1u + b;
+      const uint32_t best = block_most(mine, s);
+      const uint32_t bin = best & 0x80000000u ? kBins - (best & 0x7fffffffu) : best ? best - 1 : 0;
+      if (bin / 2 == threadIdx.x) s.list[0] = upto - v1 - (bin & 1 ? 0 : v0);
       __syncthreads();
-      n_above += static_cast<int64_t>(s.waves64[0]);
-      above += static_cast<double>(s.waves64[1]) / kOne;
-      const uint32_t here = s.count[bin];
-      __syncthreads();
+      if constexpr (COUNT) n_above += static_cast<uint32_t>(s.list[0]);
+      else above += static_cast<double>(s.list[0]) / kFixed;
       if (level == 0) {
         first = bin;
         lo = 0;
@@ -524,109 +718,139 @@ struct Pick {
         hi = h;
       }
       ++level;
-      if (here <= kList) break;
-      // the members' own range of keys
-      uint32_t least = kNan, most = 0;
+      // the bin's tokens, the range of their keys, and the masses above them
+      __syncthreads();
+      if (threadIdx.x == 0) s.n = 0;
+      __syncthreads();
+      uint32_t low = kNan, most = 0;
+      double sum = 0.;
       each([&](int64_t c, float y) {
-        if (!member(c, y)) return;
-        const uint32_t key = key_of(y);
-        least = key < least ? key : least;
-        most = key > most ? key : most;
+        const bool is = eligible(c, y);
+        const uint32_t b = is ? bin0(y) : kBins, key = key_of(y);
+        const bool member = b == first && key >= lo && key <= hi;
+        if (b < first || (b == first && key > hi)) {
+          const double w = weight(y);
+          if (w >= least) sum += w;
+        }
+        if (member) {
+          low = key < low ? key : low;
+          most = key > most ? key : most;
+        }
+        append(member, order_of(y, c));
+      }, [&](int64_t g) {
+        sum = wave_sum(sum);
+        if ((threadIdx.x & 63) == 0) s.group[g] = sum;
+        sum = 0.;
       });
-      hi = block_most(most, reinterpret_cast<uint32_t*>(s.waves));
-      lo = ~block_most(~least, reinterpret_cast<uint32_t*>(s.waves));
+      __syncthreads();
+      n = s.n;
+      if (n <= kList) break;
+      hi = block_most(most, s);
+      lo = ~block_most(~low, s);
       if (lo == hi) {   // more equal values than the list holds
         const double w = weight(value_of(hi));
-        int64_t want = k ? k - n_above : static_cast<int64_t>(fmin(ceil((goal - above) / w), static_cast<double>(here)));
-        want = want < 1 ? 1 : want > here ? here : want;
-        mass = above + static_cast<double>(want) * w;
+        int64_t want;
+        if constexpr (COUNT) want = k - n_above;
+        else want = static_cast<int64_t>(fmin(ceil((goal - above) / w), static_cast<double>(n)));
+        want = want < 1 ? 1 : want > n ? n : want;
         // the want-th of them
         uint64_t seen = 0, o = 0;
-        for (int64_t c0 = 0; c0 < a.v; c0 += kThreads) {
+        for (int64_t c0 = 0; c0 < a.v && static_cast<int64_t>(seen) < want; c0 += kThreads) {
           const int64_t c = c0 + threadIdx.x;
-          const float y = c < a.v ? at(c) : -INFINITY;
-          const bool is = c < a.v && key_of(y) == hi && member(c, y);
-          uint64_t all;
-          const uint64_t upto = seen + block_scan<uint64_t>(is ? 1 : 0, s.waves64, all);
-          if (is && static_cast<int64_t>(upto) == want) o = order_of(y, c);
-          seen += all;
-          if (static_cast<int64_t>(seen) >= want) break;
+          const float y = c < a.v ? value(static_cast<float>(x[c])) : -INFINITY;
+          const bool is = c < a.v && key_of(y) == hi && eligible(c, y);
+          uint64_t here;
+          const uint64_t at = seen + block_scan<uint64_t>(is ? 1 : 0, s, here);
+          if (is && static_cast<int64_t>(at) == want) o = order_of(y, c);
+          seen += here;
         }
-        return block_most(o, s.waves64);
+        o = block_most(o, s);
+        if (last) {
+          group_masses(o, least);
+          for (int g = threadIdx.x; g < kGroup; g += kThreads) s.mass[g] = 0;
+          __syncthreads();
+        } else {
+          block_scan(static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0., s, mass);
+          mass += static_cast<double>(want) * w;
+        }
+        return o;
       }
       shift = 0;
       while ((hi - lo) >> shift >= kBins) ++shift;
     }
-    if (threadIdx.x == 0) s.n = 0;
-    __syncthreads();
-    each([&](int64_t c, float y) { append(member(c, y), order_of(y, c)); });
-    __syncthreads();
-    const uint32_t n = s.n, size = sort(n), per = size > kThreads ? size / kThreads : 1, i0 = threadIdx.x * per;
+    const uint32_t size = sort(n), per = size > kThreads ? size / kThreads : 1, i0 = threadIdx.x * per;
     double w[kList / kThreads], mine = 0., all;
 #pragma unroll
     for (uint32_t q = 0; q < kList / kThreads; ++q) {
-      w[q] = q < per && i0 + q < n ? weight(listed(i0 + q)) : 0.;
+      w[q] = q < per && i0 + q < n ? weight(listed(s.list[i0 + q])) : 0.;
       mine += w[q];
     }
-    double sum = above + block_scan(mine, s.waves, all) - mine;
+    const double before = block_scan(mine, s, all) - mine;
+    double sum = before;
     uint32_t best = 0;   // larger: earlier
-    double through = 0.;
 #pragma unroll
     for (uint32_t q = 0; q < kList / kThreads; ++q) {
       const uint32_t i = i0 + q;
       sum += w[q];
       if (q < per && i < n && !(best & 0x80000000u)) {
-        const bool is = k ? n_above + i + 1 >= k : sum >= goal;
+        bool is;
+        if constexpr (COUNT) is = n_above + i + 1 >= k;
+        else is = above + sum >= goal;
         best = is ? 0x80000000u | (kList - i) : 1u + i;
-        through = sum;
       }
     }
-    const uint32_t found = block_most(best, reinterpret_cast<uint32_t*>(s.waves64));
-    const uint32_t i = found & 0x80000000u ? kList - (found & 0x7fffffffu) : found - 1;
-    if (best == found) s.before = through;
-    __syncthreads();
-    mass = s.before;
-    const uint64_t o = s.list[i];
-    __syncthreads();
+    const uint32_t found = block_most(best, s);
+    const uint32_t end = found & 0x80000000u ? kList - (found & 0x7fffffffu) : found ? found - 1 : 0;
+    const uint64_t o = s.list[end];
+    if (last) {
+      for (int g = threadIdx.x; g < kGroup; g += kThreads) s.mass[g] = 0;
+      __syncthreads();
+#pragma unroll
+      for (uint32_t q = 0; q < kList / kThreads; ++q)
+        if (q < per && i0 + q <= end && w[q] >= least)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[token_of(static_cast<uint32_t>(s.list[i0 + q])) / kGroup]),
+                    fixed_of(w[q]));
+      __syncthreads();
+    } else {
+      double through = 0.;
+      sum = before;
+#pragma unroll
+      for (uint32_t q = 0; q < kList / kThreads; ++q) {
+        sum += w[q];
+        if (q < per && i0 + q == end) through = sum;
+      }
+      through = block_most(through, s);
+      block_scan(static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0., s, mass);
+      mass += through;
+    }
     return o;
   }
 
   __device__ __forceinline__ void general(double all_mass) {
-    uint64_t cut = static_cast<uint64_t>(kNone + 1) << 32;
-    double mass = all_mass;
-    if (r.k) cut = select(cut, r.k, 0., mass);
-    if (r.p < 1.f) {
-      double through;
-      cut = select(cut, 0, static_cast<double>(r.p) * mass, through);
-    }
     const double least = static_cast<double>(r.m);
-    // the kept masses of the groups, a wave a group
-    __syncthreads();
-    for (int64_t g = threadIdx.x >> 6; g < a.n1024; g += kWaves) {
-      Tokens<E> t;
-      t.load(x, g, a.v);
-      double sum = 0.;
-#pragma unroll
-      for (int i = 0; i < Tokens<E>::kLoads; ++i)
-#pragma unroll
-        for (int k = 0; k < Tokens<E>::kPer; ++k) {
-          const float y = value(t.x[i * Tokens<E>::kPer + k]);
-          const double w = weight(y);
-          if (order_of(y, Tokens<E>::column(g, i) + k) >= cut && w >= least) sum += w;
-        }
-      sum = wave_sum(sum);
-      if ((threadIdx.x & 63) == 0) s.group[g] = sum;
+    uint64_t cut = static_cast<uint64_t>(kNone + 1) << 32;
+    if (r.k && r.p < 1.f) cut = select<true>(cut, false, r.k, 0., false, 0., all_mass);
+    if (r.p < 1.f) {
+      double unused;
+      cut = select<false>(cut, r.k != 0, 0, static_cast<double>(r.p) * all_mass, true, least, unused);
+    } else if (r.k) {
+      double unused;
+      cut = select<true>(cut, false, r.k, 0., true, least, unused);
+    } else {
+      group_masses(cut, least);
     }
-    __syncthreads();
-    by_groups(static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0., cut, least);
+    double mine = 0.;
+    if (static_cast<int64_t>(threadIdx.x) < a.n1024) {
+      mine = s.group[threadIdx.x];
+      if (r.k || r.p < 1.f) mine += static_cast<double>(s.mass[threadIdx.x]) / kFixed;
+    }
+    by_groups(mine, cut, least);
   }
 
   __device__ __forceinline__ void run() {
-    const uint32_t key = block_most(
-        static_cast<int64_t>(threadIdx.x) < a.n1024 ? a.firsts[row * a.n1024 + threadIdx.x] : 0u,
-        reinterpret_cast<uint32_t*>(s.waves64));
+    const uint32_t key = block_most(static_cast<int64_t>(threadIdx.x) < a.n1024 ? a.firsts[row * a.n1024 + threadIdx.x] : 0u, s);
     if (r.bad || key == kNan || key <= kNone) {
-      if (threadIdx.x == 0) done(-1, NAN);
+      none();
       return;
     }
     if (r.first) {
@@ -634,33 +858,38 @@ struct Pick {
       return;
     }
     inf = key == kInf;
-    top = inf ? 0.f : value_of(key);
-    const bool all = whole(r);
-    double mass = 0.;
-    if (all) {
+    mass_of.top = inf ? 0. : static_cast<double>(value_of(key));
+    double mass = 1.;
+    if (whole(r)) {
       const double mine = group_mass();
       if (r.p >= 1.f) {
         by_groups(mine, 0, 0.);
         return;
       }
-      block_scan(mine, s.waves, mass);
+      block_scan(mine, s, mass);
     }
+    double share;
     if (!inf) {
       if (r.k) {
-        if (r.k <= a.n64 && from_list(kth_top(r.k), true, 0.)) return;
+        if (r.k <= a.n64) {
+          if (from_list(near_top(r.k), true, mass, share)) return;
+          if (from_list(kth_top(r.k), true, mass, share)) return;   // (far from evenly spread)
+        }
       } else {
         uint32_t floor = kNone + 1;
         if (r.m > 0.f) {   // nothing under it is kept
-          const double y = top + static_cast<double>(r.t) * log(static_cast<double>(r.m));
+          const double y = mass_of.top + static_cast<double>(r.t) * log(static_cast<double>(r.m));
           // (under it by more than the roundings of y, of f and of a mass)
-          const float f = static_cast<float>(y - 1e-6 * (fabs(y) + fabs(static_cast<double>(top)) + static_cast<double>(r.t)));
+          const float f = static_cast<float>(y - 1e-6 * (fabs(y) + fabs(mass_of.top) + static_cast<double>(r.t)));
           floor = f > -INFINITY ? key_of(f) : kNone + 1;
-          if (from_list(floor, true, mass)) return;
+          if (from_list(floor, true, mass, share)) return;
         }
         if (r.p < 1.f) {
+          // Some 64 tokens, and where they hold a good part of the masses some 1000.
           for (int64_t c = 64; c <= 1024 && c <= a.n64; c *= 16) {
-            const uint32_t least = kth_top(c);
-            if (from_list(least > floor ? least : floor, least <= floor, mass)) return;
+            const uint32_t least = near_top(c);
+            if (from_list(least > floor ? least : floor, least <= floor, mass, share)) return;
+            if (share < .5 * static_cast<double>(r.p)) break;
           }
         }
       }
@@ -673,16 +902,34 @@ template <typename E>
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
   __shared__ Shared s;
   const int64_t row = blockIdx.x;
-  Pick<E> p{a, s, row, row_of(a, row), static_cast<const E*>(a.x) + row * a.ldx, 0.f, false};
+  load_powers(s.powers);   // (barriers follow before they are read)
+  const Row r = row_of(a, row);
+  Pick<E> p{a, s, row, r, static_cast<const E*>(a.x) + row * a.ldx, Exp{s.powers, 0., r.scale}, false};
   p.run();
 }
 
 template <typename E>
 hipError_t sample(const SampleArgs& a, hipStream_t stream) {
-  const int64_t blocks = (a.n * a.n1024 + 3) / 4;
-  if (blocks > most_blocks(256) || a.n > most_blocks(kThreads)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(sample_groups_kernel<E>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
-  hipLaunchKernelGGL(sample_pick_kernel<E>, dim3(static_cast<unsigned>(a.n)), dim3(kThreads), 0, stream, a);
+  constexpr int64_t kRows = 65535;   // of a launch's second dimension
+  const auto across = static_cast<unsigned>((a.n1024 + 3) / 4);
+  for (int64_t r = 0; r < a.n; r += kRows) {
+    SampleArgs p = a;
+    const int64_t n = a.n - r < kRows ? a.n - r : kRows;
+    auto past = [&](auto* q, int64_t each) { return q ? q + r * each : nullptr; };
+    p.x = static_cast<const E*>(a.x) + r * a.ldx;
+    p.u = a.u + r;
+    p.t = past(a.t, 1);
+    p.p = past(a.p, 1);
+    p.m = past(a.m, 1);
+    p.k = past(a.k, 1);
+    p.token = a.token + r;
+    p.logprob = past(a.logprob, 1);
+    p.tops = a.tops + r * a.n64;
+    p.firsts = a.firsts + r * a.n1024;
+    p.masses = a.masses + r * a.n1024;
+    hipLaunchKernelGGL(sample_groups_kernel<E>, dim3(across, static_cast<unsigned>(n)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(sample_pick_kernel<E>, dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream, p);
+  }
   return hipGetLastError();
 }
 

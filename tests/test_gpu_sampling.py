@@ -33,7 +33,7 @@ def reference(x, u, t=1.0, k=0, p=1.0, m=0.0):
         x = np.where(x == math.inf, 0.0, -math.inf)
     with np.errstate(over="ignore"):
         z = (x - x.max()) / t
-    w = np.where(z > -700, np.exp(z), 0.0)
+    w = np.where(z > -690, np.exp(z), 0.0)
     order = np.argsort(-x, kind="stable")
     ws = w[order]
     rank = np.arange(v)
