@@ -13,7 +13,7 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;   // of the kernel that picks: a workgroup a row
 constexpr int kGroup = 1024;                             // tokens whose mass is summed up first
-constexpr int kBins = 2048, kList = 4096;
+constexpr int kBins = 2048, kList = 2048, kRing = 512;
 
 // ---------------------------------------------------------------- keys, masses
 // Keys order as the values do; equal values (0 and -0) have equal keys, NaN the
@@ -27,63 +27,148 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// e^z of z <= 0 in 64 bits: z·32/ln 2 = 32·n + j + f, |f| <= 1/2, and e^z = 2^n · 2^(j/32)
-// · e^(f ln 2/32), the last by its series (the first term left out is 1.2e-12), 2^(j/32)
-// from a table in LDS whose 64 words lie in 64 banks. 15 vector instructions and a read
-// of LDS; without a table the series takes eight terms more.
-__device__ const double kPowers[32] = {
-    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
-    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
-    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
-    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
-    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
-    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
-    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
-    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+// e^z of z <= 0 in 64 bits: z·256/ln 2 = 256·n + j + f, |f| <= 1/2, and e^z = 2^n · 2^(j/256)
+// · e^y, y = f ln 2/256, the last by its series (the first term left out is 1.4e-13),
+// 2^(j/256) from a table in LDS. Nine instructions of 64 bits, whose rate bounds the
+// passes that weigh tokens: a wave's takes 8 cycles.
+constexpr int kPowers = 256;
+__device__ const double kPower[kPowers] = {
+    1.0, 1.0027112750502025, 1.0054299011128027, 1.0081558981184175,
+    1.0108892860517005, 1.0136300849514894, 1.016378314910953, 1.019133996077738,
+    1.0218971486541166, 1.0246677928971357, 1.0274459491187637, 1.030231637686041,
+    1.0330248790212284, 1.0358256936019572, 1.0386341019613787, 1.041450124688316,
+    1.0442737824274138, 1.0471050958792898, 1.0499440858006872, 1.0527907730046264,
+    1.0556451783605572, 1.0585073227945128, 1.061377227289262, 1.0642549128844645,
+    1.0671404006768237, 1.0700337118202419, 1.0729348675259756, 1.075843889062791,
+    1.0787607977571199, 1.0816856149932152, 1.0846183622133092, 1.0875590609177697,
+    1.0905077326652577, 1.0934643990728858, 1.0964290818163769, 1.099401802630222,
+    1.102382583307841, 1.1053714457017412, 1.1083684117236787, 1.1113735033448175,
+    1.1143867425958924, 1.1174081515673693, 1.1204377524096067, 1.12347556733302,
+    1.1265216186082418, 1.129575928566288, 1.1326385195987192, 1.1357094141578055,
+    1.1387886347566916, 1.1418762039695616, 1.1449721444318042, 1.148076478840179,
+    1.1511892299529827, 1.154310420590216, 1.1574400736337511, 1.1605782120274988,
+    1.1637248587775775, 1.1668800369524817, 1.1700437696832502, 1.1732160801636373,
+    1.1763969916502812, 1.1795865274628758, 1.182784710984341, 1.1859915656609938,
+    1.189207115002721, 1.1924313825831512, 1.1956643920398273, 1.1989061670743806,
+    1.202156731452703, 1.2054161090051239, 1.2086843236265816, 1.2119613992768012,
+    1.215247359980469, 1.2185422298274085, 1.2218460329727576, 1.2251587936371455,
+    1.22848053610687, 1.2318112847340759, 1.2351510639369334, 1.2384998981998165,
+    1.241857812073484, 1.245224830175258, 1.2486009771892048, 1.2519862778663162,
+    1.255380757024691, 1.2587844395497165, 1.2621973503942507, 1.2656195145788063,
+    1.2690509571917332, 1.2724917033894028, 1.275941778396392, 1.2794012075056693,
+    1.2828700160787783, 1.2863482295460256, 1.2898358734066657, 1.2933329732290895,
+    1.2968395546510096, 1.3003556433796506, 1.3038812651919358, 1.3074164459346773,
+    1.3109612115247644, 1.3145155879493546, 1.318079601266064, 1.3216532776031575,
+    1.3252366431597413, 1.3288297242059544, 1.3324325470831615, 1.3360451382041458,
+    1.339667524053303, 1.3432997311868353, 1.3469417862329458, 1.3505937158920345,
+    1.3542555469368927, 1.3579273062129011, 1.3616090206382248, 1.365300717204012,
+    1.3690024229745905, 1.3727141650876684, 1.3764359707545302, 1.380167867260238,
+    1.383909881963832, 1.387662042298529, 1.3914243757719262, 1.3951969099662003,
+    1.3989796725383112, 1.4027726912202048, 1.4065759938190154, 1.4103896082172707,
+    1.4142135623730951, 1.4180478843204152, 1.4218926021691656, 1.4257477441054942,
+    1.42961333839197, 1.433489413367789, 1.4373759974489824, 1.4412731191286257,
+    1.4451808069770467, 1.449099089642035, 1.4530279958490526, 1.4569675544014438,
+    1.460917794180647, 1.4648787441464057, 1.4688504333369818, 1.4728328908693675,
+    1.4768261459394993, 1.4808302278224719, 1.4848451658727524, 1.488870989524397,
+    1.4929077282912648, 1.4969554117672355, 1.5010140696264256, 1.5050837316234065,
+    1.5091644275934228, 1.5132561874526098, 1.5173590411982147, 1.5214730189088146,
+    1.5255981507445384, 1.529734466947287, 1.533881997840956, 1.5380407738316568,
+    1.5422108254079407, 1.5463921831410214, 1.550584877685, 1.5547889397770887,
+    1.559004400237837, 1.5632312899713576, 1.567469639965553, 1.5717194812923414,
+    1.5759808451078865, 1.5802537626528246, 1.5845382652524937, 1.588834384317164,
+    1.593142151342267, 1.597461597908627, 1.6017927556826934, 1.606135656416771,
+    1.6104903319492543, 1.6148568142048607, 1.6192351351948637, 1.6236253270173289,
+    1.6280274218573478, 1.632441451987275, 1.6368674497669644, 1.6413054476440063,
+    1.645755478153965, 1.6502175739206177, 1.6546917676561943, 1.6591780921616162,
+    1.6636765803267364, 1.6681872651305825, 1.6727101796415966, 1.6772453570178785,
+    1.681792830507429, 1.6863526334483934, 1.6909247992693053, 1.6955093614893326,
+    1.7001063537185235, 1.7047158096580513, 1.709337763100463, 1.713972247929926,
+    1.718619298122478, 1.723278947746274, 1.7279512309618377, 1.732636182022311,
+    1.7373338352737062, 1.7420442251551564, 1.746767386199169, 1.7515033530318782,
+    1.7562521603732995, 1.761013843037584, 1.7657884359332727, 1.7705759740635547,
+    1.7753764925265212, 1.7801900265154245, 1.785016611318935, 1.789856282321401,
+    1.7947090750031072, 1.7995750249405351, 1.804454167806624, 1.809346539371032,
+    1.8142521755003989, 1.8191711121586085, 1.8241033854070534, 1.8290490314048973,
+    1.8340080864093424, 1.8389805867758937, 1.843966568958626, 1.8489660695104508,
+    1.8539791250833855, 1.8590057724288205, 1.864046048397789, 1.8690999899412386,
+    1.8741676341103, 1.8792490180565602, 1.8843441790323345, 1.8894531543909392,
+    1.8945759815869656, 1.8997126981765553, 1.9048633418176741, 1.9100279502703899,
+    1.9152065613971474, 1.9203992131630474, 1.925605943636125, 1.930826790987627,
+    1.9360617934922943, 1.9413109895286405, 1.9465744175792332, 1.9518521162309783,
+    1.9571441241754002, 1.9624504802089273, 1.9677712232331759, 1.9731063922552343,
+    1.978456026387951, 1.9838201648502194, 1.9891988469672663, 1.9945921121709402,
 };
 struct Exp {
-  const double* powers;   // kPowers, in LDS
-  double top, scale;      // of e^((x - top) / t): scale = 32 / (t ln 2)
-  // (Next to nothing, not 0, below e^-690.)
-  __device__ __forceinline__ double rough(float x) const {
-    constexpr double kMagic = 6755399441055744., y = 0.021660849392498290084;   // 1.5 · 2^52; ln 2 / 32
-    const double t = fmax((static_cast<double>(x) - top) * scale, -32000.);
-    const double d = t + kMagic;   // its low word is round(t)
-    const double f = t - (d - kMagic);
-    double p = fma(f, y * y * y * y / 24., y * y * y / 6.);
-    p = fma(p, f, y * y / 2.);
-    p = fma(p, f, y);
-    p = fma(p, f, 1.);
-    const int k = __double2loint(d);
-    p *= powers[k & 31];
-    return __hiloint2double(__double2hiint(p) + (k >> 5) * (1 << 20), __double2loint(p));
+  const double* powers;   // kPower, in LDS
+  double top, inv;        // of e^((x - top) / t): inv = 1 / t
+  double shift;           // top / t, rounded
+  __device__ __forceinline__ Exp(const double* p, float t) : powers(p), top(0.), inv(1. / static_cast<double>(t)), shift(0.) {}
+  __device__ __forceinline__ void from(double largest) {
+    top = largest;
+    shift = largest * inv;
   }
-  // 0 below e^-690 (and of -infinity).
+  // e^(top / t) over e^shift: what a sum of terms of `sum` is to be divided by.
+  __device__ __forceinline__ double rest() const { return 1. + fma(top, inv, -shift); }
+  // e^u, u <= 0, and `sum` (next to nothing, not 0, below e^-700).
+  __device__ __forceinline__ double plus(double u, double sum) const {
+    constexpr double kMagic = 6755399441055744., kStep = 2.7076061740622863e-3;   // 1.5 · 2^52; ln 2 / 256
+    u = fmax(u, -700.);
+    const double d = fma(u, 1. / kStep, kMagic);   // its low word is the nearest whole number
+    const double y = fma(d - kMagic, -kStep, u);
+    double p = fma(y, 1. / 6., .5);
+    p = fma(p, y, 1.);
+    p = fma(p, y, 1.);
+    const int k = __double2loint(d);
+    const double q = powers[k & (kPowers - 1)];
+    return fma(p, __hiloint2double(__double2hiint(q) + (k >> 8) * (1 << 20), __double2loint(q)), sum);
+  }
+  // x/t - shift is one rounding of a value of its own size off: an instruction less than
+  // the difference first. Not where shift's own rounding is more than rest() corrects.
+  __device__ __forceinline__ bool near() const { return fabs(shift) < 1e6; }
+  __device__ __forceinline__ double near_plus(float x, double sum) const {
+    return plus(fma(static_cast<double>(x), inv, -shift), sum);
+  }
+  __device__ __forceinline__ double far_plus(float x, double sum) const {
+    return plus((static_cast<double>(x) - top) * inv, sum);
+  }
+  // The mass itself, 0 below e^-690 (and of -infinity).
   __device__ __forceinline__ double operator()(float x) const {
-    return (static_cast<double>(x) - top) * scale > -690. * 46.166241308446828384 ? rough(x) : 0.;
+    const double u = (static_cast<double>(x) - top) * inv;
+    return u > -690. ? plus(u, 0.) : 0.;
   }
 };
 __device__ __forceinline__ void load_powers(double* powers) {
-  if (threadIdx.x < 32) powers[threadIdx.x] = kPowers[threadIdx.x];
+  if (threadIdx.x < kPowers) powers[threadIdx.x] = kPower[threadIdx.x];
+}
+
+// A value that all lanes have, in scalar registers.
+template <typename T>
+__device__ __forceinline__ T uniform(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+  } else {
+    const auto u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
+    return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+  }
 }
 
 struct Row {
   float t, p, m, u;
   int64_t k;
-  double scale;      // 32 / (t ln 2)
   bool bad, first;   // first: only the largest logit is kept
 };
 __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
   Row r;
-  r.t = a.t ? a.t[row] : a.t1;
-  r.p = a.p ? a.p[row] : a.p1;
-  r.m = a.m ? a.m[row] : a.m1;
-  r.k = a.k ? a.k[row] : a.k1;
-  r.u = a.u[row];
+  r.t = uniform(a.t ? a.t[row] : a.t1);
+  r.p = uniform(a.p ? a.p[row] : a.p1);
+  r.m = uniform(a.m ? a.m[row] : a.m1);
+  r.k = uniform(a.k ? a.k[row] : a.k1);
+  r.u = uniform(a.u[row]);
   r.bad = !(r.t >= 0.f) || r.t == INFINITY || r.p != r.p || r.m != r.m || !(r.u >= 0.f && r.u <= 1.f);
   if (r.k <= 0 || r.k >= a.v) r.k = 0;
   r.first = r.t == 0.f || r.k == 1 || r.p <= 0.f || r.m > 1.f;
-  r.scale = 46.166241308446828384 / static_cast<double>(r.t);
   return r;
 }
 // Whether the masses of all tokens are needed.
@@ -98,16 +183,15 @@ __device__ __forceinline__ double wave_sum(double x) {
 }
 
 // A lane's 16 of a group's tokens, kPer neighbouring ones a load; -infinity past the
-// row's end.
+// row's end. Fetched as they lie in memory, so that a next group's can be under way.
 template <typename E>
 struct Tokens {
   static constexpr int kPer = 16 / sizeof(E), kLoads = 16 / kPer;
-  float x[16];
+  E w[kLoads][kPer];
   __device__ __forceinline__ static int64_t column(int64_t group, int i) {   // of load i
     return group * kGroup + (i * 64 + static_cast<int>(threadIdx.x & 63)) * int64_t{kPer};
   }
-  __device__ __forceinline__ void load(const E* row, int64_t group, int64_t v) {
-    E w[kLoads][kPer];
+  __device__ __forceinline__ void fetch(const E* row, int64_t group, int64_t v) {
     if ((group + 1) * kGroup <= v) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) __builtin_memcpy(w[i], row + column(group, i), sizeof w[i]);
@@ -120,11 +204,8 @@ struct Tokens {
           w[i][k] = c < v ? row[c] : static_cast<E>(-INFINITY);
         }
     }
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) x[i * kPer + k] = static_cast<float>(w[i][k]);
   }
+  __device__ __forceinline__ float at(int i, int k) const { return static_cast<float>(w[i][k]); }
 };
 
 // ---------------------------------------------------------------- first pass
@@ -138,20 +219,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {   // (a NaN i
 template <typename E>
 __global__ __launch_bounds__(256) void sample_groups_kernel(SampleArgs a) {
   using T = Tokens<E>;
-  __shared__ double powers[32];
+  __shared__ double powers[kPowers];
   load_powers(powers);
   __syncthreads();
   const int64_t row = blockIdx.y, group = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (group >= a.n1024) return;
-  T t;
-  t.load(static_cast<const E*>(a.x) + row * a.ldx, group, a.v);
+  T raw;
+  raw.fetch(static_cast<const E*>(a.x) + row * a.ldx, group, a.v);
+  float x[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) x[k] = raw.at(k / T::kPer, k % T::kPer);
   constexpr int kLanes = 64 / T::kPer;   // that hold 64 neighbouring tokens
   float top = -INFINITY;
   bool nan = false;
 #pragma unroll
   for (int i = 0; i < T::kLoads; ++i) {
-    const float* y = t.x + i * T::kPer;
+    const float* y = x + i * T::kPer;
     float m = max3(y[0], y[1], y[2]);
     bool bad = __builtin_isunordered(y[0], y[1]) || __builtin_isunordered(y[2], y[3]);
     if constexpr (T::kPer == 8) {
@@ -183,16 +267,22 @@ __global__ __launch_bounds__(256) void sample_groups_kernel(SampleArgs a) {
   double mass = 0.;
   if (key >= kInf) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) mass += t.x[k] == INFINITY ? 1. : 0.;
+    for (int k = 0; k < 16; ++k) mass += x[k] == INFINITY ? 1. : 0.;
   } else if (key > kNone) {
-    const Exp e{powers, static_cast<double>(value_of(key)), r.scale};
-    double part = 0.;
+    Exp e(powers, r.t);
+    e.from(static_cast<double>(value_of(key)));
+    if (e.near()) {
+      double part = 0.;
 #pragma unroll
-    for (int k = 0; k < 16; k += 2) {
-      mass += e.rough(t.x[k]);
-      part += e.rough(t.x[k + 1]);
+      for (int k = 0; k < 16; k += 2) {
+        mass = e.near_plus(x[k], mass);
+        part = e.near_plus(x[k + 1], part);
+      }
+      mass = (mass + part) / e.rest();
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) mass = e.far_plus(x[k], mass);
     }
-    mass += part;
   }
   mass = wave_sum(mass);
   if (lane == 0) a.masses[row * a.n1024 + group] = mass;
@@ -200,11 +290,16 @@ __global__ __launch_bounds__(256) void sample_groups_kernel(SampleArgs a) {
 
 // ---------------------------------------------------------------- picking
 struct Shared {
-  uint64_t list[kList];        // candidates, key over the token's complement
-  uint64_t mass[kBins];        // of bins, in fixed point; or of groups
-  uint32_t count[2 * kBins];   // of bins; or the 64s that hold candidates
+  uint64_t list[kList];            // candidates, key over the token's complement
+  union {
+    struct {
+      uint64_t mass[kBins];        // of bins, in fixed point; or of groups
+      uint32_t count[2 * kBins];   // of bins; or the 64s that hold candidates
+    };
+    float ring[kWaves][kRing];     // a wave's values to be weighed
+  };
   double group[kGroup];
-  double powers[32];
+  double powers[kPowers];
   uint64_t waves[2][kWaves];
   uint32_t n, found;
   double value;
@@ -241,7 +336,7 @@ __device__ __forceinline__ T block_most(T v, Shared& s) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) v = waves[w] > v ? waves[w] : v;
-  return v;
+  return uniform(v);
 }
 template <typename T>
 __device__ __forceinline__ T wave_scan(T v) {
@@ -269,6 +364,7 @@ __device__ __forceinline__ T block_scan(T v, Shared& s, T& all) {
     if (w == wave) before = all;
     all += waves[w];
   }
+  all = uniform(all);
   return before + v;
 }
 
@@ -321,7 +417,7 @@ struct Pick {
     const double upto = block_scan(mine, s, mass);
     const double target = static_cast<double>(r.u) * mass;
     const int64_t c = crossing(mine, upto, target) * int64_t{kGroup} + threadIdx.x;
-    const double before = s.value;
+    const double before = uniform(s.value);
     float y = -INFINITY;
     double w = 0.;
     if (c < a.v) {
@@ -382,9 +478,10 @@ struct Pick {
     if (upto >= k && upto - c0 - c1 < k) s.found = upto - c1 >= k ? b : b + 1;
     __syncthreads();
     // its lower end, and a little less for the roundings
-    const float end = high - (static_cast<float>(s.found) + 1.f) / width;
+    const uint32_t found = uniform(s.found);
+    const float end = high - (static_cast<float>(found) + 1.f) / width;
     const float less = end - 1e-6f * (fabsf(high) + fabsf(end));
-    return less > -INFINITY && s.found < kBins - 1 ? key_of(less) : kNone + 1;
+    return less > -INFINITY && found < kBins - 1 ? key_of(less) : kNone + 1;
   }
   // The k-th largest of the 64s' largest keys (1 <= k <= n64), 11, 11 and 10 bits at a time.
   __device__ __forceinline__ uint32_t kth_top(int64_t k) {
@@ -413,9 +510,9 @@ struct Pick {
         s.n = rank - (in_hi ? before : before + hi);
       }
       __syncthreads();
-      prefix |= s.found << shift;
+      prefix |= uniform(s.found) << shift;
       mask |= digits << shift;
-      rank = s.n;
+      rank = uniform(s.n);
     }
     __syncthreads();
     return prefix;
@@ -448,15 +545,24 @@ struct Pick {
         if (at < 2 * kBins) s.count[at] = static_cast<uint32_t>(i);
       }
     __syncthreads();
-    const uint32_t spans = s.found;
+    const uint32_t spans = uniform(s.found);
     if (spans > 2 * kBins) return kList + 1;
-    for (uint32_t i = threadIdx.x >> 6; i < spans; i += kWaves) {
-      const int64_t c = s.count[i] * int64_t{64} + (threadIdx.x & 63);
-      const float y = c < a.v ? static_cast<float>(x[c]) : -INFINITY;
-      append(c < a.v && key_of(y) >= least, order_of(y, c));
+    constexpr int kMany = 8;   // under way at a time
+    for (uint32_t i0 = threadIdx.x >> 6; i0 < spans; i0 += kWaves * kMany) {
+      float y[kMany];
+      int64_t c[kMany];
+#pragma unroll
+      for (int q = 0; q < kMany; ++q) {
+        const uint32_t i = i0 + q * kWaves;
+        c[q] = s.count[i < spans ? i : i0] * int64_t{64} + (threadIdx.x & 63);
+        y[q] = static_cast<float>(x[c[q] < a.v ? c[q] : 0]);
+        if (i >= spans) c[q] = a.v;
+      }
+#pragma unroll
+      for (int q = 0; q < kMany; ++q) append(c[q] < a.v && key_of(y[q]) >= least, order_of(y[q], c[q]));
     }
     __syncthreads();
-    return s.n;
+    return uniform(s.n);
   }
 
   // The list's first n in descending order; how many entries that are with the zeros
@@ -545,308 +651,207 @@ struct Pick {
       }
     }
     __syncthreads();
-    share = s.value / all_mass;
-    const bool found = s.found;
+    share = uniform(s.value) / all_mass;
+    const bool found = uniform(s.found);
     __syncthreads();
     return found;
   }
 
-  // From the tokens whose keys are at least `least`, where they are few enough and
-  // known to hold all that are kept (`complete`, or the cut is among them).
-  __device__ __forceinline__ bool from_list(uint32_t least, bool complete, double all_mass, double& share) {
-    share = 1.;
-    const uint32_t n = candidates(least);
-    if (n > kList) return false;
-    if (n <= 64) return from_few(n, complete, all_mass, share);
-    const uint32_t size = sort(n), per = size > kThreads ? size / kThreads : 1, i0 = threadIdx.x * per;
-    const uint32_t most = r.k && r.k < n ? static_cast<uint32_t>(r.k) : n;
-    double w[kList / kThreads], mine = 0., all;
+  // ---- many tokens: passes over the whole row
+  // f(group, unit, first token, values): four neighbouring tokens a lane, four units a
+  // group, a wave a group; the next group's under way. (One copy of f: the whole kernel
+  // is to stay in the instruction cache. With f 16 times it was 237 KB, and every
+  // stage waited for its code.)
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    using T = Tokens<E>;
+    int64_t g = threadIdx.x >> 6;
+    if (g >= a.n1024) return;
+    T t;
+    t.fetch(x, g, a.v);
+    while (true) {
+      float y[4][4];
 #pragma unroll
-    for (uint32_t q = 0; q < kList / kThreads; ++q) {
-      w[q] = q < per && i0 + q < most ? weight(listed(s.list[i0 + q])) : 0.;
-      mine += w[q];
-    }
-    double before = block_scan(mine, s, all) - mine;
-    const double limit = r.p < 1.f ? static_cast<double>(r.p) * (r.k ? all : all_mass) : INFINITY;
-    uint32_t kept = 0;
+      for (int k = 0; k < 16; ++k) y[k / 4][k % 4] = t.at(k / T::kPer, k % T::kPer);
+      if (inf) {
 #pragma unroll
-    for (uint32_t q = 0; q < kList / kThreads; ++q) {
-      const uint32_t i = i0 + q;
-      if (q < per && i < most && (i == 0 || (before < limit && w[q] >= static_cast<double>(r.m)))) kept = i + 1;
-      before += w[q];
-    }
-    const uint32_t count = block_most(kept, s);
-    share = all / all_mass;
-    if (!r.k && !complete && count == n) return false;
-    // the kept ones in the order of the vocabulary
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < count; i += kThreads) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;
-    const uint32_t size2 = sort(count), per2 = size2 > kThreads ? size2 / kThreads : 1, j0 = threadIdx.x * per2;
-    mine = 0.;
-#pragma unroll
-    for (uint32_t q = 0; q < kList / kThreads; ++q) {
-      w[q] = q < per2 && j0 + q < count ? weight(value_of(static_cast<uint32_t>(s.list[j0 + q]))) : 0.;
-      mine += w[q];
-    }
-    const double upto = block_scan(mine, s, all);
-    const double target = static_cast<double>(r.u) * all;
-    const int t = crossing(mine, upto, target);
-    if (static_cast<int>(threadIdx.x) == t) {
-      double sum = upto - mine;
-      uint32_t pick = j0;
-#pragma unroll
-      for (uint32_t q = 0; q < kList / kThreads; ++q) {
-        if (w[q] > 0.) {
-          if (!(sum > target)) pick = j0 + q;
-          sum += w[q];
-        }
+        for (int k = 0; k < 16; ++k) y[k / 4][k % 4] = value(y[k / 4][k % 4]);
       }
-      const uint64_t e = s.list[pick];
-      done(token_of(static_cast<uint32_t>(e >> 32)), value_of(static_cast<uint32_t>(e)), all);
-    }
-    return true;
-  }
-
-  // ---- many tokens: selection over the whole row
-  // f(token, value) of every token, a wave a group; ended(group) after each.
-  template <typename F, typename G>
-  __device__ __forceinline__ void each(F&& f, G&& ended) const {
-    for (int64_t g = threadIdx.x >> 6; g < a.n1024; g += kWaves) {
-      Tokens<E> t;
-      t.load(x, g, a.v);
+      const int64_t next = g + kWaves;
+      if (next < a.n1024) t.fetch(x, next, a.v);
+#pragma unroll 1
+      for (int unit = 0; unit < 4; ++unit) {
+        f(g, unit, T::column(g, unit * 4 / T::kPer) + unit * 4 % T::kPer, y[0]);
 #pragma unroll
-      for (int i = 0; i < Tokens<E>::kLoads; ++i)
-#pragma unroll
-        for (int k = 0; k < Tokens<E>::kPer; ++k)
-          f(Tokens<E>::column(g, i) + k, value(t.x[i * Tokens<E>::kPer + k]));
-      ended(g);
+        for (int k = 0; k < 12; ++k) y[k / 4][k % 4] = y[k / 4 + 1][k % 4];
+      }
+      if (next >= a.n1024) return;
+      g = next;
     }
   }
 
-  // The groups' masses of the tokens from `cut` on, those of at least `least`.
-  __device__ __forceinline__ void group_masses(uint64_t cut, double least) {
-    double sum = 0.;
+  __device__ __forceinline__ double sum_of_groups() {
+    double all;
+    block_scan(static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0., s, all);
+    return all;
+  }
+
+  // What a pass over the row looks at: the tokens from `limit` on in descending order;
+  // where `direct` all of them are taken, else those in bins above `first` or with keys
+  // above `hi`, and the members, in bins from `first` to `final` with keys from `lo`
+  // to `hi`, are listed.
+  struct Cut {
+    uint64_t limit;
+    bool direct, by_count;
+    uint32_t first, final, lo, hi;
+    int level, shift;
+    float high, width, slope;   // bins of equal width below the largest; of log2 of a mass
+  };
+  __device__ __forceinline__ uint32_t bin_of(const Cut& q, float y) const {
+    return static_cast<uint32_t>(fminf((q.high - y) * q.width, kBins - 1.f));
+  }
+
+  // Counts or weighs the members in bins. The first weighing is in 32 bits.
+  __device__ __forceinline__ void fill_bins(const Cut& q) {
     __syncthreads();
-    each([&](int64_t c, float y) {
-      const double w = weight(y);
-      if (order_of(y, c) >= cut && w >= least) sum += w;
-    }, [&](int64_t g) {
-      sum = wave_sum(sum);
-      if ((threadIdx.x & 63) == 0) s.group[g] = sum;
-      sum = 0.;
+    for (int b = threadIdx.x; b < kBins; b += kThreads) s.mass[b] = 0;
+    __syncthreads();
+    each([&](int64_t, int, int64_t c, const float(&y)[4]) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (!(y[k] > -INFINITY) || order_of(y[k], c + k) < q.limit) continue;
+        uint32_t b = bin_of(q, y[k]);
+        if (q.level) {
+          const uint32_t key = key_of(y[k]);
+          if (b < q.first || b > q.final || key < q.lo || key > q.hi) continue;
+          b = (q.hi - key) >> q.shift;
+        }
+        unsigned long long one = 1;
+        if (!q.by_count) {
+          if (q.level) one = fixed_of(weight(y[k]));
+          else one = static_cast<uint32_t>(__builtin_amdgcn_exp2f((q.high - y[k]) * q.slope) * 2147483648.f);
+        }
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), one);
+      }
     });
     __syncthreads();
   }
 
-  // Of the tokens from `cut` on in descending order the last one kept: the k-th (COUNT),
-  // or the first up to which the masses add to `goal`. With `last` leaves the kept
-  // tokens' masses of at least `least` in s.group and, those that stood in the list,
-  // in s.mass; else returns all kept tokens' mass in `mass`.
-  //
-  // A pass counts or weighs the tokens in bins of equal width below the largest; the
-  // bin that the cut is in goes to a list in the next, which also adds up what lies
-  // above it, and the list is sorted. Where it is too long its keys are cut into bins
-  // again.
-  template <bool COUNT>
-  __device__ __forceinline__ uint64_t select(uint64_t cut, bool cut_is, int64_t k, double goal, bool last, double least, double& mass) {
-    // 24 units of e^x hold all masses that count; by ranks, what the 64s' largest span.
-    float span = 24.f * r.t;
-    if constexpr (COUNT) {
-      uint32_t most = 0;
-      for (int64_t i = threadIdx.x; i < a.n64; i += kThreads) {
-        const uint32_t key = a.tops[row * a.n64 + i];
-        if (key > kNone) most = ~key > most ? ~key : most;
-      }
-      const float low = value_of(~block_most(most, s));
-      if (!inf) span = (top() - low) * 1.25f;
-    }
-    const float high = top(), width = fminf(static_cast<float>(kBins) / span, 1e30f);
-    uint32_t first = 0, lo = 0, hi = 0;
-    int level = 0, shift = 0;
-    double above = 0.;
-    uint32_t n_above = 0, n;
-    auto bin0 = [&](float y) { return static_cast<uint32_t>(fminf((high - y) * width, kBins - 1.f)); };
-    auto eligible = [&](int64_t c, float y) { return y > -INFINITY && (!cut_is || order_of(y, c) >= cut); };
-    while (true) {
-      __syncthreads();
-      for (int b = threadIdx.x; b < kBins; b += kThreads) {
-        if constexpr (COUNT) s.count[b] = 0;
-        else s.mass[b] = 0;
-      }
-      __syncthreads();
-      each([&](int64_t c, float y) {
-        if (!eligible(c, y)) return;
-        uint32_t b = bin0(y);
-        if (level) {
-          const uint32_t key = key_of(y);
-          if (b != first || key < lo || key > hi) return;
-          b = (hi - key) >> shift;
-        }
-        if constexpr (COUNT) atomicAdd(&s.count[b], 1u);
-        else atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), fixed_of(mass_of.rough(y)));
-      }, [](int64_t) {});
-      __syncthreads();
-      // the first bin that reaches it, or else the last one with tokens
-      const int b = 2 * static_cast<int>(threadIdx.x);
-      uint64_t v0, v1;
-      if constexpr (COUNT) v0 = s.count[b], v1 = s.count[b + 1];
-      else v0 = s.mass[b], v1 = s.mass[b + 1];
-      uint64_t all;
-      const uint64_t upto = block_scan<uint64_t>(v0 + v1, s, all);
-      auto reached = [&](uint64_t q) {
-        if constexpr (COUNT) return n_above + static_cast<int64_t>(q) >= k;
-        else return above + static_cast<double>(q) / kFixed >= goal;
-      };
-      uint32_t mine = 0;
-      if (v0 && reached(upto - v1)) mine = 0x80000000u | (kBins - b);
-      else if (v1 && reached(upto)) mine = 0x80000000u | (kBins - b - 1);
-      else if (v1) mine = 2u + b;
-      else if (v0) mine = 1u + b;
-      const uint32_t best = block_most(mine, s);
-      const uint32_t bin = best & 0x80000000u ? kBins - (best & 0x7fffffffu) : best ? best - 1 : 0;
-      if (bin / 2 == threadIdx.x) s.list[0] = upto - v1 - (bin & 1 ? 0 : v0);
-      __syncthreads();
-      if constexpr (COUNT) n_above += static_cast<uint32_t>(s.list[0]);
-      else above += static_cast<double>(s.list[0]) / kFixed;
-      if (level == 0) {
-        first = bin;
-        lo = 0;
-        hi = kNan;
-      } else {
-        const uint32_t h = hi - (bin << shift);
-        lo = h - lo > (uint32_t{1} << shift) - 1 ? h - ((uint32_t{1} << shift) - 1) : lo;
-        hi = h;
-      }
-      ++level;
-      // the bin's tokens, the range of their keys, and the masses above them
-      __syncthreads();
-      if (threadIdx.x == 0) s.n = 0;
-      __syncthreads();
-      uint32_t low = kNan, most = 0;
-      double sum = 0.;
-      each([&](int64_t c, float y) {
-        const bool is = eligible(c, y);
-        const uint32_t b = is ? bin0(y) : kBins, key = key_of(y);
-        const bool member = b == first && key >= lo && key <= hi;
-        if (b < first || (b == first && key > hi)) {
-          const double w = weight(y);
-          if (w >= least) sum += w;
+  // The first bin for which reached(its sum and those of the bins before), the last one
+  // with a share where there is none.
+  template <typename F>
+  __device__ __forceinline__ uint32_t bin_where(uint64_t v0, uint64_t v1, uint64_t upto, F&& reached) {
+    const int b = 2 * static_cast<int>(threadIdx.x);
+    uint32_t mine = 0;
+    if (v0 && reached(upto - v1)) mine = 0x80000000u | (kBins - b);
+    else if (v1 && reached(upto)) mine = 0x80000000u | (kBins - b - 1);
+    else if (v1) mine = 2u + b;
+    else if (v0) mine = 1u + b;
+    const uint32_t best = block_most(mine, s);
+    return best & 0x80000000u ? kBins - (best & 0x7fffffffu) : best ? best - 1 : 0;
+  }
+
+  // Adds up the masses of at least `least` of the tokens taken, by group in s.group, and
+  // lists the members: s.n of them, `above` their number; the range of their keys. The
+  // taken ones are put together and weighed 64 at a time, so that the others cost no
+  // exponential.
+  __device__ __forceinline__ void gather(const Cut& q, double least, uint32_t& above, uint32_t& low, uint32_t& most) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.n = s.found = 0;
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    const uint64_t under = (uint64_t{1} << lane) - 1;
+    float* ring = s.ring[threadIdx.x >> 6];
+    uint32_t from = 0, held = 0, taken = 0;
+    double sum = 0.;
+    low = kNan;
+    most = 0;
+    each([&](int64_t g, int unit, int64_t c, const float(&y)[4]) {
+      uint64_t members[4], any = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t key = key_of(y[k]);
+        bool take = y[k] > -INFINITY && order_of(y[k], c + k) >= q.limit, member = false;
+        if (!q.direct) {
+          const uint32_t b = bin_of(q, y[k]);
+          const bool within = take && b >= q.first && b <= q.final;
+          member = within && key >= q.lo && key <= q.hi;
+          take = take && (b < q.first || (within && key > q.hi));
         }
         if (member) {
           low = key < low ? key : low;
           most = key > most ? key : most;
         }
-        append(member, order_of(y, c));
-      }, [&](int64_t g) {
+        members[k] = __ballot(member);
+        any |= members[k];
+        const uint64_t who = __ballot(take);
+        if (take) ring[(from + held + static_cast<uint32_t>(__popcll(who & under))) % kRing] = y[k];
+        held += static_cast<uint32_t>(__popcll(who));
+      }
+      if (any) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) n += static_cast<uint32_t>(__popcll(members[k]));
+        uint32_t place = 0;
+        if (lane == 0) place = atomicAdd(&s.n, n);
+        place = __shfl(place, 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t at = place + static_cast<uint32_t>(__popcll(members[k] & under));
+          if ((members[k] >> lane & 1) && at < kList) s.list[at] = order_of(y[k], c + k);
+          place += static_cast<uint32_t>(__popcll(members[k]));
+        }
+      }
+      while (held >= (unit < 3 ? 64u : 1u)) {
+        const uint32_t n = held < 64 ? held : 64;
+        wave_sync();
+        const float v = ring[(from + lane) % kRing];
+        wave_sync();
+        const double w = lane < static_cast<int>(n) ? weight(v) : 0.;
+        if (w >= least) sum += w;
+        from += n;
+        held -= n;
+        taken += n;
+      }
+      if (unit == 3) {
         sum = wave_sum(sum);
-        if ((threadIdx.x & 63) == 0) s.group[g] = sum;
+        if (lane == 0) s.group[g] = sum;
         sum = 0.;
-      });
-      __syncthreads();
-      n = s.n;
-      if (n <= kList) break;
-      hi = block_most(most, s);
-      lo = ~block_most(~low, s);
-      if (lo == hi) {   // more equal values than the list holds
-        const double w = weight(value_of(hi));
-        int64_t want;
-        if constexpr (COUNT) want = k - n_above;
-        else want = static_cast<int64_t>(fmin(ceil((goal - above) / w), static_cast<double>(n)));
-        want = want < 1 ? 1 : want > n ? n : want;
-        // the want-th of them
-        uint64_t seen = 0, o = 0;
-        for (int64_t c0 = 0; c0 < a.v && static_cast<int64_t>(seen) < want; c0 += kThreads) {
-          const int64_t c = c0 + threadIdx.x;
-          const float y = c < a.v ? value(static_cast<float>(x[c])) : -INFINITY;
-          const bool is = c < a.v && key_of(y) == hi && eligible(c, y);
-          uint64_t here;
-          const uint64_t at = seen + block_scan<uint64_t>(is ? 1 : 0, s, here);
-          if (is && static_cast<int64_t>(at) == want) o = order_of(y, c);
-          seen += here;
-        }
-        o = block_most(o, s);
-        if (last) {
-          group_masses(o, least);
-          for (int g = threadIdx.x; g < kGroup; g += kThreads) s.mass[g] = 0;
-          __syncthreads();
-        } else {
-          block_scan(static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0., s, mass);
-          mass += static_cast<double>(want) * w;
-        }
-        return o;
       }
-      shift = 0;
-      while ((hi - lo) >> shift >= kBins) ++shift;
-    }
-    const uint32_t size = sort(n), per = size > kThreads ? size / kThreads : 1, i0 = threadIdx.x * per;
-    double w[kList / kThreads], mine = 0., all;
-#pragma unroll
-    for (uint32_t q = 0; q < kList / kThreads; ++q) {
-      w[q] = q < per && i0 + q < n ? weight(listed(s.list[i0 + q])) : 0.;
-      mine += w[q];
-    }
-    const double before = block_scan(mine, s, all) - mine;
-    double sum = before;
-    uint32_t best = 0;   // larger: earlier
-#pragma unroll
-    for (uint32_t q = 0; q < kList / kThreads; ++q) {
-      const uint32_t i = i0 + q;
-      sum += w[q];
-      if (q < per && i < n && !(best & 0x80000000u)) {
-        bool is;
-        if constexpr (COUNT) is = n_above + i + 1 >= k;
-        else is = above + sum >= goal;
-        best = is ? 0x80000000u | (kList - i) : 1u + i;
-      }
-    }
-    const uint32_t found = block_most(best, s);
-    const uint32_t end = found & 0x80000000u ? kList - (found & 0x7fffffffu) : found ? found - 1 : 0;
-    const uint64_t o = s.list[end];
-    if (last) {
-      for (int g = threadIdx.x; g < kGroup; g += kThreads) s.mass[g] = 0;
-      __syncthreads();
-#pragma unroll
-      for (uint32_t q = 0; q < kList / kThreads; ++q)
-        if (q < per && i0 + q <= end && w[q] >= least)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[token_of(static_cast<uint32_t>(s.list[i0 + q])) / kGroup]),
-                    fixed_of(w[q]));
-      __syncthreads();
-    } else {
-      double through = 0.;
-      sum = before;
-#pragma unroll
-      for (uint32_t q = 0; q < kList / kThreads; ++q) {
-        sum += w[q];
-        if (q < per && i0 + q == end) through = sum;
-      }
-      through = block_most(through, s);
-      block_scan(static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0., s, mass);
-      mass += through;
-    }
-    return o;
+    });
+    if (lane == 0) atomicAdd(&s.found, taken);
+    __syncthreads();
+    above = uniform(s.found);
   }
 
-  __device__ __forceinline__ void general(double all_mass) {
-    const double least = static_cast<double>(r.m);
-    uint64_t cut = static_cast<uint64_t>(kNone + 1) << 32;
-    if (r.k && r.p < 1.f) cut = select<true>(cut, false, r.k, 0., false, 0., all_mass);
-    if (r.p < 1.f) {
-      double unused;
-      cut = select<false>(cut, r.k != 0, 0, static_cast<double>(r.p) * all_mass, true, least, unused);
-    } else if (r.k) {
-      double unused;
-      cut = select<true>(cut, false, r.k, 0., true, least, unused);
-    } else {
-      group_masses(cut, least);
+  // The `want`-th in the order of the vocabulary of the tokens with this key.
+  __device__ __forceinline__ uint64_t tied(uint32_t key, int64_t want, uint64_t limit) {
+    uint64_t seen = 0, o = 0;
+    for (int64_t c0 = 0; c0 < a.v && static_cast<int64_t>(seen) < want; c0 += kThreads) {
+      const int64_t c = c0 + threadIdx.x;
+      const float y = c < a.v ? value(static_cast<float>(x[c])) : -INFINITY;
+      const bool is = c < a.v && key_of(y) == key && order_of(y, c) >= limit;
+      uint64_t here;
+      const uint64_t at = seen + block_scan<uint64_t>(is ? 1 : 0, s, here);
+      if (is && static_cast<int64_t>(at) == want) o = order_of(y, c);
+      seen += here;
     }
-    double mine = 0.;
-    if (static_cast<int64_t>(threadIdx.x) < a.n1024) {
-      mine = s.group[threadIdx.x];
-      if (r.k || r.p < 1.f) mine += static_cast<double>(s.mass[threadIdx.x]) / kFixed;
-    }
-    by_groups(mine, cut, least);
+    return block_most(o, s);
   }
 
+  // Where lists come from, in the order in which they are tried: the tokens over what
+  // min-p keeps (all of few); over what about 64, 1024 or k of the 64s' largest reach; the bin of the
+  // k-th token; the bin where the masses reach top-p's. Direct: no list, the cut is known.
+  enum Source { kFloor, kSome, kMore, kNear, kExact, kCount, kMass, kDirect };
+
+  // A list is cut by top-k, top-p and min-p, and the kept masses go to their groups. The
+  // bins that are listed: a pass counts or weighs the tokens in bins of equal width below
+  // the largest (24 units of e^x hold all masses that count; by ranks, what the 64s'
+  // largest span), the next lists the bin that the cut is in and adds up what lies above
+  // it. The first weighing takes all bins that the cut may be in by what its sums can be
+  // off: a mass by 1e-5 of itself (24 units of the exponent, four roundings each) and
+  // 2^-31 (a whole number of them is added). A list that is too long has its keys cut
+  // into bins again.
   __device__ __forceinline__ void run() {
     const uint32_t key = block_most(static_cast<int64_t>(threadIdx.x) < a.n1024 ? a.firsts[row * a.n1024 + threadIdx.x] : 0u, s);
     if (r.bad || key == kNan || key <= kNone) {
@@ -858,43 +863,194 @@ struct Pick {
       return;
     }
     inf = key == kInf;
-    mass_of.top = inf ? 0. : static_cast<double>(value_of(key));
-    double mass = 1.;
+    mass_of.from(inf ? 0. : static_cast<double>(value_of(key)));
+    const double least = static_cast<double>(r.m);
+    double mine = 0., all_mass = 1.;
+    uint64_t cut = 0;
+    double cut_least = 0.;
     if (whole(r)) {
-      const double mine = group_mass();
-      if (r.p >= 1.f) {
-        by_groups(mine, 0, 0.);
-        return;
-      }
-      block_scan(mine, s, mass);
+      mine = group_mass();
+      if (r.p < 1.f) block_scan(mine, s, all_mass);
     }
-    double share;
-    if (!inf) {
-      if (r.k) {
-        if (r.k <= a.n64) {
-          if (from_list(near_top(r.k), true, mass, share)) return;
-          if (from_list(kth_top(r.k), true, mass, share)) return;   // (far from evenly spread)
-        }
-      } else {
-        uint32_t floor = kNone + 1;
-        if (r.m > 0.f) {   // nothing under it is kept
-          const double y = mass_of.top + static_cast<double>(r.t) * log(static_cast<double>(r.m));
-          // (under it by more than the roundings of y, of f and of a mass)
-          const float f = static_cast<float>(y - 1e-6 * (fabs(y) + fabs(mass_of.top) + static_cast<double>(r.t)));
-          floor = f > -INFINITY ? key_of(f) : kNone + 1;
-          if (from_list(floor, true, mass, share)) return;
-        }
-        if (r.p < 1.f) {
-          // Some 64 tokens, and where they hold a good part of the masses some 1000.
-          for (int64_t c = 64; c <= 1024 && c <= a.n64; c *= 16) {
-            const uint32_t least = near_top(c);
-            if (from_list(least > floor ? least : floor, least <= floor, mass, share)) return;
-            if (share < .5 * static_cast<double>(r.p)) break;
+    if (!whole(r) || r.p < 1.f) {
+      uint32_t floor = kNone + 1;   // nothing under it is kept
+      if (r.m > 0.f) {
+        const double y = mass_of.top + static_cast<double>(r.t) * log(least);
+        // (under it by more than the roundings of y, of f and of a mass)
+        const float f = static_cast<float>(y - 1e-6 * (fabs(y) + fabs(mass_of.top) + static_cast<double>(r.t)));
+        if (f > -INFINITY) floor = key_of(f);
+      }
+      Cut q{static_cast<uint64_t>(kNone + 1) << 32, false, false, 0, 0, 0, kNan, 0, 0, top(), 0.f, 0.f};
+      double goal = static_cast<double>(r.p) * all_mass, off = 0.;
+      int source;
+      if (inf) source = r.k ? kCount : r.p < 1.f ? kMass : kDirect;
+      else if (a.v <= kList) source = kFloor;   // all tokens
+      else if (r.k) source = r.k <= a.n64 ? kNear : kCount;
+      else source = r.m > 0.f ? kFloor : kSome;
+      if (source == kDirect) q.limit = static_cast<uint64_t>(floor) << 32;
+      while (true) {
+        double above = 0.;   // of the masses before the list
+        uint32_t n, before = 0;
+        bool complete = true;
+        if (source < kCount) {
+          uint32_t from = floor;
+          if (source != kFloor) {
+            const int64_t c = source == kSome ? 64 : source == kMore ? 1024 : r.k;
+            // (No mass is over 1.)
+            const bool hopeless = !r.k && (goal > 1.25 * static_cast<double>(c) || c > a.n64);
+            from = hopeless ? 0 : source == kExact ? kth_top(c) : near_top(c);
+            if (!r.k && from < floor) from = hopeless ? 0 : floor;
+            complete = r.k || from == floor;
+          } else if (r.k) {
+            from = kNone + 1;
+          }
+          n = from ? candidates(from) : kList + 1;
+          double share = 1.;
+          if (n <= 64 && from_few(n, complete, all_mass, share)) return;
+          if (n <= 64 || n > kList) {
+            if (source == kSome && n <= 64 && share < .5 * static_cast<double>(r.p)) source = kMore;
+            source = source == kFloor ? (r.p < 1.f ? kSome : kDirect) : source == kSome ? kMore : source == kMore ? kMass
+                     : source == kNear ? kExact : kCount;
+            if (source == kDirect) q.limit = static_cast<uint64_t>(floor) << 32;
+            continue;
+          }
+        } else {
+          if (source != kDirect) {
+            if (q.level == 0) {
+              q.by_count = source == kCount;
+              float span = 24.f * r.t;
+              if (q.by_count && !inf) {
+                uint32_t most = 0;
+                for (int64_t i = threadIdx.x; i < a.n64; i += kThreads) {
+                  const uint32_t k = a.tops[row * a.n64 + i];
+                  if (k > kNone) most = ~k > most ? ~k : most;
+                }
+                span = (q.high - value_of(~block_most(most, s))) * 1.25f;
+              }
+              q.width = fminf(static_cast<float>(kBins) / span, 1e30f);
+              q.slope = -1.44269504f * fminf(static_cast<float>(mass_of.inv), 1e30f);
+              off = mass_of.inv > 1e30 ? INFINITY : 1e-5 * all_mass + static_cast<double>(a.v) / 2147483648.;
+            }
+            fill_bins(q);
+            const uint64_t v0 = s.mass[2 * threadIdx.x], v1 = s.mass[2 * threadIdx.x + 1];
+            uint64_t all;
+            const uint64_t upto = block_scan<uint64_t>(v0 + v1, s, all);
+            const double base = uniform(s.value);   // the masses above the bins, from level 1 on
+            const int64_t k = r.k - (q.level ? static_cast<int64_t>(uniform(s.found)) : 0);
+            const double unit = q.level ? 1. / kFixed : 1. / 2147483648.;
+            const double low = q.level ? goal - base : goal - off, high = q.level ? low : goal + off;
+            const bool count = q.by_count;
+            const uint32_t b0 = bin_where(v0, v1, upto, [&](uint64_t m) { return count ? static_cast<int64_t>(m) >= k : static_cast<double>(m) * unit >= low; });
+            uint32_t b1 = b0;
+            if (!count && q.level == 0) {
+              b1 = bin_where(v0, v1, upto, [&](uint64_t m) { return static_cast<double>(m) * unit >= high; });
+              if (static_cast<double>(all) * unit < high) b1 = kBins - 1;
+            }
+            if (q.level == 0) {
+              q.first = b0;
+              q.final = b1;
+              q.lo = 0;
+              q.hi = kNan;
+            } else {
+              const uint32_t h = q.hi - (b0 << q.shift), wide = (uint32_t{1} << q.shift) - 1;
+              q.lo = h - q.lo > wide ? h - wide : q.lo;
+              q.hi = h;
+            }
+          }
+          q.direct = source == kDirect;
+          uint32_t low, most;
+          gather(q, q.direct ? least : 0., before, low, most);
+          n = uniform(s.n);
+          if (q.direct) {
+            mine = static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0.;
+            cut = q.limit;
+            cut_least = least;
+            break;
+          }
+          above = sum_of_groups();
+          if (n > kList) {
+            q.hi = block_most(most, s);
+            q.lo = ~block_most(~low, s);
+            ++q.level;
+            q.shift = 0;
+            while ((q.hi - q.lo) >> q.shift >= kBins) ++q.shift;
+            if (threadIdx.x == 0) s.value = above;
+            __syncthreads();
+            if (q.lo != q.hi) continue;
+            // more equal values than the list holds
+            const double w = weight(value_of(q.hi));
+            double want = static_cast<double>(n);
+            if (source == kCount) {
+              want = static_cast<double>(r.k - before);
+              goal = r.p < 1.f ? static_cast<double>(r.p) * (above + want * w) : INFINITY;
+            }
+            if (goal > above) want = fmin(want, ceil((goal - above) / w));
+            const uint64_t o = tied(q.hi, static_cast<int64_t>(fmax(want, 1.)), q.limit);
+            q.level = 0;
+            if (goal > above) {
+              source = kDirect;
+              q.limit = o;
+            } else {   // top-p's cut is among the ones above
+              source = kMass;
+              q.limit = o;
+              all_mass = goal / static_cast<double>(r.p);
+            }
+            continue;
           }
         }
+        // the list, and its cut
+        const uint32_t size = sort(n), per = size > kThreads ? 2 : 1, i0 = threadIdx.x * per;
+        uint32_t end = n;
+        if (r.k && source != kMass && static_cast<int64_t>(end) > r.k - before) end = static_cast<uint32_t>(r.k - before);
+        double w[2], all;
+        w[0] = i0 < end ? weight(listed(s.list[i0])) : 0.;
+        w[1] = per == 2 && i0 + 1 < end ? weight(listed(s.list[i0 + 1])) : 0.;
+        const double sum = above + block_scan(w[0] + w[1], s, all) - (w[0] + w[1]);
+        if (r.k && source != kMass) {
+          all_mass = above + all;
+          goal = static_cast<double>(r.p) * all_mass;
+        }
+        if (source == kCount && r.p < 1.f && !(goal > above)) {
+          q.limit = uniform(s.list[end - 1]);
+          source = kMass;
+          q.level = 0;
+          continue;
+        }
+        const double limit = r.p < 1.f ? goal : INFINITY;
+        uint32_t kept = 0;
+        if (i0 < end && ((i0 == 0 && before == 0) || (sum < limit && w[0] >= least))) kept = i0 + 1;
+        if (per == 2 && i0 + 1 < end && sum + w[0] < limit && w[1] >= least) kept = i0 + 2;
+        end = block_most(kept, s);
+        if (source < kCount && !complete && end == n) {   // it may go on below the list
+          source = source == kSome && all >= .5 * goal ? kMore : kMass;
+          continue;
+        }
+        if (end == 0) {   // min-p's cut is above the list
+          source = kDirect;
+          q.limit = static_cast<uint64_t>(floor) << 32;
+          continue;
+        }
+        cut = uniform(s.list[end - 1]);
+        for (int g = threadIdx.x; g < kGroup; g += kThreads) s.mass[g] = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i)
+          if (i < per && i0 + i < end && w[i] > 0.) {
+            // (a mass of next to nothing is one all the same, u may be 0: the highest bit, which
+            // 2048 masses do not reach)
+            const unsigned long long f = fixed_of(w[i]);
+            auto* m = reinterpret_cast<unsigned long long*>(&s.mass[token_of(static_cast<uint32_t>(s.list[i0 + i])) / kGroup]);
+            if (f) atomicAdd(m, f);
+            else atomicOr(m, 1ull << 63);
+          }
+        __syncthreads();
+        const uint64_t m = s.mass[threadIdx.x];
+        mine = static_cast<double>(m & ~(uint64_t{1} << 63)) / kFixed + (m >> 63 ? 1e-300 : 0.);
+        if (source >= kCount && static_cast<int64_t>(threadIdx.x) < a.n1024) mine += s.group[threadIdx.x];
+        break;
       }
     }
-    general(mass);
+    by_groups(mine, cut, cut_least);
   }
 };
 
@@ -904,7 +1060,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
   const int64_t row = blockIdx.x;
   load_powers(s.powers);   // (barriers follow before they are read)
   const Row r = row_of(a, row);
-  Pick<E> p{a, s, row, r, static_cast<const E*>(a.x) + row * a.ldx, Exp{s.powers, 0., r.scale}, false};
+  Pick<E> p{a, s, row, r, static_cast<const E*>(a.x) + row * a.ldx, Exp(s.powers, r.t), false};
   p.run();
 }
 
