@@ -176,11 +176,61 @@ __device__ __forceinline__ bool whole(const Row& r) {
   return !r.bad && !r.first && r.k == 0 && (r.p < 1.f || r.m <= 0.f);
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int d = 32; d; d /= 2) x += __shfl_xor(x, d);
-  return x;
+// Over a wave's lanes, by moves between neighbouring lanes (no LDS): each lane's value
+// and those before it; and of 16 lanes alone.
+struct Sum {
+  template <typename T>
+  __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
+};
+struct Most {   // of whole numbers from 0 on
+  template <typename T>
+  __device__ __forceinline__ T operator()(T a, T b) const { return a > b ? a : b; }
+};
+template <int MOVE, int ROWS, typename T>
+__device__ __forceinline__ T moved(T v) {   // 0 where nothing is moved to
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), MOVE, ROWS, 0xf, false));
+  } else {
+    const auto u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), MOVE, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), MOVE, ROWS, 0xf, false);
+    return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+  }
 }
+template <typename Op, typename T>
+__device__ __forceinline__ T row_scan(T v, Op op) {
+  v = op(v, moved<0x111, 0xf>(v));   // from 1, 2, 4 and 8 lanes before
+  v = op(v, moved<0x112, 0xf>(v));
+  v = op(v, moved<0x114, 0xf>(v));
+  return op(v, moved<0x118, 0xf>(v));
+}
+template <typename Op, typename T>
+__device__ __forceinline__ T wave_scan(T v, Op op) {
+  v = row_scan(v, op);
+  v = op(v, moved<0x142, 0xa>(v));   // a row's last to the row after, then to the two after
+  return op(v, moved<0x143, 0xc>(v));
+}
+// The largest of each LANES (8 or 16) neighbouring lanes, in all of them.
+template <int LANES>
+__device__ __forceinline__ uint32_t most_of(uint32_t v) {
+  const Most op;
+  v = op(v, moved<0xb1, 0xf>(v));    // from the lane 1 and then 2 apart,
+  v = op(v, moved<0x4e, 0xf>(v));
+  v = op(v, moved<0x141, 0xf>(v));   // the mirrored ones of 8 and of 16
+  return LANES == 8 ? v : op(v, moved<0x140, 0xf>(v));
+}
+template <typename T>
+__device__ __forceinline__ T lane_of(T v, int lane) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else {
+    const auto u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane);
+    return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+  }
+}
+__device__ __forceinline__ double wave_sum(double x) { return lane_of(wave_scan(x, Sum{}), 63); }
 
 // A lane's 16 of a group's tokens, kPer neighbouring ones a load; -infinity past the
 // row's end. Fetched as they lie in memory, so that a next group's can be under way.
@@ -245,22 +295,14 @@ __global__ __launch_bounds__(256) void sample_groups_kernel(SampleArgs a) {
       m = max3(m, y[3], y[3]);
     }
     uint32_t key = bad ? kNan : key_of(m);
-#pragma unroll
-    for (int d = 1; d < kLanes; d *= 2) {
-      const uint32_t o = __shfl_xor(key, d);
-      key = o > key ? o : key;
-    }
+    key = most_of<kLanes>(key);
     const int64_t at = group * (kGroup / 64) + i * T::kPer + lane / kLanes;
     if (lane % kLanes == 0 && at < a.n64) a.tops[row * a.n64 + at] = key;
     nan = nan || key == kNan;
     top = max3(top, value_of(key), top);
   }
   uint32_t key = nan ? kNan : key_of(top);
-#pragma unroll
-  for (int d = kLanes; d < 64; d *= 2) {
-    const uint32_t o = __shfl_xor(key, d);
-    key = o > key ? o : key;
-  }
+  key = lane_of(wave_scan(key, Most{}), 63);
   if (lane == 0) a.firsts[row * a.n1024 + group] = key;
   const Row r = row_of(a, row);
   if (!whole(r)) return;
@@ -322,52 +364,6 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
-// Over the workgroup: the largest.
-template <typename T>
-__device__ __forceinline__ T block_most(T v, Shared& s) {
-  T* waves = reinterpret_cast<T*>(s.waves[0]);
-#pragma unroll
-  for (int d = 32; d; d /= 2) {
-    const T o = __shfl_xor(v, d);
-    v = o > v ? o : v;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) v = waves[w] > v ? waves[w] : v;
-  return uniform(v);
-}
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const T o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
-}
-// Sum of the values up to this thread's, and of all.
-template <typename T>
-__device__ __forceinline__ T block_scan(T v, Shared& s, T& all) {
-  T* waves = reinterpret_cast<T*>(s.waves[1]);
-  const int wave = threadIdx.x >> 6;
-  v = wave_scan(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) waves[wave] = v;
-  __syncthreads();
-  T before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w == wave) before = all;
-    all += waves[w];
-  }
-  all = uniform(all);
-  return before + v;
-}
-
 // One row's picking; every thread of the workgroup calls each member.
 template <typename E>
 struct Pick {
@@ -378,22 +374,48 @@ struct Pick {
   const E* x;
   Exp mass_of;
   bool inf;   // the largest is +infinity: those tokens count as 0, the others as -infinity
+  uint32_t tops[2];   // this thread's first two of the 64s' largest keys (most have no more)
+  int turn = 0;       // of two places in LDS for the waves' values: a barrier a use is enough
+
+  // Over the workgroup: the largest; the sum of the values up to this thread's, and of all.
+  template <typename T>
+  __device__ __forceinline__ T block_most(T v) {
+    T* waves = reinterpret_cast<T*>(s.waves[turn]);
+    turn ^= 1;
+    v = wave_scan(v, Most{});
+    if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return lane_of(row_scan(waves[threadIdx.x % kWaves], Most{}), kWaves - 1);
+  }
+  template <typename T>
+  __device__ __forceinline__ T block_scan(T v, T& all) {
+    T* waves = reinterpret_cast<T*>(s.waves[turn]);
+    turn ^= 1;
+    v = wave_scan(v, Sum{});
+    const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    if ((threadIdx.x & 63) == 63) waves[wave] = v;
+    __syncthreads();
+    const T upto = row_scan(waves[threadIdx.x % kWaves], Sum{});
+    all = lane_of(upto, kWaves - 1);
+    return wave ? v + lane_of(upto, wave - 1) : v;
+  }
 
   __device__ __forceinline__ float top() const { return static_cast<float>(mass_of.top); }
   __device__ __forceinline__ float value(float y) const { return inf ? (y == INFINITY ? 0.f : -INFINITY) : y; }
   __device__ __forceinline__ double weight(float y) const { return mass_of(y); }
 
-  __device__ __forceinline__ void none() const {
-    if (threadIdx.x) return;
-    a.token[row] = -1;
-    if (a.logprob) a.logprob[row] = NAN;
+  // What the thread that finds the token sets, for finish().
+  int64_t token = INT64_MIN;   // none
+  double log_mass = 0., of = 1.;   // the log of its mass, the sum of the kept ones
+  __device__ __forceinline__ void found(int64_t c, float y, double mass) {
+    token = c;
+    log_mass = (static_cast<double>(y) - mass_of.top) / static_cast<double>(r.t);
+    of = mass;
   }
-  __device__ __forceinline__ void done(int64_t c, double logp) const {
-    a.token[row] = c;
-    if (a.logprob) a.logprob[row] = static_cast<float>(logp);
-  }
-  __device__ __forceinline__ void done(int64_t c, float y, double mass) const {
-    done(c, (static_cast<double>(y) - mass_of.top) / static_cast<double>(r.t) - log(mass));
+  __device__ __forceinline__ void finish() const {
+    if (token == INT64_MIN) return;
+    a.token[row] = token;
+    if (a.logprob) a.logprob[row] = static_cast<float>(log_mass - log(of));
   }
 
   // The thread in whose share a sum crosses `target`: the first whose sum up to it is
@@ -402,7 +424,7 @@ struct Pick {
   __device__ __forceinline__ int crossing(double share, double upto, double target) {
     uint32_t mine = 0;   // larger: earlier
     if (share > 0.) mine = upto > target ? 0x80000000u | (kThreads - threadIdx.x) : 1u + threadIdx.x;
-    const uint32_t best = block_most(mine, s);
+    const uint32_t best = block_most(mine);
     const int t = best & 0x80000000u ? kThreads - static_cast<int>(best & 0x7fffffffu) : best ? static_cast<int>(best) - 1 : 0;
     if (static_cast<int>(threadIdx.x) == t) s.value = upto - share;
     __syncthreads();
@@ -414,7 +436,7 @@ struct Pick {
   // least `least`.
   __device__ __forceinline__ void by_groups(double mine, uint64_t cut, double least) {
     double mass, all;
-    const double upto = block_scan(mine, s, mass);
+    const double upto = block_scan(mine, mass);
     const double target = static_cast<double>(r.u) * mass;
     const int64_t c = crossing(mine, upto, target) * int64_t{kGroup} + threadIdx.x;
     const double before = uniform(s.value);
@@ -425,9 +447,9 @@ struct Pick {
       w = weight(y);
       if (order_of(y, c) < cut || w < least) w = 0.;
     }
-    const double sum = before + block_scan(w, s, all);
+    const double sum = before + block_scan(w, all);
     const int t = crossing(w, sum, target);
-    if (static_cast<int>(threadIdx.x) == t) done(c, y, mass);
+    if (static_cast<int>(threadIdx.x) == t) found(c, y, mass);
   }
 
   // The mass of thread t's group, all tokens counted.
@@ -443,38 +465,42 @@ struct Pick {
   __device__ __forceinline__ void largest(uint32_t key) {
     uint32_t mine = 0;
     if (static_cast<int64_t>(threadIdx.x) < a.n1024 && a.firsts[row * a.n1024 + threadIdx.x] == key) mine = kThreads - threadIdx.x;
-    const int64_t group = kThreads - static_cast<int64_t>(block_most(mine, s));
+    const int64_t group = kThreads - static_cast<int64_t>(block_most(mine));
     const int64_t c = group * kGroup + threadIdx.x;
     mine = c < a.v && key_of(static_cast<float>(x[c])) == key ? kThreads - threadIdx.x : 0;
-    const int t = kThreads - static_cast<int>(block_most(mine, s));
-    if (static_cast<int>(threadIdx.x) == t) done(c, 0.);
+    const int t = kThreads - static_cast<int>(block_most(mine));
+    if (static_cast<int>(threadIdx.x) == t) token = c;
   }
 
   // ---- few tokens: lists
-  // A key that at least k of the 64s' largest keys reach, and not many more: from their
-  // counts in bins of equal width.
-  __device__ __forceinline__ uint32_t near_top(int64_t k) {
-    const uint32_t* tops = a.tops + row * a.n64;
+  template <typename F>
+  __device__ __forceinline__ void each_top(F&& f) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) f(static_cast<int64_t>(threadIdx.x) + k * kThreads, tops[k]);
+    for (int64_t i = threadIdx.x + 2 * int64_t{kThreads}; i < a.n64; i += kThreads) f(i, a.tops[row * a.n64 + i]);
+  }
+  // The smallest of them over -infinity.
+  __device__ __forceinline__ float least_top() {
     uint32_t most = 0;   // of the complements
-    for (int64_t i = threadIdx.x; i < a.n64; i += kThreads) {
-      const uint32_t key = tops[i];
-      if (key > kNone) most = ~key > most ? ~key : most;
-    }
+    each_top([&](int64_t, uint32_t key) { most = key > kNone && ~key > most ? ~key : most; });
+    return value_of(~block_most(most));
+  }
+  // A key that at least k of them reach, and not many more: from their counts in bins of
+  // equal width.
+  __device__ __forceinline__ uint32_t near_top(int64_t k) {
     for (int b = threadIdx.x; b < kBins; b += kThreads) s.count[b] = 0;
-    const float high = top(), low = value_of(~block_most(most, s));
+    const float high = top(), low = least_top();
     const float width = static_cast<float>(kBins - 1) / (high - low);   // (none: infinite)
-    auto bin = [&](float y) { return static_cast<uint32_t>(fminf(fmaxf((high - y) * width, 0.f), kBins - 1.f)); };
-    for (int64_t i = threadIdx.x; i < a.n64; i += kThreads) {
-      const uint32_t key = tops[i];
-      if (key > kNone) atomicAdd(&s.count[bin(value_of(key))], 1u);
-    }
+    each_top([&](int64_t, uint32_t key) {
+      if (key > kNone)
+        atomicAdd(&s.count[static_cast<uint32_t>(fminf(fmaxf((high - value_of(key)) * width, 0.f), kBins - 1.f))], 1u);
+    });
     __syncthreads();
     const int b = 2 * static_cast<int>(threadIdx.x);
     const uint32_t c0 = s.count[b], c1 = s.count[b + 1];
     uint32_t all;
-    const uint32_t upto = block_scan(c0 + c1, s, all);
-    if (threadIdx.x == 0) s.found = kBins - 1;
-    __syncthreads();
+    const uint32_t upto = block_scan(c0 + c1, all);
+    if (threadIdx.x == 0 && all < k) s.found = kBins - 1;
     if (upto >= k && upto - c0 - c1 < k) s.found = upto - c1 >= k ? b : b + 1;
     __syncthreads();
     // its lower end, and a little less for the roundings
@@ -483,26 +509,25 @@ struct Pick {
     const float less = end - 1e-6f * (fabsf(high) + fabsf(end));
     return less > -INFINITY && found < kBins - 1 ? key_of(less) : kNone + 1;
   }
-  // The k-th largest of the 64s' largest keys (1 <= k <= n64), 11, 11 and 10 bits at a time.
+  // The k-th largest of them (1 <= k <= n64), 11, 11 and 10 bits at a time.
   __device__ __forceinline__ uint32_t kth_top(int64_t k) {
-    const uint32_t* tops = a.tops + row * a.n64;
     uint32_t prefix = 0, mask = 0;
     uint32_t rank = static_cast<uint32_t>(k);
+#pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       const uint32_t digits = pass == 2 ? 1023 : 2047;
       __syncthreads();
       for (int b = threadIdx.x; b < kBins; b += kThreads) s.count[b] = 0;
       __syncthreads();
-      for (int64_t i = threadIdx.x; i < a.n64; i += kThreads) {
-        const uint32_t key = tops[i];
-        if ((key & mask) == prefix) atomicAdd(&s.count[key >> shift & digits], 1u);
-      }
+      each_top([&](int64_t i, uint32_t key) {
+        if (i < a.n64 && (key & mask) == prefix) atomicAdd(&s.count[key >> shift & digits], 1u);
+      });
       __syncthreads();
       const int b = kBins - 2 - 2 * static_cast<int>(threadIdx.x);   // bins b + 1, then b
       const uint32_t hi = s.count[b + 1], lo = s.count[b];
       uint32_t all;
-      const uint32_t upto = block_scan(hi + lo, s, all);
+      const uint32_t upto = block_scan(hi + lo, all);
       if (upto >= rank && upto - hi - lo < rank) {
         const uint32_t before = upto - hi - lo;
         const bool in_hi = before + hi >= rank;
@@ -518,48 +543,75 @@ struct Pick {
     return prefix;
   }
 
-  // Puts o into the list where `take`.
-  __device__ __forceinline__ void append(bool take, uint64_t o) {
-    const uint64_t who = __ballot(take);
-    if (!who) return;
+  // Puts a lane's N neighbouring tokens from c on into the list where `take`.
+  template <int N>
+  __device__ __forceinline__ void append(const bool (&take)[N], const float (&y)[N], int64_t c) {
+    uint64_t who[N];
+    uint32_t n = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      who[k] = __ballot(take[k]);
+      n += static_cast<uint32_t>(__popcll(who[k]));
+    }
+    if (!n) return;
     const int lane = threadIdx.x & 63;
-    uint32_t base = 0;
-    if (lane == 0) base = atomicAdd(&s.n, static_cast<uint32_t>(__popcll(who)));
-    base = __shfl(base, 0);
-    const uint32_t place = base + static_cast<uint32_t>(__popcll(who & ((uint64_t{1} << lane) - 1)));
-    if (take && place < kList) s.list[place] = o;
+    uint32_t place = 0;
+    if (lane == 0) place = atomicAdd(&s.n, n);
+    place = __builtin_amdgcn_readfirstlane(place);
+    const uint64_t under = (uint64_t{1} << lane) - 1;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const uint32_t at = place + static_cast<uint32_t>(__popcll(who[k] & under));
+      if (take[k] && at < kList) s.list[at] = order_of(y[k], c + k);
+      place += static_cast<uint32_t>(__popcll(who[k]));
+    }
   }
 
-  // Tokens with keys from `least` on; how many there are (over kList: too many).
+  // Tokens with keys from `least` on, from the 64s whose largest reach it, several of
+  // them a load; how many tokens there are (over kList: too many).
   __device__ __forceinline__ uint32_t candidates(uint32_t least) {
+    using T = Tokens<E>;
     __syncthreads();
     if (threadIdx.x == 0) {
       s.n = 0;
       s.found = 0;
     }
     __syncthreads();
-    const uint32_t* tops = a.tops + row * a.n64;
-    for (int64_t i = threadIdx.x; i < a.n64; i += kThreads)
-      if (tops[i] >= least) {
-        const uint32_t at = atomicAdd(&s.found, 1u);
-        if (at < 2 * kBins) s.count[at] = static_cast<uint32_t>(i);
-      }
+    each_top([&](int64_t i, uint32_t key) {
+      if (i >= a.n64 || key < least) return;
+      const uint32_t at = atomicAdd(&s.found, 1u);
+      if (at < 2 * kBins) s.count[at] = static_cast<uint32_t>(i);
+    });
     __syncthreads();
     const uint32_t spans = uniform(s.found);
     if (spans > 2 * kBins) return kList + 1;
-    constexpr int kMany = 8;   // under way at a time
-    for (uint32_t i0 = threadIdx.x >> 6; i0 < spans; i0 += kWaves * kMany) {
-      float y[kMany];
+    constexpr uint32_t kLanes = 64 / T::kPer, kMany = 2;   // lanes of a span; loads under way
+    const uint32_t lane = threadIdx.x & 63, step = 64 / kLanes;
+    for (uint32_t i0 = (threadIdx.x >> 6) * step; i0 < spans; i0 += kWaves * step * kMany) {
+      E w[kMany][T::kPer];
       int64_t c[kMany];
 #pragma unroll
-      for (int q = 0; q < kMany; ++q) {
-        const uint32_t i = i0 + q * kWaves;
-        c[q] = s.count[i < spans ? i : i0] * int64_t{64} + (threadIdx.x & 63);
-        y[q] = static_cast<float>(x[c[q] < a.v ? c[q] : 0]);
-        if (i >= spans) c[q] = a.v;
+      for (uint32_t q = 0; q < kMany; ++q) {
+        const uint32_t i = i0 + q * kWaves * step + lane / kLanes;
+        c[q] = i < spans ? s.count[i] * int64_t{64} + lane % kLanes * T::kPer : a.v;
+        if (c[q] + T::kPer <= a.v) {
+          __builtin_memcpy(w[q], x + c[q], sizeof w[q]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < T::kPer; ++k) w[q][k] = c[q] + k < a.v ? x[c[q] + k] : static_cast<E>(-INFINITY);
+        }
       }
 #pragma unroll
-      for (int q = 0; q < kMany; ++q) append(c[q] < a.v && key_of(y[q]) >= least, order_of(y[q], c[q]));
+      for (uint32_t q = 0; q < kMany; ++q) {
+        float y[T::kPer];
+        bool take[T::kPer];
+#pragma unroll
+        for (int k = 0; k < T::kPer; ++k) {
+          y[k] = static_cast<float>(w[q][k]);
+          take[k] = c[q] + k < a.v && key_of(y[k]) >= least;
+        }
+        append(take, y, c[q]);
+      }
     }
     __syncthreads();
     return uniform(s.n);
@@ -608,53 +660,56 @@ struct Pick {
   __device__ __forceinline__ static float listed(uint64_t o) { return value_of(static_cast<uint32_t>(o >> 32)); }
 
   // Up to 64 candidates by one wave (the others wait): each entry's rank is how many are
-  // over it. The token, or false where the cut is not among them; `share`: of all masses.
-  __device__ __forceinline__ bool from_few(uint32_t n, bool complete, double all_mass, double& share) {
+  // over it. The token, or false where the cut is not among them.
+  __device__ __forceinline__ bool from_few(uint32_t n, bool complete, double all_mass) {
     if (threadIdx.x < 64) {
       const uint32_t i = threadIdx.x;
       uint64_t o = i < n ? s.list[i] : 0;
+      wave_sync();
+      s.list[i] = o;
+      wave_sync();
       uint32_t rank = 0;
-      for (uint32_t j = 0; j < n; ++j) rank += s.list[j] > o;
+      for (uint32_t j = 0; j < n; j += 8)
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) rank += s.list[j + q] > o;
       wave_sync();
       if (i < n) s.list[rank] = o;
       wave_sync();
       const uint32_t most = r.k && r.k < n ? static_cast<uint32_t>(r.k) : n;
       o = i < most ? s.list[i] : 0;
       const double w = i < most ? weight(listed(o)) : 0.;
-      const double upto = wave_scan(w), all = __shfl(upto, 63);
+      const double upto = wave_scan(w, Sum{}), all = lane_of(upto, 63);
       const double limit = r.p < 1.f ? static_cast<double>(r.p) * (r.k ? all : all_mass) : INFINITY;
       const bool keep = i < most && (i == 0 || (upto - w < limit && w >= static_cast<double>(r.m)));
       const uint32_t count = static_cast<uint32_t>(__popcll(__ballot(keep)));
-      const bool found = r.k || complete || count < n;
-      if (found) {
+      const bool is = r.k || complete || count < n;
+      if (is) {
         // in the order of the vocabulary
-        if (keep) s.list[i] = o << 32 | o >> 32;
+        const uint64_t mine = keep ? o << 32 | o >> 32 : 0;
+        s.list[i] = mine;
         wave_sync();
-        const uint64_t mine = keep ? s.list[i] : 0;
         uint32_t place = 0;
-        for (uint32_t j = 0; j < count; ++j) place += s.list[j] > mine;
+        for (uint32_t j = 0; j < count; j += 8)
+#pragma unroll
+          for (uint32_t q = 0; q < 8; ++q) place += s.list[j + q] > mine;
         wave_sync();
         if (keep) s.list[place] = mine;
         wave_sync();
         const uint64_t e = i < count ? s.list[i] : 0;
         const float y = value_of(static_cast<uint32_t>(e));
         const double m = i < count ? weight(y) : 0.;
-        const double sum = wave_scan(m), mass = __shfl(sum, 63);
+        const double sum = wave_scan(m, Sum{}), mass = lane_of(sum, 63);
         const double target = static_cast<double>(r.u) * mass;
         const uint64_t over = __ballot(m > 0. && sum > target), any = __ballot(m > 0.);
         const int t = over ? __ffsll(static_cast<unsigned long long>(over)) - 1 : 63 - __clzll(static_cast<long long>(any));
-        if (static_cast<int>(i) == t) done(token_of(static_cast<uint32_t>(e >> 32)), y, mass);
+        if (static_cast<int>(i) == t) found(token_of(static_cast<uint32_t>(e >> 32)), y, mass);
       }
-      if (i == 0) {
-        s.found = found;
-        s.value = all;
-      }
+      if (i == 0) s.found = is;
     }
     __syncthreads();
-    share = uniform(s.value) / all_mass;
-    const bool found = uniform(s.found);
+    const bool is = uniform(s.found);
     __syncthreads();
-    return found;
+    return is;
   }
 
   // ---- many tokens: passes over the whole row
@@ -692,46 +747,64 @@ struct Pick {
 
   __device__ __forceinline__ double sum_of_groups() {
     double all;
-    block_scan(static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0., s, all);
+    block_scan(static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0., all);
     return all;
   }
 
-  // What a pass over the row looks at: the tokens from `limit` on in descending order;
-  // where `direct` all of them are taken, else those in bins above `first` or with keys
-  // above `hi`, and the members, in bins from `first` to `final` with keys from `lo`
-  // to `hi`, are listed.
+  // What a pass over the row looks at: the tokens from `limit` on in descending order,
+  // where there is one; of these it takes the ones over `hi` and lists the members, from
+  // `lo` to `hi`.
   struct Cut {
     uint64_t limit;
-    bool direct, by_count;
-    uint32_t first, final, lo, hi;
+    bool limited, by_count;
+    float lo, hi;
+    uint32_t most;              // hi's key, from which the bins of keys count down
     int level, shift;
-    float high, width, slope;   // bins of equal width below the largest; of log2 of a mass
+    float high, width, slope, unit;   // bins of equal width below the largest; of log2 of a mass; what 1 weighs
   };
-  __device__ __forceinline__ uint32_t bin_of(const Cut& q, float y) const {
+  __device__ __forceinline__ static uint32_t bin_of(const Cut& q, float y) {
     return static_cast<uint32_t>(fminf((q.high - y) * q.width, kBins - 1.f));
   }
+  // The largest finite key whose value is in bin b or a later one (0: none), 64 of them
+  // looked at at a time.
+  __device__ __forceinline__ static uint32_t last_of(const Cut& q, uint32_t b) {
+    uint32_t at = kNone + 1, n = key_of(q.high) - at;   // `at` is one, none of the n after it known
+    if (bin_of(q, value_of(at)) < b) return 0;
+    const uint32_t lane = threadIdx.x & 63;
+    while (n) {
+      const uint32_t step = (n + 63) / 64, past = (lane + 1) * step < n ? (lane + 1) * step : n;
+      const uint32_t is = static_cast<uint32_t>(__popcll(__ballot(bin_of(q, value_of(at + past)) >= b)));
+      const uint32_t move = is * step < n ? is * step : n;
+      at += move;
+      n = n - move < step - 1 ? n - move : step - 1;
+    }
+    return at;
+  }
 
-  // Counts or weighs the members in bins. The first weighing is in 32 bits.
+  // Counts or weighs the members in bins: all in 32 bits first, then (and by keys) in 64.
   __device__ __forceinline__ void fill_bins(const Cut& q) {
     __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += kThreads) s.mass[b] = 0;
+    for (int b = threadIdx.x; b < kBins; b += kThreads) {
+      s.mass[b] = 0;
+      s.count[b] = 0;
+    }
     __syncthreads();
     each([&](int64_t, int, int64_t c, const float(&y)[4]) {
+      if (q.level == 0) {
 #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (!(y[k] >= q.lo) || (q.limited && order_of(y[k], c + k) < q.limit)) continue;
+          const uint32_t w = q.by_count ? 1u : static_cast<uint32_t>(__builtin_amdgcn_exp2f((q.high - y[k]) * q.slope) * q.unit);
+          atomicAdd(&s.count[bin_of(q, y[k])], w);
+        }
+        return;
+      }
+#pragma unroll 1
       for (int k = 0; k < 4; ++k) {
-        if (!(y[k] > -INFINITY) || order_of(y[k], c + k) < q.limit) continue;
-        uint32_t b = bin_of(q, y[k]);
-        if (q.level) {
-          const uint32_t key = key_of(y[k]);
-          if (b < q.first || b > q.final || key < q.lo || key > q.hi) continue;
-          b = (q.hi - key) >> q.shift;
-        }
-        unsigned long long one = 1;
-        if (!q.by_count) {
-          if (q.level) one = fixed_of(weight(y[k]));
-          else one = static_cast<uint32_t>(__builtin_amdgcn_exp2f((q.high - y[k]) * q.slope) * 2147483648.f);
-        }
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), one);
+        const float v = k < 2 ? (k ? y[1] : y[0]) : k == 2 ? y[2] : y[3];
+        if (!(v >= q.lo && v <= q.hi) || (q.limited && order_of(v, c + k) < q.limit)) continue;
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[(q.most - key_of(v)) >> q.shift]),
+                  q.by_count ? 1ull : fixed_of(weight(v)));
       }
     });
     __syncthreads();
@@ -747,15 +820,15 @@ struct Pick {
     else if (v1 && reached(upto)) mine = 0x80000000u | (kBins - b - 1);
     else if (v1) mine = 2u + b;
     else if (v0) mine = 1u + b;
-    const uint32_t best = block_most(mine, s);
+    const uint32_t best = block_most(mine);
     return best & 0x80000000u ? kBins - (best & 0x7fffffffu) : best ? best - 1 : 0;
   }
 
   // Adds up the masses of at least `least` of the tokens taken, by group in s.group, and
-  // lists the members: s.n of them, `above` their number; the range of their keys. The
-  // taken ones are put together and weighed 64 at a time, so that the others cost no
+  // lists the members, s.n of them; `above`: how many are taken, `low` and `most`: this
+  // thread's smallest and largest member. The taken ones are put together and weighed 64 at a time, so that the others cost no
   // exponential.
-  __device__ __forceinline__ void gather(const Cut& q, double least, uint32_t& above, uint32_t& low, uint32_t& most) {
+  __device__ __forceinline__ void gather(const Cut& q, double least, uint32_t& above, float& low, float& most) {
     __syncthreads();
     if (threadIdx.x == 0) s.n = s.found = 0;
     __syncthreads();
@@ -764,43 +837,31 @@ struct Pick {
     float* ring = s.ring[threadIdx.x >> 6];
     uint32_t from = 0, held = 0, taken = 0;
     double sum = 0.;
-    low = kNan;
-    most = 0;
+    low = INFINITY;
+    most = -INFINITY;
     each([&](int64_t g, int unit, int64_t c, const float(&y)[4]) {
-      uint64_t members[4], any = 0;
+      bool member[4], any = false;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t key = key_of(y[k]);
-        bool take = y[k] > -INFINITY && order_of(y[k], c + k) >= q.limit, member = false;
-        if (!q.direct) {
-          const uint32_t b = bin_of(q, y[k]);
-          const bool within = take && b >= q.first && b <= q.final;
-          member = within && key >= q.lo && key <= q.hi;
-          take = take && (b < q.first || (within && key > q.hi));
+        bool take = y[k] > q.hi;
+        member[k] = y[k] >= q.lo && !take;
+        if (q.limited) {
+          const bool is = order_of(y[k], c + k) >= q.limit;
+          take = take && is;
+          member[k] = member[k] && is;
         }
-        if (member) {
-          low = key < low ? key : low;
-          most = key > most ? key : most;
-        }
-        members[k] = __ballot(member);
-        any |= members[k];
+        any = any || member[k];
         const uint64_t who = __ballot(take);
         if (take) ring[(from + held + static_cast<uint32_t>(__popcll(who & under))) % kRing] = y[k];
         held += static_cast<uint32_t>(__popcll(who));
       }
-      if (any) {
-        uint32_t n = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) n += static_cast<uint32_t>(__popcll(members[k]));
-        uint32_t place = 0;
-        if (lane == 0) place = atomicAdd(&s.n, n);
-        place = __shfl(place, 0);
+      if (__any(any)) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t at = place + static_cast<uint32_t>(__popcll(members[k] & under));
-          if ((members[k] >> lane & 1) && at < kList) s.list[at] = order_of(y[k], c + k);
-          place += static_cast<uint32_t>(__popcll(members[k]));
+          low = member[k] ? fminf(low, y[k]) : low;
+          most = member[k] ? fmaxf(most, y[k]) : most;
         }
+        append(member, y, c);
       }
       while (held >= (unit < 3 ? 64u : 1u)) {
         const uint32_t n = held < 64 ? held : 64;
@@ -832,236 +893,275 @@ struct Pick {
       const float y = c < a.v ? value(static_cast<float>(x[c])) : -INFINITY;
       const bool is = c < a.v && key_of(y) == key && order_of(y, c) >= limit;
       uint64_t here;
-      const uint64_t at = seen + block_scan<uint64_t>(is ? 1 : 0, s, here);
+      const uint64_t at = seen + block_scan<uint64_t>(is ? 1 : 0, here);
       if (is && static_cast<int64_t>(at) == want) o = order_of(y, c);
       seen += here;
     }
-    return block_most(o, s);
+    return block_most(o);
   }
 
-  // Where lists come from, in the order in which they are tried: the tokens over what
-  // min-p keeps (all of few); over what about 64, 1024 or k of the 64s' largest reach; the bin of the
-  // k-th token; the bin where the masses reach top-p's. Direct: no list, the cut is known.
-  enum Source { kFloor, kSome, kMore, kNear, kExact, kCount, kMass, kDirect };
-
-  // A list is cut by top-k, top-p and min-p, and the kept masses go to their groups. The
-  // bins that are listed: a pass counts or weighs the tokens in bins of equal width below
-  // the largest (24 units of e^x hold all masses that count; by ranks, what the 64s'
-  // largest span), the next lists the bin that the cut is in and adds up what lies above
-  // it. The first weighing takes all bins that the cut may be in by what its sums can be
-  // off: a mass by 1e-5 of itself (24 units of the exponent, four roundings each) and
-  // 2^-31 (a whole number of them is added). A list that is too long has its keys cut
-  // into bins again.
-  __device__ __forceinline__ void run() {
-    const uint32_t key = block_most(static_cast<int64_t>(threadIdx.x) < a.n1024 ? a.firsts[row * a.n1024 + threadIdx.x] : 0u, s);
+  // ---- a row
+  // Whether the row has an answer that needs no masses, and what its masses refer to.
+  __device__ __forceinline__ bool begin() {
+    const uint32_t first = static_cast<int64_t>(threadIdx.x) < a.n1024 ? a.firsts[row * a.n1024 + threadIdx.x] : 0u;
+    if (r.k || r.p < 1.f || r.m > 0.f) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int64_t i = threadIdx.x + k * int64_t{kThreads};
+        tops[k] = i < a.n64 ? a.tops[row * a.n64 + i] : 0u;
+      }
+    }
+    const uint32_t key = block_most(first);
     if (r.bad || key == kNan || key <= kNone) {
-      none();
-      return;
+      if (threadIdx.x == 0) token = -1, log_mass = NAN;
+      return true;
     }
     if (r.first) {
       largest(key);
-      return;
+      return true;
     }
     inf = key == kInf;
     mass_of.from(inf ? 0. : static_cast<double>(value_of(key)));
+    return false;
+  }
+  // A key that every token of a mass of at least m reaches.
+  __device__ __forceinline__ uint32_t least_key() const {
+    if (!(r.m > 0.f)) return kNone + 1;
+    const double y = mass_of.top + static_cast<double>(r.t) * static_cast<double>(logf(r.m));
+    // (under it by more than the roundings of the logarithm, of y, of f and of a mass)
+    const float f = static_cast<float>(y - 1e-6 * (fabs(y) + fabs(mass_of.top) + 100. * static_cast<double>(r.t)));
+    return f > -INFINITY ? key_of(f) : kNone + 1;
+  }
+
+  // The kept ones of a list's n tokens, `above` the masses and `before` the number of
+  // those that stand before them: `end` of the list, by top-k where by_k, top-p and
+  // min-p. Their masses go to their groups in s.mass. all_mass: of what top-p refers to,
+  // where top-k does not set it. 0: min-p's cut is above the list.
+  __device__ __forceinline__ uint32_t cut_list(uint32_t n, bool by_k, double above, uint32_t before, double& all_mass,
+                                               bool& passed) {
+    const uint32_t size = sort(n), per = size > kThreads ? 2 : 1, i0 = threadIdx.x * per;
+    uint32_t end = n;
+    if (by_k && static_cast<int64_t>(end) > r.k - before) end = static_cast<uint32_t>(r.k - before);
+    double w[2], all;
+#pragma unroll 1
+    for (uint32_t i = 0; i < 2; ++i) {
+      const double v = i < per && i0 + i < end ? weight(listed(s.list[i0 + i])) : 0.;
+      w[0] = i ? w[0] : v;
+      w[1] = v;
+    }
+    if (per == 1) w[1] = 0.;
+    const double sum = above + block_scan(w[0] + w[1], all) - (w[0] + w[1]);
+    if (by_k) all_mass = above + all;
+    const double goal = static_cast<double>(r.p) * all_mass, limit = r.p < 1.f ? goal : INFINITY;
+    passed = by_k && !(limit > above);   // top-p's cut is above a list of top-k's
+    if (passed) return end;
     const double least = static_cast<double>(r.m);
+    uint32_t kept = 0;
+    if (i0 < end && ((i0 == 0 && before == 0) || (sum < limit && w[0] >= least))) kept = i0 + 1;
+    if (per == 2 && i0 + 1 < end && sum + w[0] < limit && w[1] >= least) kept = i0 + 2;
+    end = block_most(kept);
+    for (int g = threadIdx.x; g < kGroup; g += kThreads) s.mass[g] = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i)
+      if (i < per && i0 + i < end && w[i] > 0.) {
+        // (a mass of next to nothing is one all the same, u may be 0: the highest bit, which
+        // 2048 masses do not reach)
+        const unsigned long long f = fixed_of(w[i]);
+        auto* m = reinterpret_cast<unsigned long long*>(&s.mass[token_of(static_cast<uint32_t>(s.list[i0 + i])) / kGroup]);
+        if (f) atomicAdd(m, f);
+        else atomicOr(m, 1ull << 63);
+      }
+    __syncthreads();
+    return end;
+  }
+  // What cut_list has left for thread t's group.
+  __device__ __forceinline__ double listed_mass() const {
+    const uint64_t m = s.mass[threadIdx.x];
+    return static_cast<double>(m & ~(uint64_t{1} << 63)) / kFixed + (m >> 63 ? 1e-300 : 0.);
+  }
+
+  // A row that is not filtered, or of which a list of at most kList tokens is known to
+  // hold the kept ones; else false. Lists are, in the order in which they are tried: the
+  // tokens over what min-p keeps (all of few), those over what about 64 or k of the 64s'
+  // largest reach.
+  __device__ __forceinline__ bool pick() {
+    if (begin()) return true;
     double mine = 0., all_mass = 1.;
     uint64_t cut = 0;
-    double cut_least = 0.;
-    if (whole(r)) {
-      mine = group_mass();
-      if (r.p < 1.f) block_scan(mine, s, all_mass);
-    }
+    if (whole(r)) mine = group_mass();
     if (!whole(r) || r.p < 1.f) {
-      uint32_t floor = kNone + 1;   // nothing under it is kept
-      if (r.m > 0.f) {
-        const double y = mass_of.top + static_cast<double>(r.t) * log(least);
-        // (under it by more than the roundings of y, of f and of a mass)
-        const float f = static_cast<float>(y - 1e-6 * (fabs(y) + fabs(mass_of.top) + static_cast<double>(r.t)));
-        if (f > -INFINITY) floor = key_of(f);
-      }
-      Cut q{static_cast<uint64_t>(kNone + 1) << 32, false, false, 0, 0, 0, kNan, 0, 0, top(), 0.f, 0.f};
-      double goal = static_cast<double>(r.p) * all_mass, off = 0.;
-      int source;
-      if (inf) source = r.k ? kCount : r.p < 1.f ? kMass : kDirect;
-      else if (a.v <= kList) source = kFloor;   // all tokens
-      else if (r.k) source = r.k <= a.n64 ? kNear : kCount;
-      else source = r.m > 0.f ? kFloor : kSome;
-      if (source == kDirect) q.limit = static_cast<uint64_t>(floor) << 32;
+      if (inf) return false;
+      if (whole(r)) block_scan(mine, all_mass);
+      enum Source { kFloor, kSome, kNear, kExact };
+      const uint32_t floor = r.k ? kNone + 1 : least_key();
+      int source = a.v <= kList ? kFloor : r.k ? kNear : r.m > 0.f ? kFloor : kSome;
+      if (r.k > a.n64 && source == kNear) return false;
       while (true) {
-        double above = 0.;   // of the masses before the list
-        uint32_t n, before = 0;
+        uint32_t from = floor;
         bool complete = true;
-        if (source < kCount) {
-          uint32_t from = floor;
-          if (source != kFloor) {
-            const int64_t c = source == kSome ? 64 : source == kMore ? 1024 : r.k;
-            // (No mass is over 1.)
-            const bool hopeless = !r.k && (goal > 1.25 * static_cast<double>(c) || c > a.n64);
-            from = hopeless ? 0 : source == kExact ? kth_top(c) : near_top(c);
-            if (!r.k && from < floor) from = hopeless ? 0 : floor;
-            complete = r.k || from == floor;
-          } else if (r.k) {
-            from = kNone + 1;
-          }
-          n = from ? candidates(from) : kList + 1;
-          double share = 1.;
-          if (n <= 64 && from_few(n, complete, all_mass, share)) return;
-          if (n <= 64 || n > kList) {
-            if (source == kSome && n <= 64 && share < .5 * static_cast<double>(r.p)) source = kMore;
-            source = source == kFloor ? (r.p < 1.f ? kSome : kDirect) : source == kSome ? kMore : source == kMore ? kMass
-                     : source == kNear ? kExact : kCount;
-            if (source == kDirect) q.limit = static_cast<uint64_t>(floor) << 32;
-            continue;
-          }
+        if (source != kFloor) {
+          const int64_t c = source == kSome ? 64 : r.k;
+          // (No mass is over 1.)
+          if (source == kSome && (static_cast<double>(r.p) * all_mass > 1.25 * static_cast<double>(c) || c > a.n64)) return false;
+          const uint32_t least = source == kExact ? kth_top(c) : near_top(c);
+          complete = r.k || least <= floor;
+          if (least > from) from = least;
+        }
+        const uint32_t n = candidates(from);
+        if (n <= 64) {
+          if (from_few(n, complete, all_mass)) return true;
+          return false;
+        }
+        if (n <= kList) {
+          bool passed;
+          const uint32_t end = cut_list(n, r.k != 0, 0., 0, all_mass, passed);
+          if (!complete && end == n) return false;   // it may go on below the list
+          cut = uniform(s.list[end - 1]);
+          mine = listed_mass();
+          break;
+        }
+        if (source == kNear) source = kExact;   // (far from evenly spread)
+        else if (source == kFloor && r.p < 1.f) source = kSome;
+        else return false;
+      }
+    }
+    by_groups(mine, cut, 0.);
+    return true;
+  }
+
+  // The other rows: bins of which one is listed. A pass counts or weighs the tokens in
+  // bins of equal width below the largest (24 units of e^x hold all masses that count; by
+  // ranks, what the 64s' largest span), the next lists the bin that the cut is in and
+  // adds up what lies above it. The first weighing is in 32 bits and takes all bins that
+  // the cut may be in by what its sums can be off: a mass by 1e-5 of itself (24 units of
+  // the exponent, four roundings each) and by 2^-31 of all (a whole number of them is
+  // added). A list that is too long has its keys cut into bins again.
+  __device__ __forceinline__ void select() {
+    if (begin()) return;
+    double all_mass = 1.;
+    if (whole(r)) block_scan(group_mass(), all_mass);
+    const uint64_t floor = static_cast<uint64_t>(least_key()) << 32;
+    Cut q{};
+    q.high = top();
+    double off = 0., mine, cut_least = 0.;
+    uint64_t cut;
+    enum Source { kCount, kMass, kDirect };   // direct: the cut is known
+    int source = r.k ? kCount : r.p < 1.f ? kMass : kDirect;
+    while (true) {
+      const double goal = static_cast<double>(r.p) * all_mass;
+      if (source == kDirect) {   // with the cut in q.limit, or min-p's
+        if (!q.limited || q.limit < floor) q.limit = floor;
+        q.limited = true;
+        q.lo = INFINITY;
+        q.hi = -INFINITY;
+      } else {
+        if (q.level == 0) {
+          q.by_count = source == kCount;
+          const float span = q.by_count && !inf ? (q.high - least_top()) * 1.25f : 24.f * r.t;
+          q.width = fminf(static_cast<float>(kBins) / span, 1e30f);
+          q.slope = -1.44269504f * fminf(static_cast<float>(mass_of.inv), 1e30f);
+          q.unit = static_cast<float>(2147483648. / all_mass);
+          off = mass_of.inv > 1e30 ? INFINITY : (1e-5 + static_cast<double>(a.v) / 2147483648.) * all_mass;
+          q.lo = -3.4028234664e38f;
+          q.hi = q.high;
+        }
+        fill_bins(q);
+        const int b = 2 * static_cast<int>(threadIdx.x);
+        const uint64_t v0 = q.level ? s.mass[b] : s.count[b], v1 = q.level ? s.mass[b + 1] : s.count[b + 1];
+        uint64_t all;
+        const uint64_t upto = block_scan<uint64_t>(v0 + v1, all);
+        const double base = uniform(s.value);   // the masses above the bins, from level 1 on
+        const int64_t k = r.k - (q.level ? static_cast<int64_t>(uniform(s.found)) : 0);
+        const double unit = q.level ? 1. / kFixed : all_mass / 2147483648.;
+        const double low = q.level ? goal - base : goal - off, high = q.level ? low : goal + off;
+        const bool count = q.by_count;
+        const uint32_t b0 = bin_where(v0, v1, upto, [&](uint64_t m) { return count ? static_cast<int64_t>(m) >= k : static_cast<double>(m) * unit >= low; });
+        uint32_t b1 = b0;
+        if (!count && q.level == 0) {
+          b1 = bin_where(v0, v1, upto, [&](uint64_t m) { return static_cast<double>(m) * unit >= high; });
+          if (static_cast<double>(all) * unit < high) b1 = kBins - 1;
+        }
+        if (q.level == 0) {
+          q.hi = b0 ? value_of(last_of(q, b0)) : q.high;
+          const uint32_t under = b1 < kBins - 1 ? last_of(q, b1 + 1) : 0;
+          q.lo = under ? value_of(under + 1) : -3.4028234664e38f;
         } else {
-          if (source != kDirect) {
-            if (q.level == 0) {
-              q.by_count = source == kCount;
-              float span = 24.f * r.t;
-              if (q.by_count && !inf) {
-                uint32_t most = 0;
-                for (int64_t i = threadIdx.x; i < a.n64; i += kThreads) {
-                  const uint32_t k = a.tops[row * a.n64 + i];
-                  if (k > kNone) most = ~k > most ? ~k : most;
-                }
-                span = (q.high - value_of(~block_most(most, s))) * 1.25f;
-              }
-              q.width = fminf(static_cast<float>(kBins) / span, 1e30f);
-              q.slope = -1.44269504f * fminf(static_cast<float>(mass_of.inv), 1e30f);
-              off = mass_of.inv > 1e30 ? INFINITY : 1e-5 * all_mass + static_cast<double>(a.v) / 2147483648.;
-            }
-            fill_bins(q);
-            const uint64_t v0 = s.mass[2 * threadIdx.x], v1 = s.mass[2 * threadIdx.x + 1];
-            uint64_t all;
-            const uint64_t upto = block_scan<uint64_t>(v0 + v1, s, all);
-            const double base = uniform(s.value);   // the masses above the bins, from level 1 on
-            const int64_t k = r.k - (q.level ? static_cast<int64_t>(uniform(s.found)) : 0);
-            const double unit = q.level ? 1. / kFixed : 1. / 2147483648.;
-            const double low = q.level ? goal - base : goal - off, high = q.level ? low : goal + off;
-            const bool count = q.by_count;
-            const uint32_t b0 = bin_where(v0, v1, upto, [&](uint64_t m) { return count ? static_cast<int64_t>(m) >= k : static_cast<double>(m) * unit >= low; });
-            uint32_t b1 = b0;
-            if (!count && q.level == 0) {
-              b1 = bin_where(v0, v1, upto, [&](uint64_t m) { return static_cast<double>(m) * unit >= high; });
-              if (static_cast<double>(all) * unit < high) b1 = kBins - 1;
-            }
-            if (q.level == 0) {
-              q.first = b0;
-              q.final = b1;
-              q.lo = 0;
-              q.hi = kNan;
-            } else {
-              const uint32_t h = q.hi - (b0 << q.shift), wide = (uint32_t{1} << q.shift) - 1;
-              q.lo = h - q.lo > wide ? h - wide : q.lo;
-              q.hi = h;
-            }
-          }
-          q.direct = source == kDirect;
-          uint32_t low, most;
-          gather(q, q.direct ? least : 0., before, low, most);
-          n = uniform(s.n);
-          if (q.direct) {
-            mine = static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0.;
-            cut = q.limit;
-            cut_least = least;
-            break;
-          }
-          above = sum_of_groups();
-          if (n > kList) {
-            q.hi = block_most(most, s);
-            q.lo = ~block_most(~low, s);
-            ++q.level;
-            q.shift = 0;
-            while ((q.hi - q.lo) >> q.shift >= kBins) ++q.shift;
-            if (threadIdx.x == 0) s.value = above;
-            __syncthreads();
-            if (q.lo != q.hi) continue;
-            // more equal values than the list holds
-            const double w = weight(value_of(q.hi));
-            double want = static_cast<double>(n);
-            if (source == kCount) {
-              want = static_cast<double>(r.k - before);
-              goal = r.p < 1.f ? static_cast<double>(r.p) * (above + want * w) : INFINITY;
-            }
-            if (goal > above) want = fmin(want, ceil((goal - above) / w));
-            const uint64_t o = tied(q.hi, static_cast<int64_t>(fmax(want, 1.)), q.limit);
-            q.level = 0;
-            if (goal > above) {
-              source = kDirect;
-              q.limit = o;
-            } else {   // top-p's cut is among the ones above
-              source = kMass;
-              q.limit = o;
-              all_mass = goal / static_cast<double>(r.p);
-            }
-            continue;
-          }
+          const uint32_t h = q.most - (b0 << q.shift), l = h - ((uint32_t{1} << q.shift) - 1), least = key_of(q.lo);
+          q.hi = value_of(h);
+          q.lo = l <= h && l > least ? value_of(l) : q.lo;
         }
-        // the list, and its cut
-        const uint32_t size = sort(n), per = size > kThreads ? 2 : 1, i0 = threadIdx.x * per;
-        uint32_t end = n;
-        if (r.k && source != kMass && static_cast<int64_t>(end) > r.k - before) end = static_cast<uint32_t>(r.k - before);
-        double w[2], all;
-        w[0] = i0 < end ? weight(listed(s.list[i0])) : 0.;
-        w[1] = per == 2 && i0 + 1 < end ? weight(listed(s.list[i0 + 1])) : 0.;
-        const double sum = above + block_scan(w[0] + w[1], s, all) - (w[0] + w[1]);
-        if (r.k && source != kMass) {
-          all_mass = above + all;
-          goal = static_cast<double>(r.p) * all_mass;
-        }
-        if (source == kCount && r.p < 1.f && !(goal > above)) {
-          q.limit = uniform(s.list[end - 1]);
-          source = kMass;
-          q.level = 0;
-          continue;
-        }
-        const double limit = r.p < 1.f ? goal : INFINITY;
-        uint32_t kept = 0;
-        if (i0 < end && ((i0 == 0 && before == 0) || (sum < limit && w[0] >= least))) kept = i0 + 1;
-        if (per == 2 && i0 + 1 < end && sum + w[0] < limit && w[1] >= least) kept = i0 + 2;
-        end = block_most(kept, s);
-        if (source < kCount && !complete && end == n) {   // it may go on below the list
-          source = source == kSome && all >= .5 * goal ? kMore : kMass;
-          continue;
-        }
-        if (end == 0) {   // min-p's cut is above the list
-          source = kDirect;
-          q.limit = static_cast<uint64_t>(floor) << 32;
-          continue;
-        }
-        cut = uniform(s.list[end - 1]);
-        for (int g = threadIdx.x; g < kGroup; g += kThreads) s.mass[g] = 0;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t i = 0; i < 2; ++i)
-          if (i < per && i0 + i < end && w[i] > 0.) {
-            // (a mass of next to nothing is one all the same, u may be 0: the highest bit, which
-            // 2048 masses do not reach)
-            const unsigned long long f = fixed_of(w[i]);
-            auto* m = reinterpret_cast<unsigned long long*>(&s.mass[token_of(static_cast<uint32_t>(s.list[i0 + i])) / kGroup]);
-            if (f) atomicAdd(m, f);
-            else atomicOr(m, 1ull << 63);
-          }
-        __syncthreads();
-        const uint64_t m = s.mass[threadIdx.x];
-        mine = static_cast<double>(m & ~(uint64_t{1} << 63)) / kFixed + (m >> 63 ? 1e-300 : 0.);
-        if (source >= kCount && static_cast<int64_t>(threadIdx.x) < a.n1024) mine += s.group[threadIdx.x];
+      }
+      uint32_t before;
+      float low, most;
+      gather(q, source == kDirect ? static_cast<double>(r.m) : 0., before, low, most);
+      if (source == kDirect) {
+        mine = static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0.;
+        cut = q.limit;
+        cut_least = static_cast<double>(r.m);
         break;
       }
+      const uint32_t n = uniform(s.n);
+      const double above = sum_of_groups();
+      if (n > kList) {
+        q.most = block_most(key_of(most));
+        const uint32_t span = q.most - ~block_most(~key_of(low));
+        q.hi = value_of(q.most);
+        q.lo = value_of(q.most - span);
+        ++q.level;
+        q.shift = 0;
+        while (span >> q.shift >= kBins) ++q.shift;
+        if (threadIdx.x == 0) s.value = above;
+        __syncthreads();
+        if (span) continue;
+        // more equal values than the list holds
+        const double w = weight(q.hi);
+        double want = static_cast<double>(n);
+        if (source == kCount) {
+          want = static_cast<double>(r.k - before);
+          all_mass = above + want * w;
+        }
+        const double limit = r.p < 1.f ? static_cast<double>(r.p) * all_mass : INFINITY;
+        if (limit > above) want = fmin(want, ceil((limit - above) / w));
+        q.limit = tied(q.most, static_cast<int64_t>(fmax(want, 1.)), q.limited ? q.limit : 0);
+        q.limited = true;
+        q.level = 0;
+        source = limit > above ? kDirect : kMass;   // (or top-p's cut is among the ones above)
+        continue;
+      }
+      bool passed;
+      const uint32_t end = cut_list(n, source == kCount, above, before, all_mass, passed);
+      if (passed || end == 0) {
+        if (passed) {
+          q.limit = uniform(s.list[end - 1]);
+          q.limited = true;
+        }
+        source = passed ? kMass : kDirect;
+        q.level = 0;
+        continue;
+      }
+      cut = uniform(s.list[end - 1]);
+      mine = listed_mass() + (static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0.);
+      break;
     }
     by_groups(mine, cut, cut_least);
   }
 };
 
-template <typename E>
-__global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a) {
+// A row that pick() leaves to select() has this for its token meanwhile.
+constexpr int64_t kLeft = -2;
+
+template <typename E, bool SELECT>
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
   __shared__ Shared s;
   const int64_t row = blockIdx.x;
+  if (SELECT && a.token[row] != kLeft) return;
   load_powers(s.powers);   // (barriers follow before they are read)
   const Row r = row_of(a, row);
-  Pick<E> p{a, s, row, r, static_cast<const E*>(a.x) + row * a.ldx, Exp(s.powers, r.t), false};
-  p.run();
+  Pick<E> p{a, s, row, r, static_cast<const E*>(a.x) + row * a.ldx, Exp(s.powers, r.t), false, {0, 0}};
+  if constexpr (SELECT) p.select();
+  else if (!p.pick() && threadIdx.x == 0) a.token[row] = kLeft;
+  p.finish();
 }
 
 template <typename E>
@@ -1084,7 +1184,10 @@ hipError_t sample(const SampleArgs& a, hipStream_t stream) {
     p.firsts = a.firsts + r * a.n1024;
     p.masses = a.masses + r * a.n1024;
     hipLaunchKernelGGL(sample_groups_kernel<E>, dim3(across, static_cast<unsigned>(n)), dim3(256), 0, stream, p);
-    hipLaunchKernelGGL(sample_pick_kernel<E>, dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((sample_row_kernel<E, false>), dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream, p);
+    // (not where nothing is filtered in any row)
+    if (a.k || a.p || a.m || a.k1 > 0 || a.p1 < 1.f || a.m1 > 0.f)
+      hipLaunchKernelGGL((sample_row_kernel<E, true>), dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream, p);
   }
   return hipGetLastError();
 }
