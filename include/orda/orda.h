@@ -509,7 +509,8 @@ typedef struct {
     float temperature, top_p, min_p;
     int32_t top_k;
 } orda_sampling;
-int32_t orda_sample_tokens_workspace(int64_t n, int64_t v, int64_t *bytes, char *err, size_t err_len);
+int32_t orda_sample_tokens_workspace(int64_t n, int64_t v, int32_t logits_dtype, int64_t *bytes, char *err,
+                                     size_t err_len);
 /* tokens [N]; logprobs [N] or NULL. */
 int32_t orda_sample_tokens(int32_t device, void *hip_stream, const orda_sampling *args, int64_t *tokens,
                            float *logprobs, void *workspace, int64_t workspace_bytes, char *err,

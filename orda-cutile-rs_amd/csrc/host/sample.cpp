@@ -22,12 +22,12 @@ using namespace orda;
 
 extern "C" {
 
-int32_t orda_sample_tokens_workspace(int64_t n, int64_t v, int64_t* bytes, char* err, size_t err_len) {
+int32_t orda_sample_tokens_workspace(int64_t n, int64_t v, int32_t dtype, int64_t* bytes, char* err, size_t err_len) {
   return guarded(err, err_len, [&] {
     if (!bytes) fail(ORDA_ERR_INVALID, "null argument");
     check_shape(n, v);
-    int64_t tops, firsts;
-    *bytes = sample_scratch(n, v, &tops, &firsts);
+    int64_t tops, firsts, tails;
+    *bytes = sample_scratch(to_dtype(dtype, "logits"), n, v, &tops, &firsts, &tails);
   });
 }
 
@@ -49,8 +49,8 @@ int32_t orda_sample_tokens(int32_t device, void* hip_stream, const orda_sampling
     if (x.rows == 0) return;
     if (x.cols == 0) fail(ORDA_ERR_INVALID, "logits must have columns");
     if (!args->uniform || !tokens) fail(ORDA_ERR_INVALID, "null argument");
-    int64_t tops, firsts;
-    const int64_t need = sample_scratch(x.rows, x.cols, &tops, &firsts);
+    int64_t tops, firsts, tails;
+    const int64_t need = sample_scratch(t, x.rows, x.cols, &tops, &firsts, &tails);
     if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) fail(ORDA_ERR_INVALID, "workspace must be 256-byte aligned");
     if (workspace_bytes < need || !workspace)
       fail(ORDA_ERR_INVALID, "workspace of %lld bytes, %lld needed", static_cast<long long>(workspace_bytes),
@@ -77,6 +77,7 @@ int32_t orda_sample_tokens(int32_t device, void* hip_stream, const orda_sampling
     a.masses = reinterpret_cast<double*>(ws);
     a.tops = reinterpret_cast<uint32_t*>(ws + tops);
     a.firsts = reinterpret_cast<uint32_t*>(ws + firsts);
+    a.tails = ws + tails;
     const DeviceScope scope(device);
     hip_check(launch_sample(a, t, static_cast<hipStream_t>(hip_stream)), "drawing tokens");
   });

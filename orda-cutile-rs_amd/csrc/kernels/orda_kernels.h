@@ -670,9 +670,10 @@ struct SampleArgs {
   float* logprob;          // or null
   uint32_t *tops, *firsts; // largest keys of the row's 64s and of its 1024s
   double* masses;          // of its 1024s
+  void* tails;             // 1024 logits a row: its last, where they are fewer
   int64_t n64, n1024;
 };
-int64_t sample_scratch(int64_t n, int64_t v, int64_t* tops, int64_t* firsts);   // bytes; masses come first
+int64_t sample_scratch(DType t, int64_t n, int64_t v, int64_t* tops, int64_t* firsts, int64_t* tails);   // bytes; masses come first
 hipError_t launch_sample(const SampleArgs& a, DType t, hipStream_t stream);
 
 }  // namespace orda

@@ -232,35 +232,38 @@ __device__ __forceinline__ T lane_of(T v, int lane) {
 }
 __device__ __forceinline__ double wave_sum(double x) { return lane_of(wave_scan(x, Sum{}), 63); }
 
-// A lane's 16 of a group's tokens, kPer neighbouring ones a load; -infinity past the
-// row's end. Fetched as they lie in memory, so that a next group's can be under way.
+// A lane's 16 of a group's tokens, kPer neighbouring ones a load, as they lie in memory,
+// so that a next group's can be under way.
 template <typename E>
 struct Tokens {
   static constexpr int kPer = 16 / sizeof(E), kLoads = 16 / kPer;
   E w[kLoads][kPer];
-  __device__ __forceinline__ static int64_t column(int64_t group, int i) {   // of load i
-    return group * kGroup + (i * 64 + static_cast<int>(threadIdx.x & 63)) * int64_t{kPer};
+  __device__ __forceinline__ static int column(int i) {   // within the group, of load i
+    return (i * 64 + static_cast<int>(threadIdx.x & 63)) * kPer;
   }
-  __device__ __forceinline__ void fetch(const E* row, int64_t group, int64_t v) {
-    if ((group + 1) * kGroup <= v) {
+  __device__ __forceinline__ void fetch(const E* group) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) __builtin_memcpy(w[i], row + column(group, i), sizeof w[i]);
-    } else {
+    for (int i = 0; i < kLoads; ++i) __builtin_memcpy(w[i], group + column(i), sizeof w[i]);
+  }
+  // -infinity past the row's end, n tokens on.
+  __device__ __forceinline__ void fetch(const E* group, int64_t n) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
+    for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-          const int64_t c = column(group, i) + k;
-          w[i][k] = c < v ? row[c] : static_cast<E>(-INFINITY);
-        }
-    }
+      for (int k = 0; k < kPer; ++k) w[i][k] = column(i) + k < n ? group[column(i) + k] : static_cast<E>(-INFINITY);
+  }
+  __device__ __forceinline__ void store(E* group) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) __builtin_memcpy(group + column(i), w[i], sizeof w[i]);
   }
   __device__ __forceinline__ float at(int i, int k) const { return static_cast<float>(w[i][k]); }
 };
 
 // ---------------------------------------------------------------- first pass
 // The largest of each 64 and of each 1024 tokens, as keys, and where they are needed
-// the sum of each 1024's masses, relative to its largest: one read of the logits.
+// the sum of each 1024's masses, relative to its largest: one read of the logits. A
+// row's last 1024, where they are fewer, are copied and filled up, so that later passes
+// read whole ones.
 __device__ __forceinline__ float max3(float a, float b, float c) {   // (a NaN is looked for apart)
   float m;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
@@ -276,7 +279,13 @@ __global__ __launch_bounds__(256) void sample_groups_kernel(SampleArgs a) {
   const int lane = threadIdx.x & 63;
   if (group >= a.n1024) return;
   T raw;
-  raw.fetch(static_cast<const E*>(a.x) + row * a.ldx, group, a.v);
+  const E* at0 = static_cast<const E*>(a.x) + row * a.ldx + group * kGroup;
+  if ((group + 1) * kGroup <= a.v) {
+    raw.fetch(at0);
+  } else {
+    raw.fetch(at0, a.v - group * kGroup);
+    raw.store(static_cast<E*>(a.tails) + row * kGroup);
+  }
   float x[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) x[k] = raw.at(k / T::kPer, k % T::kPer);
@@ -720,10 +729,12 @@ struct Pick {
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
     using T = Tokens<E>;
-    int64_t g = threadIdx.x >> 6;
-    if (g >= a.n1024) return;
+    int g = uniform(static_cast<int>(threadIdx.x >> 6));
+    const int groups = static_cast<int>(a.n1024), whole = static_cast<int>(a.v / kGroup);
+    if (g >= groups) return;
+    const E* tail = static_cast<const E*>(a.tails) + row * kGroup;
     T t;
-    t.fetch(x, g, a.v);
+    t.fetch(g < whole ? x + g * int64_t{kGroup} : tail);
     while (true) {
       float y[4][4];
 #pragma unroll
@@ -732,15 +743,15 @@ struct Pick {
 #pragma unroll
         for (int k = 0; k < 16; ++k) y[k / 4][k % 4] = value(y[k / 4][k % 4]);
       }
-      const int64_t next = g + kWaves;
-      if (next < a.n1024) t.fetch(x, next, a.v);
+      const int next = g + kWaves;
+      if (next < groups) t.fetch(next < whole ? x + next * int64_t{kGroup} : tail);
 #pragma unroll 1
       for (int unit = 0; unit < 4; ++unit) {
-        f(g, unit, T::column(g, unit * 4 / T::kPer) + unit * 4 % T::kPer, y[0]);
+        f(g, unit, g * int64_t{kGroup} + T::column(unit * 4 / T::kPer) + unit * 4 % T::kPer, y[0]);
 #pragma unroll
         for (int k = 0; k < 12; ++k) y[k / 4][k % 4] = y[k / 4 + 1][k % 4];
       }
-      if (next >= a.n1024) return;
+      if (next >= groups) return;
       g = next;
     }
   }
@@ -789,7 +800,7 @@ struct Pick {
       s.count[b] = 0;
     }
     __syncthreads();
-    each([&](int64_t, int, int64_t c, const float(&y)[4]) {
+    each([&](int, int, int64_t c, const float(&y)[4]) {
       if (q.level == 0) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -799,12 +810,11 @@ struct Pick {
         }
         return;
       }
-#pragma unroll 1
+#pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float v = k < 2 ? (k ? y[1] : y[0]) : k == 2 ? y[2] : y[3];
-        if (!(v >= q.lo && v <= q.hi) || (q.limited && order_of(v, c + k) < q.limit)) continue;
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[(q.most - key_of(v)) >> q.shift]),
-                  q.by_count ? 1ull : fixed_of(weight(v)));
+        if (!(y[k] >= q.lo && y[k] <= q.hi) || (q.limited && order_of(y[k], c + k) < q.limit)) continue;
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[(q.most - key_of(y[k])) >> q.shift]),
+                  q.by_count ? 1ull : fixed_of(weight(y[k])));
       }
     });
     __syncthreads();
@@ -839,7 +849,7 @@ struct Pick {
     double sum = 0.;
     low = INFINITY;
     most = -INFINITY;
-    each([&](int64_t g, int unit, int64_t c, const float(&y)[4]) {
+    each([&](int g, int unit, int64_t c, const float(&y)[4]) {
       bool member[4], any = false;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -1183,6 +1193,7 @@ hipError_t sample(const SampleArgs& a, hipStream_t stream) {
     p.tops = a.tops + r * a.n64;
     p.firsts = a.firsts + r * a.n1024;
     p.masses = a.masses + r * a.n1024;
+    p.tails = static_cast<E*>(a.tails) + r * kGroup;
     hipLaunchKernelGGL(sample_groups_kernel<E>, dim3(across, static_cast<unsigned>(n)), dim3(256), 0, stream, p);
     hipLaunchKernelGGL((sample_row_kernel<E, false>), dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream, p);
     // (not where nothing is filtered in any row)
@@ -1194,12 +1205,13 @@ hipError_t sample(const SampleArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int64_t sample_scratch(int64_t n, int64_t v, int64_t* tops, int64_t* firsts) {
+int64_t sample_scratch(DType t, int64_t n, int64_t v, int64_t* tops, int64_t* firsts, int64_t* tails) {
   auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
   const int64_t n64 = (v + 63) / 64, n1024 = (v + kGroup - 1) / kGroup;
   *tops = up(n * n1024 * 8);
   *firsts = *tops + up(n * n64 * 4);
-  return *firsts + up(n * n1024 * 4);
+  *tails = *firsts + up(n * n1024 * 4);
+  return *tails + (v % kGroup ? up(n * kGroup * dtype_size(t)) : 0);
 }
 
 hipError_t launch_sample(const SampleArgs& a, DType t, hipStream_t stream) {

@@ -194,7 +194,7 @@ SIGNATURES = [
      [C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_double, C.c_double, C.c_void_p, C.c_void_p,
       C.c_int64, C.c_char_p, C.c_size_t]),
     ("orda_sample_tokens_workspace", C.c_int32,
-     [C.c_int64, C.c_int64, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
+     [C.c_int64, C.c_int64, C.c_int32, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
     ("orda_sample_tokens", C.c_int32,
      [C.c_int32, C.c_void_p, C.POINTER(SamplingC), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
       C.c_char_p, C.c_size_t]),

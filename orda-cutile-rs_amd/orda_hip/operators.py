@@ -652,9 +652,9 @@ def _per_row(value, n: int, shape, device, what: str, dtype, none):
 
 
 @functools.lru_cache(maxsize=1024)
-def _sample_bytes(n: int, v: int) -> int:
+def _sample_bytes(n: int, v: int, dtype: int) -> int:
     b = C.c_int64()
-    _call(L.load().orda_sample_tokens_workspace, n, v, C.byref(b))
+    _call(L.load().orda_sample_tokens_workspace, n, v, dtype, C.byref(b))
     return b.value
 
 
@@ -707,7 +707,7 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=None, top_p=None, m
         a.top_ps = p.data_ptr()
     if q is not None:
         a.min_ps = q.data_ptr()
-    b = _sample_bytes(n, v)
+    b = _sample_bytes(n, v, a.logits.dtype)
     ws = _bytes(b, d)
     tokens = torch.empty(shape, dtype=torch.int64, device=d)
     logprobs = torch.empty(shape, dtype=torch.float32, device=d)

@@ -40,11 +40,12 @@ def test_refused(kw, message):
 
 @pytest.mark.parametrize("n, v", [(0, 1000), (1, 1), (1, 131072), (512, 131072), (1 << 20, 64), (3, 1 << 20)])
 def test_workspace(n, v):
-    """Of every 64 tokens a key, of every 1024 a key and a sum."""
-    out, err = C.c_int64(), C.create_string_buffer(512)
-    assert L.load().orda_sample_tokens_workspace(n, v, C.byref(out), err, 512) == L.ORDA_OK
-    need = n * (-(-v // 64) * 4 + -(-v // 1024) * 12)
-    assert need <= out.value < need + 3 * 256
+    """Of every 64 tokens a key, of every 1024 a key and a sum; and a row's last 1024 where they are fewer."""
+    for dtype, es in ((L.F32, 4), (L.BF16, 2)):
+        out, err = C.c_int64(), C.create_string_buffer(512)
+        assert L.load().orda_sample_tokens_workspace(n, v, dtype, C.byref(out), err, 512) == L.ORDA_OK
+        need = n * (-(-v // 64) * 4 + -(-v // 1024) * 12 + (1024 * es if v % 1024 else 0))
+        assert need <= out.value < need + 4 * 256
 
 
 def test_python_refuses_cpu_tensors():
