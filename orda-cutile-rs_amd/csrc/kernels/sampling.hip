@@ -835,54 +835,56 @@ struct Pick {
   }
 
   // Adds up the masses of at least `least` of the tokens taken, by group in s.group, and
-  // lists the members, s.n of them; `above`: how many are taken, `low` and `most`: this
-  // thread's smallest and largest member. The taken ones are put together and weighed 64 at a time, so that the others cost no
-  // exponential.
-  __device__ __forceinline__ void gather(const Cut& q, double least, uint32_t& above, float& low, float& most) {
+  // lists the members: `n` of them, false where they are too many for their wave's part
+  // of the list; `above`: how many are taken; `low` and `most`: this thread's smallest
+  // and largest member. The taken ones are put together and weighed 64 at a time, so that
+  // the others cost no exponential.
+  __device__ __forceinline__ bool gather(const Cut& q, double least, uint32_t& n, uint32_t& above, float& low, float& most) {
+    constexpr uint32_t kPart = kList / kWaves, kOgt = 2, kOge = 3;   // (comparisons' codes)
     __syncthreads();
-    if (threadIdx.x == 0) s.n = s.found = 0;
-    __syncthreads();
-    const int lane = threadIdx.x & 63;
-    const uint64_t under = (uint64_t{1} << lane) - 1;
-    float* ring = s.ring[threadIdx.x >> 6];
-    uint32_t from = 0, held = 0, taken = 0;
+    if (threadIdx.x == 0) s.found = 0;
+    const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    float* ring = s.ring[wave];
+    uint64_t* part = s.list + wave * kPart;
+    uint32_t from = 0, held = 0, taken = 0, members = 0;
     double sum = 0.;
     low = INFINITY;
     most = -INFINITY;
+    // this lane's place after `base` among those of a mask
+    auto place = [](uint64_t who, uint32_t base) {
+      return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), base));
+    };
     each([&](int g, int unit, int64_t c, const float(&y)[4]) {
-      bool member[4], any = false;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        bool take = y[k] > q.hi;
-        member[k] = y[k] >= q.lo && !take;
+        uint64_t take = __builtin_amdgcn_fcmpf(y[k], q.hi, kOgt), list = __builtin_amdgcn_fcmpf(y[k], q.lo, kOge) & ~take;
         if (q.limited) {
-          const bool is = order_of(y[k], c + k) >= q.limit;
-          take = take && is;
-          member[k] = member[k] && is;
+          const uint64_t is = __ballot(order_of(y[k], c + k) >= q.limit);
+          take &= is;
+          list &= is;
         }
-        any = any || member[k];
-        const uint64_t who = __ballot(take);
-        if (take) ring[(from + held + static_cast<uint32_t>(__popcll(who & under))) % kRing] = y[k];
-        held += static_cast<uint32_t>(__popcll(who));
-      }
-      if (__any(any)) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          low = member[k] ? fminf(low, y[k]) : low;
-          most = member[k] ? fmaxf(most, y[k]) : most;
+        if (take >> lane & 1) ring[place(take, from + held) % kRing] = y[k];
+        held += static_cast<uint32_t>(__popcll(take));
+        if (list) {
+          if (list >> lane & 1) {
+            const uint32_t at = place(list, members);
+            if (at < kPart) part[at] = order_of(y[k], c + k);
+            low = fminf(low, y[k]);
+            most = fmaxf(most, y[k]);
+          }
+          members += static_cast<uint32_t>(__popcll(list));
         }
-        append(member, y, c);
       }
       while (held >= (unit < 3 ? 64u : 1u)) {
-        const uint32_t n = held < 64 ? held : 64;
+        const uint32_t m = held < 64 ? held : 64;
         wave_sync();
         const float v = ring[(from + lane) % kRing];
         wave_sync();
-        const double w = lane < static_cast<int>(n) ? weight(v) : 0.;
+        const double w = lane < static_cast<int>(m) ? weight(v) : 0.;
         if (w >= least) sum += w;
-        from += n;
-        held -= n;
-        taken += n;
+        from += m;
+        held -= m;
+        taken += m;
       }
       if (unit == 3) {
         sum = wave_sum(sum);
@@ -890,9 +892,31 @@ struct Pick {
         sum = 0.;
       }
     });
-    if (lane == 0) atomicAdd(&s.found, taken);
+    // the waves' parts one after another
+    uint32_t* counts = reinterpret_cast<uint32_t*>(s.waves[turn]);
+    turn ^= 1;
+    if (lane == 0) {
+      counts[wave] = members;
+      counts[kWaves + wave] = taken;
+    }
+    const uint32_t mine = members < kPart ? members : kPart;
+    uint64_t o[kPart / 64];
+#pragma unroll
+    for (uint32_t i = 0; i < kPart / 64; ++i) o[i] = i * 64 + lane < mine ? part[i * 64 + lane] : 0;
     __syncthreads();
-    above = uniform(s.found);
+    const uint32_t count = counts[threadIdx.x % kWaves], upto = row_scan(count, Sum{});
+    n = lane_of(upto, kWaves - 1);
+    above = lane_of(row_scan(counts[kWaves + threadIdx.x % kWaves], Sum{}), kWaves - 1);
+    const bool fits = lane_of(row_scan(count, Most{}), kWaves - 1) <= kPart;
+    const uint32_t to = wave ? lane_of(upto, wave - 1) : 0;
+    if (fits) {
+#pragma unroll
+      for (uint32_t i = 0; i < kPart / 64; ++i)
+        if (i * 64 + lane < mine) s.list[to + i * 64 + lane] = o[i];
+    }
+    if (threadIdx.x == 0) s.found = above;
+    __syncthreads();
+    return fits;
   }
 
   // The `want`-th in the order of the vocabulary of the tokens with this key.
@@ -1102,18 +1126,17 @@ struct Pick {
           q.lo = l <= h && l > least ? value_of(l) : q.lo;
         }
       }
-      uint32_t before;
+      uint32_t n, before;
       float low, most;
-      gather(q, source == kDirect ? static_cast<double>(r.m) : 0., before, low, most);
+      const bool fits = gather(q, source == kDirect ? static_cast<double>(r.m) : 0., n, before, low, most);
       if (source == kDirect) {
         mine = static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0.;
         cut = q.limit;
         cut_least = static_cast<double>(r.m);
         break;
       }
-      const uint32_t n = uniform(s.n);
       const double above = sum_of_groups();
-      if (n > kList) {
+      if (!fits) {
         q.most = block_most(key_of(most));
         const uint32_t span = q.most - ~block_most(~key_of(low));
         q.hi = value_of(q.most);
