@@ -473,8 +473,7 @@ typedef struct {
     orda_tensor src;
     orda_tensor dst;
 } orda_gradient;
-int32_t orda_clip_gradients_workspace(const orda_gradient *gradients, int64_t count, int64_t *bytes,
-                                      char *err, size_t err_len);
+int32_t orda_clip_gradients_workspace(int64_t count, int64_t *bytes, char *err, size_t err_len);
 int32_t orda_gradient_norm(int32_t device, void *hip_stream, const orda_gradient *gradients,
                            int64_t count, float *norm, void *workspace, int64_t workspace_bytes,
                            char *err, size_t err_len);

@@ -52,8 +52,12 @@ int64_t pieces_of(const GradPart& p, int64_t piece) { return p.rows * ceil_div(p
 // sums up by itself.
 constexpr int64_t kBlocks = 2048;
 
-Cut cut(const orda_gradient* g, int64_t count, bool scale) {
+void check_count(int64_t count) {
   if (count < 0 || count > kMostGradients) fail(ORDA_ERR_INVALID, "at most 2^20 gradients");
+}
+
+Cut cut(const orda_gradient* g, int64_t count, bool scale) {
+  check_count(count);
   if (count > 0 && !g) fail(ORDA_ERR_INVALID, "null argument");
   Cut c;
   int64_t values = 0;
@@ -135,11 +139,14 @@ void check_apart(const Cut& c) {
         fail(ORDA_ERR_INVALID, "gradients that are written share memory with others");
 }
 
-int64_t sum_bytes(const Cut& c) { return (c.sums * int64_t{8} + 255) / 256 * 256; }
+// Every launch has its share of the workgroups, and one at least.
+int64_t sum_bytes(int64_t count) {
+  return count == 0 ? 0 : ((kBlocks + ceil_div(count, kGradParts)) * 8 + 255) / 256 * 256;
+}
 
-void run(int32_t device, hipStream_t st, const Cut& c, bool scale, double max_norm, double eps, float* norm, void* ws,
+void run(int32_t device, hipStream_t st, const Cut& c, int64_t count, bool scale, double max_norm, double eps, float* norm, void* ws,
          int64_t ws_bytes) {
-  const int64_t need = sum_bytes(c);
+  const int64_t need = sum_bytes(count);
   if (reinterpret_cast<uintptr_t>(ws) % 256 != 0) fail(ORDA_ERR_INVALID, "workspace must be 256-byte aligned");
   if (ws_bytes < need || (need > 0 && !ws))
     fail(ORDA_ERR_INVALID, "workspace of %lld bytes, %lld needed", static_cast<long long>(ws_bytes),
@@ -179,11 +186,11 @@ using namespace orda;
 
 extern "C" {
 
-int32_t orda_clip_gradients_workspace(const orda_gradient* gradients, int64_t count, int64_t* bytes, char* err,
-                                      size_t err_len) {
+int32_t orda_clip_gradients_workspace(int64_t count, int64_t* bytes, char* err, size_t err_len) {
   return guarded(err, err_len, [&] {
     if (!bytes) fail(ORDA_ERR_INVALID, "null argument");
-    *bytes = std::max(sum_bytes(cut(gradients, count, true)), sum_bytes(cut(gradients, count, false)));
+    check_count(count);
+    *bytes = sum_bytes(count);
   });
 }
 
@@ -192,7 +199,7 @@ int32_t orda_gradient_norm(int32_t device, void* hip_stream, const orda_gradient
   return guarded(err, err_len, [&] {
     if (!norm) fail(ORDA_ERR_INVALID, "null argument");
     const Cut c = cut(gradients, count, false);
-    run(device, static_cast<hipStream_t>(hip_stream), c, false, 0., 0., norm, workspace, workspace_bytes);
+    run(device, static_cast<hipStream_t>(hip_stream), c, count, false, 0., 0., norm, workspace, workspace_bytes);
   });
 }
 
@@ -205,7 +212,7 @@ int32_t orda_clip_gradients(int32_t device, void* hip_stream, const orda_gradien
     if (!(eps >= 0.) || !isfinite(eps)) fail(ORDA_ERR_INVALID, "eps must be >= 0 and finite");
     const Cut c = cut(gradients, count, true);
     check_apart(c);
-    run(device, static_cast<hipStream_t>(hip_stream), c, true, max_norm, eps, norm, workspace, workspace_bytes);
+    run(device, static_cast<hipStream_t>(hip_stream), c, count, true, max_norm, eps, norm, workspace, workspace_bytes);
   });
 }
 

@@ -174,19 +174,18 @@ SIGNATURES = [
     ("orda_fp8_block_matmul", C.c_int32,
      [C.c_int32, C.c_void_p, C.POINTER(Fp8MatrixC), C.POINTER(Fp8MatrixC), C.POINTER(Tensor),
       C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t]),
+    # (structures of the following ones are packed by the caller)
     ("orda_rms_norm_forward", C.c_int32,
-     [C.c_int32, C.c_void_p, C.POINTER(RmsNormC), C.POINTER(Tensor), C.POINTER(Tensor), C.c_char_p,
-      C.c_size_t]),
+     [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
     ("orda_rms_norm_fp8", C.c_int32,
-     [C.c_int32, C.c_void_p, C.POINTER(RmsNormC), C.POINTER(Tensor), C.POINTER(Fp8MatrixC), C.c_char_p,
-      C.c_size_t]),
+     [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
     ("orda_rms_norm_backward_workspace", C.c_int32,
      [C.c_int64, C.c_int64, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
     ("orda_rms_norm_backward", C.c_int32,
-     [C.c_int32, C.c_void_p, C.POINTER(RmsNormC), C.POINTER(Tensor), C.POINTER(Tensor), C.POINTER(Tensor),
-      C.POINTER(Tensor), C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t]),
+     [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+      C.c_int64, C.c_void_p, C.c_size_t]),
     ("orda_clip_gradients_workspace", C.c_int32,
-     [C.c_void_p, C.c_int64, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
+     [C.c_int64, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
     ("orda_gradient_norm", C.c_int32,
      [C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_char_p,
       C.c_size_t]),
@@ -196,8 +195,8 @@ SIGNATURES = [
     ("orda_sample_tokens_workspace", C.c_int32,
      [C.c_int64, C.c_int64, C.c_int32, C.POINTER(C.c_int64), C.c_char_p, C.c_size_t]),
     ("orda_sample_tokens", C.c_int32,
-     [C.c_int32, C.c_void_p, C.POINTER(SamplingC), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
-      C.c_char_p, C.c_size_t]),
+     [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+      C.c_size_t]),
 ]
 
 _lib = None

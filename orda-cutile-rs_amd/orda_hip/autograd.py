@@ -21,9 +21,9 @@ from typing import Optional, Tuple
 import torch
 
 from . import (Context, distillation_loss, embedding, linear_cross_entropy,
-               linear_cross_entropy_backward, rms_norm, rms_norm_backward)
+               linear_cross_entropy_backward, rms_norm_backward)
 from . import _lib as L
-from .operators import _embed_grad, _gpu_tensor, _ids, _padding_row
+from .operators import _embed_grad, _gpu_tensor, _ids, _norm_args, _norm_forward, _norm_grad, _padding_row
 from .types import LossOptions, OrdaError, Teacher, TeacherMode
 
 
@@ -209,11 +209,18 @@ class RmsNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(fctx, x, weight, residual, eps, weight_offset):
-        if residual is None:
-            out, total = rms_norm(x, weight, eps=eps, weight_offset=weight_offset), None
-        else:
-            out, total = rms_norm(x, weight, residual=residual, eps=eps, weight_offset=weight_offset)
-        fctx.save_for_backward(x if total is None else total, weight)
+        out, total, (a, m, w, _) = _norm_forward(x, weight, residual, eps, weight_offset)
+        shape = x.shape
+        if len(shape) != 2:
+            out, total = out.view(shape), total.view(shape) if total is not None else None
+        t = x if total is None else total
+        fctx.save_for_backward(t, weight)
+        # the backward's arguments, where they point into what is saved
+        fctx.args = None
+        if m.numel() and w is weight and (total is not None or (m.data_ptr() == x.data_ptr() and x.is_contiguous())):
+            if total is not None:
+                a = _norm_args(total, weight, None, eps, weight_offset)[0]
+            fctx.args = a
         fctx.opts = eps, weight_offset
         fctx.set_materialize_grads(False)
         return out, total
@@ -222,12 +229,21 @@ class RmsNormFunction(torch.autograd.Function):
     def backward(fctx, g_out, g_total):
         want_x, want_w, want_r = fctx.needs_input_grad[:3]
         total, weight = fctx.saved_tensors
-        eps, weight_offset = fctx.opts
         if g_out is None:   # the norm's result went nowhere
             return (g_total if want_x else None, torch.zeros_like(weight) if want_w else None,
                     g_total if want_r else None, None, None)
-        gx, gw = rms_norm_backward(g_out, total, weight, grad_total=g_total, eps=eps, weight_offset=weight_offset,
-                                   grad_x=want_x or want_r, grad_weight=want_w)
+        if fctx.args is None:
+            eps, weight_offset = fctx.opts
+            gx, gw = rms_norm_backward(g_out, total, weight, grad_total=g_total, eps=eps, weight_offset=weight_offset,
+                                       grad_x=want_x or want_r, grad_weight=want_w)
+        else:
+            _gpu_tensor(g_out, "grad_out")
+            if g_total is not None:
+                _gpu_tensor(g_total, "grad_total")
+            t = total if total.dim() == 2 else total.view(-1, weight.size(0))
+            gx, gw = _norm_grad(fctx.args, t, weight, g_out, g_total, want_x or want_r, want_w)
+            if gx is not None and total.dim() != 2:
+                gx = gx.view(total.shape)
         return gx if want_x else None, gw, gx if want_r else None, None, None
 
 

@@ -407,6 +407,41 @@ def fp8_block_matmul(a, a_scales, b, b_scales, *, out_dtype=None):
     return out
 
 
+# Structures packed into one buffer with the message's place behind them: a call of a
+# few tensors costs half of what ctypes' structures take.
+_TENSOR = "Qqqqii"                                                  # orda_tensor
+_NORM = struct.Struct("=" + 3 * _TENSOR + "dd")                     # orda_rms_norm
+_ROWS = struct.Struct("=" + _TENSOR)
+_NORM_OUT = struct.Struct("=" + 2 * _TENSOR)                        # total, out
+_NORM_FP8 = struct.Struct("=" + _TENSOR + "QqqqQqqi4x")             # total, orda_fp8_matrix
+_NORM_GRADS = struct.Struct("=" + 4 * _TENSOR)                      # grad_out, grad_total, grad_x, grad_weight
+_NO_TENSOR = (0, 0, 0, 0, 0, 0)
+
+
+def _packed(data: bytes):
+    """A buffer that holds data and a message, its address and the message's."""
+    buf = C.create_string_buffer(data, len(data) + 512)
+    p = C.addressof(buf)
+    return buf, p, p + len(data)
+
+
+def _check(rc: int, message: int):
+    if rc != L.ORDA_OK:
+        raise OrdaError(C.string_at(message).decode(), rc)
+
+
+def _fields(x, what: str):
+    """orda_tensor of a _matrix."""
+    r, c = x.shape
+    return x.data_ptr(), r, c, x.stride(0) if r > 1 else c, _dtype(x, what), L.DEVICE
+
+
+def _row_fields(x, what: str):
+    """orda_tensor of a contiguous vector as one row."""
+    n = x.numel()
+    return x.data_ptr(), 1, n, n, _dtype(x, what), L.DEVICE
+
+
 # ------------------------------------------------------------------ root-mean-square norm
 def _rows(x, h: int, what: str):
     """x [..., h] as a _matrix."""
@@ -415,37 +450,53 @@ def _rows(x, h: int, what: str):
     return _matrix(x.reshape(-1, h) if h else x.new_empty((math.prod(x.shape[:-1]), 0)), what)
 
 
-def _weight(weight, h: int, device):
-    w = _gpu_tensor(weight, "weight")
-    _same_device(device, weight=w)
-    if w.dim() != 1 or w.size(0) != h:
-        raise OrdaError(f"weight must be [{h}]")
-    return w.contiguous()
-
-
-def _row_desc(w, what: str) -> L.Tensor:
-    """orda_tensor of a contiguous vector as one row."""
-    n = w.size(0)
-    return L.Tensor(w.data_ptr(), 1, n, n, _dtype(w, what), L.DEVICE)
-
-
 def _norm_args(x, weight, residual, eps: float, weight_offset: float):
-    """(orda_rms_norm, x as a matrix, the tensors it points into)."""
+    """(orda_rms_norm, x as a matrix, weight, residual as they are pointed to)."""
     x = _gpu_tensor(x, "x")
     if x.dim() < 1:
         raise OrdaError("x must be [..., H]")
     h = x.size(-1)
-    w = _weight(weight, h, x.device)
+    w = _gpu_tensor(weight, "weight")
+    if w.device != x.device:
+        raise OrdaError(f"weight is on {w.device}, not on {x.device}")
+    if w.dim() != 1 or w.size(0) != h:
+        raise OrdaError(f"weight must be [{h}]")
+    w = w.contiguous()
     m, r = _rows(x, h, "x"), None
-    a = L.RmsNormC(x=_desc(m, "x"), weight=_row_desc(w, "weight"), eps=eps, weight_offset=weight_offset)
     if residual is not None:
         r = _gpu_tensor(residual, "residual")
-        _same_device(x.device, residual=r)
+        if r.device != x.device:
+            raise OrdaError(f"residual is on {r.device}, not on {x.device}")
         if r.shape != x.shape or r.dtype != x.dtype:
             raise OrdaError("residual must have the shape and dtype of x")
         r = _rows(r, h, "residual")
-        a.residual = _desc(r, "residual")
-    return a, m, (w, r)
+    a = _NORM.pack(*_fields(m, "x"), *(_fields(r, "residual") if r is not None else _NO_TENSOR),
+                   *_row_fields(w, "weight"), eps, weight_offset)
+    return a, m, w, r
+
+
+def _like(m):
+    """An empty matrix of a _matrix's shape and type, row by row."""
+    torch = _torch()
+    return torch.empty_like(m) if m.is_contiguous() else torch.empty(m.shape, dtype=m.dtype, device=m.device)
+
+
+def _norm_forward(x, weight, residual, eps: float, weight_offset: float):
+    """rms_norm's result and sum (None without a residual) as matrices, and the arguments."""
+    a, m, w, _r = args = _norm_args(x, weight, residual, eps, weight_offset)
+    out = _like(m)
+    o = _fields(out, "out")
+    total = None
+    if residual is not None:
+        total = _like(m)
+        outs = _NORM_OUT.pack(total.data_ptr(), *o[1:], *o)
+    else:
+        outs = _NORM_OUT.pack(*_NO_TENSOR, *o)
+    _buf, p, message = _packed(a + outs)
+    device = m.device
+    _check(L.load().orda_rms_norm_forward(device.index, _stream(device), p, p + _NORM.size, p + _NORM.size + _ROWS.size,
+                                          message, 512), message)
+    return out, total, args
 
 
 def rms_norm(x, weight, *, residual=None, eps: float = 1e-6, weight_offset: float = 0.0):
@@ -456,12 +507,7 @@ def rms_norm(x, weight, *, residual=None, eps: float = 1e-6, weight_offset: floa
     them. ``t`` is rounded to x's type, the mean formed in 64 bits, the result
     rounded once to x's type. Returns the result, with a residual ``(result, t)``.
     """
-    torch = _torch()
-    a, m, _keep = _norm_args(x, weight, residual, eps, weight_offset)
-    out = torch.empty(m.shape, dtype=m.dtype, device=m.device)
-    total = torch.empty_like(out) if residual is not None else None
-    _call(L.load().orda_rms_norm_forward, m.device.index, _stream(m.device), C.byref(a),
-          C.byref(_desc(total, "total")) if total is not None else None, C.byref(_desc(out, "out")))
+    out, total, _ = _norm_forward(x, weight, residual, eps, weight_offset)
     if x.dim() != 2:
         out, total = out.view(x.shape), total.view(x.shape) if total is not None else None
     return out if total is None else (out, total)
@@ -473,17 +519,20 @@ def rms_norm_fp8(x, weight, *, residual=None, eps: float = 1e-6, weight_offset: 
     are those that ``quantize_fp8_blocks`` gives of the result in float32 (which is not
     rounded to x's type before), laid out as ``fp8_block_matmul`` reads them best."""
     torch = _torch()
-    a, m, _keep = _norm_args(x, weight, residual, eps, weight_offset)
+    a, m, _w, _r = _norm_args(x, weight, residual, eps, weight_offset)
     n, h = m.shape
+    device = m.device
     pitch, cb = -(-h // 16) * 16, -(-h // 128)
-    codes = torch.empty((n, pitch), dtype=torch.float8_e4m3fn, device=m.device)[:, :h]
-    scales = torch.empty((cb, n), dtype=torch.float32, device=m.device).t()
-    d = L.Fp8MatrixC(codes=codes.data_ptr(), rows=n, cols=h, ld=pitch, scales=scales.data_ptr(), scale_row=1,
-                     scale_col=n, block_rows=1)
-    total = torch.empty(m.shape, dtype=m.dtype, device=m.device) if residual is not None else None
-    _call(L.load().orda_rms_norm_fp8, m.device.index, _stream(m.device), C.byref(a),
-          C.byref(_desc(total, "total")) if total is not None else None, C.byref(d))
-    return (codes, scales) if total is None else (codes, scales, total.view(x.shape))
+    codes = torch.empty((n, pitch), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty((cb, n), dtype=torch.float32, device=device)
+    total = _like(m) if residual is not None else None
+    t = _fields(total, "total") if total is not None else _NO_TENSOR
+    _buf, p, message = _packed(a + _NORM_FP8.pack(*t, codes.data_ptr(), n, h, pitch, scales.data_ptr(), 1, n, 1))
+    _check(L.load().orda_rms_norm_fp8(device.index, _stream(device), p, p + _NORM.size, p + _NORM.size + _ROWS.size,
+                                      message, 512), message)
+    if pitch != h:
+        codes = codes[:, :h]
+    return (codes, scales.t()) if total is None else (codes, scales.t(), total.view(x.shape))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -501,38 +550,46 @@ def rms_norm_backward(grad_out, total, weight, *, grad_total=None, eps: float = 
     residual's gradient; ``grad_weight`` is summed over the rows in float32, in an order
     that the sizes fix, and rounded once to the weight's type. None where not asked for.
     """
-    torch = _torch()
-    a, t, _keep = _norm_args(total, weight, None, eps, weight_offset)
-    h = t.size(1)
-    grads = []
+    a, t, w, _ = _norm_args(total, weight, None, eps, weight_offset)
+    if grad_out is None:
+        raise OrdaError("grad_out must be a GPU tensor")
     for g, what in ((grad_out, "grad_out"), (grad_total, "grad_total")):
-        if g is None:
-            if what == "grad_out":
-                raise OrdaError("grad_out must be a GPU tensor")
-            grads.append(None)
-            continue
-        g = _gpu_tensor(g, what)
-        _same_device(t.device, **{what: g})
-        if g.shape != total.shape or g.dtype != t.dtype:
+        if g is not None and (_gpu_tensor(g, what).shape != total.shape or g.dtype != t.dtype):
             raise OrdaError(f"{what} must have the shape and dtype of total")
-        grads.append(_rows(g, h, what))
-    g, gt = grads
-    w = _keep[0]
-    gx = torch.empty(t.shape, dtype=t.dtype, device=t.device) if grad_x else None
-    gw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if grad_weight else None
-    b = _norm_bytes(t.size(0), h)
-    ws = _bytes(b, t.device)
-    _call(L.load().orda_rms_norm_backward, t.device.index, _stream(t.device), C.byref(a),
-          C.byref(_desc(g, "grad_out")), C.byref(_desc(gt, "grad_total")) if gt is not None else None,
-          C.byref(_desc(gx, "grad_x")) if gx is not None else None,
-          C.byref(_row_desc(gw, "grad_weight")) if gw is not None else None, ws.data_ptr(), b)
+    gx, gw = _norm_grad(a, t, w, grad_out, grad_total, grad_x, grad_weight)
     return gx.view(total.shape) if gx is not None else None, gw
 
 
+def _norm_grad(a: bytes, t, w, g, gt, want_x: bool, want_w: bool):
+    """rms_norm_backward of a matrix t, its weight and orda_rms_norm; gradients of t's
+    shape and dtype."""
+    torch = _torch()
+    n, h = t.shape
+    device = t.device
+    if g.device != device or (gt is not None and gt.device != device):
+        raise OrdaError(f"gradients must be on {device}")
+    if g.dim() != 2 or not g.is_contiguous():
+        g = _rows(g, h, "grad_out")
+    f = _fields(g, "grad_out")
+    ft = _NO_TENSOR
+    if gt is not None:
+        if gt.dim() != 2 or not gt.is_contiguous():
+            gt = _rows(gt, h, "grad_total")
+        ft = _fields(gt, "grad_total")
+    gx = _like(t) if want_x else None
+    gw = torch.empty_like(w) if want_w else None
+    b = _norm_bytes(n, h)
+    ws = _bytes(b, device)
+    buf, p, message = _packed(a + _NORM_GRADS.pack(
+        *f, *ft, *((gx.data_ptr(), n, h, h, f[4], L.DEVICE) if want_x else _NO_TENSOR),
+        *(_row_fields(gw, "grad_weight") if want_w else _NO_TENSOR)))
+    q = p + _NORM.size
+    _check(L.load().orda_rms_norm_backward(device.index, _stream(device), p, q, q + 40, q + 80, q + 120, ws.data_ptr(), b,
+                                           message, 512), message)
+    return gx, gw
+
+
 # ------------------------------------------------------------------ gradient norm and clipping
-_GRADIENT = struct.Struct("=QqqqiiQqqqii")   # orda_gradient
-
-
 def _view(g, what: str):
     """(rows, cols, pitch) of a tensor's memory: one row where it is dense, in
     whatever order of its dimensions."""
@@ -553,45 +610,72 @@ def _view(g, what: str):
     raise OrdaError(f"{what} must be dense, or a matrix with adjacent columns or rows")
 
 
+@functools.lru_cache(maxsize=64)
+def _gradient_table(n: int):
+    return struct.Struct("=" + n * 2 * _TENSOR)   # orda_gradient
+
+
 def _gradients(grads, out):
-    """(orda_gradient array, their number, device)."""
+    """(orda_gradient array, the gradients, device, destinations)."""
+    torch = _torch()
     grads = list(grads)
     if out is None:
         grads = [g for g in grads if g is not None]
+        to = (None,) * len(grads)
     else:
-        out = list(out)
+        out = to = list(out)
         if len(out) != len(grads):
             raise OrdaError(f"out must have {len(grads)} tensors")
     if not grads:
         raise OrdaError("there are no gradients")
-    buf = bytearray(_GRADIENT.size * len(grads))
     device = _gpu_tensor(grads[0], "gradient 0").device
-    for i, g in enumerate(grads):
-        what = f"gradient {i}"
-        g = _gpu_tensor(g, what)
-        if g.device != device:
-            raise OrdaError(f"{what} is on {g.device}, not on {device}")
-        r, c, ld = _view(g, what)
-        if out is None:
-            _GRADIENT.pack_into(buf, i * _GRADIENT.size, g.data_ptr(), r, c, ld, _dtype(g, what), L.DEVICE,
-                                0, 0, 0, 0, 0, 0)
+    index, strided = device.index, torch.strided
+    f32, bf16, tensor, parameter = torch.float32, torch.bfloat16, torch.Tensor, torch.nn.Parameter
+    recording = torch.is_grad_enabled()
+    fields = []
+
+    def plain(t, what):
+        """What _gpu_tensor checks, for many: (address, type)."""
+        kind, dtype = type(t), getattr(t, "dtype", None)
+        if ((kind is tensor or kind is parameter) and t.get_device() == index and t.layout is strided and not t.is_neg()
+                and (dtype is f32 or dtype is bf16)):
+            try:
+                p = t.data_ptr()
+                if p or not t.numel():
+                    return p, L.F32 if dtype is f32 else L.BF16
+            except RuntimeError:
+                pass
+        _gpu_tensor(t, what)
+        _same_device(device, **{what: t})
+        return t.data_ptr(), _dtype(t, what)
+
+    for i, (g, o) in enumerate(zip(grads, to)):
+        p, dtype = plain(g, f"gradient {i}")
+        if g.is_contiguous():
+            r, c = 1, g.numel()
+            ld = c
+        else:
+            r, c, ld = _view(g, f"gradient {i}")
+        if o is None:
+            if out is not None:
+                raise OrdaError(f"out {i} must be a GPU tensor")
+            fields += (p, r, c, ld, dtype, 1, 0, 0, 0, 0, 0, 0)
             continue
-        o = _gpu_tensor(out[i], f"out {i}")
-        if o.device != device:
-            raise OrdaError(f"out {i} is on {o.device}, not on {device}")
-        if o.shape != g.shape or (g.stride() != o.stride() and not (g.is_contiguous() and o.is_contiguous())):
-            raise OrdaError(f"out {i} must have the shape and strides of {what}")
-        if o.requires_grad and _torch().is_grad_enabled():
+        q, to_dtype = plain(o, f"out {i}")
+        if o.shape != g.shape or not ((r == 1 and c == ld and o.is_contiguous() and g.is_contiguous())
+                                      or o.stride() == g.stride()):
+            raise OrdaError(f"out {i} must have the shape and strides of gradient {i}")
+        if recording and o.requires_grad:
             raise OrdaError(f"out {i} must not require a gradient")
-        _GRADIENT.pack_into(buf, i * _GRADIENT.size, g.data_ptr(), r, c, ld, _dtype(g, what), L.DEVICE,
-                            o.data_ptr(), r, c, ld, _dtype(o, f"out {i}"), L.DEVICE)
-    return (C.c_char * len(buf)).from_buffer(buf), grads, device
+        fields += (p, r, c, ld, dtype, 1, q, r, c, ld, to_dtype, 1)
+    return _gradient_table(len(grads)).pack(*fields), grads, device, out
 
 
-def _norm_workspace(lib, a, n: int, device):
+@functools.lru_cache(maxsize=64)
+def _clip_bytes(n: int) -> int:
     b = C.c_int64()
-    _call(lib.orda_clip_gradients_workspace, a, n, C.byref(b))
-    return _bytes(b.value, device)
+    _call(L.load().orda_clip_gradients_workspace, n, C.byref(b))
+    return b.value
 
 
 def gradient_norm(grads):
@@ -599,12 +683,11 @@ def gradient_norm(grads):
     float32 or bfloat16 GPU tensors of any shape, dense in any order or matrices
     with adjacent columns; None is skipped. Squares and sums are formed in 64 bits."""
     torch = _torch()
-    a, grads, device = _gradients(grads, None)
-    lib = L.load()
-    ws = _norm_workspace(lib, a, len(grads), device)
+    a, grads, device, _ = _gradients(grads, None)
+    b = _clip_bytes(len(grads))
+    ws = _bytes(b, device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    _call(lib.orda_gradient_norm, device.index, _stream(device), a, len(grads), norm.data_ptr(), ws.data_ptr(),
-          ws.numel())
+    _call(L.load().orda_gradient_norm, device.index, _stream(device), a, len(grads), norm.data_ptr(), ws.data_ptr(), b)
     return norm
 
 
@@ -618,23 +701,27 @@ def clip_gradients(grads, max_norm: float, *, eps: float = 1e-6, out=None):
     all of them NaN. Does not wait for the device. Tensors that are written share no
     memory with others of the call."""
     torch = _torch()
-    a, grads, device = _gradients(grads, out)
-    lib = L.load()
-    ws = _norm_workspace(lib, a, len(grads), device)
+    a, grads, device, out = _gradients(grads, out)
+    b = _clip_bytes(len(grads))
+    ws = _bytes(b, device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    _call(lib.orda_clip_gradients, device.index, _stream(device), a, len(grads), max_norm, eps, norm.data_ptr(),
-          ws.data_ptr(), ws.numel())
-    for t in grads if out is None else out:
-        torch.autograd.graph.increment_version(t)   # written in place
+    _call(L.load().orda_clip_gradients, device.index, _stream(device), a, len(grads), max_norm, eps, norm.data_ptr(),
+          ws.data_ptr(), b)
+    torch.autograd.graph.increment_version(grads if out is None else out)   # written in place
     return norm
 
 
 # ------------------------------------------------------------------ drawing tokens
+_SAMPLING = struct.Struct("=" + _TENSOR + "5Q3fi")   # orda_sampling
+
+
 def _per_row(value, n: int, shape, device, what: str, dtype, none):
     """(tensor or None, the one value)."""
-    torch = _torch()
     if value is None:
         return None, none
+    if type(value) is float or type(value) is int:
+        return None, value
+    torch = _torch()
     if not isinstance(value, torch.Tensor):
         return None, value
     v = _gpu_tensor(value, what)
@@ -691,26 +778,22 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=None, top_p=None, m
     _same_device(m.device, uniform=u)
     if u.dtype != torch.float32 or u.shape != shape:
         raise OrdaError(f"uniform must be float32 {list(shape)}")
-    u = u.reshape(-1).contiguous()
+    if u.dim() != 1 or not u.is_contiguous():
+        u = u.reshape(-1).contiguous()
     d = m.device
     t, t1 = _per_row(temperature, n, shape, d, "temperature", torch.float32, 1.0)
     k, k1 = _per_row(top_k, n, shape, d, "top_k", torch.int32, 0)
     p, p1 = _per_row(top_p, n, shape, d, "top_p", torch.float32, 1.0)
     q, q1 = _per_row(min_p, n, shape, d, "min_p", torch.float32, 0.0)
-    a = L.SamplingC(logits=_desc(m, "logits"), uniform=u.data_ptr(), temperature=t1, top_p=p1, min_p=q1,
-                    top_k=max(0, min(int(k1), 2 ** 31 - 1)))
-    if t is not None:
-        a.temperatures = t.data_ptr()
-    if k is not None:
-        a.top_ks = k.data_ptr()
-    if p is not None:
-        a.top_ps = p.data_ptr()
-    if q is not None:
-        a.min_ps = q.data_ptr()
-    b = _sample_bytes(n, v, a.logits.dtype)
+    f = _fields(m, "logits")
+    a = _SAMPLING.pack(*f, u.data_ptr(), t.data_ptr() if t is not None else 0, p.data_ptr() if p is not None else 0,
+                       q.data_ptr() if q is not None else 0, k.data_ptr() if k is not None else 0, t1, p1, q1,
+                       max(0, min(int(k1), 2 ** 31 - 1)))
+    b = _sample_bytes(n, v, f[4])
     ws = _bytes(b, d)
     tokens = torch.empty(shape, dtype=torch.int64, device=d)
-    logprobs = torch.empty(shape, dtype=torch.float32, device=d)
-    _call(L.load().orda_sample_tokens, d.index, _stream(d), C.byref(a), tokens.data_ptr(), logprobs.data_ptr(),
-          ws.data_ptr(), b)
+    logprobs = torch.empty_like(u) if len(shape) == 1 else torch.empty(shape, dtype=torch.float32, device=d)
+    _buf, at, message = _packed(a)
+    _check(L.load().orda_sample_tokens(d.index, _stream(d), at, tokens.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), b,
+                                       message, 512), message)
     return tokens, logprobs

@@ -79,13 +79,10 @@ def test_gradients_beside_one_another_pass_the_checks(pairs):
     assert rc == L.ORDA_ERR_INVALID and "workspace" in err
 
 
-@pytest.mark.parametrize("count, n", [(0, 0), (1, 1), (1, 1 << 39), (57, 1), (1000, 12345), (1 << 16, 70)])
-def test_workspace_has_a_sum_for_each_workgroup(count, n):
-    a = (L.GradientC * max(1, count))()
-    for i in range(count):
-        a[i].src = mat(1, n, i * 4 * n)
+@pytest.mark.parametrize("count", [0, 1, 57, 1000, 1 << 20])
+def test_workspace_has_a_sum_for_each_workgroup(count):
     out, err = C.c_int64(), C.create_string_buffer(512)
-    assert L.load().orda_clip_gradients_workspace(a, count, C.byref(out), err, 512) == L.ORDA_OK
+    assert L.load().orda_clip_gradients_workspace(count, C.byref(out), err, 512) == L.ORDA_OK
     assert 8 * min(count, 1) <= out.value <= 8 * (4096 + count / 32 + 1) + 256
 
 
