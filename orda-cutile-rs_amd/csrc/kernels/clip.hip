@@ -9,6 +9,7 @@
 #include <math.h>
 
 #include "orda_kernels.h"
+#include "wave.h"
 
 namespace orda {
 namespace {
@@ -16,8 +17,7 @@ namespace {
 constexpr int kThreads = 256;
 
 __device__ __forceinline__ double block_sum(double x, double* part) {
-#pragma unroll
-  for (int d = 32; d; d /= 2) x += __shfl_xor(x, d);
+  x = wave_sum(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
   __syncthreads();

@@ -52,5 +52,33 @@ __device__ __forceinline__ void store8(uint8_t* row, int64_t c, int64_t cols, co
   if (c < cols) *reinterpret_cast<fp8_u32x2*>(row + c) = fp8_u32x2{codes4(x, s, r), codes4(x + 4, s, r)};
 }
 
+// The same codes, without a branch on the values: with r the rounded 1/s and q = x·r
+// rounded, x - q·s is exact and q + (x - q·s)·r the rounded quotient (P. Markstein, 1990),
+// where nothing of it is under the normal range: s from 2^-100 on, else `codes4`. (-0
+// keeps its sign, which the remainder of 0 loses.)
+__device__ __forceinline__ void store8_divided(uint8_t* row, int64_t c, int64_t cols, const float (&x)[8], float s) {
+  if (c >= cols) return;
+  if (!(s >= 7.8886e-31f)) {
+    store8(row, c, cols, x, s);
+    return;
+  }
+  const float r = 1.f / s;
+  float q[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float p = x[k] * r;
+    q[k] = __builtin_copysignf(fmaf(fmaf(-p, s, x[k]), r, p), x[k]);
+    q[k] = __builtin_amdgcn_fmed3f(q[k], -kE4m3Max, kE4m3Max);
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    int u = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * k], q[4 * k + 1], 0, false);
+    u = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * k + 2], q[4 * k + 3], u, true);
+    w[k] = static_cast<uint32_t>(u);
+  }
+  *reinterpret_cast<fp8_u32x2*>(row + c) = fp8_u32x2{w[0], w[1]};
+}
+
 }  // namespace
 }  // namespace orda

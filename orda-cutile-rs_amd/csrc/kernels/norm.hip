@@ -4,6 +4,7 @@
 
 #include "fp8_codes.h"
 #include "orda_kernels.h"
+#include "wave.h"
 
 namespace orda {
 namespace {
@@ -32,6 +33,13 @@ __device__ __forceinline__ Raw8<E> fetch8(const E* row, int64_t c, int64_t h) {
     __builtin_memcpy(&r, row + at, sizeof r);
   }
   return r;
+}
+// Makes the compiler convert them anew where they are used next, instead of keeping the
+// values, twice the registers, over a barrier.
+template <typename E>
+__device__ __forceinline__ void again(Raw8<E>& r) {
+#pragma unroll
+  for (size_t i = 0; i < sizeof(E) / 2; ++i) asm volatile("" : "+v"(r.q[i]));
 }
 // Their values, 0 past the row's end.
 template <typename E, bool TAIL>
@@ -69,43 +77,51 @@ __device__ __forceinline__ void put8(E* row, int64_t c, int64_t h, const float (
   }
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int d = 32; d; d /= 2) x += __shfl_xor(x, d);
-  return x;
-}
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int d = 32; d; d /= 2) x += __shfl_xor(x, d);
-  return x;
-}
-
 // Codes and scales of a lane's eight values; 16 lanes hold a block of 128.
 __device__ __forceinline__ void put_codes(const NormArgs& a, int64_t row, int64_t c, const float (&v)[8]) {
   uint32_t m = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) m = abs_bits(v[k]) > m ? abs_bits(v[k]) : m;
-#pragma unroll
-  for (int d = 1; d < 16; d *= 2) {
-    const uint32_t o = __shfl_xor(m, d);
-    m = o > m ? o : m;
-  }
+  m = most_of<16>(m);
   const float s = scale_of(m);
-  store8(a.codes + row * a.ldc, c, a.h, v, s);
+  store8_divided(a.codes + row * a.ldc, c, a.h, v, s);
   if ((threadIdx.x & 15) == 0 && c < a.h) a.scales[row * a.scale_row + c / 128 * a.scale_col] = s;
 }
 
-// v = t·s·(w + offset). To e4m3 in 64 bits, rounded to fp32 at the end: next to a
-// border of two codes fp32's own roundings would decide, and the codes are those of
-// the formula.
+// v = t·s·(w + offset). To e4m3 the factors and products are pairs of fp32 values, each the
+// other's rounding error, and v is their sum, rounded once: next to a border of two codes
+// fp32's own roundings would decide, and the codes are those of the formula. (In 64 bits
+// it took 27 us more at 8192 x 4096.)
+struct Factor {
+  float s, rest;   // of the row
+};
+__device__ __forceinline__ Factor factor_of(double sum, const NormArgs& a) {
+  const double s = 1. / sqrt(sum / static_cast<double>(a.h) + a.eps);
+  const float f = static_cast<float>(s);
+  return {f, static_cast<float>(s - static_cast<double>(f))};
+}
 template <bool FP8>
-__device__ __forceinline__ void normed(const float (&t)[8], double s, const float (&w)[8], double offset, float (&v)[8]) {
+__device__ __forceinline__ void normed(const float (&t)[8], const Factor& f, const float (&w)[8], double offset,
+                                       float (&v)[8]) {
+#pragma clang fp contract(off)   // (a rounding error is of the rounded product)
+  const float o = static_cast<float>(offset), o_rest = static_cast<float>(offset - static_cast<double>(o));
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    if constexpr (FP8) {
-      v[k] = static_cast<float>(static_cast<double>(t[k]) * s * (static_cast<double>(w[k]) + offset));
+    const float u = t[k] * f.s;
+    if constexpr (!FP8) {
+      v[k] = u * (w[k] + o);
     } else {
-      v[k] = t[k] * static_cast<float>(s) * (w[k] + static_cast<float>(offset));
+      const float u_rest = fmaf(t[k], f.rest, fmaf(t[k], f.s, -u));
+      float q = w[k], q_rest = 0.f;
+      if (offset != 0.) {
+        q = w[k] + o;
+        const float b = q - w[k];
+        q_rest = (w[k] - (q - b)) + (o - b) + o_rest;
+      }
+      const float p = u * q;
+      float rest = fmaf(u_rest, q, fmaf(u, q, -p));
+      if (offset != 0.) rest = fmaf(u, q_rest, rest);
+      v[k] = __builtin_copysignf(p + rest, p);   // (-0 stays)
     }
   }
 }
@@ -161,13 +177,13 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(NormArgs a) {
 #pragma unroll
     for (int q = 0; q < kWaves; ++q) sum += part[team][q];
   }
-  const double s = 1. / sqrt(sum / static_cast<double>(a.h) + a.eps);
+  const Factor f = factor_of(sum, a);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int64_t c = (i * NT + at) * int64_t{8};
     float w[8], v[8];
     widened<W, TAIL>(wr[i], c, a.h, w);
-    normed<FP8>(t[i], s, w, a.offset, v);
+    normed<FP8>(t[i], f, w, a.offset, v);
     if constexpr (FP8) {
       if (live) put_codes(a, row, c, v);
     } else {
@@ -205,13 +221,13 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
   sum = 0.;
 #pragma unroll
   for (int q = 0; q < 16; ++q) sum += part[q];
-  const double s = 1. / sqrt(sum / static_cast<double>(a.h) + a.eps);
+  const Factor f = factor_of(sum, a);
   // (Whole waves take part in a block's maximum: the columns past the end are 0.)
   for (int64_t c = threadIdx.x * int64_t{8}; c - threadIdx.x % 64 * 8 < a.h; c += 8192) {
     float t[8], w[8], v[8];
     totals(c, t);
     widened<W, true>(fetch8<W, true>(static_cast<const W*>(a.w), c, a.h), c, a.h, w);
-    normed<FP8>(t, s, w, a.offset, v);
+    normed<FP8>(t, f, w, a.offset, v);
     if constexpr (FP8) put_codes(a, row, c, v);
     else put8<E, true>(static_cast<E*>(a.out) + row * a.ldo, c, a.h, v);
   }
@@ -227,32 +243,29 @@ __device__ __forceinline__ RowGrad row_grad(double sq, float dot, const NormGrad
   return {static_cast<float>(s), static_cast<float>(s * s * (static_cast<double>(dot) / static_cast<double>(a.h)))};
 }
 
-// Workgroups of teams of NT threads, a row a team at a time; a thread's columns of
-// the weight and of its gradient stay in registers. ws: a row of fp32 a workgroup.
+// Workgroups of teams of NT threads, a row a team at a time, the next row's loads under
+// way; a thread's columns of the weight and of its gradient stay in registers. ws: a row
+// of fp32 a workgroup.
+constexpr int kGradThreads = 512;   // 256 registers each: the loads under way and the sums
 template <typename E, typename W, int NT, int NV, bool TAIL>
-__global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a) {
-  constexpr int kTeams = 1024 / NT, kWaves = NT / 64;
+__global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(NormGradArgs a) {
+  constexpr int kTeams = kGradThreads / NT, kWaves = NT / 64;
   __shared__ double part_sq[2][kTeams][kWaves];
   __shared__ float part_dot[2][kTeams][kWaves];
   __shared__ float acc[NT * NV * 8];
   const int team = threadIdx.x / NT, at = threadIdx.x % NT;
-  float q[NV][8], dw[NV][8];
+  const float offset = static_cast<float>(a.offset);
+  Raw8<W> wr[NV];
+  float dw[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int64_t c = (i * NT + at) * int64_t{8};
-    widened<W, TAIL>(fetch8<W, TAIL>(static_cast<const W*>(a.w), c, a.h), c, a.h, q[i]);
+    wr[i] = fetch8<W, TAIL>(static_cast<const W*>(a.w), (i * NT + at) * int64_t{8}, a.h);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      q[i][k] = c + k < a.h ? q[i][k] + static_cast<float>(a.offset) : 0.f;
-      dw[i][k] = 0.f;
-    }
+    for (int k = 0; k < 8; ++k) dw[i][k] = 0.f;
   }
-  const int64_t step = gridDim.x * int64_t{kTeams};
-  int turn = 0;
-  for (int64_t r0 = blockIdx.x * int64_t{kTeams}; r0 < a.n; r0 += step, turn ^= 1) {
-    const bool live = r0 + team < a.n;
-    const int64_t row = live ? r0 + team : a.n - 1;
-    Raw8<E> rg[NV], rt[NV], rx[NV];
+  Raw8<E> rg[NV], rt[NV], rx[NV];
+  auto fetch = [&](int64_t r) {
+    const int64_t row = r + team < a.n ? r + team : a.n - 1;
     const E* pg = static_cast<const E*>(a.g) + row * a.ldg;
     const E* pt = static_cast<const E*>(a.t) + row * a.ldt;
 #pragma unroll
@@ -265,18 +278,30 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) rx[i] = fetch8<E, TAIL>(px, (i * NT + at) * int64_t{8}, a.h);
     }
-    float g[NV][8], t[NV][8];
+  };
+  const int64_t step = gridDim.x * int64_t{kTeams};
+  int turn = 0;
+  fetch(blockIdx.x * int64_t{kTeams});
+  for (int64_t r0 = blockIdx.x * int64_t{kTeams}; r0 < a.n; r0 += step, turn ^= 1) {
+    const bool live = r0 + team < a.n;
+    const int64_t row = r0 + team;
+    Raw8<E> g8[NV], t8[NV], x8[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) g8[i] = rg[i], t8[i] = rt[i], x8[i] = rx[i];
+    if (r0 + step < a.n) fetch(r0 + step);
     double sq = 0.;
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t c = (i * NT + at) * int64_t{8};
-      widened<E, TAIL>(rg[i], c, a.h, g[i]);
-      widened<E, TAIL>(rt[i], c, a.h, t[i]);
+      float g[8], t[8], q[8];
+      widened<E, TAIL>(g8[i], c, a.h, g);
+      widened<E, TAIL>(t8[i], c, a.h, t);
+      widened<W, TAIL>(wr[i], c, a.h, q);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        sq = fma(static_cast<double>(t[i][k]), static_cast<double>(t[i][k]), sq);
-        dot = fmaf(g[i][k] * q[i][k], t[i][k], dot);
+        sq = fma(static_cast<double>(t[k]), static_cast<double>(t[k]), sq);
+        dot = fmaf(g[k] * (q[k] + offset), t[k], dot);
       }
     }
     sq = wave_sum(sq);
@@ -300,13 +325,19 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t c = (i * NT + at) * int64_t{8};
-      float y[8], d[8];
-      if (a.gt) widened<E, TAIL>(rx[i], c, a.h, y);
+      float g[8], t[8], q[8], y[8], d[8];
+      again(g8[i]);
+      again(t8[i]);
+      again(wr[i]);
+      widened<E, TAIL>(g8[i], c, a.h, g);
+      widened<E, TAIL>(t8[i], c, a.h, t);
+      widened<W, TAIL>(wr[i], c, a.h, q);
+      if (a.gt) widened<E, TAIL>(x8[i], c, a.h, y);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        d[k] = f.s * (g[i][k] * q[i][k] - t[i][k] * f.k);
+        d[k] = f.s * (g[k] * (q[k] + offset) - t[k] * f.k);
         if (a.gt) d[k] += y[k];
-        dw[i][k] = fmaf(g[i][k], t[i][k] * f.s, dw[i][k]);
+        dw[i][k] = fmaf(g[k], t[k] * f.s, dw[i][k]);
       }
       if (a.dx) put8<E, TAIL>(static_cast<E*>(a.dx) + row * a.ldd, c, a.h, d);
     }
@@ -326,7 +357,7 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a) {
     __syncthreads();
   }
   float* out = static_cast<float*>(a.ws) + blockIdx.x * a.h;
-  for (int64_t c = threadIdx.x; c < a.h; c += 1024) {
+  for (int64_t c = threadIdx.x; c < a.h; c += kGradThreads) {
     const int v = static_cast<int>(c / 8);
     out[c] = acc[(static_cast<int>(c % 8) * NV + v / NT) * NT + v % NT];
   }
@@ -451,14 +482,14 @@ struct GradLaunch {
 };
 template <typename E, typename W, bool TAIL>
 GradLaunch grad_launch(int64_t h) {
-  if (h <= 512) return {norm_grad_kernel<E, W, 64, 1, TAIL>, 16};
-  if (h <= 2048) return {norm_grad_kernel<E, W, 256, 1, TAIL>, 4};
-  if (h <= 4096) return {norm_grad_kernel<E, W, 256, 2, TAIL>, 4};
-  if (h <= 8192) return {norm_grad_kernel<E, W, 1024, 1, TAIL>, 1};
-  if (h <= 16384) return {norm_grad_kernel<E, W, 1024, 2, TAIL>, 1};
+  if (h <= 512) return {norm_grad_kernel<E, W, 64, 1, TAIL>, 8};
+  if (h <= 2048) return {norm_grad_kernel<E, W, 256, 1, TAIL>, 2};
+  if (h <= 4096) return {norm_grad_kernel<E, W, 256, 2, TAIL>, 2};
+  if (h <= 8192) return {norm_grad_kernel<E, W, 512, 2, TAIL>, 1};
+  if (h <= 16384) return {norm_grad_kernel<E, W, 512, 4, TAIL>, 1};
   return {nullptr, 0};
 }
-int grad_teams(int64_t h) { return h <= 512 ? 16 : h <= 4096 ? 4 : 1; }
+int grad_teams(int64_t h) { return h <= 512 ? 8 : h <= 4096 ? 2 : 1; }
 
 constexpr int64_t kGradBlocks = 256;   // workgroups that keep sums of the weight's gradient
 constexpr int64_t kLongRow = 16384;
@@ -480,7 +511,7 @@ hipError_t norm_grad(const NormGradArgs& a, hipStream_t stream) {
   const GradLaunch l = a.h % 8 ? grad_launch<E, W, true>(a.h) : grad_launch<E, W, false>(a.h);
   if (l.k) {
     count = grad_blocks(a.n, a.h);
-    hipLaunchKernelGGL(l.k, dim3(static_cast<unsigned>(count)), dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL(l.k, dim3(static_cast<unsigned>(count)), dim3(kGradThreads), 0, stream, a);
   } else {
     float* p = static_cast<float*>(a.ws) + (a.n * 2 + 63) / 64 * 64;
     const int64_t bands = grad_bands(a.n, a.h), each = (a.n + bands - 1) / bands;
