@@ -100,29 +100,36 @@ __device__ __forceinline__ Factor factor_of(double sum, const NormArgs& a) {
   const float f = static_cast<float>(s);
   return {f, static_cast<float>(s - static_cast<double>(f))};
 }
+// OFFSET: there is one.
+template <bool OFFSET>
+__device__ __forceinline__ float paired(float t, const Factor& f, float w, float o, float o_rest) {
+#pragma clang fp contract(off)   // (a rounding error is of the rounded product)
+  const float u = t * f.s, u_rest = fmaf(t, f.rest, fmaf(t, f.s, -u));
+  float q = w, q_rest = 0.f;
+  if constexpr (OFFSET) {
+    q = w + o;
+    const float b = q - w;
+    q_rest = (w - (q - b)) + (o - b) + o_rest;
+  }
+  const float p = u * q;
+  float rest = fmaf(u_rest, q, fmaf(u, q, -p));
+  if constexpr (OFFSET) rest = fmaf(u, q_rest, rest);
+  return __builtin_copysignf(p + rest, p);   // (-0 stays)
+}
 template <bool FP8>
 __device__ __forceinline__ void normed(const float (&t)[8], const Factor& f, const float (&w)[8], double offset,
                                        float (&v)[8]) {
-#pragma clang fp contract(off)   // (a rounding error is of the rounded product)
-  const float o = static_cast<float>(offset), o_rest = static_cast<float>(offset - static_cast<double>(o));
+  const float o = static_cast<float>(offset);
+  if constexpr (!FP8) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float u = t[k] * f.s;
-    if constexpr (!FP8) {
-      v[k] = u * (w[k] + o);
-    } else {
-      const float u_rest = fmaf(t[k], f.rest, fmaf(t[k], f.s, -u));
-      float q = w[k], q_rest = 0.f;
-      if (offset != 0.) {
-        q = w[k] + o;
-        const float b = q - w[k];
-        q_rest = (w[k] - (q - b)) + (o - b) + o_rest;
-      }
-      const float p = u * q;
-      float rest = fmaf(u_rest, q, fmaf(u, q, -p));
-      if (offset != 0.) rest = fmaf(u, q_rest, rest);
-      v[k] = __builtin_copysignf(p + rest, p);   // (-0 stays)
-    }
+    for (int k = 0; k < 8; ++k) v[k] = t[k] * f.s * (w[k] + o);
+  } else if (offset == 0.) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = paired<false>(t[k], f, w[k], 0.f, 0.f);
+  } else {
+    const float o_rest = static_cast<float>(offset - static_cast<double>(o));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = paired<true>(t[k], f, w[k], o, o_rest);
   }
 }
 
@@ -463,7 +470,7 @@ NormLaunch norm_launch(int64_t n, int64_t h) {
   }
   if (h <= 1024) return {norm_kernel<E, W, 64, 2, TAIL, FP8>, 256, 4};
   if (h <= 2048) return {norm_kernel<E, W, 64, 4, TAIL, FP8>, 256, 4};
-  if (h <= 4096) return {norm_kernel<E, W, 64, 8, TAIL, FP8>, 256, 4};
+  if (h <= 4096) return {norm_kernel<E, W, 128, 4, TAIL, FP8>, 256, 2};
   if (h <= 8192) return {norm_kernel<E, W, 256, 4, TAIL, FP8>, 256, 1};
   if (h <= 32768) return {norm_kernel<E, W, 1024, 4, TAIL, FP8>, 1024, 1};
   return {norm_long_kernel<E, W, FP8>, 1024, 1};
