@@ -48,6 +48,7 @@ NormArgs kernel_args(const orda_rms_norm& a, const Types& t, const orda_tensor* 
   k.n = a.x.rows;
   k.h = a.x.cols;
   k.eps = a.eps;
+  k.per_column = 1. / static_cast<double>(k.h);   // (not used where there is no column)
   k.offset = a.weight_offset;
   if (total && total->data) {
     check_like(*total, a.x, t.rows, "total");
@@ -132,6 +133,7 @@ int32_t orda_rms_norm_backward(int32_t device, void* hip_stream, const orda_rms_
     k.n = args->x.rows;
     k.h = args->x.cols;
     k.eps = args->eps;
+    k.per_column = 1. / static_cast<double>(k.h);
     k.offset = args->weight_offset;
     if (grad_x && grad_x->data) {
       check_like(*grad_x, args->x, t.rows, "grad_x");

@@ -52,24 +52,31 @@ __device__ __forceinline__ void store8(uint8_t* row, int64_t c, int64_t cols, co
   if (c < cols) *reinterpret_cast<fp8_u32x2*>(row + c) = fp8_u32x2{codes4(x, s, r), codes4(x + 4, s, r)};
 }
 
-// The same codes, without a branch on the values: with r the rounded 1/s and q = x·r
-// rounded, x - q·s is exact and q + (x - q·s)·r the rounded quotient (P. Markstein, 1990),
-// where nothing of it is under the normal range: s from 2^-100 on, else `codes4`. (-0
-// keeps its sign, which the remainder of 0 loses.)
+// The same scale and codes without divisions or a branch on the values: with r the
+// rounded 1/s and q = x·r rounded, q·s - x is exact and q - (q·s - x)·r the rounded
+// quotient (P. Markstein, 1990) where nothing of it is under the normal range: values
+// whose largest is over 2^-90. (Signs as written: a zero keeps its own.)
+__device__ __forceinline__ float quotient(float x, float s, float r) {
+  const float q = x * r;
+  return fmaf(-fmaf(q, s, -x), r, q);
+}
+__device__ __forceinline__ float scale_divided(uint32_t amax_bits) {
+  constexpr float kReciprocal = 1.f / kE4m3Max;
+  const float m = __uint_as_float(amax_bits);
+  return amax_bits - 0x12800000u < 0x7f800000u - 0x12800000u ? quotient(m, kE4m3Max, kReciprocal) : scale_of(amax_bits);
+}
 __device__ __forceinline__ void store8_divided(uint8_t* row, int64_t c, int64_t cols, const float (&x)[8], float s) {
   if (c >= cols) return;
-  if (!(s >= 7.8886e-31f)) {
+  if (!(s >= 1.8e-30f)) {   // 2^-99; also NaN
     store8(row, c, cols, x, s);
     return;
   }
-  const float r = 1.f / s;
+  float r = __builtin_amdgcn_rcpf(s);
+  r = fmaf(fmaf(-s, r, 1.f), r, r);
+  r = fmaf(fmaf(-s, r, 1.f), r, r);
   float q[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float p = x[k] * r;
-    q[k] = __builtin_copysignf(fmaf(fmaf(-p, s, x[k]), r, p), x[k]);
-    q[k] = __builtin_amdgcn_fmed3f(q[k], -kE4m3Max, kE4m3Max);
-  }
+  for (int k = 0; k < 8; ++k) q[k] = __builtin_amdgcn_fmed3f(quotient(x[k], s, r), -kE4m3Max, kE4m3Max);
   uint32_t w[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {

@@ -18,8 +18,9 @@ struct Raw8 {
 };
 
 // Columns c to c + 7 of a row of h. Every lane loads, those past the row's end from
-// within it, so that no branch makes a load wait for the one before. TAIL (h no
-// multiple of 8): the last eight that the row has, moved into place by `widened`.
+// within it, so that no branch makes a load wait for the one before; `settle` then puts
+// zeros there. TAIL (h no multiple of 8): the last eight that the row has, which it moves
+// into place.
 template <typename E, bool TAIL>
 __device__ __forceinline__ Raw8<E> fetch8(const E* row, int64_t c, int64_t h) {
   Raw8<E> r;
@@ -34,6 +35,41 @@ __device__ __forceinline__ Raw8<E> fetch8(const E* row, int64_t c, int64_t h) {
   }
   return r;
 }
+template <typename E, bool TAIL>
+__device__ __forceinline__ void settle(Raw8<E>& r, int64_t c, int64_t h) {
+  constexpr int kWords = 2 * sizeof(E);
+  const int64_t past = TAIL ? c - (h - 8) : c < h ? 0 : 8;
+  if ((TAIL && h < 8) || !__any(past > 0)) return;   // (whole waves: most)
+  const int d = past < 0 ? 0 : past < 8 ? static_cast<int>(past) : 8;
+  uint32_t w[kWords];
+  __builtin_memcpy(w, &r, sizeof r);
+  if constexpr (TAIL) {   // by d values: 4, 2 and 1 of them
+    auto move = [&](int b, int words) {
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) w[k] = (d & b) ? (k + words < kWords ? w[k + words] : 0u) : w[k];
+    };
+    move(4, sizeof(E));
+    move(2, sizeof(E) / 2);
+    if constexpr (sizeof(E) == 4) {
+      move(1, 1);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) {
+        const uint32_t next = k + 1 < kWords ? w[k + 1] : 0u;
+        w[k] = (d & 1) ? __builtin_amdgcn_alignbit(next, w[k], 16) : w[k];
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kWords; ++k) w[k] = d >= 8 ? 0u : w[k];
+  __builtin_memcpy(&r, w, sizeof r);
+}
+template <typename E, bool TAIL>
+__device__ __forceinline__ Raw8<E> settled8(const E* row, int64_t c, int64_t h) {
+  Raw8<E> r = fetch8<E, TAIL>(row, c, h);
+  settle<E, TAIL>(r, c, h);
+  return r;
+}
 // Makes the compiler convert them anew where they are used next, instead of keeping the
 // values, twice the registers, over a barrier.
 template <typename E>
@@ -41,33 +77,17 @@ __device__ __forceinline__ void again(Raw8<E>& r) {
 #pragma unroll
   for (size_t i = 0; i < sizeof(E) / 2; ++i) asm volatile("" : "+v"(r.q[i]));
 }
-// Their values, 0 past the row's end.
-template <typename E, bool TAIL>
-__device__ __forceinline__ void widened(const Raw8<E>& r, int64_t c, int64_t h, float (&x)[8]) {
+template <typename E>
+__device__ __forceinline__ void widened(const Raw8<E>& r, float (&x)[8]) {
   E v[8];
   __builtin_memcpy(v, &r, sizeof r);
 #pragma unroll
   for (int k = 0; k < 8; ++k) x[k] = static_cast<float>(v[k]);
-  if constexpr (TAIL) {
-    if (h < 8) return;
-    const int64_t past = c - (h - 8);
-    const int d = past < 0 ? 0 : past < 8 ? static_cast<int>(past) : 8;
-#pragma unroll
-    for (int b = 4; b; b /= 2)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = (d & b) ? (k + b < 8 ? x[k + b] : 0.f) : x[k];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = d >= 8 ? 0.f : x[k];
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = c < h ? x[k] : 0.f;
-  }
 }
 template <typename E, bool TAIL>
-__device__ __forceinline__ void put8(E* row, int64_t c, int64_t h, const float (&x)[8]) {
+__device__ __forceinline__ void put8(E* row, int64_t c, int64_t h, const Raw8<E>& x) {
   E v[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = static_cast<E>(x[k]);
+  __builtin_memcpy(v, &x, sizeof v);
   if (c + 8 <= h) {
     __builtin_memcpy(row + c, v, sizeof v);
   } else if (TAIL) {
@@ -77,13 +97,23 @@ __device__ __forceinline__ void put8(E* row, int64_t c, int64_t h, const float (
   }
 }
 
+template <typename E, bool TAIL>
+__device__ __forceinline__ void put8(E* row, int64_t c, int64_t h, const float (&x)[8]) {
+  E v[8];
+  Raw8<E> r;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = static_cast<E>(x[k]);
+  __builtin_memcpy(&r, v, sizeof v);
+  put8<E, TAIL>(row, c, h, r);
+}
+
 // Codes and scales of a lane's eight values; 16 lanes hold a block of 128.
 __device__ __forceinline__ void put_codes(const NormArgs& a, int64_t row, int64_t c, const float (&v)[8]) {
   uint32_t m = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) m = abs_bits(v[k]) > m ? abs_bits(v[k]) : m;
   m = most_of<16>(m);
-  const float s = scale_of(m);
+  const float s = scale_divided(m);
   store8_divided(a.codes + row * a.ldc, c, a.h, v, s);
   if ((threadIdx.x & 15) == 0 && c < a.h) a.scales[row * a.scale_row + c / 128 * a.scale_col] = s;
 }
@@ -95,8 +125,18 @@ __device__ __forceinline__ void put_codes(const NormArgs& a, int64_t row, int64_
 struct Factor {
   float s, rest;   // of the row
 };
+// 1/sqrt(x) from the instruction's 24 bits and Newton's steps (0 and infinity as they
+// come): a sixth of the instructions of a square root and a division.
+__device__ __forceinline__ double reciprocal_root(double x) {
+  const double y0 = __builtin_amdgcn_rsq(x);
+  const double half = .5 * x;
+  double y = y0;
+  y = fma(y, fma(-half * y, y, .5), y);
+  y = fma(y, fma(-half * y, y, .5), y);
+  return y0 > 0. && y0 < INFINITY ? y : y0;
+}
 __device__ __forceinline__ Factor factor_of(double sum, const NormArgs& a) {
-  const double s = 1. / sqrt(sum / static_cast<double>(a.h) + a.eps);
+  const double s = reciprocal_root(fma(sum, a.per_column, a.eps));
   const float f = static_cast<float>(s);
   return {f, static_cast<float>(s - static_cast<double>(f))};
 }
@@ -111,10 +151,11 @@ __device__ __forceinline__ float paired(float t, const Factor& f, float w, float
     const float b = q - w;
     q_rest = (w - (q - b)) + (o - b) + o_rest;
   }
+  // (what is to be added with its sign turned: a -0 stays one)
   const float p = u * q;
-  float rest = fmaf(u_rest, q, fmaf(u, q, -p));
-  if constexpr (OFFSET) rest = fmaf(u, q_rest, rest);
-  return __builtin_copysignf(p + rest, p);   // (-0 stays)
+  float less = fmaf(-u_rest, q, fmaf(-u, q, p));
+  if constexpr (OFFSET) less = fmaf(-u, q_rest, less);
+  return p - less;
 }
 template <bool FP8>
 __device__ __forceinline__ void normed(const float (&t)[8], const Factor& f, const float (&w)[8], double offset,
@@ -142,40 +183,51 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(NormArgs a) {
   const int64_t row0 = blockIdx.x * int64_t{kTeams} + team;
   const bool live = row0 < a.n;
   const int64_t row = live ? row0 : a.n - 1;
-  Raw8<E> x[NV], r[NV];
-  Raw8<W> wr[NV];
+  Raw8<E> t[NV];   // the sum, as it lies in memory
   const E* px = static_cast<const E*>(a.x) + row * a.ldx;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) x[i] = fetch8<E, TAIL>(px, (i * NT + at) * int64_t{8}, a.h);
+  for (int i = 0; i < NV; ++i) t[i] = fetch8<E, TAIL>(px, (i * NT + at) * int64_t{8}, a.h);
+  double sum = 0.;
+  auto add = [&](const float (&v)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum = fma(static_cast<double>(v[k]), static_cast<double>(v[k]), sum);
+  };
   if (a.r) {
+    Raw8<E> r[NV];
     const E* pr = static_cast<const E*>(a.r) + row * a.ldr;
 #pragma unroll
     for (int i = 0; i < NV; ++i) r[i] = fetch8<E, TAIL>(pr, (i * NT + at) * int64_t{8}, a.h);
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) wr[i] = fetch8<W, TAIL>(static_cast<const W*>(a.w), (i * NT + at) * int64_t{8}, a.h);
-  float t[NV][8];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) widened<E, TAIL>(x[i], (i * NT + at) * int64_t{8}, a.h, t[i]);
-  if (a.r) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float y[8];
-      widened<E, TAIL>(r[i], (i * NT + at) * int64_t{8}, a.h, y);
+      const int64_t c = (i * NT + at) * int64_t{8};
+      float v[8], y[8];
+      E e[8];
+      settle<E, TAIL>(t[i], c, a.h);
+      settle<E, TAIL>(r[i], c, a.h);
+      widened(t[i], v);
+      widened(r[i], y);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) t[i][k] = static_cast<float>(static_cast<E>(t[i][k] + y[k]));
+      for (int k = 0; k < 8; ++k) e[k] = static_cast<E>(v[k] + y[k]);
+      __builtin_memcpy(&t[i], e, sizeof e);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(e[k]);
+      add(v);
+      if (a.total && live) put8<E, TAIL>(static_cast<E*>(a.total) + row * a.ldt, c, a.h, t[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (i * NT + at) * int64_t{8};
+      float v[8];
+      settle<E, TAIL>(t[i], c, a.h);
+      widened(t[i], v);
+      add(v);
+      if (a.total && live) put8<E, TAIL>(static_cast<E*>(a.total) + row * a.ldt, c, a.h, t[i]);
     }
   }
-  if (a.total && live) {
+  Raw8<W> wr[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      put8<E, TAIL>(static_cast<E*>(a.total) + row * a.ldt, (i * NT + at) * int64_t{8}, a.h, t[i]);
-  }
-  double sum = 0.;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sum = fma(static_cast<double>(t[i][k]), static_cast<double>(t[i][k]), sum);
+  for (int i = 0; i < NV; ++i) wr[i] = fetch8<W, TAIL>(static_cast<const W*>(a.w), (i * NT + at) * int64_t{8}, a.h);
   sum = wave_sum(sum);
   if constexpr (kWaves > 1) {
     if ((at & 63) == 0) part[team][at >> 6] = sum;
@@ -188,9 +240,12 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_kernel(NormArgs a) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int64_t c = (i * NT + at) * int64_t{8};
-    float w[8], v[8];
-    widened<W, TAIL>(wr[i], c, a.h, w);
-    normed<FP8>(t[i], f, w, a.offset, v);
+    float w[8], v[8], y[8];
+    again(t[i]);
+    settle<W, TAIL>(wr[i], c, a.h);
+    widened(wr[i], w);
+    widened(t[i], y);
+    normed<FP8>(y, f, w, a.offset, v);
     if constexpr (FP8) {
       if (live) put_codes(a, row, c, v);
     } else {
@@ -207,10 +262,10 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
   const E* px = static_cast<const E*>(a.x) + row * a.ldx;
   const E* pr = a.r ? static_cast<const E*>(a.r) + row * a.ldr : nullptr;
   auto totals = [&](int64_t c, float (&t)[8]) {
-    widened<E, true>(fetch8<E, true>(px, c, a.h), c, a.h, t);
+    widened(settled8<E, true>(px, c, a.h), t);
     if (!pr) return;
     float y[8];
-    widened<E, true>(fetch8<E, true>(pr, c, a.h), c, a.h, y);
+    widened(settled8<E, true>(pr, c, a.h), y);
 #pragma unroll
     for (int k = 0; k < 8; ++k) t[k] = static_cast<float>(static_cast<E>(t[k] + y[k]));
   };
@@ -233,7 +288,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a) {
   for (int64_t c = threadIdx.x * int64_t{8}; c - threadIdx.x % 64 * 8 < a.h; c += 8192) {
     float t[8], w[8], v[8];
     totals(c, t);
-    widened<W, true>(fetch8<W, true>(static_cast<const W*>(a.w), c, a.h), c, a.h, w);
+    widened(settled8<W, true>(static_cast<const W*>(a.w), c, a.h), w);
     normed<FP8>(t, f, w, a.offset, v);
     if constexpr (FP8) put_codes(a, row, c, v);
     else put8<E, true>(static_cast<E*>(a.out) + row * a.ldo, c, a.h, v);
@@ -246,8 +301,8 @@ struct RowGrad {
   float s, k;   // dx = s·(g·q - t·k) + gt
 };
 __device__ __forceinline__ RowGrad row_grad(double sq, float dot, const NormGradArgs& a) {
-  const double s = 1. / sqrt(sq / static_cast<double>(a.h) + a.eps);
-  return {static_cast<float>(s), static_cast<float>(s * s * (static_cast<double>(dot) / static_cast<double>(a.h)))};
+  const double s = reciprocal_root(fma(sq, a.per_column, a.eps));
+  return {static_cast<float>(s), static_cast<float>(s * s * (static_cast<double>(dot) * a.per_column))};
 }
 
 // Workgroups of teams of NT threads, a row a team at a time, the next row's loads under
@@ -266,7 +321,7 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(NormGradArgs a)
   float dw[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    wr[i] = fetch8<W, TAIL>(static_cast<const W*>(a.w), (i * NT + at) * int64_t{8}, a.h);
+    wr[i] = settled8<W, TAIL>(static_cast<const W*>(a.w), (i * NT + at) * int64_t{8}, a.h);
 #pragma unroll
     for (int k = 0; k < 8; ++k) dw[i][k] = 0.f;
   }
@@ -294,17 +349,22 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(NormGradArgs a)
     const int64_t row = r0 + team;
     Raw8<E> g8[NV], t8[NV], x8[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) g8[i] = rg[i], t8[i] = rt[i], x8[i] = rx[i];
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = (i * NT + at) * int64_t{8};
+      g8[i] = rg[i], t8[i] = rt[i], x8[i] = rx[i];
+      settle<E, TAIL>(g8[i], c, a.h);
+      settle<E, TAIL>(t8[i], c, a.h);
+      if (a.gt) settle<E, TAIL>(x8[i], c, a.h);
+    }
     if (r0 + step < a.n) fetch(r0 + step);
     double sq = 0.;
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c = (i * NT + at) * int64_t{8};
       float g[8], t[8], q[8];
-      widened<E, TAIL>(g8[i], c, a.h, g);
-      widened<E, TAIL>(t8[i], c, a.h, t);
-      widened<W, TAIL>(wr[i], c, a.h, q);
+      widened(g8[i], g);
+      widened(t8[i], t);
+      widened(wr[i], q);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         sq = fma(static_cast<double>(t[k]), static_cast<double>(t[k]), sq);
@@ -336,10 +396,10 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(NormGradArgs a)
       again(g8[i]);
       again(t8[i]);
       again(wr[i]);
-      widened<E, TAIL>(g8[i], c, a.h, g);
-      widened<E, TAIL>(t8[i], c, a.h, t);
-      widened<W, TAIL>(wr[i], c, a.h, q);
-      if (a.gt) widened<E, TAIL>(x8[i], c, a.h, y);
+      widened(g8[i], g);
+      widened(t8[i], t);
+      widened(wr[i], q);
+      if (a.gt) widened(x8[i], y);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         d[k] = f.s * (g[k] * (q[k] + offset) - t[k] * f.k);
@@ -383,9 +443,9 @@ __global__ __launch_bounds__(1024) void norm_grad_rows_kernel(NormGradArgs a) {
   float dot = 0.f;
   for (int64_t c = threadIdx.x * int64_t{8}; c < a.h; c += 8192) {
     float g[8], t[8], q[8];
-    widened<E, true>(fetch8<E, true>(pg, c, a.h), c, a.h, g);
-    widened<E, true>(fetch8<E, true>(pt, c, a.h), c, a.h, t);
-    widened<W, true>(fetch8<W, true>(static_cast<const W*>(a.w), c, a.h), c, a.h, q);
+    widened(settled8<E, true>(pg, c, a.h), g);
+    widened(settled8<E, true>(pt, c, a.h), t);
+    widened(settled8<W, true>(static_cast<const W*>(a.w), c, a.h), q);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       sq = fma(static_cast<double>(t[k]), static_cast<double>(t[k]), sq);
@@ -414,7 +474,7 @@ __global__ __launch_bounds__(256) void norm_grad_tiles_kernel(NormGradArgs a, co
   const int64_t across = (a.h + 2047) / 2048, tile = blockIdx.x % across, band = blockIdx.x / across;
   const int64_t c = (tile * 256 + threadIdx.x) * 8;
   float q[8], dw[8];
-  widened<W, true>(fetch8<W, true>(static_cast<const W*>(a.w), c, a.h), c, a.h, q);
+  widened(settled8<W, true>(static_cast<const W*>(a.w), c, a.h), q);
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     q[k] += static_cast<float>(a.offset);
@@ -423,9 +483,9 @@ __global__ __launch_bounds__(256) void norm_grad_tiles_kernel(NormGradArgs a, co
   const int64_t end = (band + 1) * each < a.n ? (band + 1) * each : a.n;
   for (int64_t row = band * each; row < end; ++row) {
     float g[8], t[8], y[8], d[8];
-    widened<E, true>(fetch8<E, true>(static_cast<const E*>(a.g) + row * a.ldg, c, a.h), c, a.h, g);
-    widened<E, true>(fetch8<E, true>(static_cast<const E*>(a.t) + row * a.ldt, c, a.h), c, a.h, t);
-    if (a.gt) widened<E, true>(fetch8<E, true>(static_cast<const E*>(a.gt) + row * a.ldgt, c, a.h), c, a.h, y);
+    widened(settled8<E, true>(static_cast<const E*>(a.g) + row * a.ldg, c, a.h), g);
+    widened(settled8<E, true>(static_cast<const E*>(a.t) + row * a.ldt, c, a.h), t);
+    if (a.gt) widened(settled8<E, true>(static_cast<const E*>(a.gt) + row * a.ldgt, c, a.h), y);
     const RowGrad f = rows[row];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {

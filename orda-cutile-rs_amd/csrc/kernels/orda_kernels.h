@@ -608,7 +608,7 @@ struct NormArgs {
   int64_t ldx, ldr;
   const void* w;
   int64_t n, h;
-  double eps, offset;
+  double eps, offset, per_column;   // per_column: 1 / h
   void *total, *out;
   int64_t ldt, ldo;
   uint8_t* codes;         // pitch a multiple of 8, as Fp8QuantArgs
@@ -624,7 +624,7 @@ struct NormGradArgs {
   int64_t ldg, ldt, ldgt;
   const void* w;
   int64_t n, h;
-  double eps, offset;
+  double eps, offset, per_column;
   void *dx, *dw;           // written where set
   int64_t ldd;
   void* ws;
