@@ -23,7 +23,8 @@ import torch
 from . import (Context, distillation_loss, embedding, linear_cross_entropy,
                linear_cross_entropy_backward, rms_norm_backward)
 from . import _lib as L
-from .operators import _embed_grad, _gpu_tensor, _ids, _norm_args, _norm_forward, _norm_grad, _padding_row
+from .operators import (_embed_grad, _gpu_tensor, _ids, _norm_args, _norm_bytes, _norm_forward, _NormGrad,
+                        _padding_row)
 from .types import LossOptions, OrdaError, Teacher, TeacherMode
 
 
@@ -207,20 +208,26 @@ class RmsNormFunction(torch.autograd.Function):
     """out, total = RmsNormFunction.apply(x, weight, residual, eps, weight_offset);
     total is None without a residual."""
 
+    # Up to this many bytes of gradients and scratch the backward call is made ready by
+    # the forward's: torch's engine runs a backward's Python on another thread, where it
+    # takes three times as long.
+    READY_BYTES = 8 << 20
+
     @staticmethod
     def forward(fctx, x, weight, residual, eps, weight_offset):
         out, total, (a, m, w, _) = _norm_forward(x, weight, residual, eps, weight_offset)
+        t = m if total is None else total
+        fctx.ready = None
+        want_x, want_w, want_r = fctx.needs_input_grad[:3]
+        if w is weight and m.numel() and t.is_contiguous() and (want_x or want_w or want_r):
+            if t.numel() * t.element_size() + _norm_bytes(*t.shape) <= RmsNormFunction.READY_BYTES:
+                if total is not None:
+                    a = _norm_args(total, weight, None, eps, weight_offset)[0]
+                fctx.ready = _NormGrad(a, t, w, want_x or want_r, want_w)
         shape = x.shape
         if len(shape) != 2:
             out, total = out.view(shape), total.view(shape) if total is not None else None
-        t = x if total is None else total
-        fctx.save_for_backward(t, weight)
-        # the backward's arguments, where they point into what is saved
-        fctx.args = None
-        if m.numel() and w is weight and (total is not None or (m.data_ptr() == x.data_ptr() and x.is_contiguous())):
-            if total is not None:
-                a = _norm_args(total, weight, None, eps, weight_offset)[0]
-            fctx.args = a
+        fctx.save_for_backward(x if total is None else total, weight)
         fctx.opts = eps, weight_offset
         fctx.set_materialize_grads(False)
         return out, total
@@ -232,18 +239,18 @@ class RmsNormFunction(torch.autograd.Function):
         if g_out is None:   # the norm's result went nowhere
             return (g_total if want_x else None, torch.zeros_like(weight) if want_w else None,
                     g_total if want_r else None, None, None)
-        if fctx.args is None:
-            eps, weight_offset = fctx.opts
-            gx, gw = rms_norm_backward(g_out, total, weight, grad_total=g_total, eps=eps, weight_offset=weight_offset,
-                                       grad_x=want_x or want_r, grad_weight=want_w)
-        else:
+        ready, fctx.ready = fctx.ready, None   # (a second backward makes its own)
+        if ready is not None and (ready.gx is not None) == (want_x or want_r) and (ready.gw is not None) == want_w:
             _gpu_tensor(g_out, "grad_out")
             if g_total is not None:
                 _gpu_tensor(g_total, "grad_total")
-            t = total if total.dim() == 2 else total.view(-1, weight.size(0))
-            gx, gw = _norm_grad(fctx.args, t, weight, g_out, g_total, want_x or want_r, want_w)
+            gx, gw = ready.run(g_out, g_total)
             if gx is not None and total.dim() != 2:
                 gx = gx.view(total.shape)
+        else:
+            eps, weight_offset = fctx.opts
+            gx, gw = rms_norm_backward(g_out, total, weight, grad_total=g_total, eps=eps, weight_offset=weight_offset,
+                                       grad_x=want_x or want_r, grad_weight=want_w)
         return gx if want_x else None, gw, gx if want_r else None, None, None
 
 

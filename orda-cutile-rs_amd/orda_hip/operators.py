@@ -556,37 +556,47 @@ def rms_norm_backward(grad_out, total, weight, *, grad_total=None, eps: float = 
     for g, what in ((grad_out, "grad_out"), (grad_total, "grad_total")):
         if g is not None and (_gpu_tensor(g, what).shape != total.shape or g.dtype != t.dtype):
             raise OrdaError(f"{what} must have the shape and dtype of total")
-    gx, gw = _norm_grad(a, t, w, grad_out, grad_total, grad_x, grad_weight)
+    gx, gw = _NormGrad(a, t, w, grad_x, grad_weight).run(grad_out, grad_total)
     return gx.view(total.shape) if gx is not None else None, gw
 
 
-def _norm_grad(a: bytes, t, w, g, gt, want_x: bool, want_w: bool):
-    """rms_norm_backward of a matrix t, its weight and orda_rms_norm; gradients of t's
-    shape and dtype."""
-    torch = _torch()
-    n, h = t.shape
-    device = t.device
-    if g.device != device or (gt is not None and gt.device != device):
-        raise OrdaError(f"gradients must be on {device}")
-    if g.dim() != 2 or not g.is_contiguous():
-        g = _rows(g, h, "grad_out")
-    f = _fields(g, "grad_out")
-    ft = _NO_TENSOR
-    if gt is not None:
-        if gt.dim() != 2 or not gt.is_contiguous():
+class _NormGrad:
+    """A backward call of a matrix t, its weight and orda_rms_norm, made ready: its
+    outputs and scratch, and its arguments but for the gradients that come in."""
+    __slots__ = "buf", "at", "message", "gx", "gw", "ws", "bytes", "t"
+
+    def __init__(self, a: bytes, t, w, want_x: bool, want_w: bool):
+        torch = _torch()
+        n, h = t.shape
+        self.t = t
+        self.gx = _like(t) if want_x else None
+        self.gw = torch.empty_like(w) if want_w else None
+        self.bytes = _norm_bytes(n, h)
+        self.ws = _bytes(self.bytes, t.device)
+        self.buf, self.at, self.message = _packed(a + _NORM_GRADS.pack(
+            *_NO_TENSOR, *_NO_TENSOR, *(_fields(self.gx, "grad_x") if want_x else _NO_TENSOR),
+            *(_row_fields(self.gw, "grad_weight") if want_w else _NO_TENSOR)))
+
+    def run(self, g, gt):
+        """(grad_x, grad_weight), given gradients of t's number of values and dtype."""
+        t = self.t
+        n, h = t.shape
+        device = t.device
+        if g.device != device or (gt is not None and gt.device != device):
+            raise OrdaError(f"gradients must be on {device}")
+        q = self.at + _NORM.size
+        if g.is_contiguous():
+            _ROWS.pack_into(self.buf, _NORM.size, g.data_ptr(), n, h, h, _dtype(g, "grad_out"), L.DEVICE)
+        else:
+            g = _rows(g, h, "grad_out")
+            _ROWS.pack_into(self.buf, _NORM.size, *_fields(g, "grad_out"))
+        if gt is not None:
             gt = _rows(gt, h, "grad_total")
-        ft = _fields(gt, "grad_total")
-    gx = _like(t) if want_x else None
-    gw = torch.empty_like(w) if want_w else None
-    b = _norm_bytes(n, h)
-    ws = _bytes(b, device)
-    buf, p, message = _packed(a + _NORM_GRADS.pack(
-        *f, *ft, *((gx.data_ptr(), n, h, h, f[4], L.DEVICE) if want_x else _NO_TENSOR),
-        *(_row_fields(gw, "grad_weight") if want_w else _NO_TENSOR)))
-    q = p + _NORM.size
-    _check(L.load().orda_rms_norm_backward(device.index, _stream(device), p, q, q + 40, q + 80, q + 120, ws.data_ptr(), b,
-                                           message, 512), message)
-    return gx, gw
+            _ROWS.pack_into(self.buf, _NORM.size + _ROWS.size, *_fields(gt, "grad_total"))
+        message = self.message
+        _check(L.load().orda_rms_norm_backward(device.index, _stream(device), self.at, q, q + 40, q + 80, q + 120,
+                                               self.ws.data_ptr(), self.bytes, message, 512), message)
+        return self.gx, self.gw
 
 
 # ------------------------------------------------------------------ gradient norm and clipping

@@ -342,3 +342,21 @@ def test_refusals():
                   ((x, x, w[:60]), {}), ((x.cpu(), x, w), {})):
         with pytest.raises(H.OrdaError):
             H.rms_norm_backward(*a, **kw)
+
+
+@pytest.mark.parametrize("n", [20, 3000])
+def test_a_second_backward_and_one_that_wants_less(n):
+    """Small and large backward calls, of which the first has its gradients' memory made by the forward."""
+    h = 1024
+    x, w = normal((n, h), "f32").requires_grad_(True), normal((h,), "f32", mean=1.0).requires_grad_(True)
+    g, g2 = normal((n, h), "f32", seed=2), normal((n, h), "f32", seed=3)
+    out = rms_norm_autograd(x, w)
+    first = torch.autograd.grad(out, [x, w], g, retain_graph=True)
+    kept = [t.clone() for t in first]
+    second = torch.autograd.grad(out, [x, w], g2, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, kept))
+    check_grads(*second, g2, x.detach(), w.detach())
+    (gx,) = torch.autograd.grad(out, [x], g, retain_graph=True)
+    assert torch.equal(gx, first[0])
+    (gw,) = torch.autograd.grad(out, [w], g)
+    assert torch.equal(gw, first[1])
