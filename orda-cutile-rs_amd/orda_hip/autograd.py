@@ -23,8 +23,7 @@ import torch
 from . import (Context, distillation_loss, embedding, linear_cross_entropy,
                linear_cross_entropy_backward, rms_norm_backward)
 from . import _lib as L
-from .operators import (_embed_grad, _gpu_tensor, _ids, _norm_args, _norm_bytes, _norm_forward, _NormGrad,
-                        _padding_row)
+from .operators import (_embed_grad, _gpu_tensor, _ids, _norm_args, _norm_forward, _NormGrad, _padding_row)
 from .types import LossOptions, OrdaError, Teacher, TeacherMode
 
 
@@ -208,10 +207,10 @@ class RmsNormFunction(torch.autograd.Function):
     """out, total = RmsNormFunction.apply(x, weight, residual, eps, weight_offset);
     total is None without a residual."""
 
-    # Up to this many bytes of gradients and scratch the backward call is made ready by
-    # the forward's: torch's engine runs a backward's Python on another thread, where it
-    # takes three times as long.
-    READY_BYTES = 8 << 20
+    # The backward call is made ready by the forward's (up to this many bytes of rows
+    # with grad_x and the scratch): torch's engine runs a backward's Python on another thread, where it takes
+    # three times as long.
+    READY_BYTES = 4 << 20
 
     @staticmethod
     def forward(fctx, x, weight, residual, eps, weight_offset):
@@ -220,10 +219,10 @@ class RmsNormFunction(torch.autograd.Function):
         fctx.ready = None
         want_x, want_w, want_r = fctx.needs_input_grad[:3]
         if w is weight and m.numel() and t.is_contiguous() and (want_x or want_w or want_r):
-            if t.numel() * t.element_size() + _norm_bytes(*t.shape) <= RmsNormFunction.READY_BYTES:
-                if total is not None:
-                    a = _norm_args(total, weight, None, eps, weight_offset)[0]
-                fctx.ready = _NormGrad(a, t, w, want_x or want_r, want_w)
+            if total is not None:
+                a = _norm_args(total, weight, None, eps, weight_offset)[0]
+            small = t.numel() * t.element_size() <= RmsNormFunction.READY_BYTES
+            fctx.ready = _NormGrad(a, t.detach(), w.detach(), want_x or want_r, want_w, small)
         shape = x.shape
         if len(shape) != 2:
             out, total = out.view(shape), total.view(shape) if total is not None else None
@@ -240,7 +239,7 @@ class RmsNormFunction(torch.autograd.Function):
             return (g_total if want_x else None, torch.zeros_like(weight) if want_w else None,
                     g_total if want_r else None, None, None)
         ready, fctx.ready = fctx.ready, None   # (a second backward makes its own)
-        if ready is not None and (ready.gx is not None) == (want_x or want_r) and (ready.gw is not None) == want_w:
+        if ready is not None and ready.want_x == (want_x or want_r) and (ready.gw is not None) == want_w:
             _gpu_tensor(g_out, "grad_out")
             if g_total is not None:
                 _gpu_tensor(g_total, "grad_total")

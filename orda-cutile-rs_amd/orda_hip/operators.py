@@ -562,41 +562,48 @@ def rms_norm_backward(grad_out, total, weight, *, grad_total=None, eps: float = 
 
 class _NormGrad:
     """A backward call of a matrix t, its weight and orda_rms_norm, made ready: its
-    outputs and scratch, and its arguments but for the gradients that come in."""
-    __slots__ = "buf", "at", "message", "gx", "gw", "ws", "bytes", "t"
+    arguments but for the gradients that come in and the weight's gradient; with `rows`
+    also grad_x and the scratch, which else are made when it runs."""
+    __slots__ = "buf", "at", "message", "want_x", "gx", "gw", "ws", "bytes", "t", "shape", "dtype"
 
-    def __init__(self, a: bytes, t, w, want_x: bool, want_w: bool):
+    def __init__(self, a: bytes, t, w, want_x: bool, want_w: bool, rows: bool = True):
         torch = _torch()
-        n, h = t.shape
+        n, h = self.shape = t.shape
         self.t = t
-        self.gx = _like(t) if want_x else None
+        self.dtype = _dtype(t, "total")
+        self.want_x = want_x
+        self.gx = _like(t) if want_x and rows else None
         self.gw = torch.empty_like(w) if want_w else None
         self.bytes = _norm_bytes(n, h)
-        self.ws = _bytes(self.bytes, t.device)
+        self.ws = _bytes(self.bytes, t.device) if rows else None
         self.buf, self.at, self.message = _packed(a + _NORM_GRADS.pack(
-            *_NO_TENSOR, *_NO_TENSOR, *(_fields(self.gx, "grad_x") if want_x else _NO_TENSOR),
+            *_NO_TENSOR, *_NO_TENSOR, *(_fields(self.gx, "grad_x") if self.gx is not None else _NO_TENSOR),
             *(_row_fields(self.gw, "grad_weight") if want_w else _NO_TENSOR)))
 
     def run(self, g, gt):
-        """(grad_x, grad_weight), given gradients of t's number of values and dtype."""
-        t = self.t
-        n, h = t.shape
+        """(grad_x, grad_weight), given plain gradients of t's number of values and dtype."""
+        buf, at, t, dtype, gx = self.buf, self.at, self.t, self.dtype, self.gx
+        n, h = self.shape
         device = t.device
         if g.device != device or (gt is not None and gt.device != device):
             raise OrdaError(f"gradients must be on {device}")
-        q = self.at + _NORM.size
-        if g.is_contiguous():
-            _ROWS.pack_into(self.buf, _NORM.size, g.data_ptr(), n, h, h, _dtype(g, "grad_out"), L.DEVICE)
-        else:
+        if not g.is_contiguous():
             g = _rows(g, h, "grad_out")
-            _ROWS.pack_into(self.buf, _NORM.size, *_fields(g, "grad_out"))
+        ld = h if g.dim() != 2 or n == 1 else g.stride(0)
+        _ROWS.pack_into(buf, _NORM.size, g.data_ptr(), n, h, ld, dtype, L.DEVICE)
         if gt is not None:
-            gt = _rows(gt, h, "grad_total")
-            _ROWS.pack_into(self.buf, _NORM.size + _ROWS.size, *_fields(gt, "grad_total"))
-        message = self.message
-        _check(L.load().orda_rms_norm_backward(device.index, _stream(device), self.at, q, q + 40, q + 80, q + 120,
-                                               self.ws.data_ptr(), self.bytes, message, 512), message)
-        return self.gx, self.gw
+            if not gt.is_contiguous():
+                gt = _rows(gt, h, "grad_total")
+            ld = h if gt.dim() != 2 or n == 1 else gt.stride(0)
+            _ROWS.pack_into(buf, _NORM.size + _ROWS.size, gt.data_ptr(), n, h, ld, dtype, L.DEVICE)
+        if gx is None and self.want_x:
+            gx = _like(t)
+            _ROWS.pack_into(buf, _NORM.size + 2 * _ROWS.size, gx.data_ptr(), n, h, h, dtype, L.DEVICE)
+        ws = self.ws if self.ws is not None else _bytes(self.bytes, device)
+        q, message = at + _NORM.size, self.message
+        _check(L.load().orda_rms_norm_backward(device.index, _stream(device), at, q, q + 40, q + 80, q + 120,
+                                               ws.data_ptr(), self.bytes, message, 512), message)
+        return gx, self.gw
 
 
 # ------------------------------------------------------------------ gradient norm and clipping
