@@ -34,7 +34,6 @@ GradPart part_of(const orda_tensor& src, const orda_tensor& dst) {
 // How the gradients are cut: launches of up to kGradParts of them, pieces of a row,
 // one sum for each workgroup.
 struct Cut {
-  int64_t piece;
   std::vector<GradPart> parts;   // those that have values
   struct Launch {
     size_t from, to;
@@ -43,14 +42,20 @@ struct Cut {
   };
   std::vector<Launch> launches;
   int sums = 0;
+  int64_t bytes = 0;             // of all gradients
   bool in_place = false;
 };
 
-int64_t pieces_of(const GradPart& p, int64_t piece) { return p.rows * ceil_div(p.cols, piece); }
+int64_t pieces_of(const GradPart& p) { return p.rows * ceil_div(p.cols, kGradPiece); }
 
-// Workgroups of all launches together: eight a CU. Each of the scaling ones adds all
-// sums up by itself.
-constexpr int64_t kBlocks = 2048;
+// Workgroups of a launch: eight a CU; and of all together, each of which has a sum that
+// every scaling workgroup adds up by itself.
+constexpr int64_t kBlocks = 2048, kSums = 4096;
+
+// The memory's cache: gradients beyond it are read past it for the norm (4.29 GB of fp32:
+// 612 us, through it 730), smaller ones are read from it by the scaling (42 MB: 12 us,
+// had the norm's reads gone past it 16).
+constexpr int64_t kCache = int64_t{256} << 20;
 
 void check_count(int64_t count) {
   if (count < 0 || count > kMostGradients) fail(ORDA_ERR_INVALID, "at most 2^20 gradients");
@@ -60,17 +65,16 @@ Cut cut(const orda_gradient* g, int64_t count, bool scale) {
   check_count(count);
   if (count > 0 && !g) fail(ORDA_ERR_INVALID, "null argument");
   Cut c;
+  c.parts.reserve(count);
   int64_t values = 0;
   bool placed[2] = {false, false};
   for (int64_t i = 0; i < count; ++i) {
     const orda_tensor &s = g[i].src, &d = g[i].dst;
-    char what[48];
-    snprintf(what, sizeof what, "gradient %lld", static_cast<long long>(i));
-    check_view(s, what);
-    to_dtype(s.dtype, what);
-    if (s.location != ORDA_DEVICE) fail(ORDA_ERR_INVALID, "%s must be on the device", what);
+    check_view(s, "a gradient");
+    to_dtype(s.dtype, "a gradient");
+    if (s.location != ORDA_DEVICE) fail(ORDA_ERR_INVALID, "a gradient must be on the device");
     if (s.rows > kMostValues || s.cols > kMostValues || (s.cols > 0 && s.rows > kMostValues / s.cols))
-      fail(ORDA_ERR_INVALID, "%s: at most 2^40 values", what);
+      fail(ORDA_ERR_INVALID, "at most 2^40 values");
     values += s.rows * s.cols;
     if (values > kMostValues) fail(ORDA_ERR_INVALID, "at most 2^40 values");
     if (s.rows == 0 || s.cols == 0) continue;
@@ -80,25 +84,25 @@ Cut cut(const orda_gradient* g, int64_t count, bool scale) {
       to_dtype(d.dtype, "a destination");
       if (d.location != ORDA_DEVICE) fail(ORDA_ERR_INVALID, "a destination must be on the device");
       if (d.rows != s.rows || d.cols != s.cols)
-        fail(ORDA_ERR_INVALID, "the destination of %s must be [%lld, %lld]", what, static_cast<long long>(s.rows),
-             static_cast<long long>(s.cols));
+        fail(ORDA_ERR_INVALID, "the destination of gradient %lld must be [%lld, %lld]", static_cast<long long>(i),
+             static_cast<long long>(s.rows), static_cast<long long>(s.cols));
     }
+    c.bytes += s.rows * s.cols * (s.dtype == ORDA_BF16 ? 2 : 4);
     c.parts.push_back(part_of(s, scale && d.data ? d : s));
   }
   if (scale && placed[0] && placed[1]) fail(ORDA_ERR_INVALID, "either all gradients have a destination or none");
   c.in_place = !placed[1];
-  // Pieces of 4096 values or more: sixteen a thread; larger where there are many.
-  c.piece = std::min<int64_t>(std::max<int64_t>(ceil_div(ceil_div(values, kBlocks * 4), 2048) * 2048, 4096), 1 << 16);
   int64_t pieces = 0;
-  for (const GradPart& p : c.parts) pieces += pieces_of(p, c.piece);
+  for (const GradPart& p : c.parts) pieces += pieces_of(p);
   for (size_t at = 0; at < c.parts.size();) {
     Cut::Launch l{at, std::min(at + kGradParts, c.parts.size()), 0, 0, c.sums};
     for (; at < l.to; ++at) {
       c.parts[at].first = l.pieces;
-      l.pieces += pieces_of(c.parts[at], c.piece);
+      l.pieces += pieces_of(c.parts[at]);
     }
-    // its share of the workgroups
-    l.blocks = static_cast<int>(std::min<int64_t>(l.pieces, std::max<int64_t>(1, kBlocks * l.pieces / pieces)));
+    // its share of 2048, or as many as have eight pieces each
+    const int64_t share = kBlocks * l.pieces / pieces, most = kSums * l.pieces / pieces;
+    l.blocks = static_cast<int>(std::max<int64_t>(1, std::min({l.pieces, std::max(share, std::min(kBlocks, l.pieces / 8)), most})));
     c.sums += l.blocks;
     c.launches.push_back(l);
   }
@@ -124,6 +128,7 @@ bool meet(const Span& a, const Span& b) {
 }
 void check_apart(const Cut& c) {
   std::vector<Span> spans;
+  spans.reserve(2 * c.parts.size());
   auto add = [&](const void* p, const GradPart& g, int64_t ld, int64_t es, bool written) {
     const auto from = reinterpret_cast<uintptr_t>(p);
     spans.push_back({from, from + ((g.rows - 1) * ld + g.cols) * es, g.cols * es, g.rows == 1 ? 0 : ld * es, written});
@@ -141,7 +146,8 @@ void check_apart(const Cut& c) {
 
 // Every launch has its share of the workgroups, and one at least.
 int64_t sum_bytes(int64_t count) {
-  return count == 0 ? 0 : ((kBlocks + ceil_div(count, kGradParts)) * 8 + 255) / 256 * 256;
+  const int64_t launches = ceil_div(count, kGradParts);
+  return count == 0 ? 0 : ((std::min(launches * kBlocks, kSums) + launches) * 8 + 255) / 256 * 256;
 }
 
 void run(int32_t device, hipStream_t st, const Cut& c, int64_t count, bool scale, double max_norm, double eps, float* norm, void* ws,
@@ -158,11 +164,10 @@ void run(int32_t device, hipStream_t st, const Cut& c, int64_t count, bool scale
     std::copy(c.parts.begin() + l.from, c.parts.begin() + l.to, a.part);
     a.count = static_cast<int32_t>(l.to - l.from);
     a.pieces = l.pieces;
-    a.piece = c.piece;
     a.sums = sums + l.first;
     return a;
   };
-  for (const Cut::Launch& l : c.launches) hip_check(launch_grad_sums(args(l), l.blocks, st), "gradient norm");
+  for (const Cut::Launch& l : c.launches) hip_check(launch_grad_sums(args(l), l.blocks, c.bytes > kCache, st), "gradient norm");
   if (!scale || c.launches.empty()) {
     hip_check(launch_grad_norm(sums, c.sums, norm, st), "gradient norm");
     return;

@@ -641,11 +641,12 @@ struct GradPart {
   int64_t first;           // of its pieces among the launch's
   int32_t src_bf16, dst_bf16;
 };
-constexpr int kGradParts = 56;   // of one launch: they travel in its arguments
+constexpr int kGradParts = 56;     // of one launch: they travel in its arguments
+constexpr int kGradPiece = 2048;   // values: eight of a thread (a row's last piece has fewer)
 struct GradArgs {
   GradPart part[kGradParts];
   int32_t count;
-  int64_t pieces, piece;   // of `piece` values each (a row's last one fewer)
+  int64_t pieces;          // of which each workgroup has as many in a row
   double* sums;            // the launch's, one a workgroup
   // clipping: all launches' sums
   const double* all;
@@ -653,7 +654,8 @@ struct GradArgs {
   double max_norm, eps;
   float* norm;             // written by one workgroup where set
 };
-hipError_t launch_grad_sums(const GradArgs& a, int blocks, hipStream_t stream);
+// once: the gradients are more than the cache holds
+hipError_t launch_grad_sums(const GradArgs& a, int blocks, bool once, hipStream_t stream);
 hipError_t launch_grad_scale(const GradArgs& a, int blocks, hipStream_t stream);
 hipError_t launch_grad_norm(const double* sums, int n, float* norm, hipStream_t stream);
 
