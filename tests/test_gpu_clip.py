@@ -106,6 +106,23 @@ def test_any_start_pitch_and_order(dtype):
     check_scaled(x, old, norm, 0.5 * norm)
 
 
+@pytest.mark.parametrize("dtype, to", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_more_than_the_cache_holds(dtype, to):
+    """Over 256 MB, in two launches, from any start."""
+    base = normal((75_000_003 * 4 // (4 if dtype == "f32" else 2),), dtype)
+    grads = [base[5:-4_000_000]] + [base[i:i + 57001] for i in range(base.numel() - 4_000_000, base.numel() - 57001, 57003)]
+    assert len(grads) > 57
+    norm = norm_of(grads)
+    check_norm(H.gradient_norm(grads), norm)
+    out = [torch.empty_like(g, dtype=DT[to]) for g in grads]
+    check_norm(H.clip_gradients(grads, 0.5 * norm, out=out), norm)
+    for o, g in zip(out, grads):
+        check_scaled(o, g, norm, 0.5 * norm)
+    H.clip_gradients(grads, 0.5 * norm)
+    if to == dtype:
+        assert all(torch.equal(a, b) for a, b in zip(out, grads))
+
+
 def test_long_rows_of_a_frame():
     """Rows of several pieces, apart from one another."""
     frame = normal((3, 300000))
