@@ -207,9 +207,11 @@ class RmsNormFunction(torch.autograd.Function):
     """out, total = RmsNormFunction.apply(x, weight, residual, eps, weight_offset);
     total is None without a residual."""
 
-    # The backward call is made ready by the forward's (up to this many bytes of rows
-    # with grad_x and the scratch): torch's engine runs a backward's Python on another thread, where it takes
-    # three times as long.
+    # The backward call is made ready by the forward's: torch's engine runs a backward's
+    # Python on another thread, where it takes three times as long (a step of few rows 98 us,
+    # 108 where the backward packs its arguments). grad_x and the scratch too, up to this many bytes of
+    # rows: larger ones are not held from the forward on, and their kernels take longer
+    # than the two allocations.
     READY_BYTES = 4 << 20
 
     @staticmethod
@@ -222,7 +224,7 @@ class RmsNormFunction(torch.autograd.Function):
             if total is not None:
                 a = _norm_args(total, weight, None, eps, weight_offset)[0]
             small = t.numel() * t.element_size() <= RmsNormFunction.READY_BYTES
-            fctx.ready = _NormGrad(a, t.detach(), w.detach(), want_x or want_r, want_w, small)
+            fctx.ready = _NormGrad(a, t, w, want_x or want_r, want_w, small)
         shape = x.shape
         if len(shape) != 2:
             out, total = out.view(shape), total.view(shape) if total is not None else None
@@ -239,11 +241,13 @@ class RmsNormFunction(torch.autograd.Function):
             return (g_total if want_x else None, torch.zeros_like(weight) if want_w else None,
                     g_total if want_r else None, None, None)
         ready, fctx.ready = fctx.ready, None   # (a second backward makes its own)
-        if ready is not None and ready.want_x == (want_x or want_r) and (ready.gw is not None) == want_w:
+        if (ready is not None and ready.want_x == (want_x or want_r) and (ready.gw is not None) == want_w
+                and total.is_contiguous() and weight.is_contiguous() and total.device == weight.device == ready.device):
+            # (saved tensors' hooks and whoever holds weights apart may have moved them)
             _gpu_tensor(g_out, "grad_out")
             if g_total is not None:
                 _gpu_tensor(g_total, "grad_total")
-            gx, gw = ready.run(g_out, g_total)
+            gx, gw = ready.run(total, weight, g_out, g_total)
             if gx is not None and total.dim() != 2:
                 gx = gx.view(total.shape)
         else:

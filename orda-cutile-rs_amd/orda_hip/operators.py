@@ -25,6 +25,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import operator
 import struct
 from typing import Optional, Tuple
 
@@ -412,6 +413,7 @@ def fp8_block_matmul(a, a_scales, b, b_scales, *, out_dtype=None):
 _TENSOR = "Qqqqii"                                                  # orda_tensor
 _NORM = struct.Struct("=" + 3 * _TENSOR + "dd")                     # orda_rms_norm
 _ROWS = struct.Struct("=" + _TENSOR)
+_ADDRESS = struct.Struct("=Q")
 _NORM_OUT = struct.Struct("=" + 2 * _TENSOR)                        # total, out
 _NORM_FP8 = struct.Struct("=" + _TENSOR + "QqqqQqqi4x")             # total, orda_fp8_matrix
 _NORM_GRADS = struct.Struct("=" + 4 * _TENSOR)                      # grad_out, grad_total, grad_x, grad_weight
@@ -556,21 +558,20 @@ def rms_norm_backward(grad_out, total, weight, *, grad_total=None, eps: float = 
     for g, what in ((grad_out, "grad_out"), (grad_total, "grad_total")):
         if g is not None and (_gpu_tensor(g, what).shape != total.shape or g.dtype != t.dtype):
             raise OrdaError(f"{what} must have the shape and dtype of total")
-    gx, gw = _NormGrad(a, t, w, grad_x, grad_weight).run(grad_out, grad_total)
+    gx, gw = _NormGrad(a, t, w, grad_x, grad_weight).run(t, w, grad_out, grad_total)
     return gx.view(total.shape) if gx is not None else None, gw
 
 
 class _NormGrad:
-    """A backward call of a matrix t, its weight and orda_rms_norm, made ready: its
-    arguments but for the gradients that come in and the weight's gradient; with `rows`
+    """A backward call of a matrix like t, a weight like w and orda_rms_norm, made ready:
+    its arguments but for the tensors that come in, and the weight's gradient; with `rows`
     also grad_x and the scratch, which else are made when it runs."""
-    __slots__ = "buf", "at", "message", "want_x", "gx", "gw", "ws", "bytes", "t", "shape", "dtype"
+    __slots__ = "buf", "at", "message", "want_x", "gx", "gw", "ws", "bytes", "device", "shape", "dtype"
 
     def __init__(self, a: bytes, t, w, want_x: bool, want_w: bool, rows: bool = True):
         torch = _torch()
         n, h = self.shape = t.shape
-        self.t = t
-        self.dtype = _dtype(t, "total")
+        self.device, self.dtype = t.device, _dtype(t, "total")
         self.want_x = want_x
         self.gx = _like(t) if want_x and rows else None
         self.gw = torch.empty_like(w) if want_w else None
@@ -580,13 +581,15 @@ class _NormGrad:
             *_NO_TENSOR, *_NO_TENSOR, *(_fields(self.gx, "grad_x") if self.gx is not None else _NO_TENSOR),
             *(_row_fields(self.gw, "grad_weight") if want_w else _NO_TENSOR)))
 
-    def run(self, g, gt):
-        """(grad_x, grad_weight), given plain gradients of t's number of values and dtype."""
-        buf, at, t, dtype, gx = self.buf, self.at, self.t, self.dtype, self.gx
+    def run(self, t, w, g, gt):
+        """(grad_x, grad_weight), given the sum and the weight (which may have moved, but are
+        as the ones it was made for) and plain gradients of t's number of values and dtype."""
+        buf, at, device, dtype, gx = self.buf, self.at, self.device, self.dtype, self.gx
         n, h = self.shape
-        device = t.device
         if g.device != device or (gt is not None and gt.device != device):
             raise OrdaError(f"gradients must be on {device}")
+        _ADDRESS.pack_into(buf, 0, t.data_ptr())
+        _ADDRESS.pack_into(buf, 2 * _ROWS.size, w.data_ptr())
         if not g.is_contiguous():
             g = _rows(g, h, "grad_out")
         ld = h if g.dim() != 2 or n == 1 else g.stride(0)
@@ -597,7 +600,7 @@ class _NormGrad:
             ld = h if gt.dim() != 2 or n == 1 else gt.stride(0)
             _ROWS.pack_into(buf, _NORM.size + _ROWS.size, gt.data_ptr(), n, h, ld, dtype, L.DEVICE)
         if gx is None and self.want_x:
-            gx = _like(t)
+            gx = _torch().empty((n, h), dtype=t.dtype, device=device)
             _ROWS.pack_into(buf, _NORM.size + 2 * _ROWS.size, gx.data_ptr(), n, h, h, dtype, L.DEVICE)
         ws = self.ws if self.ws is not None else _bytes(self.bytes, device)
         q, message = at + _NORM.size, self.message
@@ -813,9 +816,12 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=None, top_p=None, m
     p, p1 = _per_row(top_p, n, shape, d, "top_p", torch.float32, 1.0)
     q, q1 = _per_row(min_p, n, shape, d, "min_p", torch.float32, 0.0)
     f = _fields(m, "logits")
-    a = _SAMPLING.pack(*f, u.data_ptr(), t.data_ptr() if t is not None else 0, p.data_ptr() if p is not None else 0,
-                       q.data_ptr() if q is not None else 0, k.data_ptr() if k is not None else 0, t1, p1, q1,
-                       max(0, min(int(k1), 2 ** 31 - 1)))
+    try:
+        a = _SAMPLING.pack(*f, u.data_ptr(), t.data_ptr() if t is not None else 0, p.data_ptr() if p is not None else 0,
+                           q.data_ptr() if q is not None else 0, k.data_ptr() if k is not None else 0, t1, p1, q1,
+                           max(0, min(operator.index(k1), 2 ** 31 - 1)))
+    except (struct.error, OverflowError, TypeError):
+        raise OrdaError("temperature, top_p and min_p must be numbers within float32, top_k a whole number") from None
     b = _sample_bytes(n, v, f[4])
     ws = _bytes(b, d)
     tokens = torch.empty(shape, dtype=torch.int64, device=d)

@@ -360,3 +360,35 @@ def test_a_second_backward_and_one_that_wants_less(n):
     assert torch.equal(gx, first[0])
     (gw,) = torch.autograd.grad(out, [w], g)
     assert torch.equal(gw, first[1])
+
+
+@pytest.mark.parametrize("n", [5, 1500])   # (the second is over the bytes up to which grad_x is made ready)
+def test_tensors_that_move_between_forward_and_backward(n):
+    """Saved tensors kept on the host meanwhile, and a weight whose memory is exchanged, as
+    sharded training does it: the gradients of those that the backward is given."""
+    x, r, w = (normal(s, "f32", seed=i) for i, s in enumerate([(n, 1000), (n, 1000), (1000,)]))
+    g = normal((n, 1000), "f32", seed=3)
+    want_x, want_w = H.rms_norm_backward(g, x + r, w)
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    with torch.autograd.graph.save_on_cpu():
+        out, _ = rms_norm_autograd(a, b, residual=r)
+    out.backward(g)
+    assert torch.equal(a.grad, want_x) and torch.equal(b.grad, want_w)
+    a.grad = b.grad = None
+    out, _ = rms_norm_autograd(a, b, residual=r)
+    old, b.data = b.data, b.data.clone()
+    old.fill_(float("nan"))
+    out.backward(g)
+    assert torch.equal(a.grad, want_x) and torch.equal(b.grad, want_w)
+
+
+def test_nothing_but_the_saved_tensors_is_held():
+    """A forward whose saved tensors are put elsewhere leaves no rows behind."""
+    x, w = normal((4096, 2048), "f32").requires_grad_(True), normal((2048,), "f32").requires_grad_(True)
+    r = normal((4096, 2048), "f32", seed=1)
+    rms_norm_autograd(x, w, residual=r)[0].sum().backward()   # (what torch allocates once)
+    x.grad = w.grad = None
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        out = rms_norm_autograd(x, w, residual=r)[0]
+    assert torch.cuda.memory_allocated() - before <= out.numel() * 4 + (1 << 20)

@@ -288,3 +288,10 @@ def test_refusals():
                   ((x, u), dict(min_p=ones.cpu())), ((x, u), dict(temperature=float("nan")))):
         with pytest.raises(H.OrdaError):
             H.sample_tokens(*a, **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=2.5), dict(top_k="2"), dict(temperature=1e39), dict(temperature="1"),
+                                dict(top_p="0.9"), dict(min_p=[0.1]), dict(top_k=float("inf"))], ids=str)
+def test_parameters_that_are_no_numbers(kw):
+    with pytest.raises(H.OrdaError, match="numbers"):
+        H.sample_tokens(torch.zeros(2, 8, device="cuda"), torch.zeros(2, device="cuda"), **kw)
