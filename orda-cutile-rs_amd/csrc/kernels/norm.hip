@@ -506,7 +506,13 @@ __global__ __launch_bounds__(1024) void norm_grad_join_kernel(const float* parts
   const int64_t c = blockIdx.x * int64_t{64} + k;
   float s = 0.f;
   if (c < h)
-    for (int64_t p = p0; p < count; p += 16) s += parts[p * h + c];
+    for (int64_t p = p0; p < count; p += 256) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = p + 16 * i < count ? parts[(p + 16 * i) * h + c] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s += v[i];
+    }
   sums[p0][k] = s;
   __syncthreads();
   if (p0 == 0 && c < h) {
@@ -523,11 +529,15 @@ struct NormLaunch {
 };
 template <typename E, typename W, bool TAIL, bool FP8>
 NormLaunch norm_launch(int64_t n, int64_t h) {
-  // Few rows: as many threads as a row has vectors.
-  if (n < 1024) {
+  // Few rows: as many threads as a row has vectors (bf16 with residual, 1 and 64 rows: 2048
+  // columns 2.0 and 2.8 us, in the other form 3.0 and 3.9; 4096 2.4 and 3.6, 3.0 and 4.1;
+  // 512 rows of 4096 5.6 and 5.2).
+  if (n < 512) {
     if (h <= 2048) return {norm_kernel<E, W, 256, 1, TAIL, FP8>, 256, 1};
     if (h <= 8192) return {norm_kernel<E, W, 1024, 1, TAIL, FP8>, 1024, 1};
   }
+  // Many: four vectors a thread, whose loads are under way together, and few waves that
+  // wait for one another (8192 x 4096 to e4m3: two waves a row 44 us, four 62).
   if (h <= 1024) return {norm_kernel<E, W, 64, 2, TAIL, FP8>, 256, 4};
   if (h <= 2048) return {norm_kernel<E, W, 64, 4, TAIL, FP8>, 256, 4};
   if (h <= 4096) return {norm_kernel<E, W, 128, 4, TAIL, FP8>, 256, 2};
@@ -542,6 +552,7 @@ NormLaunch norm_launch(const NormArgs& a) {
   return a.h % 8 ? norm_launch<E, W, true, false>(a.n, a.h) : norm_launch<E, W, false, false>(a.n, a.h);
 }
 
+constexpr int64_t kLongRow = 16384, kLongRowF32 = 8192;   // longer ones are read twice
 using GradKernel = void (*)(NormGradArgs);
 struct GradLaunch {
   GradKernel k;   // null: rows too long for registers
@@ -549,18 +560,23 @@ struct GradLaunch {
 };
 template <typename E, typename W, bool TAIL>
 GradLaunch grad_launch(int64_t h) {
+  // As many rows at a time as registers hold (8192 rows of bf16, one thread a vector and
+  // two rows in their place: 1024 columns 13 us against 25, 2048 19 against 27; 64 rows
+  // take 5 us against 4).
   if (h <= 512) return {norm_grad_kernel<E, W, 64, 1, TAIL>, 8};
-  if (h <= 2048) return {norm_grad_kernel<E, W, 256, 1, TAIL>, 2};
+  if (h <= 1024) return {norm_grad_kernel<E, W, 64, 2, TAIL>, 8};
+  if (h <= 2048) return {norm_grad_kernel<E, W, 128, 2, TAIL>, 4};
   if (h <= 4096) return {norm_grad_kernel<E, W, 256, 2, TAIL>, 2};
   if (h <= 8192) return {norm_grad_kernel<E, W, 512, 2, TAIL>, 1};
-  if (h <= 16384) return {norm_grad_kernel<E, W, 512, 4, TAIL>, 1};
+  // (fp32's do not fit: with spills 2000 x 16384 took 153 us, read twice 114; bf16 takes 36,
+  // and read twice half of 32768 columns' 112.)
+  if constexpr (sizeof(E) == 2)
+    if (h <= kLongRow) return {norm_grad_kernel<E, W, 512, 4, TAIL>, 1};
   return {nullptr, 0};
 }
-int grad_teams(int64_t h) { return h <= 512 ? 8 : h <= 4096 ? 2 : 1; }
+int grad_teams(int64_t h) { return h <= 1024 ? 8 : h <= 2048 ? 4 : h <= 4096 ? 2 : 1; }
 
 constexpr int64_t kGradBlocks = 256;   // workgroups that keep sums of the weight's gradient
-constexpr int64_t kLongRow = 16384;
-
 int64_t grad_blocks(int64_t n, int64_t h) {
   const int64_t b = (n + grad_teams(h) - 1) / grad_teams(h);
   return b < kGradBlocks ? b : kGradBlocks;
@@ -624,8 +640,10 @@ hipError_t launch_norm(const NormArgs& a, DType rows, DType weight, hipStream_t 
 
 int64_t norm_grad_scratch(int64_t n, int64_t h) {
   if (n == 0 || h == 0) return 0;
-  const int64_t words = h <= kLongRow ? grad_blocks(n, h) * h : (n * 2 + 63) / 64 * 64 + grad_bands(n, h) * h;
-  return (words * 4 + 255) / 256 * 256;
+  // (of either type)
+  const int64_t sums = h <= kLongRow ? grad_blocks(n, h) * h : 0;
+  const int64_t twice = h > kLongRowF32 ? (n * 2 + 63) / 64 * 64 + grad_bands(n, h) * h : 0;
+  return ((sums > twice ? sums : twice) * 4 + 255) / 256 * 256;
 }
 
 hipError_t launch_norm_grad(const NormGradArgs& a, DType rows, DType weight, hipStream_t stream) {
