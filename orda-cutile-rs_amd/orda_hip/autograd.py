@@ -23,7 +23,7 @@ import torch
 from . import (Context, distillation_loss, embedding, linear_cross_entropy,
                linear_cross_entropy_backward, rms_norm_backward)
 from . import _lib as L
-from .operators import (_embed_grad, _gpu_tensor, _ids, _norm_args, _norm_forward, _NormGrad, _padding_row)
+from .operators import (_embed_grad, _gpu_tensor, _ids, _norm_forward, _NormGrad, _padding_row, _without_residual)
 from .types import LossOptions, OrdaError, Teacher, TeacherMode
 
 
@@ -208,11 +208,11 @@ class RmsNormFunction(torch.autograd.Function):
     total is None without a residual."""
 
     # The backward call is made ready by the forward's: torch's engine runs a backward's
-    # Python on another thread, where it takes three times as long (a step of few rows 98 us,
-    # 108 where the backward packs its arguments). grad_x and the scratch too, up to this many bytes of
-    # rows: larger ones are not held from the forward on, and their kernels take longer
-    # than the two allocations.
-    READY_BYTES = 4 << 20
+    # Python on another thread, where it takes two to three times as long (a step of few rows
+    # 96 us, 108 where the backward packs its arguments). grad_x and the scratch too, up to
+    # this many bytes of rows (1000 x 1531 fp32 101 us, 107 where the backward makes them):
+    # larger ones are not held from the forward on.
+    READY_BYTES = 16 << 20
 
     @staticmethod
     def forward(fctx, x, weight, residual, eps, weight_offset):
@@ -220,14 +220,12 @@ class RmsNormFunction(torch.autograd.Function):
         t = m if total is None else total
         fctx.ready = None
         want_x, want_w, want_r = fctx.needs_input_grad[:3]
-        if w is weight and m.numel() and t.is_contiguous() and (want_x or want_w or want_r):
-            if total is not None:
-                a = _norm_args(total, weight, None, eps, weight_offset)[0]
+        if w is weight and t.numel() and t.is_contiguous() and (want_x or want_w or want_r):
             small = t.numel() * t.element_size() <= RmsNormFunction.READY_BYTES
-            fctx.ready = _NormGrad(a, t, w, want_x or want_r, want_w, small)
-        shape = x.shape
-        if len(shape) != 2:
-            out, total = out.view(shape), total.view(shape) if total is not None else None
+            # (the forward's arguments; of a sum those without the residual, its address is put in)
+            fctx.ready = _NormGrad(a if total is None else _without_residual(a), t, w, want_x or want_r, want_w, small)
+        if x.dim() != 2:
+            out, total = out.view(x.shape), total.view(x.shape) if total is not None else None
         fctx.save_for_backward(x if total is None else total, weight)
         fctx.opts = eps, weight_offset
         fctx.set_materialize_grads(False)
@@ -241,9 +239,9 @@ class RmsNormFunction(torch.autograd.Function):
             return (g_total if want_x else None, torch.zeros_like(weight) if want_w else None,
                     g_total if want_r else None, None, None)
         ready, fctx.ready = fctx.ready, None   # (a second backward makes its own)
-        if (ready is not None and ready.want_x == (want_x or want_r) and (ready.gw is not None) == want_w
-                and total.is_contiguous() and weight.is_contiguous() and total.device == weight.device == ready.device):
-            # (saved tensors' hooks and whoever holds weights apart may have moved them)
+        # (saved tensors' hooks and whoever holds weights apart may have moved them)
+        if (ready is not None and ready.want_x == (want_x or want_r) and ready.want_w == want_w
+                and total.is_contiguous() and weight.is_contiguous()):
             _gpu_tensor(g_out, "grad_out")
             if g_total is not None:
                 _gpu_tensor(g_total, "grad_total")

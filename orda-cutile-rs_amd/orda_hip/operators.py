@@ -27,6 +27,7 @@ import functools
 import math
 import operator
 import struct
+import threading
 from typing import Optional, Tuple
 
 from . import _lib as L
@@ -408,8 +409,8 @@ def fp8_block_matmul(a, a_scales, b, b_scales, *, out_dtype=None):
     return out
 
 
-# Structures packed into one buffer with the message's place behind them: a call of a
-# few tensors costs half of what ctypes' structures take.
+# Structures packed into one buffer, and a message's place for each thread: a call of a
+# few tensors costs half of what ctypes' structures and a new message take.
 _TENSOR = "Qqqqii"                                                  # orda_tensor
 _NORM = struct.Struct("=" + 3 * _TENSOR + "dd")                     # orda_rms_norm
 _ROWS = struct.Struct("=" + _TENSOR)
@@ -420,16 +421,27 @@ _NORM_GRADS = struct.Struct("=" + 4 * _TENSOR)                      # grad_out, 
 _NO_TENSOR = (0, 0, 0, 0, 0, 0)
 
 
+_thread = threading.local()
+
+
+def _message() -> int:
+    try:
+        return _thread.message
+    except AttributeError:
+        _thread.buffer = C.create_string_buffer(512)
+        _thread.message = C.addressof(_thread.buffer)
+        return _thread.message
+
+
 def _packed(data: bytes):
-    """A buffer that holds data and a message, its address and the message's."""
-    buf = C.create_string_buffer(data, len(data) + 512)
-    p = C.addressof(buf)
-    return buf, p, p + len(data)
+    """A buffer that holds data, and its address."""
+    buf = bytearray(data)
+    return buf, C.addressof(C.c_char.from_buffer(buf))
 
 
-def _check(rc: int, message: int):
+def _check(rc: int):
     if rc != L.ORDA_OK:
-        raise OrdaError(C.string_at(message).decode(), rc)
+        raise OrdaError(C.string_at(_message()).decode(), rc)
 
 
 def _fields(x, what: str):
@@ -459,7 +471,8 @@ def _norm_args(x, weight, residual, eps: float, weight_offset: float):
         raise OrdaError("x must be [..., H]")
     h = x.size(-1)
     w = _gpu_tensor(weight, "weight")
-    if w.device != x.device:
+    index = x.get_device()
+    if w.get_device() != index:
         raise OrdaError(f"weight is on {w.device}, not on {x.device}")
     if w.dim() != 1 or w.size(0) != h:
         raise OrdaError(f"weight must be [{h}]")
@@ -467,7 +480,7 @@ def _norm_args(x, weight, residual, eps: float, weight_offset: float):
     m, r = _rows(x, h, "x"), None
     if residual is not None:
         r = _gpu_tensor(residual, "residual")
-        if r.device != x.device:
+        if r.get_device() != index:
             raise OrdaError(f"residual is on {r.device}, not on {x.device}")
         if r.shape != x.shape or r.dtype != x.dtype:
             raise OrdaError("residual must have the shape and dtype of x")
@@ -487,17 +500,17 @@ def _norm_forward(x, weight, residual, eps: float, weight_offset: float):
     """rms_norm's result and sum (None without a residual) as matrices, and the arguments."""
     a, m, w, _r = args = _norm_args(x, weight, residual, eps, weight_offset)
     out = _like(m)
-    o = _fields(out, "out")
-    total = None
+    n, h = m.shape
+    kind, total = _DTYPES[m.dtype], None
     if residual is not None:
         total = _like(m)
-        outs = _NORM_OUT.pack(total.data_ptr(), *o[1:], *o)
+        outs = _NORM_OUT.pack(total.data_ptr(), n, h, h, kind, L.DEVICE, out.data_ptr(), n, h, h, kind, L.DEVICE)
     else:
-        outs = _NORM_OUT.pack(*_NO_TENSOR, *o)
-    _buf, p, message = _packed(a + outs)
-    device = m.device
-    _check(L.load().orda_rms_norm_forward(device.index, _stream(device), p, p + _NORM.size, p + _NORM.size + _ROWS.size,
-                                          message, 512), message)
+        outs = _NORM_OUT.pack(0, 0, 0, 0, 0, 0, out.data_ptr(), n, h, h, kind, L.DEVICE)
+    _buf, p = _packed(a + outs)
+    index = m.get_device()
+    _check(L.load().orda_rms_norm_forward(index, _torch()._C._cuda_getCurrentRawStream(index), p, p + _NORM.size,
+                                          p + _NORM.size + _ROWS.size, _message(), 512))
     return out, total, args
 
 
@@ -507,7 +520,8 @@ def rms_norm(x, weight, *, residual=None, eps: float = 1e-6, weight_offset: floa
 
     ``x`` and ``residual`` are [..., H], float32 or bfloat16, ``weight`` [H] either of
     them. ``t`` is rounded to x's type, the mean formed in 64 bits, the result
-    rounded once to x's type. Returns the result, with a residual ``(result, t)``.
+    rounded once to x's type. A root below 3e-39 (of ``eps`` 0) counts as 0. Returns the
+    result, with a residual ``(result, t)``.
     """
     out, total, _ = _norm_forward(x, weight, residual, eps, weight_offset)
     if x.dim() != 2:
@@ -529,9 +543,9 @@ def rms_norm_fp8(x, weight, *, residual=None, eps: float = 1e-6, weight_offset: 
     scales = torch.empty((cb, n), dtype=torch.float32, device=device)
     total = _like(m) if residual is not None else None
     t = _fields(total, "total") if total is not None else _NO_TENSOR
-    _buf, p, message = _packed(a + _NORM_FP8.pack(*t, codes.data_ptr(), n, h, pitch, scales.data_ptr(), 1, n, 1))
+    _buf, p = _packed(a + _NORM_FP8.pack(*t, codes.data_ptr(), n, h, pitch, scales.data_ptr(), 1, n, 1))
     _check(L.load().orda_rms_norm_fp8(device.index, _stream(device), p, p + _NORM.size, p + _NORM.size + _ROWS.size,
-                                      message, 512), message)
+                                      _message(), 512))
     if pitch != h:
         codes = codes[:, :h]
     return (codes, scales.t()) if total is None else (codes, scales.t(), total.view(x.shape))
@@ -562,50 +576,63 @@ def rms_norm_backward(grad_out, total, weight, *, grad_total=None, eps: float = 
     return gx.view(total.shape) if gx is not None else None, gw
 
 
+def _without_residual(a: bytes) -> bytes:
+    """orda_rms_norm of a contiguous sum, given that of the rows."""
+    n, h = _ROWS.unpack_from(a)[1:3]
+    return a[:24] + struct.pack("=q", h) + a[32:40] + bytes(40) + a[80:]
+
+
 class _NormGrad:
     """A backward call of a matrix like t, a weight like w and orda_rms_norm, made ready:
-    its arguments but for the tensors that come in, and the weight's gradient; with `rows`
-    also grad_x and the scratch, which else are made when it runs."""
-    __slots__ = "buf", "at", "message", "want_x", "gx", "gw", "ws", "bytes", "device", "shape", "dtype"
+    its arguments but for the addresses that come in, and the weight's gradient; with
+    `rows` also grad_x and the scratch, which else are made when it runs."""
+    __slots__ = "buf", "at", "want_x", "want_w", "gx", "gw", "ws", "bytes", "device", "shape", "dtype"
 
     def __init__(self, a: bytes, t, w, want_x: bool, want_w: bool, rows: bool = True):
         torch = _torch()
-        n, h = self.shape = t.shape
-        self.device, self.dtype = t.device, _dtype(t, "total")
-        self.want_x = want_x
-        self.gx = _like(t) if want_x and rows else None
-        self.gw = torch.empty_like(w) if want_w else None
+        self.shape = shape = n, h = t.shape
+        self.device, self.dtype = device, dtype = t.device, t.dtype
+        self.want_x, self.want_w = want_x, want_w
+        self.gx = self.ws = self.gw = None
         self.bytes = _norm_bytes(n, h)
-        self.ws = _bytes(self.bytes, t.device) if rows else None
-        self.buf, self.at, self.message = _packed(a + _NORM_GRADS.pack(
-            *_NO_TENSOR, *_NO_TENSOR, *(_fields(self.gx, "grad_x") if self.gx is not None else _NO_TENSOR),
-            *(_row_fields(self.gw, "grad_weight") if want_w else _NO_TENSOR)))
+        kind, x, weight = _DTYPES[dtype], 0, _NO_TENSOR
+        if want_x and rows:
+            self.gx = gx = torch.empty(shape, dtype=dtype, device=device)
+            x = gx.data_ptr()
+        if rows:
+            self.ws = _bytes(self.bytes, device)
+        if want_w:
+            self.gw = gw = torch.empty_like(w)
+            weight = gw.data_ptr(), 1, h, h, _DTYPES[w.dtype], L.DEVICE
+        self.buf, self.at = _packed(a + _NORM_GRADS.pack(0, n, h, h, kind, L.DEVICE, 0, n, h, h, kind, L.DEVICE,
+                                                         x, n, h, h, kind, L.DEVICE, *weight))
 
     def run(self, t, w, g, gt):
         """(grad_x, grad_weight), given the sum and the weight (which may have moved, but are
         as the ones it was made for) and plain gradients of t's number of values and dtype."""
-        buf, at, device, dtype, gx = self.buf, self.at, self.device, self.dtype, self.gx
-        n, h = self.shape
-        if g.device != device or (gt is not None and gt.device != device):
-            raise OrdaError(f"gradients must be on {device}")
-        _ADDRESS.pack_into(buf, 0, t.data_ptr())
-        _ADDRESS.pack_into(buf, 2 * _ROWS.size, w.data_ptr())
+        buf, gx, ws, put = self.buf, self.gx, self.ws, _ADDRESS.pack_into
+        index = self.device.index
+        if not index == t.get_device() == w.get_device() == g.get_device() or (gt is not None and gt.get_device() != index):
+            raise OrdaError(f"weight and gradients must be on {self.device}")
         if not g.is_contiguous():
-            g = _rows(g, h, "grad_out")
-        ld = h if g.dim() != 2 or n == 1 else g.stride(0)
-        _ROWS.pack_into(buf, _NORM.size, g.data_ptr(), n, h, ld, dtype, L.DEVICE)
+            g = _rows(g, self.shape[1], "grad_out")
+            _ROWS.pack_into(buf, 136, *_fields(g, "grad_out"))
         if gt is not None:
             if not gt.is_contiguous():
-                gt = _rows(gt, h, "grad_total")
-            ld = h if gt.dim() != 2 or n == 1 else gt.stride(0)
-            _ROWS.pack_into(buf, _NORM.size + _ROWS.size, gt.data_ptr(), n, h, ld, dtype, L.DEVICE)
+                gt = _rows(gt, self.shape[1], "grad_total")
+                _ROWS.pack_into(buf, 176, *_fields(gt, "grad_total"))
+            put(buf, 176, gt.data_ptr())
+        put(buf, 0, t.data_ptr())
+        put(buf, 80, w.data_ptr())
+        put(buf, 136, g.data_ptr())
         if gx is None and self.want_x:
-            gx = _torch().empty((n, h), dtype=t.dtype, device=device)
-            _ROWS.pack_into(buf, _NORM.size + 2 * _ROWS.size, gx.data_ptr(), n, h, h, dtype, L.DEVICE)
-        ws = self.ws if self.ws is not None else _bytes(self.bytes, device)
-        q, message = at + _NORM.size, self.message
-        _check(L.load().orda_rms_norm_backward(device.index, _stream(device), at, q, q + 40, q + 80, q + 120,
-                                               ws.data_ptr(), self.bytes, message, 512), message)
+            gx = _torch().empty(self.shape, dtype=self.dtype, device=self.device)
+            put(buf, 216, gx.data_ptr())
+        if ws is None:
+            ws = _bytes(self.bytes, self.device)
+        at = self.at
+        _check(L.load().orda_rms_norm_backward(index, _torch()._C._cuda_getCurrentRawStream(index), at, at + 136, at + 176,
+                                               at + 216, at + 256, ws.data_ptr(), self.bytes, _message(), 512))
         return gx, self.gw
 
 
@@ -636,8 +663,8 @@ def _gradient_table(n: int):
 
 
 def _plain_gradients(grads, out, index):
-    """The table of contiguous gradients and destinations, as most are (36 us for 37 of
-    both, 77 in the general way); None where one is anything else."""
+    """The table of contiguous gradients and destinations, as most are (37 us for 37 of
+    both, 56 with the checks below); None where one is anything else."""
     torch = _torch()
     kinds = torch.Tensor, torch.nn.Parameter
     dtypes = {torch.float32: L.F32, torch.bfloat16: L.BF16}
@@ -826,7 +853,7 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=None, top_p=None, m
     ws = _bytes(b, d)
     tokens = torch.empty(shape, dtype=torch.int64, device=d)
     logprobs = torch.empty_like(u) if len(shape) == 1 else torch.empty(shape, dtype=torch.float32, device=d)
-    _buf, at, message = _packed(a)
+    _buf, at = _packed(a)
     _check(L.load().orda_sample_tokens(d.index, _stream(d), at, tokens.data_ptr(), logprobs.data_ptr(), ws.data_ptr(), b,
-                                       message, 512), message)
+                                       _message(), 512))
     return tokens, logprobs

@@ -362,7 +362,7 @@ def test_a_second_backward_and_one_that_wants_less(n):
     assert torch.equal(gw, first[1])
 
 
-@pytest.mark.parametrize("n", [5, 1500])   # (the second is over the bytes up to which grad_x is made ready)
+@pytest.mark.parametrize("n", [5, 1500, 5000])   # (the last is over the bytes up to which grad_x is made ready)
 def test_tensors_that_move_between_forward_and_backward(n):
     """Saved tensors kept on the host meanwhile, and a weight whose memory is exchanged, as
     sharded training does it: the gradients of those that the backward is given."""
