@@ -4,6 +4,23 @@
 // The distribution function of a row has as many borders as tokens, so an error of
 // d in it gives another token with a probability of about 2·d·V: masses and their
 // sums are held in 64 bits.
+//
+// Nothing is sorted but a list of at most 2048 candidates. A first pass over the logits
+// leaves the largest of each 64 tokens and, where all masses are needed, the mass of each
+// 1024; then a workgroup a row takes the candidates from the 64s whose largest reach a
+// bound (`pick`), and where the kept tokens are more than the list holds it finds the cut by
+// bins, of which it lists one (`select`). (Both in one kernel, 42 KB of code: with
+// `select` in a launch of its own the rows that need it waited for all others, 61 us in
+// place of 45 for 64 x 50257 of mixed parameters.) The drawn token is then sought in its
+// group of 1024 alone. Largest logits, masses and counts do not depend on the order
+// in which they are formed, or are summed in fixed point or in a fixed order: the same bits
+// in every run.
+//
+// 1 x 131072 fp32, top-k 50 and top-p 0.9: 3 us and 9 of kernels (the host's 15 are more).
+// 256 x 131072 fp32, top-p 0.95 of a flat distribution, the slowest kind: 32 us (4.2 TB/s)
+// and 85, of which the binning's and the listing's passes over the row, one workgroup a
+// row, are the most. 512 x 131072 bf16, unfiltered: 56 us (2.4 TB/s: the exponentials in 64
+// bits) and 10.
 #include <math.h>
 
 #include "orda_kernels.h"
@@ -194,9 +211,12 @@ struct Tokens {
 
 // ---------------------------------------------------------------- first pass
 // The largest of each 64 and of each 1024 tokens, as keys, and where they are needed
-// the sum of each 1024's masses, relative to its largest: one read of the logits. A
-// row's last 1024, where they are fewer, are copied and filled up, so that later passes
-// read whole ones.
+// the sum of each 1024's masses, relative to its largest: one read of the logits, a wave
+// a group (so that many rows and one row alike fill the device). A row's last 1024, where
+// they are fewer, are copied and filled up, so that later passes read whole ones. Bound by
+// HBM for fp32 and by the nine instructions of 64 bits a token for bf16; reads past the
+// caches gain 2 us of 66 there and nothing for fp32, and would take from the next pass
+// what it finds in them.
 __device__ __forceinline__ float max3(float a, float b, float c) {   // (a NaN is looked for apart)
   float m;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
@@ -951,7 +971,10 @@ struct Pick {
   // A row that is not filtered, or of which a list of at most kList tokens is known to
   // hold the kept ones; else false. Lists are, in the order in which they are tried: the
   // tokens over what min-p keeps (all of few), those over what about 64 or k of the 64s'
-  // largest reach.
+  // largest reach. (64: one wave settles them, 5 us where a sort of 1024 takes 8; with 256 top-p
+  // took 14 us in place of 4.6 on a row whose list did not suffice, and 17 in place of 13 on
+  // one whose did. Where top-p's share is over what so many can have, by a quarter, no
+  // list is made: 4.5 us in place of 9.)
   __device__ __forceinline__ bool pick() {
     if (begin()) return true;
     double mine = 0., all_mass = 1.;
@@ -1114,19 +1137,17 @@ struct Pick {
   }
 };
 
-// A row that pick() leaves to select() has this for its token meanwhile.
-constexpr int64_t kLeft = -2;
-
-template <typename E, bool SELECT>
+template <typename E>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
   __shared__ Shared s;
   const int64_t row = blockIdx.x;
-  if (SELECT && a.token[row] != kLeft) return;
   load_powers(s.powers);   // (barriers follow before they are read)
   const Row r = row_of(a, row);
   Pick<E> p{a, s, row, r, static_cast<const E*>(a.x) + row * a.ldx, Exp(s.powers, r.t), false, {0, 0}};
-  if constexpr (SELECT) p.select();
-  else if (!p.pick() && threadIdx.x == 0) a.token[row] = kLeft;
+  if (!p.pick()) {
+    __syncthreads();
+    p.select();
+  }
   p.finish();
 }
 
@@ -1151,10 +1172,7 @@ hipError_t sample(const SampleArgs& a, hipStream_t stream) {
     p.masses = a.masses + r * a.n1024;
     p.tails = static_cast<E*>(a.tails) + r * kGroup;
     hipLaunchKernelGGL(sample_groups_kernel<E>, dim3(across, static_cast<unsigned>(n)), dim3(256), 0, stream, p);
-    hipLaunchKernelGGL((sample_row_kernel<E, false>), dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream, p);
-    // (not where nothing is filtered in any row)
-    if (a.k || a.p || a.m || a.k1 > 0 || a.p1 < 1.f || a.m1 > 0.f)
-      hipLaunchKernelGGL((sample_row_kernel<E, true>), dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL(sample_row_kernel<E>, dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream, p);
   }
   return hipGetLastError();
 }
