@@ -698,12 +698,9 @@ struct Pick {
       }
       const int next = g + kWaves;
       if (next < groups) t.fetch(next < whole ? x + next * int64_t{kGroup} : tail);
-#pragma unroll 1
-      for (int unit = 0; unit < 4; ++unit) {
-        f(g, unit, g * int64_t{kGroup} + T::column(unit * 4 / T::kPer) + unit * 4 % T::kPer, y[0]);
 #pragma unroll
-        for (int k = 0; k < 12; ++k) y[k / 4][k % 4] = y[k / 4 + 1][k % 4];
-      }
+      for (int unit = 0; unit < 4; ++unit)
+        f(g, unit, g * int64_t{kGroup} + T::column(unit * 4 / T::kPer) + unit * 4 % T::kPer, y[unit]);
       if (next >= groups) return;
       g = next;
     }
