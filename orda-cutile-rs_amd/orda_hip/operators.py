@@ -485,8 +485,11 @@ def _norm_args(x, weight, residual, eps: float, weight_offset: float):
         if r.shape != x.shape or r.dtype != x.dtype:
             raise OrdaError("residual must have the shape and dtype of x")
         r = _rows(r, h, "residual")
-    a = _NORM.pack(*_fields(m, "x"), *(_fields(r, "residual") if r is not None else _NO_TENSOR),
-                   *_row_fields(w, "weight"), eps, weight_offset)
+    try:
+        a = _NORM.pack(*_fields(m, "x"), *(_fields(r, "residual") if r is not None else _NO_TENSOR),
+                       *_row_fields(w, "weight"), eps, weight_offset)
+    except (struct.error, OverflowError, TypeError):
+        raise OrdaError("eps and weight_offset must be numbers") from None
     return a, m, w, r
 
 
@@ -762,8 +765,11 @@ def clip_gradients(grads, max_norm: float, *, eps: float = 1e-6, out=None):
     b = _clip_bytes(len(grads))
     ws = _bytes(b, device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    _call(L.load().orda_clip_gradients, device.index, _stream(device), a, len(grads), max_norm, eps, norm.data_ptr(),
-          ws.data_ptr(), b)
+    try:
+        _call(L.load().orda_clip_gradients, device.index, _stream(device), a, len(grads), max_norm, eps, norm.data_ptr(),
+              ws.data_ptr(), b)
+    except (C.ArgumentError, OverflowError):
+        raise OrdaError("max_norm and eps must be numbers") from None
     torch.autograd.graph.increment_version(grads if out is None else out)   # written in place
     return norm
 

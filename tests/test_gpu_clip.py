@@ -224,3 +224,12 @@ def test_refusals():
             H.clip_gradients(grads, kw.pop("max_norm", 1.0), **kw)
     old = g.clone()
     assert torch.equal(g, old)
+
+
+@pytest.mark.parametrize("limit, kw", [("1", {}), (None, {}), (1.0, dict(eps="0")), (10 ** 400, {})], ids=lambda v: str(v)[:8])
+def test_limits_that_are_no_numbers(limit, kw):
+    g = normal((8,))
+    old = g.clone()
+    with pytest.raises(H.OrdaError, match="numbers"):
+        H.clip_gradients([g], limit, **kw)
+    assert torch.equal(g, old)

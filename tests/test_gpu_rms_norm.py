@@ -392,3 +392,11 @@ def test_nothing_but_the_saved_tensors_is_held():
     with torch.autograd.graph.save_on_cpu():
         out = rms_norm_autograd(x, w, residual=r)[0]
     assert torch.cuda.memory_allocated() - before <= out.numel() * 4 + (1 << 20)
+
+
+@pytest.mark.parametrize("kw", [dict(eps="1e-6"), dict(eps=None), dict(weight_offset=[1.0])], ids=str)
+def test_options_that_are_no_numbers(kw):
+    x, w = normal((3, 8), "f32"), normal((8,), "f32")
+    for call in (H.rms_norm, H.rms_norm_fp8, rms_norm_autograd, lambda x, w, **kw: H.rms_norm_backward(x, x, w, **kw)):
+        with pytest.raises(H.OrdaError, match="numbers"):
+            call(x, w, **kw)
