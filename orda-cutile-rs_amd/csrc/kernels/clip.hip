@@ -6,8 +6,8 @@
 // launches' arguments, so that nothing is copied to the device and a captured graph
 // holds them. Bound by HBM: one read for the norm, and where it is over the limit
 // another read and a write. 4.29 GB of fp32: 613 us (7.0 TB/s) and 1640 (5.2 both ways; a
-// copy reaches 4.8); 1.07 GB of bf16 in 110 tensors, two launches: 204 (5.2: the additions
-// in 64 bits, of which a wave's takes 8 cycles, beside the conversions).
+// copy reaches 4.8); 1.05 GB of bf16 in 110 tensors at any address, two launches: 180 (5.8;
+// 208 before the loads began at whole 16 bytes).
 //
 // The gradients' values are one row of pieces, of which each workgroup has an equal run:
 // with whole tensors or a piece at a time the last ones left the others waiting.
@@ -69,8 +69,16 @@ __device__ __forceinline__ void take(E (&v)[N], const E* p) {
   __builtin_memcpy(v, &w, sizeof v);
 }
 
+// Values before the first that lies at 16 bytes, of n.
+template <typename E>
+__device__ __forceinline__ int64_t to_aligned(const E* p, int64_t n) {
+  const int64_t k = (16 - reinterpret_cast<uintptr_t>(p) % 16) % 16 / sizeof(E);
+  return k < n ? k : n;
+}
+
 // Loads that a thread has under way: 64 bytes of fp32 (4.29 GB past the caches: 612 us,
-// 640 with 32) or 32 of bf16, whose arithmetic takes longer (1.07 GB: 204 us, 231 with 64).
+// 640 with 32) or 32 of bf16, whose values take twice the registers (1.05 GB: 180 us, 188
+// with 64).
 template <typename E>
 constexpr int kAhead = sizeof(E) == 4 ? 4 : 2;
 
@@ -79,6 +87,10 @@ __device__ __forceinline__ double squares(const E* p, int64_t n) {
   constexpr int N = 16 / sizeof(E), kStep = kThreads * N, kU = kAhead<E>;
   double s[kU] = {};
   auto add = [](double& s, float v) { s = fma(static_cast<double>(v), static_cast<double>(v), s); };
+  const int64_t first = to_aligned(p, n);
+  if (threadIdx.x < first) add(s[1], p[threadIdx.x]);
+  p += first;
+  n -= first;
   const int64_t whole = n / N * N;
   int64_t c = threadIdx.x * int64_t{N};
   for (; c + (kU - 1) * kStep < whole; c += kU * kStep) {
@@ -138,6 +150,11 @@ __device__ __forceinline__ void scaled(const S* s, D* d, int64_t n, float f) {
     for (int k = 0; k < N; ++k) o[k] = static_cast<D>(static_cast<float>(v[k]) * f);
     __builtin_memcpy(d + c, o, sizeof o);
   };
+  const int64_t first = to_aligned(s, n);
+  if (threadIdx.x < first) d[threadIdx.x] = static_cast<D>(static_cast<float>(s[threadIdx.x]) * f);
+  s += first;
+  d += first;
+  n -= first;
   const int64_t whole = n / N * N;
   int64_t c = threadIdx.x * int64_t{N};
   for (; c + (kU - 1) * kStep < whole; c += kU * kStep) {

@@ -17,10 +17,10 @@
 // in every run.
 //
 // 1 x 131072 fp32, top-k 50 and top-p 0.9: 3 us and 9 of kernels (the host's 15 are more).
-// 256 x 131072 fp32, top-p 0.95 of a flat distribution, the slowest kind: 32 us (4.2 TB/s)
-// and 85, of which the binning's and the listing's passes over the row, one workgroup a
-// row, are the most. 512 x 131072 bf16, unfiltered: 56 us (2.4 TB/s: the exponentials in 64
-// bits) and 10.
+// 256 x 131072 fp32, top-p 0.95 of a flat distribution, the slowest kind: 30 us (4.5 TB/s)
+// and 80, of which the binning's and the listing's passes over the row, one workgroup a
+// row, are the most. 512 x 131072 bf16, unfiltered: 48 us (2.8 TB/s: 20 instructions a
+// token, nine of them in 64 bits) and 10.
 #include <math.h>
 
 #include "orda_kernels.h"
@@ -37,18 +37,19 @@ constexpr int kBins = 2048, kList = 2048, kRing = 512;
 // Keys order as the values do; equal values (0 and -0) have equal keys, NaN the
 // largest.
 constexpr uint32_t kNan = 0xffffffffu, kInf = 0xff800000u, kNone = 0x007fffffu;   // kNone: -infinity
-__device__ __forceinline__ uint32_t key_of(float x) {
+__device__ __forceinline__ uint32_t key_of_number(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
-  return x != x ? kNan : u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ uint32_t key_of(float x) { return x != x ? kNan : key_of_number(x); }
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
 // e^z of z <= 0 in 64 bits: z·256/ln 2 = 256·n + j + f, |f| <= 1/2, and e^z = 2^n · 2^(j/256)
 // · e^y, y = f ln 2/256, the last by its series (the first term left out is 1.4e-13),
-// 2^(j/256) from a table in LDS. Nine instructions of 64 bits, whose rate bounds the
-// passes that weigh tokens: a wave's takes 8 cycles.
+// 2^(j/256) from a table in LDS. Nine instructions of 64 bits (2.2 ns a wave's on its SIMD,
+// where one of 32 takes 1.9) and three more, which bound the passes that weigh tokens.
 constexpr int kPowers = 256;
 __device__ const double kPower[kPowers] = {
     1.0, 1.0027112750502025, 1.0054299011128027, 1.0081558981184175,
@@ -117,20 +118,23 @@ __device__ const double kPower[kPowers] = {
     1.978456026387951, 1.9838201648502194, 1.9891988469672663, 1.9945921121709402,
 };
 struct Exp {
-  const double* powers;   // kPower, in LDS
+  const double* powers;   // in LDS, as load_powers puts them there
   double top, inv;        // of e^((x - top) / t): inv = 1 / t
   double shift;           // top / t, rounded
-  __device__ __forceinline__ Exp(const double* p, float t) : powers(p), top(0.), inv(1. / static_cast<double>(t)), shift(0.) {}
-  __device__ __forceinline__ void from(double largest) {
-    top = largest;
-    shift = largest * inv;
+  float t, low;           // low: of a mass next to nothing
+  __device__ __forceinline__ Exp(const double* p, float t)
+      : powers(p), top(0.), inv(1. / static_cast<double>(t)), shift(0.), t(t), low(0.f) {}
+  __device__ __forceinline__ void from(float largest) {
+    top = static_cast<double>(largest);
+    shift = top * inv;
+    low = fmaf(-700.f, t, largest);
   }
-  // e^(top / t) over e^shift: what a sum of terms of `sum` is to be divided by.
-  __device__ __forceinline__ double rest() const { return 1. + fma(top, inv, -shift); }
-  // e^u, u <= 0, and `sum` (next to nothing, not 0, below e^-700).
+  // A sum of `sum`'s terms, which are e^shift / e^(top / t) too large: by a factor of 1 and
+  // next to nothing.
+  __device__ __forceinline__ double corrected(double sum) const { return fma(-fma(top, inv, -shift), sum, sum); }
+  // e^u, -707 <= u <= 0, and `sum`.
   __device__ __forceinline__ double plus(double u, double sum) const {
     constexpr double kMagic = 6755399441055744., kStep = 2.7076061740622863e-3;   // 1.5 · 2^52; ln 2 / 256
-    u = fmax(u, -700.);
     const double d = fma(u, 1. / kStep, kMagic);   // its low word is the nearest whole number
     const double y = fma(d - kMagic, -kStep, u);
     double p = fma(y, 1. / 6., .5);
@@ -138,16 +142,18 @@ struct Exp {
     p = fma(p, y, 1.);
     const int k = __double2loint(d);
     const double q = powers[k & (kPowers - 1)];
-    return fma(p, __hiloint2double(__double2hiint(q) + (k >> 8) * (1 << 20), __double2loint(q)), sum);
+    return fma(p, __hiloint2double(__double2hiint(q) + k * (1 << 12), __double2loint(q)), sum);
   }
   // x/t - shift is one rounding of a value of its own size off: an instruction less than
-  // the difference first. Not where shift's own rounding is more than rest() corrects.
-  __device__ __forceinline__ bool near() const { return fabs(shift) < 1e6; }
+  // the difference first. Not where shift's own rounding is more than `corrected` corrects,
+  // nor where 700 t is no fp32 value. Masses under e^-700 are next to nothing, not 0: the
+  // logit is held from `low` on (in 32 bits: a maximum in 64 takes twice as long).
+  __device__ __forceinline__ bool near() const { return fabs(shift) < 1e6 && t < 1e35f; }
   __device__ __forceinline__ double near_plus(float x, double sum) const {
-    return plus(fma(static_cast<double>(x), inv, -shift), sum);
+    return plus(fma(static_cast<double>(__builtin_amdgcn_fmed3f(x, low, INFINITY)), inv, -shift), sum);
   }
   __device__ __forceinline__ double far_plus(float x, double sum) const {
-    return plus((static_cast<double>(x) - top) * inv, sum);
+    return plus(fmax((static_cast<double>(x) - top) * inv, -700.), sum);
   }
   // The mass itself, 0 below e^-690 (and of -infinity).
   __device__ __forceinline__ double operator()(float x) const {
@@ -155,8 +161,13 @@ struct Exp {
     return u > -690. ? plus(u, 0.) : 0.;
   }
 };
+// k = 256 n + j added to the exponent as k · 2^12 is n and j / 256: the latter is taken out
+// of the table's entry j before, for an instruction less than n alone.
 __device__ __forceinline__ void load_powers(double* powers) {
-  if (threadIdx.x < kPowers) powers[threadIdx.x] = kPower[threadIdx.x];
+  const int j = threadIdx.x;
+  if (j >= kPowers) return;
+  const double q = kPower[j];
+  powers[j] = __hiloint2double(__double2hiint(q) - j * (1 << 12), __double2loint(q));
 }
 
 struct Row {
@@ -214,7 +225,7 @@ struct Tokens {
 // the sum of each 1024's masses, relative to its largest: one read of the logits, a wave
 // a group (so that many rows and one row alike fill the device). A row's last 1024, where
 // they are fewer, are copied and filled up, so that later passes read whole ones. Bound by
-// HBM for fp32 and by the nine instructions of 64 bits a token for bf16; reads past the
+// HBM for fp32 and by 20 instructions a token for bf16; reads past the
 // caches gain 2 us of 66 there and nothing for fp32, and would take from the next pass
 // what it finds in them.
 __device__ __forceinline__ float max3(float a, float b, float c) {   // (a NaN is looked for apart)
@@ -223,73 +234,78 @@ __device__ __forceinline__ float max3(float a, float b, float c) {   // (a NaN i
   return m;
 }
 template <typename E>
-__global__ __launch_bounds__(256) void sample_groups_kernel(SampleArgs a) {
+__global__ __launch_bounds__(256) void sample_groups_kernel(SampleArgs a, int each) {
   using T = Tokens<E>;
   __shared__ double powers[kPowers];
-  load_powers(powers);
-  __syncthreads();
-  const int64_t row = blockIdx.y, group = blockIdx.x * int64_t{4} + (threadIdx.x >> 6);
+  const int64_t row = blockIdx.y, from = blockIdx.x * int64_t{4} * each;
+  const int64_t end = from + 4 * each < a.n1024 ? from + 4 * each : a.n1024;
   const int lane = threadIdx.x & 63;
-  if (group >= a.n1024) return;
+  int64_t group = from + uniform(static_cast<int>(threadIdx.x >> 6));
+  const E* const logits = static_cast<const E*>(a.x) + row * a.ldx;
   T raw;
-  const E* at0 = static_cast<const E*>(a.x) + row * a.ldx + group * kGroup;
-  if ((group + 1) * kGroup <= a.v) {
-    raw.fetch(at0);
-  } else {
-    raw.fetch(at0, a.v - group * kGroup);
-    raw.store(static_cast<E*>(a.tails) + row * kGroup);
-  }
-  float x[16];
-#pragma unroll
-  for (int k = 0; k < 16; ++k) x[k] = raw.at(k / T::kPer, k % T::kPer);
-  constexpr int kLanes = 64 / T::kPer;   // that hold 64 neighbouring tokens
-  float top = -INFINITY;
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < T::kLoads; ++i) {
-    const float* y = x + i * T::kPer;
-    float m = max3(y[0], y[1], y[2]);
-    bool bad = __builtin_isunordered(y[0], y[1]) || __builtin_isunordered(y[2], y[3]);
-    if constexpr (T::kPer == 8) {
-      m = max3(max3(m, y[3], y[4]), y[5], max3(y[6], y[7], y[7]));
-      bad = bad || __builtin_isunordered(y[4], y[5]) || __builtin_isunordered(y[6], y[7]);
+  auto fetch = [&](int64_t g) {
+    if ((g + 1) * kGroup <= a.v) {
+      raw.fetch(logits + g * kGroup);
     } else {
-      m = max3(m, y[3], y[3]);
+      raw.fetch(logits + g * kGroup, a.v - g * kGroup);
+      raw.store(static_cast<E*>(a.tails) + row * kGroup);
     }
-    uint32_t key = bad ? kNan : key_of(m);
-    key = most_of<kLanes>(key);
-    const int64_t at = group * (kGroup / 64) + i * T::kPer + lane / kLanes;
-    if (lane % kLanes == 0 && at < a.n64) a.tops[row * a.n64 + at] = key;
-    nan = nan || key == kNan;
-    top = max3(top, value_of(key), top);
-  }
-  uint32_t key = nan ? kNan : key_of(top);
-  key = lane_of(wave_scan(key, Most{}), 63);
-  if (lane == 0) a.firsts[row * a.n1024 + group] = key;
+  };
+  if (group < end) fetch(group);
+  load_powers(powers);
   const Row r = row_of(a, row);
-  if (!whole(r)) return;
-  double mass = 0.;
-  if (key >= kInf) {
+  const bool weigh = whole(r);
+  Exp e(powers, r.t);
+  __syncthreads();
+  for (; group < end; group += 4) {
+    float x[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) mass += x[k] == INFINITY ? 1. : 0.;
-  } else if (key > kNone) {
-    Exp e(powers, r.t);
-    e.from(static_cast<double>(value_of(key)));
-    if (e.near()) {
-      double part = 0.;
+    for (int k = 0; k < 16; ++k) x[k] = raw.at(k / T::kPer, k % T::kPer);
+    if (group + 4 < end) fetch(group + 4);
+    constexpr int kLanes = 64 / T::kPer;   // that hold 64 neighbouring tokens
+    uint32_t key = 0, mine = 0;            // the largest; of lane i of each kLanes, load i's
 #pragma unroll
-      for (int k = 0; k < 16; k += 2) {
-        mass = e.near_plus(x[k], mass);
-        part = e.near_plus(x[k + 1], part);
+    for (int i = 0; i < T::kLoads; ++i) {
+      const float* y = x + i * T::kPer;
+      float m = max3(y[0], y[1], y[2]);
+      bool bad = __builtin_isunordered(y[0], y[1]) | __builtin_isunordered(y[2], y[3]);
+      if constexpr (T::kPer == 8) {
+        m = max3(max3(m, y[3], y[4]), y[5], max3(y[6], y[7], y[7]));
+        bad |= __builtin_isunordered(y[4], y[5]) | __builtin_isunordered(y[6], y[7]);
+      } else {
+        m = max3(m, y[3], y[3]);
       }
-      mass = (mass + part) / e.rest();
-    } else {
-#pragma unroll
-      for (int k = 0; k < 16; ++k) mass = e.far_plus(x[k], mass);
+      const uint32_t k64 = most_of<kLanes>(bad ? kNan : key_of_number(m));
+      mine = lane % kLanes == i ? k64 : mine;
+      key = k64 > key ? k64 : key;
     }
+    const int64_t at = group * (kGroup / 64) + lane % kLanes * (64 / kLanes) + lane / kLanes;
+    if (lane % kLanes < T::kLoads && at < a.n64) a.tops[row * a.n64 + at] = mine;
+    key = most_of_rows<kLanes>(key);
+    if (lane == 0) a.firsts[row * a.n1024 + group] = key;
+    if (!weigh) continue;
+    double mass = 0.;
+    if (key >= kInf) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) mass += x[k] == INFINITY ? 1. : 0.;
+    } else if (key > kNone) {
+      e.from(value_of(key));
+      if (e.near()) {
+        double part = 0.;
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+          mass = e.near_plus(x[k], mass);
+          part = e.near_plus(x[k + 1], part);
+        }
+        mass = e.corrected(mass + part);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) mass = e.far_plus(x[k], mass);
+      }
+    }
+    mass = wave_sum(mass);
+    if (lane == 0) a.masses[row * a.n1024 + group] = mass;
   }
-  mass = wave_sum(mass);
-  if (lane == 0) a.masses[row * a.n1024 + group] = mass;
 }
 
 // ---------------------------------------------------------------- picking
@@ -905,7 +921,7 @@ struct Pick {
       return true;
     }
     inf = key == kInf;
-    mass_of.from(inf ? 0. : static_cast<double>(value_of(key)));
+    mass_of.from(inf ? 0.f : value_of(key));
     return false;
   }
   // A key that every token of a mass of at least m reaches.
@@ -1148,10 +1164,13 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
   p.finish();
 }
 
+// Of the first pass: groups of a wave, one after another, where there are enough of them
+// for two waves a SIMD all the same (512 x 131072 bf16, the whole call: one 66 us, two 65.7,
+// four 63.1, eight and sixteen 62.5, before the maxima took fewer instructions).
+constexpr int64_t kMostEach = 8;
 template <typename E>
 hipError_t sample(const SampleArgs& a, hipStream_t stream) {
   constexpr int64_t kRows = 65535;   // of a launch's second dimension
-  const auto across = static_cast<unsigned>((a.n1024 + 3) / 4);
   for (int64_t r = 0; r < a.n; r += kRows) {
     SampleArgs p = a;
     const int64_t n = a.n - r < kRows ? a.n - r : kRows;
@@ -1168,7 +1187,9 @@ hipError_t sample(const SampleArgs& a, hipStream_t stream) {
     p.firsts = a.firsts + r * a.n1024;
     p.masses = a.masses + r * a.n1024;
     p.tails = static_cast<E*>(a.tails) + r * kGroup;
-    hipLaunchKernelGGL(sample_groups_kernel<E>, dim3(across, static_cast<unsigned>(n)), dim3(256), 0, stream, p);
+    const int64_t quads = (a.n1024 + 3) / 4, many = n * quads / 2048, each = many < 1 ? 1 : many > kMostEach ? kMostEach : many;
+    hipLaunchKernelGGL(sample_groups_kernel<E>, dim3(static_cast<unsigned>((quads + each - 1) / each), static_cast<unsigned>(n)),
+                       dim3(256), 0, stream, p, static_cast<int>(each));
     hipLaunchKernelGGL(sample_row_kernel<E>, dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream, p);
   }
   return hipGetLastError();

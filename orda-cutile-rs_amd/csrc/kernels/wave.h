@@ -51,6 +51,16 @@ __device__ __forceinline__ uint32_t most_of(uint32_t v) {
   return LANES == 8 ? v : op(v, moved<0x140, 0xf>(v));
 }
 template <typename T>
+__device__ __forceinline__ T lane_of(T v, int lane);
+// The wave's largest, given values that each LANES (8 or 16) neighbouring lanes have alike.
+template <int LANES>
+__device__ __forceinline__ uint32_t most_of_rows(uint32_t v) {
+  const Most op;
+  if constexpr (LANES == 8) v = op(v, moved<0x118, 0xf>(v));
+  v = op(v, moved<0x142, 0xa>(v));
+  return lane_of(op(v, moved<0x143, 0xc>(v)), 63);
+}
+template <typename T>
 __device__ __forceinline__ T lane_of(T v, int lane) {
   if constexpr (sizeof(T) == 4) {
     return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
