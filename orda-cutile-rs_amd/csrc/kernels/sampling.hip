@@ -148,7 +148,7 @@ struct Exp {
   // the difference first. Not where shift's own rounding is more than `corrected` corrects,
   // nor where 700 t is no fp32 value. Masses under e^-700 are next to nothing, not 0: the
   // logit is held from `low` on (in 32 bits: a maximum in 64 takes twice as long).
-  __device__ __forceinline__ bool near() const { return fabs(shift) < 1e6 && t < 1e35f; }
+  __device__ __forceinline__ bool near() const { return fabs(shift) < 1e6 && t < 1e35f && low > -INFINITY; }
   __device__ __forceinline__ double near_plus(float x, double sum) const {
     return plus(fma(static_cast<double>(__builtin_amdgcn_fmed3f(x, low, INFINITY)), inv, -shift), sum);
   }

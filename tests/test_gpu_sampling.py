@@ -295,3 +295,18 @@ def test_refusals():
 def test_parameters_that_are_no_numbers(kw):
     with pytest.raises(H.OrdaError, match="numbers"):
         H.sample_tokens(torch.zeros(2, 8, device="cuda"), torch.zeros(2, device="cuda"), **kw)
+
+
+@pytest.mark.parametrize("t", [1e30, 1e33, 1e34, 1e36, 3e38])
+@pytest.mark.parametrize("v", [10, 3000])
+def test_logits_and_temperatures_at_the_types_end(v, t):
+    """Masses that are all alike, or nothing, and tokens that are banned beside them."""
+    g = torch.Generator().manual_seed(v)
+    x = -3.3e38 + 1e37 * torch.randn(6, v, generator=g).clamp(-0.9, 2)
+    x[:, torch.rand(v, generator=g) < 0.3] = -math.inf
+    x[:, 3] = -3.35e38
+    x[3:] = -x[3:].abs().clamp_max(3.4e38) * torch.where(torch.isinf(x[3:]), 1.0, -1.0)   # large, some banned
+    u = torch.rand(6, generator=g)
+    u[0] = 0
+    for kw in (dict(), dict(p=0.9), dict(k=7), dict(m=0.5), dict(k=2000, p=0.5)):
+        compare(x.cuda(), u.cuda(), t=t, **kw)
