@@ -593,14 +593,14 @@ class _NormGrad:
 
     def __init__(self, a: bytes, t, w, want_x: bool, want_w: bool, rows: bool = True):
         torch = _torch()
-        self.shape = shape = n, h = t.shape
+        self.shape = n, h = t.shape
         self.device, self.dtype = device, dtype = t.device, t.dtype
         self.want_x, self.want_w = want_x, want_w
         self.gx = self.ws = self.gw = None
         self.bytes = _norm_bytes(n, h)
         kind, x, weight = _DTYPES[dtype], 0, _NO_TENSOR
         if want_x and rows:
-            self.gx = gx = torch.empty(shape, dtype=dtype, device=device)
+            self.gx = gx = _like(t)
             x = gx.data_ptr()
         if rows:
             self.ws = _bytes(self.bytes, device)

@@ -2,6 +2,8 @@
 use them: serving (norm in e4m3, the head's product, tokens) and training (lookup, norm,
 linear cross entropy, gradients, clipping). Each operator's values are tested against
 float64 where it stands alone; here what one gives the next is checked on the way."""
+import threading
+
 import pytest
 import torch
 
@@ -211,3 +213,37 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for i, out in enumerate(got):
         assert all(torch.equal(bits(x), bits(y)) for x, y in zip(out, want[i % 2]))
+
+
+def test_threads_at_once():
+    """Calls of several threads, each on a stream of its own, refused ones (with their own messages) among them."""
+    errors = []
+
+    def work(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                x, w = normal((300, 700), seed, 1.0, torch.float32), normal((700,), seed, 0.2, torch.float32)
+                logits, u = normal((20, 5000), seed, 2.0, torch.float32), torch.full((20,), 0.37, device="cuda")
+                first = None
+                for _ in range(20):
+                    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+                    rms_norm_autograd(a, b)[0].square().sum().backward()
+                    tokens, logprobs = H.sample_tokens(logits, u, top_p=0.9)
+                    grads = [a.grad.clone(), b.grad.clone()]
+                    now = [a.grad, b.grad, tokens, logprobs, H.clip_gradients(grads, 0.5), *grads]
+                    with pytest.raises(H.OrdaError, match="weight must be"):
+                        H.rms_norm(x, w[:5])
+                    with pytest.raises(H.OrdaError, match="temperature must be"):
+                        H.sample_tokens(logits, u, temperature=-1.0)
+                    with pytest.raises(H.OrdaError, match="eps must be"):
+                        H.rms_norm(x, w, eps=-1.0)
+                    first = first or now
+                    assert all(torch.equal(p, q) for p, q in zip(first, now))
+        except BaseException as e:   # (pytest sees the main thread's alone)
+            errors.append(repr(e))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors

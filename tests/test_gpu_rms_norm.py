@@ -5,6 +5,7 @@ once; a value t·s·(w + o) has then at most four more roundings, and one to its
 """
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import orda_hip as H
 from orda_hip.autograd import rms_norm_autograd
@@ -400,3 +401,52 @@ def test_options_that_are_no_numbers(kw):
     for call in (H.rms_norm, H.rms_norm_fp8, rms_norm_autograd, lambda x, w, **kw: H.rms_norm_backward(x, x, w, **kw)):
         with pytest.raises(H.OrdaError, match="numbers"):
             call(x, w, **kw)
+
+
+def test_autograd_of_unusual_calls():
+    """Shapes, strides and uses beside the usual ones, against torch's gradients in 64 bits. Both gradients are sums
+    of at most 100 terms of magnitude 30 or less: 1e-4 is 500 roundings of fp32 of them."""
+    def check(x, w, r=None, offset=0.0, both=False):
+        own = [None if a is None else a.detach().requires_grad_(True) for a in (x, w, r)]
+        ref = [None if a is None else a.detach().double().requires_grad_(True) for a in (x, w, r)]
+        y = rms_norm_autograd(own[0], own[1], residual=own[2], weight_offset=offset, eps=EPS)
+        y, t = y if r is not None else (y, None)
+        t64 = ref[0] if r is None else ref[0] + ref[2]
+        y64 = t64 * (t64.square().mean(-1, keepdim=True) + EPS).rsqrt() * (ref[1] + offset)
+        g = torch.linspace(-1, 1, y.numel(), device="cuda").reshape(y.shape)
+        ((y * g).sum() + ((t * g).sum() if both else 0)).backward()
+        ((y64 * g.double()).sum() + ((t64 * g.double()).sum() if both else 0)).backward()
+        for a, b in zip(own, ref):
+            assert a is None or (a.grad.shape == a.shape and ((a.grad.double() - b.grad).abs() <= 1e-4).all())
+
+    def rnd(*shape):
+        return normal(shape, "f32")
+    check(rnd(0, 8), rnd(8))
+    check(rnd(8), rnd(8), rnd(8), 1.0, True)
+    check(rnd(2, 3, 4, 16), rnd(16), rnd(2, 3, 4, 16), 0.0, True)
+    check(rnd(3, 1), rnd(1))
+    check(rnd(16, 5).t(), rnd(16))
+    check(rnd(6, 20)[:, 3:17], rnd(28)[::2], rnd(6, 21)[:, 1:15], 1.0, True)
+    # one tensor in both places, and a broadcast one
+    x, w = rnd(5, 33).requires_grad_(True), rnd(33).requires_grad_(True)
+    y, t = rms_norm_autograd(x, w, residual=x)
+    gx = torch.autograd.grad(y.sum() + t.sum(), x)[0]
+    alone = torch.autograd.grad(sum(o.sum() for o in rms_norm_autograd(x, w, residual=x.detach())), x)[0]
+    assert torch.equal(gx, 2 * alone)
+    row = rnd(1, 33).requires_grad_(True)
+    rms_norm_autograd(row.expand(7, 33), w).sum().backward()
+    assert row.grad.shape == (1, 33)
+    # the sum alone is used; a part of the gradients is asked for
+    r = rnd(5, 33).requires_grad_(True)
+    _, t = rms_norm_autograd(x, w, residual=r)
+    gx, gr, gw = torch.autograd.grad(t.sum(), [x, r, w])
+    assert (gx == 1).all() and (gr == 1).all() and (gw == 0).all()
+    y = rms_norm_autograd(x, w)
+    part = torch.autograd.grad(y.sum(), [w], retain_graph=True)[0]
+    assert torch.equal(part, torch.autograd.grad(y.sum(), [x, w])[1])
+    # recomputed in the backward
+    want = torch.autograd.grad(rms_norm_autograd(x, w).tanh().sum(), [x, w])
+    for reentrant in (True, False):
+        x.grad = w.grad = None
+        torch.utils.checkpoint.checkpoint(lambda x: rms_norm_autograd(x, w).tanh(), x, use_reentrant=reentrant).sum().backward()
+        assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
