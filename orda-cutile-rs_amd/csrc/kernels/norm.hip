@@ -585,7 +585,9 @@ GradLaunch grad_launch(int64_t h) {
 }
 int grad_teams(int64_t h) { return h <= 1024 ? 8 : h <= 2048 ? 4 : h <= 4096 ? 2 : 1; }
 
-constexpr int64_t kGradBlocks = 256;   // workgroups that keep sums of the weight's gradient
+// Workgroups that keep sums of the weight's gradient, one a CU (of 512 the kernel takes as long
+// and the join 4 us more; 8192 x 4096 bf16).
+constexpr int64_t kGradBlocks = 256;
 int64_t grad_blocks(int64_t n, int64_t h) {
   const int64_t b = (n + grad_teams(h) - 1) / grad_teams(h);
   return b < kGradBlocks ? b : kGradBlocks;
