@@ -101,7 +101,7 @@ Cut cut(const orda_gradient* g, int64_t count, bool scale) {
       l.pieces += pieces_of(c.parts[at]);
     }
     // its share of 2048, or as many as have eight pieces each: with the share alone 110
-    // gradients of 1.05 GB, two launches, took 226 us for the norm, so 190
+    // gradients of 1.05 GB, two launches, took 226 us for the norm, so 212
     const int64_t share = kBlocks * l.pieces / pieces, most = kSums * l.pieces / pieces;
     l.blocks = static_cast<int>(std::max<int64_t>(1, std::min({l.pieces, std::max(share, std::min(kBlocks, l.pieces / 8)), most})));
     c.sums += l.blocks;
