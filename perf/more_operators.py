@@ -127,7 +127,8 @@ def _logits(case, g):
         likely = torch.randint(0, v, (n, 30), generator=g, device="cuda")
         sharp = 1.0 + 6.0 * torch.rand((n, 1), generator=g, device="cuda")
         above = 4.0 + torch.empty((n, 30), device="cuda").exponential_(1.0, generator=g) * sharp.sqrt()
-        x.scatter_(1, likely, above.clamp_max(20.0))
+        # (places may repeat: the largest, whatever the order in which they are written)
+        x.scatter_reduce_(1, likely, above.clamp_max(20.0), "amax", include_self=False)
     if case["banned"]:
         mask = torch.rand(v, generator=g, device="cuda") < case["banned"]
         x.masked_fill_(mask, -math.inf)
