@@ -1105,6 +1105,15 @@ struct Pick {
         break;
       }
       const double above = sum_of_groups();
+      if (source == kMass && above >= goal) {
+        // Sums in fixed point, off by up to 2^-44 a token, found the cut a bin too late:
+        // kept is what lies above the members.
+        const uint64_t over = (static_cast<uint64_t>(key_of(q.hi)) + 1) << 32;
+        if (!q.limited || q.limit < over) q.limit = over;
+        q.limited = true;
+        source = kDirect;
+        continue;
+      }
       if (!fits) {
         q.most = block_most(key_of(most));
         const uint32_t span = q.most - ~block_most(~key_of(low));
