@@ -1129,7 +1129,7 @@ struct Pick {
         const double w = weight(q.hi);
         double want = static_cast<double>(n);
         if (source == kCount) {
-          want = static_cast<double>(r.k - before);
+          want = fmin(want, static_cast<double>(r.k - before));   // (fewer than k may be over -infinity)
           all_mass = above + want * w;
         }
         const double limit = r.p < 1.f ? static_cast<double>(r.p) * all_mass : INFINITY;

@@ -62,3 +62,21 @@ def test_a_border_within_the_roundings_of_fixed_point(beside, k):
     w = kept(x.astype(np.float64), k=k, p=0.5)
     assert (w > 0).sum() == 10001
     check(torch.from_numpy(x), k=k, p=0.5)
+
+
+@pytest.mark.parametrize("v, n, largest", [(32000, 10000, 0), (32000, 10000, 20), (5000, 2600, 3)])
+@pytest.mark.parametrize("banned", [-math.inf, math.inf], ids=["banned", "infinite"])
+def test_top_k_of_more_than_there_are_among_equal_ones(v, n, largest, banned):
+    """n equal logits and a few over them, the others banned (or n of +infinity, which alone count): top-p's share
+    is of the tokens that there are, not of k."""
+    at = np.random.default_rng(v + n).permutation(v)
+    if banned < 0:
+        x = np.full(v, -math.inf)
+        x[at[:n]], x[at[:largest]] = 1.5, 2.0
+    else:
+        x = np.random.default_rng(n).standard_normal(v)
+        x[at[:n]] = math.inf
+    for k, p in ((n + n // 2, 0.5), (n + 1, 0.9), (n, 0.5), (n - 100, 0.5), (n + n // 2, 1.0), (n + n // 2, 0.001)):
+        for dtype in (torch.float32, torch.bfloat16):
+            check(torch.from_numpy(x).to(dtype), k=k, p=p)
+            check(torch.from_numpy(x).to(dtype), k=k, p=p, m=0.9, t=0.7)
