@@ -207,12 +207,11 @@ class RmsNormFunction(torch.autograd.Function):
     """out, total = RmsNormFunction.apply(x, weight, residual, eps, weight_offset);
     total is None without a residual."""
 
-    # The backward call is made ready by the forward's: torch's engine runs a backward's
-    # Python on another thread, where it takes two to three times as long (a step of few rows
-    # 96 us, 108 where the backward packs its arguments). grad_x and the scratch too, up to
-    # this many bytes of rows (1000 x 1531 fp32 101 us, 107 where the backward makes them):
-    # larger ones are not held from the forward on.
-    READY_BYTES = 16 << 20
+    # The backward's arguments are packed by the forward: torch's engine runs a backward's
+    # Python on another thread, where it takes two to three times as long. Gradients and
+    # scratch are not made ready, for a graph that is captured of the backward alone owns
+    # what it writes, and no rows are held beside the saved ones (a step of up to 4 M values
+    # 100 us; with both made ready 95).
 
     @staticmethod
     def forward(fctx, x, weight, residual, eps, weight_offset):
@@ -221,9 +220,8 @@ class RmsNormFunction(torch.autograd.Function):
         fctx.ready = None
         want_x, want_w, want_r = fctx.needs_input_grad[:3]
         if w is weight and t.numel() and t.is_contiguous() and (want_x or want_w or want_r):
-            small = t.numel() * t.element_size() <= RmsNormFunction.READY_BYTES
             # (the forward's arguments; of a sum those without the residual, its address is put in)
-            fctx.ready = _NormGrad(a if total is None else _without_residual(a), t, w, want_x or want_r, want_w, small)
+            fctx.ready = _NormGrad(a if total is None else _without_residual(a), t, w, want_x or want_r, want_w)
         if x.dim() != 2:
             out, total = out.view(x.shape), total.view(x.shape) if total is not None else None
         fctx.save_for_backward(x if total is None else total, weight)

@@ -587,34 +587,25 @@ def _without_residual(a: bytes) -> bytes:
 
 class _NormGrad:
     """A backward call of a matrix like t, a weight like w and orda_rms_norm, made ready:
-    its arguments but for the addresses that come in, and the weight's gradient; with
-    `rows` also grad_x and the scratch, which else are made when it runs."""
-    __slots__ = "buf", "at", "want_x", "want_w", "gx", "gw", "ws", "bytes", "device", "shape", "dtype"
+    its arguments but for the addresses. It holds no device memory; gradients and scratch
+    are made when it runs, from the pool of the stream or the graph that it runs in."""
+    __slots__ = "buf", "at", "want_x", "want_w", "bytes", "device", "shape", "dtype"
 
-    def __init__(self, a: bytes, t, w, want_x: bool, want_w: bool, rows: bool = True):
-        torch = _torch()
+    def __init__(self, a: bytes, t, w, want_x: bool, want_w: bool):
         self.shape = n, h = t.shape
-        self.device, self.dtype = device, dtype = t.device, t.dtype
+        self.device, self.dtype = t.device, t.dtype
         self.want_x, self.want_w = want_x, want_w
-        self.gx = self.ws = self.gw = None
         self.bytes = _norm_bytes(n, h)
-        kind, x, weight = _DTYPES[dtype], 0, _NO_TENSOR
-        if want_x and rows:
-            self.gx = gx = _like(t)
-            x = gx.data_ptr()
-        if rows:
-            self.ws = _bytes(self.bytes, device)
-        if want_w:
-            self.gw = gw = torch.empty_like(w)
-            weight = gw.data_ptr(), 1, h, h, _DTYPES[w.dtype], L.DEVICE
+        kind = _DTYPES[t.dtype]
         self.buf, self.at = _packed(a + _NORM_GRADS.pack(0, n, h, h, kind, L.DEVICE, 0, n, h, h, kind, L.DEVICE,
-                                                         x, n, h, h, kind, L.DEVICE, *weight))
+                                                         0, n, h, h, kind, L.DEVICE,
+                                                         0, 1, h, h, _DTYPES[w.dtype], L.DEVICE))
 
     def run(self, t, w, g, gt):
         """(grad_x, grad_weight), given the sum and the weight (which may have moved, but are
         as the ones it was made for) and plain gradients of t's number of values and dtype."""
-        buf, gx, ws, put = self.buf, self.gx, self.ws, _ADDRESS.pack_into
-        index = self.device.index
+        torch, buf, put = _torch(), self.buf, _ADDRESS.pack_into
+        index, gx, gw = self.device.index, None, None
         if not index == t.get_device() == w.get_device() == g.get_device() or (gt is not None and gt.get_device() != index):
             raise OrdaError(f"weight and gradients must be on {self.device}")
         if not g.is_contiguous():
@@ -628,15 +619,17 @@ class _NormGrad:
         put(buf, 0, t.data_ptr())
         put(buf, 80, w.data_ptr())
         put(buf, 136, g.data_ptr())
-        if gx is None and self.want_x:
-            gx = _torch().empty(self.shape, dtype=self.dtype, device=self.device)
+        if self.want_x:
+            gx = torch.empty(self.shape, dtype=self.dtype, device=self.device)
             put(buf, 216, gx.data_ptr())
-        if ws is None:
-            ws = _bytes(self.bytes, self.device)
+        if self.want_w:
+            gw = torch.empty_like(w)
+            put(buf, 256, gw.data_ptr())
+        ws = _bytes(self.bytes, self.device)
         at = self.at
-        _check(L.load().orda_rms_norm_backward(index, _torch()._C._cuda_getCurrentRawStream(index), at, at + 136, at + 176,
+        _check(L.load().orda_rms_norm_backward(index, torch._C._cuda_getCurrentRawStream(index), at, at + 136, at + 176,
                                                at + 216, at + 256, ws.data_ptr(), self.bytes, _message(), 512))
-        return gx, self.gw
+        return gx, gw
 
 
 # ------------------------------------------------------------------ gradient norm and clipping
