@@ -658,9 +658,10 @@ def _gradient_table(n: int):
     return struct.Struct("=" + n * 2 * _TENSOR)   # orda_gradient
 
 
-def _plain_gradients(grads, out, index):
+def _plain_gradients(grads, out, index, unwritten):
     """The table of contiguous gradients and destinations, as most are (37 us for 37 of
-    both, 56 with the checks below); None where one is anything else."""
+    both, 56 with the checks below); None where one is anything else. unwritten: leaves
+    that require a gradient are refused."""
     torch = _torch()
     kinds = torch.Tensor, torch.nn.Parameter
     dtypes = {torch.float32: L.F32, torch.bfloat16: L.BF16}
@@ -669,6 +670,8 @@ def _plain_gradients(grads, out, index):
     try:
         for g, o in zip(grads, grads if out is None else out):
             if type(g) not in kinds or g.get_device() != index or not g.is_contiguous() or g.is_neg():
+                return None
+            if unwritten and g.requires_grad and g.is_leaf:
                 return None
             p, n = g.data_ptr(), g.numel()
             if not p and n:
@@ -689,8 +692,8 @@ def _plain_gradients(grads, out, index):
     return fields
 
 
-def _gradients(grads, out):
-    """(orda_gradient array, the gradients, device, destinations)."""
+def _gradients(grads, out, scale: bool):
+    """(orda_gradient array, the gradients, device, destinations). scale: they are written."""
     torch = _torch()
     grads = list(grads)
     if out is None:
@@ -703,14 +706,17 @@ def _gradients(grads, out):
     if not grads:
         raise OrdaError("there are no gradients")
     device = _gpu_tensor(grads[0], "gradient 0").device
-    fields = _plain_gradients(grads, out, device.index)
+    recording = torch.is_grad_enabled()
+    unwritten = scale and recording and out is None
+    fields = _plain_gradients(grads, out, device.index, unwritten)
     if fields is not None:
         return _gradient_table(len(grads)).pack(*fields), grads, device, out
-    recording = torch.is_grad_enabled()
     fields = []
     for i, (g, o) in enumerate(zip(grads, to)):
         _same_device(device, **{f"gradient {i}": _gpu_tensor(g, f"gradient {i}")})
         r, c, ld = _view(g, f"gradient {i}")
+        if unwritten and g.requires_grad and g.is_leaf:
+            raise OrdaError(f"gradient {i} is a leaf that requires a gradient: it is not written in place")
         fields += g.data_ptr(), r, c, ld, _dtype(g, f"gradient {i}"), L.DEVICE
         if out is None:
             fields += _NO_TENSOR
@@ -736,7 +742,7 @@ def gradient_norm(grads):
     float32 or bfloat16 GPU tensors of any shape, dense in any order or matrices
     with adjacent columns; None is skipped. Squares and sums are formed in 64 bits."""
     torch = _torch()
-    a, grads, device, _ = _gradients(grads, None)
+    a, grads, device, _ = _gradients(grads, None, False)
     b = _clip_bytes(len(grads))
     ws = _bytes(b, device)
     norm = torch.empty((), dtype=torch.float32, device=device)
@@ -752,9 +758,10 @@ def clip_gradients(grads, max_norm: float, *, eps: float = 1e-6, out=None):
     of the same shapes and strides, float32 or bfloat16, whatever the factor (the
     gradients then stay as they are, and none may be None). A norm that is NaN makes
     all of them NaN. Does not wait for the device. Tensors that are written share no
-    memory with others of the call."""
+    memory with others of the call, and while torch records none is a leaf that requires
+    a gradient (a parameter in its gradient's place)."""
     torch = _torch()
-    a, grads, device, out = _gradients(grads, out)
+    a, grads, device, out = _gradients(grads, out, True)
     b = _clip_bytes(len(grads))
     ws = _bytes(b, device)
     norm = torch.empty((), dtype=torch.float32, device=device)
