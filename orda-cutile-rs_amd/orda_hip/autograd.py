@@ -238,8 +238,7 @@ class RmsNormFunction(torch.autograd.Function):
                     g_total if want_r else None, None, None)
         ready, fctx.ready = fctx.ready, None   # (a second backward makes its own)
         # (saved tensors' hooks and whoever holds weights apart may have moved them)
-        if (ready is not None and ready.want_x == (want_x or want_r) and ready.want_w == want_w
-                and total.is_contiguous() and weight.is_contiguous()):
+        if ready is not None and ready.want_x == (want_x or want_r) and ready.want_w == want_w and ready.takes(total, weight):
             _gpu_tensor(g_out, "grad_out")
             if g_total is not None:
                 _gpu_tensor(g_total, "grad_total")

@@ -589,11 +589,12 @@ class _NormGrad:
     """A backward call of a matrix like t, a weight like w and orda_rms_norm, made ready:
     its arguments but for the addresses. It holds no device memory; gradients and scratch
     are made when it runs, from the pool of the stream or the graph that it runs in."""
-    __slots__ = "buf", "at", "want_x", "want_w", "bytes", "device", "shape", "dtype"
+    __slots__ = "buf", "at", "want_x", "want_w", "bytes", "device", "shape", "values", "dtype", "weight"
 
     def __init__(self, a: bytes, t, w, want_x: bool, want_w: bool):
-        self.shape = n, h = t.shape
-        self.device, self.dtype = t.device, t.dtype
+        self.shape, self.values = t.shape, t.numel()
+        n, h = t.shape
+        self.device, self.dtype, self.weight = t.device, t.dtype, w.dtype
         self.want_x, self.want_w = want_x, want_w
         self.bytes = _norm_bytes(n, h)
         kind = _DTYPES[t.dtype]
@@ -601,9 +602,14 @@ class _NormGrad:
                                                          0, n, h, h, kind, L.DEVICE,
                                                          0, 1, h, h, _DTYPES[w.dtype], L.DEVICE))
 
+    def takes(self, t, w) -> bool:
+        """Whether they are as the sum and the weight that it was made for, but for their place."""
+        return (t.dtype is self.dtype and w.dtype is self.weight and t.numel() == self.values
+                and w.shape == self.shape[1:] and t.is_contiguous() and w.is_contiguous())
+
     def run(self, t, w, g, gt):
-        """(grad_x, grad_weight), given the sum and the weight (which may have moved, but are
-        as the ones it was made for) and plain gradients of t's number of values and dtype."""
+        """(grad_x, grad_weight), given a sum and a weight that it `takes` and plain gradients
+        of t's number of values and dtype."""
         torch, buf, put = _torch(), self.buf, _ADDRESS.pack_into
         index, gx, gw = self.device.index, None, None
         if not index == t.get_device() == w.get_device() == g.get_device() or (gt is not None and gt.get_device() != index):
