@@ -69,15 +69,20 @@ def _same_device(device, **tensors):
             raise OrdaError(f"{name} is on {t.device}, not on {device}")
 
 
+def _is_matrix(x) -> bool:
+    """Whether a 2-D tensor has adjacent columns and rows that do not overlap."""
+    if x.is_contiguous():
+        return True
+    (r, c), (sr, sc) = x.shape, x.stride()
+    return not ((c > 1 and sc != 1) or (r > 1 and sr < c))
+
+
 def _matrix(x, what: str):
     """x as a 2-D tensor with adjacent columns and rows that do not overlap (a
     copy where it is none)."""
     if x.dim() != 2:
         raise OrdaError(f"{what} must be 2-D")
-    if x.is_contiguous():
-        return x
-    (r, c), (sr, sc) = x.shape, x.stride()
-    return x.contiguous() if (c > 1 and sc != 1) or (r > 1 and sr < c) else x
+    return x if _is_matrix(x) else x.contiguous()
 
 
 def _overlap(a, b) -> bool:
@@ -652,9 +657,9 @@ def _view(g, what: str):
         at *= size
     else:
         return 1, n, n
-    if g.dim() == 2 and _matrix(g, what) is g:
+    if g.dim() == 2 and _is_matrix(g):
         return g.size(0), g.size(1), g.stride(0)
-    if g.dim() == 2 and _matrix(g.t(), what).data_ptr() == g.data_ptr():
+    if g.dim() == 2 and _is_matrix(g.t()):
         return g.size(1), g.size(0), g.stride(1)
     raise OrdaError(f"{what} must be dense, or a matrix with adjacent columns or rows")
 
