@@ -465,7 +465,8 @@ int32_t orda_rms_norm_backward(int32_t device, void *hip_stream, const orda_rms_
  * gradient is a matrix, fp32 or bf16 (a contiguous tensor of any shape: one row);
  * dst without data: scaled in place, and where the norm is within max_norm not
  * touched; else written to dst, of the same shape. A norm that is NaN makes every
- * gradient NaN, an infinite one makes the finite values 0 and the others NaN.
+ * gradient NaN, an infinite one makes the finite values 0 and the others NaN. The
+ * factor is 1 wherever norm + eps <= max_norm, where both are infinite or 0 too.
  * Destinations (in place: the gradients) share no memory with one another or with
  * other gradients. norm is one float32. At most 2^20 gradients of 2^40 values
  * together. Device, stream and workspace as above. No counterpart in the reference. */

@@ -177,8 +177,8 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(GradArgs a) {
   __shared__ double part[kThreads / 64];
   const double n = sqrt(total(a.all, a.n_sums, part));
   if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = static_cast<float>(n);
-  const double f64 = a.max_norm / (n + a.eps);
-  const float f = f64 >= 1. ? 1.f : static_cast<float>(f64);   // (a NaN stays one)
+  // (1 too where both are 0 or both infinite; a NaN stays one)
+  const float f = n + a.eps <= a.max_norm ? 1.f : static_cast<float>(a.max_norm / (n + a.eps));
   if (a.in_place && f == 1.f) return;
   const int64_t from = share(a, blockIdx.x);
   for (int64_t to = share(a, blockIdx.x + 1); to > from;) {

@@ -768,7 +768,8 @@ def clip_gradients(grads, max_norm: float, *, eps: float = 1e-6, out=None):
     In place, where nothing is written if the factor is 1; or to the tensors of ``out``,
     of the same shapes and strides, float32 or bfloat16, whatever the factor (the
     gradients then stay as they are, and none may be None). A norm that is NaN makes
-    all of them NaN. Does not wait for the device. Tensors that are written share no
+    all of them NaN; the factor is 1 wherever ``norm + eps <= max_norm``, infinite ones
+    included. Does not wait for the device. Tensors that are written share no
     memory with others of the call, and while torch records none is a leaf that requires
     a gradient (a parameter in its gradient's place)."""
     torch = _torch()
