@@ -6,7 +6,7 @@
 // launches' arguments, so that nothing is copied to the device and a captured graph
 // holds them. Bound by HBM: one read for the norm, and where it is over the limit
 // another read and a write. 4.29 GB of fp32: 613 us (7.0 TB/s) and 1640 (5.2 both ways; a
-// copy reaches 4.8); 1.05 GB of bf16 in 110 tensors at any address, two launches: 180 (5.8;
+// copy reaches 4.8); 1.05 GB of bf16 in 110 tensors at any address, two launches: 181 (5.8;
 // 208 before the loads began at whole 16 bytes).
 //
 // The gradients' values are one row of pieces, of which each workgroup has an equal run:

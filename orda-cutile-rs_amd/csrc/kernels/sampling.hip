@@ -16,11 +16,13 @@
 // in which they are formed, or are summed in fixed point or in a fixed order: the same bits
 // in every run.
 //
-// 1 x 131072 fp32, top-k 50 and top-p 0.9: 3 us and 9 of kernels (the host's 15 are more).
-// 256 x 131072 fp32, top-p 0.95 of a flat distribution, the slowest kind: 30 us (4.5 TB/s)
-// and 80, of which the binning's and the listing's passes over the row, one workgroup a
-// row, are the most. 512 x 131072 bf16, unfiltered: 48 us (2.8 TB/s: 20 instructions a
-// token, nine of them in 64 bits) and 10.
+// By the profiler, which keeps launches apart (a call of those after one another beside it):
+// 1 x 131072 fp32, top-k 50 and top-p 0.9: 3 us and 9 (16, of the host).
+// 256 x 131072 fp32, top-p 0.95 of a flat distribution, the slowest kind: 34 us (4.0 TB/s)
+// and 83 (107), of which the binning's and the listing's passes over the row, one workgroup
+// a row, are the most. 512 x 131072 bf16, unfiltered: 58 us (20 instructions a token, nine
+// of them in 64 bits) and 10 (58); greedy, without masses: 30 (4.5 TB/s)
+// and 6 (35).
 #include <math.h>
 
 #include "orda_kernels.h"
