@@ -902,6 +902,18 @@ struct Pick {
     return block_most(o);
   }
 
+  // The token after the one at o, in descending order (o where none is over -infinity
+  // and at or over `limit`).
+  __device__ __forceinline__ uint64_t after(uint64_t o, uint64_t limit) {
+    uint64_t best = 0;
+    for (int64_t c = threadIdx.x; c < a.v; c += kThreads) {
+      const uint64_t at = order_of(value(static_cast<float>(x[c])), c);
+      if (at < o && at > best) best = at;
+    }
+    best = block_most(best);
+    return best >> 32 > kNone && best >= limit ? best : o;
+  }
+
   // ---- a row
   // Whether the row has an answer that needs no masses, and what its masses refer to.
   __device__ __forceinline__ bool begin() {
@@ -938,7 +950,8 @@ struct Pick {
   // The kept ones of a list's n tokens, `above` the masses and `before` the number of
   // those that stand before them: `end` of the list, by top-k where by_k, top-p and
   // min-p. Their masses go to their groups in s.mass. all_mass: of what top-p refers to,
-  // where top-k does not set it. 0: min-p's cut is above the list.
+  // where top-k does not set it. 0: min-p's cut is above the list. passed: top-p's cut is
+  // not in the list, by_k above it, else below.
   __device__ __forceinline__ uint32_t cut_list(uint32_t n, bool by_k, double above, uint32_t before, double& all_mass,
                                                bool& passed) {
     const uint32_t size = sort(n), per = size > kThreads ? 2 : 1, i0 = threadIdx.x * per;
@@ -955,13 +968,14 @@ struct Pick {
     const double sum = above + block_scan(w[0] + w[1], all) - (w[0] + w[1]);
     if (by_k) all_mass = above + all;
     const double goal = static_cast<double>(r.p) * all_mass, limit = r.p < 1.f ? goal : INFINITY;
-    passed = by_k && !(limit > above);   // top-p's cut is above a list of top-k's
+    passed = by_k && !(limit > above);
     if (passed) return end;
     const double least = static_cast<double>(r.m);
     uint32_t kept = 0;
     if (i0 < end && ((i0 == 0 && before == 0) || (sum < limit && w[0] >= least))) kept = i0 + 1;
     if (per == 2 && i0 + 1 < end && sum + w[0] < limit && w[1] >= least) kept = i0 + 2;
     end = block_most(kept);
+    passed = !by_k && n && end == n && above + all < limit;
     for (int g = threadIdx.x; g < kGroup; g += kThreads) s.mass[g] = 0;
     __syncthreads();
 #pragma unroll
@@ -1050,7 +1064,7 @@ struct Pick {
     Cut q{};
     q.high = top();
     double off = 0., mine, cut_least = 0.;
-    uint64_t cut;
+    uint64_t cut = 0;
     enum Source { kCount, kMass, kDirect };   // direct: the cut is known
     int source = r.k ? kCount : r.p < 1.f ? kMass : kDirect;
     while (true) {
@@ -1109,7 +1123,7 @@ struct Pick {
       const double above = sum_of_groups();
       if (source == kMass && above >= goal) {
         // Sums in fixed point, off by up to 2^-44 a token, found the cut a bin too late:
-        // kept is what lies above the members.
+        // kept is what lies above the members. (A bin too early: `after`.)
         const uint64_t over = (static_cast<uint64_t>(key_of(q.hi)) + 1) << 32;
         if (!q.limited || q.limit < over) q.limit = over;
         q.limited = true;
@@ -1136,7 +1150,9 @@ struct Pick {
         }
         const double limit = r.p < 1.f ? static_cast<double>(r.p) * all_mass : INFINITY;
         if (limit > above) want = fmin(want, ceil((limit - above) / w));
-        q.limit = tied(q.most, static_cast<int64_t>(fmax(want, 1.)), q.limited ? q.limit : 0);
+        const uint64_t old = q.limited ? q.limit : 0;
+        q.limit = tied(q.most, static_cast<int64_t>(fmax(want, 1.)), old);
+        if (source == kMass && limit > above + static_cast<double>(n) * w) q.limit = after(q.limit, old);   // (a bin too early)
         q.limited = true;
         q.level = 0;
         source = limit > above ? kDirect : kMass;   // (or top-p's cut is among the ones above)
@@ -1144,16 +1160,19 @@ struct Pick {
       }
       bool passed;
       const uint32_t end = cut_list(n, source == kCount, above, before, all_mass, passed);
-      if (passed || end == 0) {
-        if (passed) {
-          q.limit = uniform(s.list[end - 1]);
-          q.limited = true;
-        }
-        source = passed ? kMass : kDirect;
+      if (end) cut = uniform(s.list[end - 1]);
+      if (source == kCount ? passed : q.level && passed) {
+        // above a list of top-k's; or a bin too early, when one more token is kept
+        q.limit = source == kCount ? cut : after(cut, q.limited ? q.limit : 0);
+        q.limited = true;
+        source = source == kCount ? kMass : kDirect;
         q.level = 0;
         continue;
       }
-      cut = uniform(s.list[end - 1]);
+      if (end == 0) {
+        source = kDirect;
+        continue;
+      }
       mine = listed_mass() + (static_cast<int64_t>(threadIdx.x) < a.n1024 ? s.group[threadIdx.x] : 0.);
       break;
     }

@@ -80,3 +80,24 @@ def test_top_k_of_more_than_there_are_among_equal_ones(v, n, largest, banned):
         for dtype in (torch.float32, torch.bfloat16):
             check(torch.from_numpy(x).to(dtype), k=k, p=p)
             check(torch.from_numpy(x).to(dtype), k=k, p=p, m=0.9, t=0.7)
+
+
+@pytest.mark.parametrize("listed", [0, 100])
+@pytest.mark.parametrize("k", [0, 1])
+def test_a_border_past_a_bin_that_fixed_point_ends_in(listed, k):
+    """The same with masses that round up: half of all is 3e-10 over the sum up to the last of 10000 tokens at a (or
+    of 100 at b, which a list holds), which in fixed point is 5e-10 too large. The token after those is kept too."""
+    n = 10001 + listed
+    a = np.float32(-3500.45 * 2.0 ** -43)
+    b = np.nextafter(a, np.float32(-1))
+    x = np.full(2 * n, np.nextafter(b, np.float32(-1)) if listed else b, np.float32)
+    at = np.random.default_rng(2).permutation(2 * n)
+    x[at[0]], x[at[1:10001]], x[at[10001:n]] = 0, a, b
+    x = np.insert(x, 999, np.float32(math.log(1e-9)))
+    if k:   # top-k first: all but one more
+        k, x = len(x), np.insert(x, 7777, np.float32(-30))
+    assert (kept(x.astype(np.float64), k=k, p=0.5) > 0).sum() == n + 1
+    check(torch.from_numpy(x), k=k, p=0.5)
+    m = float(np.float32(1 - 2.0 ** -24))   # (under all of them)
+    assert (kept(x.astype(np.float64), k=k, p=0.5, m=m) > 0).sum() == n + 1
+    check(torch.from_numpy(x), k=k, p=0.5, m=m)
